@@ -12,6 +12,7 @@
 #define IFAB_STATUS_PEER_TIMEOUT 1u   // a bounded wait on a peer flag ran out
 #define IFAB_STATUS_MBAR_TIMEOUT 2u   // a bounded wait on an mbarrier ran out
 #define IFAB_STATUS_BAD_INDEX 4u      // a page / expert / token index was out of range and skipped
+#define IFAB_STATUS_NO_PAGES 8u       // a pool had fewer free pages than a call needed
 
 typedef __nv_bfloat16 bf16;
 

@@ -511,6 +511,46 @@ int ifab_gqa_decode_attention(const void* q, long ldq, const void* k_cache, cons
                               int keys_per_split, int max_splits, float* scratch, uint64_t scratch_bytes, void* out,
                               long ldo, uint32_t* status, void* stream);
 
+/* ---- weights of 4 bits with group scales (csrc/kernels/int4.cuh) ----
+ * A packed matrix: `units` (16-byte aligned, ifab_int4_bytes of them) for N rows by K columns (multiples of 8), twice N rows (gate rows, then up rows) where `gated`;
+ * group: 32, 64 or 128 columns of a scale; zeros: zero points beside the scales; f16: scales in f16 instead of bf16. */
+typedef struct IfabInt4 {
+  void* units;
+  int32_t N, K, group, zeros, gated, f16;
+} IfabInt4;
+uint64_t ifab_int4_bytes(int N, int K, int group, int zeros, int gated);      /* 0: refused */
+int ifab_int4_quantise(const IfabInt4* d, const void* w, long ldw, void* stream);
+int ifab_int4_pack(const IfabInt4* d, const uint8_t* codes, long ldc, const void* scales, const uint8_t* zeros, void* stream);
+int ifab_int4_dequantise(const IfabInt4* d, void* out, long ldo, void* stream);
+int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr, void* y, long ldy, int out_f32, int T,
+                   void* stream);
+
+/* ---- pages of a cache that sequences share (csrc/kernels/pages.cu) ----
+ * A set of caches: `ptrs` and `row_bytes` [caches] on the device (base address, bytes of a row, a multiple of 16), pages of `page_tokens` rows back to back.
+ * A pool: table [slots, max_pages] (-1: none), lengths [slots], refs [pages] (entries that name a page), free_bits [(pages + 31) / 32] (a bit per page with refs 0),
+ * and a workspace of ifab_pages_work_words. Every list of slots is on the device; a list that names a slot out of range or, where slots are written, twice does nothing
+ * but set IFAB_STATUS_BAD_INDEX, one that needs more pages than there are nothing but set IFAB_STATUS_NO_PAGES. */
+typedef struct IfabPageSet {
+  const uint64_t* ptrs;
+  const int64_t* row_bytes;
+  int32_t caches, pages, page_tokens;
+  int64_t max_row_bytes;
+} IfabPageSet;
+typedef struct IfabPagePool {
+  IfabPageSet set;
+  int32_t *table, *lengths, *refs;
+  uint32_t* free_bits;
+  int32_t* work;
+  uint32_t* status;
+  int32_t slots, max_pages;
+} IfabPagePool;
+uint64_t ifab_pages_work_words(int slots, int max_pages, int pages);
+int ifab_pages_copy(const IfabPageSet* src, const IfabPageSet* dst, const int32_t* src_ids, const int32_t* dst_ids, const int32_t* rows, int n, uint32_t* status, void* stream);
+int ifab_pages_extend(const IfabPagePool* p, const int32_t* slots, const int32_t* tokens, int n, void* stream);
+int ifab_pages_fork(const IfabPagePool* p, const int32_t* src, const int32_t* dst, int n, void* stream);
+int ifab_pages_free(const IfabPagePool* p, const int32_t* slots, const int32_t* below, int n, void* stream);
+int ifab_pages_compact(const IfabPagePool* p, int32_t* live, void* stream);
+
 /* ---- GQA decode attention without any allocation (this entry point has no counterpart in the reference) ----
  * Same computation and same results as ifab_gqa_decode_attention, but the split-partials workspace is a
  * fixed array inside the library, so neither the caller nor the library calls cudaMalloc / cudaFree or any

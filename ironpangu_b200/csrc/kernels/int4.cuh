@@ -1,0 +1,52 @@
+// Weights of 4 bits with a scale (and a zero point) per group of columns:  w[n][k] = s[n][k / G] (q[n][k] - z[n][k / G]), q and z in 0 .. 15, z = 8 without zero points.
+//
+// A unit holds 16 rows by 128 columns in one piece of memory, codes first, then its scales and zero points, so that whoever multiplies streams one range of
+// bytes: 1024 bytes of codes and 32 a group of scales (16 a group of zero points); units of a tile of 16 rows follow one another along K. Rows and columns beyond
+// the matrix have the code of the value zero. A packed gate | up matrix is two halves of whole tiles.
+//   codes    block of 64 columns b (512 bytes), columns 8 c .. 8 c + 7 and 32 + 8 c .. of it (c < 4), rows g and g + 8 (g < 8): 16 bytes at b 512 + c 128 +
+//            (g ^ 2 c) 16, row g's 8 bytes first, a word for each run of eight columns. A warp whose lane is 4 g + c reads a block without meeting a bank twice and
+//            has the operands of four m16n8k16 products (with K permuted alike in the other operand), each of columns of one group; threads that are rows read
+//            128 bytes in a row for a fixed c.
+//   a word   columns k .. k + 7: column k + 2 j in bits 4 j, column k + 2 j + 1 in bits 4 j + 16. (w >> 4 j) & 0x000f000f is a pair.
+//   scales   [group][g][row g, row g + 8], 16 bits each (bf16 or f16); zero points the same in bytes
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace ifab::int4 {
+
+constexpr int TILE = 16, CHUNK = 128, CODES = 1024;          // rows and columns of a unit, bytes of its codes
+
+struct View {
+  unsigned char* units;
+  int N, K, group, zeros, f16;      // N: rows of one half where gated
+  int halves, tiles, chunks, unit;  // tiles of one half, units of a tile, bytes of a unit
+  __host__ __device__ int groups() const { return CHUNK / group; }
+  __device__ __forceinline__ unsigned char* at(int tile, int chunk) const { return units + ((long)tile * chunks + chunk) * unit; }
+};
+__host__ __device__ inline int unit_bytes(int group, int zeros) { return CODES + CHUNK / group * (zeros ? 48 : 32); }
+
+// host: the view of a descriptor; 0 or -1
+inline int view_of(const IfabInt4* d, View* v) {
+  if (!d || !d->units || (uintptr_t)d->units % 16 || d->N < 1 || d->K < 8 || d->K % 8 || (d->group != 32 && d->group != 64 && d->group != 128)) return -1;
+  *v = View{(unsigned char*)d->units, d->N, d->K, d->group, d->zeros != 0, d->f16 != 0, d->gated ? 2 : 1, (d->N + TILE - 1) / TILE, (d->K + CHUNK - 1) / CHUNK,
+            unit_bytes(d->group, d->zeros)};
+  return 0;
+}
+
+__device__ __forceinline__ int code_at(int g, int c) { return c * 128 + ((g ^ (2 * c)) << 4); }
+
+// two bf16 of a word's pair j: 128 + q is a bf16 whose last four bits are q; `less` is twice -(128 + z), and the difference is exact
+__device__ __forceinline__ uint32_t pair_of(uint32_t word, int j, uint32_t less) {
+  uint32_t v = ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+  asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(less));
+  return v;
+}
+__device__ __forceinline__ uint32_t less_of(uint32_t z) { return 0xc300c300u | z | z << 16; }
+__device__ __forceinline__ float2 scales_of(uint32_t two, int f16) {
+  if (f16) return __half22float2(*reinterpret_cast<const __half2*>(&two));
+  return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+}
+
+}  // namespace ifab::int4

@@ -53,6 +53,15 @@ _SIGS = {
     "ifab_embedding_bf16": [_P, _P, _P, c_int, c_int, c_int, _P, _P],
     "ifab_swiglu_rows_bf16": [_P, c_long, _P, c_long, c_int, c_int, _P],
     "ifab_rmsnorm_bf16": [_P, c_long, _P, _P, c_long, c_int, c_int, c_float, c_int, _P],
+    "ifab_int4_quantise": [_P, _P, c_long, _P],
+    "ifab_int4_pack": [_P, _P, c_long, _P, _P, _P],
+    "ifab_int4_dequantise": [_P, _P, c_long, _P],
+    "ifab_int4_rows": [_P, _P, c_long, _P, c_float, _P, c_long, _P, c_long, c_int, c_int, _P],
+    "ifab_pages_copy": [_P, _P, _P, _P, _P, c_int, _P, _P],
+    "ifab_pages_extend": [_P, _P, _P, c_int, _P],
+    "ifab_pages_fork": [_P, _P, _P, c_int, _P],
+    "ifab_pages_free": [_P, _P, _P, c_int, _P],
+    "ifab_pages_compact": [_P, _P, _P],
     "ifab_gemv_bf16": [_P, c_long, _P, _P, c_float, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],
     "ifab_gemv_rows_bf16": [_P, c_long, _P, _P, c_float, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],
     "ifab_qkv_rows_bf16": [_P, c_long, _P, _P, c_float, _P, c_long, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P, _P],
@@ -245,6 +254,10 @@ def load(build: bool = True, units=None):
                 continue
             fn.argtypes = sig
             fn.restype = c_int
+        for name, n in (("ifab_int4_bytes", 5), ("ifab_pages_work_words", 3)):
+            fn = getattr(lib, name, None)
+            if fn is not None:
+                fn.argtypes, fn.restype = [c_int] * n, c_u64
         import os
         if os.environ.get("IFAB_PDL", "1") == "0":  # A/B switch: plain stream-ordered launches
             lib.ifab_set_pdl(0)

@@ -1,0 +1,118 @@
+"""Linears with weights of 4 bits and a scale - and, if wanted, a zero point - per group of columns:  ``w[n, k] = s[n, k // G] (q[n, k] - z[n, k // G])`` with ``q`` and
+``z`` in 0 .. 15 (``z = 8`` without zero points) and ``G`` of 32, 64 or 128 columns (``csrc/kernels/int4_pack.cu``, ``int4_rows.cu``).
+
+A matrix is packed once (:func:`quantise` a bf16 matrix, :func:`pack` what a checkpoint holds) and then multiplied by :func:`linear` as often as wanted. Like all weights it is
+written by nothing while linears read it: a linear's loads of it may begin before the kernel ahead of it in the stream has ended."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import check
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+GROUPS = (32, 64, 128)
+NORM_ROWS = 8            # rows up to which a linear takes the norm ahead of it
+
+
+class IfabInt4(C.Structure):
+    """Mirror of ``struct IfabInt4`` in ``csrc/kernels/ifab_kernels.h``."""
+
+    _fields_ = [("units", C.c_void_p), ("N", C.c_int32), ("K", C.c_int32), ("group", C.c_int32), ("zeros", C.c_int32), ("gated", C.c_int32), ("f16", C.c_int32)]
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(f"int4: {what}")
+
+
+class Int4Weight:
+    """A packed matrix of ``rows`` x ``k`` weights; ``gated``: gate rows, then as many up rows. ``units`` holds codes, scales and zero points together."""
+
+    def __init__(self, rows: int, k: int, *, group: int = 128, zeros: bool = False, gated: bool = False, f16: bool = False, device="cuda"):
+        _need(group in GROUPS, f"groups of {group} columns are not supported")
+        _need(rows >= 1 and k >= 8 and k % 8 == 0, f"a matrix of {rows} x {k} is not supported (columns in eights)")
+        _need(not gated or rows % 2 == 0, f"{rows} rows are not gate and up rows")
+        self.rows, self.k, self.group, self.zeros, self.gated, self.f16 = rows, k, group, bool(zeros), bool(gated), bool(f16)
+        self.n = rows // 2 if gated else rows                 # columns of a result
+        _need(max(rows, k) <= 1 << 24, f"a matrix of {rows} x {k} is too large")
+        self.units = torch.empty(_lib.load().ifab_int4_bytes(self.n, k, group, self.zeros, self.gated), dtype=torch.uint8, device=device)
+        self.device = self.units.device
+        self.desc = IfabInt4(self.units.data_ptr(), self.n, k, group, self.zeros, self.gated, self.f16)
+        self.ref = C.byref(self.desc)
+
+    @property
+    def nbytes(self) -> int:
+        return self.units.numel()
+
+    def dequantise(self, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The weights' values ``[rows, k]``, rounded to bf16."""
+        if out is None:
+            out = torch.empty(self.rows, self.k, dtype=BF16, device=self.device)
+        _need(out.shape == (self.rows, self.k) and out.dtype == BF16 and out.stride(1) == 1 and out.device == self.device, "the output must be bf16 [rows, k] beside the weights")
+        with torch.cuda.device(self.device):
+            check(_lib.load().ifab_int4_dequantise(self.ref, out.data_ptr(), out.stride(0), _stream(self.device)), "int4.dequantise")
+        return out
+
+
+def quantise(w: torch.Tensor, *, group: int = 128, zeros: bool = False, gated: bool = False) -> Int4Weight:
+    """The bf16 matrix ``w`` ``[rows, k]`` in 4 bits. Per row and group: ``s = bf16(max|w| / 7)``; with zero points ``lo = min(w, 0)``, ``hi = max(w, 0)``,
+    ``s = bf16((hi - lo) / 15)``, ``z = rint(-lo / s)``; ``q = rint(w / s) + z``, within 0 .. 15. ``s`` is 1 where it would be 0; a group with an infinity or NaN gets a
+    scale of NaN."""
+    _need(w.dim() == 2 and w.dtype == BF16 and w.stride(1) == 1 and w.is_cuda, "the matrix must be bf16 [rows, k] on the device, columns contiguous")
+    out = Int4Weight(w.shape[0], w.shape[1], group=group, zeros=zeros, gated=gated, device=w.device)
+    with torch.cuda.device(w.device):
+        check(_lib.load().ifab_int4_quantise(out.ref, w.data_ptr(), w.stride(0), _stream(w.device)), "int4.quantise")
+    return out
+
+
+def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *, group: int = 128, gated: bool = False) -> Int4Weight:
+    """A checkpoint's matrix: ``codes`` uint8 ``[rows, k]`` (a code in the low four bits of a byte), ``scales`` bf16 or f16 and ``zeros`` uint8 (or none: 8), both
+    ``[rows, ceil(k / group)]``."""
+    _need(codes.dim() == 2 and codes.dtype == torch.uint8 and codes.stride(1) == 1 and codes.is_cuda, "codes must be uint8 [rows, k] on the device, columns contiguous")
+    rows, k = codes.shape
+    _need(scales.dtype in (BF16, F16), "scales must be bf16 or f16")
+    for t, what in ((scales, "scales"), (zeros, "zero points")):
+        _need(t is None or (t.shape == (rows, -(-k // group)) and t.is_contiguous() and t.device == codes.device), f"{what} must be contiguous [rows, groups] beside the codes")
+    _need(zeros is None or zeros.dtype == torch.uint8, "zero points must be uint8")
+    out = Int4Weight(rows, k, group=group, zeros=zeros is not None, gated=gated, f16=scales.dtype == F16, device=codes.device)
+    with torch.cuda.device(codes.device):
+        check(_lib.load().ifab_int4_pack(out.ref, codes.data_ptr(), codes.stride(0), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _stream(codes.device)), "int4.pack")
+    return out
+
+
+def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = None, eps: float = 1e-5, residual: Optional[torch.Tensor] = None, out_f32: bool = False,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y = x @ w.T (+ residual)``, or of a gated matrix ``silu(x @ gate.T) * (x @ up.T)``, for any number of bf16 rows ``x`` ``[T, k]``. ``norm_w`` (up to eight rows): the
+    rows are RMS-normalised first, as :func:`ops.decode.rmsnorm` does it. ``residual`` (bf16, not of a gated matrix) may be ``out``. Sums are f32 and the result is rounded
+    once, to bf16 or with ``out_f32`` not at all."""
+    T = x.shape[0]
+    _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
+    _need(x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 or T == 0, "rows must lie on 16 bytes")
+    if norm_w is not None:
+        _need(norm_w.shape == (w.k,) and norm_w.dtype == BF16 and norm_w.is_contiguous() and norm_w.device == w.device and norm_w.data_ptr() % 16 == 0, f"gains must be bf16 [{w.k}] on 16 bytes")
+        _need(T <= NORM_ROWS, f"a norm ahead of {T} rows is a launch of its own (ops.decode.rmsnorm)")
+    if out is None:
+        out = torch.empty(T, w.n, dtype=F32 if out_f32 else BF16, device=x.device)
+    else:
+        _need(out.shape == (T, w.n) and out.dtype in (BF16, F32) and out.stride(1) == 1 and out.device == w.device, f"the output must be bf16 or f32 [T, {w.n}] beside the weights")
+    if residual is not None:
+        _need(not w.gated, "a gated unit takes no residual")
+        _need(residual.shape == (T, w.n) and residual.dtype == BF16 and residual.stride(1) == 1 and residual.device == w.device, f"the residual must be bf16 [T, {w.n}] beside the weights")
+    if T == 0:
+        return out
+    dev = x.device.index
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return linear(x, w, norm_w=norm_w, eps=eps, residual=residual, out=out)
+    check(_lib.load().ifab_int4_rows(w.ref, x.data_ptr(), x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps,
+                                     None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
+                                     out.dtype == F32, T, _stream(x.device)), "int4.linear")
+    return out

@@ -1,0 +1,227 @@
+"""Linears with 4-bit weights against 64 bits: groups, zero points, scales in both types, gated matrices, norms, residuals; widths and lengths that no tile divides; rows
+that no launch holds at once. Bounds: products of a group are exact in f32 and added by tensor cores that cut off, at worst 17 addends a product and 8 products a group at
+2^-23 of the group's sum of magnitudes: 2^-16 of it; the result's rounding to bf16 is 2^-8 of the value."""
+import pytest
+import torch
+
+BF16, F16 = torch.bfloat16, torch.float16
+CUT = 2.0 ** -16
+
+
+def _codes(rows, k, group, zeros, seed, f16=False):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    groups = -(-k // group)
+    q = torch.randint(0, 16, (rows, k), generator=g, device="cuda", dtype=torch.uint8)
+    s = (torch.rand(rows, groups, generator=g, device="cuda") * 0.01 + 0.001).to(F16 if f16 else BF16)
+    z = torch.randint(0, 16, (rows, groups), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    return q, s, z
+
+
+def _values(q, s, z, group):
+    at = torch.arange(q.shape[1], device=q.device) // group
+    return (q.double() - (8 if z is None else z.double()[:, at])) * s.double()[:, at]
+
+
+def _rows(T, k, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(T, k + 8, generator=g, device="cuda").to(BF16)[:, :k]
+
+
+def _close(out, want, bound):
+    bad = ~((out.double() - want).abs() <= bound)
+    assert not bool(bad.any()), (int(bad.sum()), float(((out.double() - want).abs() - bound).max()))
+
+
+# -- refusals, on any machine -----------------------------------------------------------------------------------------------
+def test_refusals_without_a_device():
+    from ironpangu_b200.ops import int4
+
+    w = torch.zeros(16, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="on the device"):
+        int4.quantise(w)
+    for rows, k, kw, what in ((16, 60, {}, "eights"), (0, 64, {}, "not supported"), (16, 64, dict(group=48), "groups of 48"), (15, 64, dict(gated=True), "gate and up")):
+        with pytest.raises(ValueError, match=what):
+            int4.Int4Weight(rows, k, device="cpu", **kw)
+    h = int4.Int4Weight(33, 136, group=64, zeros=True, device="cpu")
+    assert h.nbytes == 3 * 2 * (1024 + 2 * 48) and h.n == 33
+    x = torch.zeros(2, 136, dtype=BF16)
+    for bad, kw, what in ((x.float(), {}, "rows must be bf16"), (x[:, :128], {}, "rows must be bf16"), (torch.zeros(2, 140, dtype=BF16)[:, :136], {}, "16 bytes"),
+                          (torch.zeros(9, 136, dtype=BF16), dict(norm_w=torch.ones(136, dtype=BF16)), "a launch of its own"), (x, dict(norm_w=torch.ones(136)), "gains"),
+                          (x, dict(residual=torch.zeros(2, 32, dtype=BF16)), "residual"), (x, dict(out=torch.zeros(2, 33, dtype=F16)), "output")):
+        with pytest.raises(ValueError, match=what):
+            int4.linear(bad, h, **kw)
+    with pytest.raises(ValueError, match="no residual"):
+        int4.linear(torch.zeros(1, 64, dtype=BF16), int4.Int4Weight(32, 64, gated=True, device="cpu"), residual=torch.zeros(1, 16, dtype=BF16))
+    assert int4.linear(torch.zeros(0, 136, dtype=BF16), h).shape == (0, 33)
+    q, s = torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 1, dtype=BF16)
+    with pytest.raises(ValueError, match="on the device"):
+        int4.pack(q, s)
+
+
+# -- on the device ----------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows,k,gated", [(1, 8, False), (17, 72, False), (40, 136, False), (64, 256, True), (70, 1000, True)])
+def test_pack_and_back(rows, k, gated, zeros, group):
+    from ironpangu_b200.ops import int4
+
+    for f16 in (False, True):
+        q, s, z = _codes(rows, k, group, zeros, rows + k, f16)
+        w = int4.pack(q, s, z, group=group, gated=gated)
+        assert w.nbytes == w.units.numel() and w.rows == rows
+        out = torch.full((rows + 1, k + 8), 7.0, dtype=BF16, device="cuda")
+        w.dequantise(out[:rows, :k])
+        assert torch.equal(out[:rows, :k], _values(q, s, z, group).to(BF16))         # 4 bits by 8 or 11: exact in f32, rounded once
+        assert bool((out[rows:] == 7).all()) and bool((out[:, k:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows,k,gated", [(3, 24, False), (130, 264, True), (257, 2048, False)])
+def test_quantise(rows, k, gated, zeros, group):
+    from ironpangu_b200.ops import int4
+
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    w = (torch.randn(rows, k + 8, generator=g, device="cuda") * 0.02).to(BF16)[:, :k]
+    w[0] = 0                                             # a group of zeros
+    w[1] = torch.arange(k, device="cuda") % 15 - 7.0     # symmetric: s = 1; without ties
+    w[2] = (torch.arange(k, device="cuda") % 2) * 0.5 + 0.25        # of one sign
+    f = torch.nn.functional.pad(w.double(), (0, -k % group)).view(rows, -1, group)
+    if zeros:
+        lo, hi = f.amin(-1).clamp(max=0), f.amax(-1).clamp(min=0)
+        s = ((hi - lo) / 15).float().to(BF16).double()
+    else:
+        s = (f.abs().amax(-1) / 7).float().to(BF16).double()
+    s = torch.where(s == 0, 1.0, s)[..., None]
+    z = torch.round(-lo[..., None] / s).clamp(0, 15) if zeros else 8
+    q = (torch.round(f / s) + z).clamp(0, 15)
+    want = ((q - z) * s).reshape(rows, -1)[:, :k].to(BF16)
+    h = int4.quantise(w, group=group, zeros=zeros, gated=gated)
+    assert torch.equal(h.dequantise(), want)
+    # within half a step of the matrix, but for what the scale's rounding to bf16 clips at the ends
+    if group == 128 and not zeros:
+        step = s.expand_as(f).reshape(rows, -1)[:, :k]
+        assert bool(((want.double() - w.double()).abs() <= step * (0.5 + 7 * 2.0 ** -8) + want.double().abs() * 2.0 ** -8).all())
+
+
+@pytest.mark.gpu
+def test_quantise_groups_without_a_value():
+    from ironpangu_b200.ops import int4
+
+    w = torch.randn(20, 256, device="cuda").to(BF16)
+    w[3, 5], w[4, 200], w[7, 130] = float("nan"), float("inf"), float("-inf")
+    for zeros in (False, True):
+        back = int4.quantise(w, group=128, zeros=zeros).dequantise()
+        nan = torch.zeros(20, 2, dtype=torch.bool, device="cuda")
+        nan[3, 0] = nan[4, 1] = nan[7, 1] = True
+        assert torch.equal(back.isnan().view(20, 2, 128).all(-1), nan) and torch.equal(back.isnan().view(20, 2, 128).any(-1), nan)
+        y = int4.linear(torch.ones(1, 256, device="cuda", dtype=BF16), int4.quantise(w, group=128, zeros=zeros))
+        assert torch.equal(y[0].isnan(), nan.any(-1))
+
+
+SHAPES = [(1, 8, 1), (16, 128, 1), (17, 72, 2), (1, 4096, 3), (300, 1032, 5), (1024, 1024, 1), (2741, 2056, 3), (2368, 264, 8), (5000, 136, 7), (64, 16392, 8), (200, 9000, 2),
+          (48, 640, 9), (333, 2056, 16), (70, 9000, 13), (130, 520, 21), (40, 264, 67)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,zeros,f16", [(128, False, False), (128, True, False), (64, False, True), (64, True, False), (32, False, False), (32, True, True)])
+@pytest.mark.parametrize("N,K,T", SHAPES)
+def test_linear(N, K, T, group, zeros, f16):
+    from ironpangu_b200.ops import int4
+
+    q, s, z = _codes(N, K, group, zeros, N + K, f16)
+    w, v, x = int4.pack(q, s, z, group=group), _values(q, s, z, group), _rows(T, K, T)
+    want, scale = x.double() @ v.T, x.double().abs() @ v.abs().T
+    out = torch.full((T + 1, N + 3), 7.0, device="cuda")
+    int4.linear(x, w, out=out[:T, :N])
+    _close(out[:T, :N], want, CUT * scale + 1e-30)
+    assert bool((out[T:] == 7).all()) and bool((out[:, N:] == 7).all())
+    y = _rows(T, N + (-N) % 8, 3)[:, :N].contiguous()
+    res = y.double()
+    int4.linear(x, w, residual=y, out=y)                 # in place
+    _close(y, want + res, CUT * scale + 2.0 ** -8 * (want + res).abs() + 1e-30)
+    assert int4.linear(x, w).dtype == BF16 and int4.linear(x, w, out_f32=True).dtype == torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,zeros", [(128, False), (64, True), (32, True)])
+@pytest.mark.parametrize("F,K,T", [(1, 8, 1), (17, 264, 3), (150, 1544, 8), (3000, 512, 1), (16, 4096, 11), (1237, 1032, 5), (96, 520, 33)])
+def test_gated(F, K, T, group, zeros):
+    from ironpangu_b200.ops import int4
+
+    q, s, z = _codes(2 * F, K, group, zeros, F + K)
+    w, v, x = int4.pack(q, s, z, group=group, gated=True), _values(q, s, z, group), _rows(T, K, T)
+    y, scale = x.double() @ v.T, CUT * (x.double().abs() @ v.abs().T)
+    gate, up, a, b = y[:, :F], y[:, F:], scale[:, :F], scale[:, F:]
+    want = gate * torch.sigmoid(gate) * up
+    out = torch.full((T + 1, F + 3), 7.0, dtype=BF16, device="cuda")
+    int4.linear(x, w, out=out[:T, :F])
+    # the unit's slope is at most 1.1; its exponential and quotient are off by a few steps of f32
+    _close(out[:T, :F], want, (2.0 ** -8 + 2.0 ** -20) * want.abs() + 1.1 * a * (up.abs() + b) + (gate.abs() + a) * b + 1e-30)
+    assert bool((out[T:] == 7).all()) and bool((out[:, F:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,T", [(33, 8, 1), (1024, 1024, 1), (300, 1032, 8), (130, 9000, 3), (64, 20000, 8)])
+def test_norm_ahead(N, K, T):
+    from ironpangu_b200.ops import int4
+
+    q, s, z = _codes(N, K, 64, True, N + K)
+    w, v, x = int4.pack(q, s, z, group=64), _values(q, s, z, 64), _rows(T, K, T)
+    gain = (torch.randn(K, device="cuda") * 0.1 + 1).to(BF16)
+    xn = (x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + 1e-6) * gain.double()).to(BF16).double()
+    want, scale = xn @ v.T, xn.abs() @ v.abs().T
+    out = int4.linear(x, w, norm_w=gain, eps=1e-6, out_f32=True)
+    # an f32 norm rounds to the other bf16 value (2^-7 of it) where it ends within some 2^-21 of their border: one operand of 2^13, four more allowed
+    flips = (4 + K // 1024) * 2.0 ** -7 * float((xn.abs().amax() * v.abs().amax()))
+    _close(out, want, CUT * scale + flips)
+    alone = torch.cat([int4.linear(x[t:t + 1], w, norm_w=gain, eps=1e-6, out_f32=True) for t in range(T)])
+    assert torch.equal(out, alone)                       # the bits that a row has alone
+
+
+@pytest.mark.gpu
+def test_rows_beside_a_row_change_nothing():
+    from ironpangu_b200.ops import int4
+
+    q, s, z = _codes(500, 1160, 128, False, 5)
+    w, x = int4.pack(q, s, z, group=128), _rows(16, 1160, 1)
+    alone = torch.cat([int4.linear(x[t:t + 1], w) for t in range(16)])
+    for T in (2, 8, 9, 16):
+        assert torch.equal(int4.linear(x[:T], w), alone[:T])
+    x[1] = float("nan")
+    x[2, 7] = float("inf")
+    y = int4.linear(x, w)
+    assert torch.equal(y[0], alone[0]) and torch.equal(y[3:], alone[3:]) and bool(y[1].isnan().all()) and not bool(y[2].isfinite().any())
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    """A captured linear, replayed on other rows; the matrix packed on another stream; the row ahead of it written by a kernel of the same stream."""
+    from ironpangu_b200.ops import int4
+
+    q, s, z = _codes(600, 2048, 128, True, 2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        w = int4.pack(q, s, z, group=128)
+        x = _rows(4, 2048, 1).contiguous()
+        first = int4.linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(int4.linear(x, w), first)
+    out = torch.empty(4, 600, dtype=BF16, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        int4.linear(x * 2, w, out=out)
+    for seed in (3, 4):
+        x.copy_(_rows(4, 2048, seed))
+        g.replay()
+        assert torch.equal(out, int4.linear(x * 2, w))
+    for _ in range(20):                                  # a matrix that the launch ahead has just packed
+        m = torch.randn(600, 2048, device="cuda").to(BF16)
+        h = int4.quantise(m)
+        got = int4.linear(x, h)
+        torch.cuda.synchronize()
+        assert torch.equal(got, int4.linear(x, h))
