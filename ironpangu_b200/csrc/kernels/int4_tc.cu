@@ -1,0 +1,317 @@
+// Products of many rows with 4-bit weights (int4.cuh) on tcgen05:  y[t][n] = sum_k x[t][k] w[n][k] (+ residual), or of a gate | up matrix silu(gate) up.
+//
+// The 128 rows of an MMA are weight rows, the tokens its columns. Weights become bf16(s (q - z)) - rounded once, as a checkpoint that is opened in bf16 has them - in
+// registers, where a thread is a row, and go straight into tensor memory as the MMA's first operand: neither codes nor weights pass through shared memory, whose
+// bandwidth belongs to the tokens' tiles. Two groups of four warps take the chunks of 128 columns in turn, with the codes of their next chunk on the way.
+//   warp 0      copies of the tokens' tiles (64 columns, 128-byte swizzle)
+//   warp 1      MMAs
+//   warps 2-9   weights into tensor memory; then 2-5 read the accumulator
+// Two CTAs an SM (128 columns of sums and four stages of 32 columns of weights each), so that one multiplies while the other starts or stores. With few tiles the
+// chunks along K are shared by the CTAs of a cluster: each leaves its part of the sum in its shared memory as f32 and every CTA adds up a share of the tokens over
+// distributed shared memory, in the order of the parts.
+// Every wait is bounded. One that runs out raises the CTA's flag and the status word; the warps that read the accumulator then wait for what the CTA has started and
+// leave NaN as their part of the sum.
+#include <algorithm>
+
+#include "int4.cuh"
+#include "tc_common.cuh"
+#include "ifab_kernels.h"
+
+using namespace ifab;
+using namespace ifab::tc;
+using namespace ifab::int4;
+
+namespace {
+
+constexpr int FT = 128, BK = 64, TOK = 128, STAGES = 4, THREADS = 320;
+constexpr int STAGE = TOK * BK * 2, SMEM = STAGES * STAGE + 1024 + 256;
+constexpr uint32_t COLS = 256, A_COL = 128;          // of tensor memory; first column of the weights' stages
+constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
+static_assert(TOK * FT * 4 <= STAGES * STAGE, "the part of the sum takes the ring's place");
+
+struct TcP {
+  View v;
+  void* y; long ldy; int out_f32;
+  const bf16* residual; long ldr;
+  int T, tok, splits;            // tokens of a tile (a multiple of 16), CTAs of a cluster
+  uint32_t* status; uint32_t spin_limit;
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_part4(uint32_t addr, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+// D[tmem] (+)= A[tmem] * B[smem]; issued by ONE thread
+__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
+// eight weights of a word, rounded to bf16; s2: the scale twice in bf16, s: in f32 where it is f16
+template <bool F16>
+__device__ __forceinline__ void weights_of(uint32_t word, uint32_t less, uint32_t s2, float s, uint32_t* out) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t d = pair_of(word, j, less);
+    if (F16) {
+      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&d));
+      const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * s, f.y * s);
+      out[j] = *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(out[j]) : "r"(d), "r"(s2));
+    }
+  }
+}
+
+// grid (feature tiles x splits, token tiles), clusters of `splits` along x
+template <int GROUP, bool ZEROS, bool F16>
+__global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, TcP p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
+  uint64_t *weights = full + STAGES, *empty = weights + STAGES, *acc_full = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* requested = abort_flag + 1;      // blocks whose copies were requested, once no more will be; until then -1
+  const View& v = p.v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
+  const bool gated = v.halves == 2;
+  const int n0 = tile * (gated ? FT / 2 : FT), m0 = blockIdx.y * p.tok;
+  const int c0 = (int)((long)v.chunks * part / p.splits), nc = (int)((long)v.chunks * (part + 1) / p.splits) - c0, nk = 2 * nc;      // chunks, blocks of 64 columns
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&weights[s], 4);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    *requested = -1;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_x);
+  }
+  // this thread's row: its units along K, and the first codes, which no kernel of the stream writes
+  const int row = (warp & 3) * 32 + lane, group = (warp - 2) >> 2;
+  const unsigned char* unit = nullptr;
+  uint2 next[8];
+  uint32_t next_s[CHUNK / GROUP];
+  int next_z[CHUNK / GROUP];
+  const int g = row & 7, h = (row >> 3) & 1;
+  auto fetch = [&](int ch) {
+    const unsigned char* at = unit + (long)ch * v.unit;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) next[i] = *reinterpret_cast<const uint2*>(at + (i >> 2) * 512 + code_at(g, i & 3) + h * 8);
+#pragma unroll
+    for (int i = 0; i < CHUNK / GROUP; ++i) {
+      next_s[i] = *reinterpret_cast<const uint16_t*>(at + CODES + i * 32 + g * 4 + h * 2);
+      next_z[i] = ZEROS ? at[CODES + CHUNK / GROUP * 32 + i * 16 + g * 2 + h] : 8;
+    }
+  };
+  if (warp >= 2) {
+    const int t = n0 / TILE + (gated ? (row & 63) : row) / TILE;
+    unit = v.at(min(t, v.tiles - 1) + (gated && row >= 64 ? v.tiles : 0), c0);
+    if (group < nc) fetch(group);
+  }
+  __syncthreads();
+  grid_dep_wait();
+  if (warp == 1) tmem_alloc(tmem_slot, COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dep_launch();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    int issued = 0;
+    for (int kb = 0; kb < nk; ++kb) {
+      const int s = kb % STAGES;
+      if (kb >= STAGES && !mbar_wait(&empty[s], (kb / STAGES - 1) & 1, p.spin_limit)) *abort_flag = 1;
+      if (*abort_flag) break;
+      mbar_expect_tx(&full[s], p.tok * BK * 2);
+      tma_load_2d(smem + s * STAGE, &tmap_x, &full[s], (2 * c0 + kb) * BK, m0);
+      issued = kb + 1;
+    }
+    *requested = issued;
+    if (*abort_flag && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = umma_idesc_bf16(FT, p.tok);
+    for (int kb = 0; kb < nk; ++kb) {
+      const int s = kb % STAGES;
+      if (!mbar_wait(&full[s], (kb / STAGES) & 1, p.spin_limit) || !mbar_wait(&weights[s], (kb / STAGES) & 1, p.spin_limit) || *abort_flag) {
+        *abort_flag = 1;
+        if (p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+        break;
+      }
+      tc_fence_after();
+      const uint64_t db = umma_desc_sw128(smem_u32(smem + s * STAGE));
+      const uint32_t a = tmem_base + A_COL + s * 32;
+#pragma unroll
+      for (int k = 0; k < BK / 16; ++k) umma_bf16_ta(tmem_base, a + 8 * k, db + (uint64_t)(2 * k), idesc, kb > 0 || k > 0);
+      umma_commit(&empty[s]);
+    }
+    umma_commit(acc_full);
+  } else if (warp >= 2) {
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+#pragma unroll 1
+    for (int ch = group; ch < nc; ch += 2) {
+      uint2 codes[8];
+      uint32_t s2[CHUNK / GROUP], less[CHUNK / GROUP];
+      float sf[CHUNK / GROUP];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) codes[i] = next[i];
+#pragma unroll
+      for (int i = 0; i < CHUNK / GROUP; ++i) {
+        s2[i] = next_s[i] | next_s[i] << 16;
+        sf[i] = F16 ? scales_of(next_s[i], 1).x : 0.f;
+        less[i] = less_of(next_z[i]);
+      }
+      if (ch + 2 < nc) fetch(ch + 2);
+      bool ok = true;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int kb = 2 * ch + b, s = kb % STAGES;
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int lo = GROUP == 128 ? 0 : GROUP == 64 ? b : 2 * b, hi = GROUP == 32 ? lo + 1 : lo;
+          weights_of<F16>(codes[4 * b + i].x, less[lo], s2[lo], sf[lo], w + 4 * i);
+          weights_of<F16>(codes[4 * b + i].y, less[hi], s2[hi], sf[hi], w + 16 + 4 * i);
+        }
+        if (kb >= STAGES && !mbar_wait(&empty[s], (kb / STAGES - 1) & 1, p.spin_limit)) *abort_flag = 1;
+        ok = !__any_sync(0xffffffffu, *abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_st_32x32(tmem_base + A_COL + s * 32 + lanes, reinterpret_cast<const float*>(w));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&weights[s]);
+      }
+      if (!ok) {
+        if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+        break;
+      }
+    }
+  }
+  __syncwarp();
+  // The accumulator complete, all copies have landed and all products have read the ring: it becomes this CTA's part of the sum, [tokens][128].
+  float* sum = reinterpret_cast<float*>(smem);
+  const int tokens = min(p.tok, p.T - m0);
+  if (warp >= 2 && warp < 6) {
+    const bool ready = mbar_wait(acc_full, 0, p.spin_limit);
+    tc_fence_after();
+    if (!ready) {
+      *abort_flag = 1;
+      if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+    }
+    const uint32_t tm = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    if (__any_sync(0xffffffffu, *abort_flag)) {
+      for (uint32_t i = 0; i < DRAIN && *requested < 0; ++i) __nanosleep(64);
+      const int n = *requested;
+      for (int kb = max(0, n - STAGES); kb < n; ++kb) mbar_wait(&full[kb % STAGES], (kb / STAGES) & 1, DRAIN);
+      mbar_wait(acc_full, 0, DRAIN);
+      for (int t = 0; t < tokens; ++t) sum[t * FT + row] = __int_as_float(0x7fffffff);
+    } else {
+      for (int t0 = 0; t0 < tokens; t0 += 32) {
+        float f[32];
+        tmem_ld_32x32(tm + (uint32_t)t0, f);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (t0 + i < tokens) sum[(t0 + i) * FT + row] = f[i];
+      }
+    }
+  }
+  tc_fence_before();
+  if (p.splits > 1) cluster_barrier();
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, COLS);
+  const uint32_t sum_at = smem_u32(sum);
+  const int width = gated ? FT / 8 : FT / 4;         // pieces of four features of a token
+  for (int i = threadIdx.x;; i += THREADS) {
+    const int t = part + i / width * p.splits, f = i % width * 4, col = n0 + f;
+    if (t >= tokens) break;
+    if (col >= v.N) continue;
+    float a[4] = {}, u[4] = {};
+    for (int r = 0; r < p.splits; ++r) {
+      const float4 x = p.splits > 1 ? ld_part4(sum_at + (t * FT + f) * 4, r) : *reinterpret_cast<const float4*>(sum + t * FT + f);
+      a[0] += x.x, a[1] += x.y, a[2] += x.z, a[3] += x.w;
+      if (gated) {
+        const float4 z = p.splits > 1 ? ld_part4(sum_at + (t * FT + FT / 2 + f) * 4, r) : *reinterpret_cast<const float4*>(sum + t * FT + FT / 2 + f);
+        u[0] += z.x, u[1] += z.y, u[2] += z.z, u[3] += z.w;
+      }
+    }
+    const int live = min(4, v.N - col);
+    const long m = m0 + t;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (gated) a[e] = a[e] / (1.f + __expf(-a[e])) * u[e];
+      if (p.residual && e < live) a[e] += __bfloat162float(p.residual[m * p.ldr + col + e]);
+    }
+    if (p.out_f32) {
+      float* out = reinterpret_cast<float*>(p.y) + m * p.ldy + col;
+      if (live == 4 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) *reinterpret_cast<float4*>(out) = make_float4(a[0], a[1], a[2], a[3]);
+      else
+        for (int e = 0; e < live; ++e) out[e] = a[e];
+    } else {
+      bf16* out = reinterpret_cast<bf16*>(p.y) + m * p.ldy + col;
+      if (live == 4 && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(a[0], a[1]), hi = __floats2bfloat162_rn(a[2], a[3]);
+        *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      } else {
+        for (int e = 0; e < live; ++e) out[e] = __float2bfloat16_rn(a[e]);
+      }
+    }
+  }
+  if (p.splits > 1) cluster_barrier();               // the parts stay until every CTA has read them
+}
+
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+template <int GROUP, bool ZEROS, bool F16>
+int launch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
+  auto k = int4_tc_kernel<GROUP, ZEROS, F16>;
+  if (int rc = opt_in_smem(k, SMEM)) return rc;
+  if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(THREADS), (unsigned)p.splits, (size_t)SMEM, s, tx, p);
+  return launch_chain(k, grid, dim3(THREADS), (size_t)SMEM, s, tx, p);
+}
+template <int GROUP>
+int dispatch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
+  if (p.v.zeros) return p.v.f16 ? launch<GROUP, true, true>(tx, p, grid, s) : launch<GROUP, true, false>(tx, p, grid, s);
+  return p.v.f16 ? launch<GROUP, false, true>(tx, p, grid, s) : launch<GROUP, false, false>(tx, p, grid, s);
+}
+
+}  // namespace
+
+// x [T, K] in bf16, rows on 16 bytes. The units are written by no kernel that may still run. spin_limit: polls of a wait.
+extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const void* residual, long ldr, void* y, long ldy, int out_f32, int T, uint32_t spin_limit,
+                              uint32_t* status, void* stream) {
+  TcP p{};
+  if (view_of(d, &p.v) || T < 1 || !x || !y || (uintptr_t)x % 16 || ldx % 8 || ldx < p.v.K || (p.v.halves == 2 && residual)) return -1;
+  p.y = y, p.ldy = ldy, p.out_f32 = out_f32, p.residual = (const bf16*)residual, p.ldr = ldr, p.T = T, p.status = status;
+  p.spin_limit = spin_limit;
+  const int ty = ceil_div(T, TOK), tiles = ceil_div(p.v.N, p.v.halves == 2 ? FT / 2 : FT), sms = device_sms();
+  p.tok = ceil_div(ceil_div(T, ty), 16) * 16;
+  p.splits = 1;
+  while (p.splits < 8 && 2 * p.splits * tiles * ty <= 2 * sms && p.v.chunks >= 4 * p.splits) p.splits *= 2;
+  CUtensorMap tx;
+  if (int rc = make_tmap_bf16_2d(&tx, x, (uint64_t)T, (uint64_t)p.v.K, (uint64_t)ldx, (uint32_t)p.tok)) return rc;
+  const dim3 grid(tiles * p.splits, ty);
+  if (ty > 65535) return -1;
+  cudaStream_t s = (cudaStream_t)stream;
+  return p.v.group == 128 ? dispatch<128>(tx, p, grid, s) : p.v.group == 64 ? dispatch<64>(tx, p, grid, s) : dispatch<32>(tx, p, grid, s);
+}

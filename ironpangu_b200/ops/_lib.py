@@ -15,7 +15,7 @@ from .. import _build
 _lock = threading.Lock()
 _lib = None
 
-c_void_p, c_int, c_long, c_float, c_u64 = C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_uint64
+c_void_p, c_int, c_uint, c_long, c_float, c_u64 = C.c_void_p, C.c_int, C.c_uint32, C.c_long, C.c_float, C.c_uint64
 MAX_RANKS = 8
 
 
@@ -57,6 +57,7 @@ _SIGS = {
     "ifab_int4_pack": [_P, _P, c_long, _P, _P, _P],
     "ifab_int4_dequantise": [_P, _P, c_long, _P],
     "ifab_int4_rows": [_P, _P, c_long, _P, c_float, _P, c_long, _P, c_long, c_int, c_int, _P],
+    "ifab_int4_gemm": [_P, _P, c_long, _P, c_long, _P, c_long, c_int, c_int, c_uint, _P, _P],
     "ifab_pages_copy": [_P, _P, _P, _P, _P, c_int, _P, _P],
     "ifab_pages_extend": [_P, _P, _P, c_int, _P],
     "ifab_pages_fork": [_P, _P, _P, c_int, _P],

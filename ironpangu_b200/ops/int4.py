@@ -1,5 +1,5 @@
 """Linears with weights of 4 bits and a scale - and, if wanted, a zero point - per group of columns:  ``w[n, k] = s[n, k // G] (q[n, k] - z[n, k // G])`` with ``q`` and
-``z`` in 0 .. 15 (``z = 8`` without zero points) and ``G`` of 32, 64 or 128 columns (``csrc/kernels/int4_pack.cu``, ``int4_rows.cu``).
+``z`` in 0 .. 15 (``z = 8`` without zero points) and ``G`` of 32, 64 or 128 columns (``csrc/kernels/int4_pack.cu``, ``int4_rows.cu``, ``int4_tc.cu``).
 
 A matrix is packed once (:func:`quantise` a bf16 matrix, :func:`pack` what a checkpoint holds) and then multiplied by :func:`linear` as often as wanted. Like all weights it is
 written by nothing while linears read it: a linear's loads of it may begin before the kernel ahead of it in the stream has ended."""
@@ -16,6 +16,8 @@ from ._lib import check
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 GROUPS = (32, 64, 128)
 NORM_ROWS = 8            # rows up to which a linear takes the norm ahead of it
+STREAM_ROWS = 16         # rows up to which the weights' stream is the work; more go through the tensor cores' tiles
+SPIN_LIMIT = 4000000     # polls of a wait inside a kernel
 
 
 class IfabInt4(C.Structure):
@@ -89,10 +91,11 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor
 
 
 def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = None, eps: float = 1e-5, residual: Optional[torch.Tensor] = None, out_f32: bool = False,
-           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+           out: Optional[torch.Tensor] = None, status_ptr: Optional[int] = None) -> torch.Tensor:
     """``y = x @ w.T (+ residual)``, or of a gated matrix ``silu(x @ gate.T) * (x @ up.T)``, for any number of bf16 rows ``x`` ``[T, k]``. ``norm_w`` (up to eight rows): the
     rows are RMS-normalised first, as :func:`ops.decode.rmsnorm` does it. ``residual`` (bf16, not of a gated matrix) may be ``out``. Sums are f32 and the result is rounded
-    once, to bf16 or with ``out_f32`` not at all."""
+    once, to bf16 or with ``out_f32`` not at all. Beyond sixteen rows a weight is rounded to bf16 ahead of its product; below, it is not. ``status_ptr``: a status word for
+    waits that run out."""
     T = x.shape[0]
     _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
     _need(x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 or T == 0, "rows must lie on 16 bytes")
@@ -111,7 +114,11 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
     dev = x.device.index
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return linear(x, w, norm_w=norm_w, eps=eps, residual=residual, out=out)
+            return linear(x, w, norm_w=norm_w, eps=eps, residual=residual, out=out, status_ptr=status_ptr)
+    if T > STREAM_ROWS:
+        check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
+                                         out.data_ptr(), out.stride(0), out.dtype == F32, T, SPIN_LIMIT, status_ptr, _stream(x.device)), "int4.linear")
+        return out
     check(_lib.load().ifab_int4_rows(w.ref, x.data_ptr(), x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps,
                                      None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
                                      out.dtype == F32, T, _stream(x.device)), "int4.linear")
