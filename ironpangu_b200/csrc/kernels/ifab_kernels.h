@@ -524,8 +524,9 @@ int ifab_int4_pack(const IfabInt4* d, const uint8_t* codes, long ldc, const void
 int ifab_int4_dequantise(const IfabInt4* d, void* out, long ldo, void* stream);
 int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr, void* y, long ldy, int out_f32, int T,
                    void* stream);
-int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const void* residual, long ldr, void* y, long ldy, int out_f32, int T, uint32_t spin_limit, uint32_t* status,
-                   void* stream);
+int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const void* residual, long ldr, void* y, long ldy, int out_f32, int T, void* scratch,
+                   uint32_t spin_limit, uint32_t* status, void* stream);
+uint64_t ifab_int4_gemm_scratch(int T, int K);
 
 /* ---- pages of a cache that sequences share (csrc/kernels/pages.cu) ----
  * A set of caches: `ptrs` and `row_bytes` [caches] on the device (base address, bytes of a row, a multiple of 16), pages of `page_tokens` rows back to back.

@@ -2,13 +2,14 @@
 //
 // A unit holds 16 rows by 128 columns in one piece of memory, codes first, then its scales and zero points, so that whoever multiplies streams one range of
 // bytes: 1024 bytes of codes and 32 a group of scales (16 a group of zero points); units of a tile of 16 rows follow one another along K. Rows and columns beyond
-// the matrix have the code of the value zero. A packed gate | up matrix is two halves of whole tiles.
+// the matrix have the code of the value zero, groups beyond it a scale of zero. A packed gate | up matrix is two halves of whole tiles.
 //   codes    block of 64 columns b (512 bytes), columns 8 c .. 8 c + 7 and 32 + 8 c .. of it (c < 4), rows g and g + 8 (g < 8): 16 bytes at b 512 + c 128 +
 //            (g ^ 2 c) 16, row g's 8 bytes first, a word for each run of eight columns. A warp whose lane is 4 g + c reads a block without meeting a bank twice and
 //            has the operands of four m16n8k16 products (with K permuted alike in the other operand), each of columns of one group; threads that are rows read
 //            128 bytes in a row for a fixed c.
 //   a word   columns k .. k + 7: column k + 2 j in bits 4 j, column k + 2 j + 1 in bits 4 j + 16. (w >> 4 j) & 0x000f000f is a pair.
 //   scales   [group][g][row g, row g + 8], 16 bits each (bf16 or f16); zero points the same in bytes
+// Behind the units: per row the largest of its finite scales, in f32.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -20,6 +21,7 @@ constexpr int TILE = 16, CHUNK = 128, CODES = 1024;          // rows and columns
 
 struct View {
   unsigned char* units;
+  float* most;                      // [halves * tiles * 16]: a row's largest finite scale
   int N, K, group, zeros, f16;      // N: rows of one half where gated
   int halves, tiles, chunks, unit;  // tiles of one half, units of a tile, bytes of a unit
   __host__ __device__ int groups() const { return CHUNK / group; }
@@ -30,8 +32,9 @@ __host__ __device__ inline int unit_bytes(int group, int zeros) { return CODES +
 // host: the view of a descriptor; 0 or -1
 inline int view_of(const IfabInt4* d, View* v) {
   if (!d || !d->units || (uintptr_t)d->units % 16 || d->N < 1 || d->K < 8 || d->K % 8 || (d->group != 32 && d->group != 64 && d->group != 128)) return -1;
-  *v = View{(unsigned char*)d->units, d->N, d->K, d->group, d->zeros != 0, d->f16 != 0, d->gated ? 2 : 1, (d->N + TILE - 1) / TILE, (d->K + CHUNK - 1) / CHUNK,
+  *v = View{(unsigned char*)d->units, nullptr, d->N, d->K, d->group, d->zeros != 0, d->f16 != 0, d->gated ? 2 : 1, (d->N + TILE - 1) / TILE, (d->K + CHUNK - 1) / CHUNK,
             unit_bytes(d->group, d->zeros)};
+  v->most = (float*)(v->units + (uint64_t)v->halves * v->tiles * v->chunks * v->unit);
   return 0;
 }
 

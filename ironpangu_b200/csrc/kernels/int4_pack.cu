@@ -1,7 +1,7 @@
 // 4-bit weights into their units (int4.cuh) and out of them.
 //
 //   quantise     s = bf16(max |w| / 7), z = 8, or with zero points lo = min(w, 0), hi = max(w, 0), s = bf16((hi - lo) / 15), z = rint(-lo / s) within 0 .. 15;
-//                q = rint(w / s) + z within 0 .. 15, divisions and roundings as IEEE 754 has them (halves to even); s = 1 where it would be 0. A group that holds an
+//                q = rint(w / s) + z within 0 .. 15, divisions and roundings as IEEE 754 has them (halves to even); where s is 0, so are the weights. A group that holds an
 //                infinity or NaN gets a scale of NaN: what it multiplies is NaN, not something else.
 //   pack         codes, scales and zero points of a checkpoint
 //   dequantise   bf16(s (q - z))
@@ -20,8 +20,20 @@ __device__ __forceinline__ uint32_t word_of(const uint8_t* q) {
   for (int j = 0; j < 4; ++j) w |= (uint32_t)q[2 * j] << (4 * j) | (uint32_t)q[2 * j + 1] << (4 * j + 16);
   return w;
 }
-// the launch behind these kernels may read units ahead of its wait for the one before it (int4_rows.cu): this one ends theirs
-__global__ void settle_kernel() {}
+// Rows' largest finite scales. The launch behind this one may read units ahead of its wait for the kernel before it (int4_rows.cu): this one is launched behind the end of the
+// kernels that write them, and `settled_kernel` behind its own.
+__global__ void __launch_bounds__(256) most_kernel(View v) {
+  const int row = blockIdx.x * 256 + threadIdx.x, tile = row / TILE, r = row % TILE;
+  if (tile >= v.halves * v.tiles) return;
+  float most = 0.f;
+  for (int ch = 0; ch < v.chunks; ++ch)
+    for (int i = 0; i < v.groups(); ++i) {
+      const float s = fabsf(scales_of(reinterpret_cast<const uint16_t*>(v.at(tile, ch) + CODES)[i * 16 + (r & 7) * 2 + (r >> 3)], v.f16).x);
+      if (s <= 3.4028234e38f) most = fmaxf(most, s);
+    }
+  v.most[row] = most;
+}
+__global__ void settled_kernel() {}
 
 struct Place {           // of a lane in its unit
   int tile, chunk, half, row0, g, c;
@@ -81,8 +93,7 @@ __global__ void __launch_bounds__(256) quantise_kernel(View v, const bf16* w, lo
         bad |= __shfl_xor_sync(0xffffffffu, bad, o);
       }
       bf16 sb = __float2bfloat16_rn(ZEROS ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f));
-      float s = __bfloat162float(sb);
-      if (s == 0.f) sb = __float2bfloat16_rn(1.f), s = 1.f;
+      const float s = __bfloat162float(sb) == 0.f ? 1.f : __bfloat162float(sb);
       const float z = ZEROS ? fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f) : 8.f;
 #pragma unroll
       for (int r = r0; r < r0 + RUNS; ++r) {
@@ -106,7 +117,6 @@ __global__ void __launch_bounds__(256) pack_kernel(View v, const uint8_t* codes,
   const Place at(v, unit);
   unsigned char* out = v.at(at.tile, at.chunk);
   const int per = (v.K + v.group - 1) / v.group;       // groups of a row
-  const uint16_t one = v.f16 ? 0x3c00 : 0x3f80;
   for (int h = 0; h < 2; ++h) {
     const long row = at.row(v, h);
     for (int r = 0; r < 4; ++r) {
@@ -120,7 +130,7 @@ __global__ void __launch_bounds__(256) pack_kernel(View v, const uint8_t* codes,
     if (at.c < v.groups()) {
       const int group = at.chunk * v.groups() + at.c;
       const bool in = row >= 0 && group < per;
-      reinterpret_cast<uint16_t*>(out + CODES)[at.c * 16 + at.g * 2 + h] = in ? scales[row * per + group] : one;
+      reinterpret_cast<uint16_t*>(out + CODES)[at.c * 16 + at.g * 2 + h] = in ? scales[row * per + group] : 0;
       // a group beyond K: the zero point that its codes were given above
       if (v.zeros) (out + CODES + v.groups() * 32)[at.c * 16 + at.g * 2 + h] = row < 0 ? 8 : zeros[row * per + min(group, per - 1)] & 15;
     }
@@ -163,8 +173,9 @@ template <int GROUP>
 int launch_quantise(const View& v, const bf16* w, long ldw, long units, cudaStream_t s) {
   return launch_chain(v.zeros ? quantise_kernel<GROUP, true> : quantise_kernel<GROUP, false>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, s, v, w, ldw, units);
 }
-int settle(cudaStream_t s) {
-  settle_kernel<<<1, 32, 0, s>>>();
+int settle(const View& v, cudaStream_t s) {
+  most_kernel<<<(v.halves * v.tiles * TILE + 255) / 256, 256, 0, s>>>(v);
+  settled_kernel<<<1, 32, 0, s>>>();
   return (int)cudaGetLastError();
 }
 
@@ -172,7 +183,7 @@ int settle(cudaStream_t s) {
 
 extern "C" uint64_t ifab_int4_bytes(int N, int K, int group, int zeros, int gated) {
   if (N < 1 || K < 8 || K % 8 || (group != 32 && group != 64 && group != 128)) return 0;
-  return (uint64_t)((N + TILE - 1) / TILE) * (gated ? 2 : 1) * ((K + CHUNK - 1) / CHUNK) * unit_bytes(group, zeros);
+  return (uint64_t)((N + TILE - 1) / TILE) * (gated ? 2 : 1) * ((uint64_t)((K + CHUNK - 1) / CHUNK) * unit_bytes(group, zeros) + TILE * 4);
 }
 
 // w [N or 2 N, K] in bf16, rows on 16 bytes
@@ -183,7 +194,7 @@ extern "C" int ifab_int4_quantise(const IfabInt4* d, const void* w, long ldw, vo
   cudaStream_t s = (cudaStream_t)stream;
   const bf16* p = (const bf16*)w;
   int rc = v.group == 128 ? launch_quantise<128>(v, p, ldw, units, s) : v.group == 64 ? launch_quantise<64>(v, p, ldw, units, s) : launch_quantise<32>(v, p, ldw, units, s);
-  return rc ? rc : settle(s);
+  return rc ? rc : settle(v, s);
 }
 
 // codes [N or 2 N, K] a byte each (low four bits), scales and zero points [N or 2 N, ceil(K / group)]
@@ -193,7 +204,7 @@ extern "C" int ifab_int4_pack(const IfabInt4* d, const uint8_t* codes, long ldc,
   const long units = (long)v.halves * v.tiles * v.chunks;
   cudaStream_t s = (cudaStream_t)stream;
   int rc = launch_chain(pack_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, s, v, codes, ldc, (const uint16_t*)scales, zeros, units);
-  return rc ? rc : settle(s);
+  return rc ? rc : settle(v, s);
 }
 
 // out [N or 2 N, K] in bf16, rows on 16 bytes

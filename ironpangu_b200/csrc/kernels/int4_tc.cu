@@ -1,8 +1,12 @@
 // Products of many rows with 4-bit weights (int4.cuh) on tcgen05:  y[t][n] = sum_k x[t][k] w[n][k] (+ residual), or of a gate | up matrix silu(gate) up.
 //
-// The 128 rows of an MMA are weight rows, the tokens its columns. Weights become bf16(s (q - z)) - rounded once, as a checkpoint that is opened in bf16 has them - in
-// registers, where a thread is a row, and go straight into tensor memory as the MMA's first operand: neither codes nor weights pass through shared memory, whose
-// bandwidth belongs to the tokens' tiles. Two groups of four warps take the chunks of 128 columns in turn, with the codes of their next chunk on the way.
+// The 128 rows of an MMA are weight rows, the tokens its columns. Weights become s (q - z) in registers, where a thread is a row, and go straight into tensor memory
+// as the MMA's first operand: neither codes nor weights pass through shared memory, whose bandwidth belongs to the tokens' tiles. Two groups of four warps take the
+// chunks of 128 columns in turn, with the codes of their next chunk on the way.
+// The operands are f16, each row with a power of two of its own. A product s (q - z) has up to 13 bits: bf16 leaves 8 of them, and a gated unit's result was off by 1.6
+// times its rounding; f16 leaves 11. Rows of x keep all their 8 bits: a launch ahead (rows_kernel) brings a row's largest magnitude to 2^14 .. 2^15, so that what falls below
+// f16's normal range is off by 2^-40 of that at most, and a row of weights has its largest scale at 2^11 .. 2^12 (15 of them stay below 65504). Both powers are taken out of
+// the f32 sums.
 //   warp 0      copies of the tokens' tiles (64 columns, 128-byte swizzle)
 //   warp 1      MMAs
 //   warps 2-9   weights into tensor memory; then 2-5 read the accumulator
@@ -33,6 +37,7 @@ struct TcP {
   View v;
   void* y; long ldy; int out_f32;
   const bf16* residual; long ldr;
+  const float* factor;           // of the rows of x
   int T, tok, splits;            // tokens of a tile (a multiple of 16), CTAs of a cluster
   uint32_t* status; uint32_t spin_limit;
 };
@@ -48,8 +53,10 @@ __device__ __forceinline__ float4 ld_part4(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
   return v;
 }
+// kind::f16 instruction descriptor: f16 x f16 -> f32, both operands K-major
+__device__ __forceinline__ uint32_t umma_idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 // D[tmem] (+)= A[tmem] * B[smem]; issued by ONE thread
-__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
@@ -58,24 +65,52 @@ __device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, u
       : "memory");
 }
 
-// eight weights of a word, rounded to bf16; s2: the scale twice in bf16, s: in f32 where it is f16
-template <bool F16>
-__device__ __forceinline__ void weights_of(uint32_t word, uint32_t less, uint32_t s2, float s, uint32_t* out) {
+// eight weights of a word in f16: 1024 + q is an f16 whose last four bits are q, and the difference is exact. less: twice -(1024 + z), s2: twice the scale
+__device__ __forceinline__ void weights_of(uint32_t word, uint32_t less, uint32_t s2, uint32_t* out) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t d = pair_of(word, j, less);
-    if (F16) {
-      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&d));
-      const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * s, f.y * s);
-      out[j] = *reinterpret_cast<const uint32_t*>(&r);
-    } else {
-      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(out[j]) : "r"(d), "r"(s2));
-    }
+    uint32_t d = ((word >> (4 * j)) & 0x000f000fu) | 0x64006400u;
+    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(d) : "r"(less));
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(out[j]) : "r"(d), "r"(s2));
+  }
+}
+// the exponent of a magnitude within -112 .. 127, so that its powers below are normal f32
+__device__ __forceinline__ int exponent_of(float most) { return max(min((int)(__float_as_uint(most) >> 23) - 127, 127), -112); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// rows of x in f16 by a power of two each, which `factor` takes out again. A CTA a row
+__global__ void __launch_bounds__(256) rows_kernel(const bf16* x, long ldx, __half* out, long ldo, float* factor, int K) {
+  __shared__ float red[8];
+  grid_dep_launch();
+  grid_dep_wait();
+  const bf16* row = x + (long)blockIdx.x * ldx;
+  float most = 0.f;
+  for (int i = threadIdx.x; i < K / 8; i += 256) {
+    float f[8];
+    unpack8(*reinterpret_cast<const uint4*>(row + i * 8), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) <= 3.4028234e38f ? fabsf(f[e]) : 0.f);
+  }
+  most = warp_max(most);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
+  const int e = exponent_of(most);
+  const float by = power_of_two(min(14 - e, 126));
+  if (threadIdx.x == 0) factor[blockIdx.x] = power_of_two(max(e - 14, -126));
+  for (int i = threadIdx.x; i < K / 8; i += 256) {
+    float f[8];
+    unpack8(*reinterpret_cast<const uint4*>(row + i * 8), f);
+    uint4 u;
+    __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(f[2 * j] * by, f[2 * j + 1] * by);
+    *reinterpret_cast<uint4*>(out + (long)blockIdx.x * ldo + i * 8) = u;
   }
 }
 
 // grid (feature tiles x splits, token tiles), clusters of `splits` along x
-template <int GROUP, bool ZEROS, bool F16>
+template <int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, TcP p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -107,7 +142,8 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
   const int row = (warp & 3) * 32 + lane, group = (warp - 2) >> 2;
   const unsigned char* unit = nullptr;
   uint2 next[8];
-  uint32_t next_s[CHUNK / GROUP];
+  uint16_t next_s[CHUNK / GROUP];
+  float by = 0.f;                    // the row's power of two
   int next_z[CHUNK / GROUP];
   const int g = row & 7, h = (row >> 3) & 1;
   auto fetch = [&](int ch) {
@@ -122,7 +158,9 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
   };
   if (warp >= 2) {
     const int t = n0 / TILE + (gated ? (row & 63) : row) / TILE;
-    unit = v.at(min(t, v.tiles - 1) + (gated && row >= 64 ? v.tiles : 0), c0);
+    const int at = min(t, v.tiles - 1) + (gated && row >= 64 ? v.tiles : 0);
+    unit = v.at(at, c0);
+    by = power_of_two(11 - exponent_of(v.most[at * TILE + (row & 15)]));
     if (group < nc) fetch(group);
   }
   __syncthreads();
@@ -147,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     *requested = issued;
     if (*abort_flag && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
   } else if (warp == 1 && lane == 0) {
-    const uint32_t idesc = umma_idesc_bf16(FT, p.tok);
+    const uint32_t idesc = umma_idesc_f16(FT, p.tok);
     for (int kb = 0; kb < nk; ++kb) {
       const int s = kb % STAGES;
       if (!mbar_wait(&full[s], (kb / STAGES) & 1, p.spin_limit) || !mbar_wait(&weights[s], (kb / STAGES) & 1, p.spin_limit) || *abort_flag) {
@@ -159,7 +197,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
       const uint64_t db = umma_desc_sw128(smem_u32(smem + s * STAGE));
       const uint32_t a = tmem_base + A_COL + s * 32;
 #pragma unroll
-      for (int k = 0; k < BK / 16; ++k) umma_bf16_ta(tmem_base, a + 8 * k, db + (uint64_t)(2 * k), idesc, kb > 0 || k > 0);
+      for (int k = 0; k < BK / 16; ++k) umma_f16_ta(tmem_base, a + 8 * k, db + (uint64_t)(2 * k), idesc, kb > 0 || k > 0);
       umma_commit(&empty[s]);
     }
     umma_commit(acc_full);
@@ -169,14 +207,13 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     for (int ch = group; ch < nc; ch += 2) {
       uint2 codes[8];
       uint32_t s2[CHUNK / GROUP], less[CHUNK / GROUP];
-      float sf[CHUNK / GROUP];
 #pragma unroll
       for (int i = 0; i < 8; ++i) codes[i] = next[i];
 #pragma unroll
       for (int i = 0; i < CHUNK / GROUP; ++i) {
-        s2[i] = next_s[i] | next_s[i] << 16;
-        sf[i] = F16 ? scales_of(next_s[i], 1).x : 0.f;
-        less[i] = less_of(next_z[i]);
+        const __half2 s = __float2half2_rn(scales_of(next_s[i], v.f16).x * by);
+        s2[i] = *reinterpret_cast<const uint32_t*>(&s);
+        less[i] = 0xe400e400u | next_z[i] | next_z[i] << 16;
       }
       if (ch + 2 < nc) fetch(ch + 2);
       bool ok = true;
@@ -187,8 +224,8 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int lo = GROUP == 128 ? 0 : GROUP == 64 ? b : 2 * b, hi = GROUP == 32 ? lo + 1 : lo;
-          weights_of<F16>(codes[4 * b + i].x, less[lo], s2[lo], sf[lo], w + 4 * i);
-          weights_of<F16>(codes[4 * b + i].y, less[hi], s2[hi], sf[hi], w + 16 + 4 * i);
+          weights_of(codes[4 * b + i].x, less[lo], s2[lo], w + 4 * i);
+          weights_of(codes[4 * b + i].y, less[hi], s2[hi], w + 16 + 4 * i);
         }
         if (kb >= STAGES && !mbar_wait(&empty[s], (kb / STAGES - 1) & 1, p.spin_limit)) *abort_flag = 1;
         ok = !__any_sync(0xffffffffu, *abort_flag);
@@ -225,13 +262,14 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
       mbar_wait(acc_full, 0, DRAIN);
       for (int t = 0; t < tokens; ++t) sum[t * FT + row] = __int_as_float(0x7fffffff);
     } else {
+      const float out = __uint_as_float((254u << 23) - __float_as_uint(by));          // 1 / by
       for (int t0 = 0; t0 < tokens; t0 += 32) {
         float f[32];
         tmem_ld_32x32(tm + (uint32_t)t0, f);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (t0 + i < tokens) sum[(t0 + i) * FT + row] = f[i];
+          if (t0 + i < tokens) sum[(t0 + i) * FT + row] = f[i] * out;
       }
     }
   }
@@ -257,8 +295,11 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     }
     const int live = min(4, v.N - col);
     const long m = m0 + t;
+    const float factor = p.factor[m];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
+      a[e] *= factor;
+      u[e] *= factor;
       if (gated) a[e] = a[e] / (1.f + __expf(-a[e])) * u[e];
       if (p.residual && e < live) a[e] += __bfloat162float(p.residual[m * p.ldr + col + e]);
     }
@@ -282,36 +323,38 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-template <int GROUP, bool ZEROS, bool F16>
+template <int GROUP, bool ZEROS>
 int launch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
-  auto k = int4_tc_kernel<GROUP, ZEROS, F16>;
+  auto k = int4_tc_kernel<GROUP, ZEROS>;
   if (int rc = opt_in_smem(k, SMEM)) return rc;
   if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(THREADS), (unsigned)p.splits, (size_t)SMEM, s, tx, p);
   return launch_chain(k, grid, dim3(THREADS), (size_t)SMEM, s, tx, p);
 }
-template <int GROUP>
-int dispatch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
-  if (p.v.zeros) return p.v.f16 ? launch<GROUP, true, true>(tx, p, grid, s) : launch<GROUP, true, false>(tx, p, grid, s);
-  return p.v.f16 ? launch<GROUP, false, true>(tx, p, grid, s) : launch<GROUP, false, false>(tx, p, grid, s);
-}
 
 }  // namespace
 
-// x [T, K] in bf16, rows on 16 bytes. The units are written by no kernel that may still run. spin_limit: polls of a wait.
-extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const void* residual, long ldr, void* y, long ldy, int out_f32, int T, uint32_t spin_limit,
-                              uint32_t* status, void* stream) {
+// bytes of the workspace of T rows
+extern "C" uint64_t ifab_int4_gemm_scratch(int T, int K) { return T < 1 || K < 8 ? 0 : (uint64_t)T * K * 2 + ((uint64_t)T * 4 + 15) / 16 * 16; }
+
+// x [T, K] in bf16, rows on 16 bytes; scratch: ifab_int4_gemm_scratch bytes on 16 bytes, for this call alone. The units are written by no kernel that may still run. spin_limit: polls of a wait.
+extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const void* residual, long ldr, void* y, long ldy, int out_f32, int T, void* scratch,
+                              uint32_t spin_limit, uint32_t* status, void* stream) {
   TcP p{};
-  if (view_of(d, &p.v) || T < 1 || !x || !y || (uintptr_t)x % 16 || ldx % 8 || ldx < p.v.K || (p.v.halves == 2 && residual)) return -1;
-  p.y = y, p.ldy = ldy, p.out_f32 = out_f32, p.residual = (const bf16*)residual, p.ldr = ldr, p.T = T, p.status = status;
+  if (view_of(d, &p.v) || T < 1 || !x || !y || !scratch || ((uintptr_t)x | (uintptr_t)scratch) % 16 || ldx % 8 || (p.v.halves == 2 && residual)) return -1;
+  __half* rows = (__half*)scratch;
+  float* factor = (float*)((char*)scratch + (uint64_t)T * p.v.K * 2);
+  p.y = y, p.ldy = ldy, p.out_f32 = out_f32, p.residual = (const bf16*)residual, p.ldr = ldr, p.factor = factor, p.T = T, p.status = status;
   p.spin_limit = spin_limit;
   const int ty = ceil_div(T, TOK), tiles = ceil_div(p.v.N, p.v.halves == 2 ? FT / 2 : FT), sms = device_sms();
+  if (ty > 65535) return -1;
   p.tok = ceil_div(ceil_div(T, ty), 16) * 16;
   p.splits = 1;
   while (p.splits < 8 && 2 * p.splits * tiles * ty <= 2 * sms && p.v.chunks >= 4 * p.splits) p.splits *= 2;
-  CUtensorMap tx;
-  if (int rc = make_tmap_bf16_2d(&tx, x, (uint64_t)T, (uint64_t)p.v.K, (uint64_t)ldx, (uint32_t)p.tok)) return rc;
+  CUtensorMap tx;          // of 16-bit elements: the type is the products' to know
+  if (int rc = make_tmap_bf16_2d(&tx, rows, (uint64_t)T, (uint64_t)p.v.K, (uint64_t)p.v.K, (uint32_t)p.tok)) return rc;
   const dim3 grid(tiles * p.splits, ty);
-  if (ty > 65535) return -1;
   cudaStream_t s = (cudaStream_t)stream;
-  return p.v.group == 128 ? dispatch<128>(tx, p, grid, s) : p.v.group == 64 ? dispatch<64>(tx, p, grid, s) : dispatch<32>(tx, p, grid, s);
+  if (int rc = launch_chain(rows_kernel, dim3(T), dim3(256), 0, s, (const bf16*)x, ldx, rows, (long)p.v.K, factor, p.v.K)) return rc;
+  if (p.v.zeros) return p.v.group == 128 ? launch<128, true>(tx, p, grid, s) : p.v.group == 64 ? launch<64, true>(tx, p, grid, s) : launch<32, true>(tx, p, grid, s);
+  return p.v.group == 128 ? launch<128, false>(tx, p, grid, s) : p.v.group == 64 ? launch<64, false>(tx, p, grid, s) : launch<32, false>(tx, p, grid, s);
 }

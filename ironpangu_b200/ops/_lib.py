@@ -57,7 +57,7 @@ _SIGS = {
     "ifab_int4_pack": [_P, _P, c_long, _P, _P, _P],
     "ifab_int4_dequantise": [_P, _P, c_long, _P],
     "ifab_int4_rows": [_P, _P, c_long, _P, c_float, _P, c_long, _P, c_long, c_int, c_int, _P],
-    "ifab_int4_gemm": [_P, _P, c_long, _P, c_long, _P, c_long, c_int, c_int, c_uint, _P, _P],
+    "ifab_int4_gemm": [_P, _P, c_long, _P, c_long, _P, c_long, c_int, c_int, _P, c_uint, _P, _P],
     "ifab_pages_copy": [_P, _P, _P, _P, _P, c_int, _P, _P],
     "ifab_pages_extend": [_P, _P, _P, c_int, _P],
     "ifab_pages_fork": [_P, _P, _P, c_int, _P],
@@ -255,7 +255,7 @@ def load(build: bool = True, units=None):
                 continue
             fn.argtypes = sig
             fn.restype = c_int
-        for name, n in (("ifab_int4_bytes", 5), ("ifab_pages_work_words", 3)):
+        for name, n in (("ifab_int4_bytes", 5), ("ifab_int4_gemm_scratch", 2), ("ifab_pages_work_words", 3)):
             fn = getattr(lib, name, None)
             if fn is not None:
                 fn.argtypes, fn.restype = [c_int] * n, c_u64

@@ -66,7 +66,7 @@ class Int4Weight:
 
 def quantise(w: torch.Tensor, *, group: int = 128, zeros: bool = False, gated: bool = False) -> Int4Weight:
     """The bf16 matrix ``w`` ``[rows, k]`` in 4 bits. Per row and group: ``s = bf16(max|w| / 7)``; with zero points ``lo = min(w, 0)``, ``hi = max(w, 0)``,
-    ``s = bf16((hi - lo) / 15)``, ``z = rint(-lo / s)``; ``q = rint(w / s) + z``, within 0 .. 15. ``s`` is 1 where it would be 0; a group with an infinity or NaN gets a
+    ``s = bf16((hi - lo) / 15)``, ``z = rint(-lo / s)``; ``q = rint(w / s) + z``, within 0 .. 15. Where ``s`` is 0 (a group of zeros, or of less than bf16's smallest) the weights are 0; a group with an infinity or NaN gets a
     scale of NaN."""
     _need(w.dim() == 2 and w.dtype == BF16 and w.stride(1) == 1 and w.is_cuda, "the matrix must be bf16 [rows, k] on the device, columns contiguous")
     out = Int4Weight(w.shape[0], w.shape[1], group=group, zeros=zeros, gated=gated, device=w.device)
@@ -94,7 +94,8 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
            out: Optional[torch.Tensor] = None, status_ptr: Optional[int] = None) -> torch.Tensor:
     """``y = x @ w.T (+ residual)``, or of a gated matrix ``silu(x @ gate.T) * (x @ up.T)``, for any number of bf16 rows ``x`` ``[T, k]``. ``norm_w`` (up to eight rows): the
     rows are RMS-normalised first, as :func:`ops.decode.rmsnorm` does it. ``residual`` (bf16, not of a gated matrix) may be ``out``. Sums are f32 and the result is rounded
-    once, to bf16 or with ``out_f32`` not at all. Beyond sixteen rows a weight is rounded to bf16 ahead of its product; below, it is not. ``status_ptr``: a status word for
+    once, to bf16 or with ``out_f32`` not at all. Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product; up to
+    there it is not. ``status_ptr``: a status word for
     waits that run out."""
     T = x.shape[0]
     _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
@@ -116,8 +117,9 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
         with torch.cuda.device(dev):
             return linear(x, w, norm_w=norm_w, eps=eps, residual=residual, out=out, status_ptr=status_ptr)
     if T > STREAM_ROWS:
+        scratch = torch.empty(_lib.load().ifab_int4_gemm_scratch(T, w.k), dtype=torch.uint8, device=x.device)
         check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
-                                         out.data_ptr(), out.stride(0), out.dtype == F32, T, SPIN_LIMIT, status_ptr, _stream(x.device)), "int4.linear")
+                                         out.data_ptr(), out.stride(0), out.dtype == F32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr, _stream(x.device)), "int4.linear")
         return out
     check(_lib.load().ifab_int4_rows(w.ref, x.data_ptr(), x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps,
                                      None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),

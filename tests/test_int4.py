@@ -1,5 +1,5 @@
 """Linears with 4-bit weights against 64 bits: groups, zero points, scales in both types, gated matrices, norms, residuals; widths and lengths that no tile divides; rows
-that no launch holds at once. Beyond sixteen rows a weight is bf16, and the reference rounds it too. Bounds: products of a group are exact in f32 and added by tensor cores that cut off, at worst 17 addends a product and 8 products a group at
+that no launch holds at once. Beyond sixteen rows a weight has the 11 bits of f16, and the reference rounds it too. Bounds: products of a group are exact in f32 and added by tensor cores that cut off, at worst 17 addends a product and 8 products a group at
 2^-23 of the group's sum of magnitudes: 2^-16 of it (a whole row of K in one chain: 2^-23 of it a product, K / 16 of them); the result's rounding to bf16 is 2^-8 of the value."""
 import pytest
 import torch
@@ -25,7 +25,8 @@ def _values(q, s, z, group):
 def _operands(v, x):
     """Weights as the products have them, and the bound of their sums."""
     if x.shape[0] > 16:
-        v = v.to(BF16).double()
+        m, e = torch.frexp(v)                            # scales of a row are within a factor of 16 here: no weight is below f16's normal range
+        v = torch.ldexp(torch.round(m * 2 ** 11) / 2 ** 11, e)
     return v, (x.double().abs() @ v.abs().T) * (CUT if x.shape[0] <= 16 else max(CUT, 17 * x.shape[1] / 16 * 2.0 ** -23))
 
 
@@ -50,7 +51,7 @@ def test_refusals_without_a_device():
         with pytest.raises(ValueError, match=what):
             int4.Int4Weight(rows, k, device="cpu", **kw)
     h = int4.Int4Weight(33, 136, group=64, zeros=True, device="cpu")
-    assert h.nbytes == 3 * 2 * (1024 + 2 * 48) and h.n == 33
+    assert h.nbytes == 3 * (2 * (1024 + 2 * 48) + 64) and h.n == 33
     x = torch.zeros(2, 136, dtype=BF16)
     for bad, kw, what in ((x.float(), {}, "rows must be bf16"), (x[:, :128], {}, "rows must be bf16"), (torch.zeros(2, 140, dtype=BF16)[:, :136], {}, "16 bytes"),
                           (torch.zeros(9, 136, dtype=BF16), dict(norm_w=torch.ones(136, dtype=BF16)), "a launch of its own"), (x, dict(norm_w=torch.ones(136)), "gains"),
@@ -244,9 +245,40 @@ def test_a_wait_that_runs_out():
     q, s, z = _codes(700, 8192, 128, False, 1)
     w, x = int4.pack(q, s, z, group=128), _rows(300, 8192, 1).contiguous()
     want = int4.linear(x, w)
+    scratch = torch.empty(_lib.load().ifab_int4_gemm_scratch(300, 8192), dtype=torch.uint8, device="cuda")
     status, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(300, 700, dtype=BF16, device="cuda")
-    _lib.check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), 8192, None, 0, out.data_ptr(), 700, 0, 300, 0, status.data_ptr(), torch.cuda.current_stream().cuda_stream), "gemm")
+    _lib.check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), 8192, None, 0, out.data_ptr(), 700, 0, 300, scratch.data_ptr(), 0, status.data_ptr(), torch.cuda.current_stream().cuda_stream), "gemm")
     torch.cuda.synchronize()
     assert int(status) == 2 and bool(out.isnan().all())
     status.zero_()
     assert torch.equal(int4.linear(x, w, status_ptr=status.data_ptr()), want) and int(status) == 0
+
+
+@pytest.mark.gpu
+def test_ranges_of_rows_and_scales():
+    """Many rows: scales and rows of x of any magnitude, an infinity or NaN in one row of x, a scale of NaN in one row of the matrix."""
+    from ironpangu_b200.ops import int4
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    N, K, T = 150, 520, 40
+    q, s, z = _codes(N, K, 64, True, 7)
+    rowwise, token = torch.linspace(-30, 30, N, device="cuda"), torch.linspace(-60, 60, T, device="cuda")
+    s = (s.double() * torch.exp2(rowwise.round().double())[:, None]).to(BF16)
+    x = (torch.randn(T, K, generator=g, device="cuda").double() * torch.exp2(token.round().double())[:, None]).to(BF16)
+    x[:, 7] *= 2.0 ** -20                                # far below its row's largest
+    v = _values(q, s, z, 64)
+    w = int4.pack(q, s, z, group=64)
+    out = int4.linear(x, w, out_f32=True)
+    v, bound = _operands(v, x)
+    _close(out, x.double() @ v.T, bound)
+    s[5, 3] = float("nan")
+    x[3, 9], x[4, 10], x[6] = float("inf"), float("nan"), 0
+    bad = int4.linear(x, int4.pack(q, s, z, group=64), out_f32=True)
+    keep_n, keep_t = torch.ones(N, dtype=torch.bool, device="cuda"), torch.ones(T, dtype=torch.bool, device="cuda")
+    keep_n[5], keep_t[3], keep_t[4], keep_t[6] = False, False, False, False
+    assert torch.equal(bad[keep_t][:, keep_n], out[keep_t][:, keep_n]) and bool(bad[:, 5].isnan().all())
+    assert not bool(bad[3].isfinite().any()) and bool(bad[4].isnan().all()) and bool((bad[6, keep_n] == 0).all())
+    tiny = torch.full((20, K), 2.0 ** -133, dtype=BF16, device="cuda")
+    y, scale = int4.linear(tiny, w, out_f32=True), tiny.double().abs() @ v[:20].abs().T
+    # the smallest bf16 numbers: a result below f32's normal range has steps of 2^-149
+    _close(y, tiny.double() @ v.T, _operands(v, tiny)[1] + 2.0 ** -148)
