@@ -17,13 +17,17 @@
 // leave NaN as their part of the sum.
 #include <algorithm>
 
-#include "int4.cuh"
-#include "tc_common.cuh"
+#include "int4_tc.cuh"
 #include "ifab_kernels.h"
 
 using namespace ifab;
 using namespace ifab::tc;
 using namespace ifab::int4;
+
+namespace ifab::int4 {
+int pair_product(const View& v, const void* rows, const float* factor, const bf16* residual, long ldr, void* y, long ldy, int out_f32, int T, int tok, int pairs,
+                 uint32_t spin_limit, uint32_t* status, cudaStream_t s);      // int4_tc_pair.cu
+}
 
 namespace {
 
@@ -53,8 +57,6 @@ __device__ __forceinline__ float4 ld_part4(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
   return v;
 }
-// kind::f16 instruction descriptor: f16 x f16 -> f32, both operands K-major
-__device__ __forceinline__ uint32_t umma_idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 // D[tmem] (+)= A[tmem] * B[smem]; issued by ONE thread
 __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
   asm volatile(
@@ -64,19 +66,6 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, ui
       "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
-
-// eight weights of a word in f16: 1024 + q is an f16 whose last four bits are q, and the difference is exact. less: twice -(1024 + z), s2: twice the scale
-__device__ __forceinline__ void weights_of(uint32_t word, uint32_t less, uint32_t s2, uint32_t* out) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t d = ((word >> (4 * j)) & 0x000f000fu) | 0x64006400u;
-    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(d) : "r"(less));
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(out[j]) : "r"(d), "r"(s2));
-  }
-}
-// the exponent of a magnitude within -112 .. 127, so that its powers below are normal f32
-__device__ __forceinline__ int exponent_of(float most) { return max(min((int)(__float_as_uint(most) >> 23) - 127, 127), -112); }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // rows of x in f16 by a power of two each, which `factor` takes out again. A CTA a row
 __global__ void __launch_bounds__(256) rows_kernel(const bf16* x, long ldx, __half* out, long ldo, float* factor, int K) {
@@ -118,6 +107,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
   uint64_t *weights = full + STAGES, *empty = weights + STAGES, *acc_full = empty + STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ float factors[TOK];
   volatile int* requested = abort_flag + 1;      // blocks whose copies were requested, once no more will be; until then -1
   const View& v = p.v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,28 +130,11 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
   }
   // this thread's row: its units along K, and the first codes, which no kernel of the stream writes
   const int row = (warp & 3) * 32 + lane, group = (warp - 2) >> 2;
-  const unsigned char* unit = nullptr;
-  uint2 next[8];
-  uint16_t next_s[CHUNK / GROUP];
-  float by = 0.f;                    // the row's power of two
-  int next_z[CHUNK / GROUP];
-  const int g = row & 7, h = (row >> 3) & 1;
-  auto fetch = [&](int ch) {
-    const unsigned char* at = unit + (long)ch * v.unit;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) next[i] = *reinterpret_cast<const uint2*>(at + (i >> 2) * 512 + code_at(g, i & 3) + h * 8);
-#pragma unroll
-    for (int i = 0; i < CHUNK / GROUP; ++i) {
-      next_s[i] = *reinterpret_cast<const uint16_t*>(at + CODES + i * 32 + g * 4 + h * 2);
-      next_z[i] = ZEROS ? at[CODES + CHUNK / GROUP * 32 + i * 16 + g * 2 + h] : 8;
-    }
-  };
+  RowOfWeights<GROUP, ZEROS> mine;
   if (warp >= 2) {
     const int t = n0 / TILE + (gated ? (row & 63) : row) / TILE;
-    const int at = min(t, v.tiles - 1) + (gated && row >= 64 ? v.tiles : 0);
-    unit = v.at(at, c0);
-    by = power_of_two(11 - exponent_of(v.most[at * TILE + (row & 15)]));
-    if (group < nc) fetch(group);
+    mine.start(v, min(t, v.tiles - 1) + (gated && row >= 64 ? v.tiles : 0), row & 15);
+    if (group < nc) mine.fetch(c0 + group);
   }
   __syncthreads();
   grid_dep_wait();
@@ -171,6 +144,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
   tc_fence_after();
   grid_dep_launch();
   const uint32_t tmem_base = *tmem_slot;
+  if (threadIdx.x < TOK && m0 + threadIdx.x < p.T) factors[threadIdx.x] = p.factor[m0 + threadIdx.x];
 
   if (warp == 0 && lane == 0) {
     int issued = 0;
@@ -205,28 +179,14 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
 #pragma unroll 1
     for (int ch = group; ch < nc; ch += 2) {
-      uint2 codes[8];
-      uint32_t s2[CHUNK / GROUP], less[CHUNK / GROUP];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) codes[i] = next[i];
-#pragma unroll
-      for (int i = 0; i < CHUNK / GROUP; ++i) {
-        const __half2 s = __float2half2_rn(scales_of(next_s[i], v.f16).x * by);
-        s2[i] = *reinterpret_cast<const uint32_t*>(&s);
-        less[i] = 0xe400e400u | next_z[i] | next_z[i] << 16;
-      }
-      if (ch + 2 < nc) fetch(ch + 2);
+      mine.turn();
+      if (ch + 2 < nc) mine.fetch(c0 + ch + 2);
       bool ok = true;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int kb = 2 * ch + b, s = kb % STAGES;
         uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int lo = GROUP == 128 ? 0 : GROUP == 64 ? b : 2 * b, hi = GROUP == 32 ? lo + 1 : lo;
-          weights_of(codes[4 * b + i].x, less[lo], s2[lo], w + 4 * i);
-          weights_of(codes[4 * b + i].y, less[hi], s2[hi], w + 16 + 4 * i);
-        }
+        mine.block(b, w);
         if (kb >= STAGES && !mbar_wait(&empty[s], (kb / STAGES - 1) & 1, p.spin_limit)) *abort_flag = 1;
         ok = !__any_sync(0xffffffffu, *abort_flag);
         if (!ok) break;
@@ -262,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
       mbar_wait(acc_full, 0, DRAIN);
       for (int t = 0; t < tokens; ++t) sum[t * FT + row] = __int_as_float(0x7fffffff);
     } else {
-      const float out = __uint_as_float((254u << 23) - __float_as_uint(by));          // 1 / by
+      const float out = mine.out();
       for (int t0 = 0; t0 < tokens; t0 += 32) {
         float f[32];
         tmem_ld_32x32(tm + (uint32_t)t0, f);
@@ -295,7 +255,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     }
     const int live = min(4, v.N - col);
     const long m = m0 + t;
-    const float factor = p.factor[m];
+    const float factor = factors[t];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       a[e] *= factor;
@@ -333,6 +293,18 @@ int launch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
 
 }  // namespace
 
+// Tokens of a pair's tile (int4_tc_pair.cu): the width whose waves of tiles over the pairs take least, or 0 where the pairs would not have a tile each.
+static int pair_tokens(int T, int rows, int pairs) {
+  const int tn = ceil_div(rows, 2 * FT);
+  int best = 0;
+  long least = 0;
+  for (int tok = 256; tok >= 128; tok -= 16) {
+    const long tiles = (long)tn * ceil_div(T, tok), cost = (tiles + pairs - 1) / pairs * (tok + 32);
+    if (T > 128 && tiles * 8 >= 7l * pairs && (!least || cost < least)) least = cost, best = tok;
+  }
+  return best;
+}
+
 // bytes of the workspace of T rows
 extern "C" uint64_t ifab_int4_gemm_scratch(int T, int K) { return T < 1 || K < 8 ? 0 : (uint64_t)T * K * 2 + ((uint64_t)T * 4 + 15) / 16 * 16; }
 
@@ -345,7 +317,12 @@ extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const 
   float* factor = (float*)((char*)scratch + (uint64_t)T * p.v.K * 2);
   p.y = y, p.ldy = ldy, p.out_f32 = out_f32, p.residual = (const bf16*)residual, p.ldr = ldr, p.factor = factor, p.T = T, p.status = status;
   p.spin_limit = spin_limit;
-  const int ty = ceil_div(T, TOK), tiles = ceil_div(p.v.N, p.v.halves == 2 ? FT / 2 : FT), sms = device_sms();
+  const int halves = p.v.halves, sms = device_sms();
+  cudaStream_t s = (cudaStream_t)stream;
+  if (int rc = launch_chain(rows_kernel, dim3(T), dim3(256), 0, s, (const bf16*)x, ldx, rows, (long)p.v.K, factor, p.v.K)) return rc;
+  if (const int tok = pair_tokens(T, p.v.N * halves, sms / 2))
+    return pair_product(p.v, rows, factor, p.residual, ldr, y, ldy, out_f32, T, tok, std::min(sms / 2, ceil_div(p.v.N * halves, 2 * FT) * ceil_div(T, tok)), spin_limit, status, s);
+  const int ty = ceil_div(T, TOK), tiles = ceil_div(p.v.N, halves == 2 ? FT / 2 : FT);
   if (ty > 65535) return -1;
   p.tok = ceil_div(ceil_div(T, ty), 16) * 16;
   p.splits = 1;
@@ -353,8 +330,6 @@ extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const 
   CUtensorMap tx;          // of 16-bit elements: the type is the products' to know
   if (int rc = make_tmap_bf16_2d(&tx, rows, (uint64_t)T, (uint64_t)p.v.K, (uint64_t)p.v.K, (uint32_t)p.tok)) return rc;
   const dim3 grid(tiles * p.splits, ty);
-  cudaStream_t s = (cudaStream_t)stream;
-  if (int rc = launch_chain(rows_kernel, dim3(T), dim3(256), 0, s, (const bf16*)x, ldx, rows, (long)p.v.K, factor, p.v.K)) return rc;
   if (p.v.zeros) return p.v.group == 128 ? launch<128, true>(tx, p, grid, s) : p.v.group == 64 ? launch<64, true>(tx, p, grid, s) : launch<32, true>(tx, p, grid, s);
   return p.v.group == 128 ? launch<128, false>(tx, p, grid, s) : p.v.group == 64 ? launch<64, false>(tx, p, grid, s) : launch<32, false>(tx, p, grid, s);
 }

@@ -130,7 +130,7 @@ def test_quantise_groups_without_a_value():
 
 
 SHAPES = [(1, 8, 1), (16, 128, 1), (17, 72, 2), (1, 4096, 3), (300, 1032, 5), (1024, 1024, 1), (2741, 2056, 3), (2368, 264, 8), (5000, 136, 7), (64, 16392, 8), (200, 9000, 2),
-          (48, 640, 9), (333, 2056, 16), (70, 9000, 13), (130, 520, 21), (40, 264, 67), (1, 8, 17), (1237, 1032, 129), (5000, 136, 203), (333, 9000, 40), (129, 4096, 255), (300, 640, 1000)]
+          (48, 640, 9), (333, 2056, 16), (70, 9000, 13), (130, 520, 21), (40, 264, 67), (1, 8, 17), (1237, 1032, 129), (5000, 136, 203), (333, 9000, 40), (129, 4096, 255), (300, 640, 1000), (5000, 520, 700), (2741, 1032, 1501), (9500, 136, 300), (18000, 72, 140)]
 
 
 @pytest.mark.gpu
@@ -156,7 +156,7 @@ def test_linear(N, K, T, group, zeros, f16):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("group,zeros", [(128, False), (64, True), (32, True)])
-@pytest.mark.parametrize("F,K,T", [(1, 8, 1), (17, 264, 3), (150, 1544, 8), (3000, 512, 1), (16, 4096, 11), (1237, 1032, 5), (96, 520, 33), (1, 8, 17), (1237, 1032, 130), (65, 9000, 20), (200, 2048, 600)])
+@pytest.mark.parametrize("F,K,T", [(1, 8, 1), (17, 264, 3), (150, 1544, 8), (3000, 512, 1), (16, 4096, 11), (1237, 1032, 5), (96, 520, 33), (1, 8, 17), (1237, 1032, 130), (65, 9000, 20), (200, 2048, 600), (1237, 520, 1101), (5000, 264, 333), (2736, 1160, 500)])
 def test_gated(F, K, T, group, zeros):
     from ironpangu_b200.ops import int4
 
@@ -238,16 +238,19 @@ def test_streams_and_graphs():
 
 
 @pytest.mark.gpu
-def test_a_wait_that_runs_out():
+@pytest.mark.parametrize("T,N,gated", [(300, 700, False), (1300, 4100, False), (1300, 2052, True)])
+def test_a_wait_that_runs_out(T, N, gated):
     """With a limit of no polls every warp gives up at its first wait: the status word says so, the result is NaN and the next call is right."""
     from ironpangu_b200.ops import _lib, int4
 
-    q, s, z = _codes(700, 8192, 128, False, 1)
-    w, x = int4.pack(q, s, z, group=128), _rows(300, 8192, 1).contiguous()
+    K = 2048
+    q, s, z = _codes(N * (1 + gated), K, 128, False, 1)
+    w, x = int4.pack(q, s, z, group=128, gated=gated), _rows(T, K, 1).contiguous()
     want = int4.linear(x, w)
-    scratch = torch.empty(_lib.load().ifab_int4_gemm_scratch(300, 8192), dtype=torch.uint8, device="cuda")
-    status, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(300, 700, dtype=BF16, device="cuda")
-    _lib.check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), 8192, None, 0, out.data_ptr(), 700, 0, 300, scratch.data_ptr(), 0, status.data_ptr(), torch.cuda.current_stream().cuda_stream), "gemm")
+    scratch = torch.empty(_lib.load().ifab_int4_gemm_scratch(T, K), dtype=torch.uint8, device="cuda")
+    status, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(T, N, dtype=BF16, device="cuda")
+    _lib.check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), K, None, 0, out.data_ptr(), N, 0, T, scratch.data_ptr(), 0, status.data_ptr(), torch.cuda.current_stream().cuda_stream),
+               "gemm")
     torch.cuda.synchronize()
     assert int(status) == 2 and bool(out.isnan().all())
     status.zero_()
