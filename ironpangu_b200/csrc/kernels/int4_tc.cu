@@ -2,13 +2,14 @@
 //
 // The 128 rows of an MMA are weight rows, the tokens its columns. Weights become s (q - z) in registers, where a thread is a row, and go straight into tensor memory
 // as the MMA's first operand: neither codes nor weights pass through shared memory, whose bandwidth belongs to the tokens' tiles. Two groups of four warps take the
-// chunks of 128 columns in turn, with the codes of their next chunk on the way.
+// chunks of 128 columns in turn.
 // The operands are f16, each row with a power of two of its own. A product s (q - z) has up to 13 bits: bf16 leaves 8 of them, and a gated unit's result was off by 1.6
 // times its rounding; f16 leaves 11. Rows of x keep all their 8 bits: a launch ahead (rows_kernel) brings a row's largest magnitude to 2^14 .. 2^15, so that what falls below
 // f16's normal range is off by 2^-40 of that at most, and a row of weights has its largest scale at 2^11 .. 2^12 (15 of them stay below 65504). Both powers are taken out of
 // the f32 sums.
 //   warp 0      copies of the tokens' tiles (64 columns, 128-byte swizzle)
 //   warp 1      MMAs
+//   warp 10     copies of codes, the first of them ahead of the wait for the preceding kernel
 //   warps 2-9   weights into tensor memory; then 2-5 read the accumulator
 // Two CTAs an SM (128 columns of sums and four stages of 32 columns of weights each), so that one multiplies while the other starts or stores. With few tiles the
 // chunks along K are shared by the CTAs of a cluster: each leaves its part of the sum in its shared memory as f32 and every CTA adds up a share of the tokens over
@@ -31,8 +32,10 @@ int pair_product(const View& v, const void* rows, const float* factor, const bf1
 
 namespace {
 
-constexpr int FT = 128, BK = 64, TOK = 128, STAGES = 4, THREADS = 320;
-constexpr int STAGE = TOK * BK * 2, SMEM = STAGES * STAGE + 1024 + 256;
+constexpr int FT = 128, BK = 64, TOK = 128, STAGES = 4, CHUNKS = 4, THREADS = 352;
+constexpr int STAGE = TOK * BK * 2;
+template <int GROUP, bool ZEROS>
+constexpr int SMEM = STAGES * STAGE + CHUNKS * Units<GROUP, ZEROS>::BYTES + 1024 + 512;
 constexpr uint32_t COLS = 256, A_COL = 128;          // of tensor memory; first column of the weights' stages
 constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
 static_assert(TOK * FT * 4 <= STAGES * STAGE, "the part of the sum takes the ring's place");
@@ -101,11 +104,13 @@ __global__ void __launch_bounds__(256) rows_kernel(const bf16* x, long ldx, __ha
 // grid (feature tiles x splits, token tiles), clusters of `splits` along x
 template <int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, TcP p) {
+  using U = Units<GROUP, ZEROS>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
-  uint64_t *weights = full + STAGES, *empty = weights + STAGES, *acc_full = empty + STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  unsigned char* ring = smem + STAGES * STAGE;         // chunks of units
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + CHUNKS * U::BYTES);
+  uint64_t *weights = full + STAGES, *empty = weights + STAGES, *acc_full = empty + STAGES, *units_full = acc_full + 1, *units_empty = units_full + CHUNKS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units_empty + CHUNKS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ float factors[TOK];
   volatile int* requested = abort_flag + 1;      // blocks whose copies were requested, once no more will be; until then -1
@@ -122,21 +127,37 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
       mbar_init(&weights[s], 4);
       mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < CHUNKS; ++s) {
+      mbar_init(&units_full[s], 1);
+      mbar_init(&units_empty[s], 4);
+    }
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     *requested = -1;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_x);
   }
-  // this thread's row: its units along K, and the first codes, which no kernel of the stream writes
   const int row = (warp & 3) * 32 + lane, group = (warp - 2) >> 2;
-  RowOfWeights<GROUP, ZEROS> mine;
-  if (warp >= 2) {
-    const int t = n0 / TILE + (gated ? (row & 63) : row) / TILE;
-    mine.start(v, min(t, v.tiles - 1) + (gated && row >= 64 ? v.tiles : 0), row & 15);
-    if (group < nc) mine.fetch(c0 + group);
-  }
+  // the tile of sixteen rows that is unit u of this CTA's (a tile beyond the matrix: its last one, whose results are not stored): gate rows first
+  auto tile_of = [&](int u) { return min(n0 / TILE + (gated ? u & 3 : u), v.tiles - 1) + (gated && u >= 4 ? v.tiles : 0); };
   __syncthreads();
+  // Codes are written by no kernel of the stream: the first ones are on their way ahead of the wait
+  int chunk = 0;                                       // requested
+  const unsigned char* from = v.at(tile_of(lane & 7), c0);
+  auto request = [&]() {
+    const int q = chunk % CHUNKS;
+    if (lane == 0) mbar_expect_tx(&units_full[q], U::BYTES);
+    __syncwarp();
+    if (lane < 8) bulk_load(ring + q * U::BYTES + lane * U::UNIT, from + (long)chunk * U::UNIT, U::UNIT, &units_full[q]);
+    ++chunk;
+  };
+  if (warp == 10)
+    while (chunk < min(nc, CHUNKS)) request();
+  RowOfWeights<GROUP, ZEROS> mine;
+  if (warp >= 2 && warp < 10) {
+    mine.start(v, row >> 4, row & 15);
+    mine.scale(v.most[tile_of(row >> 4) * TILE + (row & 15)]);
+  }
   grid_dep_wait();
   if (warp == 1) tmem_alloc(tmem_slot, COLS);
   tc_fence_before();
@@ -175,12 +196,23 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
       umma_commit(&empty[s]);
     }
     umma_commit(acc_full);
+  } else if (warp == 10) {
+    while (chunk < nc) {
+      if (!mbar_wait(&units_empty[chunk % CHUNKS], (chunk / CHUNKS - 1) & 1, p.spin_limit)) *abort_flag = 1;
+      if (__any_sync(0xffffffffu, *abort_flag)) break;
+      request();
+    }
+    // what has been requested lands before the CTA ends, whoever gives up
+    for (int i = max(0, chunk - CHUNKS); i < chunk; ++i) mbar_wait(&units_full[i % CHUNKS], (i / CHUNKS) & 1, DRAIN);
   } else if (warp >= 2) {
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
 #pragma unroll 1
     for (int ch = group; ch < nc; ch += 2) {
-      mine.turn();
-      if (ch + 2 < nc) mine.fetch(c0 + ch + 2);
+      const int q = ch % CHUNKS;
+      if (!mbar_wait(&units_full[q], (ch / CHUNKS) & 1, p.spin_limit)) *abort_flag = 1;
+      mine.load(ring + q * U::BYTES, row & 15);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&units_empty[q]);
       bool ok = true;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -286,9 +318,10 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 template <int GROUP, bool ZEROS>
 int launch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
   auto k = int4_tc_kernel<GROUP, ZEROS>;
-  if (int rc = opt_in_smem(k, SMEM)) return rc;
-  if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(THREADS), (unsigned)p.splits, (size_t)SMEM, s, tx, p);
-  return launch_chain(k, grid, dim3(THREADS), (size_t)SMEM, s, tx, p);
+  constexpr int smem = SMEM<GROUP, ZEROS>;
+  if (int rc = opt_in_smem(k, smem)) return rc;
+  if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(THREADS), (unsigned)p.splits, (size_t)smem, s, tx, p);
+  return launch_chain(k, grid, dim3(THREADS), (size_t)smem, s, tx, p);
 }
 
 }  // namespace

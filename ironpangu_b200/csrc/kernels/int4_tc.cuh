@@ -21,49 +21,46 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 // kind::f16 instruction descriptor: f16 x f16 -> f32, both operands K-major
 __device__ __forceinline__ uint32_t umma_idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 
-// A thread's row of the matrix, chunk by chunk: codes, scales and zero points of the next chunk are on the way while the last one's become operands.
+// Units of a chunk of 128 rows in shared memory: eight of them back to back, brought by bulk copies. (With the codes of the next chunk in registers, a warp's other waits -
+// for its stores into tensor memory, for the barriers - waited for those loads too: 4096 rows of 2 x 16384 by 4096 1276 us on pairs, so SOON.)
+template <int GROUP, bool ZEROS>
+struct Units {
+  static constexpr int UNIT = CODES + CHUNK / GROUP * (ZEROS ? 48 : 32), BYTES = 8 * UNIT;
+};
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar)) : "memory");
+}
+
+// A thread's row (of 128) in a chunk
 template <int GROUP, bool ZEROS>
 struct RowOfWeights {
-  const unsigned char* unit;         // of the row's tile, first chunk
-  int step, f16, g, h;
+  using U = Units<GROUP, ZEROS>;
   float by;                          // the row's power of two
-  uint2 next[8], codes[8];
-  uint16_t next_s[CHUNK / GROUP];
-  uint8_t next_z[CHUNK / GROUP];
+  int at, f16;                       // of the row in a chunk's units
+  uint2 codes[8];
   uint32_t s2[CHUNK / GROUP], less[CHUNK / GROUP];
 
-  // row `r` (of sixteen) of tile `tile`
-  __device__ __forceinline__ void start(const View& v, int tile, int r) {
-    unit = v.at(tile, 0);
-    step = v.unit;
+  // unit `u` of the eight, row `r` of its sixteen
+  __device__ __forceinline__ void start(const View& v, int u, int r) {
+    at = u * U::UNIT + (r >> 3) * 8;
     f16 = v.f16;
-    g = r & 7;
-    h = r >> 3;
-    by = power_of_two(11 - exponent_of(v.most[tile * TILE + r]));
   }
+  __device__ __forceinline__ void scale(float most) { by = power_of_two(11 - exponent_of(most)); }
   __device__ __forceinline__ float out() const { return __uint_as_float((254u << 23) - __float_as_uint(by)); }       // 1 / by
-  __device__ __forceinline__ void fetch(int chunk) {
-    const unsigned char* at = unit + (long)chunk * step;
+  __device__ __forceinline__ void load(const unsigned char* chunk, int r) {
+    const int g = r & 7, h = r >> 3;
+    const unsigned char* unit = chunk + at - h * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) next[i] = *reinterpret_cast<const uint2*>(at + (i >> 2) * 512 + code_at(g, i & 3) + h * 8);
-#pragma unroll
-    for (int i = 0; i < CHUNK / GROUP; ++i) {
-      next_s[i] = *reinterpret_cast<const uint16_t*>(at + CODES + i * 32 + g * 4 + h * 2);
-      next_z[i] = ZEROS ? at[CODES + CHUNK / GROUP * 32 + i * 16 + g * 2 + h] : 8;
-    }
-  }
-  // what was fetched last becomes the chunk at hand
-  __device__ __forceinline__ void turn() {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) codes[i] = next[i];
+    for (int i = 0; i < 8; ++i) codes[i] = *reinterpret_cast<const uint2*>(chunk + at + (i >> 2) * 512 + code_at(g, i & 3));
 #pragma unroll
     for (int i = 0; i < CHUNK / GROUP; ++i) {
-      const __half2 s = __float2half2_rn(scales_of(next_s[i], f16).x * by);
+      const __half2 s = __float2half2_rn(scales_of(*reinterpret_cast<const uint16_t*>(unit + CODES + i * 32 + g * 4 + h * 2), f16).x * by);
+      const uint32_t z = ZEROS ? unit[CODES + CHUNK / GROUP * 32 + i * 16 + g * 2 + h] : 8;
       s2[i] = *reinterpret_cast<const uint32_t*>(&s);
-      less[i] = 0xe400e400u | next_z[i] | next_z[i] << 16;
+      less[i] = 0xe400e400u | z | z << 16;
     }
   }
-  // block b (64 columns) of the chunk at hand: 32 pairs in the order of the columns
+  // block b (64 columns) of the chunk: 32 pairs in the order of the columns
   __device__ __forceinline__ void block(int b, uint32_t (&w)[32]) const {
     const int lo = GROUP == 128 ? 0 : GROUP == 64 ? b : 2 * b, hi = GROUP == 32 ? lo + 1 : lo;
 #pragma unroll

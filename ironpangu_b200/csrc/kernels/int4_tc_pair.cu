@@ -7,6 +7,7 @@
 //   warp 0       copies of this CTA's half of the tokens; both CTAs' bytes complete on the leader's barrier
 //   warp 1       allocates tensor memory; in the leader, MMAs
 //   warps 2-9    this CTA's weights into its tensor memory (256 columns: eight stages), signalled to the leader
+//   warp 18      copies of this CTA's codes
 //   warps 10-17  sums out of tensor memory (256 columns), two warps for 32 rows. A lane is a weight row, so that a token's results leave as 64 bytes a warp. Gate and up rows
 //                lie in the two halves of a warp's rows, sixteen each: a lane gives every other token's value to its partner and has both of the others
 // Every wait is bounded; one that runs out raises the CTA's flag and the status word, tiles that are not complete are stored as NaN, and both CTAs meet at the closing barrier.
@@ -21,8 +22,10 @@ using namespace ifab::int4;
 
 namespace {
 
-constexpr int FT = 128, BK = 64, TOK = 256, STAGES = 8, THREADS = 576, READERS = 8;
-constexpr int STAGE = TOK / 2 * BK * 2, SMEM = STAGES * STAGE + 1024 + 256;
+constexpr int FT = 128, BK = 64, TOK = 256, STAGES = 8, CHUNKS = 6, THREADS = 608, READERS = 8;
+constexpr int STAGE = TOK / 2 * BK * 2;
+template <int GROUP, bool ZEROS>
+constexpr int SMEM = STAGES * STAGE + CHUNKS * Units<GROUP, ZEROS>::BYTES + 1024 + 512;
 constexpr uint32_t A_COL = 256;                      // first column of the weights' stages
 constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
 constexpr int RASTER = 8;                            // token tiles that pairs share weights over
@@ -50,7 +53,7 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // as mbar_wait, for a barrier that the peer arrives on
 __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, uint32_t limit) {
   for (uint32_t i = 0; i < limit; ++i) {
@@ -143,13 +146,16 @@ __device__ __forceinline__ void store32(const PairP& p, float (&f)[32], float ou
 // grid (2 * pairs), clusters of 2
 template <int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, PairP p) {
+  using U = Units<GROUP, ZEROS>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);       // leader's: both halves of the tokens
+  unsigned char* ring = smem + STAGES * STAGE;                               // chunks of units
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + CHUNKS * U::BYTES);    // leader's: both halves of the tokens
   uint64_t* weights = full + STAGES;                                         // leader's: an arrival of every warp that wrote rows of the stage
   uint64_t* empty = weights + STAGES;                                        // each CTA's own, as acc_full
   uint64_t *acc_full = empty + STAGES, *acc_empty = acc_full + 1;            // acc_empty: leader's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  uint64_t *units_full = acc_empty + 1, *units_empty = units_full + CHUNKS;   // each CTA's own
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units_empty + CHUNKS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const View& v = p.v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
@@ -158,11 +164,20 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
   const int per_cta = gated ? FT / 2 : FT;               // columns of the result
   const int tiles_n = (v.N + 2 * per_cta - 1) / (2 * per_cta), tiles_t = (p.T + p.tok - 1) / p.tok, tiles = tiles_n * tiles_t, nc = v.chunks, nk = 2 * nc;
 
+  // the tile of sixteen rows that is unit u of this CTA's part of a pair's tile (a tile beyond the matrix: its last one, whose results are not stored)
+  auto tile_of = [&](int tn, int u) {
+    const int at = (tn * 2 + rank) * (per_cta / TILE) + (gated ? u >> 1 : u);
+    return min(at, v.tiles - 1) + (gated && (u & 1) ? v.tiles : 0);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&weights[s], 8);
       mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < CHUNKS; ++s) {
+      mbar_init(&units_full[s], 1);
+      mbar_init(&units_empty[s], 4);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 2 * READERS);
@@ -197,11 +212,9 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
         load_pair(smem + s * STAGE, &tmap_x, in_leader(&full[s]), kb * BK, m);
       }
     }
-    if (*abort_flag) {
-      if (p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
-      if (rank == 0)                                     // what has been requested lands before the CTAs end
-        for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, DRAIN);
-    }
+    if (*abort_flag && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+    if (rank == 0)                                       // what has been requested lands before the CTAs end, whoever gives up
+      for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, DRAIN);
   } else if (warp == 1 && lane == 0 && rank == 0) {
     const uint32_t idesc = umma_idesc_f16(2 * FT, p.tok);
     uint32_t it = 0;
@@ -230,25 +243,25 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
   } else if (warp >= 2 && warp < 10) {
     const int group = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;
     RowOfWeights<GROUP, ZEROS> mine;
-    auto open = [&](int t) {                             // this thread's row of tile t, with its group's first chunk on the way
+    mine.start(v, row >> 4, row & 15);
+    uint32_t base = 0;                                   // chunks of the tiles ahead
+    bool ok = true;
+#pragma unroll 1
+    for (int t = pair; t < tiles && ok; t += pairs, base += nc) {
       int tt, tn;
       tile_at(t, tiles_t, tiles_n, &tt, &tn);
-      const int at = (tn * 2 + rank) * (per_cta / TILE) + (gated ? row >> 5 : row >> 4);
-      mine.start(v, min(at, v.tiles - 1) + (gated && lane >= 16 ? v.tiles : 0), row & 15);
-      if (group < nc) mine.fetch(group);
-    };
-    uint32_t base = 0;                                   // blocks of the tiles ahead
-    bool ok = true;
-    if (pair < tiles) open(pair);
-#pragma unroll 1
-    for (int t = pair; t < tiles && ok; t += pairs, base += nk) {
+      mine.scale(v.most[tile_of(tn, row >> 4) * TILE + (row & 15)]);
 #pragma unroll 1
       for (int ch = group; ch < nc && ok; ch += 2) {
-        mine.turn();
-        if (ch + 2 < nc) mine.fetch(ch + 2);
+        const uint32_t ic = base + ch;
+        const int q = ic % CHUNKS;
+        if (!mbar_wait(&units_full[q], (ic / CHUNKS) & 1, p.spin_limit)) *abort_flag = 1;
+        mine.load(ring + q * U::BYTES, row & 15);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&units_empty[q]);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const uint32_t it = base + 2 * ch + b;
+          const uint32_t it = 2 * ic + b;
           const int s = it % STAGES;
           uint32_t w[32];
           mine.block(b, w);
@@ -263,10 +276,27 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
           if (lane == 0) arrive_cluster(in_leader(&weights[s]));
         }
       }
-      if (ok && t + pairs < tiles) open(t + pairs);
     }
     if (!ok && lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
-  } else if (warp >= 10) {
+  } else if (warp == 18) {
+    uint32_t ic = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      int tt, tn;
+      tile_at(t, tiles_t, tiles_n, &tt, &tn);
+      const unsigned char* from = v.at(tile_of(tn, lane & 7), 0);
+      for (int ch = 0; ch < nc; ++ch, ++ic) {
+        const int q = ic % CHUNKS;
+        if (ic >= CHUNKS && !mbar_wait(&units_empty[q], (ic / CHUNKS - 1) & 1, p.spin_limit)) *abort_flag = 1;
+        ok = !__any_sync(0xffffffffu, *abort_flag);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&units_full[q], U::BYTES);
+        __syncwarp();
+        if (lane < 8) bulk_load(ring + q * U::BYTES + lane * U::UNIT, from + (long)ch * U::UNIT, U::UNIT, &units_full[q]);
+      }
+    }
+    for (uint32_t i = ic > CHUNKS ? ic - CHUNKS : 0; i < ic; ++i) mbar_wait(&units_full[i % CHUNKS], (i / CHUNKS) & 1, DRAIN);
+  } else if (warp >= 10 && warp < 18) {
     const int half = (warp - 10) >> 2, row = (warp & 3) * 32 + lane;
     bool ok = true;
     int j = 0;
@@ -275,8 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       int tt, tn;
       tile_at(t, tiles_t, tiles_n, &tt, &tn);
       const int n0 = (tn * 2 + rank) * per_cta, n = n0 + (gated ? (row >> 5) * 16 + (lane & 15) : row), m = tt * p.tok, tokens = min(p.tok, p.T - m);
-      const int at = min(n0 / TILE + (gated ? row >> 5 : row >> 4), v.tiles - 1) + (gated && lane >= 16 ? v.tiles : 0);
-      const float out = power_of_two(exponent_of(v.most[at * TILE + (row & 15)]) - 11);
+      const float out = power_of_two(exponent_of(v.most[tile_of(tn, row >> 4) * TILE + (row & 15)]) - 11);
       if (ok && !mbar_wait(acc_full, j & 1, p.spin_limit)) *abort_flag = 1;
       if (__any_sync(0xffffffffu, *abort_flag)) {
         if (ok && lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
@@ -314,8 +343,9 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
 template <int GROUP, bool ZEROS>
 int launch(const CUtensorMap& tx, const PairP& p, int pairs, cudaStream_t s) {
   auto k = int4_tc_pair_kernel<GROUP, ZEROS>;
-  if (int rc = opt_in_smem(k, SMEM)) return rc;
-  return launch_chain_cluster(k, dim3(2 * pairs), dim3(THREADS), 2, (size_t)SMEM, s, tx, p);
+  constexpr int smem = SMEM<GROUP, ZEROS>;
+  if (int rc = opt_in_smem(k, smem)) return rc;
+  return launch_chain_cluster(k, dim3(2 * pairs), dim3(THREADS), 2, (size_t)smem, s, tx, p);
 }
 
 }  // namespace
