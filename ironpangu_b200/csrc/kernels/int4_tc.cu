@@ -206,34 +206,39 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     for (int i = max(0, chunk - CHUNKS); i < chunk; ++i) mbar_wait(&units_full[i % CHUNKS], (i / CHUNKS) & 1, DRAIN);
   } else if (warp >= 2) {
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    int written = -1;                                    // a stage is signalled when the next one's operands are there
+    auto settle = [&]() {
+      if (written < 0) return;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&weights[written]);
+    };
 #pragma unroll 1
     for (int ch = group; ch < nc; ch += 2) {
       const int q = ch % CHUNKS;
-      if (!mbar_wait(&units_full[q], (ch / CHUNKS) & 1, p.spin_limit)) *abort_flag = 1;
+      bool late = !mbar_wait(&units_full[q], (ch / CHUNKS) & 1, p.spin_limit);
       mine.load(ring + q * U::BYTES, row & 15);
       __syncwarp();
       if (lane == 0) mbar_arrive(&units_empty[q]);
-      bool ok = true;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int kb = 2 * ch + b, s = kb % STAGES;
         uint32_t w[32];
         mine.block(b, w);
-        if (kb >= STAGES && !mbar_wait(&empty[s], (kb / STAGES - 1) & 1, p.spin_limit)) *abort_flag = 1;
-        ok = !__any_sync(0xffffffffu, *abort_flag);
-        if (!ok) break;
+        settle();                                        // the block before this one
+        if (kb >= STAGES) late |= !mbar_wait(&empty[s], (kb / STAGES - 1) & 1, p.spin_limit);
         tc_fence_after();
         tmem_st_32x32(tmem_base + A_COL + s * 32 + lanes, reinterpret_cast<const float*>(w));
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&weights[s]);
+        written = s;
       }
-      if (!ok) {
+      if (late) *abort_flag = 1;
+      if (__any_sync(0xffffffffu, *abort_flag)) {
         if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
         break;
       }
     }
+    settle();
   }
   __syncwarp();
   // The accumulator complete, all copies have landed and all products have read the ring: it becomes this CTA's part of the sum, [tokens][128].
@@ -292,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     for (int e = 0; e < 4; ++e) {
       a[e] *= factor;
       u[e] *= factor;
-      if (gated) a[e] = a[e] / (1.f + __expf(-a[e])) * u[e];
+      if (gated) a[e] = gated_unit(a[e], u[e]);
       if (p.residual && e < live) a[e] += __bfloat162float(p.residual[m * p.ldr + col + e]);
     }
     if (p.out_f32) {

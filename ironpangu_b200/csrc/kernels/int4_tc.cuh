@@ -31,6 +31,14 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
   asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar)) : "memory");
 }
 
+// silu(a) u, off by a few steps of f32: the exponential is at most 1 and the divisor between 1 and 2
+__device__ __forceinline__ float gated_unit(float a, float u) {
+  const float e = __expf(-fabsf(a));
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return (a >= 0.f ? a : a * e) * r * u;
+}
+
 // A thread's row (of 128) in a chunk
 template <int GROUP, bool ZEROS>
 struct RowOfWeights {

@@ -12,6 +12,7 @@
 //                lie in the two halves of a warp's rows, sixteen each: a lane gives every other token's value to its partner and has both of the others
 // Every wait is bounded; one that runs out raises the CTA's flag and the status word, tiles that are not complete are stored as NaN, and both CTAs meet at the closing barrier.
 #include <algorithm>
+#include <type_traits>
 
 #include "int4_tc.cuh"
 #include "ifab_kernels.h"
@@ -96,50 +97,36 @@ __device__ __forceinline__ void tile_at(int t, int tiles_t, int tiles_n, int* tt
   *tn = within / rows;
 }
 
-// 32 tokens from m on of this lane's row; `f`: the sums
-template <bool GATED>
-__device__ __forceinline__ void store32(const PairP& p, float (&f)[32], float out, int n, int m, int live, int lane) {
-  const float mine = lane < live ? p.factor[m + lane] : 0.f;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] *= out;
+template <bool F32>
+__device__ __forceinline__ void put(void* y, long at, float v) {
+  if (F32) reinterpret_cast<float*>(y)[at] = v;
+  else reinterpret_cast<bf16*>(y)[at] = __float2bfloat16_rn(v);
+}
+// Tokens 0 .. live - 1 (of 32) of this lane's row; `f`: the sums, `factor`: of token `lane`; y and the residual from the first token's result on
+template <bool GATED, bool F32, bool WHOLE>
+__device__ __forceinline__ void store32(float (&f)[32], float out, float factor, void* y, long ldy, const bf16* residual, long ldr, int live, bool there, int lane) {
   if constexpr (GATED) {
     const bool up = lane >= 16;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float got = __shfl_xor_sync(0xffffffffu, up ? f[2 * i] : f[2 * i + 1], 16), kept = up ? f[2 * i + 1] : f[2 * i];
-      const float factor = __shfl_sync(0xffffffffu, mine, 2 * i + up);
-      const float a = (up ? got : kept) * factor, u = (up ? kept : got) * factor;
-      f[i] = a / (1.f + __expf(-a)) * u;
-    }
-    if (n < p.v.N) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = 2 * i + up;
-        if (t >= live) break;
-        const long at = (long)(m + t) * p.ldy + n;
-        if (p.out_f32) reinterpret_cast<float*>(p.y)[at] = f[i];
-        else reinterpret_cast<bf16*>(p.y)[at] = __float2bfloat16_rn(f[i]);
-      }
+      const float lo = f[2 * i] * out, hi = f[2 * i + 1] * out, got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, 16), by = __shfl_sync(0xffffffffu, factor, 2 * i + up);
+      const float v = gated_unit((up ? got : lo) * by, (up ? hi : got) * by);
+      if (there && (WHOLE || 2 * i + up < live)) put<F32>(y, (2 * i + up) * ldy, v);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] *= __shfl_sync(0xffffffffu, mine, i);
-    if (n >= p.v.N) return;
-    if (p.residual) {
-      const bf16* r = p.residual + (long)m * p.ldr + n;
-      bf16 v[32];
+    for (int i = 0; i < 32; ++i) f[i] = f[i] * out * __shfl_sync(0xffffffffu, factor, i);
+    if (!there) return;
+    if (residual) {
+      bf16 r[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = i < live ? r[i * p.ldr] : __float2bfloat16_rn(0.f);
+      for (int i = 0; i < 32; ++i) r[i] = WHOLE || i < live ? residual[i * ldr] : __float2bfloat16_rn(0.f);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] += __bfloat162float(v[i]);
+      for (int i = 0; i < 32; ++i) f[i] += __bfloat162float(r[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (i >= live) break;
-      const long at = (long)(m + i) * p.ldy + n;
-      if (p.out_f32) reinterpret_cast<float*>(p.y)[at] = f[i];
-      else reinterpret_cast<bf16*>(p.y)[at] = __float2bfloat16_rn(f[i]);
-    }
+    for (int i = 0; i < 32; ++i)
+      if (WHOLE || i < live) put<F32>(y, i * ldy, f[i]);
   }
 }
 
@@ -246,6 +233,16 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
     mine.start(v, row >> 4, row & 15);
     uint32_t base = 0;                                   // chunks of the tiles ahead
     bool ok = true;
+    // A stage is signalled when the next one's operands are there: the wait for its stores costs nothing then. (Each block signalled at once: a group of warps took 1400
+    // cycles for a chunk, the products 1024.)
+    int written = -1;
+    auto settle = [&]() {
+      if (written < 0) return;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(in_leader(&weights[written]));
+    };
 #pragma unroll 1
     for (int t = pair; t < tiles && ok; t += pairs, base += nc) {
       int tt, tn;
@@ -255,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       for (int ch = group; ch < nc && ok; ch += 2) {
         const uint32_t ic = base + ch;
         const int q = ic % CHUNKS;
-        if (!mbar_wait(&units_full[q], (ic / CHUNKS) & 1, p.spin_limit)) *abort_flag = 1;
+        bool late = !mbar_wait(&units_full[q], (ic / CHUNKS) & 1, p.spin_limit);
         mine.load(ring + q * U::BYTES, row & 15);
         __syncwarp();
         if (lane == 0) mbar_arrive(&units_empty[q]);
@@ -265,18 +262,17 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
           const int s = it % STAGES;
           uint32_t w[32];
           mine.block(b, w);
-          if (it >= STAGES && !mbar_wait(&empty[s], (it / STAGES - 1) & 1, p.spin_limit)) *abort_flag = 1;
-          ok = !__any_sync(0xffffffffu, *abort_flag);
-          if (!ok) break;
+          settle();                                      // the block before this one
+          if (it >= STAGES) late |= !mbar_wait(&empty[s], (it / STAGES - 1) & 1, p.spin_limit);
           tc_fence_after();
           tmem_st_32x32(tmem_base + A_COL + s * 32 + quarter, reinterpret_cast<const float*>(w));
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_cluster(in_leader(&weights[s]));
+          written = s;
         }
+        if (late) *abort_flag = 1;
+        ok = !__any_sync(0xffffffffu, *abort_flag);
       }
     }
+    settle();
     if (!ok && lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
   } else if (warp == 18) {
     uint32_t ic = 0;
@@ -322,8 +318,20 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = __int_as_float(0x7fffffff);
         }
-        if (gated) store32<true>(p, f, out, n, m + c, min(32, tokens - c), lane);
-        else store32<false>(p, f, out, n, m + c, min(32, tokens - c), lane);
+        const int live = min(32, tokens - c);
+        const float factor = lane < live ? p.factor[m + c + lane] : 0.f;
+        const long first = (long)(m + c) * p.ldy + n;
+        void* y = p.out_f32 ? (void*)(reinterpret_cast<float*>(p.y) + first) : (void*)(reinterpret_cast<bf16*>(p.y) + first);
+        const bf16* residual = p.residual ? p.residual + (long)(m + c) * p.ldr + n : nullptr;
+        const bool there = n < v.N;
+        auto store = [&](auto g, auto f32) {
+          if (live == 32) store32<decltype(g)::value, decltype(f32)::value, true>(f, out, factor, y, p.ldy, residual, p.ldr, 32, there, lane);
+          else store32<decltype(g)::value, decltype(f32)::value, false>(f, out, factor, y, p.ldy, residual, p.ldr, live, there, lane);
+        };
+        using yes = std::true_type;
+        using no = std::false_type;
+        if (gated) p.out_f32 ? store(yes{}, yes{}) : store(yes{}, no{});
+        else p.out_f32 ? store(no{}, yes{}) : store(no{}, no{});
       }
       tc_fence_before();
       __syncwarp();
