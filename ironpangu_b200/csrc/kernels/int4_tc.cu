@@ -75,14 +75,23 @@ __global__ void __launch_bounds__(256) rows_kernel(const bf16* x, long ldx, __ha
   __shared__ float red[8];
   grid_dep_launch();
   grid_dep_wait();
-  const bf16* row = x + (long)blockIdx.x * ldx;
+  const uint4* row = reinterpret_cast<const uint4*>(x + (long)blockIdx.x * ldx);
+  uint4* to = reinterpret_cast<uint4*>(out + (long)blockIdx.x * ldo);
+  constexpr int HELD = 4;              // pieces of eight columns that a thread keeps: rows of up to 8192 are read once
+  const int pieces = K / 8, first = threadIdx.x;
+  uint4 held[HELD];
   float most = 0.f;
-  for (int i = threadIdx.x; i < K / 8; i += 256) {
+  auto widest = [&](const uint4& u) {
     float f[8];
-    unpack8(*reinterpret_cast<const uint4*>(row + i * 8), f);
+    unpack8(u, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) <= 3.4028234e38f ? fabsf(f[e]) : 0.f);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) held[i] = first + i * 256 < pieces ? row[first + i * 256] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) widest(held[i]);
+  for (int c = first + HELD * 256; c < pieces; c += 256) widest(row[c]);
   most = warp_max(most);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
   __syncthreads();
@@ -90,15 +99,19 @@ __global__ void __launch_bounds__(256) rows_kernel(const bf16* x, long ldx, __ha
   const int e = exponent_of(most);
   const float by = power_of_two(min(14 - e, 126));
   if (threadIdx.x == 0) factor[blockIdx.x] = power_of_two(max(e - 14, -126));
-  for (int i = threadIdx.x; i < K / 8; i += 256) {
+  auto scaled = [&](const uint4& in) {
     float f[8];
-    unpack8(*reinterpret_cast<const uint4*>(row + i * 8), f);
+    unpack8(in, f);
     uint4 u;
     __half2* h = reinterpret_cast<__half2*>(&u);
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(f[2 * j] * by, f[2 * j + 1] * by);
-    *reinterpret_cast<uint4*>(out + (long)blockIdx.x * ldo + i * 8) = u;
-  }
+    return u;
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if (first + i * 256 < pieces) to[first + i * 256] = scaled(held[i]);
+  for (int c = first + HELD * 256; c < pieces; c += 256) to[c] = scaled(row[c]);
 }
 
 // grid (feature tiles x splits, token tiles), clusters of `splits` along x

@@ -2,14 +2,15 @@
 // rows (a gate | up matrix: 128 features) by up to 256 tokens.
 //
 // A lone CTA with 128 weight rows loads 16 KB of tokens for 256 cycles of products, as much as an SM gets out of L2; a pair shares the tokens' tile, half in each CTA's
-// shared memory (tcgen05.mma.cta_group::2), and each CTA brings its 128 rows of weights into its own tensor memory. One pair an SM pair walks the tiles; copies and
-// weights of the next tile go on while this one's sums are stored.
+// shared memory (tcgen05.mma.cta_group::2), and each CTA makes its 128 rows of weights. One pair an SM pair walks the tiles, with two sums in tensor memory: while one is
+// stored, the next tile's products go into the other.
 //   warp 0       copies of this CTA's half of the tokens; both CTAs' bytes complete on the leader's barrier
 //   warp 1       allocates tensor memory; in the leader, MMAs
-//   warps 2-9    this CTA's weights into its tensor memory (256 columns: eight stages), signalled to the leader
-//   warp 18      copies of this CTA's codes
-//   warps 10-17  sums out of tensor memory (256 columns), two warps for 32 rows. A lane is a weight row, so that a token's results leave as 64 bytes a warp. Gate and up rows
-//                lie in the two halves of a warp's rows, sixteen each: a lane gives every other token's value to its partner and has both of the others
+//   warp 2       copies of this CTA's codes
+//   warps 3-10   this CTA's weights into its shared memory, signalled to the leader; two groups take the chunks of 128 columns in turn
+//   warps 11-18  sums out of tensor memory, two warps for 32 rows. A lane is a weight row, so that a token's results leave as 64 bytes a warp. Gate and up rows lie in the two halves of a warp's
+//                rows, sixteen each: a lane gives every other token's value to its partner and has both of the others
+// Weights go by way of shared memory: in tensor memory, where the MMA takes its first operand as well (int4_tc.cu), they leave no room for a second sum.
 // Every wait is bounded; one that runs out raises the CTA's flag and the status word, tiles that are not complete are stored as NaN, and both CTAs meet at the closing barrier.
 #include <algorithm>
 #include <type_traits>
@@ -23,11 +24,11 @@ using namespace ifab::int4;
 
 namespace {
 
-constexpr int FT = 128, BK = 64, TOK = 256, STAGES = 8, CHUNKS = 6, THREADS = 608, READERS = 8;
-constexpr int STAGE = TOK / 2 * BK * 2;
+constexpr int FT = 128, BK = 64, TOK = 256, STAGES = 6, CHUNKS = 3, THREADS = 608, READERS = 8;
+constexpr int W_BYTES = FT * BK * 2, STAGE = W_BYTES + TOK / 2 * BK * 2;      // weights, then tokens
 template <int GROUP, bool ZEROS>
 constexpr int SMEM = STAGES * STAGE + CHUNKS * Units<GROUP, ZEROS>::BYTES + 1024 + 512;
-constexpr uint32_t A_COL = 256;                      // first column of the weights' stages
+constexpr uint32_t SUM_COLS = 256;                   // of tensor memory
 constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
 constexpr int RASTER = 8;                            // token tiles that pairs share weights over
 
@@ -55,35 +56,19 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// as mbar_wait, for a barrier that the peer arrives on
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, uint32_t limit) {
-  for (uint32_t i = 0; i < limit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (i > 256) __nanosleep(64);
-  }
-  return false;
-}
 // this CTA's tile; its bytes go to the barrier at `bar` (the leader's)
 __device__ __forceinline__ void load_pair(void* dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)), "l"(m), "r"(bar),
                "r"(x), "r"(y)
                : "memory");
 }
-// D[tmem of both] (+)= A[tmem of both] * B[smem of both]; issued by ONE thread of the leader
-__device__ __forceinline__ void umma_f16_pair_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+// D[tmem of both] (+)= A[smem of both] * B[smem of both]; issued by ONE thread of the leader
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"((uint32_t)accumulate)
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 // arrive on the barrier at this place in both CTAs once the products issued so far have completed
@@ -102,30 +87,39 @@ __device__ __forceinline__ void put(void* y, long at, float v) {
   if (F32) reinterpret_cast<float*>(y)[at] = v;
   else reinterpret_cast<bf16*>(y)[at] = __float2bfloat16_rn(v);
 }
-// Tokens 0 .. live - 1 (of 32) of this lane's row; `f`: the sums, `factor`: of token `lane`; y and the residual from the first token's result on
+// 32 lanes x 16 consecutive f32 columns
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
+// Tokens 0 .. live - 1 (of 16) of this lane's row; `f`: the sums, `factor`: of token `lane & 15`; y and the residual from the first token's result on
 template <bool GATED, bool F32, bool WHOLE>
-__device__ __forceinline__ void store32(float (&f)[32], float out, float factor, void* y, long ldy, const bf16* residual, long ldr, int live, bool there, int lane) {
+__device__ __forceinline__ void store16(float (&f)[16], float out, float factor, void* y, long ldy, const bf16* residual, long ldr, int live, bool there, int lane) {
   if constexpr (GATED) {
     const bool up = lane >= 16;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const float lo = f[2 * i] * out, hi = f[2 * i + 1] * out, got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, 16), by = __shfl_sync(0xffffffffu, factor, 2 * i + up);
       const float v = gated_unit((up ? got : lo) * by, (up ? hi : got) * by);
       if (there && (WHOLE || 2 * i + up < live)) put<F32>(y, (2 * i + up) * ldy, v);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = f[i] * out * __shfl_sync(0xffffffffu, factor, i);
+    for (int i = 0; i < 16; ++i) f[i] = f[i] * out * __shfl_sync(0xffffffffu, factor, i);
     if (!there) return;
     if (residual) {
-      bf16 r[32];
+      bf16 r[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = WHOLE || i < live ? residual[i * ldr] : __float2bfloat16_rn(0.f);
+      for (int i = 0; i < 16; ++i) r[i] = WHOLE || i < live ? residual[i * ldr] : __float2bfloat16_rn(0.f);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] += __bfloat162float(r[i]);
+      for (int i = 0; i < 16; ++i) f[i] += __bfloat162float(r[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 16; ++i)
       if (WHOLE || i < live) put<F32>(y, i * ldy, f[i]);
   }
 }
@@ -137,11 +131,10 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* ring = smem + STAGES * STAGE;                               // chunks of units
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + CHUNKS * U::BYTES);    // leader's: both halves of the tokens
-  uint64_t* weights = full + STAGES;                                         // leader's: an arrival of every warp that wrote rows of the stage
-  uint64_t* empty = weights + STAGES;                                        // each CTA's own, as acc_full
-  uint64_t *acc_full = empty + STAGES, *acc_empty = acc_full + 1;            // acc_empty: leader's
-  uint64_t *units_full = acc_empty + 1, *units_empty = units_full + CHUNKS;   // each CTA's own
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + CHUNKS * U::BYTES);    // leader's: both halves of the tokens, and an arrival of every warp that wrote weights
+  uint64_t* empty = full + STAGES;                                           // each CTA's own, as acc_full
+  uint64_t *acc_full = empty + STAGES, *acc_empty = acc_full + 2;            // of each sum; acc_empty: leader's
+  uint64_t *units_full = acc_empty + 2, *units_empty = units_full + CHUNKS;   // each CTA's own
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units_empty + CHUNKS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const View& v = p.v;
@@ -158,16 +151,17 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&weights[s], 8);
+      mbar_init(&full[s], 1 + 8);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < CHUNKS; ++s) {
       mbar_init(&units_full[s], 1);
       mbar_init(&units_empty[s], 4);
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 2 * READERS);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * READERS);
+    }
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_x);
@@ -196,53 +190,51 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
         if (it >= STAGES && !mbar_wait(&empty[s], (it / STAGES - 1) & 1, p.spin_limit)) *abort_flag = 1;
         if (*abort_flag) break;
         if (rank == 0) mbar_expect_tx(&full[s], p.tok * BK * 2);
-        load_pair(smem + s * STAGE, &tmap_x, in_leader(&full[s]), kb * BK, m);
+        load_pair(smem + s * STAGE + W_BYTES, &tmap_x, in_leader(&full[s]), kb * BK, m);
       }
     }
     if (*abort_flag && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
     if (rank == 0)                                       // what has been requested lands before the CTAs end, whoever gives up
       for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, DRAIN);
-  } else if (warp == 1 && lane == 0 && rank == 0) {
-    const uint32_t idesc = umma_idesc_f16(2 * FT, p.tok);
-    uint32_t it = 0;
-    int j = 0;
+  } else if (warp == 1 && rank == 0) {
+    // The whole warp walks and one lane issues: a block's products take 512 cycles, and with a lane alone on this path, two barriers to look at and stages by division the path
+    // took 930.
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+    const uint32_t idesc = umma_idesc_f16(2 * FT, p.tok), at = smem_u32(smem);
+    const uint64_t first = umma_desc_sw128(at);
+    int s = 0, j = 0;
+    uint32_t parity = 0;
     bool ok = true;
     for (int t = pair; t < tiles && ok; t += pairs, ++j) {
-      if (j && !wait_cluster(acc_empty, (j - 1) & 1, p.spin_limit)) { ok = false; break; }
+      const uint32_t d = tmem_base + (j & 1) * SUM_COLS;
+      ok = j < 2 || mbar_wait(&acc_empty[j & 1], ((j >> 1) - 1) & 1, p.spin_limit);
       tc_fence_after();
-      for (int kb = 0; kb < nk; ++kb, ++it) {
-        const int s = it % STAGES;
-        const uint32_t parity = (it / STAGES) & 1;
-        if (!wait_cluster(&full[s], parity, p.spin_limit) || !wait_cluster(&weights[s], parity, p.spin_limit) || *abort_flag) { ok = false; break; }
+#pragma unroll 1
+      for (int kb = 0; kb < nk && ok; ++kb) {
+        ok = mbar_wait(&full[s], parity, p.spin_limit);
         tc_fence_after();
-        const uint64_t db = umma_desc_sw128(smem_u32(smem + s * STAGE));
-        const uint32_t a = tmem_base + A_COL + s * 32;
+        if (ok && elected) {
+          const uint64_t da = first + (uint64_t)(s * (STAGE >> 4)), db = da + (W_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k) umma_f16_pair_ta(tmem_base, a + 8 * k, db + (uint64_t)(2 * k), idesc, kb > 0 || k > 0);
-        commit_pair(&empty[s]);
+          for (int k = 0; k < BK / 16; ++k) umma_f16_pair(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, kb > 0 || k > 0);
+          commit_pair(&empty[s]);
+        }
+        if (++s == STAGES) s = 0, parity ^= 1;
       }
-      commit_pair(acc_full);
+      ok = !__any_sync(0xffffffffu, !ok || *abort_flag);
+      if (ok && elected) commit_pair(&acc_full[j & 1]);
     }
     if (!ok) {
       *abort_flag = 1;
-      if (p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+      if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
     }
-  } else if (warp >= 2 && warp < 10) {
-    const int group = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;
+  } else if (warp >= 3 && warp < 11) {
+    const int group = (warp - 3) >> 2, row = ((warp - 3) & 3) * 32 + lane;
     RowOfWeights<GROUP, ZEROS> mine;
     mine.start(v, row >> 4, row & 15);
     uint32_t base = 0;                                   // chunks of the tiles ahead
     bool ok = true;
-    // A stage is signalled when the next one's operands are there: the wait for its stores costs nothing then. (Each block signalled at once: a group of warps took 1400
-    // cycles for a chunk, the products 1024.)
-    int written = -1;
-    auto settle = [&]() {
-      if (written < 0) return;
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_cluster(in_leader(&weights[written]));
-    };
 #pragma unroll 1
     for (int t = pair; t < tiles && ok; t += pairs, base += nc) {
       int tt, tn;
@@ -262,19 +254,21 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
           const int s = it % STAGES;
           uint32_t w[32];
           mine.block(b, w);
-          settle();                                      // the block before this one
           if (it >= STAGES) late |= !mbar_wait(&empty[s], (it / STAGES - 1) & 1, p.spin_limit);
-          tc_fence_after();
-          tmem_st_32x32(tmem_base + A_COL + s * 32 + quarter, reinterpret_cast<const float*>(w));
-          written = s;
+          // a row of 128 bytes in pieces of 16, where the 128-byte swizzle has them
+          uint4* to = reinterpret_cast<uint4*>(smem + s * STAGE + row * 128);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) to[i ^ (row & 7)] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) arrive_cluster(in_leader(&full[s]));
         }
         if (late) *abort_flag = 1;
         ok = !__any_sync(0xffffffffu, *abort_flag);
       }
     }
-    settle();
     if (!ok && lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
-  } else if (warp == 18) {
+  } else if (warp == 2) {
     uint32_t ic = 0;
     bool ok = true;
     for (int t = pair; t < tiles && ok; t += pairs) {
@@ -292,8 +286,8 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       }
     }
     for (uint32_t i = ic > CHUNKS ? ic - CHUNKS : 0; i < ic; ++i) mbar_wait(&units_full[i % CHUNKS], (i / CHUNKS) & 1, DRAIN);
-  } else if (warp >= 10 && warp < 18) {
-    const int half = (warp - 10) >> 2, row = (warp & 3) * 32 + lane;
+  } else if (warp >= 11) {
+    const int half = (warp - 11) >> 2, row = (warp & 3) * 32 + lane;
     bool ok = true;
     int j = 0;
 #pragma unroll 1
@@ -302,31 +296,31 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       tile_at(t, tiles_t, tiles_n, &tt, &tn);
       const int n0 = (tn * 2 + rank) * per_cta, n = n0 + (gated ? (row >> 5) * 16 + (lane & 15) : row), m = tt * p.tok, tokens = min(p.tok, p.T - m);
       const float out = power_of_two(exponent_of(v.most[tile_of(tn, row >> 4) * TILE + (row & 15)]) - 11);
-      if (ok && !mbar_wait(acc_full, j & 1, p.spin_limit)) *abort_flag = 1;
+      if (ok && !mbar_wait(&acc_full[j & 1], (j >> 1) & 1, p.spin_limit)) *abort_flag = 1;
       if (__any_sync(0xffffffffu, *abort_flag)) {
         if (ok && lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
         ok = false;
       }
       tc_fence_after();
 #pragma unroll 1
-      for (int c = half * 32; c < tokens; c += 64) {
-        float f[32];
+      for (int c = half * 16; c < tokens; c += 32) {
+        float f[16];
         if (ok) {
-          tmem_ld_32x32(tmem_base + quarter + (uint32_t)c, f);
+          tmem_ld_32x16(tmem_base + quarter + (j & 1) * SUM_COLS + (uint32_t)c, f);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __int_as_float(0x7fffffff);
+          for (int i = 0; i < 16; ++i) f[i] = __int_as_float(0x7fffffff);
         }
-        const int live = min(32, tokens - c);
-        const float factor = lane < live ? p.factor[m + c + lane] : 0.f;
+        const int live = min(16, tokens - c);
+        const float factor = (lane & 15) < live ? p.factor[m + c + (lane & 15)] : 0.f;
         const long first = (long)(m + c) * p.ldy + n;
         void* y = p.out_f32 ? (void*)(reinterpret_cast<float*>(p.y) + first) : (void*)(reinterpret_cast<bf16*>(p.y) + first);
         const bf16* residual = p.residual ? p.residual + (long)(m + c) * p.ldr + n : nullptr;
         const bool there = n < v.N;
         auto store = [&](auto g, auto f32) {
-          if (live == 32) store32<decltype(g)::value, decltype(f32)::value, true>(f, out, factor, y, p.ldy, residual, p.ldr, 32, there, lane);
-          else store32<decltype(g)::value, decltype(f32)::value, false>(f, out, factor, y, p.ldy, residual, p.ldr, live, there, lane);
+          if (live == 16) store16<decltype(g)::value, decltype(f32)::value, true>(f, out, factor, y, p.ldy, residual, p.ldr, 16, there, lane);
+          else store16<decltype(g)::value, decltype(f32)::value, false>(f, out, factor, y, p.ldy, residual, p.ldr, live, there, lane);
         };
         using yes = std::true_type;
         using no = std::false_type;
@@ -335,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       }
       tc_fence_before();
       __syncwarp();
-      if (ok && lane == 0) arrive_cluster(in_leader(acc_empty));
+      if (ok && lane == 0) arrive_cluster(in_leader(&acc_empty[j & 1]));
     }
   }
   __syncwarp();
