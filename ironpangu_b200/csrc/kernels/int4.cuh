@@ -42,7 +42,8 @@ __device__ __forceinline__ int code_at(int g, int c) { return c * 128 + ((g ^ (2
 
 // two bf16 of a word's pair j: 128 + q is a bf16 whose last four bits are q; `less` is twice -(128 + z), and the difference is exact
 __device__ __forceinline__ uint32_t pair_of(uint32_t word, int j, uint32_t less) {
-  uint32_t v = ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(word >> (4 * j)), "r"(0x000f000fu), "r"(0x43004300u));       // (a & b) | c
   asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(less));
   return v;
 }

@@ -6,6 +6,8 @@
 // no barrier among the warps), filled before the wait for the preceding kernel. Operands of x come from shared memory, where a CTA lays the columns of a segment
 // once, normalised on the way. The warps' sums are added in one order, so a row's bits do not depend on the rows beside it.
 // Few tiles and a long K: the units along K are shared by the CTAs of a cluster, whose sums are added over distributed shared memory.
+#include <algorithm>
+
 #include "int4.cuh"
 #include "mma16816.cuh"
 #include "tc_common.cuh"
@@ -16,8 +18,8 @@ using namespace ifab::int4;
 
 namespace {
 
-constexpr int WARPS = 8, TB = 8, DEPTH = 4;
-constexpr int SEGMENT = 4096;                     // columns of x in shared memory by eight rows; half of it by sixteen
+constexpr int WARPS = 8, TB = 8;
+constexpr int X_BYTES = 65536;                    // of shared memory for columns of x
 
 struct RowsP {
   View v;
@@ -26,7 +28,8 @@ struct RowsP {
   const bf16* residual; long ldr;
   void* y; long ldy; int out_f32;
   int T;
-  int per, splits;      // tiles of a CTA (pairs of them where gated), CTAs of a cluster
+  int groups, more, splits;      // CTAs (clusters) that share the tiles (pairs of them where gated), how many of them have one more than the others; CTAs of a cluster
+  int cols;                      // columns of x in shared memory at a time
 };
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -56,20 +59,19 @@ __device__ __forceinline__ uint32_t lds2(uint32_t at) {
   return v;
 }
 
-template <int GROUP, bool ZEROS, int NT>
+// MR: most rows of x
+template <int GROUP, bool ZEROS, int MR>
 struct RowsSmem {
+  static constexpr int NT = (MR + 7) / 8, DEPTH = MR <= 2 ? 6 : 4;
   static constexpr int UNIT = CODES + CHUNK / GROUP * (ZEROS ? 48 : 32), RING = WARPS * DEPTH * UNIT;
-  static constexpr int SEG = SEGMENT / NT;
-  static constexpr int RED = WARPS * TB * TILE * 8 * NT * 4;         // takes the place of ring and rows
-  static constexpr int bytes(int T, int cols) {
-    const int x = RING + T * ((cols < SEG ? cols : SEG) * 2 + 64);
-    return x > RED + TB * TILE * 8 * NT * 4 ? x : RED + TB * TILE * 8 * NT * 4;
-  }
+  static constexpr int RED = WARPS * TB * TILE * 8 * NT * 4 + TB * TILE * 8 * NT * 4;         // takes the place of ring and rows
+  static constexpr int bytes(int T, int cols) { return RING + T * (cols * 2 + 64) > RED ? RING + T * (cols * 2 + 64) : RED; }
 };
 
-template <int GROUP, bool ZEROS, int NT>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 2 : 1) int4_rows_kernel(RowsP p) {
-  using S = RowsSmem<GROUP, ZEROS, NT>;
+template <int GROUP, bool ZEROS, int MR>
+__global__ void __launch_bounds__(WARPS * 32, MR <= 8 ? 2 : 1) int4_rows_kernel(RowsP p) {
+  using S = RowsSmem<GROUP, ZEROS, MR>;
+  constexpr int NT = S::NT, DEPTH = S::DEPTH;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float sums[WARPS * 8];
   grid_dep_launch();
@@ -77,22 +79,31 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 2 : 1) int4_rows_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x % p.splits, group = blockIdx.x / p.splits;
   const bool gated = v.halves == 2;
-  const int first = group * p.per, tiles = min(p.per, v.tiles - first) * v.halves;       // the CTA's: 2 i gate, 2 i + 1 up where gated
+  const int fewest = v.tiles / p.groups, mine = fewest + (group < p.more), first = group * fewest + min(group, p.more);
+  const int tiles = mine * v.halves;               // the CTA's: gate tiles, then up tiles
   const int chunk0 = (int)((long)v.chunks * split / p.splits), chunk1 = (int)((long)v.chunks * (split + 1) / p.splits);
   const uint32_t ring = smem_addr(smem) + warp * DEPTH * S::UNIT, xs = smem_addr(smem) + S::RING;
-  const int cols = min(S::SEG, (chunk1 - chunk0 + WARPS - 1) / WARPS * WARPS * CHUNK), pitch = cols * 2 + 64;      // of a segment in shared memory
+  const int cols = p.cols, pitch = cols * 2 + 64;
 
-  int rc = chunk0 + warp, ri = 0;                  // the next unit to be requested
+  // the next unit to be requested: tile ri of chunk rc
+  int rc = chunk0 + warp, ri = 0;
+  const long row = (long)v.chunks * S::UNIT, up = (long)(v.tiles - mine) * row;      // from a tile to the next one, and to the first up tile besides
+  const unsigned char* head = v.units + (long)first * row + (long)rc * S::UNIT + lane * 16;
+  const unsigned char* from = head;
   auto request = [&](int slot) {
     if (rc < chunk1) {
-      const unsigned char* from = gated ? v.at((ri & 1) * v.tiles + first + (ri >> 1), rc) : v.at(first + ri, rc);
-      const uint32_t to = ring + slot * S::UNIT;
-      copy16(to + lane * 16, from + lane * 16, true);
-      copy16(to + 512 + lane * 16, from + 512 + lane * 16, true);
-      if (lane < (S::UNIT - CODES) / 16) copy16(to + CODES + lane * 16, from + CODES + lane * 16, true);
-      if (++ri == tiles) {
+      const uint32_t to = ring + slot * S::UNIT + lane * 16;
+      copy16(to, from, true);
+      copy16(to + 512, from + 512, true);
+      if (lane < (S::UNIT - CODES) / 16) copy16(to + CODES, from + CODES, true);
+      from += row;
+      ++ri;
+      if (gated && ri == mine) from += up;
+      if (ri == tiles) {
         ri = 0;
         rc += WARPS;
+        head += WARPS * S::UNIT;
+        from = head;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -101,49 +112,83 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 2 : 1) int4_rows_kernel(
   for (int i = 0; i < DEPTH; ++i) request(i);
   grid_dep_wait();
 
-  float inv[8];                                    // of the rows, where there is a norm
-  if (p.norm_w) {
-    for (int t = 0; t < p.T; ++t) {
-      float ss = 0.f;
-      for (int i = threadIdx.x; i < v.K / 8; i += WARPS * 32) {
-        float f[8];
-        unpack8(*reinterpret_cast<const uint4*>(p.x + t * p.ldx + i * 8), f);
+  float inv[NT == 1 ? MR : 1];                     // of the rows, where there is a norm
+  if (NT == 1 && p.norm_w) {
+    // MR 8: a warp a row; otherwise all of them every row. The sum of squares in one order whatever the rows: of 256 threads' pieces, 32 threads at a time
+    constexpr int PIECES = MR == 8 ? WARPS : 1, STEP = MR == 8 ? 32 : 256;
+    const int start = MR == 8 ? lane : threadIdx.x;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+    for (int r = 0; r < (MR == 8 ? 1 : MR); ++r) {
+      const int t = MR == 8 ? warp : r;
+      float ss[PIECES] = {};
+      if (t < p.T) {
+        const bf16* xr = p.x + t * p.ldx;
+        for (int i = start; i < v.K / 8; i += STEP * PIECES) {
+          uint4 u[PIECES];
+#pragma unroll
+          for (int q = 0; q < PIECES; ++q) u[q] = i + q * STEP < v.K / 8 ? *reinterpret_cast<const uint4*>(xr + (i + q * STEP) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int q = 0; q < PIECES; ++q) {
+            float f[8];
+            unpack8(u[q], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss[q] += f[e] * f[e];
+          }
+        }
       }
-      ss = warp_sum(ss);
-      if (lane == 0) sums[warp * 8 + t] = ss;
+#pragma unroll
+      for (int q = 0; q < PIECES; ++q) ss[q] = warp_sum(ss[q]);
+      if (lane == 0) {
+        if (MR == 8) {
+#pragma unroll
+          for (int q = 1; q < PIECES; ++q) ss[0] += ss[q];
+          sums[t] = ss[0];
+        } else {
+          sums[warp * 8 + t] = ss[0];
+        }
+      }
     }
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      float s = 0.f;
-      for (int w = 0; w < WARPS; ++w) s += sums[w * 8 + t];
+    for (int t = 0; t < MR; ++t) {
+      float s = sums[t];
+      if (MR != 8)
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) s += sums[w * 8 + t];
       inv[t] = rsqrtf(s / (float)v.K + p.eps);
     }
   }
   // columns of a segment from chunk `at` on, zeros beyond K
   auto stage = [&](int at) {
+    constexpr int HELD = MR < 8 ? MR : 8;          // rows whose pieces are on their way together
     const int pieces = cols / 8;
 #pragma unroll 1
     for (int i = threadIdx.x; i < pieces; i += WARPS * 32) {
       const int k = at * CHUNK + i * 8;
+      const bool in = k < v.K;
       uint4 gain = make_uint4(0, 0, 0, 0);
-      if (p.norm_w && k < v.K) gain = *reinterpret_cast<const uint4*>(p.norm_w + k);
+      if (NT == 1 && p.norm_w && in) gain = *reinterpret_cast<const uint4*>(p.norm_w + k);
 #pragma unroll
-      for (int t = 0; t < 8 * NT; ++t) {
-        if (t >= p.T) break;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (k < v.K) u = *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k);
+      for (int t0 = 0; t0 < MR; t0 += HELD) {
+        uint4 u[HELD];
+#pragma unroll
+        for (int t = 0; t < HELD; ++t) u[t] = in && t0 + t < p.T ? *reinterpret_cast<const uint4*>(p.x + (t0 + t) * p.ldx + k) : make_uint4(0, 0, 0, 0);
         if (NT == 1 && p.norm_w) {
-          float f[8], w[8];
-          unpack8(u, f);
+          float w[8];
           unpack8(gain, w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = f[e] * inv[t & 7] * w[e];
-          u = pack8(f);
+          for (int t = 0; t < HELD; ++t) {
+            float f[8];
+            unpack8(u[t], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = f[e] * inv[NT == 1 ? t : 0] * w[e];
+            u[t] = pack8(f);
+          }
         }
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(xs + t * pitch + i * 16), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+#pragma unroll
+        for (int t = 0; t < HELD; ++t)
+          if (t0 + t < p.T)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(xs + (t0 + t) * pitch + i * 16), "r"(u[t].x), "r"(u[t].y), "r"(u[t].z), "r"(u[t].w) : "memory");
       }
     }
   };
@@ -240,16 +285,16 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 2 : 1) int4_rows_kernel(
   }
   if (p.splits > 1) cluster_barrier();
   else __syncthreads();
-  const int rows = tiles / v.halves * TILE;        // of the result
+  const int rows = mine * TILE;                    // of the result
   const uint32_t part_at = smem_addr(part);
   for (int i = threadIdx.x + split * WARPS * 32; i < rows * p.T; i += p.splits * WARPS * 32) {
     const int r = i % rows, t = i / rows, n = first * TILE + r;
     if (n >= v.N) continue;
-    const int at = gated ? (r / TILE * 2 * TILE + r % TILE) * W + t : r * W + t;
+    const int at = r * W + t, up_at = at + mine * TILE * W;
     float a = 0.f, u = 0.f;
     for (int s = 0; s < p.splits; ++s) {
       a += p.splits > 1 ? ld_part(part_at + at * 4, s) : part[at];
-      if (gated) u += p.splits > 1 ? ld_part(part_at + (at + TILE * W) * 4, s) : part[at + TILE * W];
+      if (gated) u += p.splits > 1 ? ld_part(part_at + up_at * 4, s) : part[up_at];
     }
     if (gated) a = a / (1.f + __expf(-a)) * u;
     if (p.residual) a += __bfloat162float(p.residual[t * p.ldr + n]);
@@ -261,25 +306,39 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 2 : 1) int4_rows_kernel(
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-template <int GROUP, bool ZEROS, int NT>
+// CTAs of a cluster that share K: the most an SM has to do (units of its tiles, at 24 ns of an SM's share of memory) is weighed against a cluster's two barriers and the trips
+// between its CTAs, 1 us, and against the barriers around every further segment of eight rows of x, 1.5 us. Nothing of it goes by the rows, so that a row's bits do not either.
+int splits_of(const View& v, int sms) {
+  int best = 1;
+  long least = 0;
+  for (int s = 1; s <= 8 && s * WARPS <= std::max(v.chunks, WARPS); s *= 2) {
+    const int chunks = ceil_div(v.chunks, s);
+    const long cost = (long)ceil_div(v.tiles * s, sms) * v.halves * chunks + (s > 1 ? 40 : 0) + 60 * (ceil_div(chunks * CHUNK, X_BYTES / 16) - 1);
+    if (!least || cost < least) least = cost, best = s;
+  }
+  return best;
+}
+
+template <int GROUP, bool ZEROS, int MR>
 int launch(RowsP p, cudaStream_t s) {
-  using S = RowsSmem<GROUP, ZEROS, NT>;
-  auto k = int4_rows_kernel<GROUP, ZEROS, NT>;
+  using S = RowsSmem<GROUP, ZEROS, MR>;
+  auto k = int4_rows_kernel<GROUP, ZEROS, MR>;
   const int sms = tc::device_sms();
-  p.splits = 1;
-  while (p.splits < 8 && p.v.tiles * p.v.halves * p.splits < sms && p.v.chunks >= 16 * p.splits) p.splits *= 2;
-  p.per = min(TB / p.v.halves, max(1, ceil_div(p.v.tiles * p.splits, (NT == 1 ? 2 : 1) * sms)));
-  const int cols = ceil_div(ceil_div(p.v.chunks, p.splits), WARPS) * WARPS * CHUNK;
-  const int smem = S::bytes(min(p.T, 8 * NT), cols);
-  if (int rc = (int)cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(8 * NT, S::SEG))) return rc;
-  const dim3 grid(ceil_div(p.v.tiles, p.per) * p.splits);
+  p.splits = splits_of(p.v, sms);
+  // as many CTAs as run at once, two on an SM, unless their tiles are too many for them; those with one tile more come first, so that an SM has one of either kind
+  p.groups = std::max(std::min(p.v.tiles, 2 * sms / p.splits), ceil_div(p.v.tiles, TB / p.v.halves));
+  p.more = p.v.tiles % p.groups;
+  p.cols = std::min(ceil_div(ceil_div(p.v.chunks, p.splits), WARPS) * WARPS * CHUNK, X_BYTES / 2 / MR / (WARPS * CHUNK) * (WARPS * CHUNK));
+  if (int rc = (int)cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(MR, X_BYTES / 2 / MR))) return rc;
+  const int smem = S::bytes(p.T, p.cols);
+  const dim3 grid(p.groups * p.splits);
   if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(WARPS * 32), (unsigned)p.splits, (size_t)smem, s, p);
   return launch_chain(k, grid, dim3(WARPS * 32), (size_t)smem, s, p);
 }
-template <int NT>
+template <int MR>
 int dispatch(const RowsP& p, cudaStream_t s) {
-  if (p.v.zeros) return p.v.group == 128 ? launch<128, true, NT>(p, s) : p.v.group == 64 ? launch<64, true, NT>(p, s) : launch<32, true, NT>(p, s);
-  return p.v.group == 128 ? launch<128, false, NT>(p, s) : p.v.group == 64 ? launch<64, false, NT>(p, s) : launch<32, false, NT>(p, s);
+  if (p.v.zeros) return p.v.group == 128 ? launch<128, true, MR>(p, s) : p.v.group == 64 ? launch<64, true, MR>(p, s) : launch<32, true, MR>(p, s);
+  return p.v.group == 128 ? launch<128, false, MR>(p, s) : p.v.group == 64 ? launch<64, false, MR>(p, s) : launch<32, false, MR>(p, s);
 }
 
 }  // namespace
@@ -301,7 +360,7 @@ extern "C" int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const 
     p.y = out_f32 ? (void*)((float*)y + t * ldy) : (void*)((bf16*)y + t * ldy);
     p.ldy = ldy;
     p.out_f32 = out_f32;
-    if (int rc = p.T <= 8 ? dispatch<1>(p, s) : dispatch<2>(p, s)) return rc;
+    if (int rc = p.T <= 2 ? dispatch<2>(p, s) : p.T <= 8 ? dispatch<8>(p, s) : dispatch<16>(p, s)) return rc;
   }
   return 0;
 }
