@@ -7,7 +7,8 @@
 //            (g ^ 2 c) 16, row g's 8 bytes first, a word for each run of eight columns. A warp whose lane is 4 g + c reads a block without meeting a bank twice and
 //            has the operands of four m16n8k16 products (with K permuted alike in the other operand), each of columns of one group; threads that are rows read
 //            128 bytes in a row for a fixed c.
-//   a word   columns k .. k + 7: column k + 2 j in bits 4 j, column k + 2 j + 1 in bits 4 j + 16. (w >> 4 j) & 0x000f000f is a pair.
+//   a word   columns k .. k + 7: rotated right by 4 j, column k + 2 j in bits 3 .. 6 and column k + 2 j + 1 in bits 19 .. 22, the upper mantissa bits of two bf16. That way
+//            three rotations make four pairs.
 //   scales   [group][g][row g, row g + 8], 16 bits each (bf16 or f16); zero points the same in bytes
 // Behind the units: per row the largest of its finite scales, in f32.
 #pragma once
@@ -40,14 +41,12 @@ inline int view_of(const IfabInt4* d, View* v) {
 
 __device__ __forceinline__ int code_at(int g, int c) { return c * 128 + ((g ^ (2 * c)) << 4); }
 
-// two bf16 of a word's pair j: 128 + q is a bf16 whose last four bits are q; `less` is twice -(128 + z), and the difference is exact
-__device__ __forceinline__ uint32_t pair_of(uint32_t word, int j, uint32_t less) {
+// pair j of a word, its codes eight times in the lower bits of two 16-bit numbers with `high` above them
+__device__ __forceinline__ uint32_t pair_under(uint32_t word, int j, uint32_t high) {
   uint32_t v;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(word >> (4 * j)), "r"(0x000f000fu), "r"(0x43004300u));       // (a & b) | c
-  asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(less));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(j ? __funnelshift_r(word, word, 4 * j) : word), "r"(0x00780078u), "r"(high));       // (a & b) | c
   return v;
 }
-__device__ __forceinline__ uint32_t less_of(uint32_t z) { return 0xc300c300u | z | z << 16; }
 __device__ __forceinline__ float2 scales_of(uint32_t two, int f16) {
   if (f16) return __half22float2(*reinterpret_cast<const __half2*>(&two));
   return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));

@@ -18,7 +18,7 @@ __device__ __forceinline__ uint32_t word_of(const uint8_t* q) {
   uint32_t w = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) w |= (uint32_t)q[2 * j] << (4 * j) | (uint32_t)q[2 * j + 1] << (4 * j + 16);
-  return w;
+  return w << 3 | w >> 29;
 }
 // Rows' largest finite scales. The launch behind this one may read units ahead of its wait for the kernel before it (int4_rows.cu): this one is launched behind the end of the
 // kernels that write them, and `settled_kernel` behind its own.
@@ -159,10 +159,10 @@ __global__ void __launch_bounds__(256) dequantise_kernel(View v, bf16* w, long l
       float f[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t two = pair_of(word, j, less_of(z));
+        const uint32_t two = pair_under(word, j, 0x41804180u);          // 16 + q
         const float2 d = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two));
-        f[2 * j] = d.x * (h ? s.y : s.x);
-        f[2 * j + 1] = d.y * (h ? s.y : s.x);
+        f[2 * j] = (d.x - (float)(16 + z)) * (h ? s.y : s.x);
+        f[2 * j + 1] = (d.y - (float)(16 + z)) * (h ? s.y : s.x);
       }
       if (row >= 0 && k < v.K) *reinterpret_cast<uint4*>(w + row * ldw + k) = pack8(f);
     }

@@ -1,10 +1,15 @@
 // Products of one to sixteen rows with 4-bit weights (int4.cuh):  y[t][n] = sum_k x[t][k] w[n][k] (+ residual), or of a gate | up matrix silu(gate) up.
 //
-// Bound by the stream of codes (half a byte a weight) as long as a weight costs little else, so no weight becomes more than a bf16 difference q - z, which is exact:
-// the products of a group are added up by the tensor cores (weights are the sixteen rows of A, rows of x the eight columns of B) and the group's scale multiplies
-// their f32 sum. A CTA has up to eight tiles of sixteen rows; its eight warps take every eighth unit along K, with a ring of their own in shared memory (cp.async,
-// no barrier among the warps), filled before the wait for the preceding kernel. Operands of x come from shared memory, where a CTA lays the columns of a segment
-// once, normalised on the way. The warps' sums are added in one order, so a row's bits do not depend on the rows beside it.
+// Bound by the stream of codes (half a byte a weight) as long as a weight costs little else: at 6.5 TB/s an SM has 2.8 lane operations for each. So no weight is made at all.
+// A code q goes into the upper mantissa bits of a bf16 whose exponent makes it 16 + q, two codes in a rotation and a logical operation; weights are the sixteen rows of A of
+// an m16n8k16, rows of x the eight columns of B, and what the offset and the zero point add to a group's sum, (16 + z) times the sum of x, is where that sum starts from
+// (with the opposite sign). The sums of x come out of products with ones, once for all tiles of a CTA. The group's scale multiplies its f32 sum. Products are exact; sums run
+// up to 24 |x| instead of 8 |x| a weight, which costs them two bits of f32.
+// A CTA has a share of the tiles of sixteen rows, and its eight warps share K: a warp takes every eighth run of one or two units, for all tiles of the CTA, so that its operands
+// of x - from L2 into registers, normalised on the way - are loaded once. Units come by bulk copies into a ring of the warp's own, the first ones ahead
+// of the wait for the preceding kernel. (Loads ahead into registers waited for one another, whatever their number: 3.4 TB/s without any products.) Sums of the tiles lie in
+// shared memory, a float4 a lane. What a unit costs is its instructions (two cycles of a scheduler for one on integers, eight for a product), so a ninth warp computes the
+// copies' addresses and requests them, and a stage costs the others a look at its barrier and an arrival. The warps' sums are added in one order, and so a row's bits do not depend on the rows beside it.
 // Few tiles and a long K: the units along K are shared by the CTAs of a cluster, whose sums are added over distributed shared memory.
 #include <algorithm>
 
@@ -18,8 +23,8 @@ using namespace ifab::int4;
 
 namespace {
 
-constexpr int WARPS = 8, TB = 8;
-constexpr int X_BYTES = 65536;                    // of shared memory for columns of x
+constexpr int WARPS = 8;
+constexpr uint32_t POLLS = 4000000u;              // of a wait for a copy
 
 struct RowsP {
   View v;
@@ -29,7 +34,10 @@ struct RowsP {
   void* y; long ldy; int out_f32;
   int T;
   int groups, more, splits;      // CTAs (clusters) that share the tiles (pairs of them where gated), how many of them have one more than the others; CTAs of a cluster
-  int cols;                      // columns of x in shared memory at a time
+  int most;                      // tiles of a CTA, at most
+  int depth;                     // stages of a ring
+  int wide;                      // units of a run: 2 also where they are taken one by one (J 1), so that sums are added in the same order
+  uint32_t* status;
 };
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -48,6 +56,14 @@ __device__ __forceinline__ uint4 lds16(uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 lds_f4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_f4(uint32_t at, const float4& v) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
 __device__ __forceinline__ uint32_t lds4(uint32_t at) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
@@ -58,22 +74,47 @@ __device__ __forceinline__ uint32_t lds2(uint32_t at) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
   return v;
 }
+// 16 bytes that the preceding kernel has written (issued where it stands)
+__device__ __forceinline__ uint4 ld_now16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void mma_from(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 
-// MR: most rows of x
-template <int GROUP, bool ZEROS, int MR>
-struct RowsSmem {
-  static constexpr int NT = (MR + 7) / 8, DEPTH = MR <= 2 ? 6 : 4;
-  static constexpr int UNIT = CODES + CHUNK / GROUP * (ZEROS ? 48 : 32), RING = WARPS * DEPTH * UNIT;
-  static constexpr int RED = WARPS * TB * TILE * 8 * NT * 4 + TB * TILE * 8 * NT * 4;         // takes the place of ring and rows
-  static constexpr int bytes(int T, int cols) { return RING + T * (cols * 2 + 64) > RED ? RING + T * (cols * 2 + 64) : RED; }
-};
+// the warps that multiply (the ninth one is at its copies)
+__device__ __forceinline__ void consumers() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
+__device__ __forceinline__ bool ready(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_more(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < POLLS; ++i) {
+    if (ready(bar, parity)) return true;
+    if (i > 256) __nanosleep(64);
+  }
+  return false;
+}
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) { return ready(bar, parity) || wait_more(bar, parity); }
 
-template <int GROUP, bool ZEROS, int MR>
-__global__ void __launch_bounds__(WARPS * 32, MR <= 8 ? 2 : 1) int4_rows_kernel(RowsP p) {
-  using S = RowsSmem<GROUP, ZEROS, MR>;
-  constexpr int NT = S::NT, DEPTH = S::DEPTH;
+// MR: most rows of x; J: units of a run
+template <int GROUP, bool ZEROS, bool F16, int MR, int J>
+__global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) {
+  constexpr int NT = (MR + 7) / 8, RUNS = GROUP / 32, NG = 4 / RUNS, UNIT = CODES + NG * (ZEROS ? 48 : 32);      // runs of 32 columns of a group, groups of a unit, its bytes
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float sums[WARPS * 8];
+  __shared__ float sums[WARPS * 8], inv[8];        // inv: of the rows, where there is a norm
+  __shared__ uint64_t bars[WARPS * 16];            // of a warp's stages: full, and eight further on empty
   grid_dep_launch();
   const View& v = p.v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -82,38 +123,52 @@ __global__ void __launch_bounds__(WARPS * 32, MR <= 8 ? 2 : 1) int4_rows_kernel(
   const int fewest = v.tiles / p.groups, mine = fewest + (group < p.more), first = group * fewest + min(group, p.more);
   const int tiles = mine * v.halves;               // the CTA's: gate tiles, then up tiles
   const int chunk0 = (int)((long)v.chunks * split / p.splits), chunk1 = (int)((long)v.chunks * (split + 1) / p.splits);
-  const uint32_t ring = smem_addr(smem) + warp * DEPTH * S::UNIT, xs = smem_addr(smem) + S::RING;
-  const int cols = p.cols, pitch = cols * 2 + 64;
+  // the run behind the one that begins with unit r
+  auto after = [&](int r) {
+    if (J == 2 || p.wide == 1) return r + WARPS * p.wide;
+    const int odd = (r - chunk0) & 1;
+    return odd || r + 1 == chunk1 ? r - odd + WARPS * 2 : r + 1;
+  };
+  // sums: [warp][tile][rows of x by eight][lane], then the rings
+  const uint32_t acc = smem_addr(smem) + (warp * p.most * NT * 32 + lane) * 16, rings = smem_addr(smem) + WARPS * p.most * NT * 512;
+  const uint32_t bar = smem_addr(bars + warp * 16);
 
-  // the next unit to be requested: tile ri of chunk rc
-  int rc = chunk0 + warp, ri = 0;
-  const long row = (long)v.chunks * S::UNIT, up = (long)(v.tiles - mine) * row;      // from a tile to the next one, and to the first up tile besides
-  const unsigned char* head = v.units + (long)first * row + (long)rc * S::UNIT + lane * 16;
-  const unsigned char* from = head;
-  auto request = [&](int slot) {
-    if (rc < chunk1) {
-      const uint32_t to = ring + slot * S::UNIT + lane * 16;
-      copy16(to, from, true);
-      copy16(to + 512, from + 512, true);
-      if (lane < (S::UNIT - CODES) / 16) copy16(to + CODES, from + CODES, true);
-      from += row;
-      ++ri;
-      if (gated && ri == mine) from += up;
-      if (ri == tiles) {
-        ri = 0;
-        rc += WARPS;
-        head += WARPS * S::UNIT;
-        from = head;
+  if (warp == WARPS && lane < WARPS) {
+    for (int i = 0; i < p.depth; ++i) {
+      tc::mbar_init(bars + lane * 16 + i, 1);
+      tc::mbar_init(bars + lane * 16 + 8 + i, 1);
+    }
+    tc::mbar_fence_init();
+  }
+  __syncthreads();
+  if (warp == WARPS) {
+    // lane w requests the runs of warp w. Codes are written by no kernel of the stream: nothing to wait for
+    if (lane < WARPS) {
+      const uint32_t ring = rings + lane * p.depth * J * UNIT, full = smem_addr(bars + lane * 16);
+      const long row = (long)v.chunks * UNIT, up = (long)(v.tiles - mine) * row;      // from a tile to the next one, and to the first up tile besides
+      int slot = 0, round = 0;
+      bool ok = true;
+      for (int rc = chunk0 + lane * p.wide; rc < chunk1 && ok; rc = after(rc)) {
+        const unsigned char* from = v.units + (long)first * row + (long)rc * UNIT;
+        const uint32_t bytes = J == 1 ? UNIT : min(J, chunk1 - rc) * UNIT;
+        for (int i = 0; i < tiles; ++i, from += row) {
+          if (gated && i == mine) from += up;
+          if (round && !wait_for(full + 64 + slot * 8, (round - 1) & 1)) { ok = false; break; }
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + slot * 8), "r"(bytes) : "memory");
+          asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * J * UNIT), "l"(from), "r"(bytes),
+                       "r"(full + slot * 8)
+                       : "memory");
+          if (++slot == p.depth) slot = 0, ++round;
+        }
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll 1
-  for (int i = 0; i < DEPTH; ++i) request(i);
+    __syncwarp();
+  } else {
+    for (int i = 0; i < tiles * NT; ++i) sts_f4(acc + i * 512, make_float4(0.f, 0.f, 0.f, 0.f));
+  }
   grid_dep_wait();
 
-  float inv[NT == 1 ? MR : 1];                     // of the rows, where there is a norm
-  if (NT == 1 && p.norm_w) {
+  if (NT == 1 && p.norm_w && warp < WARPS) {
     // MR 8: a warp a row; otherwise all of them every row. The sum of squares in one order whatever the rows: of 256 threads' pieces, 32 threads at a time
     constexpr int PIECES = MR == 8 ? WARPS : 1, STEP = MR == 8 ? 32 : 256;
     const int start = MR == 8 ? lane : threadIdx.x;
@@ -148,146 +203,152 @@ __global__ void __launch_bounds__(WARPS * 32, MR <= 8 ? 2 : 1) int4_rows_kernel(
         }
       }
     }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < MR; ++t) {
+    consumers();
+    if (threadIdx.x < MR) {
+      const int t = threadIdx.x;
       float s = sums[t];
       if (MR != 8)
 #pragma unroll
         for (int w = 1; w < WARPS; ++w) s += sums[w * 8 + t];
       inv[t] = rsqrtf(s / (float)v.K + p.eps);
     }
+    consumers();
   }
-  // columns of a segment from chunk `at` on, zeros beyond K
-  auto stage = [&](int at) {
-    constexpr int HELD = MR < 8 ? MR : 8;          // rows whose pieces are on their way together
-    const int pieces = cols / 8;
-#pragma unroll 1
-    for (int i = threadIdx.x; i < pieces; i += WARPS * 32) {
-      const int k = at * CHUNK + i * 8;
-      const bool in = k < v.K;
-      uint4 gain = make_uint4(0, 0, 0, 0);
-      if (NT == 1 && p.norm_w && in) gain = *reinterpret_cast<const uint4*>(p.norm_w + k);
-#pragma unroll
-      for (int t0 = 0; t0 < MR; t0 += HELD) {
-        uint4 u[HELD];
-#pragma unroll
-        for (int t = 0; t < HELD; ++t) u[t] = in && t0 + t < p.T ? *reinterpret_cast<const uint4*>(p.x + (t0 + t) * p.ldx + k) : make_uint4(0, 0, 0, 0);
-        if (NT == 1 && p.norm_w) {
-          float w[8];
-          unpack8(gain, w);
-#pragma unroll
-          for (int t = 0; t < HELD; ++t) {
-            float f[8];
-            unpack8(u[t], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = f[e] * inv[NT == 1 ? t : 0] * w[e];
-            u[t] = pack8(f);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < HELD; ++t)
-          if (t0 + t < p.T)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(xs + (t0 + t) * pitch + i * 16), "r"(u[t].x), "r"(u[t].y), "r"(u[t].z), "r"(u[t].w) : "memory");
-      }
-    }
-  };
 
-  float acc[TB][NT][4];
+  bool late = false;
+  if (warp < WARPS) {
+    const bf16* xr[NT];                            // this lane's row of x, its first column
 #pragma unroll
-  for (int i = 0; i < TB; ++i)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
-  int slot = 0;
+    for (int n = 0; n < NT; ++n) xr[n] = p.x + (long)min(n * 8 + g, p.T - 1) * p.ldx + c * 8;
+    const uint32_t ring = rings + warp * p.depth * J * UNIT + code_at(g, c), meta = CODES + g * 4 - code_at(g, c), end = ring + p.depth * J * UNIT;
+    uint32_t at = ring, stage = bar, parity = 0;   // the stage at hand: this lane's first codes, and its barrier
 #pragma unroll 1
-  for (int seg = chunk0; seg < chunk1; seg += cols / CHUNK) {
-    if (seg > chunk0) __syncthreads();
-    stage(seg);
-    __syncthreads();
-    const int end = min(chunk1, seg + cols / CHUNK);
-#pragma unroll 1
-    for (int ch = seg + warp; ch < end; ch += WARPS) {
-      uint4 b[NT][4];                              // this lane's operands: four runs of eight columns of a row of x
+    for (int ch = chunk0 + warp * p.wide; ch < chunk1; ch = after(ch)) {
+      uint4 b[J][NT][4];                           // this lane's operands: four runs of eight columns of a row of x
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint32_t at = xs + (n * 8 + g) * pitch + (ch - seg) * CHUNK * 2 + c * 16;
+      for (int u = 0; u < J; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[n][i] = n * 8 + g < p.T ? lds16(at + i * 64) : make_uint4(0, 0, 0, 0);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = (ch + u) * CHUNK + i * 32;
+            b[u][n][i] = (MR == 1 ? g == 0 : n * 8 + g < p.T) && k + c * 8 < v.K ? ld_now16(xr[n] + k) : make_uint4(0, 0, 0, 0);
+          }
+      if (NT == 1 && p.norm_w) {
+        const float by = inv[MR == 1 ? 0 : g];
+#pragma unroll
+        for (int u = 0; u < J; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = (ch + u) * CHUNK + i * 32 + c * 8;
+            if (k < v.K) {
+              float f[8], w[8];
+              unpack8(b[u][0][i], f);
+              unpack8(*reinterpret_cast<const uint4*>(p.norm_w + k), w);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = f[e] * by * w[e];
+              b[u][0][i] = pack8(f);
+            }
+          }
       }
+      float sum[J][NT][NG][4];                     // of the groups' columns of x, rows 2 c and 2 c + 1, twice: times -24 without zero points
 #pragma unroll
-      for (int i = 0; i < TB; ++i) {
-        if (i >= tiles) break;
-        asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
-        __syncwarp();
-        const uint32_t at = ring + slot * S::UNIT;
-        float part[NT][4];
-        uint4 w;
-        uint32_t lo = less_of(8), hi = less_of(8);
+      for (int u = 0; u < J; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {              // runs of 32 columns
-          constexpr int RUNS = GROUP / 32;
-          if (r % 2 == 0) w = lds16(at + (r >> 1) * 512 + code_at(g, c));
-          if (ZEROS && r % RUNS == 0) {
-            const uint32_t z = lds2(at + CODES + CHUNK / GROUP * 32 + r / RUNS * 16 + g * 2);
-            lo = less_of(z & 255);
-            hi = less_of(z >> 8);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int q = 0; q < NG; ++q) {
+            constexpr uint32_t one = ZEROS ? 0x3f803f80u : 0xc1c0c1c0u;      // 1 or -24
+#pragma unroll
+            for (int r = q * RUNS; r < (q + 1) * RUNS; ++r) {
+              if (r == q * RUNS) mma16816_alone(sum[u][n][q], one, one, one, one, b[u][n][r].x, b[u][n][r].y);
+              else mma16816(sum[u][n][q], one, one, one, one, b[u][n][r].x, b[u][n][r].y);
+              mma16816(sum[u][n][q], one, one, one, one, b[u][n][r].z, b[u][n][r].w);
+            }
           }
-          const uint32_t wl = r & 1 ? w.y : w.x, wh = r & 1 ? w.w : w.z;
-          uint32_t al[4], ah[4];
+      const bool whole = J == 1 || ch + 1 < chunk1;
+      uint32_t to = acc;
+#pragma unroll 1
+      for (int i = 0; i < tiles; ++i, to += NT * 512) {
+        late |= !wait_for(stage, parity);
+        float4 so_far[NT];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) al[j] = pair_of(wl, j, lo), ah[j] = pair_of(wh, j, hi);
+        for (int n = 0; n < NT; ++n) so_far[n] = lds_f4(to + n * 512);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (r % RUNS == 0) mma16816_alone(part[n], al[0], ah[0], al[1], ah[1], b[n][r].x, b[n][r].y);
-            else mma16816(part[n], al[0], ah[0], al[1], ah[1], b[n][r].x, b[n][r].y);
-            mma16816(part[n], al[2], ah[2], al[3], ah[3], b[n][r].z, b[n][r].w);
-          }
-          if (r % RUNS == RUNS - 1) {
-            const float2 s = scales_of(lds4(at + CODES + r / RUNS * 32 + g * 4), v.f16);
+        for (int u = 0; u < J; ++u) {
+          if (u == 1 && !whole) break;
+          float part[NT][4];
+          uint4 w;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {            // runs of 32 columns
+            if (r % 2 == 0) w = lds16(at + u * UNIT + (r >> 1) * 512);
+            const uint32_t wl = r & 1 ? w.y : w.x, wh = r & 1 ? w.w : w.z;
+            const int q = r / RUNS;
+            uint32_t al[4], ah[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) al[j] = pair_under(wl, j, 0x41804180u), ah[j] = pair_under(wh, j, 0x41804180u);      // 16 + q
+            float lo = 1.f, hi = 1.f;              // -(16 + z)
+            if (ZEROS && r % RUNS == 0) {
+              const uint32_t z = lds2(at + u * UNIT + meta + NG * 32 + q * 16 - g * 2);
+              lo = 8388592.f - __uint_as_float(0x4b000000u | (z & 255));
+              hi = 8388592.f - __uint_as_float(0x4b000000u | z >> 8);
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              acc[i][n][0] += s.x * part[n][0];
-              acc[i][n][1] += s.x * part[n][1];
-              acc[i][n][2] += s.y * part[n][2];
-              acc[i][n][3] += s.y * part[n][3];
+              const float(&x)[4] = sum[u][n][q];
+              if (r % RUNS == 0 && ZEROS) {
+                const float start[4] = {x[0] * lo, x[1] * lo, x[0] * hi, x[1] * hi};
+                mma_from(part[n], start, al[0], ah[0], al[1], ah[1], b[u][n][r].x, b[u][n][r].y);
+              } else if (r % RUNS == 0) {
+                mma_from(part[n], x, al[0], ah[0], al[1], ah[1], b[u][n][r].x, b[u][n][r].y);
+              } else {
+                mma16816(part[n], al[0], ah[0], al[1], ah[1], b[u][n][r].x, b[u][n][r].y);
+              }
+              mma16816(part[n], al[2], ah[2], al[3], ah[3], b[u][n][r].z, b[u][n][r].w);
+            }
+            if (r % RUNS == RUNS - 1) {
+              const float2 s = scales_of(lds4(at + u * UNIT + meta + q * 32), F16);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                so_far[n].x += s.x * part[n][0];
+                so_far[n].y += s.x * part[n][1];
+                so_far[n].z += s.y * part[n][2];
+                so_far[n].w += s.y * part[n][3];
+              }
             }
           }
         }
-        __syncwarp();                              // the unit is read
-        request(slot);
-        slot = slot + 1 == DEPTH ? 0 : slot + 1;
+        __syncwarp();                              // the stage is read
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(stage + 64) : "memory");
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sts_f4(to + n * 512, so_far[n]);
+        at += J * UNIT;
+        stage += 8;
+        if (at == end) at = ring, stage = bar, parity ^= 1;
       }
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  // the warps' sums [warp][tile][16][rows of x], added up into [tile][16][rows of x]
-  constexpr int W = 8 * NT;
-  float* red = reinterpret_cast<float*>(smem);
-  float* part = red + WARPS * TB * TILE * W;
-#pragma unroll
-  for (int i = 0; i < TB; ++i) {
-    if (i >= tiles) break;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* to = red + ((warp * TB + i) * TILE + g) * W + n * 8 + 2 * c;
-      *reinterpret_cast<float2*>(to) = make_float2(acc[i][n][0], acc[i][n][1]);
-      *reinterpret_cast<float2*>(to + 8 * W) = make_float2(acc[i][n][2], acc[i][n][3]);
-    }
+  if (__any_sync(0xffffffffu, late)) {             // a copy that did not land: nothing of the tiles is right
+    if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+    const float nan = __int_as_float(0x7fffffff);
+    for (int i = 0; i < tiles * NT; ++i) sts_f4(acc + i * 512, make_float4(nan, nan, nan, nan));
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < tiles * TILE * W; i += WARPS * 32) {
-    constexpr int STEP = TB * TILE * W;
-    const float* f = red + i;
-    part[i] = ((f[0] + f[STEP]) + (f[2 * STEP] + f[3 * STEP])) + ((f[4 * STEP] + f[5 * STEP]) + (f[6 * STEP] + f[7 * STEP]));
+  // the warps' sums, added up into [tile][16][rows of x] in the place of the rings
+  constexpr int W = 8 * NT;
+  const float* red = reinterpret_cast<const float*>(smem);
+  const int step = p.most * NT * 128;
+  float* part = reinterpret_cast<float*>(smem) + WARPS * step;
+  for (int i = threadIdx.x; i < tiles * TILE * W; i += WARPS * 32 + 32) {
+    const int t = i % W, r = i / W % TILE, tile = i / W / TILE;
+    const float* f = red + ((tile * NT + (t >> 3)) * 32 + (r & 7) * 4 + ((t & 7) >> 1)) * 4 + (r >> 3) * 2 + (t & 1);
+    part[i] = ((f[0] + f[step]) + (f[2 * step] + f[3 * step])) + ((f[4 * step] + f[5 * step]) + (f[6 * step] + f[7 * step]));
   }
   if (p.splits > 1) cluster_barrier();
   else __syncthreads();
   const int rows = mine * TILE;                    // of the result
   const uint32_t part_at = smem_addr(part);
-  for (int i = threadIdx.x + split * WARPS * 32; i < rows * p.T; i += p.splits * WARPS * 32) {
+  for (int i = threadIdx.x + split * (WARPS * 32 + 32); i < rows * p.T; i += p.splits * (WARPS * 32 + 32)) {
     const int r = i % rows, t = i / rows, n = first * TILE + r;
     if (n >= v.N) continue;
     const int at = r * W + t, up_at = at + mine * TILE * W;
@@ -307,50 +368,67 @@ __global__ void __launch_bounds__(WARPS * 32, MR <= 8 ? 2 : 1) int4_rows_kernel(
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // CTAs of a cluster that share K: the most an SM has to do (units of its tiles, at 24 ns of an SM's share of memory) is weighed against a cluster's two barriers and the trips
-// between its CTAs, 1 us, and against the barriers around every further segment of eight rows of x, 1.5 us. Nothing of it goes by the rows, so that a row's bits do not either.
+// between its CTAs, 1 us. Nothing of it goes by the rows, so that a row's bits do not either.
 int splits_of(const View& v, int sms) {
   int best = 1;
   long least = 0;
   for (int s = 1; s <= 8 && s * WARPS <= std::max(v.chunks, WARPS); s *= 2) {
-    const int chunks = ceil_div(v.chunks, s);
-    const long cost = (long)ceil_div(v.tiles * s, sms) * v.halves * chunks + (s > 1 ? 40 : 0) + 60 * (ceil_div(chunks * CHUNK, X_BYTES / 16) - 1);
+    const long cost = (long)ceil_div(v.tiles * s, sms) * v.halves * ceil_div(v.chunks, s) + (s > 1 ? 40 : 0);
     if (!least || cost < least) least = cost, best = s;
   }
   return best;
 }
+// Clusters of s CTAs that run at once, two CTAs an SM: not all SMs of a part of the chip can be divided by four or eight (of 296 CTAs, 284 and 264)
+int at_once(int s, int sms) { return s <= 2 ? 2 * sms / s : s == 4 ? 2 * sms * 15 / 64 : 2 * sms * 6 / 56; }
+constexpr int SMEM = 110 * 1024;                   // of a CTA, two of which share an SM
 
-template <int GROUP, bool ZEROS, int MR>
+template <int GROUP, bool ZEROS, bool F16, int MR, int J>
 int launch(RowsP p, cudaStream_t s) {
-  using S = RowsSmem<GROUP, ZEROS, MR>;
-  auto k = int4_rows_kernel<GROUP, ZEROS, MR>;
-  const int sms = tc::device_sms();
-  p.splits = splits_of(p.v, sms);
-  // as many CTAs as run at once, two on an SM, unless their tiles are too many for them; those with one tile more come first, so that an SM has one of either kind
-  p.groups = std::max(std::min(p.v.tiles, 2 * sms / p.splits), ceil_div(p.v.tiles, TB / p.v.halves));
+  constexpr int NT = (MR + 7) / 8, unit = CODES + CHUNK / GROUP * (ZEROS ? 48 : 32), tile = WARPS * NT * 512 + TILE * 8 * NT * 4;      // bytes of a tile's sums and their sum
+  auto k = int4_rows_kernel<GROUP, ZEROS, F16, MR, J>;
+  const int sms = tc::device_sms(), halves = p.v.halves;
+  // as many CTAs as run at once, unless their tiles' sums are too many for them; those with one tile more come first, so that an SM has some of either kind
+  const int room = (SMEM - 512 - WARPS * 3 * J * unit) / tile / halves;
+  p.groups = std::max(std::min(p.v.tiles, at_once(p.splits, sms)), ceil_div(p.v.tiles, room));
   p.more = p.v.tiles % p.groups;
-  p.cols = std::min(ceil_div(ceil_div(p.v.chunks, p.splits), WARPS) * WARPS * CHUNK, X_BYTES / 2 / MR / (WARPS * CHUNK) * (WARPS * CHUNK));
-  if (int rc = (int)cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(MR, X_BYTES / 2 / MR))) return rc;
-  const int smem = S::bytes(p.T, p.cols);
+  p.most = (p.v.tiles / p.groups + (p.more > 0)) * halves;
+  const int runs = ceil_div(ceil_div(p.v.chunks, p.splits), WARPS * p.wide) * (p.wide / J) * p.most;           // of a warp
+  p.depth = std::max(1, std::min({runs, (SMEM - 512 - p.most * WARPS * NT * 512) / (WARPS * J * unit), 8}));
+  const int smem = p.most * WARPS * NT * 512 + std::max(WARPS * p.depth * J * unit, p.most * TILE * 8 * NT * 4);
+  if (int rc = (int)cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) return rc;
   const dim3 grid(p.groups * p.splits);
-  if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(WARPS * 32), (unsigned)p.splits, (size_t)smem, s, p);
-  return launch_chain(k, grid, dim3(WARPS * 32), (size_t)smem, s, p);
+  if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(WARPS * 32 + 32), (unsigned)p.splits, (size_t)smem, s, p);
+  return launch_chain(k, grid, dim3(WARPS * 32 + 32), (size_t)smem, s, p);
+}
+template <int GROUP, bool ZEROS, bool F16, int MR>
+int launch_runs(RowsP p, cudaStream_t s) {
+  p.splits = splits_of(p.v, tc::device_sms());
+  // runs of two units while every warp has one: a copy of 1 KB costs as much as one of two
+  p.wide = ceil_div(p.v.chunks, p.splits) >= 2 * WARPS ? 2 : 1;
+  if constexpr (MR <= 8)
+    if (p.wide == 2) return launch<GROUP, ZEROS, F16, MR, 2>(p, s);
+  return launch<GROUP, ZEROS, F16, MR, 1>(p, s);
+}
+template <int GROUP, int MR>
+int by_kind(const RowsP& p, cudaStream_t s) {
+  if (p.v.zeros) return p.v.f16 ? launch_runs<GROUP, true, true, MR>(p, s) : launch_runs<GROUP, true, false, MR>(p, s);
+  return p.v.f16 ? launch_runs<GROUP, false, true, MR>(p, s) : launch_runs<GROUP, false, false, MR>(p, s);
 }
 template <int MR>
 int dispatch(const RowsP& p, cudaStream_t s) {
-  if (p.v.zeros) return p.v.group == 128 ? launch<128, true, MR>(p, s) : p.v.group == 64 ? launch<64, true, MR>(p, s) : launch<32, true, MR>(p, s);
-  return p.v.group == 128 ? launch<128, false, MR>(p, s) : p.v.group == 64 ? launch<64, false, MR>(p, s) : launch<32, false, MR>(p, s);
+  return p.v.group == 128 ? by_kind<128, MR>(p, s) : p.v.group == 64 ? by_kind<64, MR>(p, s) : by_kind<32, MR>(p, s);
 }
 
 }  // namespace
 
 // x [T, K] in bf16, rows on 16 bytes; norm_w: one to eight rows. The units are written by no kernel that may still run (ifab_int4_pack and ifab_int4_quantise see to it).
 extern "C" int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr, void* y, long ldy, int out_f32,
-                              int T, void* stream) {
+                              int T, uint32_t* status, void* stream) {
   RowsP p{};
   if (view_of(d, &p.v) || T < 1 || !x || !y || ((uintptr_t)x | (uintptr_t)norm_w) % 16 || ldx % 8 || (norm_w && T > 8) || (p.v.halves == 2 && residual)) return -1;
   cudaStream_t s = (cudaStream_t)stream;
   for (int t = 0; t < T; t += 16) {
-    p.T = min(16, T - t);
+    p.T = std::min(16, T - t);
     p.x = (const bf16*)x + t * ldx;
     p.ldx = ldx;
     p.norm_w = (const bf16*)norm_w;
@@ -360,7 +438,8 @@ extern "C" int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const 
     p.y = out_f32 ? (void*)((float*)y + t * ldy) : (void*)((bf16*)y + t * ldy);
     p.ldy = ldy;
     p.out_f32 = out_f32;
-    if (int rc = p.T <= 2 ? dispatch<2>(p, s) : p.T <= 8 ? dispatch<8>(p, s) : dispatch<16>(p, s)) return rc;
+    p.status = status;
+    if (int rc = p.T <= 1 ? dispatch<1>(p, s) : p.T <= 8 ? dispatch<8>(p, s) : dispatch<16>(p, s)) return rc;
   }
   return 0;
 }

@@ -5,11 +5,11 @@
 
 namespace ifab::int4 {
 
-// eight weights of a word in f16: 1024 + q is an f16 whose last four bits are q, and the difference is exact. less: twice -(1024 + z), s2: twice the scale
+// eight weights of a word in f16: 128 + q is an f16 with q in bits 3 .. 6, and the difference is exact. less: twice -(128 + z), s2: twice the scale
 __device__ __forceinline__ void weights_of(uint32_t word, uint32_t less, uint32_t s2, uint32_t* out) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t d = ((word >> (4 * j)) & 0x000f000fu) | 0x64006400u;
+    uint32_t d = pair_under(word, j, 0x58005800u);
     asm("add.rn.f16x2 %0, %0, %1;" : "+r"(d) : "r"(less));
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(out[j]) : "r"(d), "r"(s2));
   }
@@ -65,7 +65,7 @@ struct RowOfWeights {
       const __half2 s = __float2half2_rn(scales_of(*reinterpret_cast<const uint16_t*>(unit + CODES + i * 32 + g * 4 + h * 2), f16).x * by);
       const uint32_t z = ZEROS ? unit[CODES + CHUNK / GROUP * 32 + i * 16 + g * 2 + h] : 8;
       s2[i] = *reinterpret_cast<const uint32_t*>(&s);
-      less[i] = 0xe400e400u | z | z << 16;
+      less[i] = 0xd800d800u | z << 3 | z << 19;
     }
   }
   // block b (64 columns) of the chunk: 32 pairs in the order of the columns

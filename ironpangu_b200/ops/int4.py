@@ -123,5 +123,5 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
         return out
     check(_lib.load().ifab_int4_rows(w.ref, x.data_ptr(), x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps,
                                      None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
-                                     out.dtype == F32, T, _stream(x.device)), "int4.linear")
+                                     out.dtype == F32, T, status_ptr, _stream(x.device)), "int4.linear")
     return out

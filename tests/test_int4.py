@@ -192,11 +192,12 @@ def test_norm_ahead(N, K, T):
 
 
 @pytest.mark.gpu
-def test_rows_beside_a_row_change_nothing():
+@pytest.mark.parametrize("N,K", [(500, 1160), (300, 4104), (100, 20000)])
+def test_rows_beside_a_row_change_nothing(N, K):
     from ironpangu_b200.ops import int4
 
-    q, s, z = _codes(500, 1160, 128, False, 5)
-    w, x = int4.pack(q, s, z, group=128), _rows(16, 1160, 1)
+    q, s, z = _codes(N, K, 128, False, 5)
+    w, x = int4.pack(q, s, z, group=128), _rows(16, K, 1)
     alone = torch.cat([int4.linear(x[t:t + 1], w) for t in range(16)])
     for T in (2, 8, 9, 16):
         assert torch.equal(int4.linear(x[:T], w), alone[:T])
