@@ -14,6 +14,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ifab::int4 {
@@ -29,6 +31,31 @@ struct View {
   __device__ __forceinline__ unsigned char* at(int tile, int chunk) const { return units + ((long)tile * chunks + chunk) * unit; }
 };
 __host__ __device__ inline int unit_bytes(int group, int zeros) { return CODES + CHUNK / group * (zeros ? 48 : 32); }
+
+// host: SMs of the current device, and a kernel's dynamic shared memory, asked for and set once a device (each a part of a microsecond of a launch's three)
+struct Device {
+  int id, sms;
+};
+inline Device device_now() {
+  static std::atomic<int> known[64];
+  Device d{0, 0};
+  cudaGetDevice(&d.id);
+  const bool kept = d.id >= 0 && d.id < 64;
+  if (kept) d.sms = known[d.id].load(std::memory_order_relaxed);
+  if (!d.sms) {
+    if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, d.id) != cudaSuccess || d.sms < 1) d.sms = 148;
+    if (kept) known[d.id].store(d.sms, std::memory_order_relaxed);
+  }
+  return d;
+}
+template <typename Kernel>
+inline int allow_smem(Kernel kernel, int bytes, int device, std::atomic<uint64_t>& done) {
+  const bool kept = device >= 0 && device < 64;
+  if (kept && (done.load(std::memory_order_relaxed) >> device & 1)) return 0;
+  if (int rc = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return rc;
+  if (kept) done.fetch_or(1ull << device, std::memory_order_relaxed);
+  return 0;
+}
 
 // host: the view of a descriptor; 0 or -1
 inline int view_of(const IfabInt4* d, View* v) {

@@ -386,7 +386,9 @@ template <int GROUP, bool ZEROS, bool F16, int MR, int J>
 int launch(RowsP p, cudaStream_t s) {
   constexpr int NT = (MR + 7) / 8, unit = CODES + CHUNK / GROUP * (ZEROS ? 48 : 32), tile = WARPS * NT * 512 + TILE * 8 * NT * 4;      // bytes of a tile's sums and their sum
   auto k = int4_rows_kernel<GROUP, ZEROS, F16, MR, J>;
-  const int sms = tc::device_sms(), halves = p.v.halves;
+  static std::atomic<uint64_t> done;
+  const Device dev = device_now();
+  const int sms = dev.sms, halves = p.v.halves;
   // as many CTAs as run at once, unless their tiles' sums are too many for them; those with one tile more come first, so that an SM has some of either kind
   const int room = (SMEM - 512 - WARPS * 3 * J * unit) / tile / halves;
   p.groups = std::max(std::min(p.v.tiles, at_once(p.splits, sms)), ceil_div(p.v.tiles, room));
@@ -395,14 +397,14 @@ int launch(RowsP p, cudaStream_t s) {
   const int runs = ceil_div(ceil_div(p.v.chunks, p.splits), WARPS * p.wide) * (p.wide / J) * p.most;           // of a warp
   p.depth = std::max(1, std::min({runs, (SMEM - 512 - p.most * WARPS * NT * 512) / (WARPS * J * unit), 8}));
   const int smem = p.most * WARPS * NT * 512 + std::max(WARPS * p.depth * J * unit, p.most * TILE * 8 * NT * 4);
-  if (int rc = (int)cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) return rc;
+  if (int rc = allow_smem(k, SMEM, dev.id, done)) return rc;
   const dim3 grid(p.groups * p.splits);
   if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(WARPS * 32 + 32), (unsigned)p.splits, (size_t)smem, s, p);
   return launch_chain(k, grid, dim3(WARPS * 32 + 32), (size_t)smem, s, p);
 }
 template <int GROUP, bool ZEROS, bool F16, int MR>
 int launch_runs(RowsP p, cudaStream_t s) {
-  p.splits = splits_of(p.v, tc::device_sms());
+  p.splits = splits_of(p.v, device_now().sms);
   // runs of two units while every warp has one: a copy of 1 KB costs as much as one of two
   p.wide = ceil_div(p.v.chunks, p.splits) >= 2 * WARPS ? 2 : 1;
   if constexpr (MR <= 8)

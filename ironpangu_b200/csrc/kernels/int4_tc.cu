@@ -337,7 +337,8 @@ template <int GROUP, bool ZEROS>
 int launch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
   auto k = int4_tc_kernel<GROUP, ZEROS>;
   constexpr int smem = SMEM<GROUP, ZEROS>;
-  if (int rc = opt_in_smem(k, smem)) return rc;
+  static std::atomic<uint64_t> done;
+  if (int rc = allow_smem(k, smem, device_now().id, done)) return rc;
   if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(THREADS), (unsigned)p.splits, (size_t)smem, s, tx, p);
   return launch_chain(k, grid, dim3(THREADS), (size_t)smem, s, tx, p);
 }
@@ -368,7 +369,7 @@ extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const 
   float* factor = (float*)((char*)scratch + (uint64_t)T * p.v.K * 2);
   p.y = y, p.ldy = ldy, p.out_f32 = out_f32, p.residual = (const bf16*)residual, p.ldr = ldr, p.factor = factor, p.T = T, p.status = status;
   p.spin_limit = spin_limit;
-  const int halves = p.v.halves, sms = device_sms();
+  const int halves = p.v.halves, sms = device_now().sms;
   cudaStream_t s = (cudaStream_t)stream;
   if (int rc = launch_chain(rows_kernel, dim3(T), dim3(256), 0, s, (const bf16*)x, ldx, rows, (long)p.v.K, factor, p.v.K)) return rc;
   if (const int tok = pair_tokens(T, p.v.N * halves, sms / 2))

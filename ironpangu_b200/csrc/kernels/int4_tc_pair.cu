@@ -346,7 +346,8 @@ template <int GROUP, bool ZEROS>
 int launch(const CUtensorMap& tx, const PairP& p, int pairs, cudaStream_t s) {
   auto k = int4_tc_pair_kernel<GROUP, ZEROS>;
   constexpr int smem = SMEM<GROUP, ZEROS>;
-  if (int rc = opt_in_smem(k, smem)) return rc;
+  static std::atomic<uint64_t> done;
+  if (int rc = allow_smem(k, smem, device_now().id, done)) return rc;
   return launch_chain_cluster(k, dim3(2 * pairs), dim3(THREADS), 2, (size_t)smem, s, tx, p);
 }
 

@@ -26,10 +26,6 @@ class IfabInt4(C.Structure):
     _fields_ = [("units", C.c_void_p), ("N", C.c_int32), ("K", C.c_int32), ("group", C.c_int32), ("zeros", C.c_int32), ("gated", C.c_int32), ("f16", C.c_int32)]
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(f"int4: {what}")
@@ -60,7 +56,7 @@ class Int4Weight:
             out = torch.empty(self.rows, self.k, dtype=BF16, device=self.device)
         _need(out.shape == (self.rows, self.k) and out.dtype == BF16 and out.stride(1) == 1 and out.device == self.device, "the output must be bf16 [rows, k] beside the weights")
         with torch.cuda.device(self.device):
-            check(_lib.load().ifab_int4_dequantise(self.ref, out.data_ptr(), out.stride(0), _stream(self.device)), "int4.dequantise")
+            check(_lib.load().ifab_int4_dequantise(self.ref, out.data_ptr(), out.stride(0), _lib.current_stream(self.device.index)), "int4.dequantise")
         return out
 
 
@@ -71,7 +67,7 @@ def quantise(w: torch.Tensor, *, group: int = 128, zeros: bool = False, gated: b
     _need(w.dim() == 2 and w.dtype == BF16 and w.stride(1) == 1 and w.is_cuda, "the matrix must be bf16 [rows, k] on the device, columns contiguous")
     out = Int4Weight(w.shape[0], w.shape[1], group=group, zeros=zeros, gated=gated, device=w.device)
     with torch.cuda.device(w.device):
-        check(_lib.load().ifab_int4_quantise(out.ref, w.data_ptr(), w.stride(0), _stream(w.device)), "int4.quantise")
+        check(_lib.load().ifab_int4_quantise(out.ref, w.data_ptr(), w.stride(0), _lib.current_stream(w.device.index)), "int4.quantise")
     return out
 
 
@@ -86,7 +82,7 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor
     _need(zeros is None or zeros.dtype == torch.uint8, "zero points must be uint8")
     out = Int4Weight(rows, k, group=group, zeros=zeros is not None, gated=gated, f16=scales.dtype == F16, device=codes.device)
     with torch.cuda.device(codes.device):
-        check(_lib.load().ifab_int4_pack(out.ref, codes.data_ptr(), codes.stride(0), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _stream(codes.device)), "int4.pack")
+        check(_lib.load().ifab_int4_pack(out.ref, codes.data_ptr(), codes.stride(0), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _lib.current_stream(codes.device.index)), "int4.pack")
     return out
 
 
@@ -98,30 +94,49 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
     there it is not. ``status_ptr``: a status word for
     waits that run out."""
     T = x.shape[0]
-    _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
-    _need(x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 or T == 0, "rows must lie on 16 bytes")
-    if norm_w is not None:
-        _need(norm_w.shape == (w.k,) and norm_w.dtype == BF16 and norm_w.is_contiguous() and norm_w.device == w.device and norm_w.data_ptr() % 16 == 0, f"gains must be bf16 [{w.k}] on 16 bytes")
-        _need(T <= NORM_ROWS, f"a norm ahead of {T} rows is a launch of its own (ops.decode.rmsnorm)")
+    # the checks say what is wrong in _refuse: a message that is made for every call costs as much as the launch
+    if not (x.dim() == 2 and x.shape[1] == w.k and x.dtype is BF16 and x.device == w.device and x.stride(1) == 1 and (x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 or T == 0)):
+        _refuse(x, w, norm_w, residual, out)
     if out is None:
-        out = torch.empty(T, w.n, dtype=F32 if out_f32 else BF16, device=x.device)
-    else:
-        _need(out.shape == (T, w.n) and out.dtype in (BF16, F32) and out.stride(1) == 1 and out.device == w.device, f"the output must be bf16 or f32 [T, {w.n}] beside the weights")
-    if residual is not None:
-        _need(not w.gated, "a gated unit takes no residual")
-        _need(residual.shape == (T, w.n) and residual.dtype == BF16 and residual.stride(1) == 1 and residual.device == w.device, f"the residual must be bf16 [T, {w.n}] beside the weights")
+        out = torch.empty((T, w.n), dtype=F32 if out_f32 else BF16, device=w.device)
+    elif not (out.shape == (T, w.n) and (out.dtype is BF16 or out.dtype is F32) and out.device == w.device and out.stride(1) == 1):
+        _refuse(x, w, norm_w, residual, out)
+    if norm_w is not None and not (norm_w.shape == (w.k,) and norm_w.dtype is BF16 and norm_w.device == w.device and norm_w.stride(0) == 1 and norm_w.data_ptr() % 16 == 0 and T <= NORM_ROWS):
+        _refuse(x, w, norm_w, residual, out)
+    if residual is not None and not (not w.gated and residual.shape == (T, w.n) and residual.dtype is BF16 and residual.device == w.device and residual.stride(1) == 1):
+        _refuse(x, w, norm_w, residual, out)
     if T == 0:
         return out
-    dev = x.device.index
+    dev = w.device.index
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return linear(x, w, norm_w=norm_w, eps=eps, residual=residual, out=out, status_ptr=status_ptr)
+    lib, rp, ldr = _lib.load(), None, 0
+    if residual is not None:
+        rp, ldr = residual.data_ptr(), residual.stride(0)
+    f32 = 1 if out.dtype is F32 else 0
     if T > STREAM_ROWS:
-        scratch = torch.empty(_lib.load().ifab_int4_gemm_scratch(T, w.k), dtype=torch.uint8, device=x.device)
-        check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), x.stride(0), None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
-                                         out.data_ptr(), out.stride(0), out.dtype == F32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr, _stream(x.device)), "int4.linear")
+        scratch = torch.empty(lib.ifab_int4_gemm_scratch(T, w.k), dtype=torch.uint8, device=w.device)
+        check(lib.ifab_int4_gemm(w.ref, x.data_ptr(), x.stride(0), rp, ldr, out.data_ptr(), out.stride(0), f32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr,
+                                 _lib.current_stream(dev)), "int4.linear")
         return out
-    check(_lib.load().ifab_int4_rows(w.ref, x.data_ptr(), x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps,
-                                     None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
-                                     out.dtype == F32, T, status_ptr, _stream(x.device)), "int4.linear")
+    check(lib.ifab_int4_rows(w.ref, x.data_ptr(), x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps, rp, ldr, out.data_ptr(), out.stride(0), f32, T, status_ptr,
+                             _lib.current_stream(dev)), "int4.linear")
     return out
+
+
+def _refuse(x: torch.Tensor, w: Int4Weight, norm_w, residual, out) -> None:
+    T = x.shape[0] if x.dim() else 0
+    _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
+    _need(x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 or T == 0, "rows must lie on 16 bytes")
+    if norm_w is not None:
+        _need(norm_w.shape == (w.k,) and norm_w.dtype == BF16 and norm_w.is_contiguous() and norm_w.device == w.device and norm_w.data_ptr() % 16 == 0,
+              f"gains must be bf16 [{w.k}] on 16 bytes")
+        _need(T <= NORM_ROWS, f"a norm ahead of {T} rows is a launch of its own (ops.decode.rmsnorm)")
+    _need(out is None or (out.shape == (T, w.n) and out.dtype in (BF16, F32) and out.stride(1) == 1 and out.device == w.device),
+          f"the output must be bf16 or f32 [T, {w.n}] beside the weights")
+    if residual is not None:
+        _need(not w.gated, "a gated unit takes no residual")
+        _need(residual.shape == (T, w.n) and residual.dtype == BF16 and residual.stride(1) == 1 and residual.device == w.device,
+              f"the residual must be bf16 [T, {w.n}] beside the weights")
+    raise AssertionError("int4.linear: a call was refused without a reason")

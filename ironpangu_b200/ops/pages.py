@@ -37,10 +37,6 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(f"pages: {what}")
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 class PageSet:
     """Caches whose page ``i`` belongs together: contiguous tensors ``[pages, page_tokens, ...]`` of any types on one device, a row a multiple of 16 bytes."""
 
@@ -58,6 +54,7 @@ class PageSet:
         self._ptrs = torch.tensor([c.data_ptr() for c in caches], dtype=torch.int64, device=t.device)
         self._rows = torch.tensor(self.row_bytes, dtype=torch.int64, device=t.device)
         self.status = torch.zeros(1, dtype=I32, device=t.device)
+        self.status_ptr = self.status.data_ptr()
         self.desc = IfabPageSet(self._ptrs.data_ptr(), self._rows.data_ptr(), len(caches), self.pages, self.page_tokens, max(self.row_bytes))
         self.ref = C.byref(self.desc)
 
@@ -67,9 +64,10 @@ class PageSet:
             self.status.zero_()
             raise IndexError("pages: an index out of range was skipped")
 
-    def _list(self, t: torch.Tensor, what: str, n: Optional[int] = None) -> int:
-        _need(t.dim() == 1 and t.dtype == I32 and t.device == self.device and (t.numel() < 2 or t.stride(0) == 1), f"{what} must be a contiguous int32 list on {self.device}")
-        _need(n is None or t.numel() == n, f"{what}: {t.numel()} entries beside {n}")
+    def _list(self, t: torch.Tensor, what: str, n: int) -> int:
+        if not (t.dtype is I32 and t.dim() == 1 and t.device == self.device and (t.stride(0) == 1 or t.numel() < 2) and t.numel() == n):
+            _need(t.dim() == 1 and t.dtype == I32 and t.device == self.device and (t.numel() < 2 or t.stride(0) == 1), f"{what} must be a contiguous int32 list on {self.device}")
+            _need(False, f"{what}: {t.numel()} entries beside {n}")
         return t.data_ptr()
 
 
@@ -77,12 +75,19 @@ def copy(src: PageSet, dst: PageSet, src_ids: torch.Tensor, dst_ids: torch.Tenso
     """Page ``dst_ids[i]`` of every cache of ``dst`` becomes page ``src_ids[i]`` of ``src``, its first ``rows[i]`` rows only where ``rows`` is given. The sets have rows of
     the same sizes and may be one set; pages that are written must differ from one another and from those that are read. Entries out of range are skipped and reported in
     ``dst.status``."""
-    _need(src.row_bytes == dst.row_bytes and src.page_tokens == dst.page_tokens and src.device == dst.device, "the sets' pages are not alike")
+    if src is not dst and not (src.row_bytes == dst.row_bytes and src.page_tokens == dst.page_tokens and src.device == dst.device):
+        _need(False, "the sets' pages are not alike")
     n = src_ids.numel()
-    a, b = src._list(src_ids, "src_ids"), src._list(dst_ids, "dst_ids", n)
-    r = None if rows is None else src._list(rows, "rows", n)
-    with torch.cuda.device(src.device):
-        check(_lib.load().ifab_pages_copy(src.ref, dst.ref, a, b, r, n, dst.status.data_ptr(), _stream(src.device)), "pages.copy")
+    a, b = src._list(src_ids, "src_ids", n), src._list(dst_ids, "dst_ids", n)
+    _call(src.device.index, "ifab_pages_copy", src.ref, dst.ref, a, b, None if rows is None else src._list(rows, "rows", n), n, dst.status_ptr)
+
+
+def _call(dev: int, name: str, *args) -> None:
+    if dev == torch.cuda.current_device():
+        check(getattr(_lib.load(), name)(*args, _lib.current_stream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            check(getattr(_lib.load(), name)(*args, _lib.current_stream(dev)), name)
 
 
 class PagePool:
@@ -116,37 +121,32 @@ class PagePool:
                 raise IndexError("pages: a list of slots named one out of range or twice, or a length that no slot can hold")
             raise OverflowError("pages: the pool had fewer free pages than a call needed")
 
-    def _call(self, name: str, *args) -> None:
-        if self.device.index == torch.cuda.current_device():
-            check(getattr(_lib.load(), name)(self.ref, *args, _stream(self.device)), name)
-        else:
-            with torch.cuda.device(self.device):
-                check(getattr(_lib.load(), name)(self.ref, *args, _stream(self.device)), name)
-
     def extend(self, slots: torch.Tensor, tokens: torch.Tensor) -> None:
         """Slot ``slots[i]`` gets pages for positions below ``tokens[i]`` (where it has them already nothing changes). A slot may be named once. All or nothing."""
         n = slots.numel()
-        a, b = self.pages._list(slots, "slots"), self.pages._list(tokens, "tokens", n)
-        _need(n <= self.slots, f"{n} entries for {self.slots} slots")
-        self._call("ifab_pages_extend", a, b, n)
+        a, b = self.pages._list(slots, "slots", n), self.pages._list(tokens, "tokens", n)
+        if n > self.slots:
+            _need(False, f"{n} entries for {self.slots} slots")
+        _call(self.device.index, "ifab_pages_extend", self.ref, a, b, n)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Slot ``dst[i]`` becomes what slot ``src[i]`` was before the call; what it held before is given back. ``dst`` names a slot once, ``src`` as often as wanted, and a slot
         may be in both. Whole pages are shared. A partly filled page, which its sequence goes on writing, stays with the first child of a slot that is itself replaced; every
         other child gets a page of its own with the rows in use copied. All or nothing."""
         n = src.numel()
-        a, b = self.pages._list(src, "src"), self.pages._list(dst, "dst", n)
-        _need(n <= self.slots, f"{n} entries for {self.slots} slots")
-        self._call("ifab_pages_fork", a, b, n)
+        a, b = self.pages._list(src, "src", n), self.pages._list(dst, "dst", n)
+        if n > self.slots:
+            _need(False, f"{n} entries for {self.slots} slots")
+        _call(self.device.index, "ifab_pages_fork", self.ref, a, b, n)
 
     def free(self, slots: torch.Tensor, below: Optional[torch.Tensor] = None) -> None:
         """All pages of the slots are given back, or with ``below`` the whole pages all of whose positions lie below ``below[i]`` (a window has passed them); those
         entries of the table are -1 then. A page goes back to the pool when no other slot holds it."""
         n = slots.numel()
-        a, b = self.pages._list(slots, "slots"), None if below is None else self.pages._list(below, "below", n)
-        self._call("ifab_pages_free", a, b, n)
+        a, b = self.pages._list(slots, "slots", n), None if below is None else self.pages._list(below, "below", n)
+        _call(self.device.index, "ifab_pages_free", self.ref, a, b, n)
 
     def compact(self) -> None:
         """Live pages move into the lowest places - the first one that lies too high into the first hole, and so on - in all caches, and the table follows; their
         number lands in ``live``."""
-        self._call("ifab_pages_compact", self.live.data_ptr())
+        _call(self.device.index, "ifab_pages_compact", self.ref, self.live.data_ptr())
