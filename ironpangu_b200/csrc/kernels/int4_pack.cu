@@ -5,7 +5,10 @@
 //                infinity or NaN gets a scale of NaN: what it multiplies is NaN, not something else.
 //   pack         codes, scales and zero points of a checkpoint
 //   dequantise   bf16(s (q - z))
-// Bound by the bytes of the matrix. A warp has a unit: lane 4 g + c holds two runs of eight columns of rows g and g + 8 in both blocks; four lanes read 64 bytes of a row.
+// Bound by the bytes of the matrix. A CTA has a tile of sixteen rows and its warps the units in turn, so that the rows' largest scales are at hand in the end: lane 4 g + c
+// holds two runs of eight columns of rows g and g + 8 in both blocks; four lanes read 64 bytes of a row.
+// w / s is w times 1 / s and times what 1 / s was rounded off, off by 2^-45 ahead of its rounding to f32: a quotient that is half a step exactly comes out so, and others are
+// 2^-10 and more away from it, as w and s have eight bits.
 #include "int4.cuh"
 #include "ifab_kernels.h"
 
@@ -20,27 +23,31 @@ __device__ __forceinline__ uint32_t word_of(const uint8_t* q) {
   for (int j = 0; j < 4; ++j) w |= (uint32_t)q[2 * j] << (4 * j) | (uint32_t)q[2 * j + 1] << (4 * j + 16);
   return w << 3 | w >> 29;
 }
-// Rows' largest finite scales. The launch behind this one may read units ahead of its wait for the kernel before it (int4_rows.cu): this one is launched behind the end of the
-// kernels that write them, and `settled_kernel` behind its own.
-__global__ void __launch_bounds__(256) most_kernel(View v) {
-  const int row = blockIdx.x * 256 + threadIdx.x, tile = row / TILE, r = row % TILE;
-  if (tile >= v.halves * v.tiles) return;
-  float most = 0.f;
-  for (int ch = 0; ch < v.chunks; ++ch)
-    for (int i = 0; i < v.groups(); ++i) {
-      const float s = fabsf(scales_of(reinterpret_cast<const uint16_t*>(v.at(tile, ch) + CODES)[i * 16 + (r & 7) * 2 + (r >> 3)], v.f16).x);
-      if (s <= 3.4028234e38f) most = fmaxf(most, s);
-    }
-  v.most[row] = most;
-}
+// The launch behind a linear may read units ahead of its wait for the kernel before it (int4_rows.cu): this one is launched behind the end of the kernels that write them
 __global__ void settled_kernel() {}
+
+// rows' largest finite scales, out of the warps' (lane 4 g: rows g and g + 8) into v.most; all threads of the CTA
+__device__ __forceinline__ void keep_most(const View& v, int tile, float (&most)[2]) {
+  __shared__ float all[8][TILE];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((lane & 3) == 0) {
+    all[warp][lane >> 2] = most[0];
+    all[warp][(lane >> 2) + 8] = most[1];
+  }
+  __syncthreads();
+  if (threadIdx.x < TILE) {
+    float m = 0.f;
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, all[w][threadIdx.x]);
+    v.most[tile * TILE + threadIdx.x] = m;
+  }
+}
 
 struct Place {           // of a lane in its unit
   int tile, chunk, half, row0, g, c;
-  __device__ __forceinline__ Place(const View& v, long unit) {
+  __device__ __forceinline__ Place(const View& v, int tile_, int chunk_) {
     const int lane = threadIdx.x & 31;
-    tile = (int)(unit / v.chunks);
-    chunk = (int)(unit - (long)tile * v.chunks);
+    tile = tile_;
+    chunk = chunk_;
     half = tile >= v.tiles;
     row0 = (tile - half * v.tiles) * TILE;
     g = lane >> 2;
@@ -53,95 +60,121 @@ struct Place {           // of a lane in its unit
 };
 
 template <int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(256) quantise_kernel(View v, const bf16* w, long ldw, long units) {
+__global__ void __launch_bounds__(256) quantise_kernel(View v, const bf16* w, long ldw) {
   grid_dep_wait();
-  const long unit = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= units) return;
-  const Place at(v, unit);
-  unsigned char* out = v.at(at.tile, at.chunk);
-  float f[2][4][8];        // [row][run][column]
+  float most[2] = {0.f, 0.f};
+#pragma unroll 1
+  for (int chunk = threadIdx.x >> 5; chunk < v.chunks; chunk += 8) {
+    const Place at(v, blockIdx.x, chunk);
+    unsigned char* out = v.at(at.tile, at.chunk);
+    uint4 u[2][4];           // [row][run]
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const long row = at.row(v, h);
-      const int k = at.col(r);
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (row >= 0 && k < v.K) u = ld_stream16(w + row * ldw + k);
-      unpack8(u, f[h][r]);
-    }
-  constexpr int RUNS = GROUP / 32;      // of a group
+      for (int r = 0; r < 4; ++r) {
+        const long row = at.row(v, h);
+        const int k = at.col(r);
+        u[h][r] = make_uint4(0, 0, 0, 0);
+        if (row >= 0 && k < v.K) u[h][r] = ld_stream16(w + row * ldw + k);
+      }
+    constexpr int RUNS = GROUP / 32;      // of a group
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int r0 = 0; r0 < 4; r0 += RUNS) {
-      float lo = 0.f, hi = 0.f;
-      int bad = 0;
+      for (int r0 = 0; r0 < 4; r0 += RUNS) {
+        // the smallest and the largest, NaN where there is one
+        __nv_bfloat162 two_lo = __float2bfloat162_rn(0.f), two_hi = two_lo;
 #pragma unroll
-      for (int r = r0; r < r0 + RUNS; ++r)
+        for (int r = r0; r < r0 + RUNS; ++r) {
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&u[h][r]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x = f[h][r][i];
-          lo = fminf(lo, x);
-          hi = fmaxf(hi, x);
-          bad |= !(fabsf(x) <= 3.4028234e38f);
+          for (int i = 0; i < 4; ++i) {
+            two_lo = __hmin2_nan(two_lo, x[i]);
+            two_hi = __hmax2_nan(two_hi, x[i]);
+          }
         }
 #pragma unroll
-      for (int o = 1; o < 4; o *= 2) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-      }
-      bf16 sb = __float2bfloat16_rn(ZEROS ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f));
-      const float s = __bfloat162float(sb) == 0.f ? 1.f : __bfloat162float(sb);
-      const float z = ZEROS ? fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f) : 8.f;
+        for (int o = 1; o < 4; o *= 2) {
+          two_lo = __hmin2_nan(two_lo, __shfl_xor_sync(0xffffffffu, two_lo, o));
+          two_hi = __hmax2_nan(two_hi, __shfl_xor_sync(0xffffffffu, two_hi, o));
+        }
+        const float lo = __bfloat162float(__hmin_nan(two_lo.x, two_lo.y)), hi = __bfloat162float(__hmax_nan(two_hi.x, two_hi.y));
+        const bool bad = !(fabsf(lo) <= 3.4028234e38f && fabsf(hi) <= 3.4028234e38f);
+        const bf16 sb = __float2bfloat16_rn(ZEROS ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f));
+        const float s = __bfloat162float(sb) == 0.f ? 1.f : __bfloat162float(sb), by = __frcp_rn(s);
+        const int z = ZEROS && !bad ? (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f) : 8;
+        const float rest = fmaf(-s, by, 1.f) * by, top = (float)(15 - z);
+        const bool tiny = s < 1.1754944e-38f || bad;      // 1 / s is no number to multiply by
 #pragma unroll
-      for (int r = r0; r < r0 + RUNS; ++r) {
-        uint8_t q[8];
+        for (int r = r0; r < r0 + RUNS; ++r) {
+          constexpr float SHIFT = 12582912.f;              // 1.5 2^23: a number near it has its nearest integer in its last bits, halves to even
+          float f[8];
+          unpack8(u[h][r], f);
+          uint32_t word = (z - 0x4b400000u) * 0x11111111u;
+          if (tiny) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = (uint8_t)(bad ? z : fminf(fmaxf(rintf(__fdiv_rn(f[h][r][i], s)) + z, 0.f), 15.f));
-        *reinterpret_cast<uint32_t*>(out + (r >> 1) * 512 + code_at(at.g, at.c) + 8 * h + 4 * (r & 1)) = word_of(q);
+            for (int i = 0; i < 8; ++i) f[i] = bad ? 0.f : fminf(fmaxf(__fdiv_rn(f[i], s), -(float)z), top);
+          } else {
+            // without zero points a quotient is at most 7 (1 + 2^-8), with them at least -(z + 1/2)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              f[i] = fmaf(f[i], by, f[i] * rest);
+              if (ZEROS) f[i] = fminf(f[i], top);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) word += __float_as_uint(f[i] + SHIFT) << ((i >> 1) * 4 + (i & 1) * 16);
+          *reinterpret_cast<uint32_t*>(out + (r >> 1) * 512 + code_at(at.g, at.c) + 8 * h + 4 * (r & 1)) = word << 3 | word >> 29;
+        }
+        if (at.c == 0) {
+          const int group = r0 / RUNS;
+          reinterpret_cast<bf16*>(out + CODES)[group * 16 + at.g * 2 + h] = bad ? __ushort_as_bfloat16(0x7fc0) : sb;
+          if (ZEROS) (out + CODES + v.groups() * 32)[group * 16 + at.g * 2 + h] = (uint8_t)z;
+        }
+        if (!bad) most[h] = fmaxf(most[h], __bfloat162float(sb));
       }
-      if (at.c == 0) {
-        const int group = r0 / RUNS;
-        reinterpret_cast<bf16*>(out + CODES)[group * 16 + at.g * 2 + h] = bad ? __ushort_as_bfloat16(0x7fc0) : sb;
-        if (ZEROS) (out + CODES + v.groups() * 32)[group * 16 + at.g * 2 + h] = (uint8_t)z;
-      }
-    }
+  }
+  keep_most(v, blockIdx.x, most);
 }
 
-__global__ void __launch_bounds__(256) pack_kernel(View v, const uint8_t* codes, long ldc, const uint16_t* scales, const uint8_t* zeros, long units) {
+__global__ void __launch_bounds__(256) pack_kernel(View v, const uint8_t* codes, long ldc, const uint16_t* scales, const uint8_t* zeros) {
   grid_dep_wait();
-  const long unit = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= units) return;
-  const Place at(v, unit);
-  unsigned char* out = v.at(at.tile, at.chunk);
+  float most[2] = {0.f, 0.f};
   const int per = (v.K + v.group - 1) / v.group;       // groups of a row
-  for (int h = 0; h < 2; ++h) {
-    const long row = at.row(v, h);
-    for (int r = 0; r < 4; ++r) {
-      uint8_t q[8];
-      for (int i = 0; i < 8; ++i) {
-        const int k = at.col(r) + i;
-        q[i] = row < 0 ? 8 : k < v.K ? codes[row * ldc + k] & 15 : zeros ? zeros[row * per + min(k / v.group, per - 1)] & 15 : 8;
+  for (int chunk = threadIdx.x >> 5; chunk < v.chunks; chunk += 8)
+    for (int h = 0; h < 2; ++h) {
+      const Place at(v, blockIdx.x, chunk);
+      unsigned char* out = v.at(at.tile, at.chunk);
+      const long row = at.row(v, h);
+      for (int r = 0; r < 4; ++r) {
+        uint8_t q[8];
+        for (int i = 0; i < 8; ++i) {
+          const int k = at.col(r) + i;
+          q[i] = row < 0 ? 8 : k < v.K ? codes[row * ldc + k] & 15 : zeros ? zeros[row * per + min(k / v.group, per - 1)] & 15 : 8;
+        }
+        *reinterpret_cast<uint32_t*>(out + (r >> 1) * 512 + code_at(at.g, at.c) + 8 * h + 4 * (r & 1)) = word_of(q);
       }
-      *reinterpret_cast<uint32_t*>(out + (r >> 1) * 512 + code_at(at.g, at.c) + 8 * h + 4 * (r & 1)) = word_of(q);
+      float widest = 0.f;
+      if (at.c < v.groups()) {
+        const int group = at.chunk * v.groups() + at.c;
+        const bool in = row >= 0 && group < per;
+        if (in) widest = fabsf(scales_of(scales[row * per + group], v.f16).x);
+        reinterpret_cast<uint16_t*>(out + CODES)[at.c * 16 + at.g * 2 + h] = in ? scales[row * per + group] : 0;
+        // a group beyond K: the zero point that its codes were given above
+        if (v.zeros) (out + CODES + v.groups() * 32)[at.c * 16 + at.g * 2 + h] = row < 0 ? 8 : zeros[row * per + min(group, per - 1)] & 15;
+      }
+      if (!(widest <= 3.4028234e38f)) widest = 0.f;
+      for (int o = 1; o < 4; o *= 2) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, o));
+      most[h] = fmaxf(most[h], widest);
     }
-    if (at.c < v.groups()) {
-      const int group = at.chunk * v.groups() + at.c;
-      const bool in = row >= 0 && group < per;
-      reinterpret_cast<uint16_t*>(out + CODES)[at.c * 16 + at.g * 2 + h] = in ? scales[row * per + group] : 0;
-      // a group beyond K: the zero point that its codes were given above
-      if (v.zeros) (out + CODES + v.groups() * 32)[at.c * 16 + at.g * 2 + h] = row < 0 ? 8 : zeros[row * per + min(group, per - 1)] & 15;
-    }
-  }
+  keep_most(v, blockIdx.x, most);
 }
 
 __global__ void __launch_bounds__(256) dequantise_kernel(View v, bf16* w, long ldw, long units) {
   grid_dep_wait();
   const long unit = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (unit >= units) return;
-  const Place at(v, unit);
+  const Place at(v, (int)(unit / v.chunks), (int)(unit % v.chunks));
   const unsigned char* in = v.at(at.tile, at.chunk);
   uint4 u[2];              // [block]: row g's two runs, row g + 8's
   u[0] = ld_stream16(in + code_at(at.g, at.c));
@@ -170,11 +203,10 @@ __global__ void __launch_bounds__(256) dequantise_kernel(View v, bf16* w, long l
 }
 
 template <int GROUP>
-int launch_quantise(const View& v, const bf16* w, long ldw, long units, cudaStream_t s) {
-  return launch_chain(v.zeros ? quantise_kernel<GROUP, true> : quantise_kernel<GROUP, false>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, s, v, w, ldw, units);
+int launch_quantise(const View& v, const bf16* w, long ldw, cudaStream_t s) {
+  return launch_chain(v.zeros ? quantise_kernel<GROUP, true> : quantise_kernel<GROUP, false>, dim3(v.halves * v.tiles), dim3(256), 0, s, v, w, ldw);
 }
-int settle(const View& v, cudaStream_t s) {
-  most_kernel<<<(v.halves * v.tiles * TILE + 255) / 256, 256, 0, s>>>(v);
+int settle(cudaStream_t s) {
   settled_kernel<<<1, 32, 0, s>>>();
   return (int)cudaGetLastError();
 }
@@ -190,21 +222,19 @@ extern "C" uint64_t ifab_int4_bytes(int N, int K, int group, int zeros, int gate
 extern "C" int ifab_int4_quantise(const IfabInt4* d, const void* w, long ldw, void* stream) {
   View v;
   if (view_of(d, &v) || v.f16 || !w || (uintptr_t)w % 16 || ldw % 8 || ldw < v.K) return -1;
-  const long units = (long)v.halves * v.tiles * v.chunks;
   cudaStream_t s = (cudaStream_t)stream;
   const bf16* p = (const bf16*)w;
-  int rc = v.group == 128 ? launch_quantise<128>(v, p, ldw, units, s) : v.group == 64 ? launch_quantise<64>(v, p, ldw, units, s) : launch_quantise<32>(v, p, ldw, units, s);
-  return rc ? rc : settle(v, s);
+  int rc = v.group == 128 ? launch_quantise<128>(v, p, ldw, s) : v.group == 64 ? launch_quantise<64>(v, p, ldw, s) : launch_quantise<32>(v, p, ldw, s);
+  return rc ? rc : settle(s);
 }
 
 // codes [N or 2 N, K] a byte each (low four bits), scales and zero points [N or 2 N, ceil(K / group)]
 extern "C" int ifab_int4_pack(const IfabInt4* d, const uint8_t* codes, long ldc, const void* scales, const uint8_t* zeros, void* stream) {
   View v;
   if (view_of(d, &v) || !codes || !scales || (uintptr_t)scales % 2 || (v.zeros != 0) != (zeros != nullptr) || ldc < v.K) return -1;
-  const long units = (long)v.halves * v.tiles * v.chunks;
   cudaStream_t s = (cudaStream_t)stream;
-  int rc = launch_chain(pack_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, s, v, codes, ldc, (const uint16_t*)scales, zeros, units);
-  return rc ? rc : settle(v, s);
+  int rc = launch_chain(pack_kernel, dim3(v.halves * v.tiles), dim3(256), 0, s, v, codes, ldc, (const uint16_t*)scales, zeros);
+  return rc ? rc : settle(s);
 }
 
 // out [N or 2 N, K] in bf16, rows on 16 bytes
