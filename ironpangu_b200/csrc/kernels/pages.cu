@@ -7,9 +7,10 @@
 // right behind them. A bit a page keeps the search for free pages short: one CTA reads them all at once.
 //
 //   extend     one CTA: pages that each slot of the list lacks, free bits counted per thread, all of them handed out by rank
-//   fork       rows of the table as they were go to a workspace while counts follow (a CTA a row and piece); the last CTA to finish takes the pages for partly filled
-//              ones. Behind it, copies of those pages in all caches, and the rows into the table; or, where pages lack, the counts back.
-//   free       an entry is exchanged for -1 and the page given back by whoever got it, so that naming a slot twice is the same as once
+//   fork       rows of the table as they were go to a workspace while counts follow (a CTA a parent and piece of its row, which changes a page's count once for all its
+//              children); the last CTA to finish takes the pages for partly filled ones. Behind it, copies of those pages in all caches, and the rows into the table;
+//              or, where pages lack, the counts back.
+//   free       a thread has an entry of eight slots and changes a page's count once for those of them next to one another that name it: forks do
 //   compact    one CTA ranks holes below and pages above the number of live pages; then copies and every entry of the table
 //   copy       a CTA copies a page of a cache
 // Bound by the bytes that are copied; launches otherwise.
@@ -40,11 +41,11 @@ enum Control { COUNT, TICKET, GO, LIVE };
 uint64_t work_words(int slots, int max_pages, int pages) { return 8 + 3ull * std::max(pages, slots) + slots + (uint64_t)slots * max_pages; }
 
 __device__ __forceinline__ void turn(const IfabPagePool& p, int page) { atomicXor(p.free_bits + (page >> 5), 1u << (page & 31)); }
-__device__ __forceinline__ void take(const IfabPagePool& p, int page) {
-  if (page >= 0 && page < p.set.pages && atomicAdd(p.refs + page, 1) == 0) turn(p, page);
+__device__ __forceinline__ void take(const IfabPagePool& p, int page, int times = 1) {
+  if (page >= 0 && page < p.set.pages && atomicAdd(p.refs + page, times) == 0) turn(p, page);
 }
-__device__ __forceinline__ void give(const IfabPagePool& p, int page) {
-  if (page >= 0 && page < p.set.pages && atomicSub(p.refs + page, 1) == 1) turn(p, page);
+__device__ __forceinline__ void give(const IfabPagePool& p, int page, int times = 1) {
+  if (page >= 0 && page < p.set.pages && atomicSub(p.refs + page, times) == times) turn(p, page);
 }
 __device__ __forceinline__ void report(uint32_t* status, uint32_t bit) {
   if (status) atomicOr(status, bit);
@@ -86,20 +87,34 @@ __device__ __forceinline__ bool distinct(const int32_t* list, int n, int slots, 
   }
   return __syncthreads_and(good);
 }
-// `take_page(rank, page)` for the lowest `want` free pages (of `total` or more), threads of one CTA; words of the bits are spread over the threads in order
+// `take_page(rank, page)` for the lowest `want` free pages (there are as many), threads of one CTA that `ahead` free pages of lie below this one's; their bits are cleared.
+// Words of the bits are spread over the threads in order, pages over all threads by way of `list` (TAKEN ints of shared memory).
+constexpr int TAKEN = 2048;
 template <class F>
-__device__ __forceinline__ void lowest_free(const IfabPagePool& p, int want, int ahead, F&& take_page) {
+__device__ __forceinline__ void lowest_free(const IfabPagePool& p, int want, int ahead, int* list, F&& take_page) {
   const int words = (p.set.pages + 31) / 32, per = (words + blockDim.x - 1) / blockDim.x;
-  for (int i = 0; i < per && ahead < want; ++i) {
-    const int w = threadIdx.x * per + i;
-    if (w >= words) break;
-    uint32_t bits = *(volatile uint32_t*)(p.free_bits + w);
-    while (bits && ahead < want) {
-      const int b = __ffs(bits) - 1;
+  int w = threadIdx.x * per;
+  const int end = min(w + per, words);
+  uint32_t bits = w < end ? *(volatile uint32_t*)(p.free_bits + w) : 0;
+  bool changed = false;
+  for (int t0 = 0; t0 < want; t0 += TAKEN) {
+    const int t1 = min(t0 + TAKEN, want);
+    while (w < end && ahead < t1) {
+      if (!bits) {
+        if (changed) p.free_bits[w] = 0;
+        changed = false;
+        if (++w < end) bits = *(volatile uint32_t*)(p.free_bits + w);
+        continue;
+      }
+      list[ahead++ - t0] = w * 32 + __ffs(bits) - 1;
       bits &= bits - 1;
-      take_page(ahead++, w * 32 + b);
+      changed = true;
     }
+    __syncthreads();
+    for (int i = t0 + threadIdx.x; i < t1; i += blockDim.x) take_page(i, list[i - t0]);
+    __syncthreads();
   }
+  if (changed) p.free_bits[w] = bits;
 }
 __device__ __forceinline__ int my_free(const IfabPagePool& p) {
   const int words = (p.set.pages + 31) / 32, per = (words + blockDim.x - 1) / blockDim.x;
@@ -144,7 +159,7 @@ __global__ void __launch_bounds__(256) copy_kernel(IfabPageSet src, IfabPageSet 
 __global__ void __launch_bounds__(PLAN) extend_kernel(Pool q, const int32_t* slots, const int32_t* tokens, int n) {
   __shared__ uint32_t seen[MAX_SLOTS / 32];
   __shared__ int warps[33];
-  __shared__ int ahead[MAX_SLOTS + 1];           // pages that the slots of the list ahead of each lack
+  __shared__ int ahead[MAX_SLOTS + 1], list[TAKEN];           // ahead: pages that the slots of the list ahead of each lack
   grid_dep_launch();
   grid_dep_wait();
   const IfabPagePool& p = q.p;
@@ -174,7 +189,7 @@ __global__ void __launch_bounds__(PLAN) extend_kernel(Pool q, const int32_t* slo
     if (threadIdx.x == 0) report(p.status, good ? IFAB_STATUS_NO_PAGES : IFAB_STATUS_BAD_INDEX);
     return;
   }
-  lowest_free(p, base, mine, [&](int rank, int page) {
+  lowest_free(p, base, mine, list, [&](int rank, int page) {
     int lo = 0, hi = n - 1;                      // the last slot of the list with ahead <= rank
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -184,34 +199,56 @@ __global__ void __launch_bounds__(PLAN) extend_kernel(Pool q, const int32_t* slo
     const int s = slots[lo];
     p.table[(long)s * p.max_pages + (p.lengths[s] + pt - 1) / pt + rank - ahead[lo]] = page;
     p.refs[page] = 1;
-    turn(p, page);
   });
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x) p.lengths[slots[i]] = max(p.lengths[slots[i]], tokens[i]);
 }
 
-// grid (rows of the list, pieces of a row)
+// grid (entries of the list, pieces of a row): the CTAs of the first entry that names a parent have all of its children
 __global__ void __launch_bounds__(256) fork_kernel(Pool q, const int32_t* src, const int32_t* dst, int n) {
   __shared__ uint32_t seen[MAX_SLOTS / 32];
-  __shared__ int warps[33];
+  __shared__ int warps[33], list[TAKEN], children;
+  __shared__ uint16_t entry[MAX_SLOTS];
   __shared__ bool last;
   grid_dep_launch();
   grid_dep_wait();
   const IfabPagePool& p = q.p;
-  bool good = distinct(dst, n, p.slots, seen);
-  for (int i = threadIdx.x; i < n; i += blockDim.x) good = good && src[i] >= 0 && src[i] < p.slots;
+  const int parent = src[blockIdx.x];
+  if (threadIdx.x == 0) children = 0;
+  bool good = distinct(dst, n, p.slots, seen), earlier = false;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int a = src[i];
+    good = good && a >= 0 && a < p.slots;
+    earlier = earlier || (a == parent && i < (int)blockIdx.x);
+    if (a == parent) entry[atomicAdd(&children, 1)] = (uint16_t)i;
+  }
   good = __syncthreads_and(good);
-  if (good) {
-    const int i = blockIdx.x, a = src[i], b = dst[i], step = gridDim.y * blockDim.x;
-    for (int j = blockIdx.y * blockDim.x + threadIdx.x; j < p.max_pages; j += step) {
-      const int now = p.table[(long)b * p.max_pages + j], then = p.table[(long)a * p.max_pages + j];
-      q.staged()[(long)i * p.max_pages + j] = then;
-      if (now != then) {
-        take(p, then);
-        give(p, now);
+  earlier = __syncthreads_or(earlier);
+  if (good && !earlier) {
+    // 64 entries side by side, every fourth child a thread
+    const int32_t* row = p.table + (long)parent * p.max_pages;
+    for (int j = blockIdx.y * 64 + (threadIdx.x & 63); j < p.max_pages; j += gridDim.y * 64) {
+      const int then = row[j];
+      int times = 0;
+      for (int c0 = threadIdx.x >> 6; c0 < children; c0 += 32) {
+        int now[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c0 + 4 * c < children) now[c] = p.table[(long)dst[entry[c0 + 4 * c]] * p.max_pages + j];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c0 + 4 * c < children) {
+            q.staged()[(long)entry[c0 + 4 * c] * p.max_pages + j] = then;
+            if (now[c] != then) {
+              ++times;
+              give(p, now[c]);
+            }
+          }
       }
+      if (times) take(p, then, times);
     }
-    if (blockIdx.y == 0 && threadIdx.x == 0) q.used()[i] = p.lengths[a];
+    if (blockIdx.y == 0)
+      for (int c = threadIdx.x; c < children; c += blockDim.x) q.used()[entry[c]] = p.lengths[parent];
   }
   __threadfence();
   __syncthreads();
@@ -257,13 +294,12 @@ __global__ void __launch_bounds__(256) fork_kernel(Pool q, const int32_t* src, c
   __syncthreads();
   const bool enough = free_pages >= count;
   if (enough)
-    lowest_free(p, count, mine, [&](int rank, int page) {
+    lowest_free(p, count, mine, list, [&](int rank, int page) {
       const int i = ((volatile int32_t*)q.place())[rank], length = ((volatile int32_t*)q.used())[i];
       q.to()[rank] = page;
       q.staged()[(long)i * p.max_pages + length / p.set.page_tokens] = page;
-      give(p, ((volatile int32_t*)q.from())[rank]);
+      atomicSub(p.refs + ((volatile int32_t*)q.from())[rank], 1);      // its first owner keeps it
       p.refs[page] = 1;
-      turn(p, page);
     });
   if (threadIdx.x == 0) {
     if (!enough) report(p.status, IFAB_STATUS_NO_PAGES);
@@ -301,23 +337,55 @@ __global__ void __launch_bounds__(256) fork_rows_kernel(Pool q, const int32_t* s
   }
 }
 
-// grid (list, pieces of a row)
+// grid (eight entries of the list, pieces of a row)
+constexpr int TOGETHER = 8;
 __global__ void __launch_bounds__(256) free_kernel(Pool q, const int32_t* slots, const int32_t* below, int n) {
+  __shared__ int slot[TOGETHER], end[TOGETHER];
   grid_dep_launch();
   grid_dep_wait();
   const IfabPagePool& p = q.p;
-  const int i = blockIdx.x, s = slots[i], step = gridDim.y * blockDim.x;
-  if (s < 0 || s >= p.slots || (below && below[i] < 0)) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) report(p.status, IFAB_STATUS_BAD_INDEX);
-    return;
+  const int first = blockIdx.x * TOGETHER, count = min(TOGETHER, n - first), step = gridDim.y * blockDim.x;
+  if (threadIdx.x < count) {
+    const int i = first + threadIdx.x, s = slots[i], b = below ? below[i] : 0;
+    const bool good = s >= 0 && s < p.slots && b >= 0;
+    slot[threadIdx.x] = good ? s : -1;
+    // a page that is partly filled stays with its sequence
+    end[threadIdx.x] = !good ? 0 : below ? min(b, p.lengths[s]) / p.set.page_tokens : p.max_pages;
+    if (!good && blockIdx.y == 0) report(p.status, IFAB_STATUS_BAD_INDEX);
+    if (good && !below && blockIdx.y == 0) p.lengths[s] = 0;
   }
-  // a page that is partly filled stays with its sequence
-  const int end = below ? min(below[i], p.lengths[s]) / p.set.page_tokens : p.max_pages;
-  for (int j = blockIdx.y * blockDim.x + threadIdx.x; j < end; j += step) {
-    int32_t* entry = p.table + (long)s * p.max_pages + j;
-    if (*entry >= 0) give(p, atomicExch(entry, -1));
+  __syncthreads();
+  // a slot that is named more than once: the first entry does it, as far as the furthest of them goes
+  for (int e = threadIdx.x; e < count * n; e += blockDim.x) {
+    const int c = e / n, k = e - c * n;
+    if (k == first + c || slots[k] != slot[c] || (below && below[k] < 0)) continue;
+    if (k < first + c) atomicExch(&slot[c], -1);
+    else if (below) atomicMax(&end[c], min(below[k], p.lengths[slots[k]]) / p.set.page_tokens);
   }
-  if (!below && blockIdx.y == 0 && threadIdx.x == 0) p.lengths[s] = 0;
+  __syncthreads();
+  for (int j = blockIdx.y * blockDim.x + threadIdx.x; j < p.max_pages; j += step) {
+    int page = -1, times = 0;
+    int had[TOGETHER];
+#pragma unroll
+    for (int c = 0; c < TOGETHER; ++c) {
+      const bool mine = c < count && slot[c] >= 0 && j < end[c];
+      had[c] = mine ? p.table[(long)slot[c] * p.max_pages + j] : -1;
+    }
+#pragma unroll
+    for (int c = 0; c < TOGETHER; ++c)
+      if (had[c] >= 0) p.table[(long)slot[c] * p.max_pages + j] = -1;
+#pragma unroll
+    for (int c = 0; c < TOGETHER; ++c) {
+      if (had[c] < 0) continue;
+      if (had[c] != page) {
+        if (times) give(p, page, times);
+        page = had[c];
+        times = 0;
+      }
+      ++times;
+    }
+    if (times) give(p, page, times);
+  }
 }
 
 __global__ void __launch_bounds__(PLAN) compact_plan_kernel(Pool q, int32_t* live_out) {
@@ -396,7 +464,8 @@ bool good_pool(const IfabPagePool* p) {
   return p && good_set(&p->set) && p->table && p->lengths && p->refs && p->free_bits && p->work && p->slots > 0 && p->slots <= MAX_SLOTS && p->max_pages > 0;
 }
 int grid_of(long items) { return (int)std::min<long>(std::max<long>(items, 1), 8l * tc::device_sms()); }
-int pieces_of(int max_pages) { return std::min(std::max((max_pages + 1023) / 1024, 1), 16); }
+// CTAs that share a row by `entries` entries each, as long as they all run at once
+int pieces_of(int rows, int max_pages, int entries) { return std::max(1, std::min((max_pages + entries - 1) / entries, 8 * tc::device_sms() / std::max(rows, 1))); }
 
 }  // namespace
 
@@ -420,14 +489,15 @@ extern "C" int ifab_pages_fork(const IfabPagePool* p, const int32_t* src, const 
   if (!good_pool(p) || n < 0 || n > p->slots) return -1;
   if (n == 0) return 0;
   cudaStream_t s = (cudaStream_t)stream;
-  if (int rc = launch_chain(fork_kernel, dim3(n, pieces_of(p->max_pages)), dim3(256), 0, s, Pool{*p}, src, dst, n)) return rc;
+  if (int rc = launch_chain(fork_kernel, dim3(n, pieces_of(n, p->max_pages, 64)), dim3(256), 0, s, Pool{*p}, src, dst, n)) return rc;
   return launch_chain(fork_rows_kernel, dim3(grid_of((long)n * p->set.caches)), dim3(256), 0, s, Pool{*p}, src, dst, n);
 }
 // all pages of slots[i], or those whose positions all lie below below[i]
 extern "C" int ifab_pages_free(const IfabPagePool* p, const int32_t* slots, const int32_t* below, int n, void* stream) {
   if (!good_pool(p) || n < 0) return -1;
   if (n == 0) return 0;
-  return launch_chain(free_kernel, dim3(n, pieces_of(p->max_pages)), dim3(256), 0, (cudaStream_t)stream, Pool{*p}, slots, below, n);
+  const int groups = (n + TOGETHER - 1) / TOGETHER;
+  return launch_chain(free_kernel, dim3(groups, pieces_of(groups, p->max_pages, 256)), dim3(256), 0, (cudaStream_t)stream, Pool{*p}, slots, below, n);
 }
 // live pages into the lowest places; their number into *live (may be null)
 extern "C" int ifab_pages_compact(const IfabPagePool* p, int32_t* live, void* stream) {
