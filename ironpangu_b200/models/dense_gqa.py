@@ -7,7 +7,8 @@ down GEMV fused with all-reduce + residual. 6 launches per layer, no stand-alone
 rank 5, as the qkv launch rotates and appends, and the linears are streams through rings in shared memory.
 Query rows of different sequences (continuous batching) share every launch: each row carries its
 own position and sequence slot. Sampling is greedy (fused with the lm_head) or top-k / top-p on the
-device. The reference's dense family runs per-layer composites of vendor ops with an all-gather
+device. :func:`quantise_weights` puts the linears' weights into 4 bits (one rank). With ``page_pool`` the pages come from a pool on the device
+(``ops/pages.py``), so that sequences can be forked inside a step. The reference's dense family runs per-layer composites of vendor ops with an all-gather
 after every sharded projection (native/src/inferfabric_acl.cpp:688-755, 1236-1433).
 """
 from __future__ import annotations
@@ -19,6 +20,8 @@ from typing import Dict, Optional
 import torch
 
 from ..ops import decode as K
+from ..ops import int4
+from ..ops.pages import PagePool
 from ..parallel.fabric import Fabric
 
 BF16 = torch.bfloat16
@@ -114,6 +117,19 @@ def random_rank_weights(c: DenseConfig, rank: int, world: int, device, seed: int
     return out
 
 
+LINEARS = ("qkv", "o_proj", "gate_up", "down")
+
+
+def quantise_weights(weights: Dict[str, torch.Tensor], group: int = 128, zeros: bool = True) -> Dict[str, object]:
+    """The weights of one rank with the four linears of every layer in 4 bits (``int4.Int4Weight``: a scale and, with ``zeros``, a zero point per ``group`` columns);
+    embedding, norms and the output matrix stay as they are. The bf16 matrices are let go one by one: ``weights`` loses them."""
+    out = {}
+    for name in list(weights):
+        t = weights.pop(name) if name.split(".")[-1] in LINEARS else weights[name]
+        out[name] = int4.quantise(t, group=group, zeros=zeros, gated=name.endswith("gate_up")) if name.split(".")[-1] in LINEARS else t
+    return out
+
+
 def bundle_parameters(cfg: DenseConfig, weights: Dict[str, torch.Tensor], world: int = 1, prefix: str = "model") -> Dict[str, torch.Tensor]:
     """This module's per-rank weight tensors under the parameter names of a bundle compiled from
     ``compiler.sources.dense_gqa_source`` (``model.layers.N.self_attn.q_proj`` ..., pairs joined by ``|``). The q / k / v
@@ -140,9 +156,13 @@ class DenseDecoder:
 
     def __init__(self, cfg: DenseConfig, weights: Dict[str, torch.Tensor], fabric: Fabric, *, max_tokens: int = 8,
                  max_context: int = 1024, num_slots: int = 1, keys_per_split: int = 64, keep_logits: bool = False,
-                 num_pages: Optional[int] = None):
+                 num_pages: Optional[int] = None, page_pool: bool = False):
+        """``page_pool``: the pages belong to ``self.pool`` and a slot has none until it is extended; otherwise every slot has its own from the start."""
         self.cfg, self.w, self.fabric = cfg, weights, fabric
         self.rank, self.world = fabric.rank, fabric.world
+        self.int4 = isinstance(weights["layers.0.qkv"], int4.Int4Weight)
+        if self.int4 and fabric.world > 1:
+            raise ValueError("4-bit weights run on one rank")
         c, dev = cfg, fabric.device
         assert c.heads % self.world == 0 and c.kv_heads % self.world == 0 and c.ffn % (8 * self.world) == 0 and c.vocab % self.world == 0
         self.hq, self.hk, self.vl = c.heads // self.world, c.kv_heads // self.world, c.vocab // self.world
@@ -163,6 +183,9 @@ class DenseDecoder:
             .view(num_slots, self.max_pages).contiguous()
         self.k_cache = [torch.zeros(self.num_pages, c.page_tokens, self.hk, c.head_dim, dtype=BF16, device=dev) for _ in range(c.layers)]
         self.v_cache = [torch.zeros_like(self.k_cache[0]) for _ in range(c.layers)]
+        self.pool = PagePool(self.k_cache + self.v_cache, slots=num_slots, max_pages=self.max_pages) if page_pool else None
+        if page_pool:
+            self.page_table = self.pool.table
         e = lambda *s, dt=BF16: torch.empty(*s, dtype=dt, device=dev)
         self.x = e(T, c.hidden)
         self.qkv = e(T, (self.hq + 2 * self.hk) * c.head_dim)
@@ -173,15 +196,25 @@ class DenseDecoder:
         self.next_ids = torch.zeros(T, dtype=torch.int32, device=dev)
         self.next_vals = torch.zeros(T, dtype=torch.float32, device=dev)
         self.logits = e(T, self.vl, dt=torch.float32) if keep_logits else None
-        self.launches_per_forward = 2 + (5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
+        self.launches_per_forward = 2 + ((6 if T <= 8 else 8) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
         self._graph = None
 
     def _row_parallel(self, a: torch.Tensor, w: torch.Tensor, x: torch.Tensor) -> None:
         """``x += a @ w.T`` summed over the ranks (one rank: the same bits without the call counter)."""
-        if self.fabric.world == 1:
+        if self.int4:
+            int4.linear(a, w, residual=x, out=x, status_ptr=self.fabric.desc.status)
+        elif self.fabric.world == 1:
             K.gemv(a, w, residual=x, out=x, rings=True)
         else:
             K.gemv_allreduce(a, w, self.fabric, residual=x, out=x)
+
+    def normed_linear(self, x: torch.Tensor, w: "int4.Int4Weight", norm_w: torch.Tensor, out: torch.Tensor, h: Optional[torch.Tensor] = None) -> None:
+        """A 4-bit linear of normalised rows: in one launch while it takes the norm, behind a norm (into ``h``) beyond."""
+        st = self.fabric.desc.status
+        if x.shape[0] <= int4.NORM_ROWS:
+            int4.linear(x, w, norm_w=norm_w, eps=self.cfg.eps, out=out, status_ptr=st)
+        else:
+            int4.linear(K.rmsnorm(x, norm_w, self.cfg.eps, out=h), w, out=out, status_ptr=st)
 
     def forward(self, T: Optional[int] = None, sample: bool = True) -> torch.Tensor:
         c, w, fab = self.cfg, self.w, self.fabric
@@ -192,7 +225,11 @@ class DenseDecoder:
         for l in range(c.layers):
             p = f"layers.{l}."
             qkv = self.qkv[:T]
-            if fab.world == 1 and T <= 8:
+            if self.int4:
+                self.normed_linear(x, w[p + "qkv"], w[p + "attn_norm"], qkv)
+                K.gqa_rope_kv_write(qkv, pos, slot, self.page_table, self.k_cache[l], self.v_cache[l], heads=self.hq, kv_heads=self.hk, head_dim=c.head_dim, theta=c.theta,
+                                    status_ptr=st)
+            elif fab.world == 1 and T <= 8:
                 K.qkv_rows(x, w[p + "qkv"], w[p + "attn_norm"], pos, slot, self.page_table, self.k_cache[l], self.v_cache[l], heads=self.hq, kv_heads=self.hk,
                            head_dim=c.head_dim, theta=c.theta, eps=c.eps, out=qkv, status_ptr=st)
             else:
@@ -204,7 +241,10 @@ class DenseDecoder:
                                    keys_per_split=self.kps, max_splits=self.max_splits, scratch=self.scratch,
                                    out=self.attn[:T], status_ptr=st)
             self._row_parallel(self.attn[:T], w[p + "o_proj"], x)
-            K.gemv(x, w[p + "gate_up"], norm_w=w[p + "ffn_norm"], eps=c.eps, swiglu=True, out=self.act[:T], rings=fab.world == 1)
+            if self.int4:
+                self.normed_linear(x, w[p + "gate_up"], w[p + "ffn_norm"], self.act[:T])
+            else:
+                K.gemv(x, w[p + "gate_up"], norm_w=w[p + "ffn_norm"], eps=c.eps, swiglu=True, out=self.act[:T], rings=fab.world == 1)
             self._row_parallel(self.act[:T], w[p + "down"], x)
         if sample:
             K.lm_head_argmax(x, w["lm_head"], fab, norm_w=w["final_norm"], eps=c.eps, vocab_offset=self.rank * self.vl,

@@ -6,7 +6,7 @@ matrix-matrix work: the four linears of a layer on the tcgen05 GEMM (gate/up
 with the SwiGLU epilogue, the row-parallel o_proj and down projections through the fused GEMM + all-reduce kernel when the
 model is tensor parallel), rotary + cache append through the decode path's kernel, attention through its split-KV kernels
 with one query row per token (causality comes from the per-row positions), ``attn_rows`` query rows per launch. Up to eight rows on
-one rank take the decoder's streaming linears instead (``_few``).
+one rank take the decoder's streaming linears instead (``_few``). 4-bit weights have forms of their own for any number of rows (``ops/int4.py``).
 It shares weights, caches and the page table with the decoder, so decode continues from the state it leaves.
 
 Sequence-parallel mode (``sequence_parallel=True``, tensor-parallel models, chunks of a multiple of ``128 * world`` rows): the
@@ -25,6 +25,7 @@ import torch
 
 from ..ops import decode as K
 from ..ops import gemm as G
+from ..ops import int4
 from ..ops import prefill as P
 from ..ops import stream_norm as N
 from .dense_gqa import BF16, DenseDecoder
@@ -128,7 +129,7 @@ class DensePrefill:
     def _few(self, m: int, w: torch.Tensor) -> bool:
         """Whether ``m`` rows go through the streaming linears (one tile of eight rows, which the weights pass once, and the norm ahead of them in the same
         launch): 2B model, 8 rows, a layer's four linears and two norms 40 us as products, 28 so."""
-        return m <= 8 and self.dec.fabric.world == 1 and w.is_contiguous()
+        return m <= 8 and self.dec.fabric.world == 1 and not isinstance(w, int4.Int4Weight) and w.is_contiguous()
 
     def _layers_graphed(self, m: int) -> torch.Tensor:
         if m > self.graph_rows_max:
@@ -173,6 +174,15 @@ class DensePrefill:
         scale = 1.0 / math.sqrt(c.head_dim)
         for l in range(c.layers):
             p = f"layers.{l}."
+            if d.int4:
+                qkv = self.qkv[:m]
+                d.normed_linear(x, w[p + "qkv"], w[p + "attn_norm"], qkv, h)
+                K.gqa_rope_kv_write(qkv, pos, sl, d.page_table, d.k_cache[l], d.v_cache[l], heads=d.hq, kv_heads=d.hk, head_dim=c.head_dim, theta=c.theta, status_ptr=st)
+                self._attention(l, m, qkv, pos, sl, scale, st)
+                int4.linear(self.attn[:m], w[p + "o_proj"], residual=x, out=x, status_ptr=st)
+                d.normed_linear(x, w[p + "gate_up"], w[p + "ffn_norm"], self.act[:m], h)
+                int4.linear(self.act[:m], w[p + "down"], residual=x, out=x, status_ptr=st)
+                continue
             if self._few(m, w[p + "qkv"]):
                 qkv = self.qkv[:m]
                 K.qkv_rows(x, w[p + "qkv"], w[p + "attn_norm"], pos, sl, d.page_table, d.k_cache[l], d.v_cache[l], heads=d.hq, kv_heads=d.hk, head_dim=c.head_dim,
@@ -205,7 +215,9 @@ class DensePrefill:
                 K.gemv(self.act[:m], w[p + "down"], residual=x, out=x, rings=True)
             else:
                 G.gemm(self.act[:m], w[p + "down"], residual=x, out=x, status_ptr=st, fixed=True)
-        self.launches = 1 + c.layers * ((4 if self._few(m, w["layers.0.qkv"]) else 7) + 2 * ((m + self.QC - 1) // self.QC))
+        # 4-bit linears beyond sixteen rows are two launches each, and their norms launches of their own beyond eight
+        per_layer = (5 if m <= 8 else 7 if m <= 16 else 11) if d.int4 else 4 if self._few(m, w["layers.0.qkv"]) else 7
+        self.launches = 1 + c.layers * (per_layer + 2 * ((m + self.QC - 1) // self.QC))
         return x
 
     # -- sequence parallel ------------------------------------------------------------------------------------------------

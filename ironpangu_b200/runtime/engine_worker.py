@@ -573,9 +573,13 @@ def build_engine(args, rank: int, world: int, rec=None) -> BatchEngine:
         dcfg = G.DenseConfig.tiny(args.layers or 2) if args.model == "dense-tiny" else G.DenseConfig.qwen2b()
         if args.model == "dense2b" and args.layers:
             dcfg.layers = args.layers
+        if args.weights_int4 and world > 1:
+            raise SystemExit("--weights-int4 runs on one rank")
         dweights = G.random_rank_weights(dcfg, rank, world, dev, seed=args.seed)
+        if args.weights_int4:
+            dweights = G.quantise_weights(dweights)
         mark("weights")
-        if args.executor == "bundle":
+        if args.executor == "bundle" and not args.weights_int4:
             # the family's .inferfabric source compiled for this job's width, run by the plan engine on the same tensors
             import tempfile
 
@@ -815,6 +819,7 @@ def main() -> None:
     ap.add_argument("--prefix-cache-slots", type=int, default=0, help="device snapshots kept by the prefix cache (0 = off)")
     ap.add_argument("--kv-int8", action="store_true", help="packed int8 latent KV cache")
     ap.add_argument("--expert-fp8", action="store_true", help="block-scaled fp8 expert weights (1 x 128 scale blocks)")
+    ap.add_argument("--weights-int4", action="store_true", help="4-bit linears with a scale and a zero point per 128 columns (dense models on one rank, run by the decoder class)")
     ap.add_argument("--prefill-chunk", type=int, default=0, help="rows per tensor-core prefill call (0 = prompts go through the decode kernels)")
     ap.add_argument("--no-graphs", action="store_true", help="launch every kernel from the host instead of replaying CUDA graphs")
     ap.add_argument("--greedy-only", action="store_true", help="skip the logits buffer; refuse sampled requests")
@@ -831,10 +836,14 @@ def main() -> None:
     ropts = RuntimeOptions.from_env(os.environ, args.set)
     args.kv_int8 = args.kv_int8 or ropts.kv_int8
     args.expert_fp8 = args.expert_fp8 or ropts.expert_fp8
+    args.weights_int4 = args.weights_int4 or ropts.weights_int4
+    if args.weights_int4 and not args.model.startswith("dense"):
+        raise SystemExit(f"--weights-int4: {args.model} has no 4-bit linears")
     args.prefill_chunk = args.prefill_chunk or ropts.prefill_chunk
     args.prefix_cache_slots = args.prefix_cache_slots or ropts.prefix_cache_slots
     args.no_graphs = args.no_graphs or not ropts.decode_graph
     ropts.kv_int8, ropts.expert_fp8, ropts.prefill_chunk = args.kv_int8, args.expert_fp8, args.prefill_chunk
+    ropts.weights_int4 = args.weights_int4
     ropts.prefix_cache_slots, ropts.decode_graph = args.prefix_cache_slots, not args.no_graphs
     ropts.validate()
     if not ropts.pdl:

@@ -22,6 +22,7 @@ class RuntimeOptions:
     fused_head: Optional[bool] = None    # cluster-per-head attention kernel: None = by context limit, True / False = forced
     kv_int8: bool = False                # packed int8 latent KV cache
     expert_fp8: bool = False             # block-scaled fp8 expert weights
+    weights_int4: bool = False           # 4-bit linears with group scales (dense models, one rank)
     prefill_chunk: int = 0               # rows per tensor-core prompt call (0 = prompts through the decode kernels)
     prefix_cache_slots: int = 0          # device snapshots kept by the prefix cache
     spin_limit: int = 4_000_000          # polls a kernel waits for a peer before it reports a timeout
