@@ -1,0 +1,150 @@
+"""Continuations of one prompt over shared pages, with bf16 and with 4-bit weights: against the same sequences run one by one, drawn again, set aside and packed."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, I32 = torch.bfloat16, torch.int32
+
+
+def _decoder(int4, *, slots=6, pool=True, rows=5, context=96, pages=None):
+    from ironpangu_b200.models import dense_gqa as G
+    from ironpangu_b200.parallel.fabric import Fabric
+
+    cfg = G.DenseConfig.tiny(2)
+    w = G.shard_weights(cfg, G.random_full_weights(cfg, 3), 0, 1, "cuda")
+    fab = Fabric(0, 1)
+    if int4:
+        w = G.quantise_weights(w, group=64)
+    return cfg, fab, G.DenseDecoder(cfg, w, fab, max_tokens=rows, max_context=context, num_slots=slots, keep_logits=True, page_pool=pool, num_pages=pages)
+
+
+def _row(dec, token, position, slot):
+    dec.tokens[:1].fill_(token)
+    dec.positions[:1].fill_(position)
+    dec.slots[:1].fill_(slot)
+    dec.forward(1)
+    return dec.logits[0].clone()
+
+
+def test_a_decoder_with_4_bit_weights_is_one_with_their_values():
+    """Logits of the 4-bit decoder against the bf16 one whose weights are the 4-bit values: decode rows, a prompt of many rows, batched rows."""
+    from ironpangu_b200.models import dense_gqa as G
+    from ironpangu_b200.models.dense_prefill import DensePrefill
+    from ironpangu_b200.parallel.fabric import Fabric
+
+    cfg, fab, four = _decoder(True, pool=False, rows=8, context=256)
+    values = {k: (v.dequantise() if hasattr(v, "dequantise") else v) for k, v in four.w.items()}
+    full = G.DenseDecoder(cfg, values, Fabric(0, 1), max_tokens=8, max_context=256, num_slots=6, keep_logits=True)
+    prompt = torch.randint(0, cfg.vocab, (150,), generator=torch.Generator().manual_seed(1), dtype=I32).cuda()
+    pre = [DensePrefill(d, max_rows=100, attn_rows=32) for d in (four, full)]
+    got = []
+    for d, p in zip((four, full), pre):
+        for at in (0, 100):
+            p.forward(prompt[at:at + 100], at, 2)
+        got.append([d.logits[0].clone(), _row(d, 7, 150, 2)])
+        rows = torch.tensor([5, 9, 11, 900] * 5, dtype=I32, device="cuda")
+        slots = torch.tensor([2, 3, 4, 5] * 5, dtype=I32, device="cuda")
+        pos = torch.cat([torch.tensor([151, 0, 0, 0]) + i for i in range(5)]).to(I32).cuda()
+        got[-1].append(p.forward_rows(rows, pos, slots, torch.arange(20, device="cuda")).clone())
+    # the same values but for rounding: weights of bf16(s (q - z)) there, a unit's gate and up rounded there
+    for a, b in zip(*got):
+        torch.testing.assert_close(a, b, rtol=2e-2, atol=2e-2)
+    assert four.fabric.status() == 0 and sum(w.nbytes for w in four.w.values() if hasattr(w, "nbytes") and hasattr(w, "units")) < 0.33 * sum(
+        values[k].numel() * 2 for k, w in four.w.items() if hasattr(w, "units"))
+
+
+@pytest.mark.parametrize("int4", [False, True])
+@pytest.mark.parametrize("length", [1, 15, 16, 37])
+def test_continuations_are_the_sequences_run_alone(int4, length):
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    cfg, fab, dec = _decoder(int4)
+    c = Continuations(dec)
+    prompt = torch.randint(0, cfg.vocab, (length,), generator=torch.Generator().manual_seed(length)).tolist()
+    got = c.generate(prompt, 4, 20, temperature=0.8, top_k=20, seed=5)
+    assert len({tuple(r) for r in got}) > 1 and all(len(r) == 20 for r in got) and int(dec.pool.refs.sum()) == 0
+    # each continuation's tokens through a slot of its own: the same sampling, logits of rows that stand alone
+    from ironpangu_b200.ops import decode as K
+
+    _, _, one = _decoder(int4, pool=False)
+    for i, row in enumerate(got):
+        for p, t in enumerate(prompt):
+            logits = _row(one, t, p, 0)
+        f = lambda v, dt=torch.float32: torch.tensor([v], dtype=dt, device="cuda")
+        counter, seed = f(0, torch.int64), f(i + 5 * 0x9E3779B1, torch.int64)
+        for k, t in enumerate(row):
+            want = K.sample_topk(logits[None].contiguous(), one.fabric, top_k=20, inv_temperature=f(1 / 0.8), top_p=f(1.0), seeds=seed, counters=counter)
+            if int(want) != t:               # two candidates whose draw lies at their border: the batch rounds a sum another way
+                probs = torch.softmax(logits / 0.8, -1)
+                assert probs[t] > 0.5 * probs.topk(20).values[-1], (i, k)
+                break
+            logits = _row(one, t, length + k, 0)
+    fab.close()
+
+
+@pytest.mark.parametrize("int4", [False, True])
+def test_drawn_again_set_aside_and_packed(int4):
+    from ironpangu_b200.models.dense_prefill import DensePrefill
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    cfg, fab, dec = _decoder(int4)
+    c = Continuations(dec, prefill=DensePrefill(dec, max_rows=64, attn_rows=32), store_pages=12)
+    prompt = torch.randint(0, cfg.vocab, (37,), generator=torch.Generator().manual_seed(0)).tolist()
+    c.start(prompt, 5, temperature=1.0, top_k=30, seed=1)
+    for _ in range(6):
+        c.step()
+
+    def caches(i):
+        n = int(dec.pool.lengths[1 + i])
+        pages = dec.pool.table[1 + i, :-(-n // 16)].long()
+        return torch.stack([t[pages].flatten(0, 1)[:n] for t in dec.k_cache + dec.v_cache])
+
+    before, tokens = [caches(i) for i in range(5)], dec.tokens[:5].clone()
+    c.resample(torch.tensor([3, 0, 0, 3, 1], dtype=I32, device="cuda"))
+    c.check()
+    for i, j in enumerate((3, 0, 0, 3, 1)):
+        assert torch.equal(caches(i), before[j]) and int(dec.tokens[i]) == int(tokens[j])
+    now = [caches(i) for i in range(5)]
+    held = c.set_aside(2)
+    assert int(dec.pool.lengths[3]) == 0
+    live = c.pack()
+    assert live == int((dec.pool.refs > 0).sum()) and bool((dec.pool.refs[:live] > 0).all())
+    for i in (0, 1, 3, 4):
+        assert torch.equal(caches(i), now[i])
+    c.take_up(2, held)
+    assert torch.equal(caches(2), now[2])
+    alike = torch.tensor([0, 3], device="cuda")       # drawn from the same parent, with different seeds from here on
+    first = c.step().clone()
+    logits = dec.logits[:5].clone()
+    assert torch.equal(logits[alike[0]], logits[alike[1]])
+    for _ in range(4):
+        c.step()
+    c.check()
+    c.end()
+    assert int(dec.pool.refs.sum()) == 0 and first.shape == (5,)
+    fab.close()
+
+
+def test_refusals():
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    _, fab, dec = _decoder(False, pool=False)
+    with pytest.raises(ValueError, match="page_pool"):
+        Continuations(dec)
+    cfg, fab, dec = _decoder(False, pages=7)
+    c = Continuations(dec)
+    for args, what in (((range(5), 6), "takes 1 to 5"), (([], 2), "prompt of 0"), ((range(97), 2), "prompt of 97")):
+        with pytest.raises(ValueError, match=what):
+            c.start(list(args[0]), args[1])
+    with pytest.raises(RuntimeError, match="start"):
+        c.step()
+    c.start(list(range(40)), 4)                       # three pages, and four copies of the last one
+    for _ in range(8):
+        c.step()
+    c.check()
+    c.step()                                          # position 48: a page more for each, and none left
+    with pytest.raises(OverflowError):
+        c.check()
+    c.end()
+    c.start(list(range(20)), 2)
+    assert c.generate(list(range(20)), 2, 3, temperature=0.0)[0] == c.generate(list(range(20)), 1, 3, temperature=0.0)[0]
