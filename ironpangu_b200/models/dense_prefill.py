@@ -38,6 +38,7 @@ class DensePrefill:
 
     def __init__(self, dec: DenseDecoder, max_rows: int = 512, attn_rows: int = 64):
         self.dec, self.M, self.QC = dec, max_rows, attn_rows
+        self.int4 = getattr(dec, "int4", False)      # (a compiled bundle's engine has bf16 weights only)
         c, fab, dev = dec.cfg, dec.fabric, dec.fabric.device
         M = max_rows
         e = lambda *s, dt=BF16: torch.empty(*s, dtype=dt, device=dev)
@@ -174,7 +175,7 @@ class DensePrefill:
         scale = 1.0 / math.sqrt(c.head_dim)
         for l in range(c.layers):
             p = f"layers.{l}."
-            if d.int4:
+            if self.int4:
                 qkv = self.qkv[:m]
                 d.normed_linear(x, w[p + "qkv"], w[p + "attn_norm"], qkv, h)
                 K.gqa_rope_kv_write(qkv, pos, sl, d.page_table, d.k_cache[l], d.v_cache[l], heads=d.hq, kv_heads=d.hk, head_dim=c.head_dim, theta=c.theta, status_ptr=st)
@@ -216,7 +217,7 @@ class DensePrefill:
             else:
                 G.gemm(self.act[:m], w[p + "down"], residual=x, out=x, status_ptr=st, fixed=True)
         # 4-bit linears beyond sixteen rows are two launches each, and their norms launches of their own beyond eight
-        per_layer = (5 if m <= 8 else 7 if m <= 16 else 11) if d.int4 else 4 if self._few(m, w["layers.0.qkv"]) else 7
+        per_layer = (5 if m <= 8 else 7 if m <= 16 else 11) if self.int4 else 4 if self._few(m, w["layers.0.qkv"]) else 7
         self.launches = 1 + c.layers * (per_layer + 2 * ((m + self.QC - 1) // self.QC))
         return x
 
