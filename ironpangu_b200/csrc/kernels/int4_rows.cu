@@ -36,6 +36,7 @@ struct RowsP {
   int groups, more, splits;      // CTAs (clusters) that share the tiles (pairs of them where gated), how many of them have one more than the others; CTAs of a cluster
   int most;                      // tiles of a CTA, at most
   int depth;                     // stages of a ring
+  int staged, x_at;              // whether the one row of x lies in shared memory, normalised, and where; otherwise operands come from L2
   int wide;                      // units of a run: 2 also where they are taken one by one (J 1), so that sums are added in the same order
   uint32_t* status;
 };
@@ -63,6 +64,9 @@ __device__ __forceinline__ float4 lds_f4(uint32_t at) {
 }
 __device__ __forceinline__ void sts_f4(uint32_t at, const float4& v) {
   asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void sts_u4(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ uint32_t lds4(uint32_t at) {
   uint32_t v;
@@ -113,7 +117,7 @@ template <int GROUP, bool ZEROS, bool F16, int MR, int J>
 __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) {
   constexpr int NT = (MR + 7) / 8, RUNS = GROUP / 32, NG = 4 / RUNS, UNIT = CODES + NG * (ZEROS ? 48 : 32);      // runs of 32 columns of a group, groups of a unit, its bytes
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float sums[WARPS * 8], inv[8];        // inv: of the rows, where there is a norm
+  __shared__ float sums[WARPS], inv[8];            // inv: of the rows, where there is a norm
   __shared__ uint64_t bars[WARPS * 16];            // of a warp's stages: full, and eight further on empty
   grid_dep_launch();
   const View& v = p.v;
@@ -165,66 +169,19 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     __syncwarp();
   } else {
     for (int i = 0; i < tiles * NT; ++i) sts_f4(acc + i * 512, make_float4(0.f, 0.f, 0.f, 0.f));
+    if (NT == 1 && p.norm_w)
+      for (int i = threadIdx.x * 64; i < v.K; i += WARPS * 32 * 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.norm_w + i));
   }
   grid_dep_wait();
 
-  if (NT == 1 && p.norm_w && warp < WARPS) {
-    // MR 8: a warp a row; otherwise all of them every row. The sum of squares in one order whatever the rows: of 256 threads' pieces, 32 threads at a time
-    constexpr int PIECES = MR == 8 ? WARPS : 1, STEP = MR == 8 ? 32 : 256;
-    const int start = MR == 8 ? lane : threadIdx.x;
+  const int pieces = v.K / 8, ch0 = chunk0 + warp * p.wide;
+  const bf16* xr[NT];                              // this lane's row of x, its first column
+  uint4 b[J][NT][4];                               // this lane's operands: four runs of eight columns of a row of x
 #pragma unroll
-    for (int r = 0; r < (MR == 8 ? 1 : MR); ++r) {
-      const int t = MR == 8 ? warp : r;
-      float ss[PIECES] = {};
-      if (t < p.T) {
-        const bf16* xr = p.x + t * p.ldx;
-        for (int i = start; i < v.K / 8; i += STEP * PIECES) {
-          uint4 u[PIECES];
-#pragma unroll
-          for (int q = 0; q < PIECES; ++q) u[q] = i + q * STEP < v.K / 8 ? *reinterpret_cast<const uint4*>(xr + (i + q * STEP) * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int q = 0; q < PIECES; ++q) {
-            float f[8];
-            unpack8(u[q], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss[q] += f[e] * f[e];
-          }
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < PIECES; ++q) ss[q] = warp_sum(ss[q]);
-      if (lane == 0) {
-        if (MR == 8) {
-#pragma unroll
-          for (int q = 1; q < PIECES; ++q) ss[0] += ss[q];
-          sums[t] = ss[0];
-        } else {
-          sums[warp * 8 + t] = ss[0];
-        }
-      }
-    }
-    consumers();
-    if (threadIdx.x < MR) {
-      const int t = threadIdx.x;
-      float s = sums[t];
-      if (MR != 8)
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) s += sums[w * 8 + t];
-      inv[t] = rsqrtf(s / (float)v.K + p.eps);
-    }
-    consumers();
-  }
-
-  bool late = false;
-  if (warp < WARPS) {
-    const bf16* xr[NT];                            // this lane's row of x, its first column
-#pragma unroll
-    for (int n = 0; n < NT; ++n) xr[n] = p.x + (long)min(n * 8 + g, p.T - 1) * p.ldx + c * 8;
-    const uint32_t ring = rings + warp * p.depth * J * UNIT + code_at(g, c), meta = CODES + g * 4 - code_at(g, c), end = ring + p.depth * J * UNIT;
-    uint32_t at = ring, stage = bar, parity = 0;   // the stage at hand: this lane's first codes, and its barrier
-#pragma unroll 1
-    for (int ch = chunk0 + warp * p.wide; ch < chunk1; ch = after(ch)) {
-      uint4 b[J][NT][4];                           // this lane's operands: four runs of eight columns of a row of x
+  for (int n = 0; n < NT; ++n) xr[n] = p.x + (long)min(n * 8 + g, p.T - 1) * p.ldx + c * 8;
+  const uint32_t xs = smem_addr(smem) + p.x_at;    // the row, where it lies in shared memory
+  auto load = [&](int ch) {
+    auto each = [&](auto from) {
 #pragma unroll
       for (int u = 0; u < J; ++u)
 #pragma unroll
@@ -232,9 +189,83 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = (ch + u) * CHUNK + i * 32;
-            b[u][n][i] = (MR == 1 ? g == 0 : n * 8 + g < p.T) && k + c * 8 < v.K ? ld_now16(xr[n] + k) : make_uint4(0, 0, 0, 0);
+            b[u][n][i] = (MR == 1 ? g == 0 : n * 8 + g < p.T) && k + c * 8 < v.K ? from(n, k) : make_uint4(0, 0, 0, 0);
           }
-      if (NT == 1 && p.norm_w) {
+    };
+    if (MR == 1 && p.staged) each([&](int, int k) { return lds16(xs + (k + c * 8) * 2); });
+    else each([&](int n, int k) { return ld_now16(xr[n] + k); });
+  };
+  if (MR == 1 && p.staged && warp < WARPS) {
+    // One row: loaded in pieces of 256 threads, normalised, and kept for all warps
+    constexpr int HELD = 4;
+    uint4 x[HELD];
+    float ss = 0.f;
+    for (int i0 = threadIdx.x; i0 < pieces; i0 += 256 * HELD) {
+#pragma unroll
+      for (int q = 0; q < HELD; ++q) x[q] = i0 + q * 256 < pieces ? ld_now16(p.x + (i0 + q * 256) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int q = 0; q < HELD; ++q) {
+        if (i0 + q * 256 < pieces) sts_u4(xs + (i0 + q * 256) * 16, x[q]);
+        float f[8];
+        unpack8(x[q], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+      }
+    }
+    ss = warp_sum(ss);
+    if (lane == 0) sums[warp] = ss;
+    consumers();
+    float s = sums[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) s += sums[w];
+    const float by = rsqrtf(s / (float)v.K + p.eps);
+    for (int i = threadIdx.x; i < pieces; i += 256) {
+      float f[8], w[8];
+      unpack8(lds16(xs + i * 16), f);
+      unpack8(*reinterpret_cast<const uint4*>(p.norm_w + i * 8), w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = f[e] * by * w[e];
+      sts_u4(xs + i * 16, pack8(f));
+    }
+    consumers();
+  }
+  if (warp < WARPS && ch0 < chunk1) load(ch0);
+  const bool normed_later = NT == 1 && p.norm_w && !(MR == 1 && p.staged);
+  if (normed_later && warp < WARPS) {
+    // A warp a row. The sum of squares in one order whatever the rows: of 256 threads' pieces, 32 threads at a time
+    const int t = warp;
+    float ss[WARPS] = {};
+    if (t < p.T) {
+      const bf16* row = p.x + t * p.ldx;
+      for (int i = lane; i < pieces; i += 256) {
+        uint4 u[WARPS];
+#pragma unroll
+        for (int q = 0; q < WARPS; ++q) u[q] = i + q * 32 < pieces ? *reinterpret_cast<const uint4*>(row + (i + q * 32) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < WARPS; ++q) {
+          float f[8];
+          unpack8(u[q], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss[q] += f[e] * f[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < WARPS; ++q) ss[q] = warp_sum(ss[q]);
+#pragma unroll
+    for (int q = 1; q < WARPS; ++q) ss[0] += ss[q];
+    if (lane == 0) inv[t] = rsqrtf(ss[0] / (float)v.K + p.eps);
+    consumers();
+  }
+
+  bool late = false;
+  if (warp < WARPS) {
+    const uint32_t ring = rings + warp * p.depth * J * UNIT + code_at(g, c), meta = CODES + g * 4 - code_at(g, c), end = ring + p.depth * J * UNIT;
+    uint32_t at = ring, stage = bar, parity = 0;   // the stage at hand: this lane's first codes, and its barrier
+#pragma unroll 1
+    for (int ch = ch0; ch < chunk1; ch = after(ch)) {
+      if (ch != ch0) load(ch);
+      if (normed_later) {
         const float by = inv[MR == 1 ? 0 : g];
 #pragma unroll
         for (int u = 0; u < J; ++u)
@@ -389,14 +420,16 @@ int launch(RowsP p, cudaStream_t s) {
   static std::atomic<uint64_t> done;
   const Device dev = device_now();
   const int sms = dev.sms, halves = p.v.halves;
+  p.staged = MR == 1 && p.norm_w && p.v.K * 2 <= 32768;
+  const int x_bytes = p.staged ? (p.v.K * 2 + 127) / 128 * 128 : 0, room = SMEM - 512 - x_bytes;
   // as many CTAs as run at once, unless their tiles' sums are too many for them; those with one tile more come first, so that an SM has some of either kind
-  const int room = (SMEM - 512 - WARPS * 3 * J * unit) / tile / halves;
-  p.groups = std::max(std::min(p.v.tiles, at_once(p.splits, sms)), ceil_div(p.v.tiles, room));
+  p.groups = std::max(std::min(p.v.tiles, at_once(p.splits, sms)), ceil_div(p.v.tiles, (room - WARPS * 3 * J * unit) / tile / halves));
   p.more = p.v.tiles % p.groups;
   p.most = (p.v.tiles / p.groups + (p.more > 0)) * halves;
   const int runs = ceil_div(ceil_div(p.v.chunks, p.splits), WARPS * p.wide) * (p.wide / J) * p.most;           // of a warp
-  p.depth = std::max(1, std::min({runs, (SMEM - 512 - p.most * WARPS * NT * 512) / (WARPS * J * unit), 8}));
-  const int smem = p.most * WARPS * NT * 512 + std::max(WARPS * p.depth * J * unit, p.most * TILE * 8 * NT * 4);
+  p.depth = std::max(1, std::min({runs, (room - p.most * WARPS * NT * 512) / (WARPS * J * unit), 8}));
+  p.x_at = p.most * WARPS * NT * 512 + std::max(WARPS * p.depth * J * unit, p.most * TILE * 8 * NT * 4);
+  const int smem = p.x_at + x_bytes;
   if (int rc = allow_smem(k, SMEM, dev.id, done)) return rc;
   const dim3 grid(p.groups * p.splits);
   if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(WARPS * 32 + 32), (unsigned)p.splits, (size_t)smem, s, p);
