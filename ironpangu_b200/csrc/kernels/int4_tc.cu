@@ -11,8 +11,10 @@
 //   warp 1      MMAs
 //   warp 10     copies of codes, the first of them ahead of the wait for the preceding kernel
 //   warps 2-9   weights into tensor memory; then 2-5 read the accumulator
-// Two CTAs an SM (128 columns of sums and four stages of 32 columns of weights each), so that one multiplies while the other starts or stores. With few tiles the
-// chunks along K are shared by the CTAs of a cluster: each leaves its part of the sum in its shared memory as f32 and every CTA adds up a share of the tokens over
+// Up to 128 tokens: two CTAs an SM (128 columns of sums and four stages of 32 columns of weights each), so that one multiplies while the other starts or stores. More: tiles of
+// up to 256 tokens, a CTA an SM, so that the weights become operands once; that is what bounds the kernel there (203 rows of 6144 by 4096: 26 - 28 us, in tiles of 112 tokens 30).
+// With few tiles the chunks along K are shared by the CTAs of a cluster, of any size up to eight (17 rows of 4096 by 4096 10.5 us, of 6144 by 4096 15; in powers of two 12.8 and
+// 19.5, when all clusters did not run at once): each leaves its part of the sum in its shared memory as f32 and every CTA adds up a share of the tokens over
 // distributed shared memory, in the order of the parts.
 // Every wait is bounded. One that runs out raises the CTA's flag and the status word; the warps that read the accumulator then wait for what the CTA has started and
 // leave NaN as their part of the sum.
@@ -32,13 +34,11 @@ int pair_product(const View& v, const void* rows, const float* factor, const bf1
 
 namespace {
 
-constexpr int FT = 128, BK = 64, TOK = 128, STAGES = 4, CHUNKS = 4, THREADS = 352;
-constexpr int STAGE = TOK * BK * 2;
-template <int GROUP, bool ZEROS>
-constexpr int SMEM = STAGES * STAGE + CHUNKS * Units<GROUP, ZEROS>::BYTES + 1024 + 512;
-constexpr uint32_t COLS = 256, A_COL = 128;          // of tensor memory; first column of the weights' stages
+constexpr int FT = 128, BK = 64, TOK = 128, STAGES = 4, CHUNKS = 4, THREADS = 352;       // TOK: tokens of a tile, twice as many where it is wide
+template <int GROUP, bool ZEROS, bool WIDE>
+constexpr int SMEM = STAGES * (WIDE ? 2 : 1) * TOK * BK * 2 + CHUNKS * Units<GROUP, ZEROS>::BYTES + 1024 + 512;
 constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
-static_assert(TOK * FT * 4 <= STAGES * STAGE, "the part of the sum takes the ring's place");
+static_assert(TOK * FT * 4 <= STAGES * TOK * BK * 2, "the part of the sum takes the ring's place");
 
 struct TcP {
   View v;
@@ -115,9 +115,11 @@ __global__ void __launch_bounds__(256) rows_kernel(const bf16* x, long ldx, __ha
 }
 
 // grid (feature tiles x splits, token tiles), clusters of `splits` along x
-template <int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, TcP p) {
+template <int GROUP, bool ZEROS, bool WIDE>
+__global__ void __launch_bounds__(THREADS, WIDE ? 1 : 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, TcP p) {
   using U = Units<GROUP, ZEROS>;
+  constexpr int MOST = WIDE ? 2 * TOK : TOK, STAGE = MOST * BK * 2;
+  constexpr uint32_t COLS = 2 * MOST, A_COL = MOST;    // of tensor memory; first column of the weights' stages
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* ring = smem + STAGES * STAGE;         // chunks of units
@@ -125,7 +127,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
   uint64_t *weights = full + STAGES, *empty = weights + STAGES, *acc_full = empty + STAGES, *units_full = acc_full + 1, *units_empty = units_full + CHUNKS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units_empty + CHUNKS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ float factors[TOK];
+  __shared__ float factors[MOST];
   volatile int* requested = abort_flag + 1;      // blocks whose copies were requested, once no more will be; until then -1
   const View& v = p.v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
   tc_fence_after();
   grid_dep_launch();
   const uint32_t tmem_base = *tmem_slot;
-  if (threadIdx.x < TOK && m0 + threadIdx.x < p.T) factors[threadIdx.x] = p.factor[m0 + threadIdx.x];
+  if (threadIdx.x < MOST && m0 + threadIdx.x < p.T) factors[threadIdx.x] = p.factor[m0 + threadIdx.x];
 
   if (warp == 0 && lane == 0) {
     int issued = 0;
@@ -192,23 +194,33 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
     }
     *requested = issued;
     if (*abort_flag && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {                                // the whole warp walks and one lane issues, as among pairs
+    uint32_t elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
     const uint32_t idesc = umma_idesc_f16(FT, p.tok);
-    for (int kb = 0; kb < nk; ++kb) {
-      const int s = kb % STAGES;
-      if (!mbar_wait(&full[s], (kb / STAGES) & 1, p.spin_limit) || !mbar_wait(&weights[s], (kb / STAGES) & 1, p.spin_limit) || *abort_flag) {
-        *abort_flag = 1;
-        if (p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
-        break;
-      }
+    const uint64_t first = umma_desc_sw128(smem_u32(smem));
+    int s = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int kb = 0; kb < nk && ok; ++kb) {
+      ok = mbar_wait(&full[s], parity, p.spin_limit) && mbar_wait(&weights[s], parity, p.spin_limit);
+      ok = !__any_sync(0xffffffffu, !ok || *abort_flag);
       tc_fence_after();
-      const uint64_t db = umma_desc_sw128(smem_u32(smem + s * STAGE));
-      const uint32_t a = tmem_base + A_COL + s * 32;
+      if (ok && elected) {
+        const uint64_t db = first + (uint64_t)(s * (STAGE >> 4));
+        const uint32_t a = tmem_base + A_COL + s * 32;
 #pragma unroll
-      for (int k = 0; k < BK / 16; ++k) umma_f16_ta(tmem_base, a + 8 * k, db + (uint64_t)(2 * k), idesc, kb > 0 || k > 0);
-      umma_commit(&empty[s]);
+        for (int k = 0; k < BK / 16; ++k) umma_f16_ta(tmem_base, a + 8 * k, db + (uint64_t)(2 * k), idesc, kb > 0 || k > 0);
+        umma_commit(&empty[s]);
+      }
+      if (++s == STAGES) s = 0, parity ^= 1;
     }
-    umma_commit(acc_full);
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+    }
+    if (elected) umma_commit(acc_full);
   } else if (warp == 10) {
     while (chunk < nc) {
       if (!mbar_wait(&units_empty[chunk % CHUNKS], (chunk / CHUNKS - 1) & 1, p.spin_limit)) *abort_flag = 1;
@@ -333,14 +345,56 @@ __global__ void __launch_bounds__(THREADS, 2) int4_tc_kernel(const __grid_consta
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-template <int GROUP, bool ZEROS>
+template <int GROUP, bool ZEROS, bool WIDE>
 int launch(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
-  auto k = int4_tc_kernel<GROUP, ZEROS>;
-  constexpr int smem = SMEM<GROUP, ZEROS>;
+  auto k = int4_tc_kernel<GROUP, ZEROS, WIDE>;
+  constexpr int smem = SMEM<GROUP, ZEROS, WIDE>;
   static std::atomic<uint64_t> done;
   if (int rc = allow_smem(k, smem, device_now().id, done)) return rc;
   if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(THREADS), (unsigned)p.splits, (size_t)smem, s, tx, p);
   return launch_chain(k, grid, dim3(THREADS), (size_t)smem, s, tx, p);
+}
+// Clusters of n CTAs that run at once: an SM's neighbours are not all free to join, and of 296 CTAs (two an SM) 279 run in threes, 259 in sevens; of 148, 135 and 105
+template <bool WIDE>
+int at_once(int n, const Device& dev) {
+  static std::atomic<int> known[64][9];
+  std::atomic<int>* have = dev.id < 64 ? &known[dev.id][n] : nullptr;
+  if (have && have->load()) return have->load();
+  auto k = int4_tc_kernel<128, false, WIDE>;
+  static std::atomic<uint64_t> done;
+  constexpr int smem = SMEM<128, false, WIDE>;
+  int count = 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(n * dev.sms), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = n, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  if (allow_smem(k, smem, dev.id, done) || cudaOccupancyMaxActiveClusters(&count, k, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (have) have->store(count);
+  return count;
+}
+// CTAs along K: those that run at once, by the chunks that the busiest SM goes through and what a wave costs besides, counted as FIXED chunks
+template <bool WIDE>
+int splits_of(int tiles, int chunks, const Device& dev) {
+  constexpr int FIXED = 6;       // 2 and 12 chose the same or as good ones over 25 sizes
+  int best = 1;
+  long least = 0;
+  for (int n = 1; n <= 8 && (n == 1 || chunks >= 2 * n); ++n) {
+    const int room = at_once<WIDE>(n, dev);
+    if (!room) continue;
+    const long waves = ceil_div(tiles, room), share = WIDE ? 1 : std::min(2, ceil_div(std::min(tiles, room) * n, dev.sms));
+    const long cost = waves * (share * ceil_div(chunks, n) + FIXED);
+    if (!least || cost < least) least = cost, best = n;
+  }
+  return best;
+}
+template <int GROUP, bool ZEROS>
+int launch_wide(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) {
+  return p.tok > TOK ? launch<GROUP, ZEROS, true>(tx, p, grid, s) : launch<GROUP, ZEROS, false>(tx, p, grid, s);
 }
 
 }  // namespace
@@ -369,19 +423,19 @@ extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const 
   float* factor = (float*)((char*)scratch + (uint64_t)T * p.v.K * 2);
   p.y = y, p.ldy = ldy, p.out_f32 = out_f32, p.residual = (const bf16*)residual, p.ldr = ldr, p.factor = factor, p.T = T, p.status = status;
   p.spin_limit = spin_limit;
-  const int halves = p.v.halves, sms = device_now().sms;
+  const Device dev = device_now();
+  const int halves = p.v.halves, sms = dev.sms;
   cudaStream_t s = (cudaStream_t)stream;
   if (int rc = launch_chain(rows_kernel, dim3(T), dim3(256), 0, s, (const bf16*)x, ldx, rows, (long)p.v.K, factor, p.v.K)) return rc;
   if (const int tok = pair_tokens(T, p.v.N * halves, sms / 2))
     return pair_product(p.v, rows, factor, p.residual, ldr, y, ldy, out_f32, T, tok, std::min(sms / 2, ceil_div(p.v.N * halves, 2 * FT) * ceil_div(T, tok)), spin_limit, status, s);
-  const int ty = ceil_div(T, TOK), tiles = ceil_div(p.v.N, halves == 2 ? FT / 2 : FT);
+  const int wide = T > TOK, ty = ceil_div(T, wide ? 2 * TOK : TOK), tiles = ceil_div(p.v.N, halves == 2 ? FT / 2 : FT);
   if (ty > 65535) return -1;
-  p.tok = ceil_div(ceil_div(T, ty), 16) * 16;
-  p.splits = 1;
-  while (p.splits < 8 && 2 * p.splits * tiles * ty <= 2 * sms && p.v.chunks >= 4 * p.splits) p.splits *= 2;
+  p.tok = std::max(ceil_div(ceil_div(T, ty), 16) * 16, wide ? TOK + 16 : 16);
+  p.splits = wide ? splits_of<true>(tiles * ty, p.v.chunks, dev) : splits_of<false>(tiles * ty, p.v.chunks, dev);
   CUtensorMap tx;          // of 16-bit elements: the type is the products' to know
   if (int rc = make_tmap_bf16_2d(&tx, rows, (uint64_t)T, (uint64_t)p.v.K, (uint64_t)p.v.K, (uint32_t)p.tok)) return rc;
   const dim3 grid(tiles * p.splits, ty);
-  if (p.v.zeros) return p.v.group == 128 ? launch<128, true>(tx, p, grid, s) : p.v.group == 64 ? launch<64, true>(tx, p, grid, s) : launch<32, true>(tx, p, grid, s);
-  return p.v.group == 128 ? launch<128, false>(tx, p, grid, s) : p.v.group == 64 ? launch<64, false>(tx, p, grid, s) : launch<32, false>(tx, p, grid, s);
+  if (p.v.zeros) return p.v.group == 128 ? launch_wide<128, true>(tx, p, grid, s) : p.v.group == 64 ? launch_wide<64, true>(tx, p, grid, s) : launch_wide<32, true>(tx, p, grid, s);
+  return p.v.group == 128 ? launch_wide<128, false>(tx, p, grid, s) : p.v.group == 64 ? launch_wide<64, false>(tx, p, grid, s) : launch_wide<32, false>(tx, p, grid, s);
 }
