@@ -6,7 +6,8 @@
 // (with the opposite sign). The sums of x come out of products with ones, once for all tiles of a CTA. The group's scale multiplies its f32 sum. Products are exact; sums run
 // up to 24 |x| instead of 8 |x| a weight, which costs them two bits of f32.
 // A CTA has a share of the tiles of sixteen rows, and its eight warps share K: a warp takes every eighth run of one or two units, for all tiles of the CTA, so that its operands
-// of x - from L2 into registers, normalised on the way - are loaded once. Units come by bulk copies into a ring of the warp's own, the first ones ahead
+// of x are loaded once. Under a norm they take its gains on the way (the one rounding to bf16 that a normalised row has), and the row's factor, from the squares that
+// the warps saw, multiplies the sums: nothing waits for a whole row (2 x 16384 by 4096, 8 rows: 24.0 -> 21.1 us, 1 row 17.5 -> 17.0). Units come by bulk copies into a ring of the warp's own, the first ones ahead
 // of the wait for the preceding kernel. (Loads ahead into registers waited for one another, whatever their number: 3.4 TB/s without any products.) Sums of the tiles lie in
 // shared memory, a float4 a lane. What a unit costs is its instructions (two cycles of a scheduler for one on integers, eight for a product), so a ninth warp computes the
 // copies' addresses and requests them, and a stage costs the others a look at its barrier and an arrival. The warps' sums are added in one order, and so a row's bits do not depend on the rows beside it.
@@ -36,7 +37,6 @@ struct RowsP {
   int groups, more, splits;      // CTAs (clusters) that share the tiles (pairs of them where gated), how many of them have one more than the others; CTAs of a cluster
   int most;                      // tiles of a CTA, at most
   int depth;                     // stages of a ring
-  int staged, x_at;              // whether the one row of x lies in shared memory, normalised, and where; otherwise operands come from L2
   int wide;                      // units of a run: 2 also where they are taken one by one (J 1), so that sums are added in the same order
   uint32_t* status;
 };
@@ -90,8 +90,6 @@ __device__ __forceinline__ void mma_from(float (&d)[4], const float (&c)[4], uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// the warps that multiply (the ninth one is at its copies)
-__device__ __forceinline__ void consumers() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
 __device__ __forceinline__ bool ready(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -112,12 +110,13 @@ __device__ __noinline__ bool wait_more(uint32_t bar, uint32_t parity) {
 }
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) { return ready(bar, parity) || wait_more(bar, parity); }
 
-// MR: most rows of x; J: units of a run
-template <int GROUP, bool ZEROS, bool F16, int MR, int J>
+// MR: most rows of x; J: units of a run; NORM: under a norm (asked for in the kernel, it cost the others 4 %: 8 rows of 8192 by 8192 13.2 -> 13.7 us)
+template <int GROUP, bool ZEROS, bool F16, int MR, int J, bool NORM>
 __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) {
   constexpr int NT = (MR + 7) / 8, RUNS = GROUP / 32, NG = 4 / RUNS, UNIT = CODES + NG * (ZEROS ? 48 : 32);      // runs of 32 columns of a group, groups of a unit, its bytes
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float sums[WARPS], inv[8];            // inv: of the rows, where there is a norm
+  __shared__ float sums[WARPS][8], squares[8];     // of the rows' squares, where there is a norm: a warp's and the CTA's share
+  __shared__ __align__(16) unsigned char runs_of_x[MR == 1 ? WARPS * 512 : 16];
   __shared__ uint64_t bars[WARPS * 16];            // of a warp's stages: full, and eight further on empty
   grid_dep_launch();
   const View& v = p.v;
@@ -169,118 +168,93 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     __syncwarp();
   } else {
     for (int i = 0; i < tiles * NT; ++i) sts_f4(acc + i * 512, make_float4(0.f, 0.f, 0.f, 0.f));
-    if (NT == 1 && p.norm_w)
+    if (NORM)
       for (int i = threadIdx.x * 64; i < v.K; i += WARPS * 32 * 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.norm_w + i));
   }
   grid_dep_wait();
-
-  const int pieces = v.K / 8, ch0 = chunk0 + warp * p.wide;
-  const bf16* xr[NT];                              // this lane's row of x, its first column
-  uint4 b[J][NT][4];                               // this lane's operands: four runs of eight columns of a row of x
-#pragma unroll
-  for (int n = 0; n < NT; ++n) xr[n] = p.x + (long)min(n * 8 + g, p.T - 1) * p.ldx + c * 8;
-  const uint32_t xs = smem_addr(smem) + p.x_at;    // the row, where it lies in shared memory
-  auto load = [&](int ch) {
-    auto each = [&](auto from) {
-#pragma unroll
-      for (int u = 0; u < J; ++u)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = (ch + u) * CHUNK + i * 32;
-            b[u][n][i] = (MR == 1 ? g == 0 : n * 8 + g < p.T) && k + c * 8 < v.K ? from(n, k) : make_uint4(0, 0, 0, 0);
-          }
-    };
-    if (MR == 1 && p.staged) each([&](int, int k) { return lds16(xs + (k + c * 8) * 2); });
-    else each([&](int n, int k) { return ld_now16(xr[n] + k); });
-  };
-  if (MR == 1 && p.staged && warp < WARPS) {
-    // One row: loaded in pieces of 256 threads, normalised, and kept for all warps
-    constexpr int HELD = 4;
-    uint4 x[HELD];
-    float ss = 0.f;
-    for (int i0 = threadIdx.x; i0 < pieces; i0 += 256 * HELD) {
-#pragma unroll
-      for (int q = 0; q < HELD; ++q) x[q] = i0 + q * 256 < pieces ? ld_now16(p.x + (i0 + q * 256) * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int q = 0; q < HELD; ++q) {
-        if (i0 + q * 256 < pieces) sts_u4(xs + (i0 + q * 256) * 16, x[q]);
-        float f[8];
-        unpack8(x[q], f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
-      }
-    }
-    ss = warp_sum(ss);
-    if (lane == 0) sums[warp] = ss;
-    consumers();
-    float s = sums[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) s += sums[w];
-    const float by = rsqrtf(s / (float)v.K + p.eps);
-    for (int i = threadIdx.x; i < pieces; i += 256) {
-      float f[8], w[8];
-      unpack8(lds16(xs + i * 16), f);
-      unpack8(*reinterpret_cast<const uint4*>(p.norm_w + i * 8), w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = f[e] * by * w[e];
-      sts_u4(xs + i * 16, pack8(f));
-    }
-    consumers();
-  }
-  if (warp < WARPS && ch0 < chunk1) load(ch0);
-  const bool normed_later = NT == 1 && p.norm_w && !(MR == 1 && p.staged);
-  if (normed_later && warp < WARPS) {
-    // A warp a row. The sum of squares in one order whatever the rows: of 256 threads' pieces, 32 threads at a time
-    const int t = warp;
-    float ss[WARPS] = {};
-    if (t < p.T) {
-      const bf16* row = p.x + t * p.ldx;
-      for (int i = lane; i < pieces; i += 256) {
-        uint4 u[WARPS];
-#pragma unroll
-        for (int q = 0; q < WARPS; ++q) u[q] = i + q * 32 < pieces ? *reinterpret_cast<const uint4*>(row + (i + q * 32) * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int q = 0; q < WARPS; ++q) {
-          float f[8];
-          unpack8(u[q], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ss[q] += f[e] * f[e];
-        }
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < WARPS; ++q) ss[q] = warp_sum(ss[q]);
-#pragma unroll
-    for (int q = 1; q < WARPS; ++q) ss[0] += ss[q];
-    if (lane == 0) inv[t] = rsqrtf(ss[0] / (float)v.K + p.eps);
-    consumers();
-  }
 
   bool late = false;
   if (warp < WARPS) {
     const uint32_t ring = rings + warp * p.depth * J * UNIT + code_at(g, c), meta = CODES + g * 4 - code_at(g, c), end = ring + p.depth * J * UNIT;
     uint32_t at = ring, stage = bar, parity = 0;   // the stage at hand: this lane's first codes, and its barrier
+    const int ch0 = chunk0 + warp * p.wide, k1 = min(v.K, chunk1 * CHUNK);      // the first run, the end of the CTA's columns
+    uint4 b[J][NT][4];                             // operands: four runs of eight columns of a row of x a unit
+    float square = 0.f;                            // of this lane's columns of its row
+    // eight columns under the norm's gains; returns the sum of their squares. The row's factor comes last, into the sums: a warp sees the whole row only then
+    auto gained = [&](uint4& x, const uint4& gain) {
+      float f[8], w[8], ss = 0.f;
+      unpack8(x, f);
+      unpack8(gain, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += f[e] * f[e], f[e] *= w[e];
+      x = pack8(f);
+      return ss;
+    };
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    // One row: a lane has eight columns of a run, one run ahead, and the warp reads them from shared memory
+    const uint32_t xs = smem_addr(runs_of_x) + warp * 512;
+    uint4 ahead = none, gain = none;
+    auto fetch = [&](int ch) {
+      const int k = ch * CHUNK + lane * 8;
+      const bool in = ch < chunk1 && lane < 16 * J && k < k1;
+      ahead = in ? ld_now16(p.x + k) : none;
+      if (NORM) gain = in ? *reinterpret_cast<const uint4*>(p.norm_w + k) : none;
+    };
+    if (MR == 1) fetch(ch0);
+    const bf16* xr[NT];                            // more: this lane's row (for rows behind the last one that one, whose results nothing stores), its first column
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xr[n] = p.x + (long)min(n * 8 + g, p.T - 1) * p.ldx + c * 8;
 #pragma unroll 1
     for (int ch = ch0; ch < chunk1; ch = after(ch)) {
-      if (ch != ch0) load(ch);
-      if (normed_later) {
-        const float by = inv[MR == 1 ? 0 : g];
+      if (MR == 1) {
+        uint4 x = ahead;
+        if (NORM) {
+          float ss = gained(x, gain);
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2)
+            if (d < 16 || J == 2) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+          square += ss;
+        }
+        sts_u4(xs + lane * 16, x);
+        fetch(after(ch));
+        __syncwarp();
 #pragma unroll
         for (int u = 0; u < J; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = (ch + u) * CHUNK + i * 32 + c * 8;
-            if (k < v.K) {
-              float f[8], w[8];
-              unpack8(b[u][0][i], f);
-              unpack8(*reinterpret_cast<const uint4*>(p.norm_w + k), w);
+          for (int i = 0; i < 4; ++i) b[u][0][i] = lds16(xs + (u * 16 + i * 4 + c) * 16);
+        __syncwarp();
+      } else {
+        const int k0 = ch * CHUNK;
+        if (NT == 1 && !NORM && k0 + J * CHUNK <= k1) {         // without the look at every column's place; with gains, or with two tiles of rows, the code's length costs more
+                                                               // (8 rows of 4096 by 16384 14.4 -> 13.7 us; 2 x 16384 by 4096 under a norm 20.9 -> 21.4)
 #pragma unroll
-              for (int e = 0; e < 8; ++e) f[e] = f[e] * by * w[e];
-              b[u][0][i] = pack8(f);
+          for (int u = 0; u < J; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) b[u][n][i] = ld_now16(xr[n] + k0 + u * CHUNK + i * 32);
+        } else {
+#pragma unroll
+          for (int u = 0; u < J; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) b[u][n][i] = k0 + u * CHUNK + i * 32 + c * 8 < k1 ? ld_now16(xr[n] + k0 + u * CHUNK + i * 32) : none;
+        }
+        if (NORM) {
+          float ss[J];
+#pragma unroll
+          for (int u = 0; u < J; ++u) {
+            float of[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = k0 + u * CHUNK + i * 32 + c * 8;
+              of[i] = gained(b[u][0][i], k < k1 ? *reinterpret_cast<const uint4*>(p.norm_w + k) : none);
             }
+            ss[u] = (of[0] + of[1]) + (of[2] + of[3]);
           }
+          square += J == 2 ? ss[0] + ss[J - 1] : ss[0];
+        }
       }
       float sum[J][NT][NG][4];                     // of the groups' columns of x, rows 2 c and 2 c + 1, twice: times -24 without zero points
 #pragma unroll
@@ -358,6 +332,11 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
         if (at == end) at = ring, stage = bar, parity ^= 1;
       }
     }
+    if (NORM) {
+      square += __shfl_xor_sync(0xffffffffu, square, 1);
+      square += __shfl_xor_sync(0xffffffffu, square, 2);
+      if (c == 0) sums[warp][g] = square;
+    }
   }
   if (__any_sync(0xffffffffu, late)) {             // a copy that did not land: nothing of the tiles is right
     if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
@@ -375,6 +354,10 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     const float* f = red + ((tile * NT + (t >> 3)) * 32 + (r & 7) * 4 + ((t & 7) >> 1)) * 4 + (r >> 3) * 2 + (t & 1);
     part[i] = ((f[0] + f[step]) + (f[2 * step] + f[3 * step])) + ((f[4 * step] + f[5 * step]) + (f[6 * step] + f[7 * step]));
   }
+  if (NORM && threadIdx.x < 8) {
+    const int t = MR == 1 ? 0 : threadIdx.x;
+    squares[threadIdx.x] = ((sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t])) + ((sums[4][t] + sums[5][t]) + (sums[6][t] + sums[7][t]));
+  }
   if (p.splits > 1) cluster_barrier();
   else __syncthreads();
   const int rows = mine * TILE;                    // of the result
@@ -387,6 +370,12 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     for (int s = 0; s < p.splits; ++s) {
       a += p.splits > 1 ? ld_part(part_at + at * 4, s) : part[at];
       if (gated) u += p.splits > 1 ? ld_part(part_at + up_at * 4, s) : part[up_at];
+    }
+    if (NORM) {
+      float ss = 0.f;
+      for (int s = 0; s < p.splits; ++s) ss += p.splits > 1 ? ld_part(smem_addr(squares + t), s) : squares[t];
+      const float by = rsqrtf(ss / (float)v.K + p.eps);
+      a *= by, u *= by;
     }
     if (gated) a = a / (1.f + __expf(-a)) * u;
     if (p.residual) a += __bfloat162float(p.residual[t * p.ldr + n]);
@@ -411,25 +400,22 @@ int splits_of(const View& v, int sms) {
 }
 // Clusters of s CTAs that run at once, two CTAs an SM: not all SMs of a part of the chip can be divided by four or eight (of 296 CTAs, 284 and 264)
 int at_once(int s, int sms) { return s <= 2 ? 2 * sms / s : s == 4 ? 2 * sms * 15 / 64 : 2 * sms * 6 / 56; }
-constexpr int SMEM = 110 * 1024;                   // of a CTA, two of which share an SM
+constexpr int SMEM = 107 * 1024;                   // of a CTA, two of which share an SM (beside 5 KB that the kernel declares, and 1 KB each)
 
-template <int GROUP, bool ZEROS, bool F16, int MR, int J>
+template <int GROUP, bool ZEROS, bool F16, int MR, int J, bool NORM>
 int launch(RowsP p, cudaStream_t s) {
   constexpr int NT = (MR + 7) / 8, unit = CODES + CHUNK / GROUP * (ZEROS ? 48 : 32), tile = WARPS * NT * 512 + TILE * 8 * NT * 4;      // bytes of a tile's sums and their sum
-  auto k = int4_rows_kernel<GROUP, ZEROS, F16, MR, J>;
+  auto k = int4_rows_kernel<GROUP, ZEROS, F16, MR, J, NORM>;
   static std::atomic<uint64_t> done;
   const Device dev = device_now();
   const int sms = dev.sms, halves = p.v.halves;
-  p.staged = MR == 1 && p.norm_w && p.v.K * 2 <= 32768;
-  const int x_bytes = p.staged ? (p.v.K * 2 + 127) / 128 * 128 : 0, room = SMEM - 512 - x_bytes;
   // as many CTAs as run at once, unless their tiles' sums are too many for them; those with one tile more come first, so that an SM has some of either kind
-  p.groups = std::max(std::min(p.v.tiles, at_once(p.splits, sms)), ceil_div(p.v.tiles, (room - WARPS * 3 * J * unit) / tile / halves));
+  p.groups = std::max(std::min(p.v.tiles, at_once(p.splits, sms)), ceil_div(p.v.tiles, (SMEM - WARPS * 3 * J * unit) / tile / halves));
   p.more = p.v.tiles % p.groups;
   p.most = (p.v.tiles / p.groups + (p.more > 0)) * halves;
   const int runs = ceil_div(ceil_div(p.v.chunks, p.splits), WARPS * p.wide) * (p.wide / J) * p.most;           // of a warp
-  p.depth = std::max(1, std::min({runs, (room - p.most * WARPS * NT * 512) / (WARPS * J * unit), 8}));
-  p.x_at = p.most * WARPS * NT * 512 + std::max(WARPS * p.depth * J * unit, p.most * TILE * 8 * NT * 4);
-  const int smem = p.x_at + x_bytes;
+  p.depth = std::max(1, std::min({runs, (SMEM - p.most * WARPS * NT * 512) / (WARPS * J * unit), 8}));
+  const int smem = p.most * WARPS * NT * 512 + std::max(WARPS * p.depth * J * unit, p.most * TILE * 8 * NT * 4);
   if (int rc = allow_smem(k, SMEM, dev.id, done)) return rc;
   const dim3 grid(p.groups * p.splits);
   if (p.splits > 1) return launch_chain_cluster(k, grid, dim3(WARPS * 32 + 32), (unsigned)p.splits, (size_t)smem, s, p);
@@ -440,9 +426,11 @@ int launch_runs(RowsP p, cudaStream_t s) {
   p.splits = splits_of(p.v, device_now().sms);
   // runs of two units while every warp has one: a copy of 1 KB costs as much as one of two
   p.wide = ceil_div(p.v.chunks, p.splits) >= 2 * WARPS ? 2 : 1;
-  if constexpr (MR <= 8)
-    if (p.wide == 2) return launch<GROUP, ZEROS, F16, MR, 2>(p, s);
-  return launch<GROUP, ZEROS, F16, MR, 1>(p, s);
+  if constexpr (MR <= 8) {
+    if (p.norm_w) return p.wide == 2 ? launch<GROUP, ZEROS, F16, MR, 2, true>(p, s) : launch<GROUP, ZEROS, F16, MR, 1, true>(p, s);
+    if (p.wide == 2) return launch<GROUP, ZEROS, F16, MR, 2, false>(p, s);
+  }
+  return launch<GROUP, ZEROS, F16, MR, 1, false>(p, s);
 }
 template <int GROUP, int MR>
 int by_kind(const RowsP& p, cudaStream_t s) {
