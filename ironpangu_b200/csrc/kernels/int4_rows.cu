@@ -6,8 +6,8 @@
 // (with the opposite sign). The sums of x come out of products with ones, once for all tiles of a CTA. The group's scale multiplies its f32 sum. Products are exact; sums run
 // up to 24 |x| instead of 8 |x| a weight, which costs them two bits of f32.
 // A CTA has a share of the tiles of sixteen rows, and its eight warps share K: a warp takes every eighth run of one or two units, for all tiles of the CTA, so that its operands
-// of x are loaded once. Under a norm they take its gains on the way (the one rounding to bf16 that a normalised row has), and the row's factor, from the squares that
-// the warps saw, multiplies the sums: nothing waits for a whole row (2 x 16384 by 4096, 8 rows: 24.0 -> 21.1 us, 1 row 17.5 -> 17.0). Units come by bulk copies into a ring of the warp's own, the first ones ahead
+// of x are loaded once, and normalised on the way. (A norm's factor into the sums instead saves the pass ahead, 1.5 us of 8 rows of 4096, but rounds the row differently from
+// a norm of its own: results were off by twice their rounding.) Units come by bulk copies into a ring of the warp's own, the first ones ahead
 // of the wait for the preceding kernel. (Loads ahead into registers waited for one another, whatever their number: 3.4 TB/s without any products.) Sums of the tiles lie in
 // shared memory, a float4 a lane. What a unit costs is its instructions (two cycles of a scheduler for one on integers, eight for a product), so a ninth warp computes the
 // copies' addresses and requests them, and a stage costs the others a look at its barrier and an arrival. The warps' sums are added in one order, and so a row's bits do not depend on the rows beside it.
@@ -110,12 +110,61 @@ __device__ __noinline__ bool wait_more(uint32_t bar, uint32_t parity) {
 }
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) { return ready(bar, parity) || wait_more(bar, parity); }
 
-// MR: most rows of x; J: units of a run; NORM: under a norm (asked for in the kernel, it cost the others 4 %: 8 rows of 8192 by 8192 13.2 -> 13.7 us)
+// the warps that multiply (the ninth one is at its copies)
+__device__ __forceinline__ void consumers() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
+
+// A norm's factor of the row of this lane's operands. One row: 256 threads add up its squares; more: a warp a row. In one order whatever the rows: of 256 threads' pieces of
+// eight columns, 32 threads at a time. All loads of 4096 columns are under way at once.
+__device__ __forceinline__ float factor_of(const RowsP& p, float* sums, float* inv, int warp, int lane, int most_rows) {
+  const int pieces = p.v.K / 8;
+  auto squares = [](const uint4& u, float& ss) {
+    float f[8];
+    unpack8(u, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+  };
+  const uint4 none = make_uint4(0, 0, 0, 0);
+  if (most_rows == 1) {
+    float ss = 0.f;
+    for (int i = warp * 32 + lane; i < pieces; i += 512) {
+      const uint4 a = ld_now16(p.x + i * 8), b = i + 256 < pieces ? ld_now16(p.x + (i + 256) * 8) : none;
+      squares(a, ss);
+      squares(b, ss);
+    }
+    ss = warp_sum(ss);
+    if (lane == 0) sums[warp] = ss;
+    consumers();
+    ss = sums[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) ss += sums[w];
+    return rsqrtf(ss / (float)p.v.K + p.eps);
+  }
+  float ss[WARPS] = {};
+  if (warp < p.T) {
+    const bf16* row = p.x + (long)warp * p.ldx;
+    for (int i = lane; i < pieces; i += 512) {
+      uint4 u[16];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) u[q] = i + q * 32 < pieces ? ld_now16(row + (i + q * 32) * 8) : none;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) squares(u[q], ss[q % WARPS]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < WARPS; ++q) ss[q] = warp_sum(ss[q]);
+#pragma unroll
+  for (int q = 1; q < WARPS; ++q) ss[0] += ss[q];
+  if (lane == 0) inv[warp] = rsqrtf(ss[0] / (float)p.v.K + p.eps);
+  consumers();
+  return inv[lane >> 2];
+}
+
+// MR: most rows of x; J: units of a run; NORM: under a norm (asked for in the kernel, it cost the others 4 %: 8 rows of 8192 by 8192 13.2 us and 13.7)
 template <int GROUP, bool ZEROS, bool F16, int MR, int J, bool NORM>
 __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) {
   constexpr int NT = (MR + 7) / 8, RUNS = GROUP / 32, NG = 4 / RUNS, UNIT = CODES + NG * (ZEROS ? 48 : 32);      // runs of 32 columns of a group, groups of a unit, its bytes
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float sums[WARPS][8], squares[8];     // of the rows' squares, where there is a norm: a warp's and the CTA's share
+  __shared__ float sums[WARPS], inv[8];            // of a row's squares; the rows' factors
   __shared__ __align__(16) unsigned char runs_of_x[MR == 1 ? WARPS * 512 : 16];
   __shared__ uint64_t bars[WARPS * 16];            // of a warp's stages: full, and eight further on empty
   grid_dep_launch();
@@ -179,16 +228,14 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     uint32_t at = ring, stage = bar, parity = 0;   // the stage at hand: this lane's first codes, and its barrier
     const int ch0 = chunk0 + warp * p.wide, k1 = min(v.K, chunk1 * CHUNK);      // the first run, the end of the CTA's columns
     uint4 b[J][NT][4];                             // operands: four runs of eight columns of a row of x a unit
-    float square = 0.f;                            // of this lane's columns of its row
-    // eight columns under the norm's gains; returns the sum of their squares. The row's factor comes last, into the sums: a warp sees the whole row only then
-    auto gained = [&](uint4& x, const uint4& gain) {
-      float f[8], w[8], ss = 0.f;
+    // eight columns under the norm, rounded as a norm of its own would leave them
+    auto normed = [&](uint4& x, const uint4& gain, float by) {
+      float f[8], w[8];
       unpack8(x, f);
       unpack8(gain, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += f[e] * f[e], f[e] *= w[e];
+      for (int e = 0; e < 8; ++e) f[e] = f[e] * by * w[e];
       x = pack8(f);
-      return ss;
     };
     const uint4 none = make_uint4(0, 0, 0, 0);
     // One row: a lane has eight columns of a run, one run ahead, and the warp reads them from shared memory
@@ -201,6 +248,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
       if (NORM) gain = in ? *reinterpret_cast<const uint4*>(p.norm_w + k) : none;
     };
     if (MR == 1) fetch(ch0);
+    const float by = NORM ? factor_of(p, sums, inv, warp, lane, MR) : 1.f;      // of this lane's row
     const bf16* xr[NT];                            // more: this lane's row (for rows behind the last one that one, whose results nothing stores), its first column
 #pragma unroll
     for (int n = 0; n < NT; ++n) xr[n] = p.x + (long)min(n * 8 + g, p.T - 1) * p.ldx + c * 8;
@@ -208,13 +256,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     for (int ch = ch0; ch < chunk1; ch = after(ch)) {
       if (MR == 1) {
         uint4 x = ahead;
-        if (NORM) {
-          float ss = gained(x, gain);
-#pragma unroll
-          for (int d = 4; d < 32; d *= 2)
-            if (d < 16 || J == 2) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-          square += ss;
-        }
+        if (NORM) normed(x, gain, by);
         sts_u4(xs + lane * 16, x);
         fetch(after(ch));
         __syncwarp();
@@ -226,7 +268,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
       } else {
         const int k0 = ch * CHUNK;
         if (NT == 1 && !NORM && k0 + J * CHUNK <= k1) {         // without the look at every column's place; with gains, or with two tiles of rows, the code's length costs more
-                                                               // (8 rows of 4096 by 16384 14.4 -> 13.7 us; 2 x 16384 by 4096 under a norm 20.9 -> 21.4)
+                                                               // (8 rows of 4096 by 16384 14.4 us without, 13.7 with; of 2 x 16384 by 4096 under a norm 20.9 and 21.4)
 #pragma unroll
           for (int u = 0; u < J; ++u)
 #pragma unroll
@@ -242,18 +284,13 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
               for (int i = 0; i < 4; ++i) b[u][n][i] = k0 + u * CHUNK + i * 32 + c * 8 < k1 ? ld_now16(xr[n] + k0 + u * CHUNK + i * 32) : none;
         }
         if (NORM) {
-          float ss[J];
 #pragma unroll
-          for (int u = 0; u < J; ++u) {
-            float of[4];
+          for (int u = 0; u < J; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int k = k0 + u * CHUNK + i * 32 + c * 8;
-              of[i] = gained(b[u][0][i], k < k1 ? *reinterpret_cast<const uint4*>(p.norm_w + k) : none);
+              normed(b[u][0][i], k < k1 ? *reinterpret_cast<const uint4*>(p.norm_w + k) : none, by);
             }
-            ss[u] = (of[0] + of[1]) + (of[2] + of[3]);
-          }
-          square += J == 2 ? ss[0] + ss[J - 1] : ss[0];
         }
       }
       float sum[J][NT][NG][4];                     // of the groups' columns of x, rows 2 c and 2 c + 1, twice: times -24 without zero points
@@ -332,11 +369,6 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
         if (at == end) at = ring, stage = bar, parity ^= 1;
       }
     }
-    if (NORM) {
-      square += __shfl_xor_sync(0xffffffffu, square, 1);
-      square += __shfl_xor_sync(0xffffffffu, square, 2);
-      if (c == 0) sums[warp][g] = square;
-    }
   }
   if (__any_sync(0xffffffffu, late)) {             // a copy that did not land: nothing of the tiles is right
     if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
@@ -354,10 +386,6 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     const float* f = red + ((tile * NT + (t >> 3)) * 32 + (r & 7) * 4 + ((t & 7) >> 1)) * 4 + (r >> 3) * 2 + (t & 1);
     part[i] = ((f[0] + f[step]) + (f[2 * step] + f[3 * step])) + ((f[4 * step] + f[5 * step]) + (f[6 * step] + f[7 * step]));
   }
-  if (NORM && threadIdx.x < 8) {
-    const int t = MR == 1 ? 0 : threadIdx.x;
-    squares[threadIdx.x] = ((sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t])) + ((sums[4][t] + sums[5][t]) + (sums[6][t] + sums[7][t]));
-  }
   if (p.splits > 1) cluster_barrier();
   else __syncthreads();
   const int rows = mine * TILE;                    // of the result
@@ -370,12 +398,6 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     for (int s = 0; s < p.splits; ++s) {
       a += p.splits > 1 ? ld_part(part_at + at * 4, s) : part[at];
       if (gated) u += p.splits > 1 ? ld_part(part_at + up_at * 4, s) : part[up_at];
-    }
-    if (NORM) {
-      float ss = 0.f;
-      for (int s = 0; s < p.splits; ++s) ss += p.splits > 1 ? ld_part(smem_addr(squares + t), s) : squares[t];
-      const float by = rsqrtf(ss / (float)v.K + p.eps);
-      a *= by, u *= by;
     }
     if (gated) a = a / (1.f + __expf(-a)) * u;
     if (p.residual) a += __bfloat162float(p.residual[t * p.ldr + n]);
