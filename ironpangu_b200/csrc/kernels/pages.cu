@@ -206,66 +206,64 @@ __global__ void __launch_bounds__(PLAN) extend_kernel(Pool q, const int32_t* slo
 
 // grid (entries of the list, pieces of a row): the CTAs of the first entry that names a parent have all of its children
 __global__ void __launch_bounds__(256) fork_kernel(Pool q, const int32_t* src, const int32_t* dst, int n) {
-  __shared__ uint32_t seen[MAX_SLOTS / 32];
-  __shared__ int warps[33], list[TAKEN], children;
-  __shared__ uint16_t entry[MAX_SLOTS];
+  __shared__ uint32_t seen[MAX_SLOTS / 32], named[MAX_SLOTS / 32];
+  __shared__ int warps[33], list[TAKEN], children, parents;
+  __shared__ uint32_t child[MAX_SLOTS];          // entry of the list, slot above
   __shared__ bool last;
   grid_dep_launch();
   grid_dep_wait();
   const IfabPagePool& p = q.p;
   const int parent = src[blockIdx.x];
-  if (threadIdx.x == 0) children = 0;
+  if (threadIdx.x == 0) children = parents = 0;
+  for (int i = threadIdx.x; i < (p.slots + 31) / 32; i += blockDim.x) named[i] = 0;
   bool good = distinct(dst, n, p.slots, seen), earlier = false;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int a = src[i];
     good = good && a >= 0 && a < p.slots;
     earlier = earlier || (a == parent && i < (int)blockIdx.x);
-    if (a == parent) entry[atomicAdd(&children, 1)] = (uint16_t)i;
+    if (a == parent) child[atomicAdd(&children, 1)] = (uint32_t)i | (uint32_t)dst[i] << 16;
+    if (good && !(atomicOr(named + (a >> 5), 1u << (a & 31)) >> (a & 31) & 1)) atomicAdd(&parents, 1);
   }
   good = __syncthreads_and(good);
   earlier = __syncthreads_or(earlier);
-  if (good && !earlier) {
-    // 64 entries side by side, every fourth child a thread
-    const int32_t* row = p.table + (long)parent * p.max_pages;
-    for (int j = blockIdx.y * 64 + (threadIdx.x & 63); j < p.max_pages; j += gridDim.y * 64) {
-      const int then = row[j];
-      int times = 0;
-      for (int c0 = threadIdx.x >> 6; c0 < children; c0 += 32) {
-        int now[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (c0 + 4 * c < children) now[c] = p.table[(long)dst[entry[c0 + 4 * c]] * p.max_pages + j];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (c0 + 4 * c < children) {
-            q.staged()[(long)entry[c0 + 4 * c] * p.max_pages + j] = then;
-            if (now[c] != then) {
-              ++times;
-              give(p, now[c]);
-            }
-          }
-      }
-      if (times) take(p, then, times);
-    }
-    if (blockIdx.y == 0)
-      for (int c = threadIdx.x; c < children; c += blockDim.x) q.used()[entry[c]] = p.lengths[parent];
+  if (!good && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    report(p.status, IFAB_STATUS_BAD_INDEX);
+    q.control()[COUNT] = 0;
+    q.control()[GO] = -1;
   }
+  if (!good || earlier) return;                  // the others have no part in the ticket: of 1152 CTAs for 64 children, 18 draw one (5 us of a turn's 70)
+  // 64 entries side by side, every fourth child a thread
+  const int32_t* row = p.table + (long)parent * p.max_pages;
+  for (int j = blockIdx.y * 64 + (threadIdx.x & 63); j < p.max_pages; j += gridDim.y * 64) {
+    const int then = row[j];
+    int times = 0;
+    for (int c0 = threadIdx.x >> 6; c0 < children; c0 += 32) {
+      int now[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c0 + 4 * c < children) now[c] = p.table[(long)(child[c0 + 4 * c] >> 16) * p.max_pages + j];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c0 + 4 * c < children) {
+          q.staged()[(long)(child[c0 + 4 * c] & 0xffff) * p.max_pages + j] = then;
+          if (now[c] != then) {
+            ++times;
+            give(p, now[c]);
+          }
+        }
+    }
+    if (times) take(p, then, times);
+  }
+  if (blockIdx.y == 0)
+    for (int c = threadIdx.x; c < children; c += blockDim.x) q.used()[child[c] & 0xffff] = p.lengths[parent];
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(q.control() + TICKET, 1) == (int)(gridDim.x * gridDim.y) - 1;
+  if (threadIdx.x == 0) last = atomicAdd(q.control() + TICKET, 1) == parents * (int)gridDim.y - 1;
   __syncthreads();
   if (!last) return;
   __threadfence();
   // Every count has been changed. Children that need a page of their own for a partly filled one: all but the first of a parent that is itself replaced.
-  volatile int32_t* control = q.control();
-  if (!good) {
-    if (threadIdx.x == 0) {
-      report(p.status, IFAB_STATUS_BAD_INDEX);
-      control[TICKET] = control[COUNT] = 0;
-      control[GO] = -1;
-    }
-    return;
-  }
+  int32_t* control = q.control();
   int count = 0;
   for (int i0 = 0; i0 < n; i0 += blockDim.x) {
     const int i = i0 + threadIdx.x;
