@@ -31,6 +31,11 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(f"int4: {what}")
 
 
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from a row to the next one; of a single row, whose stride says nothing, its columns."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 class Int4Weight:
     """A packed matrix of ``rows`` x ``k`` weights; ``gated``: gate rows, then as many up rows. ``units`` holds codes, scales and zero points together."""
 
@@ -55,8 +60,9 @@ class Int4Weight:
         if out is None:
             out = torch.empty(self.rows, self.k, dtype=BF16, device=self.device)
         _need(out.shape == (self.rows, self.k) and out.dtype == BF16 and out.stride(1) == 1 and out.device == self.device, "the output must be bf16 [rows, k] beside the weights")
+        _need(_pitch(out) % 8 == 0 and _pitch(out) >= self.k and out.data_ptr() % 16 == 0, "the output's rows must lie on 16 bytes, one behind the other")
         with torch.cuda.device(self.device):
-            check(_lib.load().ifab_int4_dequantise(self.ref, out.data_ptr(), out.stride(0), _lib.current_stream(self.device.index)), "int4.dequantise")
+            check(_lib.load().ifab_int4_dequantise(self.ref, out.data_ptr(), _pitch(out), _lib.current_stream(self.device.index)), "int4.dequantise")
         return out
 
 
@@ -65,9 +71,10 @@ def quantise(w: torch.Tensor, *, group: int = 128, zeros: bool = False, gated: b
     ``s = bf16((hi - lo) / 15)``, ``z = rint(-lo / s)``; ``q = rint(w / s) + z``, within 0 .. 15. Where ``s`` is 0 (a group of zeros, or of less than bf16's smallest) the weights are 0; a group with an infinity or NaN gets a
     scale of NaN."""
     _need(w.dim() == 2 and w.dtype == BF16 and w.stride(1) == 1 and w.is_cuda, "the matrix must be bf16 [rows, k] on the device, columns contiguous")
+    _need(w.shape[0] >= 1 and _pitch(w) % 8 == 0 and _pitch(w) >= w.shape[1] and w.data_ptr() % 16 == 0, "the matrix's rows must lie on 16 bytes, one behind the other")
     out = Int4Weight(w.shape[0], w.shape[1], group=group, zeros=zeros, gated=gated, device=w.device)
     with torch.cuda.device(w.device):
-        check(_lib.load().ifab_int4_quantise(out.ref, w.data_ptr(), w.stride(0), _lib.current_stream(w.device.index)), "int4.quantise")
+        check(_lib.load().ifab_int4_quantise(out.ref, w.data_ptr(), _pitch(w), _lib.current_stream(w.device.index)), "int4.quantise")
     return out
 
 
@@ -76,13 +83,15 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor
     ``[rows, ceil(k / group)]``."""
     _need(codes.dim() == 2 and codes.dtype == torch.uint8 and codes.stride(1) == 1 and codes.is_cuda, "codes must be uint8 [rows, k] on the device, columns contiguous")
     rows, k = codes.shape
+    _need(rows >= 1 and _pitch(codes) >= k, "codes must be rows one behind the other")
+    _need(group in GROUPS, f"groups of {group} columns are not supported")
     _need(scales.dtype in (BF16, F16), "scales must be bf16 or f16")
     for t, what in ((scales, "scales"), (zeros, "zero points")):
         _need(t is None or (t.shape == (rows, -(-k // group)) and t.is_contiguous() and t.device == codes.device), f"{what} must be contiguous [rows, groups] beside the codes")
     _need(zeros is None or zeros.dtype == torch.uint8, "zero points must be uint8")
     out = Int4Weight(rows, k, group=group, zeros=zeros is not None, gated=gated, f16=scales.dtype == F16, device=codes.device)
     with torch.cuda.device(codes.device):
-        check(_lib.load().ifab_int4_pack(out.ref, codes.data_ptr(), codes.stride(0), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _lib.current_stream(codes.device.index)), "int4.pack")
+        check(_lib.load().ifab_int4_pack(out.ref, codes.data_ptr(), _pitch(codes), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _lib.current_stream(codes.device.index)), "int4.pack")
     return out
 
 
@@ -90,20 +99,20 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
            out: Optional[torch.Tensor] = None, status_ptr: Optional[int] = None) -> torch.Tensor:
     """``y = x @ w.T (+ residual)``, or of a gated matrix ``silu(x @ gate.T) * (x @ up.T)``, for any number of bf16 rows ``x`` ``[T, k]``. ``norm_w`` (up to eight rows): the
     rows are RMS-normalised first, as :func:`ops.decode.rmsnorm` does it. ``residual`` (bf16, not of a gated matrix) may be ``out``. Sums are f32 and the result is rounded
-    once, to bf16 or with ``out_f32`` not at all. Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product; up to
+    once, to bf16 or with ``out_f32`` not at all. ``out`` must not overlap ``x``. Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product; up to
     there it is not. ``status_ptr``: a status word for
     waits that run out."""
     T = x.shape[0]
     # the checks say what is wrong in _refuse: a message that is made for every call costs as much as the launch
-    if not (x.dim() == 2 and x.shape[1] == w.k and x.dtype is BF16 and x.device == w.device and x.stride(1) == 1 and (x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 or T == 0)):
+    if not (x.dim() == 2 and x.shape[1] == w.k and x.dtype is BF16 and x.device == w.device and x.stride(1) == 1 and (T == 0 or x.data_ptr() % 16 == 0 and (T == 1 or x.stride(0) % 8 == 0))):
         _refuse(x, w, norm_w, residual, out)
     if out is None:
         out = torch.empty((T, w.n), dtype=F32 if out_f32 else BF16, device=w.device)
-    elif not (out.shape == (T, w.n) and (out.dtype is BF16 or out.dtype is F32) and out.device == w.device and out.stride(1) == 1):
+    elif not (out.shape == (T, w.n) and (out.dtype is BF16 or out.dtype is F32) and out.device == w.device and (out.stride(1) == 1 or w.n == 1) and (T == 0 or out.data_ptr() != x.data_ptr())):
         _refuse(x, w, norm_w, residual, out)
     if norm_w is not None and not (norm_w.shape == (w.k,) and norm_w.dtype is BF16 and norm_w.device == w.device and norm_w.stride(0) == 1 and norm_w.data_ptr() % 16 == 0 and T <= NORM_ROWS):
         _refuse(x, w, norm_w, residual, out)
-    if residual is not None and not (not w.gated and residual.shape == (T, w.n) and residual.dtype is BF16 and residual.device == w.device and residual.stride(1) == 1):
+    if residual is not None and not (not w.gated and residual.shape == (T, w.n) and residual.dtype is BF16 and residual.device == w.device and (residual.stride(1) == 1 or w.n == 1)):
         _refuse(x, w, norm_w, residual, out)
     if T == 0:
         return out
@@ -111,16 +120,16 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return linear(x, w, norm_w=norm_w, eps=eps, residual=residual, out=out, status_ptr=status_ptr)
-    lib, rp, ldr = _lib.load(), None, 0
+    lib, rp, ldr, ldx = _lib.load(), None, 0, w.k if T == 1 else x.stride(0)
     if residual is not None:
         rp, ldr = residual.data_ptr(), residual.stride(0)
     f32 = 1 if out.dtype is F32 else 0
     if T > STREAM_ROWS:
         scratch = torch.empty(lib.ifab_int4_gemm_scratch(T, w.k), dtype=torch.uint8, device=w.device)
-        check(lib.ifab_int4_gemm(w.ref, x.data_ptr(), x.stride(0), rp, ldr, out.data_ptr(), out.stride(0), f32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr,
+        check(lib.ifab_int4_gemm(w.ref, x.data_ptr(), ldx, rp, ldr, out.data_ptr(), out.stride(0), f32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr,
                                  _lib.current_stream(dev)), "int4.linear")
         return out
-    check(lib.ifab_int4_rows(w.ref, x.data_ptr(), x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps, rp, ldr, out.data_ptr(), out.stride(0), f32, T, status_ptr,
+    check(lib.ifab_int4_rows(w.ref, x.data_ptr(), ldx, None if norm_w is None else norm_w.data_ptr(), eps, rp, ldr, out.data_ptr(), out.stride(0), f32, T, status_ptr,
                              _lib.current_stream(dev)), "int4.linear")
     return out
 
@@ -128,13 +137,14 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
 def _refuse(x: torch.Tensor, w: Int4Weight, norm_w, residual, out) -> None:
     T = x.shape[0] if x.dim() else 0
     _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
-    _need(x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 or T == 0, "rows must lie on 16 bytes")
+    _need(T == 0 or x.data_ptr() % 16 == 0 and (T == 1 or x.stride(0) % 8 == 0), "rows must lie on 16 bytes")
     if norm_w is not None:
         _need(norm_w.shape == (w.k,) and norm_w.dtype == BF16 and norm_w.is_contiguous() and norm_w.device == w.device and norm_w.data_ptr() % 16 == 0,
               f"gains must be bf16 [{w.k}] on 16 bytes")
         _need(T <= NORM_ROWS, f"a norm ahead of {T} rows is a launch of its own (ops.decode.rmsnorm)")
-    _need(out is None or (out.shape == (T, w.n) and out.dtype in (BF16, F32) and out.stride(1) == 1 and out.device == w.device),
+    _need(out is None or (out.shape == (T, w.n) and out.dtype in (BF16, F32) and (out.stride(1) == 1 or w.n == 1) and out.device == w.device),
           f"the output must be bf16 or f32 [T, {w.n}] beside the weights")
+    _need(out is None or T == 0 or out.data_ptr() != x.data_ptr(), "the output must not overlap the rows")
     if residual is not None:
         _need(not w.gated, "a gated unit takes no residual")
         _need(residual.shape == (T, w.n) and residual.dtype == BF16 and residual.stride(1) == 1 and residual.device == w.device,

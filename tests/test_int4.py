@@ -286,3 +286,48 @@ def test_ranges_of_rows_and_scales():
     y, scale = int4.linear(tiny, w, out_f32=True), tiny.double().abs() @ v[:20].abs().T
     # the smallest bf16 numbers: a result below f32's normal range has steps of 2^-149
     _close(y, tiny.double() @ v.T, _operands(v, tiny)[1] + 2.0 ** -148)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 140, 250])
+@pytest.mark.parametrize("N", [260, 2100, 3300, 4500, 5800, 7700, 12100])
+def test_shares_of_k_of_any_number(N, T):
+    """Widths whose tiles leave K to one, two, three ... CTAs of a cluster."""
+    test_linear(N, 2056, T, 64, True, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,gated", [(60, 300, False), (128, 9000, True), (129, 300, True), (250, 9000, False)])
+def test_a_wait_that_runs_out_of_fewer_rows(T, N, gated):
+    test_a_wait_that_runs_out(T, N, gated)
+
+
+@pytest.mark.gpu
+def test_where_matrices_and_rows_lie():
+    """Rows that lie too near, off 16 bytes or over one another are refused before anything is launched; of a single row the stride says nothing."""
+    from ironpangu_b200.ops import int4
+
+    m = torch.randn(40, 272, device="cuda").to(BF16)
+    for bad in (m[:, :268].reshape(-1)[:40 * 268].view(40, 268)[:, :264], m[:, 4:268], m[:1, :264].expand(40, 264), m[:0, :264]):
+        with pytest.raises(ValueError, match="rows must lie|not supported"):
+            int4.quantise(bad)
+    w = int4.quantise(m[:, :264])
+    one = torch.as_strided(m, (1, 264), (3, 1))
+    assert torch.equal(int4.quantise(one).dequantise(), w.dequantise()[:1])
+    with pytest.raises(ValueError, match="rows must lie"):
+        w.dequantise(torch.empty(40, 268, dtype=BF16, device="cuda")[:, :264])
+    q, s, z = _codes(40, 264, 64, False, 0)
+    for args, group, what in (((q[:1].expand(40, 264), s), 64, "one behind the other"), ((q, s), 0, "groups of 0"), ((q, s), 48, "groups of 48")):
+        with pytest.raises(ValueError, match=what):
+            int4.pack(*args, group=group)
+    x = torch.randn(4, 272, device="cuda").to(BF16)
+    with pytest.raises(ValueError, match="16 bytes"):
+        int4.linear(x[:, 1:265], w)
+    with pytest.raises(ValueError, match="16 bytes"):
+        int4.linear(x.reshape(-1)[:4 * 268].view(4, 268)[:, :264], w)
+    assert torch.equal(int4.linear(torch.as_strided(x, (1, 264), (3, 1)), w), int4.linear(x[:1, :264], w))
+    square = int4.quantise(torch.randn(264, 264, device="cuda").to(BF16))
+    y = x[:, :264].contiguous()
+    with pytest.raises(ValueError, match="overlap"):
+        int4.linear(y, square, out=y)
+    assert torch.equal(int4.linear(y, square, residual=(r := y.clone()), out=r), int4.linear(y, square, residual=y))
