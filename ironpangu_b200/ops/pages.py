@@ -97,7 +97,7 @@ class PagePool:
 
     def __init__(self, caches: List[torch.Tensor], *, slots: int, max_pages: int):
         self.pages = s = PageSet(caches)
-        _need(1 <= slots <= MAX_SLOTS and max_pages >= 1 and max_pages * s.page_tokens < 1 << 31, f"{slots} slots of {max_pages} pages are not supported")
+        _need(1 <= slots <= MAX_SLOTS and max_pages >= 1 and (max_pages + 1) * s.page_tokens < 1 << 31, f"{slots} slots of {max_pages} pages are not supported")
         self.slots, self.max_pages, self.page_tokens, self.device = slots, max_pages, s.page_tokens, s.device
         i32 = lambda *shape, v=0: torch.full(shape, v, dtype=I32, device=s.device)
         self.table, self.lengths, self.refs, self.live = i32(slots, max_pages, v=-1), i32(slots), i32(s.pages), i32(1)

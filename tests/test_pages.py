@@ -256,3 +256,20 @@ def test_a_step_in_a_graph():
         _same(pool, plain, before)
     pool.free(_list(list(range(6))))
     assert int(pool.refs.sum()) == 0 and bool((pool.table == -1).all())
+
+
+@pytest.mark.gpu
+def test_positions_fit_32_bits_with_a_page_to_spare():
+    from ironpangu_b200.ops import pages as P
+
+    cache = torch.zeros(2, 1 << 19, 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="not supported"):
+        P.PagePool([cache], slots=1, max_pages=(1 << 12) - 1)
+    pool = P.PagePool([cache], slots=1, max_pages=(1 << 12) - 2)
+    i32 = lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")
+    pool.extend(i32(0), i32(((1 << 12) - 2) << 19))
+    with pytest.raises(OverflowError):
+        pool.check()
+    pool.extend(i32(0), i32(1 << 20))
+    pool.check()
+    assert pool.table[0, :3].tolist() == [0, 1, -1]
