@@ -196,7 +196,7 @@ class DenseDecoder:
         self.next_ids = torch.zeros(T, dtype=torch.int32, device=dev)
         self.next_vals = torch.zeros(T, dtype=torch.float32, device=dev)
         self.logits = e(T, self.vl, dt=torch.float32) if keep_logits else None
-        self.launches_per_forward = 2 + ((6 if T <= 8 else 8) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
+        self.launches_per_forward = 2 + ((6 if T <= 8 else 8 if T <= int4.STREAM_ROWS else 12) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
         self._graph = None
 
     def _row_parallel(self, a: torch.Tensor, w: torch.Tensor, x: torch.Tensor) -> None:
