@@ -36,6 +36,7 @@ class Continuations:
         self.store = [torch.empty(store_pages, *c.shape[1:], dtype=c.dtype, device=dev) for c in decoder.k_cache + decoder.v_cache] if store_pages else []
         self._store = P.PageSet(self.store) if store_pages else None
         self._store_free = list(range(store_pages))[::-1]
+        self._aside = {}                      # continuations that were set aside: their pages in the second pool
 
     # -- prompt --------------------------------------------------------------------------------------------------------------
     def start(self, prompt: Sequence[int], n: int, *, temperature: float = 1.0, top_k: int = 50, top_p: float = 1.0, seed: int = 0) -> torch.Tensor:
@@ -98,8 +99,7 @@ class Continuations:
 
     def step(self) -> torch.Tensor:
         """The next token of every continuation (device tensor ``[n]``): one graph replay. A pool that has run out of pages shows in :meth:`check`."""
-        if not self.n:
-            raise RuntimeError("no continuations: start() first")
+        self._all_here()
         if self.length >= self.dec.max_context:
             raise OverflowError("the continuations run past the context")
         self.length += 1
@@ -116,29 +116,41 @@ class Continuations:
             self._graphs[key] = g
         return self.ids[:self.n]
 
+    def _all_here(self) -> None:
+        if not self.n:
+            raise RuntimeError("no continuations: start() first")
+        if self._aside:
+            raise RuntimeError(f"continuations {sorted(self._aside)} are set aside: take_up() first")
+
     def check(self) -> None:
-        """Raises OverflowError when a step found too few free pages (its tokens are not to be used)."""
+        """Raises IndexError when a resampling named a parent out of range (nothing was resampled then), OverflowError when a step found too few free pages (its tokens are not to be used)."""
         self.pool.check()
 
     def resample(self, parents: torch.Tensor) -> None:
         """Continuation ``i`` goes on from what ``parents[i]`` is now (int32 ``[n]`` on the device, out of 0 .. n - 1, with repeats)."""
+        self._all_here()
         n = self.n
         if parents.shape != (n,) or parents.dtype != I32:
             raise ValueError(f"parents must be int32 [{n}]")
-        self.pool.fork(parents + 1, self._children[:n])
-        self.dec.tokens[:n].copy_(self.dec.tokens[:n].index_select(0, parents.long().clamp(0, n - 1)))
+        inside = (parents >= 0) & (parents < n)
+        self.pool.fork(torch.where(inside, parents + 1, -1), self._children[:n])
+        now = self.dec.tokens[:n]
+        now.copy_(torch.where(inside.all(), now.index_select(0, parents.long().clamp(0, n - 1)), now))
 
     def end(self) -> None:
-        """Gives back all pages but those that were set aside."""
+        """Gives back all pages, those that were set aside among them."""
         if self.n:
             self.pool.free(self._children)
             self.pool.free(self._first)
+        for ids in self._aside.values():
+            self._store_free += ids.tolist()
+        self._aside = {}
         self.n = self.length = 0
 
     # -- setting aside ---------------------------------------------------------------------------------------------------------
     def set_aside(self, i: int) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Copies continuation ``i`` to the second pool and gives its pages back; :meth:`take_up` brings it back from what this returns."""
-        if not 0 <= i < self.n:
+        """Copies continuation ``i`` to the second pool and gives its pages back; :meth:`take_up` brings it back from what this returns, and no step can be taken before."""
+        if not 0 <= i < self.n or i in self._aside:
             raise ValueError(f"no continuation {i}")
         length = int(self.pool.lengths[1 + i])
         count = -(-length // self.pool.page_tokens)
@@ -149,16 +161,20 @@ class Continuations:
         rows = (length - self.pool.page_tokens * torch.arange(count, device=dev)).clamp(max=self.pool.page_tokens).to(I32)
         P.copy(self.pool.pages, self._store, self.pool.table[1 + i, :count], ids, rows)
         self.pool.free(self._children[i:i + 1])
+        self._aside[i] = ids
         return ids, rows
 
     def take_up(self, i: int, held: Tuple[torch.Tensor, torch.Tensor]) -> None:
         """Continuation ``i``, which was set aside, has its pages again."""
         ids, rows = held
+        if self._aside.get(i) is not ids:
+            raise ValueError(f"this is not what continuation {i} was set aside as")
         count = ids.numel()
         length = (count - 1) * self.pool.page_tokens + rows[-1:] if count else torch.zeros(1, dtype=I32, device=ids.device)
         self.pool.extend(self._children[i:i + 1], length.to(I32))
         self.pool.check()
         P.copy(self._store, self.pool.pages, ids, self.pool.table[1 + i, :count], rows)
+        del self._aside[i]
         self._store_free += ids.tolist()
 
     def pack(self) -> int:

@@ -148,3 +148,48 @@ def test_refusals():
     c.end()
     c.start(list(range(20)), 2)
     assert c.generate(list(range(20)), 2, 3, temperature=0.0)[0] == c.generate(list(range(20)), 1, 3, temperature=0.0)[0]
+
+
+def test_set_aside_once_and_taken_up_as_itself():
+    """While a continuation is set aside no step is taken and nothing is drawn; it comes back once, from what it was set aside as, or goes with the end."""
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    _, fab, dec = _decoder(False)
+    c = Continuations(dec, store_pages=4)
+    c.start(list(range(20)), 3, seed=2)
+    held = c.set_aside(1)
+    for call, what in ((c.step, "set aside"), (lambda: c.resample(torch.zeros(3, dtype=I32, device="cuda")), "set aside")):
+        with pytest.raises(RuntimeError, match=what):
+            call()
+    other = c.set_aside(0)
+    for call in (lambda: c.set_aside(1), lambda: c.take_up(1, other), lambda: c.take_up(2, held)):
+        with pytest.raises(ValueError):
+            call()
+    c.take_up(1, held)
+    with pytest.raises(ValueError):
+        c.take_up(1, held)
+    c.take_up(0, other)
+    c.step()
+    c.check()
+    c.set_aside(2)
+    c.end()
+    assert sorted(c._store_free) == [0, 1, 2, 3] and int(dec.pool.refs.sum()) == 0
+    fab.close()
+
+
+def test_parents_out_of_range_change_nothing():
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    _, fab, dec = _decoder(False)
+    c = Continuations(dec)
+    c.start(list(range(20)), 3, seed=2)
+    table, tokens = dec.pool.table.clone(), dec.tokens.clone()
+    for bad in ([0, -1, 1], [0, 1, 3], [2, 2, 2 ** 31 - 1]):
+        c.resample(torch.tensor(bad, dtype=I32, device="cuda"))
+        with pytest.raises(IndexError):
+            c.check()
+        assert torch.equal(dec.pool.table, table) and torch.equal(dec.tokens, tokens)
+    c.resample(torch.tensor([2, 2, 0], dtype=I32, device="cuda"))
+    c.check()
+    assert torch.equal(dec.tokens[:3], tokens[:3][[2, 2, 0]])
+    fab.close()
