@@ -47,7 +47,7 @@ class Int4Weight:
         self.n = rows // 2 if gated else rows                 # columns of a result
         _need(max(rows, k) <= 1 << 24, f"a matrix of {rows} x {k} is too large")
         self.units = torch.empty(_lib.load().ifab_int4_bytes(self.n, k, group, self.zeros, self.gated), dtype=torch.uint8, device=device)
-        self.device = self.units.device
+        self.device, self.index = self.units.device, self.units.get_device()
         self.desc = IfabInt4(self.units.data_ptr(), self.n, k, group, self.zeros, self.gated, self.f16)
         self.ref = C.byref(self.desc)
 
@@ -102,42 +102,50 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
     once, to bf16 or with ``out_f32`` not at all. ``out`` must not overlap ``x``. Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product; up to
     there it is not. ``status_ptr``: a status word for
     waits that run out."""
-    T = x.shape[0]
-    # the checks say what is wrong in _refuse: a message that is made for every call costs as much as the launch
-    if not (x.dim() == 2 and x.shape[1] == w.k and x.dtype is BF16 and x.device == w.device and x.stride(1) == 1 and (T == 0 or x.data_ptr() % 16 == 0 and (T == 1 or x.stride(0) % 8 == 0))):
+    # the checks say what is wrong in _refuse: a message that is made for every call costs as much as the launch. Device numbers, which are compared in a fifth of the time that
+    # devices are, and each attribute is asked for once
+    shape, dev, xp, n, k = x.shape, w.index, x.data_ptr(), w.n, w.k
+    if not (len(shape) == 2 and shape[1] == k and x.dtype is BF16 and x.get_device() == dev and x.stride(1) == 1):
+        _refuse(x, w, norm_w, residual, out)
+    T = shape[0]
+    ldx = x.stride(0) if T > 1 else k
+    if xp % 16 or ldx % 8:
         _refuse(x, w, norm_w, residual, out)
     if out is None:
-        out = torch.empty((T, w.n), dtype=F32 if out_f32 else BF16, device=w.device)
-    elif not (out.shape == (T, w.n) and (out.dtype is BF16 or out.dtype is F32) and out.device == w.device and (out.stride(1) == 1 or w.n == 1) and (T == 0 or out.data_ptr() != x.data_ptr())):
+        f32 = out_f32
+        out = torch.empty((T, n), dtype=F32 if f32 else BF16, device=w.device)
+        yp, ldy = out.data_ptr(), n
+    else:
+        yp, ldy, f32 = out.data_ptr(), out.stride(0), out.dtype is F32
+        if not (out.shape == (T, n) and (f32 or out.dtype is BF16) and out.get_device() == dev and (out.stride(1) == 1 or n == 1) and (yp != xp or T == 0)):
+            _refuse(x, w, norm_w, residual, out)
+    if norm_w is not None and not (norm_w.shape == (k,) and norm_w.dtype is BF16 and norm_w.get_device() == dev and norm_w.stride(0) == 1 and norm_w.data_ptr() % 16 == 0 and T <= NORM_ROWS):
         _refuse(x, w, norm_w, residual, out)
-    if norm_w is not None and not (norm_w.shape == (w.k,) and norm_w.dtype is BF16 and norm_w.device == w.device and norm_w.stride(0) == 1 and norm_w.data_ptr() % 16 == 0 and T <= NORM_ROWS):
-        _refuse(x, w, norm_w, residual, out)
-    if residual is not None and not (not w.gated and residual.shape == (T, w.n) and residual.dtype is BF16 and residual.device == w.device and (residual.stride(1) == 1 or w.n == 1)):
-        _refuse(x, w, norm_w, residual, out)
+    rp, ldr = None, 0
+    if residual is not None:
+        if not (not w.gated and residual.shape == (T, n) and residual.dtype is BF16 and residual.get_device() == dev and (residual.stride(1) == 1 or n == 1)):
+            _refuse(x, w, norm_w, residual, out)
+        rp, ldr = residual.data_ptr(), residual.stride(0)
     if T == 0:
         return out
-    dev = w.device.index
+    if dev < 0:
+        _need(False, "the weights are on the host")
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return linear(x, w, norm_w=norm_w, eps=eps, residual=residual, out=out, status_ptr=status_ptr)
-    lib, rp, ldr, ldx = _lib.load(), None, 0, w.k if T == 1 else x.stride(0)
-    if residual is not None:
-        rp, ldr = residual.data_ptr(), residual.stride(0)
-    f32 = 1 if out.dtype is F32 else 0
+    lib = _lib.load()
     if T > STREAM_ROWS:
-        scratch = torch.empty(lib.ifab_int4_gemm_scratch(T, w.k), dtype=torch.uint8, device=w.device)
-        check(lib.ifab_int4_gemm(w.ref, x.data_ptr(), ldx, rp, ldr, out.data_ptr(), out.stride(0), f32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr,
-                                 _lib.current_stream(dev)), "int4.linear")
+        scratch = torch.empty(lib.ifab_int4_gemm_scratch(T, k), dtype=torch.uint8, device=w.device)
+        check(lib.ifab_int4_gemm(w.ref, xp, ldx, rp, ldr, yp, ldy, f32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr, _lib.current_stream(dev)), "int4.linear")
         return out
-    check(lib.ifab_int4_rows(w.ref, x.data_ptr(), ldx, None if norm_w is None else norm_w.data_ptr(), eps, rp, ldr, out.data_ptr(), out.stride(0), f32, T, status_ptr,
-                             _lib.current_stream(dev)), "int4.linear")
+    check(lib.ifab_int4_rows(w.ref, xp, ldx, None if norm_w is None else norm_w.data_ptr(), eps, rp, ldr, yp, ldy, f32, T, status_ptr, _lib.current_stream(dev)), "int4.linear")
     return out
 
 
 def _refuse(x: torch.Tensor, w: Int4Weight, norm_w, residual, out) -> None:
     T = x.shape[0] if x.dim() else 0
     _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
-    _need(T == 0 or x.data_ptr() % 16 == 0 and (T == 1 or x.stride(0) % 8 == 0), "rows must lie on 16 bytes")
+    _need(x.data_ptr() % 16 == 0 and (T <= 1 or x.stride(0) % 8 == 0), "rows must lie on 16 bytes")
     if norm_w is not None:
         _need(norm_w.shape == (w.k,) and norm_w.dtype == BF16 and norm_w.is_contiguous() and norm_w.device == w.device and norm_w.data_ptr() % 16 == 0,
               f"gains must be bf16 [{w.k}] on 16 bytes")

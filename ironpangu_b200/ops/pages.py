@@ -46,7 +46,7 @@ class PageSet:
         t = caches[0]
         _need(all(c.is_cuda and c.device == t.device and c.dim() >= 2 and c.shape[:2] == t.shape[:2] and c.is_contiguous() for c in caches),
               "caches must be contiguous [pages, page_tokens, ...] on one device, with as many pages and rows each")
-        self.pages, self.page_tokens, self.device = t.shape[0], t.shape[1], t.device
+        self.pages, self.page_tokens, self.device, self.index = t.shape[0], t.shape[1], t.device, t.get_device()
         _need(self.pages > 0 and self.page_tokens > 0, "caches without pages")
         _need(self.pages < 1 << 30 and self.page_tokens < 1 << 20, "caches too large")
         self.row_bytes = [c[0, 0].numel() * c.element_size() for c in caches]
@@ -65,7 +65,7 @@ class PageSet:
             raise IndexError("pages: an index out of range was skipped")
 
     def _list(self, t: torch.Tensor, what: str, n: int) -> int:
-        if not (t.dtype is I32 and t.dim() == 1 and t.device == self.device and (t.stride(0) == 1 or t.numel() < 2) and t.numel() == n):
+        if not (t.dtype is I32 and t.shape == (n,) and t.get_device() == self.index and (n < 2 or t.stride(0) == 1)):
             _need(t.dim() == 1 and t.dtype == I32 and t.device == self.device and (t.numel() < 2 or t.stride(0) == 1), f"{what} must be a contiguous int32 list on {self.device}")
             _need(False, f"{what}: {t.numel()} entries beside {n}")
         return t.data_ptr()
@@ -79,7 +79,7 @@ def copy(src: PageSet, dst: PageSet, src_ids: torch.Tensor, dst_ids: torch.Tenso
         _need(False, "the sets' pages are not alike")
     n = src_ids.numel()
     a, b = src._list(src_ids, "src_ids", n), src._list(dst_ids, "dst_ids", n)
-    _call(src.device.index, "ifab_pages_copy", src.ref, dst.ref, a, b, None if rows is None else src._list(rows, "rows", n), n, dst.status_ptr)
+    _call(src.index, "ifab_pages_copy", src.ref, dst.ref, a, b, None if rows is None else src._list(rows, "rows", n), n, dst.status_ptr)
 
 
 def _call(dev: int, name: str, *args) -> None:
@@ -99,6 +99,7 @@ class PagePool:
         self.pages = s = PageSet(caches)
         _need(1 <= slots <= MAX_SLOTS and max_pages >= 1 and (max_pages + 1) * s.page_tokens < 1 << 31, f"{slots} slots of {max_pages} pages are not supported")
         self.slots, self.max_pages, self.page_tokens, self.device = slots, max_pages, s.page_tokens, s.device
+        self.index = s.index
         i32 = lambda *shape, v=0: torch.full(shape, v, dtype=I32, device=s.device)
         self.table, self.lengths, self.refs, self.live = i32(slots, max_pages, v=-1), i32(slots), i32(s.pages), i32(1)
         words = (s.pages + 31) // 32
@@ -127,7 +128,7 @@ class PagePool:
         a, b = self.pages._list(slots, "slots", n), self.pages._list(tokens, "tokens", n)
         if n > self.slots:
             _need(False, f"{n} entries for {self.slots} slots")
-        _call(self.device.index, "ifab_pages_extend", self.ref, a, b, n)
+        _call(self.index, "ifab_pages_extend", self.ref, a, b, n)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Slot ``dst[i]`` becomes what slot ``src[i]`` was before the call; what it held before is given back. ``dst`` names a slot once, ``src`` as often as wanted, and a slot
@@ -137,16 +138,16 @@ class PagePool:
         a, b = self.pages._list(src, "src", n), self.pages._list(dst, "dst", n)
         if n > self.slots:
             _need(False, f"{n} entries for {self.slots} slots")
-        _call(self.device.index, "ifab_pages_fork", self.ref, a, b, n)
+        _call(self.index, "ifab_pages_fork", self.ref, a, b, n)
 
     def free(self, slots: torch.Tensor, below: Optional[torch.Tensor] = None) -> None:
         """All pages of the slots are given back, or with ``below`` the whole pages all of whose positions lie below ``below[i]`` (a window has passed them); those
         entries of the table are -1 then. A page goes back to the pool when no other slot holds it."""
         n = slots.numel()
         a, b = self.pages._list(slots, "slots", n), None if below is None else self.pages._list(below, "below", n)
-        _call(self.device.index, "ifab_pages_free", self.ref, a, b, n)
+        _call(self.index, "ifab_pages_free", self.ref, a, b, n)
 
     def compact(self) -> None:
         """Live pages move into the lowest places - the first one that lies too high into the first hole, and so on - in all caches, and the table follows; their
         number lands in ``live``."""
-        _call(self.device.index, "ifab_pages_compact", self.ref, self.live.data_ptr())
+        _call(self.index, "ifab_pages_compact", self.ref, self.live.data_ptr())

@@ -331,3 +331,10 @@ def test_where_matrices_and_rows_lie():
     with pytest.raises(ValueError, match="overlap"):
         int4.linear(y, square, out=y)
     assert torch.equal(int4.linear(y, square, residual=(r := y.clone()), out=r), int4.linear(y, square, residual=y))
+
+
+def test_weights_on_the_host_multiply_nothing():
+    from ironpangu_b200.ops import int4
+
+    with pytest.raises(ValueError, match="on the host"):
+        int4.linear(torch.zeros(1, 64, dtype=BF16), int4.Int4Weight(16, 64, device="cpu"))
