@@ -60,7 +60,7 @@ struct Place {           // of a lane in its unit
 };
 
 template <int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(256) quantise_kernel(View v, const bf16* w, long ldw) {
+__global__ void __launch_bounds__(256, 4) quantise_kernel(View v, const bf16* w, long ldw) {
   grid_dep_wait();
   float most[2] = {0.f, 0.f};
 #pragma unroll 1

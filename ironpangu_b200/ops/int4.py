@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import check
+from ._lib import call_on, check
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 GROUPS = (32, 64, 128)
@@ -61,8 +61,7 @@ class Int4Weight:
             out = torch.empty(self.rows, self.k, dtype=BF16, device=self.device)
         _need(out.shape == (self.rows, self.k) and out.dtype == BF16 and out.stride(1) == 1 and out.device == self.device, "the output must be bf16 [rows, k] beside the weights")
         _need(_pitch(out) % 8 == 0 and _pitch(out) >= self.k and out.data_ptr() % 16 == 0, "the output's rows must lie on 16 bytes, one behind the other")
-        with torch.cuda.device(self.device):
-            check(_lib.load().ifab_int4_dequantise(self.ref, out.data_ptr(), _pitch(out), _lib.current_stream(self.device.index)), "int4.dequantise")
+        call_on(self.index, "ifab_int4_dequantise", self.ref, out.data_ptr(), _pitch(out))
         return out
 
 
@@ -73,8 +72,7 @@ def quantise(w: torch.Tensor, *, group: int = 128, zeros: bool = False, gated: b
     _need(w.dim() == 2 and w.dtype == BF16 and w.stride(1) == 1 and w.is_cuda, "the matrix must be bf16 [rows, k] on the device, columns contiguous")
     _need(w.shape[0] >= 1 and _pitch(w) % 8 == 0 and _pitch(w) >= w.shape[1] and w.data_ptr() % 16 == 0, "the matrix's rows must lie on 16 bytes, one behind the other")
     out = Int4Weight(w.shape[0], w.shape[1], group=group, zeros=zeros, gated=gated, device=w.device)
-    with torch.cuda.device(w.device):
-        check(_lib.load().ifab_int4_quantise(out.ref, w.data_ptr(), _pitch(w), _lib.current_stream(w.device.index)), "int4.quantise")
+    call_on(out.index, "ifab_int4_quantise", out.ref, w.data_ptr(), _pitch(w))
     return out
 
 
@@ -90,8 +88,7 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor
         _need(t is None or (t.shape == (rows, -(-k // group)) and t.is_contiguous() and t.device == codes.device), f"{what} must be contiguous [rows, groups] beside the codes")
     _need(zeros is None or zeros.dtype == torch.uint8, "zero points must be uint8")
     out = Int4Weight(rows, k, group=group, zeros=zeros is not None, gated=gated, f16=scales.dtype == F16, device=codes.device)
-    with torch.cuda.device(codes.device):
-        check(_lib.load().ifab_int4_pack(out.ref, codes.data_ptr(), _pitch(codes), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _lib.current_stream(codes.device.index)), "int4.pack")
+    call_on(out.index, "ifab_int4_pack", out.ref, codes.data_ptr(), _pitch(codes), scales.data_ptr(), None if zeros is None else zeros.data_ptr())
     return out
 
 

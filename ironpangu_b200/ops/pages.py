@@ -12,7 +12,7 @@ from typing import List, Optional
 import torch
 
 from . import _lib
-from ._lib import check
+from ._lib import call_on
 
 I32 = torch.int32
 BAD_INDEX, NO_PAGES = 4, 8          # IFAB_STATUS_* of common.cuh
@@ -79,15 +79,7 @@ def copy(src: PageSet, dst: PageSet, src_ids: torch.Tensor, dst_ids: torch.Tenso
         _need(False, "the sets' pages are not alike")
     n = src_ids.numel()
     a, b = src._list(src_ids, "src_ids", n), src._list(dst_ids, "dst_ids", n)
-    _call(src.index, "ifab_pages_copy", src.ref, dst.ref, a, b, None if rows is None else src._list(rows, "rows", n), n, dst.status_ptr)
-
-
-def _call(dev: int, name: str, *args) -> None:
-    if dev == torch.cuda.current_device():
-        check(getattr(_lib.load(), name)(*args, _lib.current_stream(dev)), name)
-    else:
-        with torch.cuda.device(dev):
-            check(getattr(_lib.load(), name)(*args, _lib.current_stream(dev)), name)
+    call_on(src.index, "ifab_pages_copy", src.ref, dst.ref, a, b, None if rows is None else src._list(rows, "rows", n), n, dst.status_ptr)
 
 
 class PagePool:
@@ -128,7 +120,7 @@ class PagePool:
         a, b = self.pages._list(slots, "slots", n), self.pages._list(tokens, "tokens", n)
         if n > self.slots:
             _need(False, f"{n} entries for {self.slots} slots")
-        _call(self.index, "ifab_pages_extend", self.ref, a, b, n)
+        call_on(self.index, "ifab_pages_extend", self.ref, a, b, n)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Slot ``dst[i]`` becomes what slot ``src[i]`` was before the call; what it held before is given back. ``dst`` names a slot once, ``src`` as often as wanted, and a slot
@@ -138,16 +130,16 @@ class PagePool:
         a, b = self.pages._list(src, "src", n), self.pages._list(dst, "dst", n)
         if n > self.slots:
             _need(False, f"{n} entries for {self.slots} slots")
-        _call(self.index, "ifab_pages_fork", self.ref, a, b, n)
+        call_on(self.index, "ifab_pages_fork", self.ref, a, b, n)
 
     def free(self, slots: torch.Tensor, below: Optional[torch.Tensor] = None) -> None:
         """All pages of the slots are given back, or with ``below`` the whole pages all of whose positions lie below ``below[i]`` (a window has passed them); those
         entries of the table are -1 then. A page goes back to the pool when no other slot holds it."""
         n = slots.numel()
         a, b = self.pages._list(slots, "slots", n), None if below is None else self.pages._list(below, "below", n)
-        _call(self.index, "ifab_pages_free", self.ref, a, b, n)
+        call_on(self.index, "ifab_pages_free", self.ref, a, b, n)
 
     def compact(self) -> None:
         """Live pages move into the lowest places - the first one that lies too high into the first hole, and so on - in all caches, and the table follows; their
         number lands in ``live``."""
-        _call(self.index, "ifab_pages_compact", self.ref, self.live.data_ptr())
+        call_on(self.index, "ifab_pages_compact", self.ref, self.live.data_ptr())
