@@ -38,7 +38,9 @@ constexpr int FT = 128, BK = 64, TOK = 128, STAGES = 4, CHUNKS = 4, THREADS = 35
 template <int GROUP, bool ZEROS, bool WIDE>
 constexpr int SMEM = STAGES * (WIDE ? 2 : 1) * TOK * BK * 2 + CHUNKS * Units<GROUP, ZEROS>::BYTES + 1024 + 512;
 constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
-static_assert(CHUNKS % 2 == 0 && STAGES >= 4, "two groups of warps tell phases of the rings apart by parity (int4_tc_pair.cu)");
+// Phases are told apart by parity (int4_tc_pair.cu): a slot of codes belongs to one group of warps, and a group's block before this one, at most three back, waited for the
+// products STAGES blocks ahead of it
+static_assert(CHUNKS % 2 == 0 && STAGES >= 3, "a group could take a phase for the one two ahead");
 static_assert(TOK * FT * 4 <= STAGES * TOK * BK * 2, "the part of the sum takes the ring's place");
 
 struct TcP {

@@ -29,9 +29,10 @@ constexpr int W_BYTES = FT * BK * 2, STAGE = W_BYTES + TOK / 2 * BK * 2;      //
 template <int GROUP, bool ZEROS>
 constexpr int SMEM = STAGES * STAGE + CHUNKS * Units<GROUP, ZEROS>::BYTES + 1024 + 512;
 constexpr uint32_t SUM_COLS = 256;                   // of tensor memory
-// A wait by parity tells a phase from the one before it only. A slot of the codes' ring belongs to one of the two groups of warps, which so has seen its last copy land; and a
-// group's wait for the stage of its block before this one implies that the stage's last but one phase is over
-static_assert(CHUNKS % 2 == 0 && STAGES >= 4, "a group could take a phase for the one two ahead");
+// A wait by parity tells a phase from the one before it only, so whoever waits has to know that the one before that is over. The groups that make operands know it by the order
+// of the products: a group's block before this one, at most five back (three chunks apart where a tile has an odd number of them), waited for the products STAGES blocks ahead of
+// it, whose own stage, and chunk of codes, were done with before.
+static_assert(STAGES >= 5 && 2 * CHUNKS >= STAGES + 5, "a group could take a phase for the one two ahead");
 constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
 constexpr int RASTER = 8;                            // token tiles that pairs share weights over
 
