@@ -380,18 +380,19 @@ int at_once(int n, const Device& dev) {
   if (have) have->store(count);
   return count;
 }
-// CTAs along K: those that run at once, by the chunks that the busiest SM goes through and what a wave costs besides, counted as FIXED chunks
+// CTAs along K: those that run at once, by the chunks that the busiest SM goes through and what a wave costs besides (start, first loads, cluster's sum: 10 us), counted in chunks.
+// 2 and 6 chose the same or as good ones over 25 sizes of one wave, but two waves of shares where one of whole tiles is as fast
+constexpr int WAVE_COST = 12;
 template <bool WIDE>
-int splits_of(int tiles, int chunks, const Device& dev) {
-  constexpr int FIXED = 6;       // 2 and 12 chose the same or as good ones over 25 sizes
+int splits_of(int tiles, int chunks, const Device& dev, int* waves) {
   int best = 1;
   long least = 0;
   for (int n = 1; n <= 8 && (n == 1 || chunks >= 2 * n); ++n) {
     const int room = at_once<WIDE>(n, dev);
     if (!room) continue;
-    const long waves = ceil_div(tiles, room), share = WIDE ? 1 : std::min(2, ceil_div(std::min(tiles, room) * n, dev.sms));
-    const long cost = waves * (share * ceil_div(chunks, n) + FIXED);
-    if (!least || cost < least) least = cost, best = n;
+    const long waves_of_n = ceil_div(tiles, room), share = WIDE ? 1 : std::min(2, ceil_div(std::min(tiles, room) * n, dev.sms));
+    const long cost = waves_of_n * (share * ceil_div(chunks, n) + WAVE_COST);
+    if (!least || cost < least) least = cost, best = n, *waves = (int)waves_of_n;
   }
   return best;
 }
@@ -402,14 +403,14 @@ int launch_wide(const CUtensorMap& tx, const TcP& p, dim3 grid, cudaStream_t s) 
 
 }  // namespace
 
-// Tokens of a pair's tile (int4_tc_pair.cu): the width whose waves of tiles over the pairs take least, or 0 where the pairs would not have a tile each.
-static int pair_tokens(int T, int rows, int pairs) {
-  const int tn = ceil_div(rows, 2 * FT);
+// What a chunk of 128 columns costs a CTA's or a pair's tile: most of it whatever the tokens (0.80 us at 176 of them, 0.91 at 256; counted in tokens)
+constexpr long CHUNK_COST = 480;
+// Tokens of a pair's tile (int4_tc_pair.cu), the width whose waves of tiles over the pairs cost least, and that cost
+static int pair_tokens(int T, int rows, int chunks, int pairs, long* cost) {
   int best = 0;
-  long least = 0;
   for (int tok = 256; tok >= 128; tok -= 16) {
-    const long tiles = (long)tn * ceil_div(T, tok), cost = (tiles + pairs - 1) / pairs * (tok + 32);
-    if (T > 128 && tiles * 8 >= 7l * pairs && (!least || cost < least)) least = cost, best = tok;
+    const long now = ((long)ceil_div(rows, 2 * FT) * ceil_div(T, tok) + pairs - 1) / pairs * chunks * (tok + CHUNK_COST);
+    if (!best || now < *cost) *cost = now, best = tok;
   }
   return best;
 }
@@ -430,12 +431,19 @@ extern "C" int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const 
   const int halves = p.v.halves, sms = dev.sms;
   cudaStream_t s = (cudaStream_t)stream;
   if (int rc = launch_chain(rows_kernel, dim3(T), dim3(256), 0, s, (const bf16*)x, ldx, rows, (long)p.v.K, factor, p.v.K)) return rc;
-  if (const int tok = pair_tokens(T, p.v.N * halves, sms / 2))
-    return pair_product(p.v, rows, factor, p.residual, ldr, y, ldy, out_f32, T, tok, std::min(sms / 2, ceil_div(p.v.N * halves, 2 * FT) * ceil_div(T, tok)), spin_limit, status, s);
   const int wide = T > TOK, ty = ceil_div(T, wide ? 2 * TOK : TOK), tiles = ceil_div(p.v.N, halves == 2 ? FT / 2 : FT);
-  if (ty > 65535) return -1;
   p.tok = std::max(ceil_div(ceil_div(T, ty), 16) * 16, wide ? TOK + 16 : 16);
-  p.splits = wide ? splits_of<true>(tiles * ty, p.v.chunks, dev) : splits_of<false>(tiles * ty, p.v.chunks, dev);
+  int waves = 1;
+  p.splits = (long)tiles * ty > 8l * sms ? 1 : wide ? splits_of<true>(tiles * ty, p.v.chunks, dev, &waves) : splits_of<false>(tiles * ty, p.v.chunks, dev, &waves);
+  if (wide) {
+    // Pairs, unless a tile a CTA whose K is shared costs less, a wave counted as twelve chunks, of which pairs have eight: 256 rows of 6144 by 4096 26 us (pairs 33), 512 of 4096 by 16384 64 (113);
+    // 256 of 10240 by 4096 42 (36), 400 of 6144 by 4096 37 (35), 2048 of 1024 by 1024 22 (19)
+    long cost = 0;
+    const int tok = pair_tokens(T, p.v.N * halves, p.v.chunks, sms / 2, &cost);
+    if ((long)tiles * ty > 8l * sms || cost <= waves * ((long)ceil_div(p.v.chunks, p.splits) * (p.tok + CHUNK_COST)) + (waves * WAVE_COST - 8) * (2 * TOK + CHUNK_COST))
+      return pair_product(p.v, rows, factor, p.residual, ldr, y, ldy, out_f32, T, tok, (int)std::min<long>(sms / 2, (long)ceil_div(p.v.N * halves, 2 * FT) * ceil_div(T, tok)), spin_limit, status, s);
+  }
+  if (ty > 65535) return -1;
   CUtensorMap tx;          // of 16-bit elements: the type is the products' to know
   if (int rc = make_tmap_bf16_2d(&tx, rows, (uint64_t)T, (uint64_t)p.v.K, (uint64_t)p.v.K, (uint32_t)p.tok)) return rc;
   const dim3 grid(tiles * p.splits, ty);
