@@ -1,7 +1,7 @@
 // Products of many rows with 4-bit weights (int4.cuh) on tcgen05:  y[t][n] = sum_k x[t][k] w[n][k] (+ residual), or of a gate | up matrix silu(gate) up.
 //
 // The 128 rows of an MMA are weight rows, the tokens its columns. Weights become s (q - z) in registers, where a thread is a row, and go straight into tensor memory
-// as the MMA's first operand: neither codes nor weights pass through shared memory, whose bandwidth belongs to the tokens' tiles. Two groups of four warps take the
+// as the MMA's first operand: they do not pass through shared memory, whose bandwidth belongs to the tokens' tiles; codes do, 8 KB for 32 of weights. Two groups of four warps take the
 // chunks of 128 columns in turn.
 // The operands are f16, each row with a power of two of its own. A product s (q - z) has up to 13 bits: bf16 leaves 8 of them, and a gated unit's result was off by 1.6
 // times its rounding; f16 leaves 11. Rows of x keep all their 8 bits: a launch ahead (rows_kernel) brings a row's largest magnitude to 2^14 .. 2^15, so that what falls below
@@ -12,10 +12,13 @@
 //   warp 10     copies of codes, the first of them ahead of the wait for the preceding kernel
 //   warps 2-9   weights into tensor memory; then 2-5 read the accumulator
 // Up to 128 tokens: two CTAs an SM (128 columns of sums and four stages of 32 columns of weights each), so that one multiplies while the other starts or stores. More: tiles of
-// up to 256 tokens, a CTA an SM, so that the weights become operands once; that is what bounds the kernel there (203 rows of 6144 by 4096: 26 - 28 us, in tiles of 112 tokens 30).
-// With few tiles the chunks along K are shared by the CTAs of a cluster, of any size up to eight (17 rows of 4096 by 4096 10.5 us, of 6144 by 4096 15; in powers of two 12.8 and
+// up to 256 tokens, a CTA an SM, so that the weights become operands once (203 rows of 6144 by 4096 24.2 us, in tiles of 112 tokens 30).
+// With few tiles the chunks along K are shared by the CTAs of a cluster, of any size up to eight (17 rows of 4096 by 4096 10.2 us, of 6144 by 4096 15; in powers of two 12.8 and
 // 19.5, when all clusters did not run at once): each leaves its part of the sum in its shared memory as f32 and every CTA adds up a share of the tokens over
 // distributed shared memory, in the order of the parts.
+// Measured: 0.65 - 0.8 us a chunk and 12 us beside them, of which the launch ahead, the first loads and the cluster's sum are most: 203 rows of 6144 by 4096 24.2 us (the bf16
+// product of the same sizes 25.1; 7 us of products), 64 of 2 x 16384 by 4096 37 (58), 203 of 4096 by 16384 37 (41). The products' pipe is busy for 28 % of an SM's time there,
+// the issue slots for 34 %; a fifth stage, and signals without the delay, gave 2 % or less.
 // Every wait is bounded. One that runs out raises the CTA's flag and the status word; the warps that read the accumulator then wait for what the CTA has started and
 // leave NaN as their part of the sum.
 #include <algorithm>
