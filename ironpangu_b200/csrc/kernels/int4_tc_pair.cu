@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
   uint64_t* empty = full + STAGES;                                           // each CTA's own, as acc_full
   uint64_t *acc_full = empty + STAGES, *acc_empty = acc_full + 2;            // of each sum; acc_empty: leader's
   uint64_t *units_full = acc_empty + 2, *units_empty = units_full + CHUNKS;   // each CTA's own
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units_empty + CHUNKS);
+  uint64_t* drained = units_empty + CHUNKS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const View& v = p.v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
@@ -169,6 +170,7 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 2 * READERS);
     }
+    mbar_init(drained, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_x);
@@ -236,6 +238,9 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       *abort_flag = 1;
       if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
     }
+    // whoever gives up: products that were issued end before the CTAs do
+    if (elected) commit_pair(drained);
+    mbar_wait(drained, 0, DRAIN);
   } else if (warp >= 3 && warp < 11) {
     const int group = (warp - 3) >> 2, row = ((warp - 3) & 3) * 32 + lane;
     RowOfWeights<GROUP, ZEROS> mine;
