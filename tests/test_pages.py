@@ -273,3 +273,31 @@ def test_positions_fit_32_bits_with_a_page_to_spare():
     pool.extend(i32(0), i32(1 << 20))
     pool.check()
     assert pool.table[0, :3].tolist() == [0, 1, -1]
+
+
+@pytest.mark.gpu
+def test_pages_beyond_4_gb_of_a_cache():
+    """Offsets that pass 32 bits: a page near the end of a cache of 5 GB is shared, copied, moved and copied out."""
+    from ironpangu_b200.ops import pages as P
+
+    n, pt = 5120, 16
+    cache = torch.zeros(n, pt, 1 << 15, dtype=torch.bfloat16, device="cuda")
+    pool = P.PagePool([cache], slots=3, max_pages=n)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    pool.extend(i32(0, 1), i32((n - 3) * pt, pt + 5))
+    assert pool.table[1, :2].tolist() == [n - 3, n - 2]
+    cache[n - 3], cache[n - 2] = 3.0, 5.0
+    pool.fork(i32(1), i32(2))
+    pool.check()
+    assert pool.table[2, :2].tolist() == [n - 3, n - 1] and bool((cache[n - 1, :5] == 5).all()) and not bool(cache[n - 1, 5:].any())
+    out = torch.zeros(2, pt, 1 << 15, dtype=torch.bfloat16, device="cuda")
+    store = P.PageSet([out])
+    P.copy(pool.pages, store, i32(n - 1), i32(1), i32(5))
+    assert bool((out[1, :5] == 5).all()) and not bool(out[0].any()) and not bool(out[1, 5:].any())
+    pool.free(i32(0))
+    pool.compact()
+    pool.check()
+    assert int(pool.live) == 3 and pool.table[2, :2].tolist() == [0, 2] and pool.table[1, :2].tolist() == [0, 1]
+    assert bool((cache[0] == 3).all()) and bool((cache[1] == 5).all()) and bool((cache[2, :5] == 5).all())
+    del cache, pool
+    torch.cuda.empty_cache()
