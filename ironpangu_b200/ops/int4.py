@@ -40,12 +40,13 @@ class Int4Weight:
     """A packed matrix of ``rows`` x ``k`` weights; ``gated``: gate rows, then as many up rows. ``units`` holds codes, scales and zero points together."""
 
     def __init__(self, rows: int, k: int, *, group: int = 128, zeros: bool = False, gated: bool = False, f16: bool = False, device="cuda"):
-        _need(group in GROUPS, f"groups of {group} columns are not supported")
-        _need(rows >= 1 and k >= 8 and k % 8 == 0, f"a matrix of {rows} x {k} is not supported (columns in eights)")
-        _need(not gated or rows % 2 == 0, f"{rows} rows are not gate and up rows")
+        if not (group in GROUPS and rows >= 1 and k >= 8 and k % 8 == 0 and not (gated and rows % 2) and max(rows, k) <= 1 << 24):      # (messages only where they are wanted)
+            _need(group in GROUPS, f"groups of {group} columns are not supported")
+            _need(rows >= 1 and k >= 8 and k % 8 == 0, f"a matrix of {rows} x {k} is not supported (columns in eights)")
+            _need(max(rows, k) <= 1 << 24, f"a matrix of {rows} x {k} is too large")
+            _need(False, f"{rows} rows are not gate and up rows")
         self.rows, self.k, self.group, self.zeros, self.gated, self.f16 = rows, k, group, bool(zeros), bool(gated), bool(f16)
         self.n = rows // 2 if gated else rows                 # columns of a result
-        _need(max(rows, k) <= 1 << 24, f"a matrix of {rows} x {k} is too large")
         self.units = torch.empty(_lib.load().ifab_int4_bytes(self.n, k, group, self.zeros, self.gated), dtype=torch.uint8, device=device)
         self.device, self.index = self.units.device, self.units.get_device()
         self.desc = IfabInt4(self.units.data_ptr(), self.n, k, group, self.zeros, self.gated, self.f16)
