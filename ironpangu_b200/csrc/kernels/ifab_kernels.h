@@ -531,8 +531,9 @@ uint64_t ifab_int4_gemm_scratch(int T, int K);
 /* ---- pages of a cache that sequences share (csrc/kernels/pages.cu) ----
  * A set of caches: `ptrs` and `row_bytes` [caches] on the device (base address, bytes of a row, a multiple of 16), pages of `page_tokens` rows back to back.
  * A pool: table [slots, max_pages] (-1: none), lengths [slots], refs [pages] (entries that name a page), free_bits [(pages + 31) / 32] (a bit per page with refs 0),
- * and a workspace of ifab_pages_work_words. Every list of slots is on the device; a list that names a slot out of range or, where slots are written, twice does nothing
- * but set IFAB_STATUS_BAD_INDEX, one that needs more pages than there are nothing but set IFAB_STATUS_NO_PAGES. */
+ * and a workspace of ifab_pages_work_words. Every list of slots is on the device; a list that names a slot out of range or, where slots are given pages, twice does nothing
+ * but set IFAB_STATUS_BAD_INDEX, one that needs more pages than there are nothing but set IFAB_STATUS_NO_PAGES. ifab_pages_copy skips entries out of range (and sets the
+ * bit in `status`) and copies the others. */
 typedef struct IfabPageSet {
   const uint64_t* ptrs;
   const int64_t* row_bytes;

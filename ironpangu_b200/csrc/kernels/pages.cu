@@ -345,20 +345,26 @@ __global__ void __launch_bounds__(256) free_kernel(Pool q, const int32_t* slots,
   grid_dep_wait();
   const IfabPagePool& p = q.p;
   const int first = blockIdx.x * TOGETHER, count = min(TOGETHER, n - first), step = gridDim.y * blockDim.x;
-  if (threadIdx.x < count) {
-    const int i = first + threadIdx.x, s = slots[i], b = below ? below[i] : 0;
-    const bool good = s >= 0 && s < p.slots && b >= 0;
-    slot[threadIdx.x] = good ? s : -1;
+  bool good = true;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int s = slots[i], b = below ? below[i] : 0, c = i - first;
+    const bool mine = s >= 0 && s < p.slots && b >= 0;
+    good = good && mine;
+    if (c < 0 || c >= count || !mine) continue;
+    slot[c] = s;
     // a page that is partly filled stays with its sequence
-    end[threadIdx.x] = !good ? 0 : below ? min(b, p.lengths[s]) / p.set.page_tokens : p.max_pages;
-    if (!good && blockIdx.y == 0) report(p.status, IFAB_STATUS_BAD_INDEX);
-    if (good && !below && blockIdx.y == 0) p.lengths[s] = 0;
+    end[c] = below ? min(b, p.lengths[s]) / p.set.page_tokens : p.max_pages;
   }
-  __syncthreads();
+  // a list with a bad entry is refused as a whole, and so every slot that is compared and looked up below is one of the pool's
+  if (!__syncthreads_and(good)) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) report(p.status, IFAB_STATUS_BAD_INDEX);
+    return;
+  }
+  if (!below && blockIdx.y == 0 && threadIdx.x < count) p.lengths[slots[first + threadIdx.x]] = 0;
   // a slot that is named more than once: the first entry does it, as far as the furthest of them goes
   for (int e = threadIdx.x; e < count * n; e += blockDim.x) {
     const int c = e / n, k = e - c * n;
-    if (k == first + c || slots[k] != slot[c] || (below && below[k] < 0)) continue;
+    if (k == first + c || slots[k] != slots[first + c]) continue;
     if (k < first + c) atomicExch(&slot[c], -1);
     else if (below) atomicMax(&end[c], min(below[k], p.lengths[slots[k]]) / p.set.page_tokens);
   }

@@ -1,8 +1,8 @@
 """Pages of key-value caches that sequences share, on the device (``csrc/kernels/pages.cu``): a pool whose pages are taken, shared by forks, packed and given back by kernels,
 so that a step which forks its sequences needs no host and runs inside a CUDA graph, and copies of pages between caches.
 
-Where a call finds an index out of range, a slot named twice that it would write, or fewer free pages than it needs, it changes nothing and sets a bit of ``status``
-(:meth:`PagePool.check` raises for it); nothing waits for the host. Calls of one pool, and kernels that read or write its pages, are ordered by the caller: one stream, or
+Where a pool's call finds a slot or a length out of range, a slot named twice that it would give pages, or fewer free pages than it needs, it changes nothing and sets a bit of
+``status`` (:meth:`PagePool.check` raises for it); :func:`copy` skips what is out of range and copies the rest. Nothing waits for the host. Calls of one pool, and kernels that read or write its pages, are ordered by the caller: one stream, or
 events. ``runtime/paged_state.py`` is the other way to hold pages, with leases on the host."""
 from __future__ import annotations
 
@@ -134,7 +134,8 @@ class PagePool:
 
     def free(self, slots: torch.Tensor, below: Optional[torch.Tensor] = None) -> None:
         """All pages of the slots are given back, or with ``below`` the whole pages all of whose positions lie below ``below[i]`` (a window has passed them); those
-        entries of the table are -1 then. A page goes back to the pool when no other slot holds it."""
+        entries of the table are -1 then. A page goes back to the pool when no other slot holds it. A slot may be named more than once (the furthest ``below`` counts). All or
+        nothing: a list with a slot out of range or a negative ``below`` frees no page."""
         n = slots.numel()
         a, b = self.pages._list(slots, "slots", n), None if below is None else self.pages._list(below, "below", n)
         call_on(self.index, "ifab_pages_free", self.ref, a, b, n)

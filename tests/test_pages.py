@@ -301,3 +301,21 @@ def test_pages_beyond_4_gb_of_a_cache():
     assert bool((cache[0] == 3).all()) and bool((cache[1] == 5).all()) and bool((cache[2, :5] == 5).all())
     del cache, pool
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slots,below", [([-1], None), ([2, -1], [9, 9]), ([-1, -1], [5, 5]), ([-1] * 20, [5] * 20), ([0, 1, 0, -1], [9, 9, 9, 9]), ([0, 0, -1, -1, 0], None),
+                                         ([1, 6], None), ([2 ** 31 - 1, 1], [8, 8]), ([-2 ** 31, 1, -1, -2 ** 31], [8, 8, 8, 8]), ([1, 2], [8, -1]), ([3] * 9 + [-1], [8] * 10)])
+def test_free_refuses_a_bad_list_as_a_whole(slots, below):
+    """A slot out of range, or a negative position, wherever it stands in the list and however often: no page is given back, no length changes, and check says so once."""
+    pool, plain, before = _pool(40, 4, 6, 9, WIDTHS[0])
+    lists = ([0, 1, 2, 3], [22, 9, 36, 13])
+    pool.extend(*map(_list, lists))
+    plain.extend(*lists)
+    pool.free(_list(slots), None if below is None else _list(below))
+    _tell(pool, "index")
+    _same(pool, plain, before)
+    pool.free(_list([0, 1, 0]), _list([4, 9, 17]))
+    plain.free([0, 1, 0], [4, 9, 17])
+    _tell(pool, None)
+    _same(pool, plain, before)
