@@ -523,7 +523,7 @@ int ifab_int4_quantise(const IfabInt4* d, const void* w, long ldw, void* stream)
 int ifab_int4_pack(const IfabInt4* d, const uint8_t* codes, long ldc, const void* scales, const uint8_t* zeros, void* stream);
 int ifab_int4_dequantise(const IfabInt4* d, void* out, long ldo, void* stream);
 int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr, void* y, long ldy, int out_f32, int T,
-                   uint32_t* status, void* stream);
+                   uint32_t spin_limit, uint32_t* status, void* stream);
 int ifab_int4_gemm(const IfabInt4* d, const void* x, long ldx, const void* residual, long ldr, void* y, long ldy, int out_f32, int T, void* scratch,
                    uint32_t spin_limit, uint32_t* status, void* stream);
 uint64_t ifab_int4_gemm_scratch(int T, int K);

@@ -29,8 +29,8 @@ using namespace ifab::int4;
 
 namespace {
 
-constexpr int WARPS = 8;
-constexpr uint32_t POLLS = 4000000u;              // of a wait for a copy
+constexpr int WARPS = 8, BARS = 17, LEFT = 16 * 8;      // BARS: words of a warp's barriers; LEFT: bytes from the first of them to its limit
+constexpr uint32_t DRAIN = 4000000u;              // limit of the waits for copies that a CTA which gives up has requested
 
 struct RowsP {
   View v;
@@ -43,7 +43,7 @@ struct RowsP {
   int most;                      // tiles of a CTA, at most
   int depth;                     // stages of a ring
   int wide;                      // units of a run: 2 also where they are taken one by one (J 1), so that sums are added in the same order
-  uint32_t* status;
+  uint32_t* status; uint32_t spin_limit;
 };
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -106,14 +106,21 @@ __device__ __forceinline__ bool ready(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __noinline__ bool wait_more(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < POLLS; ++i) {
+// `left`: of the warp in shared memory, how many polls a wait may take; 0 once one ran out, and so nothing is waited for after it
+__device__ __noinline__ bool wait_more(uint32_t bar, uint32_t parity, uint32_t left) {
+  const uint32_t limit = lds4(left);
+  for (uint32_t i = 0; i < limit; ++i) {
     if (ready(bar, parity)) return true;
     if (i > 256) __nanosleep(64);
   }
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(left), "r"(0u) : "memory");
   return false;
 }
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) { return ready(bar, parity) || wait_more(bar, parity); }
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint32_t left) { return ready(bar, parity) || wait_more(bar, parity, left); }
+__device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < DRAIN && !ready(bar, parity); ++i)
+    if (i > 256) __nanosleep(64);
+}
 
 // the warps that multiply (the ninth one is at its copies)
 __device__ __forceinline__ void consumers() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
@@ -171,7 +178,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float sums[WARPS], inv[8];            // of a row's squares; the rows' factors
   __shared__ __align__(16) unsigned char runs_of_x[MR == 1 ? WARPS * 512 : 16];
-  __shared__ uint64_t bars[WARPS * 16];            // of a warp's stages: full, and eight further on empty
+  __shared__ uint64_t bars[WARPS * BARS];          // of a warp's stages: full, and eight further on empty; behind them the polls that its waits may take
   grid_dep_launch();
   const View& v = p.v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -188,20 +195,22 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
   };
   // sums: [warp][tile][rows of x by eight][lane], then the rings
   const uint32_t acc = smem_addr(smem) + (warp * p.most * NT * 32 + lane) * 16, rings = smem_addr(smem) + WARPS * p.most * NT * 512;
-  const uint32_t bar = smem_addr(bars + warp * 16);
+  const uint32_t bar = smem_addr(bars + warp * BARS);
 
   if (warp == WARPS && lane < WARPS) {
     for (int i = 0; i < p.depth; ++i) {
-      tc::mbar_init(bars + lane * 16 + i, 1);
-      tc::mbar_init(bars + lane * 16 + 8 + i, 1);
+      tc::mbar_init(bars + lane * BARS + i, 1);
+      tc::mbar_init(bars + lane * BARS + 8 + i, 1);
     }
+    *reinterpret_cast<uint32_t*>(bars + lane * BARS + 16) = p.spin_limit;
     tc::mbar_fence_init();
   }
   __syncthreads();
+  int requested = 0;                               // copies, of a lane of the ninth warp
   if (warp == WARPS) {
     // lane w requests the runs of warp w. Codes are written by no kernel of the stream: nothing to wait for
     if (lane < WARPS) {
-      const uint32_t ring = rings + lane * p.depth * J * UNIT, full = smem_addr(bars + lane * 16);
+      const uint32_t ring = rings + lane * p.depth * J * UNIT, full = smem_addr(bars + lane * BARS);
       const long row = (long)v.chunks * UNIT, up = (long)(v.tiles - mine) * row;      // from a tile to the next one, and to the first up tile besides
       int slot = 0, round = 0;
       bool ok = true;
@@ -210,11 +219,13 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
         const uint32_t bytes = J == 1 ? UNIT : min(J, chunk1 - rc) * UNIT;
         for (int i = 0; i < tiles; ++i, from += row) {
           if (gated && i == mine) from += up;
-          if (round && !wait_for(full + 64 + slot * 8, (round - 1) & 1)) { ok = false; break; }
+          // a warp that gave up gives its stages back all the same: nothing is requested into one whose last copy may not have landed
+          if (round && (!wait_for(full + 64 + slot * 8, (round - 1) & 1, full + LEFT) || !lds4(full + LEFT))) { ok = false; break; }
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + slot * 8), "r"(bytes) : "memory");
           asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * J * UNIT), "l"(from), "r"(bytes),
                        "r"(full + slot * 8)
                        : "memory");
+          ++requested;
           if (++slot == p.depth) slot = 0, ++round;
         }
       }
@@ -227,7 +238,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
   }
   grid_dep_wait();
 
-  bool late = false;
+  bool late = p.spin_limit == 0;
   if (warp < WARPS) {
     const uint32_t ring = rings + warp * p.depth * J * UNIT + code_at(g, c), meta = CODES + g * 4 - code_at(g, c), end = ring + p.depth * J * UNIT;
     uint32_t at = ring, stage = bar, parity = 0;   // the stage at hand: this lane's first codes, and its barrier
@@ -317,7 +328,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
       uint32_t to = acc;
 #pragma unroll 1
       for (int i = 0; i < tiles; ++i, to += NT * 512) {
-        late |= !wait_for(stage, parity);
+        late |= !wait_for(stage, parity, bar + LEFT);
         float4 so_far[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) so_far[n] = lds_f4(to + n * 512);
@@ -375,12 +386,16 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
       }
     }
   }
-  if (__any_sync(0xffffffffu, late)) {             // a copy that did not land: nothing of the tiles is right
+  if (warp < WARPS && __any_sync(0xffffffffu, late)) {             // a copy that did not land: nothing of the tiles is right
     if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
     const float nan = __int_as_float(0x7fffffff);
     for (int i = 0; i < tiles * NT; ++i) sts_f4(acc + i * 512, make_float4(nan, nan, nan, nan));
   }
-  __syncthreads();
+  if (__syncthreads_or(late)) {                    // what has been requested lands before its place is used for the sums below, or by another CTA
+    if (warp == WARPS && lane < WARPS)
+      for (int i = max(0, requested - p.depth); i < requested; ++i) drain(smem_addr(bars + lane * BARS + i % p.depth), (i / p.depth) & 1);
+    __syncthreads();
+  }
   // the warps' sums, added up into [tile][16][rows of x] in the place of the rings
   constexpr int W = 8 * NT;
   const float* red = reinterpret_cast<const float*>(smem);
@@ -472,8 +487,9 @@ int dispatch(const RowsP& p, cudaStream_t s) {
 }  // namespace
 
 // x [T, K] in bf16, rows on 16 bytes; norm_w: one to eight rows. The units are written by no kernel that may still run (ifab_int4_pack and ifab_int4_quantise see to it).
+// spin_limit: polls of a wait for a copy.
 extern "C" int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr, void* y, long ldy, int out_f32,
-                              int T, uint32_t* status, void* stream) {
+                              int T, uint32_t spin_limit, uint32_t* status, void* stream) {
   RowsP p{};
   if (view_of(d, &p.v) || T < 1 || !x || !y || ((uintptr_t)x | (uintptr_t)norm_w) % 16 || ldx % 8 || (norm_w && T > 8) || (p.v.halves == 2 && residual)) return -1;
   cudaStream_t s = (cudaStream_t)stream;
@@ -489,6 +505,7 @@ extern "C" int ifab_int4_rows(const IfabInt4* d, const void* x, long ldx, const 
     p.ldy = ldy;
     p.out_f32 = out_f32;
     p.status = status;
+    p.spin_limit = spin_limit;
     if (int rc = p.T <= 1 ? dispatch<1>(p, s) : p.T <= 8 ? dispatch<8>(p, s) : dispatch<16>(p, s)) return rc;
   }
   return 0;

@@ -56,7 +56,7 @@ _SIGS = {
     "ifab_int4_quantise": [_P, _P, c_long, _P],
     "ifab_int4_pack": [_P, _P, c_long, _P, _P, _P],
     "ifab_int4_dequantise": [_P, _P, c_long, _P],
-    "ifab_int4_rows": [_P, _P, c_long, _P, c_float, _P, c_long, _P, c_long, c_int, c_int, _P, _P],
+    "ifab_int4_rows": [_P, _P, c_long, _P, c_float, _P, c_long, _P, c_long, c_int, c_int, c_uint, _P, _P],
     "ifab_int4_gemm": [_P, _P, c_long, _P, c_long, _P, c_long, c_int, c_int, _P, c_uint, _P, _P],
     "ifab_pages_copy": [_P, _P, _P, _P, _P, c_int, _P, _P],
     "ifab_pages_extend": [_P, _P, _P, c_int, _P],

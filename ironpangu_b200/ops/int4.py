@@ -136,7 +136,8 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
         scratch = torch.empty(lib.ifab_int4_gemm_scratch(T, k), dtype=torch.uint8, device=w.device)
         check(lib.ifab_int4_gemm(w.ref, xp, ldx, rp, ldr, yp, ldy, f32, T, scratch.data_ptr(), SPIN_LIMIT, status_ptr, _lib.current_stream(dev)), "int4.linear")
         return out
-    check(lib.ifab_int4_rows(w.ref, xp, ldx, None if norm_w is None else norm_w.data_ptr(), eps, rp, ldr, yp, ldy, f32, T, status_ptr, _lib.current_stream(dev)), "int4.linear")
+    check(lib.ifab_int4_rows(w.ref, xp, ldx, None if norm_w is None else norm_w.data_ptr(), eps, rp, ldr, yp, ldy, f32, T, SPIN_LIMIT, status_ptr, _lib.current_stream(dev)),
+          "int4.linear")
     return out
 
 

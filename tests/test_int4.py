@@ -338,3 +338,23 @@ def test_weights_on_the_host_multiply_nothing():
 
     with pytest.raises(ValueError, match="on the host"):
         int4.linear(torch.zeros(1, 64, dtype=BF16), int4.Int4Weight(16, 64, device="cpu"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,K,norm,gated", [(1, 64, 1024, False, False), (1, 9000, 4104, True, True), (3, 300, 16392, False, False), (8, 30000, 2056, True, False), (16, 5000, 9000, False, True), (11, 100, 520, False, False)])
+def test_a_copy_that_does_not_land_in_time(T, N, K, norm, gated):
+    """Few rows, with a limit of no polls: every warp gives up at its first wait, the copies under way are waited for, the status word says so, the result is NaN and the next
+    call is right."""
+    from ironpangu_b200.ops import _lib, int4
+
+    q, s, z = _codes(N * (1 + gated), K, 32, True, 1)
+    w, x, gain = int4.pack(q, s, z, group=32, gated=gated), _rows(T, K, 1).contiguous(), torch.ones(K, dtype=BF16, device="cuda")
+    want = int4.linear(x, w, norm_w=gain if norm else None)
+    for _ in range(3):
+        status, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(T, N, dtype=BF16, device="cuda")
+        _lib.check(_lib.load().ifab_int4_rows(w.ref, x.data_ptr(), K, gain.data_ptr() if norm else None, 1e-5, None, 0, out.data_ptr(), N, 0, T, 0, status.data_ptr(),
+                                              torch.cuda.current_stream().cuda_stream), "rows")
+        torch.cuda.synchronize()
+        assert int(status) == 2 and bool(out.isnan().all())
+        status.zero_()
+        assert torch.equal(int4.linear(x, w, norm_w=gain if norm else None, status_ptr=status.data_ptr()), want) and int(status) == 0
