@@ -343,6 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       __syncwarp();
       if (ok && lane == 0) arrive_cluster(in_leader(&acc_empty[j & 1]));
     }
+    if (rank == 1 && warp == 11) mbar_wait(drained, 0, DRAIN);      // the last of what the leader signals to this CTA, which must not end ahead of it
   }
   __syncwarp();
   tc_fence_before();

@@ -358,3 +358,23 @@ def test_a_copy_that_does_not_land_in_time(T, N, K, norm, gated):
         assert int(status) == 2 and bool(out.isnan().all())
         status.zero_()
         assert torch.equal(int4.linear(x, w, norm_w=gain if norm else None, status_ptr=status.data_ptr()), want) and int(status) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,gated", [(1300, 4100, False), (1300, 2052, True), (700, 9500, False)])
+def test_launches_right_behind_one_that_gave_up(T, N, gated):
+    """Pairs of SMs whose waits run out, and products of other rows behind them without the host between: nothing that was signalled or copied for the first meets the second."""
+    from ironpangu_b200.ops import _lib, int4
+
+    K = 1160
+    q, s, z = _codes(N * (1 + gated), K, 64, True, 1)
+    w, x, few = int4.pack(q, s, z, group=64, gated=gated), _rows(T, K, 1).contiguous(), _rows(200, K, 2).contiguous()
+    want, want_few = int4.linear(x, w), int4.linear(few, w)
+    scratch = torch.empty(_lib.load().ifab_int4_gemm_scratch(T, K), dtype=torch.uint8, device="cuda")
+    status, out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(T, N, dtype=BF16, device="cuda")
+    for _ in range(3):
+        _lib.check(_lib.load().ifab_int4_gemm(w.ref, x.data_ptr(), K, None, 0, out.data_ptr(), N, 0, T, scratch.data_ptr(), 0, status.data_ptr(),
+                                              torch.cuda.current_stream().cuda_stream), "gemm")
+        a, b = int4.linear(few, w), int4.linear(x, w)
+        assert torch.equal(a, want_few) and torch.equal(b, want) and int(status) == 2 and bool(out.isnan().all())
+        status.zero_()
