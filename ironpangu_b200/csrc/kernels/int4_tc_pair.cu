@@ -37,6 +37,7 @@ constexpr uint32_t SUM_COLS = 256;                   // of tensor memory
 // it, whose own stage, and chunk of codes, were done with before.
 static_assert(STAGES >= 5 && 2 * CHUNKS >= STAGES + 5, "a group could take a phase for the one two ahead");
 constexpr uint32_t DRAIN = 4000000u;                 // limit of the waits for what a CTA that gives up has started
+constexpr int QUIET = 2000;
 constexpr int RASTER = 8;                            // token tiles that pairs share weights over
 
 struct PairP {
@@ -236,8 +237,15 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
     }
     if (!ok) {
       *abort_flag = 1;
-      if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+      if (lane == 0) {
+        uint32_t peers;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(peers) : "r"(smem_u32(const_cast<int*>(abort_flag))));
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peers), "r"(1) : "memory");
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        if (p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
+      }
     }
+    __syncwarp();
     // whoever gives up: products that were issued end before the CTAs do
     if (elected) commit_pair(drained);
     mbar_wait(drained, 0, DRAIN);
@@ -346,6 +354,12 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
     if (rank == 1 && warp == 11) mbar_wait(drained, 0, DRAIN);      // the last of what the leader signals to this CTA, which must not end ahead of it
   }
   __syncwarp();
+  if (rank == 1) {
+    // Where either CTA gave up, tokens that this one requested may still be under way, and their bytes count on the leader's barrier, in phases that may never end: they get
+    // QUIET microseconds, a thousand times what a copy takes
+    if (__syncthreads_or(*abort_flag) && warp == 0)
+      for (int i = 0; i < QUIET; ++i) __nanosleep(1000);
+  }
   tc_fence_before();
   __syncthreads();
   cluster_barrier();
