@@ -132,6 +132,27 @@ __device__ __forceinline__ void store16(float (&f)[16], float out, float factor,
   }
 }
 
+// What lies behind the rings in shared memory
+struct Signals {
+  uint64_t full[STAGES];                             // leader's: both halves of the tokens, and an arrival of every warp that wrote weights
+  uint64_t empty[STAGES];                            // each CTA's own, as acc_full
+  uint64_t acc_full[2], acc_empty[2];                // of each sum; acc_empty: leader's
+  uint64_t units_full[CHUNKS], units_empty[CHUNKS];  // each CTA's own
+  uint64_t drained;
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+// The second CTA, all threads: behind the last of what the leader signals to it. Where either gave up, tokens that it requested may still be under way, and their bytes count on
+// the leader's barrier, in phases that may never end: they get QUIET microseconds, a thousand times what a copy takes. (A call, as its addresses spill where it is not: 4096 rows
+// of 2 x 16384 by 4096 928 us with it, 957 without.)
+__device__ __noinline__ void second_ends(int units) {
+  extern __shared__ unsigned char smem_raw[];
+  Signals* s = reinterpret_cast<Signals*>(((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023) + STAGES * STAGE + units);
+  if (threadIdx.x < 32) mbar_wait(&s->drained, 0, DRAIN);
+  if (__syncthreads_or(*(volatile int*)&s->abort_flag) && threadIdx.x < 32)
+    for (int i = 0; i < QUIET; ++i) __nanosleep(1000);
+}
+
 // grid (2 * pairs), clusters of 2
 template <int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, PairP p) {
@@ -139,13 +160,11 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* ring = smem + STAGES * STAGE;                               // chunks of units
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + CHUNKS * U::BYTES);    // leader's: both halves of the tokens, and an arrival of every warp that wrote weights
-  uint64_t* empty = full + STAGES;                                           // each CTA's own, as acc_full
-  uint64_t *acc_full = empty + STAGES, *acc_empty = acc_full + 2;            // of each sum; acc_empty: leader's
-  uint64_t *units_full = acc_empty + 2, *units_empty = units_full + CHUNKS;   // each CTA's own
-  uint64_t* drained = units_empty + CHUNKS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  Signals& sig = *reinterpret_cast<Signals*>(ring + CHUNKS * U::BYTES);
+  uint64_t *full = sig.full, *empty = sig.empty, *acc_full = sig.acc_full, *acc_empty = sig.acc_empty, *units_full = sig.units_full, *units_empty = sig.units_empty;
+  uint64_t* drained = &sig.drained;
+  uint32_t* tmem_slot = &sig.tmem_slot;
+  volatile int* abort_flag = &sig.abort_flag;
   const View& v = p.v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -351,15 +370,9 @@ __global__ void __launch_bounds__(THREADS, 1) int4_tc_pair_kernel(const __grid_c
       __syncwarp();
       if (ok && lane == 0) arrive_cluster(in_leader(&acc_empty[j & 1]));
     }
-    if (rank == 1 && warp == 11) mbar_wait(drained, 0, DRAIN);      // the last of what the leader signals to this CTA, which must not end ahead of it
   }
   __syncwarp();
-  if (rank == 1) {
-    // Where either CTA gave up, tokens that this one requested may still be under way, and their bytes count on the leader's barrier, in phases that may never end: they get
-    // QUIET microseconds, a thousand times what a copy takes
-    if (__syncthreads_or(*abort_flag) && warp == 0)
-      for (int i = 0; i < QUIET; ++i) __nanosleep(1000);
-  }
+  if (cluster_rank() == 1) second_ends(CHUNKS * U::BYTES);
   tc_fence_before();
   __syncthreads();
   cluster_barrier();
