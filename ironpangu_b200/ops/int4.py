@@ -58,6 +58,7 @@ class Int4Weight:
 
     def dequantise(self, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The weights' values ``[rows, k]``, rounded to bf16."""
+        _need(self.index >= 0, "the weights are on the host")
         if out is None:
             out = torch.empty(self.rows, self.k, dtype=BF16, device=self.device)
         _need(out.shape == (self.rows, self.k) and out.dtype == BF16 and out.stride(1) == 1 and out.device == self.device, "the output must be bf16 [rows, k] beside the weights")

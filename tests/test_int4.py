@@ -378,3 +378,12 @@ def test_launches_right_behind_one_that_gave_up(T, N, gated):
         a, b = int4.linear(few, w), int4.linear(x, w)
         assert torch.equal(a, want_few) and torch.equal(b, want) and int(status) == 2 and bool(out.isnan().all())
         status.zero_()
+
+
+def test_weights_on_the_host_have_no_values():
+    from ironpangu_b200.ops import int4
+
+    w = int4.Int4Weight(16, 64, device="cpu")
+    for out in (None, torch.zeros(16, 64, dtype=BF16)):
+        with pytest.raises(ValueError, match="on the host"):
+            w.dequantise(out)
