@@ -467,7 +467,8 @@ __global__ void __launch_bounds__(256) compact_kernel(Pool q) {
 
 bool good_set(const IfabPageSet* s) { return s && s->ptrs && s->row_bytes && s->caches > 0 && s->pages > 0 && s->page_tokens > 0; }
 bool good_pool(const IfabPagePool* p) {
-  return p && good_set(&p->set) && p->table && p->lengths && p->refs && p->free_bits && p->work && p->slots > 0 && p->slots <= MAX_SLOTS && p->max_pages > 0;
+  return p && good_set(&p->set) && p->table && p->lengths && p->refs && p->free_bits && p->work && p->slots > 0 && p->slots <= MAX_SLOTS && p->max_pages > 0 &&
+         (p->max_pages + 1l) * p->set.page_tokens < 1l << 31 && (long)p->slots * p->max_pages < 1l << 31;      // positions and entries are counted in 32 bits
 }
 int grid_of(long items) { return (int)std::min<long>(std::max<long>(items, 1), 8l * tc::device_sms()); }
 // CTAs that share a row by `entries` entries each, as long as they all run at once

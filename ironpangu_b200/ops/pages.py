@@ -89,7 +89,9 @@ class PagePool:
 
     def __init__(self, caches: List[torch.Tensor], *, slots: int, max_pages: int):
         self.pages = s = PageSet(caches)
-        _need(1 <= slots <= MAX_SLOTS and max_pages >= 1 and (max_pages + 1) * s.page_tokens < 1 << 31, f"{slots} slots of {max_pages} pages are not supported")
+        # positions, and the table's entries, are counted in 32 bits
+        _need(1 <= slots <= MAX_SLOTS and max_pages >= 1 and (max_pages + 1) * s.page_tokens < 1 << 31 and slots * max_pages < 1 << 31,
+              f"{slots} slots of {max_pages} pages are not supported")
         self.slots, self.max_pages, self.page_tokens, self.device = slots, max_pages, s.page_tokens, s.device
         self.index = s.index
         i32 = lambda *shape, v=0: torch.full(shape, v, dtype=I32, device=s.device)

@@ -319,3 +319,24 @@ def test_free_refuses_a_bad_list_as_a_whole(slots, below):
     plain.free([0, 1, 0], [4, 9, 17])
     _tell(pool, None)
     _same(pool, plain, before)
+
+
+@pytest.mark.gpu
+def test_entries_of_a_table_fit_32_bits():
+    from ironpangu_b200.ops import _lib, pages as P
+
+    cache = torch.zeros(2, 1, 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="not supported"):
+        P.PagePool([cache], slots=8192, max_pages=1 << 18)
+    pool = P.PagePool([cache], slots=2, max_pages=2)
+    i32 = lambda v: torch.tensor([v], dtype=I32, device="cuda")
+    where = [i32(0), i32(1)]
+    for slots, most in ((8192, 1 << 18), (1, (1 << 31) - 1)):          # nothing is launched for a pool that the kernels cannot count
+        pool.desc.slots, pool.desc.max_pages = slots, most
+        for call, args in (("extend", where), ("fork", where), ("free", where[:1]), ("compact", ())):
+            with pytest.raises(RuntimeError):
+                getattr(pool, call)(*args)
+    pool.desc.slots, pool.desc.max_pages = 2, 2
+    pool.extend(*where)
+    pool.check()
+    assert pool.table.tolist() == [[0, -1], [-1, -1]]
