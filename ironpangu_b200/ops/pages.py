@@ -107,13 +107,14 @@ class PagePool:
         self.ref = C.byref(self.desc)
 
     def check(self) -> None:
-        """Raises when a call was refused on the device since the last check (waits for the device): OverflowError where pages lacked, IndexError where a list named a slot
-        out of range, a slot twice or a length that no slot can hold."""
+        """Raises when a call was refused on the device since the last check (waits for the device): IndexError where a list named a slot out of range, a slot twice or a length
+        that no slot can hold, OverflowError where pages lacked (where both happened, the next check raises for the other)."""
         bits = int(self.status)
+        if bits & BAD_INDEX:
+            self.status.bitwise_and_(~BAD_INDEX)
+            raise IndexError("pages: a list of slots named one out of range or twice, or a length that no slot can hold")
         if bits:
             self.status.zero_()
-            if bits & BAD_INDEX:
-                raise IndexError("pages: a list of slots named one out of range or twice, or a length that no slot can hold")
             raise OverflowError("pages: the pool had fewer free pages than a call needed")
 
     def extend(self, slots: torch.Tensor, tokens: torch.Tensor) -> None:

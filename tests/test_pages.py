@@ -340,3 +340,15 @@ def test_entries_of_a_table_fit_32_bits():
     pool.extend(*where)
     pool.check()
     assert pool.table.tolist() == [[0, -1], [-1, -1]]
+
+
+@pytest.mark.gpu
+def test_check_raises_for_every_kind_of_refusal():
+    """A bad list and a lack of pages between two checks: neither hides the other, whichever came first."""
+    for calls in (([0, 0], [4]), ([4], [0, 0])):
+        pool, plain, before = _pool(3, 4, 5, 6, WIDTHS[0])
+        for pick in calls:
+            pool.extend(_list(pick), _list([17] * len(pick)))
+        _ = [pytest.raises(e, pool.check) for e in (IndexError, OverflowError)]
+        _tell(pool, None)
+        _same(pool, plain, before)
