@@ -37,10 +37,12 @@ class Continuations:
         self._store = P.PageSet(self.store) if store_pages else None
         self._store_free = list(range(store_pages))[::-1]
         self._aside = {}                      # continuations that were set aside: their pages in the second pool
+        self._ran = self._broken = False      # there was a run, whose reports may still lie in the status words; the continuations are not what their tokens say
 
     # -- prompt --------------------------------------------------------------------------------------------------------------
     def start(self, prompt: Sequence[int], n: int, *, temperature: float = 1.0, top_k: int = 50, top_p: float = 1.0, seed: int = 0) -> torch.Tensor:
-        """Runs the prompt, forks it ``n`` times and samples the first token of each continuation (device tensor ``[n]``). ``temperature`` 0: greedy."""
+        """Runs the prompt, forks it ``n`` times and samples the first token of each continuation (device tensor ``[n]``). ``temperature`` 0: greedy. Continuations that were
+        there are ended first, and nothing that :meth:`check` would have said about them is said any more. Where this raises there are none."""
         d = self.dec
         if not 1 <= n <= self.width:
             raise ValueError(f"{n} continuations: this decoder takes 1 to {self.width}")
@@ -49,7 +51,23 @@ class Continuations:
         if not 1 <= top_k <= 64:
             raise ValueError(f"top_k of {top_k}: 1 to 64")
         self.end()
-        self.n, self.length, self.top_k = n, len(prompt), 1 if temperature <= 0 else top_k
+        if self._ran:
+            self.pool.status.zero_()
+            if d.fabric.status():             # (waits for the kernels that may still set it)
+                d.fabric.clear_status()
+        self._ran = True
+        try:
+            self._begin(prompt, n, temperature, top_k, top_p, seed)
+            self.check()
+        except BaseException:
+            self._release()
+            raise
+        self.n, self.length = n, len(prompt)
+        return self.ids[:n]
+
+    def _begin(self, prompt: Sequence[int], n: int, temperature: float, top_k: int, top_p: float, seed: int) -> None:
+        d = self.dec
+        self.top_k = 1 if temperature <= 0 else top_k
         self.inv_temp[:n].fill_(1e4 if temperature <= 0 else 1.0 / temperature)
         self.top_p[:n].fill_(1.0 if temperature <= 0 else top_p)
         self.seeds[:n].copy_(torch.arange(n, dtype=torch.int64) + seed * 0x9E3779B1)
@@ -77,10 +95,8 @@ class Continuations:
         if n > 1:
             d.logits[1:n].copy_(d.logits[:1].expand(n - 1, -1))
         self._sample(n)
-        d.positions[:n].fill_(self.length)
+        d.positions[:n].fill_(len(prompt))
         d.slots[:n].copy_(self._children[:n])
-        self.pool.check()
-        return self.ids[:n]
 
     def _sample(self, n: int) -> None:
         d = self.dec
@@ -98,7 +114,8 @@ class Continuations:
         d.positions[:n].add_(1)
 
     def step(self) -> torch.Tensor:
-        """The next token of every continuation (device tensor ``[n]``): one graph replay. A pool that has run out of pages shows in :meth:`check`."""
+        """The next token of every continuation (device tensor ``[n]``): one graph replay. A pool that has run out of pages shows in :meth:`check`, and the tokens since the check
+        before it are not to be used then."""
         self._all_here()
         if self.length >= self.dec.max_context:
             raise OverflowError("the continuations run past the context")
@@ -117,17 +134,32 @@ class Continuations:
         return self.ids[:self.n]
 
     def _all_here(self) -> None:
-        if not self.n:
-            raise RuntimeError("no continuations: start() first")
+        self._sound()
         if self._aside:
             raise RuntimeError(f"continuations {sorted(self._aside)} are set aside: take_up() first")
 
+    def _sound(self) -> None:
+        if not self.n:
+            raise RuntimeError("no continuations: start() first")
+        if self._broken:
+            raise RuntimeError("a step was refused: the continuations have to be ended")
+
     def check(self) -> None:
-        """Raises IndexError when a resampling named a parent out of range (nothing was resampled then), OverflowError when a step found too few free pages (its tokens are not to be used)."""
-        self.pool.check()
+        """Raises IndexError when a resampling named a parent out of range (nothing was resampled then), OverflowError when a step or a resampling found too few free pages,
+        RuntimeError when a kernel gave up or met an index out of range. After the latter two the continuations are not what their tokens say - positions whose keys and values
+        were never written - and nothing but :meth:`end` and :meth:`start` takes them (waits for the device)."""
+        if self._broken:
+            self._sound()
+        lacked, word = int(self.pool.status) & P.NO_PAGES, self.dec.fabric.status()
+        self._broken = bool(lacked or word)
+        if word:
+            self.dec.fabric.clear_status()
+        self.pool.check()                     # (pages that lacked are what kernels reported as out of range)
+        if word:
+            raise RuntimeError(f"continuations: kernel status word = {word}")
 
     def resample(self, parents: torch.Tensor) -> None:
-        """Continuation ``i`` goes on from what ``parents[i]`` is now (int32 ``[n]`` on the device, out of 0 .. n - 1, with repeats)."""
+        """Continuation ``i`` goes on from what ``parents[i]`` is now (int32 ``[n]`` on the device, out of 0 .. n - 1, with repeats). What is refused shows in :meth:`check`."""
         self._all_here()
         n = self.n
         if parents.shape != (n,) or parents.dtype != I32:
@@ -140,11 +172,15 @@ class Continuations:
     def end(self) -> None:
         """Gives back all pages, those that were set aside among them."""
         if self.n:
-            self.pool.free(self._children)
-            self.pool.free(self._first)
+            self._release()
+
+    def _release(self) -> None:
+        self.pool.free(self._children)
+        self.pool.free(self._first)
         for ids in self._aside.values():
             self._store_free += ids.tolist()
         self._aside = {}
+        self._broken = False
         self.n = self.length = 0
 
     # -- setting aside ---------------------------------------------------------------------------------------------------------
@@ -152,7 +188,11 @@ class Continuations:
         """Copies continuation ``i`` to the second pool and gives its pages back; :meth:`take_up` brings it back from what this returns, and no step can be taken before."""
         if not 0 <= i < self.n or i in self._aside:
             raise ValueError(f"no continuation {i}")
+        self._sound()
         length = int(self.pool.lengths[1 + i])
+        if length != self.length:             # a step was refused
+            self.check()
+            raise RuntimeError(f"continuation {i} holds {length} positions of {self.length}")
         count = -(-length // self.pool.page_tokens)
         if count > len(self._store_free):
             raise OverflowError(f"{count} pages to set aside, {len(self._store_free)} free")
@@ -165,10 +205,11 @@ class Continuations:
         return ids, rows
 
     def take_up(self, i: int, held: Tuple[torch.Tensor, torch.Tensor]) -> None:
-        """Continuation ``i``, which was set aside, has its pages again."""
+        """Continuation ``i``, which was set aside, has its pages again. OverflowError where pages lack: nothing has changed then, and it can be asked for again."""
         ids, rows = held
         if self._aside.get(i) is not ids:
             raise ValueError(f"this is not what continuation {i} was set aside as")
+        self.check()
         count = ids.numel()
         length = (count - 1) * self.pool.page_tokens + rows[-1:] if count else torch.zeros(1, dtype=I32, device=ids.device)
         self.pool.extend(self._children[i:i + 1], length.to(I32))
