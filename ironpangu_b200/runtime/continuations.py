@@ -224,11 +224,15 @@ class Continuations:
         return int(self.pool.live)
 
     def generate(self, prompt: Sequence[int], n: int, max_new_tokens: int, eos: int = -1, **sampling) -> List[List[int]]:
-        """``n`` continuations of up to ``max_new_tokens`` tokens, each cut off behind its first ``eos``."""
-        steps = [self.start(prompt, n, **sampling).clone()]
-        for _ in range(max_new_tokens - 1):
-            steps.append(self.step().clone())
-        self.check()
-        rows = torch.stack(steps, 1).tolist()
-        self.end()
+        """``n`` continuations of up to ``max_new_tokens`` tokens, each cut off behind its first ``eos``. Ended also where this raises."""
+        if max_new_tokens < 1:
+            raise ValueError(f"{max_new_tokens} tokens: at least one")
+        try:
+            steps = [self.start(prompt, n, **sampling).clone()]
+            for _ in range(max_new_tokens - 1):
+                steps.append(self.step().clone())
+            self.check()
+            rows = torch.stack(steps, 1).tolist()
+        finally:
+            self.end()
         return [r[:r.index(eos) + 1] if eos in r else r for r in rows]

@@ -162,6 +162,15 @@ def test_kernels_that_gave_up_show(faked):
     c.check()
 
 
+def test_generate_ends_what_it_started(faked):
+    for pages, length, tokens, error in ((12, 30, 40, OverflowError), (1000, 190, 20, OverflowError), (1000, 20, 0, ValueError), (1000, 20, -3, ValueError)):
+        c = faked(pages)
+        with pytest.raises(error):                 # no pages; past the context; no tokens wanted
+            c.generate(list(range(length)), 4, tokens)
+        assert c.n == 0 and int(c.pool.lengths.sum()) == 0
+        assert c.generate(list(range(20)), 2, 3) == [[1, 1, 1]] * 2 and c.generate(list(range(20)), 2, 1) == [[1]] * 2
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("int4", [False, True])
 def test_on_the_device(int4):
