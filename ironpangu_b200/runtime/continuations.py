@@ -70,7 +70,8 @@ class Continuations:
         self.top_k = 1 if temperature <= 0 else top_k
         self.inv_temp[:n].fill_(1e4 if temperature <= 0 else 1.0 / temperature)
         self.top_p[:n].fill_(1.0 if temperature <= 0 else top_p)
-        self.seeds[:n].copy_(torch.arange(n, dtype=torch.int64) + seed * 0x9E3779B1)
+        first = (seed * 0x9E3779B1 + (1 << 63)) % (1 << 64) - (1 << 63)      # of 64 bits, as any seed is
+        self.seeds[:n].copy_(torch.arange(n, dtype=torch.int64) + first)
         self.counters.zero_()
         self._tokens.fill_(len(prompt))
         self.pool.extend(self._first, self._tokens)

@@ -171,6 +171,13 @@ def test_generate_ends_what_it_started(faked):
         assert c.generate(list(range(20)), 2, 3) == [[1, 1, 1]] * 2 and c.generate(list(range(20)), 2, 1) == [[1]] * 2
 
 
+def test_seeds_of_any_size(faked):
+    c = faked(100)
+    for seed in (0, 5, -7, (1 << 32) - 1, 1 << 32, (1 << 63) - 1, (1 << 64) - 1, -(1 << 63), 1 << 100):
+        c.start([1, 2, 3], 4, seed=seed)
+        assert [int(v) % (1 << 64) for v in c.seeds] == [(seed * 0x9E3779B1 + i) % (1 << 64) for i in range(4)]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("int4", [False, True])
 def test_on_the_device(int4):
