@@ -228,8 +228,9 @@ class Continuations:
         """``n`` continuations of up to ``max_new_tokens`` tokens, each cut off behind its first ``eos``. Ended also where this raises."""
         if max_new_tokens < 1:
             raise ValueError(f"{max_new_tokens} tokens: at least one")
+        first = self.start(prompt, n, **sampling)
         try:
-            steps = [self.start(prompt, n, **sampling).clone()]
+            steps = [first.clone()]
             for _ in range(max_new_tokens - 1):
                 steps.append(self.step().clone())
             self.check()

@@ -171,6 +171,17 @@ def test_generate_ends_what_it_started(faked):
         assert c.generate(list(range(20)), 2, 3) == [[1, 1, 1]] * 2 and c.generate(list(range(20)), 2, 1) == [[1]] * 2
 
 
+def test_generate_refused_for_its_arguments_ends_nothing(faked):
+    c = faked(100)
+    c.start(list(range(20)), 2)
+    for args in (([], 2, 3), ([1], 9, 3), ([1], 2, 0)):
+        with pytest.raises(ValueError):
+            c.generate(*args)
+    assert c.n == 2
+    c.step()
+    c.check()
+
+
 def test_seeds_of_any_size(faked):
     c = faked(100)
     for seed in (0, 5, -7, (1 << 32) - 1, 1 << 32, (1 << 63) - 1, (1 << 64) - 1, -(1 << 63), 1 << 100):
