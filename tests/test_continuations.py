@@ -193,3 +193,57 @@ def test_parents_out_of_range_change_nothing():
     c.check()
     assert torch.equal(dec.tokens[:3], tokens[:3][[2, 2, 0]])
     fab.close()
+
+
+@pytest.mark.parametrize("int4", [False, True])
+@pytest.mark.parametrize("length,prompt_kernels", [(1, False), (15, False), (16, True), (37, True)])
+def test_logits_are_those_of_sequences_that_share_nothing(int4, length, prompt_kernels):
+    """Every step's logits, bit for bit, against a decoder whose slots have pages of their own and which runs the same launches with the tokens that were drawn: over ends of pages,
+    draws with repeats (whose caches are copied whole there), packing, and a continuation that was away."""
+    from ironpangu_b200.models.dense_prefill import DensePrefill
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    n = 4
+    cfg, fab, dec = _decoder(int4)
+    _, _, own = _decoder(int4, pool=False)
+    pre = [DensePrefill(d, max_rows=24, attn_rows=32) if prompt_kernels else None for d in (dec, own)]
+    c = Continuations(dec, prefill=pre[0], store_pages=8)
+    prompt = torch.randint(0, cfg.vocab, (length,), generator=torch.Generator().manual_seed(length)).to(I32)
+    tokens = c.start(prompt.tolist(), n, temperature=1.2, top_k=40, seed=9).clone()
+    for slot in range(1, n + 1):                      # the prompt, in each slot
+        for p in range(0, length, 24 if prompt_kernels else own.T):
+            part = prompt[p:p + (24 if prompt_kernels else own.T)].cuda()
+            if prompt_kernels:
+                pre[1].forward(part, p, slot)
+            else:
+                m = part.numel()
+                own.tokens[:m].copy_(part)
+                own.positions[:m].copy_(torch.arange(p, p + m, dtype=I32))
+                own.slots[:m].fill_(slot)
+                own.forward(m)
+        last = 0 if prompt_kernels else part.numel() - 1
+        assert torch.equal(own.logits[last], dec.logits[slot - 1])
+    parents = {3: [1, 1, 3, 0], 18: [2, 2, 2, 2], 33: [3, 0, 1, 0]}
+    for k in range(40):
+        own.tokens[:n].copy_(tokens)
+        own.positions[:n].fill_(length + k)
+        own.slots[:n].copy_(torch.arange(1, n + 1, dtype=I32))
+        own.forward(n)
+        want = own.logits[:n].clone()
+        tokens = c.step().clone()
+        assert torch.equal(dec.logits[:n], want), k
+        if k in parents:
+            at = torch.tensor(parents[k], device="cuda")
+            c.resample(at.to(I32))
+            tokens = tokens[at]
+            of = own.page_table.long()
+            for t in own.k_cache + own.v_cache:
+                t[of[1:n + 1]] = t[of[1 + at]]
+        if k % 10 == 4:
+            c.pack()
+        if k % 10 == 7:
+            c.take_up(2, c.set_aside(2))
+    c.check()
+    c.end()
+    assert int(dec.pool.refs.sum()) == 0 and own.fabric.status() == 0
+    fab.close()
