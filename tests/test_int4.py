@@ -387,3 +387,44 @@ def test_weights_on_the_host_have_no_values():
     for out in (None, torch.zeros(16, 64, dtype=BF16)):
         with pytest.raises(ValueError, match="on the host"):
             w.dequantise(out)
+
+
+EXACT = [(200, 16392, 1), (333, 9000, 3), (64, 16392, 8), (48, 9000, 16), (130, 9000, 17), (333, 9000, 40), (1237, 4104, 64), (300, 16392, 129), (129, 4096, 255), (1000, 9000, 300), (2741, 4104, 700),
+         (9500, 4104, 300), (5000, 2056, 1101)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,zeros", [(128, True), (64, False), (32, True)])
+@pytest.mark.parametrize("N,K,T", EXACT)
+def test_sums_without_any_rounding(N, K, T, group, zeros):
+    """Small integers and scales of 1/2, 1 and 2: products are multiples of 1/2 and the sums of their magnitudes stay below 16392 x 4 x 31 x 2 < 2^22 (with the offset of 16 that up
+    to sixteen rows have), so every order of f32 sums is exact, and a column that is left out, taken twice or met by another's weight shows."""
+    from ironpangu_b200.ops import int4
+
+    g = torch.Generator(device="cuda").manual_seed(N + K + T)
+    q, s, z = _codes(N, K, group, zeros, N + K)
+    s = torch.exp2(torch.randint(-1, 2, s.shape, generator=g, device="cuda").float()).to(BF16)
+    x = torch.randint(-4, 5, (T, K + 8), generator=g, device="cuda").to(BF16)[:, :K]
+    want = x.double() @ _values(q, s, z, group).T
+    assert torch.equal(int4.linear(x, int4.pack(q, s, z, group=group), out_f32=True).double(), want)
+    if N % 2 == 0:
+        y = int4.linear(x, int4.pack(q, s, z, group=group, gated=True), out_f32=True).double()
+        gate, up = want[:, :N // 2], want[:, N // 2:]
+        unit = gate * torch.sigmoid(gate) * up
+        # CUDA's fast exponential is documented to be off by up to 2 + floor(1.173 |a|) steps of f32, 2^-23 of it each; 1 + it, the quotient or reciprocal and two products take
+        # six more at most. Below e^-87 the unit is less than 87 e^-87 2^19 < 1e-30
+        steps = 8 + 1.173 * gate.abs().clamp(max=90)
+        assert bool(((y - unit).abs() <= 2.0 ** -23 * steps * unit.abs() + 1e-30).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,zeros,f16", [(128, False, False), (64, True, True), (32, True, False)])
+@pytest.mark.parametrize("N,K,T", [(333, 520, 17), (130, 9000, 40), (1237, 1032, 129), (129, 4096, 255), (5000, 520, 700), (2741, 1032, 1501)])
+def test_many_rows_against_the_matrix_that_was_packed(N, K, T, group, zeros, f16):
+    """Without the rounding of weights in the reference: half a step of f16, 2^-11 of a weight, beside the bound of the sums."""
+    from ironpangu_b200.ops import int4
+
+    q, s, z = _codes(N, K, group, zeros, N + K, f16)
+    x, v = _rows(T, K, T), _values(q, s, z, group)
+    bound = _operands(v, x)[1] + 2.0 ** -11 * (x.double().abs() @ v.abs().T)
+    _close(int4.linear(x, int4.pack(q, s, z, group=group), out_f32=True), x.double() @ v.T, bound)
