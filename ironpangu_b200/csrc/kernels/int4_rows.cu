@@ -4,7 +4,7 @@
 // A code q goes into the upper mantissa bits of a bf16 whose exponent makes it 16 + q, two codes in a rotation and a logical operation; weights are the sixteen rows of A of
 // an m16n8k16, rows of x the eight columns of B, and what the offset and the zero point add to a group's sum, (16 + z) times the sum of x, is where that sum starts from
 // (with the opposite sign). The sums of x come out of products with ones, once for all tiles of a CTA. The group's scale multiplies its f32 sum. Products are exact; sums run
-// up to 24 |x| instead of 8 |x| a weight, which costs them two bits of f32.
+// up to 24 |x| instead of 8 |x| a weight, which costs them two bits of f32; a result that comes out as no finite number is taken from the definition instead.
 // A CTA has a share of the tiles of sixteen rows, and its eight warps share K: a warp takes every eighth run of one or two units, for all tiles of the CTA, so that its operands
 // of x are loaded once, and normalised on the way. (A norm's factor into the sums instead saves the pass ahead, 1.5 us of 8 rows of 4096, but rounds the row differently from
 // a norm of its own: results were off by twice their rounding.) Units come by bulk copies into a ring of the warp's own, the first ones ahead
@@ -125,6 +125,13 @@ __device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
 // the warps that multiply (the ninth one is at its copies)
 __device__ __forceinline__ void consumers() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
 
+// One row: its factor out of the eight warps' sums of squares
+__device__ __forceinline__ float factor_of_sums(const RowsP& p, const float* sums) {
+  float ss = sums[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) ss += sums[w];
+  return rsqrtf(ss / (float)p.v.K + p.eps);
+}
 // A norm's factor of the row of this lane's operands. One row: 256 threads add up its squares; more: a warp a row. In one order whatever the rows: of 256 threads' pieces of
 // eight columns, 32 threads at a time. All loads of 4096 columns are under way at once.
 __device__ __forceinline__ float factor_of(const RowsP& p, float* sums, float* inv, int warp, int lane, int most_rows) {
@@ -146,10 +153,7 @@ __device__ __forceinline__ float factor_of(const RowsP& p, float* sums, float* i
     ss = warp_sum(ss);
     if (lane == 0) sums[warp] = ss;
     consumers();
-    ss = sums[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) ss += sums[w];
-    return rsqrtf(ss / (float)p.v.K + p.eps);
+    return factor_of_sums(p, sums);
   }
   float ss[WARPS] = {};
   if (warp < p.T) {
@@ -171,12 +175,37 @@ __device__ __forceinline__ float factor_of(const RowsP& p, float* sums, float* i
   return inv[lane >> 2];
 }
 
+// One result from the definition, in 64 bits: for sums that are not finite. 16 + q times an infinity and the offset's part of it are a NaN where q - z times it is an infinity, and
+// (16 + q) x may pass f32's range where the result does not. `units`: of the tile; `r`: row of it; `gains`, `by`: the norm's (or null)
+template <int GROUP, bool ZEROS, bool F16>
+__device__ __noinline__ float from_definition(const unsigned char* units, int r, const bf16* x, int K, const bf16* gains, float by) {
+  constexpr int NG = CHUNK / GROUP, UNIT = CODES + NG * (ZEROS ? 48 : 32);
+  const int g = r & 7, h = r >> 3;
+  double sum = 0.;
+  for (int k = 0; k < K && sum == sum; k += 8) {      // (NaN stays NaN)
+    const unsigned char* unit = units + (long)(k / CHUNK) * UNIT;
+    const int group = k % CHUNK / GROUP;
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(unit + (k >> 6 & 1) * 512 + code_at(g, k >> 3 & 3) + h * 8 + (k >> 5 & 1) * 4);
+    const float s = scales_of(*reinterpret_cast<const uint16_t*>(unit + CODES + group * 32 + g * 4 + h * 2), F16).x;
+    const int z = ZEROS ? unit[CODES + NG * 32 + group * 16 + g * 2 + h] : 8;
+    for (int i = 0; i < 8; ++i) {
+      const int q = (int)(__funnelshift_r(word, word, i / 2 * 4) >> (3 + i % 2 * 16) & 15u);
+      float v = __bfloat162float(x[k + i]);
+      if (gains) v = __bfloat162float(__float2bfloat16_rn(v * by * __bfloat162float(gains[k + i])));
+      sum += (double)v * ((double)s * (q - z));
+    }
+  }
+  return (float)sum;
+}
+
 // MR: most rows of x; J: units of a run; NORM: under a norm (asked for in the kernel, it cost the others 4 %: 8 rows of 8192 by 8192 13.2 us and 13.7)
 template <int GROUP, bool ZEROS, bool F16, int MR, int J, bool NORM>
 __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) {
   constexpr int NT = (MR + 7) / 8, RUNS = GROUP / 32, NG = 4 / RUNS, UNIT = CODES + NG * (ZEROS ? 48 : 32);      // runs of 32 columns of a group, groups of a unit, its bytes
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float sums[WARPS], inv[8];            // of a row's squares; the rows' factors
+  __shared__ int3 share;                           // what the CTA has: its part of K, tiles, first tile
+  __shared__ uint32_t gone;                        // a wait of this CTA ran out
   __shared__ __align__(16) unsigned char runs_of_x[MR == 1 ? WARPS * 512 : 16];
   __shared__ uint64_t bars[WARPS * BARS];          // of a warp's stages: full, and eight further on empty; behind them the polls that its waits may take
   grid_dep_launch();
@@ -185,6 +214,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
   const int split = blockIdx.x % p.splits, group = blockIdx.x / p.splits;
   const bool gated = v.halves == 2;
   const int fewest = v.tiles / p.groups, mine = fewest + (group < p.more), first = group * fewest + min(group, p.more);
+  if (threadIdx.x == 0) share = make_int3(split, mine, first);
   const int tiles = mine * v.halves;               // the CTA's: gate tiles, then up tiles
   const int chunk0 = (int)((long)v.chunks * split / p.splits), chunk1 = (int)((long)v.chunks * (split + 1) / p.splits);
   // the run behind the one that begins with unit r
@@ -203,6 +233,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
       tc::mbar_init(bars + lane * BARS + 8 + i, 1);
     }
     *reinterpret_cast<uint32_t*>(bars + lane * BARS + 16) = p.spin_limit;
+    if (lane == 0) gone = 0;
     tc::mbar_fence_init();
   }
   __syncthreads();
@@ -387,37 +418,52 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     }
   }
   if (warp < WARPS && __any_sync(0xffffffffu, late)) {             // a copy that did not land: nothing of the tiles is right
+    gone = 1;
     if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
     const float nan = __int_as_float(0x7fffffff);
     for (int i = 0; i < tiles * NT; ++i) sts_f4(acc + i * 512, make_float4(nan, nan, nan, nan));
   }
-  if (__syncthreads_or(late)) {                    // what has been requested lands before its place is used for the sums below, or by another CTA
+  __syncthreads();
+  if (*(volatile uint32_t*)&gone) {                // what has been requested lands before its place is used for the sums below, or by another CTA
     if (warp == WARPS && lane < WARPS)
       for (int i = max(0, requested - p.depth); i < requested; ++i) drain(smem_addr(bars + lane * BARS + i % p.depth), (i / p.depth) & 1);
     __syncthreads();
   }
   // the warps' sums, added up into [tile][16][rows of x] in the place of the rings
   constexpr int W = 8 * NT;
+  // (out of shared memory, as the loop above has no registers to keep them in)
+  const struct { int split, mine, first; } end{*(volatile int*)&share.x, *(volatile int*)&share.y, *(volatile int*)&share.z};
   const float* red = reinterpret_cast<const float*>(smem);
   const int step = p.most * NT * 128;
   float* part = reinterpret_cast<float*>(smem) + WARPS * step;
-  for (int i = threadIdx.x; i < tiles * TILE * W; i += WARPS * 32 + 32) {
+  for (int i = threadIdx.x; i < end.mine * v.halves * TILE * W; i += WARPS * 32 + 32) {
     const int t = i % W, r = i / W % TILE, tile = i / W / TILE;
     const float* f = red + ((tile * NT + (t >> 3)) * 32 + (r & 7) * 4 + ((t & 7) >> 1)) * 4 + (r >> 3) * 2 + (t & 1);
     part[i] = ((f[0] + f[step]) + (f[2 * step] + f[3 * step])) + ((f[4 * step] + f[5 * step]) + (f[6 * step] + f[7 * step]));
   }
   if (p.splits > 1) cluster_barrier();
   else __syncthreads();
-  const int rows = mine * TILE;                    // of the result
+  const int rows = end.mine * TILE;                // of the result
   const uint32_t part_at = smem_addr(part);
-  for (int i = threadIdx.x + split * (WARPS * 32 + 32); i < rows * p.T; i += p.splits * (WARPS * 32 + 32)) {
-    const int r = i % rows, t = i / rows, n = first * TILE + r;
+  for (int i = threadIdx.x + end.split * (WARPS * 32 + 32); i < rows * p.T; i += p.splits * (WARPS * 32 + 32)) {
+    const int r = i % rows, t = i / rows, n = end.first * TILE + r;
     if (n >= v.N) continue;
-    const int at = r * W + t, up_at = at + mine * TILE * W;
+    const int at = r * W + t, up_at = at + rows * W;
     float a = 0.f, u = 0.f;
     for (int s = 0; s < p.splits; ++s) {
       a += p.splits > 1 ? ld_part(part_at + at * 4, s) : part[at];
       if (gated) u += p.splits > 1 ? ld_part(part_at + up_at * 4, s) : part[up_at];
+    }
+    if (!(fabsf(a) <= 3.4028234e38f && fabsf(u) <= 3.4028234e38f)) {      // no finite number: from the definition, unless a wait ran out
+      bool right = true;
+      for (int s = 0; s < p.splits; ++s) right = right && (p.splits > 1 ? __float_as_uint(ld_part(smem_addr(&gone), s)) : gone) == 0;
+      if (right) {
+        const bf16 *x = p.x + (long)t * p.ldx, *gains = NORM ? p.norm_w : nullptr;
+        const int tile = end.first + r / TILE;
+        const float by = !NORM ? 1.f : MR == 1 ? factor_of_sums(p, sums) : inv[t & 7];
+        a = from_definition<GROUP, ZEROS, F16>(v.at(tile, 0), r % TILE, x, v.K, gains, by);
+        if (gated) u = from_definition<GROUP, ZEROS, F16>(v.at(tile + v.tiles, 0), r % TILE, x, v.K, gains, by);
+      }
     }
     if (gated) a = a / (1.f + __expf(-a)) * u;
     if (p.residual) a += __bfloat162float(p.residual[t * p.ldr + n]);

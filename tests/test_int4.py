@@ -428,3 +428,50 @@ def test_many_rows_against_the_matrix_that_was_packed(N, K, T, group, zeros, f16
     x, v = _rows(T, K, T), _values(q, s, z, group)
     bound = _operands(v, x)[1] + 2.0 ** -11 * (x.double().abs() @ v.abs().T)
     _close(int4.linear(x, int4.pack(q, s, z, group=group), out_f32=True), x.double() @ v.T, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,zeros,f16", [(128, False, False), (64, True, True), (32, True, False)])
+@pytest.mark.parametrize("N,K,T", [(300, 1032, 1), (70, 520, 3), (5000, 136, 8), (64, 16392, 2), (333, 2056, 16), (130, 520, 21), (333, 1032, 140), (300, 640, 600)])
+def test_infinities_and_rows_near_the_end_of_the_range(N, K, T, group, zeros, f16):
+    """An infinity in a row of x gives infinities of the weights' signs, and NaN where the weight is 0 or two of them meet with opposite signs, whatever the number of rows; rows whose
+    products with 16 + q pass f32's range give the finite results that they have."""
+    from ironpangu_b200.ops import int4
+
+    q, s, z = _codes(N, K, group, zeros, N + K, f16)
+    x, v = _rows(T, K, T), _values(q, s, z, group)
+    w = int4.pack(q, s, z, group=group)
+    x[0, 5] = float("inf")
+    if T > 1:
+        x[1, K - 1], x[1, 3] = float("-inf"), 0
+    if T > 2:
+        x[2] *= 2.0 ** 124
+    if T > 3:
+        x[3, 0], x[3, K // 2] = float("inf"), float("inf")
+    want = x.double() @ v.T
+    out = int4.linear(x, w, out_f32=True)
+    fine = want.isfinite()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf() & ~fine, want.isinf()) and torch.equal(out[want.isinf()].double(), want[want.isinf()])
+    bound = (x.double().abs() @ v.abs().T)[fine] * (max(CUT, 17 * K / 16 * 2.0 ** -23) + (2.0 ** -11 if T > 16 else 0)) + 1e-30
+    assert bool(((out.double() - want)[fine].abs() <= bound).all())
+    both = int4.linear(x, w, residual=torch.ones(T, N, dtype=BF16, device="cuda"))
+    assert torch.equal(both.isnan(), want.isnan()) and torch.equal(both[want.isinf()].double(), want[want.isinf()])
+
+
+@pytest.mark.gpu
+def test_infinite_gains_and_gated_units():
+    from ironpangu_b200.ops import int4
+
+    F, K = 90, 520
+    q, s, z = _codes(2 * F, K, 64, True, 5)
+    w, v = int4.pack(q, s, z, group=64, gated=True), _values(q, s, z, 64)
+    for T in (1, 5):
+        x, gain = _rows(T, K, T), torch.ones(K, dtype=BF16, device="cuda")
+        gain[17] = float("inf")
+        xn = (x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + 1e-5)).to(BF16).double()
+        xn[:, 17] = torch.where(xn[:, 17] > 0, float("inf"), float("-inf"))
+        y = xn @ v.T
+        gate, up = y[:, :F], y[:, F:]
+        want = gate / (1 + torch.exp(-gate)) * up
+        out = int4.linear(x, w, norm_w=gain, eps=1e-5, out_f32=True)
+        assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf()) and torch.equal(out[want.isinf()].double(), want[want.isinf()])
