@@ -10,7 +10,7 @@
 // Measured, 32768 x 4096 in groups of 64 with zero points: quantise 77 us in the kernel (4.4 TB/s of 6.5; instructions are issued in 61 % of the cycles, the rounding's seven a weight), without zero
 // points and groups of 128 68 with the call; dequantise 58 (5.8 TB/s). 1024 x 4096: 16 and 6.5, the calls' own time.
 // w / s is w times 1 / s and times what 1 / s was rounded off, off by 2^-45 ahead of its rounding to f32: a quotient that is half a step exactly comes out so, and others are
-// 2^-10 and more away from it, as w and s have eight bits.
+// 2^-10 and more away from it, as w and s have eight bits. Scales below 2^-126 and above 2^100 divide.
 #include "int4.cuh"
 #include "ifab_kernels.h"
 
@@ -102,18 +102,20 @@ __global__ void __launch_bounds__(256, 4) quantise_kernel(View v, const bf16* w,
         }
         const float lo = __bfloat162float(__hmin_nan(two_lo.x, two_lo.y)), hi = __bfloat162float(__hmax_nan(two_hi.x, two_hi.y));
         const bool bad = !(fabsf(lo) <= 3.4028234e38f && fabsf(hi) <= 3.4028234e38f);
-        const bf16 sb = __float2bfloat16_rn(ZEROS ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f));
+        float range = ZEROS ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f);
+        if (ZEROS && range > 3.4028234e38f) range = 2.f * __fdiv_rn(0.5f * hi - 0.5f * lo, 15.f);      // hi - lo passes f32's range, a fifteenth of it does not
+        const bf16 sb = __float2bfloat16_rn(range);
         const float s = __bfloat162float(sb) == 0.f ? 1.f : __bfloat162float(sb), by = __frcp_rn(s);
         const int z = ZEROS && !bad ? (int)fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f) : 8;
         const float rest = fmaf(-s, by, 1.f) * by, top = (float)(15 - z);
-        const bool tiny = s < 1.1754944e-38f || bad;      // 1 / s is no number to multiply by
+        const bool plain = s < 1.1754944e-38f || s > 1.2676506e30f || bad;      // 1 / s is no number to multiply by, or (above 2^100) what it was rounded off is none
 #pragma unroll
         for (int r = r0; r < r0 + RUNS; ++r) {
           constexpr float SHIFT = 12582912.f;              // 1.5 2^23: a number near it has its nearest integer in its last bits, halves to even
           float f[8];
           unpack8(u[h][r], f);
           uint32_t word = (z - 0x4b400000u) * 0x11111111u;
-          if (tiny) {
+          if (plain) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = bad ? 0.f : fminf(fmaxf(__fdiv_rn(f[i], s), -(float)z), top);
           } else {

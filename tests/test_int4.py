@@ -475,3 +475,29 @@ def test_infinite_gains_and_gated_units():
         want = gate / (1 + torch.exp(-gate)) * up
         out = int4.linear(x, w, norm_w=gain, eps=1e-5, out_f32=True)
         assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf()) and torch.equal(out[want.isinf()].double(), want[want.isinf()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("power", [-133, -126, -120, -60, 96, 104, 115, 122, 124, 126, 127])
+def test_quantise_at_the_ends_of_the_range(power, zeros):
+    """Matrices near bf16's smallest and largest numbers, quotients halfway between two codes among them: codes, scales and zero points are the definition's, also where the largest
+    less the smallest passes f32's range."""
+    from ironpangu_b200.ops import int4
+
+    g = torch.Generator(device="cuda").manual_seed(power + 200)
+    w = (torch.randn(70, 264, generator=g, device="cuda").clamp(-1.9, 1.9).double() * 2.0 ** power)
+    w[1] = (torch.arange(264, device="cuda") % 31 - 15).double() / 2 * 2.0 ** (power - 3)        # halves of a scale of 2^(power - 3)
+    w[2] = torch.where(torch.arange(264, device="cuda") % 2 == 0, 1.99, -1.99).double() * 2.0 ** power
+    w = w.to(BF16)
+    assert bool(w.isfinite().all())
+    f = torch.nn.functional.pad(w.double(), (0, -264 % 128)).view(70, -1, 128)
+    lo, hi = f.amin(-1).clamp(max=0), f.amax(-1).clamp(min=0)
+    # f32 and then bf16, as it is defined; a quotient by 15 or 7 is rounded to f32 first (f32's subnormals have steps of 2^-149)
+    exact = (hi - lo) / 15 if zeros else torch.maximum(hi, -lo) / 7
+    s = exact.float().to(BF16).double()
+    s = torch.where(s == 0, 1.0, s)[..., None]
+    z = torch.round(-lo[..., None] / s).clamp(0, 15) if zeros else 8
+    q = (torch.round(f / s) + z).clamp(0, 15)
+    want = ((q - z) * s).reshape(70, -1)[:, :264].float().to(BF16)
+    assert torch.equal(int4.quantise(w, group=128, zeros=zeros).dequantise(), want)
