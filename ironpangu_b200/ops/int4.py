@@ -97,8 +97,8 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor
 def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = None, eps: float = 1e-5, residual: Optional[torch.Tensor] = None, out_f32: bool = False,
            out: Optional[torch.Tensor] = None, status_ptr: Optional[int] = None) -> torch.Tensor:
     """``y = x @ w.T (+ residual)``, or of a gated matrix ``silu(x @ gate.T) * (x @ up.T)``, for any number of bf16 rows ``x`` ``[T, k]``. ``norm_w`` (up to eight rows): the
-    rows are RMS-normalised first, as :func:`ops.decode.rmsnorm` does it. ``residual`` (bf16, not of a gated matrix) may be ``out``. Sums are f32 and the result is rounded
-    once, to bf16 or with ``out_f32`` not at all. ``out`` must not overlap ``x``. Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product; up to
+    rows are RMS-normalised first, as :func:`ops.decode.rmsnorm` does it. ``residual`` (bf16, not of a gated matrix) may be ``out``, or lie apart from it. Sums are f32 and the
+    result is rounded once, to bf16 or with ``out_f32`` not at all. ``out``, whose rows lie apart, must not overlap ``x``. Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product; up to
     there it is not. ``status_ptr``: a status word for
     waits that run out."""
     # the checks say what is wrong in _refuse: a message that is made for every call costs as much as the launch. Device numbers, which are compared in a fifth of the time that
@@ -110,13 +110,17 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
     ldx = x.stride(0) if T > 1 else k
     if xp % 16 or ldx % 8:
         _refuse(x, w, norm_w, residual, out)
-    if out is None:
+    fresh = out is None
+    if fresh:
         f32 = out_f32
         out = torch.empty((T, n), dtype=F32 if f32 else BF16, device=w.device)
         yp, ldy = out.data_ptr(), n
     else:
         yp, ldy, f32 = out.data_ptr(), out.stride(0), out.dtype is F32
-        if not (out.shape == (T, n) and (f32 or out.dtype is BF16) and out.get_device() == dev and (out.stride(1) == 1 or n == 1) and (yp != xp or T == 0)):
+        if not (out.shape == (T, n) and (f32 or out.dtype is BF16) and out.get_device() == dev and (out.stride(1) == 1 or n == 1) and (ldy >= n or T < 2)):
+            _refuse(x, w, norm_w, residual, out)
+        # most outputs lie wholly ahead of or behind the rows
+        if yp < xp + 2 * ((T - 1) * ldx + k) and xp < yp + (4 if f32 else 2) * ((T - 1) * ldy + n) and _meet(x, out):
             _refuse(x, w, norm_w, residual, out)
     if norm_w is not None and not (norm_w.shape == (k,) and norm_w.dtype is BF16 and norm_w.get_device() == dev and norm_w.stride(0) == 1 and norm_w.data_ptr() % 16 == 0 and T <= NORM_ROWS):
         _refuse(x, w, norm_w, residual, out)
@@ -125,6 +129,8 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
         if not (not w.gated and residual.shape == (T, n) and residual.dtype is BF16 and residual.get_device() == dev and (residual.stride(1) == 1 or n == 1)):
             _refuse(x, w, norm_w, residual, out)
         rp, ldr = residual.data_ptr(), residual.stride(0)
+        if not (fresh or residual is out or _same(residual, out)) and _meet(residual, out):
+            _refuse(x, w, norm_w, residual, out)
     if T == 0:
         return out
     if dev < 0:
@@ -142,6 +148,25 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
     return out
 
 
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices ``[T, n]`` are one in memory."""
+    return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and (a.shape[0] < 2 or a.stride(0) == b.stride(0))
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices of as many rows share a byte."""
+    T = a.shape[0]
+    if T == 0:
+        return False
+    (ap, aw, al), (bp, bw, bl) = ((t.data_ptr(), t.shape[1] * t.element_size(), (t.stride(0) if T > 1 else 0) * t.element_size()) for t in (a, b))
+    if ap >= bp + (T - 1) * bl + bw or bp >= ap + (T - 1) * al + aw:
+        return False
+    if al != bl or al == 0:
+        return True
+    ahead = (bp - ap) % al                           # columns side by side, in rows of one pitch
+    return ahead < aw or ahead + bw > al
+
+
 def _refuse(x: torch.Tensor, w: Int4Weight, norm_w, residual, out) -> None:
     T = x.shape[0] if x.dim() else 0
     _need(x.dim() == 2 and x.shape[1] == w.k and x.dtype == BF16 and x.stride(1) == 1 and x.device == w.device, f"the rows must be bf16 [T, {w.k}] beside the weights")
@@ -152,9 +177,11 @@ def _refuse(x: torch.Tensor, w: Int4Weight, norm_w, residual, out) -> None:
         _need(T <= NORM_ROWS, f"a norm ahead of {T} rows is a launch of its own (ops.decode.rmsnorm)")
     _need(out is None or (out.shape == (T, w.n) and out.dtype in (BF16, F32) and (out.stride(1) == 1 or w.n == 1) and out.device == w.device),
           f"the output must be bf16 or f32 [T, {w.n}] beside the weights")
-    _need(out is None or T == 0 or out.data_ptr() != x.data_ptr(), "the output must not overlap the rows")
+    _need(out is None or T < 2 or out.stride(0) >= w.n, "the output's rows must lie apart")
+    _need(out is None or not _meet(x, out), "the output must not overlap the rows")
     if residual is not None:
         _need(not w.gated, "a gated unit takes no residual")
         _need(residual.shape == (T, w.n) and residual.dtype == BF16 and residual.stride(1) == 1 and residual.device == w.device,
               f"the residual must be bf16 [T, {w.n}] beside the weights")
+        _need(out is None or _same(residual, out) or not _meet(residual, out), "the residual must be the output or lie apart from it")
     raise AssertionError("int4.linear: a call was refused without a reason")

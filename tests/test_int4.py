@@ -501,3 +501,34 @@ def test_quantise_at_the_ends_of_the_range(power, zeros):
     q = (torch.round(f / s) + z).clamp(0, 15)
     want = ((q - z) * s).reshape(70, -1)[:, :264].float().to(BF16)
     assert torch.equal(int4.quantise(w, group=128, zeros=zeros).dequantise(), want)
+
+
+def test_outputs_that_overlap_are_refused():
+    """Rows of an output over one another, over the rows that are read or over a residual that is another matrix; side by side in one buffer is no overlap. On the host, where what
+    is not refused for this is refused for the weights' place."""
+    from ironpangu_b200.ops import int4
+
+    w, F32 = int4.Int4Weight(64, 64, device="cpu"), torch.float32
+    buffer = torch.zeros(40, 256, dtype=BF16)
+    flat = buffer.view(-1)
+    x, apart, wide = buffer[:9, :64], buffer[:9, 64:128], torch.zeros(9, 128, dtype=F32)
+    rows = lambda at, pitch: torch.as_strided(flat, (9, 64), (pitch, 1), at)
+    for out, what in ((torch.zeros(1, 64, dtype=BF16).expand(9, 64), "lie apart"), (rows(5000, 32), "lie apart"), (x, "overlap"), (buffer[:9, 32:96], "overlap"), (buffer[8:17, :64], "overlap"),
+                      (buffer[:9, 200:][:, :56].new_zeros(0), "output must be"), (rows(0, 512), "overlap"), (rows(256 - 8, 256), "overlap"), (buffer.view(F32)[:9, 16:80], "overlap"),
+                      (rows(64, 264), "overlap")):
+        with pytest.raises(ValueError, match=what):
+            int4.linear(x, w, out=out)
+    for residual in (buffer[:9, 128:192], buffer[:9, 64:128].clone(), buffer[1:10, 64:128], rows(64, 512), buffer[:9, 100:164]):
+        with pytest.raises(ValueError, match="the output or lie apart|on the host") as e:
+            int4.linear(x, w, out=apart, residual=residual)
+        meet = residual.data_ptr() in (buffer[1:10, 64:128].data_ptr(), rows(64, 512).data_ptr(), buffer[:9, 100:164].data_ptr()) and residual.untyped_storage().data_ptr() == flat.data_ptr()
+        assert ("lie apart" in str(e.value)) == meet
+    for call in (dict(out=apart, residual=apart), dict(out=apart, residual=buffer[:9, 64:128]), dict(out=wide[:, :64]), dict(out=buffer[9:18, :64]), dict(out=buffer[20:29, 7:71]),
+                 dict(residual=x), dict(out=apart, residual=x)):
+        with pytest.raises(ValueError, match="on the host"):
+            int4.linear(x, w, **call)
+    one = torch.zeros(1, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="on the host"):
+        int4.linear(one, w, out=torch.zeros(2, 64, dtype=BF16)[:1].as_strided((1, 64), (0, 1)))
+    with pytest.raises(ValueError, match="overlap"):
+        int4.linear(flat[:64].view(1, 64), w, out=flat[63:127].view(1, 64))
