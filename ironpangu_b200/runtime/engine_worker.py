@@ -837,8 +837,8 @@ def main() -> None:
     args.kv_int8 = args.kv_int8 or ropts.kv_int8
     args.expert_fp8 = args.expert_fp8 or ropts.expert_fp8
     args.weights_int4 = args.weights_int4 or ropts.weights_int4
-    if args.weights_int4 and not args.model.startswith("dense"):
-        raise SystemExit(f"--weights-int4: {args.model} has no 4-bit linears")
+    if args.weights_int4 and (args.bundle or not args.model.startswith("dense")):
+        raise SystemExit(f"--weights-int4: {args.bundle or args.model} has no 4-bit linears")
     args.prefill_chunk = args.prefill_chunk or ropts.prefill_chunk
     args.prefix_cache_slots = args.prefix_cache_slots or ropts.prefix_cache_slots
     args.no_graphs = args.no_graphs or not ropts.decode_graph
