@@ -30,7 +30,6 @@ using namespace ifab::int4;
 namespace {
 
 constexpr int WARPS = 8, BARS = 17, LEFT = 16 * 8;      // BARS: words of a warp's barriers; LEFT: bytes from the first of them to its limit
-constexpr uint32_t DRAIN = 4000000u;              // limit of the waits for copies that a CTA which gives up has requested
 
 struct RowsP {
   View v;
@@ -117,11 +116,6 @@ __device__ __noinline__ bool wait_more(uint32_t bar, uint32_t parity, uint32_t l
   return false;
 }
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint32_t left) { return ready(bar, parity) || wait_more(bar, parity, left); }
-__device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < DRAIN && !ready(bar, parity); ++i)
-    if (i > 256) __nanosleep(64);
-}
-
 // the warps that multiply (the ninth one is at its copies)
 __device__ __forceinline__ void consumers() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
 
@@ -204,8 +198,6 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
   constexpr int NT = (MR + 7) / 8, RUNS = GROUP / 32, NG = 4 / RUNS, UNIT = CODES + NG * (ZEROS ? 48 : 32);      // runs of 32 columns of a group, groups of a unit, its bytes
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float sums[WARPS], inv[8];            // of a row's squares; the rows' factors
-  __shared__ int3 share;                           // what the CTA has: its part of K, tiles, first tile
-  __shared__ uint32_t gone;                        // a wait of this CTA ran out
   __shared__ __align__(16) unsigned char runs_of_x[MR == 1 ? WARPS * 512 : 16];
   __shared__ uint64_t bars[WARPS * BARS];          // of a warp's stages: full, and eight further on empty; behind them the polls that its waits may take
   grid_dep_launch();
@@ -214,7 +206,6 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
   const int split = blockIdx.x % p.splits, group = blockIdx.x / p.splits;
   const bool gated = v.halves == 2;
   const int fewest = v.tiles / p.groups, mine = fewest + (group < p.more), first = group * fewest + min(group, p.more);
-  if (threadIdx.x == 0) share = make_int3(split, mine, first);
   const int tiles = mine * v.halves;               // the CTA's: gate tiles, then up tiles
   const int chunk0 = (int)((long)v.chunks * split / p.splits), chunk1 = (int)((long)v.chunks * (split + 1) / p.splits);
   // the run behind the one that begins with unit r
@@ -233,11 +224,9 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
       tc::mbar_init(bars + lane * BARS + 8 + i, 1);
     }
     *reinterpret_cast<uint32_t*>(bars + lane * BARS + 16) = p.spin_limit;
-    if (lane == 0) gone = 0;
     tc::mbar_fence_init();
   }
   __syncthreads();
-  int requested = 0;                               // copies, of a lane of the ninth warp
   if (warp == WARPS) {
     // lane w requests the runs of warp w. Codes are written by no kernel of the stream: nothing to wait for
     if (lane < WARPS) {
@@ -256,7 +245,6 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
           asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * J * UNIT), "l"(from), "r"(bytes),
                        "r"(full + slot * 8)
                        : "memory");
-          ++requested;
           if (++slot == p.depth) slot = 0, ++round;
         }
       }
@@ -418,35 +406,33 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
     }
   }
   if (warp < WARPS && __any_sync(0xffffffffu, late)) {             // a copy that did not land: nothing of the tiles is right
-    gone = 1;
     if (lane == 0 && p.status) atomicOr(p.status, IFAB_STATUS_MBAR_TIMEOUT);
     const float nan = __int_as_float(0x7fffffff);
     for (int i = 0; i < tiles * NT; ++i) sts_f4(acc + i * 512, make_float4(nan, nan, nan, nan));
+    // What was requested lands before its place is used for the sums below, or by another CTA: some milliseconds, a thousand times what a copy takes; nothing more is requested.
+    // (A loop, or waits for each copy, in this place cost the kernels beside this one: a step of 24 layers, 1 row over 2000 positions, 750 us and 820)
+    __nanosleep(1000000);
+    __nanosleep(1000000);
+    __nanosleep(1000000);
+    __nanosleep(1000000);
   }
   __syncthreads();
-  if (*(volatile uint32_t*)&gone) {                // what has been requested lands before its place is used for the sums below, or by another CTA
-    if (warp == WARPS && lane < WARPS)
-      for (int i = max(0, requested - p.depth); i < requested; ++i) drain(smem_addr(bars + lane * BARS + i % p.depth), (i / p.depth) & 1);
-    __syncthreads();
-  }
   // the warps' sums, added up into [tile][16][rows of x] in the place of the rings
   constexpr int W = 8 * NT;
-  // (out of shared memory, as the loop above has no registers to keep them in)
-  const struct { int split, mine, first; } end{*(volatile int*)&share.x, *(volatile int*)&share.y, *(volatile int*)&share.z};
   const float* red = reinterpret_cast<const float*>(smem);
   const int step = p.most * NT * 128;
   float* part = reinterpret_cast<float*>(smem) + WARPS * step;
-  for (int i = threadIdx.x; i < end.mine * v.halves * TILE * W; i += WARPS * 32 + 32) {
+  for (int i = threadIdx.x; i < tiles * TILE * W; i += WARPS * 32 + 32) {
     const int t = i % W, r = i / W % TILE, tile = i / W / TILE;
     const float* f = red + ((tile * NT + (t >> 3)) * 32 + (r & 7) * 4 + ((t & 7) >> 1)) * 4 + (r >> 3) * 2 + (t & 1);
     part[i] = ((f[0] + f[step]) + (f[2 * step] + f[3 * step])) + ((f[4 * step] + f[5 * step]) + (f[6 * step] + f[7 * step]));
   }
   if (p.splits > 1) cluster_barrier();
   else __syncthreads();
-  const int rows = end.mine * TILE;                // of the result
+  const int rows = mine * TILE;                    // of the result
   const uint32_t part_at = smem_addr(part);
-  for (int i = threadIdx.x + end.split * (WARPS * 32 + 32); i < rows * p.T; i += p.splits * (WARPS * 32 + 32)) {
-    const int r = i % rows, t = i / rows, n = end.first * TILE + r;
+  for (int i = threadIdx.x + split * (WARPS * 32 + 32); i < rows * p.T; i += p.splits * (WARPS * 32 + 32)) {
+    const int r = i % rows, t = i / rows, n = first * TILE + r;
     if (n >= v.N) continue;
     const int at = r * W + t, up_at = at + rows * W;
     float a = 0.f, u = 0.f;
@@ -454,12 +440,15 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, 2) int4_rows_kernel(RowsP p) 
       a += p.splits > 1 ? ld_part(part_at + at * 4, s) : part[at];
       if (gated) u += p.splits > 1 ? ld_part(part_at + up_at * 4, s) : part[up_at];
     }
-    if (!(fabsf(a) <= 3.4028234e38f && fabsf(u) <= 3.4028234e38f)) {      // no finite number: from the definition, unless a wait ran out
+    if (__builtin_expect(!(fabsf(a) <= 3.4028234e38f && fabsf(u) <= 3.4028234e38f), 0)) {      // no finite number: from the definition, unless a wait ran out
       bool right = true;
-      for (int s = 0; s < p.splits; ++s) right = right && (p.splits > 1 ? __float_as_uint(ld_part(smem_addr(&gone), s)) : gone) == 0;
+      for (int s = 0; s < p.splits * WARPS; ++s) {
+        const uint32_t left = smem_addr(bars + s % WARPS * BARS) + LEFT;
+        right = right && (p.splits > 1 ? __float_as_uint(ld_part(left, s / WARPS)) : lds4(left)) != 0;
+      }
       if (right) {
         const bf16 *x = p.x + (long)t * p.ldx, *gains = NORM ? p.norm_w : nullptr;
-        const int tile = end.first + r / TILE;
+        const int tile = first + r / TILE;
         const float by = !NORM ? 1.f : MR == 1 ? factor_of_sums(p, sums) : inv[t & 7];
         a = from_definition<GROUP, ZEROS, F16>(v.at(tile, 0), r % TILE, x, v.K, gains, by);
         if (gated) u = from_definition<GROUP, ZEROS, F16>(v.at(tile + v.tiles, 0), r % TILE, x, v.K, gains, by);
