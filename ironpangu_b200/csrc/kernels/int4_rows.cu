@@ -13,10 +13,11 @@
 // copies' addresses and requests them, and a stage costs the others a look at its barrier and an arrival. The warps' sums are added in one order, and so a row's bits do not
 // depend on the rows beside it.
 // Few tiles and a long K: the units along K are shared by the CTAs of a cluster, whose sums are added over distributed shared memory.
-// Measured, us (GB/s of codes and scales), weights not in L2: one row of 37888 by 8192 33.9 (4730; copies without products 6000), of 2 x 16384 by 4096 behind a norm 16.9 (4110), of 4096 by
-// 16384 11.9, 4096 by 4096 4.5, 1024 by 1024 2.3; eight rows of these 22.0 (3150), 13.7, 5.2, 2.4; 16 of 4096 by 4096 7.0 (tiles on the tensor cores 9.9), 17 as two passes
-// 11.8 (10.2). Long streams are bound by a unit's 116 instructions a warp (75 of them on integers); a scheduler issues one in 35 % of its cycles over the whole of a launch, whose
-// start, first copies and last sums are 4 us.
+// Measured, us (GB/s of codes and scales), weights not in L2: one row of 37888 by 8192 33.3 (4810; copies without products 6000), of 2 x 16384 by 4096 behind a norm 16.6 (4170), of 4096 by
+// 16384 12.0, 4096 by 4096 4.6, 1024 by 1024 2.4; eight rows of these 21.9 (3170), 13.8, 5.3, 2.5; 16 of 4096 by 4096 7.7 (tiles on the tensor cores 9.9), 17 as two passes
+// 11.8 (10.0). No pipe is full (one row of 2 x 16384 by 4096 under a profiler: issue slots 47 % and integers 54 % of the cycles of an SM at work, DRAM 38 %): what is left is latency. Four
+// such warps a scheduler each wait at a stage's barrier, load from shared memory and go through a chain of eight dependent products a unit; a launch's start, first copies and last
+// sums are 4 us of it. Two CTAs an SM leave a thread 96 registers, and 38 of the 108 forms spill (20 of them in groups of 32, up to 84 bytes; in groups of 128 up to 20).
 #include <algorithm>
 
 #include "int4.cuh"
@@ -475,7 +476,8 @@ int splits_of(const View& v, int sms) {
   }
   return best;
 }
-// Clusters of s CTAs that run at once, two CTAs an SM: not all SMs of a part of the chip can be divided by four or eight (of 296 CTAs, 284 and 264)
+// Clusters of s CTAs that are counted on to run at once, two CTAs an SM: not all SMs of a part of the chip can be divided by four or eight. Of 148 SMs 148, 69 and 31 clusters of two,
+// four and eight; the device has room for up to 71 and 33 of the latter
 int at_once(int s, int sms) { return s <= 2 ? 2 * sms / s : s == 4 ? 2 * sms * 15 / 64 : 2 * sms * 6 / 56; }
 constexpr int SMEM = 107 * 1024;                   // of a CTA, two of which share an SM (beside 5 KB that the kernel declares, and 1 KB each)
 

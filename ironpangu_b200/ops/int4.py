@@ -98,8 +98,10 @@ def linear(x: torch.Tensor, w: Int4Weight, *, norm_w: Optional[torch.Tensor] = N
            out: Optional[torch.Tensor] = None, status_ptr: Optional[int] = None) -> torch.Tensor:
     """``y = x @ w.T (+ residual)``, or of a gated matrix ``silu(x @ gate.T) * (x @ up.T)``, for any number of bf16 rows ``x`` ``[T, k]``. ``norm_w`` (up to eight rows): the
     rows are RMS-normalised first, as :func:`ops.decode.rmsnorm` does it. ``residual`` (bf16, not of a gated matrix) may be ``out``, or lie apart from it. Sums are f32 and the
-    result is rounded once, to bf16 or with ``out_f32`` not at all. ``out``, whose rows lie apart, must not overlap ``x``. Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product; up to
-    there it is not. ``status_ptr``: a status word for
+    result is rounded once, to bf16 or with ``out_f32`` not at all. ``out``, whose rows lie apart, must not overlap ``x``.
+
+    Beyond sixteen rows a weight is rounded to the 11 bits of f16 ahead of its product (in units of its row's largest scale, so that weights 2^-25 of that and less lose more), which
+    is the largest error of an f32 result there; up to sixteen rows it is not, and sums run over ``16 + q``, which costs two bits of f32. ``status_ptr``: a status word for
     waits that run out."""
     # the checks say what is wrong in _refuse: a message that is made for every call costs as much as the launch. Device numbers, which are compared in a fifth of the time that
     # devices are, and each attribute is asked for once
