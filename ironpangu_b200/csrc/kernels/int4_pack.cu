@@ -7,8 +7,8 @@
 //   dequantise   bf16(s (q - z))
 // Bound by the bytes of the matrix. A CTA has a tile of sixteen rows and its warps the units in turn, so that the rows' largest scales are at hand in the end: lane 4 g + c
 // holds two runs of eight columns of rows g and g + 8 in both blocks; four lanes read 64 bytes of a row.
-// Measured, 32768 x 4096 in groups of 64 with zero points: quantise 77 us in the kernel (4.4 TB/s of 6.5; instructions are issued in 61 % of the cycles, the rounding's seven a weight), without zero
-// points and groups of 128 68 with the call; dequantise 58 (5.8 TB/s). 1024 x 4096: 16 and 6.5, the calls' own time.
+// Measured, 32768 x 4096 in groups of 64 with zero points: quantise 78 us in the kernel (4.4 TB/s of 6.5; instructions are issued in 61 % of the cycles, the rounding's seven a
+// weight; with zero points 8 bytes a thread spill), without zero points and groups of 128 68 with the call; dequantise 58 (5.8 TB/s). 1024 x 4096: 16 and 6.5, the calls' own time.
 // w / s is w times 1 / s and times what 1 / s was rounded off, off by 2^-45 ahead of its rounding to f32: a quotient that is half a step exactly comes out so, and others are
 // 2^-10 and more away from it, as w and s have eight bits. Scales below 2^-126 and above 2^100 divide.
 #include "int4.cuh"

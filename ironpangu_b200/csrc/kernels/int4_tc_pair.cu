@@ -12,7 +12,7 @@
 //                rows, sixteen each: a lane gives every other token's value to its partner and has both of the others
 // Measured: 4096 rows of 2 x 16384 by 4096 803 - 820 us (the bf16 product of the same sizes 750; 1.1 TFLOP, 658 at the rate of a short burst), of 6144 by 4096 178 (152), 509 rows of the latter
 // 35 (29). Long prompts are bound by the products at the clocks that the power limit leaves (their pipe is busy for 64 % of the time of 1024 rows, issue slots for 44 %);
-// few tiles by 0.8 us a chunk, whatever their width, and 9.5 us beside.
+// few tiles by 0.8 us a chunk, whatever their width, and 9.5 us beside. A thread has 96 registers; groups of 32, and of 64 with zero points, spill one.
 // Weights go by way of shared memory: in tensor memory, where the MMA takes its first operand as well (int4_tc.cu), they leave no room for a second sum.
 // Every wait is bounded; one that runs out raises the CTA's flag and the status word, tiles that are not complete are stored as NaN, and both CTAs meet at the closing barrier.
 #include <algorithm>
