@@ -151,8 +151,8 @@ def bundle_parameters(cfg: DenseConfig, weights: Dict[str, torch.Tensor], world:
 
 
 class DenseDecoder:
-    """Per-rank executor for up to ``max_tokens`` (<= 8) query rows per launch group; larger batches are
-    processed in tiles of 8 rows by :meth:`forward`."""
+    """Per-rank executor for up to ``max_tokens`` query rows per launch group. Kernels that take eight rows at most run
+    in tiles of 8 rows."""
 
     def __init__(self, cfg: DenseConfig, weights: Dict[str, torch.Tensor], fabric: Fabric, *, max_tokens: int = 8,
                  max_context: int = 1024, num_slots: int = 1, keys_per_split: int = 64, keep_logits: bool = False,
@@ -196,7 +196,7 @@ class DenseDecoder:
         self.next_ids = torch.zeros(T, dtype=torch.int32, device=dev)
         self.next_vals = torch.zeros(T, dtype=torch.float32, device=dev)
         self.logits = e(T, self.vl, dt=torch.float32) if keep_logits else None
-        self.launches_per_forward = 2 + ((6 if T <= 8 else 8 if T <= int4.STREAM_ROWS else 12) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
+        self.launches_per_forward = 1 + (T + 7) // 8 + ((6 if T <= 8 else 8 if T <= int4.STREAM_ROWS else 12) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
         self._graph = None
 
     def _row_parallel(self, a: torch.Tensor, w: torch.Tensor, x: torch.Tensor) -> None:
@@ -246,10 +246,11 @@ class DenseDecoder:
             else:
                 K.gemv(x, w[p + "gate_up"], norm_w=w[p + "ffn_norm"], eps=c.eps, swiglu=True, out=self.act[:T], rings=fab.world == 1)
             self._row_parallel(self.act[:T], w[p + "down"], x)
-        if sample:
-            K.lm_head_argmax(x, w["lm_head"], fab, norm_w=w["final_norm"], eps=c.eps, vocab_offset=self.rank * self.vl,
-                             partial=self.partial, logits=None if self.logits is None else self.logits[:T],
-                             out_ids=self.next_ids[:T], out_vals=self.next_vals[:T])
+        for t in range(0, T if sample else 0, 8):      # the head takes eight rows
+            e = min(T, t + 8)
+            K.lm_head_argmax(x[t:e], w["lm_head"], fab, norm_w=w["final_norm"], eps=c.eps, vocab_offset=self.rank * self.vl,
+                             partial=self.partial, logits=None if self.logits is None else self.logits[t:e],
+                             out_ids=self.next_ids[t:e], out_vals=self.next_vals[t:e])
         return self.next_ids[:T]
 
     def capture(self, T: Optional[int] = None, feedback: bool = False):

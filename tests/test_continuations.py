@@ -247,3 +247,37 @@ def test_logits_are_those_of_sequences_that_share_nothing(int4, length, prompt_k
     c.end()
     assert int(dec.pool.refs.sum()) == 0 and own.fabric.status() == 0
     fab.close()
+
+
+@pytest.mark.parametrize("int4", [False, True])
+@pytest.mark.parametrize("n", [9, 16, 20])
+def test_more_rows_than_the_head_takes(int4, n):
+    """Steps of more than eight continuations - with 4-bit weights of more than sixteen, whose rows are operands made in a launch ahead - in a captured graph: every step's logits against the
+    same launches over slots that share nothing."""
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    cfg, fab, dec = _decoder(int4, slots=22, rows=20)
+    _, _, own = _decoder(int4, pool=False, slots=22, rows=20)
+    c = Continuations(dec)
+    prompt = torch.randint(0, cfg.vocab, (25,), generator=torch.Generator().manual_seed(n)).to(I32)
+    tokens = c.start(prompt.tolist(), n, temperature=1.2, top_k=40, seed=4).clone()
+    for slot in range(1, n + 1):
+        for p in range(0, 25, 20):
+            m = min(20, 25 - p)
+            own.tokens[:m].copy_(prompt[p:p + m])
+            own.positions[:m].copy_(torch.arange(p, p + m, dtype=I32))
+            own.slots[:m].fill_(slot)
+            own.forward(m)
+        assert torch.equal(own.logits[4], dec.logits[slot - 1])
+    for k in range(12):
+        own.tokens[:n].copy_(tokens)
+        own.positions[:n].fill_(25 + k)
+        own.slots[:n].copy_(torch.arange(1, n + 1, dtype=I32))
+        ids = own.forward(n)
+        tokens = c.step().clone()
+        assert torch.equal(dec.logits[:n], own.logits[:n]), k
+        assert torch.equal(ids.long(), own.logits[:n].argmax(-1))
+    c.check()
+    c.end()
+    assert own.fabric.status() == 0
+    fab.close()
