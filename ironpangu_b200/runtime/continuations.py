@@ -101,8 +101,10 @@ class Continuations:
 
     def _sample(self, n: int) -> None:
         d = self.dec
-        K.sample_topk(d.logits[:n], d.fabric, top_k=self.top_k, inv_temperature=self.inv_temp[:n], top_p=self.top_p[:n], seeds=self.seeds[:n], counters=self.counters[:n],
-                      scratch=self._scratch, out_ids=self.ids[:n])
+        for t in range(0, n, 64):             # the sampling kernel takes 64 rows
+            e = min(n, t + 64)
+            K.sample_topk(d.logits[t:e], d.fabric, top_k=self.top_k, inv_temperature=self.inv_temp[t:e], top_p=self.top_p[t:e], seeds=self.seeds[t:e],
+                          counters=self.counters[t:e], scratch=self._scratch, out_ids=self.ids[t:e])
         d.tokens[:n].copy_(self.ids[:n])
 
     # -- steps ---------------------------------------------------------------------------------------------------------------

@@ -281,3 +281,29 @@ def test_more_rows_than_the_head_takes(int4, n):
     c.end()
     assert own.fabric.status() == 0
     fab.close()
+
+
+def test_more_rows_than_the_sampling_takes():
+    """130 continuations: drawn with seeds of their own, from logits that are alike for a prompt's first token; each row's tokens are those of the sampling of that row alone."""
+    from ironpangu_b200.ops import decode as K
+    from ironpangu_b200.runtime.continuations import Continuations
+
+    n = 130
+    cfg, fab, dec = _decoder(True, slots=n + 1, rows=n)
+    c = Continuations(dec, store_pages=8)
+    for k in range(8):
+        ids = c.start(list(range(20)), n, temperature=1.1, top_k=30, seed=6).clone() if k == 0 else c.step().clone()
+        for i in (0, 63, 64, 100, 127, 128, 129):
+            f = lambda v, dt=torch.float32: torch.tensor([v], dtype=dt, device="cuda")
+            want = K.sample_topk(dec.logits[i:i + 1].contiguous(), fab, top_k=30, inv_temperature=f(1 / 1.1), top_p=f(1.0), seeds=f(i + 6 * 0x9E3779B1, torch.int64),
+                                 counters=f(k, torch.int64))
+            assert int(ids[i]) == int(want), (k, i)
+    c.resample(torch.arange(n, dtype=I32, device="cuda") // 2)
+    c.step()
+    c.pack()
+    c.take_up(n - 1, c.set_aside(n - 1))
+    c.step()
+    c.check()
+    c.end()
+    assert int(dec.pool.refs.sum()) == 0 and fab.status() == 0
+    fab.close()
