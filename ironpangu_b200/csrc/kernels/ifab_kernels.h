@@ -555,6 +555,12 @@ int ifab_pages_fork(const IfabPagePool* p, const int32_t* src, const int32_t* ds
 int ifab_pages_free(const IfabPagePool* p, const int32_t* slots, const int32_t* below, int n, void* stream);
 int ifab_pages_compact(const IfabPagePool* p, int32_t* live, void* stream);
 
+/* ---- a token a row from the whole vocabulary (draw.cu) -------------------------------------------
+ * logits [T, V] f32 or bf16, ld elements from a row to the next, V <= 2^18. Per row, each may be NULL: inverse temperature (not above 0, infinite or NaN: the largest logit), top_k
+ * (below 1 or V and more: all), top_p (1 and more: all), min_p (0 and less: all). uniforms [T] within [0, 1). A row of nothing but -inf and NaN gives id -1, probability 0. */
+int ifab_draw(const void* logits, long ld, int f32, int T, int V, const float* inv_temperature, const int32_t* top_k, const float* top_p, const float* min_p, const float* uniforms,
+              int32_t* out_ids, float* out_probs, void* stream);
+
 /* ---- GQA decode attention without any allocation (this entry point has no counterpart in the reference) ----
  * Same computation and same results as ifab_gqa_decode_attention, but the split-partials workspace is a
  * fixed array inside the library, so neither the caller nor the library calls cudaMalloc / cudaFree or any
