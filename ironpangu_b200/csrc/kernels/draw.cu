@@ -23,8 +23,8 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int NT = 512, WARPS = NT / 32, BINS = 1024, LIST = 1024, MAX_CLUSTER = 8, ID_BITS = 20;
-constexpr int MAX_VOCAB = 1 << 18;
+constexpr int NT = 512, WARPS = NT / 32, BINS = 1024, LIST = 1024, MAX_CLUSTER = 8, ID_BITS = 20, PARTS = 32;
+constexpr int MAX_VOCAB = 1 << 18, MAX_SLICE = MAX_VOCAB / MAX_CLUSTER;
 typedef unsigned long long u64;
 
 struct DrawParams {
@@ -42,16 +42,18 @@ struct DrawParams {
 struct Cut {
   float x;
   int i;
-  __device__ __forceinline__ bool has(float v, int id) const { return v > x || (v == x && id <= i); }
+  __device__ __forceinline__ bool has(float v, int id) const { return (v > x) | ((v == x) & (id <= i)); }      // (no branches in the loops over a row)
 };
 
+struct __align__(16) Entry {
+  u64 place, mass;
+};
 struct Shared {
-  uint32_t cnt[BINS], lo[BINS], hi[BINS];      // this CTA's tokens and their mass (two words)
-  uint32_t total_cnt[BINS];                    // the row's
-  u64 total[BINS];
-  float list_v[LIST];
-  int list_id[LIST];
-  uint32_t listed;
+  uint32_t part[3][BINS];                      // this CTA's tokens by bin: their number, or their mass in three words (which its tokens cannot overflow: 17 bits of each, 2^15 tokens)
+  Entry list[LIST];
+  u64 total[BINS];                             // the row's
+  double parts[PARTS];                         // 2^(i / 32)
+  uint32_t listed[2];                          // by turns
   u64 from[MAX_CLUSTER];                       // a value of each CTA
   float most[MAX_CLUSTER], least[MAX_CLUSTER];
   int best[MAX_CLUSTER];
@@ -59,10 +61,10 @@ struct Shared {
   float warp_a[WARPS], warp_b[WARPS];
   int warp_i[WARPS];
   int bin;
-  uint32_t members;
   u64 above;
   Cut cut;
 };
+static_assert(MAX_SLICE <= 1 << 15, "17 bits of each token's mass in 32");
 
 // of values that are no NaN: unsigned integers in their order
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -74,12 +76,27 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k
 __device__ __forceinline__ u64 place_of(float v, int id) { return (u64)key_of(v) << ID_BITS | (u64)((1 << ID_BITS) - 1 - id); }
 
 struct Weights {
-  float most;
+  float most, floor;           // below `floor` a weight is less than 2^-45
   double it, z_most;
+  const double* parts;
+  __device__ __forceinline__ Weights(float most, float it_, const double* parts) : most(most), it((double)it_), z_most((double)most * (double)it_), parts(parts) {
+    const double lowest = (z_most - 32.0) / it;          // e^-32 < 2^-46
+    floor = most == INFINITY ? INFINITY : lowest > -3.4e38 ? __double2float_rd(lowest) : -3.4028234664e38f;
+  }
   // of `most` itself 1, an infinite one among them; a product of two floats is exact
   __device__ __forceinline__ double real(float v) const { return v == most ? 1.0 : exp((double)v * it - z_most); }
-  // in units of 2^-44, rounded: 256 + w has its last bit there
-  __device__ __forceinline__ u64 fixed(float v) const { return (u64)__double_as_longlong(real(v) + 256.0) & ((1ull << 52) - 1); }
+  // In units of 2^-44, rounded. e^d = 2^(n / 32) e^r, r = d - n ln 2 / 32 of at most 0.011 by Taylor's series up to r^5 / 120 (what it leaves is below 2^-48), without a branch, so that
+  // several tokens' chains run side by side: exp() took 25 cycles a token of each lane with 16 warps.
+  __device__ __forceinline__ u64 fixed(float v) const {
+    const double d = (double)fmaxf(v, floor) * it - z_most;
+    const double turn = fma(d, 32 * 1.4426950408889634, 6755399441055744.0);          // 1.5 2^52: the last bits are n
+    const int n = (int)__double_as_longlong(turn);
+    const double r = fma(turn - 6755399441055744.0, -0.6931471805599453 / 32, d);
+    const double e = fma(fma(fma(fma(fma(r, 1.0 / 120, 1.0 / 24), r, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0) * parts[n & (PARTS - 1)];
+    const double scaled = __longlong_as_double(__double_as_longlong(e) + ((u64)(long long)(n >> 5) << 52));
+    const u64 m = (u64)__double_as_longlong(scaled + 256.0) & ((1ull << 52) - 1);       // 256 + w has its last bit at 2^-44
+    return v == most ? 1ull << 44 : v < floor ? 0 : m;
+  }
 };
 
 __device__ __forceinline__ u64 shfl_up64(u64 v, int by) { return __shfl_up_sync(0xffffffffu, v, by); }
@@ -91,69 +108,83 @@ __device__ __forceinline__ u64 warp_total(u64 v) {
 
 __device__ __forceinline__ float clean(float v) { return v != v ? -INFINITY : v + 0.f; }      // a NaN is never drawn; -0 is 0
 
-// Where the row's bins, lowest place first, pass `want(total)`: bin, what lies above it, its tokens
-struct Level {
-  int bin;
-  u64 above;
-  uint32_t members;
-};
-
+// The place in the order at which what lies ahead reaches a number of tokens, or a share of their mass
 template <bool MASS>
 struct Search {
   Shared* s;
-  const float* vals;
-  int n, base, tid, rank, ranks;
+  const float4* vals;
+  int quads, base, tid, rank, ranks;           // quads: fours of tokens in this CTA; those behind the last one are -inf, with ids that no place reaches
+  uint32_t* turn;
   Cut cut;
   Weights w;
   float top, scale;            // bins of equal stretches below `top`
-  int first_bin;
+  float first_bin;
   u64 lo, hi;                  // places within first_bin, once it is split
+  bool split;
 
-  __device__ __forceinline__ int stretch(float v) const { return scale > 0.f ? (int)fminf((top - v) * scale, (float)(BINS - 1)) : 0; }
+  __device__ __forceinline__ float stretch(float v) const { return scale > 0.f ? fminf((top - v) * scale, (float)(BINS - 1)) : 0.f; }
+  __device__ __forceinline__ bool member(float v, int id) const {
+    const float at = stretch(v);
+    bool in = (at >= first_bin) & (at < first_bin + 1.f) & cut.has(v, id);
+    if (split) in = in & (place_of(v, id) >= lo) & (place_of(v, id) <= hi);
+    return in;
+  }
 
   template <typename Bin>
   __device__ void count(Bin bin) {
-    for (int b = tid; b < BINS; b += NT) s->cnt[b] = s->lo[b] = s->hi[b] = 0;
+    for (int b = tid; b < BINS * (MASS ? 3 : 1); b += NT) s->part[0][b] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-      const float v = vals[i];
-      if (!cut.has(v, base + i)) continue;
-      const int b = bin(v, base + i);
-      if (b < 0) continue;
-      atomicAdd(&s->cnt[b], 1u);
-      if (MASS) {
-        const u64 m = w.fixed(v);
-        const uint32_t part = (uint32_t)m, was = part ? atomicAdd(&s->lo[b], part) : 0u;
-        const uint32_t up = (uint32_t)(m >> 32) + (part && was + part < was);
-        if (up) atomicAdd(&s->hi[b], up);
+    for (int c = tid; c < quads; c += NT) {
+      const float4 q = vals[c];
+      const float v[4] = {q.x, q.y, q.z, q.w};
+      u64 m[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[j] = MASS ? w.fixed(v[j]) : 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int id = base + 4 * c + j;
+        if (!cut.has(v[j], id)) continue;
+        const int b = bin(v[j], id);
+        if (b < 0) continue;
+        if (!MASS) {
+          atomicAdd(&s->part[0][b], 1u);
+          continue;
+        }
+        constexpr uint32_t low = (1u << 17) - 1;
+        const uint32_t a0 = (uint32_t)m[j] & low, a1 = (uint32_t)(m[j] >> 17) & low, a2 = (uint32_t)(m[j] >> 34);
+        if (a0) atomicAdd(&s->part[0][b], a0);
+        if (a1) atomicAdd(&s->part[1][b], a1);
+        if (a2) atomicAdd(&s->part[2][b], a2);
       }
     }
   }
-  // sums over the cluster, then the bin at which the order passes the place: count `k` (COUNT), or `share` of the mass (MASS). `above` counts on from `from`.
-  __device__ Level find(cg::cluster_group& cluster, u64 from, bool fresh, u64* want, float share) {
+  // Sums over the cluster, then the bin at which the order passes the place `want`; `above` counts on from `from`. fresh: `want` follows from `share` and the total
+  __device__ void find(cg::cluster_group& cluster, u64 from, bool fresh, u64* want, float share) {
     cluster.sync();
-    const int mine = BINS / ranks;
-    for (int j = tid; j < mine; j += NT) {
-      const int b = rank * mine + j;
-      uint32_t c = 0;
+    // each CTA adds up its share of the bins, four threads a bin
+    const int lane = tid & 31, warp = tid >> 5, four = tid & 3;
+    for (int b = rank * (BINS / ranks) + (tid >> 2); b < (rank + 1) * (BINS / ranks); b += NT / 4) {
       u64 m = 0;
-      for (int r = 0; r < ranks; ++r) {
-        const Shared* o = cluster.map_shared_rank(s, r);
-        c += o->cnt[b];
-        if (MASS) m += ((u64)o->hi[b] << 32) + o->lo[b];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = four + 4 * h;
+        if (r < ranks) {
+          const Shared* o = cluster.map_shared_rank(s, r);
+          m += o->part[0][b];
+          if (MASS) m += ((u64)o->part[1][b] << 17) + ((u64)o->part[2][b] << 34);
+        }
       }
-      for (int r = 0; r < ranks; ++r) {
-        Shared* o = cluster.map_shared_rank(s, r);
-        o->total_cnt[b] = c;
-        o->total[b] = MASS ? m : c;
-      }
+      m += __shfl_xor_sync(0xffffffffu, m, 1);
+      m += __shfl_xor_sync(0xffffffffu, m, 2);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (four + 4 * h < ranks) cluster.map_shared_rank(s, four + 4 * h)->total[b] = m;
     }
     cluster.sync();
     // scan of two bins a thread
     static_assert(BINS == 2 * NT, "two bins a thread");
     const u64 a = s->total[2 * tid], b = s->total[2 * tid + 1];
     u64 sum = a + b;
-    const int lane = tid & 31, warp = tid >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u64 x = shfl_up64(sum, o);
@@ -162,9 +193,11 @@ struct Search {
     if (lane == 31) s->warp_sum[warp] = sum;
     __syncthreads();
     u64 before = from, all = from;
+#pragma unroll
     for (int i = 0; i < WARPS; ++i) {
-      if (i < warp) before += s->warp_sum[i];
-      all += s->warp_sum[i];
+      const u64 x = s->warp_sum[i];
+      if (i < warp) before += x;
+      all += x;
     }
     if (MASS && fresh) {                         // a token is kept while the mass ahead of it is below share * all
       const double t = ceil((double)share * (double)all);
@@ -175,61 +208,64 @@ struct Search {
       const bool second = mid < *want;
       s->bin = 2 * tid + second;
       s->above = second ? mid : excl;
-      s->members = s->total_cnt[2 * tid + second];
     }
     __syncthreads();
-    const Level l{s->bin, s->above, s->members};
-    return l;
   }
-  __device__ __forceinline__ bool member(float v, int id) const {
-    const u64 at = place_of(v, id);
-    return cut.has(v, id) && stretch(v) == first_bin && at >= lo && at <= hi;
+  // the members into every CTA's list; their number (of which the list holds LIST at most)
+  __device__ uint32_t gather(cg::cluster_group& cluster) {
+    uint32_t* counter = &cluster.map_shared_rank(s, 0)->listed[*turn & 1];
+    if (rank == 0 && tid == 0) s->listed[(*turn + 1) & 1] = 0;        // the next turn's; the turn before has been read ahead of a barrier of the cluster
+    *turn += 1;
+    for (int c = tid; c < quads; c += NT) {
+      const float4 q = vals[c];
+      const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int id = base + 4 * c + j;
+        if (!member(v[j], id)) continue;
+        const uint32_t at = atomicAdd(counter, 1u);
+        if (at < LIST) {
+          const Entry e{place_of(v[j], id), MASS ? w.fixed(v[j]) : 1};
+          for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(s, r)->list[at] = e;
+        }
+      }
+    }
+    cluster.sync();
+    return *counter;
   }
 
   __device__ Cut run(cg::cluster_group& cluster, u64 want, float share) {
-    count([&](float v, int) { return stretch(v); });
-    Level l = find(cluster, 0, true, &want, share);
-    first_bin = l.bin;
+    count([&](float v, int) { return (int)stretch(v); });
+    find(cluster, 0, true, &want, share);
+    first_bin = (float)s->bin;
+    u64 above = s->above;
+    split = false;
     lo = 0;
     hi = (1ull << (32 + ID_BITS)) - 1;
-    for (int shift = 32 + ID_BITS - 10; l.members > LIST; shift = max(0, shift - 10)) {
-      __syncthreads();
+    uint32_t m = gather(cluster);
+    for (int shift = 32 + ID_BITS - 10; m > LIST; shift = max(0, shift - 10)) {
+      split = true;
       count([&](float v, int id) { return member(v, id) ? (int)((hi - place_of(v, id)) >> shift) : -1; });
-      l = find(cluster, l.above, false, &want, share);
-      hi -= (u64)l.bin << shift;
+      find(cluster, above, false, &want, share);
+      above = s->above;
+      hi -= (u64)s->bin << shift;
       lo = hi - ((1ull << shift) - 1);
+      m = gather(cluster);
     }
-    uint32_t* counter = &cluster.map_shared_rank(s, 0)->listed;
-    for (int i = tid; i < n; i += NT) {
-      const float v = vals[i];
-      if (!member(v, base + i)) continue;
-      const uint32_t at = atomicAdd(counter, 1u);
-      if (at < LIST)
-        for (int r = 0; r < ranks; ++r) {
-          Shared* o = cluster.map_shared_rank(s, r);
-          o->list_v[at] = v;
-          o->list_id[at] = base + i;
-        }
-    }
-    cluster.sync();
-    if (tid == 0) s->listed = 0;                 // (appended to again two cluster barriers from here at the earliest)
-    const int m = l.members;
-    u64* mass = s->total;                        // LIST <= BINS
-    for (int i = tid; i < m; i += NT) mass[i] = MASS ? w.fixed(s->list_v[i]) : 1;
-    __syncthreads();
-    for (int i = tid; i < m; i += NT) {
-      const float v = s->list_v[i];
-      const int id = s->list_id[i];
-      u64 ahead = l.above;
-      for (int j = 0; j < m; ++j)
-        if (s->list_v[j] > v || (s->list_v[j] == v && s->list_id[j] < id)) ahead += mass[j];
-      if (ahead < want && want <= ahead + mass[i]) s->cut = Cut{v, id};
+    for (uint32_t i = tid; i < m; i += NT) {
+      const Entry mine = s->list[i];
+      u64 ahead = above;
+#pragma unroll 8
+      for (uint32_t j = 0; j < m; ++j) {
+        const Entry e = s->list[j];
+        ahead += e.place > mine.place ? e.mass : 0;
+      }
+      if (ahead < want && want <= ahead + mine.mass) s->cut = Cut{value_of((uint32_t)(mine.place >> ID_BITS)), (1 << ID_BITS) - 1 - (int)(mine.place & ((1 << ID_BITS) - 1))};
     }
     __syncthreads();
     return s->cut;
   }
 };
-static_assert(LIST <= BINS, "the list's masses lie in the bins' place");
 
 __device__ __forceinline__ float load_one(const float* p) { return __ldcs(p); }
 __device__ __forceinline__ float load_one(const bf16* p) { return __bfloat162float(*p); }
@@ -241,35 +277,45 @@ __device__ __forceinline__ void load_eight(const float* p, float (&f)[8]) {
 __device__ __forceinline__ void load_eight(const bf16* p, float (&f)[8]) { unpack8(__ldcs(reinterpret_cast<const uint4*>(p)), f); }
 
 template <typename In>
-__global__ void __launch_bounds__(NT) draw_kernel(DrawParams p) {
+__global__ void __launch_bounds__(NT, 2) draw_kernel(DrawParams p) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared* s = reinterpret_cast<Shared*>(raw);
   float* vals = reinterpret_cast<float*>(raw + (sizeof(Shared) + 15) / 16 * 16);
+  float4* quad = reinterpret_cast<float4*>(vals);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / ranks;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int base = rank * p.slice, n = max(0, min(p.slice, p.V - base));
+  const int base = rank * p.slice, n = max(0, min(p.slice, p.V - base)), quads = (n + 3) / 4;
   grid_dep_launch();
-  if (tid == 0) s->listed = 0;
+  if (tid < 2) s->listed[tid] = 0;
+  if (tid < PARTS) s->parts[tid] = exp2((double)tid / PARTS);
   auto here = cluster.barrier_arrive();          // the others' memory is written to once they run
   grid_dep_wait();
   const In* src = reinterpret_cast<const In*>(p.logits) + (long)row * p.ld + base;
   float most = -INFINITY, least = INFINITY;
   const int whole = p.wide ? n / 8 : 0;
-  for (int c = tid; c < whole; c += NT) {
-    float f[8];
-    load_eight(src + 8 * c, f);
+  constexpr int AT_ONCE = 4;
+  for (int c0 = tid; c0 < whole; c0 += AT_ONCE * NT) {
+    float f[AT_ONCE][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f[j] = clean(f[j]);
-      most = fmaxf(most, f[j]);
-      if (f[j] != -INFINITY) least = fminf(least, f[j]);
+    for (int k = 0; k < AT_ONCE; ++k)
+      if (c0 + k * NT < whole) load_eight(src + 8 * (c0 + k * NT), f[k]);
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int c = c0 + k * NT;
+      if (c >= whole) break;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[k][j] = clean(f[k][j]);
+        most = fmaxf(most, f[k][j]);
+        if (f[k][j] != -INFINITY) least = fminf(least, f[k][j]);
+      }
+      quad[2 * c] = make_float4(f[k][0], f[k][1], f[k][2], f[k][3]);
+      quad[2 * c + 1] = make_float4(f[k][4], f[k][5], f[k][6], f[k][7]);
     }
-    reinterpret_cast<float4*>(vals)[2 * c] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(vals)[2 * c + 1] = make_float4(f[4], f[5], f[6], f[7]);
   }
-  for (int i = 8 * whole + tid; i < n; i += NT) {
-    const float v = clean(load_one(src + i));
+  for (int i = 8 * whole + tid; i < 4 * quads; i += NT) {
+    const float v = i < n ? clean(load_one(src + i)) : -INFINITY;
     vals[i] = v;
     most = fmaxf(most, v);
     if (v != -INFINITY) least = fminf(least, v);
@@ -320,17 +366,21 @@ __global__ void __launch_bounds__(NT) draw_kernel(DrawParams p) {
     return;
   }
 
-  Cut cut{-INFINITY, INT_MAX};
-  Weights w{most, (double)it, (double)most * (double)it};
+  const Cut all{-INFINITY, INT_MAX};
+  Cut cut = all;
+  const Weights w(most, it, s->parts);
   const float span = fminf(most, 3.0e38f) - least;
   const float scale = span > 0.f && span < 3.0e38f && most < INFINITY ? (float)(BINS - 1) / span : 0.f;
+  uint32_t turn = 0;
   const int k = p.top_k ? p.top_k[row] : 0;
-  if (k >= 1 && k < p.V) {
-    Search<false> f{s, vals, n, base, tid, rank, ranks, cut, w, most, scale};
-    cut = f.run(cluster, k, 0.f);
+  const float least_share = p.min_p ? p.min_p[row] : 0.f, share = p.top_p ? p.top_p[row] : 1.f;
+  // of a weight limit above 1 the first token is left
+  const int count = least_share > 1.f ? 1 : k;
+  if (count >= 1 && count < p.V) {
+    Search<false> f{s, quad, quads, base, tid, rank, ranks, &turn, all, w, most, scale};
+    cut = f.run(cluster, count, 0.f);
   }
-  const float least_share = p.min_p ? p.min_p[row] : 0.f;
-  if (least_share > 0.f) {
+  if (least_share > 0.f && least_share <= 1.f) {
     // the lowest value whose weight is enough: the predicate is monotone in the value's key, so each lane tries one of 32 places, 32 times finer every round
     uint32_t at = key_of(-INFINITY), step = 1u << 27;         // the value lies in (at, at + 32 steps], or is the largest itself
     const uint32_t end = key_of(most);
@@ -345,32 +395,43 @@ __global__ void __launch_bounds__(NT) draw_kernel(DrawParams p) {
     const u64 key = (u64)at + 1;
     const float v = key >= end ? most : value_of((uint32_t)key);
     if (v > cut.x) cut = Cut{v, INT_MAX};
-    // of a weight limit above 1 the first token is left
-    if (1.0 < (double)least_share) cut = Cut{most, -1};
   }
-  const float share = p.top_p ? p.top_p[row] : 1.f;
-  if (cut.i == -1) {
-    Search<false> f{s, vals, n, base, tid, rank, ranks, Cut{-INFINITY, INT_MAX}, w, most, scale};
-    cut = f.run(cluster, 1, 0.f);
-  } else if (share < 1.f) {
-    Search<true> f{s, vals, n, base, tid, rank, ranks, cut, w, most, scale};
+  if (share < 1.f) {
+    Search<true> f{s, quad, quads, base, tid, rank, ranks, &turn, cut, w, most, scale};
     cut = f.run(cluster, 0, share);
   }
 
   // the kept tokens' masses: a warp's stretch of ids each, so that sums by rising ids need no more than the stretches' sums
-  const int stretch = (n + WARPS - 1) / WARPS, first = min(n, warp * stretch), last = min(n, first + stretch);
+  const int each = (quads + WARPS - 1) / WARPS, first = min(quads, warp * each), last = min(quads, first + each);
+  auto kept = [&](int c, u64 (&m)[4]) {
+    const float4 q = quad[c];
+    const float v[4] = {q.x, q.y, q.z, q.w};
+    bool has[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) has[j] = cut.has(v[j], base + 4 * c + j);
+    if (__any_sync(__activemask(), has[0] || has[1] || has[2] || has[3])) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = w.fixed(v[j]);
+        if (!has[j]) m[j] = 0;
+      }
+    } else {
+      m[0] = m[1] = m[2] = m[3] = 0;
+    }
+  };
   u64 sum = 0;
-  for (int i = first + lane; i < last; i += 32) {
-    const float v = vals[i];
-    if (cut.has(v, base + i)) sum += w.fixed(v);
+  for (int c = first + lane; c < last; c += 32) {
+    u64 m[4];
+    kept(c, m);
+    sum += (m[0] + m[1]) + (m[2] + m[3]);
   }
   sum = warp_total(sum);
   if (lane == 0) s->warp_sum[warp] = sum;
   __syncthreads();
   if (tid < ranks) {
-    u64 all = 0;
-    for (int i = 0; i < WARPS; ++i) all += s->warp_sum[i];
-    cluster.map_shared_rank(s, tid)->from[rank] = all;
+    u64 mine = 0;
+    for (int i = 0; i < WARPS; ++i) mine += s->warp_sum[i];
+    cluster.map_shared_rank(s, tid)->from[rank] = mine;
   }
   cluster.sync();
   u64 before = 0, total = 0;
@@ -384,10 +445,11 @@ __global__ void __launch_bounds__(NT) draw_kernel(DrawParams p) {
   if (target < before || target >= before + s->from[rank]) return;
   for (int i = 0; i < warp; ++i) before += s->warp_sum[i];
   if (target < before || target >= before + s->warp_sum[warp]) return;
-  for (int i0 = first; i0 < last; i0 += 32) {
-    const int i = i0 + lane;
-    const float v = i < last ? vals[i] : -INFINITY;
-    const u64 mine = i < last && cut.has(v, base + i) ? w.fixed(v) : 0;
+  for (int c0 = first; c0 < last && target >= before; c0 += 32) {
+    const int c = c0 + lane;
+    u64 m[4] = {0, 0, 0, 0};
+    if (c < last) kept(c, m);
+    const u64 mine = (m[0] + m[1]) + (m[2] + m[3]);
     u64 incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -396,11 +458,17 @@ __global__ void __launch_bounds__(NT) draw_kernel(DrawParams p) {
     }
     incl += before;
     if (target < incl && target >= incl - mine) {
-      p.out_ids[row] = base + i;
-      if (p.out_probs) p.out_probs[row] = (float)(w.real(v) / ((double)total * 0x1p-44));
+      u64 run = incl - mine;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (target >= run && target < run + m[j]) {
+          p.out_ids[row] = base + 4 * c + j;
+          if (p.out_probs) p.out_probs[row] = (float)(w.real(vals[4 * c + j]) / ((double)total * 0x1p-44));
+        }
+        run += m[j];
+      }
     }
     before = __shfl_sync(0xffffffffu, incl, 31);
-    if (target < before) break;
   }
 }
 
