@@ -63,6 +63,7 @@ _SIGS = {
     "ifab_pages_fork": [_P, _P, _P, c_int, _P],
     "ifab_pages_free": [_P, _P, _P, c_int, _P],
     "ifab_pages_compact": [_P, _P, _P],
+    "ifab_shared_prefix_attention": [_P, c_long, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, c_int, c_float, c_int, c_int, c_int, c_int, _P, c_u64, _P, c_long, _P, _P],
     "ifab_draw": [_P, c_long, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P],
     "ifab_gemv_bf16": [_P, c_long, _P, _P, c_float, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],
     "ifab_gemv_rows_bf16": [_P, c_long, _P, _P, c_float, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],
@@ -256,7 +257,7 @@ def load(build: bool = True, units=None):
                 continue
             fn.argtypes = sig
             fn.restype = c_int
-        for name, n in (("ifab_int4_bytes", 5), ("ifab_int4_gemm_scratch", 2), ("ifab_pages_work_words", 3)):
+        for name, n in (("ifab_int4_bytes", 5), ("ifab_int4_gemm_scratch", 2), ("ifab_pages_work_words", 3), ("ifab_shared_prefix_scratch", 5)):
             fn = getattr(lib, name, None)
             if fn is not None:
                 fn.argtypes, fn.restype = [c_int] * n, c_u64

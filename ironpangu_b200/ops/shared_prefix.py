@@ -1,0 +1,85 @@
+"""Attention of query rows that share a long prefix, whose keys and values are read once for all of them (``csrc/kernels/shared_prefix.cu``): decode steps of several continuations of
+one prompt, or questions behind one document. ``ops.decode.gqa_decode_attention`` reads them once for every row."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+BF16, I32 = torch.bfloat16, torch.int32
+MAX_GROUPS = 64
+MAX_ROWS = 1 << 20
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(f"shared_prefix: {what}")
+
+
+def scratch_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, groups: int = 1) -> int:
+    """Bytes that :func:`attention` takes as ``scratch`` for a call of so many rows (and for any of fewer in as many groups, the most of all of them)."""
+    _need(rows >= 0 and groups >= 0 and kv_heads >= 1 and heads % kv_heads == 0, f"{rows} rows of {heads} heads over {kv_heads} in {groups} groups")
+    return max((_lib.load().ifab_shared_prefix_scratch(t, heads, kv_heads, head_dim, groups) for t in range(1, rows + 1)), default=0)
+
+
+def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor, groups: torch.Tensor, *, heads: int,
+              kv_heads: int, head_dim: int, scale: float, scratch: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, status_ptr: Optional[int] = None) -> torch.Tensor:
+    """Softmax attention of bf16 rows ``q`` ``[T, >= heads * head_dim]`` (the q columns of a packed projection's rows) over the positions up to their own. ``out`` ``[T, heads * head_dim]`` bf16.
+
+    ``positions`` / ``slots`` int32 ``[T]``: a row's position (negative: nobody's row, whose result is left as it was) and the slot of its sequence; ``page_table`` int32 ``[slots, pages of one]``;
+    caches bf16 ``[pages, page_tokens, kv_heads, head_dim]`` that hold the keys and values of these rows already. ``groups`` int32 ``[n, 4]`` on the device, up to 64: first row, rows, shared
+    positions, slot. The rows of a group see the positions below the shared ones through that slot's pages, which are read once for all, and the others through their own; a row whose own position
+    lies within the prefix sees the prefix up to it. Groups come in the order of their rows; rows that none names see everything through their own slot; a group of no rows counts as none.
+
+    Heads of 64 or 128 columns, up to 16 of them over a key head. Scores, maxima, sums and sums of values are f32, weights enter their products with 15 bits, the result is rounded once. Pages that
+    are not there, slots, positions and groups out of range are skipped and set ``IFAB_STATUS_BAD_INDEX`` in the status word; a row that sees nothing gets zeros. ``scratch``: uint8 on 16 bytes,
+    :func:`scratch_bytes`; calls that may run at the same time need one each."""
+    dev, T = q.get_device(), q.shape[0]
+    if not (q.dim() == 2 and q.dtype is BF16 and dev >= 0 and q.stride(1) == 1 and kv_heads >= 1 and heads % kv_heads == 0 and heads // kv_heads <= 16 and head_dim in (64, 128)
+            and q.shape[1] >= heads * head_dim and T <= MAX_ROWS):
+        _need(q.dim() == 2 and q.dtype == BF16 and (q.stride(1) == 1), "queries must be bf16 [T, heads * head_dim], columns contiguous")
+        _need(dev >= 0, "the queries are on the host")
+        _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0 and heads // kv_heads <= 16 and head_dim in (64, 128), f"{heads} heads over {kv_heads} of {head_dim} columns are not supported")
+        _need(T <= MAX_ROWS, f"{T} rows are not supported")
+        _need(False, f"queries of {q.shape[1]} columns for {heads} heads of {head_dim}")
+    pages, pt = k_cache.shape[:2] if k_cache.dim() == 4 else (0, 0)
+    for t, what in ((k_cache, "keys"), (v_cache, "values")):
+        if not (t.dtype is BF16 and t.get_device() == dev and t.shape == (pages, pt, kv_heads, head_dim) and t.is_contiguous() and pages > 0 and pt > 0):
+            _need(False, f"{what} must be contiguous bf16 [pages, page_tokens, {kv_heads}, {head_dim}] beside the queries")
+    for t, what in ((positions, "positions"), (slots, "slots")):
+        if not (t.dtype is I32 and t.shape == (T,) and t.get_device() == dev and (T < 2 or t.stride(0) == 1)):
+            _need(False, f"{what} must be contiguous int32 [{T}] beside the queries")
+    for t, what in ((page_table, "page_table"), (groups, "groups")):
+        if not (t.dim() == 2 and t.dtype is I32 and t.get_device() == dev and t.is_contiguous()):
+            _need(False, f"{what} must be contiguous int32 beside the queries")
+    n = groups.shape[0]
+    if not (n <= MAX_GROUPS and groups.shape[1] == 4):
+        _need(False, f"groups must be [up to {MAX_GROUPS}, 4]")
+    num_slots, max_pages = page_table.shape
+    if not (num_slots >= 1 and max_pages >= 1 and pages * pt < 1 << 31 and max_pages * pt < (1 << 31) - 128):
+        _need(False, f"{pages} pages of {pt} positions, {max_pages} of {num_slots} slots are not supported")
+    if out is None:
+        out = torch.empty(T, heads * head_dim, dtype=BF16, device=q.device)
+    elif not (out.dtype is BF16 and out.shape == (T, heads * head_dim) and out.get_device() == dev and out.stride(1) == 1 and (T < 2 or out.stride(0) >= heads * head_dim)):
+        _need(False, f"the output must be bf16 [{T}, {heads * head_dim}] beside the queries, its rows apart")
+    if T == 0:
+        return out
+    lib = _lib.load()
+    need = lib.ifab_shared_prefix_scratch(T, heads, kv_heads, head_dim, n)
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif not (scratch.dtype is torch.uint8 and scratch.get_device() == dev and scratch.is_contiguous() and scratch.numel() >= need):
+        _need(False, f"scratch must be {need} bytes (uint8) beside the queries")
+    ldq, ldo = (q.stride(0), out.stride(0)) if T > 1 else (heads * head_dim, heads * head_dim)
+    qp, kp, vp, op, sp, gp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), scratch.data_ptr(), groups.data_ptr()
+    if (qp | kp | vp | op | sp | gp) % 16 or ldq % 8 or ldo % 8:
+        _need(False, "rows, caches, groups and scratch must lie on 16 bytes")
+    args = (qp, ldq, kp, vp, positions.data_ptr(), slots.data_ptr(), page_table.data_ptr(), num_slots, max_pages, pt, pages, gp, n, scale, T, heads, kv_heads, head_dim, sp, scratch.numel(), op, ldo,
+            status_ptr)
+    if dev == torch.cuda.current_device():
+        _lib.check(lib.ifab_shared_prefix_attention(*args, _lib.current_stream(dev)), "shared_prefix.attention")
+    else:
+        _lib.call_on(dev, "ifab_shared_prefix_attention", *args)
+    return out
