@@ -36,6 +36,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
   constexpr int WK = WARPS / WM, KW = KEYS / WK;                // warps of other keys, keys of a warp
   __shared__ int rows[STAGES + 1][KEYS];
   __shared__ int whole[STAGES + 1][2];
+  __shared__ long pair_q[16 * WM], pair_part[16 * WM];          // where a pair's query and result lie, -1: nobody's
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
   const int wm = warp % WM, wk = warp / WM;
   const uint32_t ring = smem_addr(smem);
@@ -70,6 +71,13 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
   };
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) locate(i);
+  if (threadIdx.x >= NT - 16 * WM) {
+    const int i = threadIdx.x - (NT - 16 * WM);
+    int t, h;
+    const bool live = pair(i, &t, &h);
+    pair_q[i] = live ? (long)t * p.ldq + (long)h * HD : -1;
+    pair_part[i] = live ? p.part_of(t, h, part) : -1;
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) load(i);
@@ -79,8 +87,8 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
     const bf16* src[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      int t, h;
-      src[e] = pair(wm * 16 + g + 8 * e, &t, &h) ? p.q + (long)t * p.ldq + (long)h * HD + c2 : nullptr;
+      const long at = pair_q[wm * 16 + g + 8 * e];
+      src[e] = at >= 0 ? p.q + at + c2 : nullptr;
     }
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i)
@@ -178,8 +186,8 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
     float* sm_acc = reinterpret_cast<float*>(smem) + warp * 16 * HD;
     float2* sm_ml = reinterpret_cast<float2*>(smem + R::BYTES);
     if ((lane & 3) == 0) {
-      sm_ml[warp * 16 + g] = make_float2(m[0], l[0]);
-      sm_ml[warp * 16 + g + 8] = make_float2(m[1], l[1]);
+      sm_ml[warp * 16 + g] = prefix_sums(m[0], l[0]);
+      sm_ml[warp * 16 + g + 8] = prefix_sums(m[1], l[1]);
     }
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) {
@@ -188,8 +196,8 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
     }
     __syncthreads();
     for (int i = warp; i < 16 * WM; i += WARPS) {
-      int t, h;
-      if (!pair(i, &t, &h)) continue;
+      const long at = pair_part[i];
+      if (at < 0) continue;
       float w[WK], M = -INFINITY, L = 0.f;
 #pragma unroll
       for (int k = 0; k < WK; ++k) M = fmaxf(M, w[k] = sm_ml[(k * WM + i / 16) * 16 + i % 16].x);
@@ -198,7 +206,6 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
         w[k] = w[k] == -INFINITY ? 0.f : exp2f(w[k] - M);
         L += w[k] * sm_ml[(k * WM + i / 16) * 16 + i % 16].y;
       }
-      const long at = p.part_of(t, h, part);
       for (int c = lane * 2; c < HD; c += 64) {
         float2 v = make_float2(0.f, 0.f);
 #pragma unroll
@@ -215,12 +222,11 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      int t, h;
-      if (!pair(wm * 16 + g + 8 * e, &t, &h)) continue;
-      const long at = p.part_of(t, h, part);
+      const long at = pair_part[wm * 16 + g + 8 * e];
+      if (at < 0) continue;
 #pragma unroll
       for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<float2*>(p.parts + at * HD + 8 * j + c2) = make_float2(acc[j][2 * e], acc[j][2 * e + 1]);
-      if ((lane & 3) == 0) p.sums[at] = make_float2(m[e], l[e]);
+      if ((lane & 3) == 0) p.sums[at] = prefix_sums(m[e], l[e]);
     }
   }
 }
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
     const PrefixOwn own = p.own(t0, p.naming(t0));
     const int per = p.per_split(own.end - own.begin, p.own_splits), begin = own.begin + split * per;
     if (begin >= own.end) return;
-    attend<HD, 1>(p, smem, begin, min(begin + per, own.end), own.slot, kvh, p.prefix_splits + split, [&](int i, int* t, int* h) {
+    attend<HD, 1>(p, smem, begin, min(begin + per, own.end), own.slot, kvh, p.streams * p.prefix_splits + split, [&](int i, int* t, int* h) {
       *t = t0;
       *h = kvh * p.G + i;
       return i < p.G;
@@ -266,37 +272,63 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
   }
 }
 
-// a warp per (row, head)
-template <int HD>
+// W warps per (row, head), each every W-th part, several parts' loads in flight
+template <int HD, int W>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(PrefixParams p, bf16* out, long ldo) {
+  constexpr int E = HD / 32, AT_ONCE = 4;
+  __shared__ float sm[W > 1 ? W : 1][W > 1 ? HD + 1 : 1];
   grid_dep_launch();
   grid_dep_wait();
-  const long pair = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = (int)(pair / p.Hq), h = (int)(pair % p.Hq), lane = threadIdx.x & 31;
-  if (t >= p.T || p.positions[t] < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w0 = warp % W;
+  const long pair = (long)blockIdx.x * (4 / W) + warp / W;
+  const int t = (int)(pair / p.Hq), h = (int)(pair % p.Hq);
+  if (t >= p.T || p.positions[t] < 0) return;    // (with W = 4 a whole CTA)
   const PrefixGroup gr = p.naming(t);
   const PrefixOwn own = p.own(t, gr);
   const int n = p.sees(gr, t) ? gr.shared : 0, own_n = own.end - own.begin;
-  const int ns = n > 0 ? (n + p.per_split(n, p.prefix_splits) - 1) / p.per_split(n, p.prefix_splits) : 0;
-  const int no = own_n > 0 ? (own_n + p.per_split(own_n, p.own_splits) - 1) / p.per_split(own_n, p.own_splits) : 0;
+  const int per = p.per_split(n, max(1, p.prefix_splits)), own_per = p.per_split(own_n, p.own_splits);
+  const int ns = n > 0 ? (n + per - 1) / per * p.streams : 0, no = own_n > 0 ? (own_n + own_per - 1) / own_per : 0;
   const long base = p.part_of(t, h, 0);
-  auto slot_of = [&](int i) { return base + (i < ns ? i : p.prefix_splits + i - ns); };
+  auto slot_of = [&](int i) { return base + (i < ns ? i : p.streams * p.prefix_splits + i - ns); };
   float M = -INFINITY;
   for (int i = lane; i < ns + no; i += 32) M = fmaxf(M, p.sums[slot_of(i)].x);
   M = warp_max(M);
-  constexpr int E = HD / 32;
   float v[E] = {}, L = 0.f;
-  for (int i = 0; i < ns + no; ++i) {
-    const long s = slot_of(i);
-    const float2 ml = p.sums[s];
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-    if (w == 0.f) continue;                      // (an infinite value that weighs nothing is nothing)
-    L += w * ml.y;
+  for (int i0 = w0; i0 < ns + no; i0 += AT_ONCE * W) {
+    float2 ml[AT_ONCE], a[AT_ONCE][E / 2];
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 a = *reinterpret_cast<const float2*>(p.parts + s * HD + lane * E + e);
-      v[e] += w * a.x;
-      v[e + 1] += w * a.y;
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int i = i0 + k * W;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (i >= ns + no) continue;
+      const long s = slot_of(i);
+      ml[k] = p.sums[s];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) a[k][e] = *reinterpret_cast<const float2*>(p.parts + s * HD + lane * E + 2 * e);
+    }
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const float w = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - M);
+      if (w == 0.f) continue;                    // nothing, or an infinite value that weighs nothing
+      L += w * ml[k].y;
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        v[2 * e] += w * a[k][e].x;
+        v[2 * e + 1] += w * a[k][e].y;
+      }
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sm[w0][lane * E + e] = v[e];
+    if (lane == 0) sm[w0][HD] = L;
+    __syncthreads();
+    if (w0) return;
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+      L += sm[k][HD];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] += sm[k][lane * E + e];
     }
   }
   const float inv = L != 0.f ? 1.f / L : 0.f;      // (a NaN among the scores stays one)
@@ -305,33 +337,42 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(PrefixParams p, bf16*
   for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(v[e] * inv, v[e + 1] * inv);
 }
 
+// how a call is shared out
 struct Plan {
-  int wm, tiles, prefix_splits, own_splits;
+  int wm, tiles, prefix_splits, own_splits, streams, least;     // wm 0: the prefix on tcgen05
 };
 Plan plan_of(int T, int Hkv, int G, int groups) {
-  Plan a;
+  Plan a{};
+  auto splits = [](long items, long ctas, int most) { return (int)std::max(1l, std::min((long)most, (ctas + items - 1) / std::max(1l, items))); };
   const int rows = groups ? (T + groups - 1) / groups * G : 1;
-  a.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  a.tiles = groups ? T * G / (16 * a.wm) + groups : 0;                  // at most, however the rows are shared out
-  auto splits = [](long items, int most) { return (int)std::max(1l, std::min((long)most, (296 + items - 1) / std::max(1l, items))); };
-  a.prefix_splits = groups ? splits((long)a.tiles * Hkv, 64) : 0;
-  a.own_splits = splits((long)T * Hkv, 16);
+  a.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+  a.streams = a.wm ? 1 : 2;
+  const int tile = a.wm ? 16 * a.wm : 256;
+  a.tiles = groups ? (int)std::max((long)groups, ((long)T * G - groups) / tile + groups) : 0;        // at most, however the rows are shared out
+  a.prefix_splits = groups ? a.wm ? splits((long)a.tiles * Hkv, 296, 64) : std::max(1, std::min(148, (int)(148 / std::max(1l, (long)a.tiles * Hkv)))) : 0;
+  a.own_splits = splits((long)T * Hkv, 296, 16);
+  a.least = 128;
   return a;
 }
 
 template <int HD, int WM>
-int launch_parts(const PrefixParams& p, const Plan& a, cudaStream_t s) {
+int launch_parts(const PrefixParams& p, long prefix_items, cudaStream_t s) {
   auto k = prefix_parts_kernel<HD, WM>;
   if (int rc = opt_in_smem(k, Ring<HD>::SMEM)) return rc;
-  const long prefix_items = (long)a.tiles * p.Hkv * a.prefix_splits, items = prefix_items + (long)p.T * p.Hkv * a.own_splits;
+  const long items = prefix_items + (long)p.T * p.Hkv * p.own_splits;
   if (items > 0x7fffffff) return -1;
   return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)Ring<HD>::SMEM, s, p, (int)prefix_items);
 }
 template <int HD>
 int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream_t s) {
-  const int rc = a.wm == 1 ? launch_parts<HD, 1>(p, a, s) : a.wm == 2 ? launch_parts<HD, 2>(p, a, s) : launch_parts<HD, 4>(p, a, s);
-  if (rc) return rc;
-  return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)(((long)p.T * p.Hq + 3) / 4)), dim3(128), 0, s, p, out, ldo);
+  const long items = (long)a.tiles * p.Hkv * a.prefix_splits;
+  if (items > 0x7fffffff) return -1;
+  if (!a.wm)
+    if (int rc = launch_prefix_tiles(p, HD, items, s)) return rc;
+  if (int rc = a.wm == 2 ? launch_parts<HD, 2>(p, items, s) : launch_parts<HD, 1>(p, a.wm ? items : 0, s)) return rc;
+  const long pairs = (long)p.T * p.Hq;
+  if (a.streams * a.prefix_splits + a.own_splits > 4 && pairs <= 0x7fffffff) return launch_chain(prefix_merge_kernel<HD, 4>, dim3((unsigned)pairs), dim3(128), 0, s, p, out, ldo);
+  return launch_chain(prefix_merge_kernel<HD, 1>, dim3((unsigned)((pairs + 3) / 4)), dim3(128), 0, s, p, out, ldo);
 }
 
 }  // namespace
@@ -339,7 +380,7 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
 extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_dim, int groups) {
   if (T < 1 || Hkv < 1 || Hq % Hkv || groups < 0) return 0;
   const Plan a = plan_of(T, Hkv, Hq / Hkv, groups);
-  return (uint64_t)T * Hq * (a.prefix_splits + a.own_splits) * (head_dim + 2) * sizeof(float);
+  return (uint64_t)T * Hq * (a.streams * a.prefix_splits + a.own_splits) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
@@ -356,9 +397,9 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   p.num_slots = num_slots; p.max_pages = max_pages; p.page_tokens = page_tokens; p.num_pages = num_pages; p.groups = num_groups;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
-  p.prefix_splits = a.prefix_splits; p.own_splits = a.own_splits;
+  p.prefix_splits = a.prefix_splits; p.own_splits = a.own_splits; p.streams = a.streams; p.least = a.least;
   p.parts = (float*)scratch;
-  p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.prefix_splits + a.own_splits) * head_dim);
+  p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.streams * a.prefix_splits + a.own_splits) * head_dim);
   p.status = status;
   return head_dim == 64 ? launch<64>(p, a, (bf16*)out, ldo, (cudaStream_t)stream) : launch<128>(p, a, (bf16*)out, ldo, (cudaStream_t)stream);
 }

@@ -23,8 +23,9 @@ struct PrefixParams {
   float scale_log2;                              // of a score in powers of two
   int T, Hq, Hkv, G;
   int prefix_splits, own_splits;                 // stretches that a group's prefix, a row's own positions are shared out to at most
-  float* parts;                                  // [T, Hq, prefix_splits + own_splits, head_dim]: sums of values
-  float2* sums;                                  // [T, Hq, prefix_splits + own_splits]: maximum (in powers of two), sum of weights
+  int streams, least;                            // parts of a stretch of the prefix; fewest keys of one
+  float* parts;                                  // [T, Hq, streams prefix_splits + own_splits, head_dim]: sums of values
+  float2* sums;                                  // [T, Hq, streams prefix_splits + own_splits]: maximum (in powers of two), sum of weights
   uint32_t* status;
 
   // row of the caches; -1: there is none
@@ -62,11 +63,9 @@ struct PrefixParams {
     if (!g.rows) return {0, end, slots[t]};
     return end >= g.shared ? PrefixOwn{g.shared, end, slots[t]} : PrefixOwn{0, end, g.slot};       // a position within the prefix
   }
-  __device__ __forceinline__ int per_split(int n, int splits) const {
-    const int share = (n + splits - 1) / splits;
-    return max(128, (share + 63) / 64 * 64);
-  }
-  __device__ __forceinline__ long part_of(int t, int h, int i) const { return ((long)t * Hq + h) * (prefix_splits + own_splits) + i; }
+  // keys of a stretch: whole tiles of the kernels'
+  __device__ __forceinline__ int per_split(int n, int splits) const { return max(least, ((n + splits - 1) / splits + 127) / 128 * 128); }
+  __device__ __forceinline__ long part_of(int t, int h, int i) const { return ((long)t * Hq + h) * (streams * prefix_splits + own_splits) + i; }
 };
 
 // Weights of a softmax, powers of two, as two bf16 terms: both are cut off below the value, so that none is 0 or negative and an infinite value of a key stays infinite (as in
@@ -78,10 +77,15 @@ __device__ __forceinline__ float prefix_weight(float x) {       // 2^x; NaN stay
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
   return x;
 }
+// what a part leaves beside its sums of values: a NaN counts wherever its maximum lies
+__device__ __forceinline__ float2 prefix_sums(float m, float l) { return make_float2(l != l ? INFINITY : m, l); }
 __device__ __forceinline__ void two_terms(float a, float b, uint32_t* hi, uint32_t* lo) {
   const float a0 = __uint_as_float((__float_as_uint(a) - 1u) & 0xffff0000u), b0 = __uint_as_float((__float_as_uint(b) - 1u) & 0xffff0000u);
   *hi = __byte_perm(__float_as_uint(a0), __float_as_uint(b0), 0x7632);
   *lo = __byte_perm(__float_as_uint(a - a0), __float_as_uint(b - b0), 0x7632);
 }
+
+// shared_prefix_tiles.cu: `items` = tiles of 256 pairs, however the rows are shared out, by kv heads by stretches
+int launch_prefix_tiles(const PrefixParams& p, int head_dim, long items, cudaStream_t s);
 
 }  // namespace ifab
