@@ -341,11 +341,11 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(PrefixParams p, bf16*
 struct Plan {
   int wm, tiles, prefix_splits, own_splits, streams, least;     // wm 0: the prefix on tcgen05
 };
-Plan plan_of(int T, int Hkv, int G, int groups) {
+Plan plan_of(int T, int Hkv, int G, int groups, bool tiles) {          // tiles: pages that tcgen05's form takes
   Plan a{};
   auto splits = [](long items, long ctas, int most) { return (int)std::max(1l, std::min((long)most, (ctas + items - 1) / std::max(1l, items))); };
   const int rows = groups ? (T + groups - 1) / groups * G : 1;
-  a.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+  a.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : tiles ? 0 : 4;
   a.streams = a.wm ? 1 : 2;
   const int tile = a.wm ? 16 * a.wm : 256;
   a.tiles = groups ? (int)std::max((long)groups, ((long)T * G - groups) / tile + groups) : 0;        // at most, however the rows are shared out
@@ -369,7 +369,7 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
   if (items > 0x7fffffff) return -1;
   if (!a.wm)
     if (int rc = launch_prefix_tiles(p, HD, items, s)) return rc;
-  if (int rc = a.wm == 2 ? launch_parts<HD, 2>(p, items, s) : launch_parts<HD, 1>(p, a.wm ? items : 0, s)) return rc;
+  if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, items, s) : a.wm == 2 ? launch_parts<HD, 2>(p, items, s) : launch_parts<HD, 1>(p, a.wm ? items : 0, s)) return rc;
   const long pairs = (long)p.T * p.Hq;
   if (a.streams * a.prefix_splits + a.own_splits > 4 && pairs <= 0x7fffffff) return launch_chain(prefix_merge_kernel<HD, 4>, dim3((unsigned)pairs), dim3(128), 0, s, p, out, ldo);
   return launch_chain(prefix_merge_kernel<HD, 1>, dim3((unsigned)((pairs + 3) / 4)), dim3(128), 0, s, p, out, ldo);
@@ -379,8 +379,8 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
 
 extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_dim, int groups) {
   if (T < 1 || Hkv < 1 || Hq % Hkv || groups < 0) return 0;
-  const Plan a = plan_of(T, Hkv, Hq / Hkv, groups);
-  return (uint64_t)T * Hq * (a.streams * a.prefix_splits + a.own_splits) * (head_dim + 2) * sizeof(float);
+  const Plan a = plan_of(T, Hkv, Hq / Hkv, groups, true), b = plan_of(T, Hkv, Hq / Hkv, groups, false);
+  return (uint64_t)T * Hq * (std::max(a.streams * a.prefix_splits, b.streams * b.prefix_splits) + a.own_splits) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
@@ -389,7 +389,7 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   if (T < 1 || T > 1 << 20 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || (head_dim != 64 && head_dim != 128) || num_groups < 0 || num_groups > 64 || (num_groups && !groups)) return -1;
   if (num_slots < 1 || max_pages < 1 || page_tokens < 1 || num_pages < 1 || (long)num_pages * page_tokens > 0x7fffffff || (long)max_pages * page_tokens > 0x7fffffff - 2 * KEYS) return -1;
   if (ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)scratch | (uintptr_t)groups) % 16) return -1;
-  const Plan a = plan_of(T, Hkv, Hq / Hkv, num_groups);
+  const Plan a = plan_of(T, Hkv, Hq / Hkv, num_groups, page_tokens % 8 == 0);
   if (ifab_shared_prefix_scratch(T, Hq, Hkv, head_dim, num_groups) > scratch_bytes) return -5;
   PrefixParams p;
   p.q = (const bf16*)q; p.ldq = ldq; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache;

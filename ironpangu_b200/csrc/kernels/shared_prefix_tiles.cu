@@ -7,7 +7,8 @@
 //                    of two; then the sums of values are rescaled in place), weights back as two bf16 terms in the scores' place
 //   warp 8           tensor memory and the products: S = Q K^T with both operands from shared memory, O += P V with P from tensor memory. V lies as it does in its pages, so it is an operand whose
 //                    columns run along the keys' rows (MN-major)
-//   warps 12-15      keys and values into rings of tiles in shared memory, 128-byte swizzle, by cp.async: a key's row may lie in any page, and one that is not there is read as zeros
+//   warps 12, 13     keys, values into rings of tiles in shared memory, 128-byte swizzle: a lane a box of rows of one page. (By cp.async an SM took in 19 bytes a cycle, however many were under way:
+//                    1024 rows over 16384 positions 814 us.)
 //
 // What each thread of a tile costs is balanced: 1536 cycles of products (a third of them for the weights' second terms, without which the result would be off by half as much again as its own
 // rounding) and about as many instructions of softmax.
@@ -20,7 +21,7 @@ using namespace ifab::tc;
 
 namespace {
 
-constexpr int TILE = 128, NT = 512, PRODUCERS = 128;
+constexpr int TILE = 128, NT = 512;
 constexpr uint32_t SPIN_LIMIT = 4000000u;
 
 template <int HD>
@@ -31,7 +32,7 @@ struct Layout {
 };
 template <int STAGES>
 struct Bars {
-  uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_ready[2], o_full[2], drained;
+  uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_ready[2], o_full[2], cut, drained;
   uint32_t tmem;
   int abort, holes;
 };
@@ -64,12 +65,8 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void copy16_zero(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-
 template <int HD>
-__global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
+__global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PrefixParams p, int box) {
   using L = Layout<HD>;
   constexpr int ST = L::STAGES;
   extern __shared__ unsigned char smem_raw[];
@@ -79,8 +76,8 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&B->k_full[s], PRODUCERS / 32);
-      mbar_init(&B->v_full[s], PRODUCERS / 32);
+      mbar_init(&B->k_full[s], 1);
+      mbar_init(&B->v_full[s], 1);
       mbar_init(&B->k_empty[s], 1);
       mbar_init(&B->v_empty[s], 1);
     }
@@ -89,9 +86,12 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
       mbar_init(&B->p_ready[x], 4);
       mbar_init(&B->o_full[x], 1);
     }
+    mbar_init(&B->cut, 1);
     mbar_init(&B->drained, 1);
     B->abort = B->holes = 0;
     mbar_fence_init();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
   }
   if (warp == 8) tmem_alloc(&B->tmem, 512);      // S of the streams at 0 and 128, O at 256 and 384. Ahead of the launch of dependents, which might hold some and wait for this kernel
   tc_fence_before();
@@ -120,7 +120,6 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
   const int x0 = tile * 2 * TILE, pairs = gr.rows * p.G, nt = (end - begin + TILE - 1) / TILE;
   const bool two = pairs - x0 > TILE;            // two halves of pairs, or two streams of keys
   const int units = two ? 2 * nt : nt;           // products of scores: unit u is stream u & 1
-  const long kv_elems = (long)p.Hkv * HD;
 
   for (int i = begin / p.page_tokens + tid; i <= (end - 1) / p.page_tokens; i += NT)
     if (p.row_of(i * p.page_tokens, gr.slot) < 0) B->holes = 1;
@@ -140,7 +139,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
   };
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const int X = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16, s_addr = tmem + lane_addr + X * 128, o_addr = tmem + lane_addr + 256 + X * 128;
     const int steps = two ? nt : (nt - X + 1) / 2;
@@ -150,25 +149,33 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
     for (int j = 0; j < steps; ++j) {
       if (!__all_sync(0xffffffffu, mbar_wait(&B->s_full[X], j & 1, SPIN_LIMIT) && !*abort_flag)) { ok = false; break; }
       tc_fence_after();
-      float s[TILE];
-#pragma unroll
-      for (int c = 0; c < TILE; c += 32) tmem_ld_32x32(s_addr + c, s + c);
-      tmem_ld_wait();
       const int key0 = begin + (two ? j : 2 * j + X) * TILE;
-      if (holes || key0 + TILE > end) {
-#pragma unroll
-        for (int c = 0; c < TILE; c += 32) {
-          uint32_t there = 0;
+      if (holes || key0 + TILE > end) {          // keys that are not there: their scores are put out in place
 #pragma unroll 1
-          for (int i = 0; i < 32; ++i) there |= (uint32_t)(key0 + c + i < end && !(holes && p.row_of(key0 + c + i, gr.slot) < 0)) << i;
+        for (int c = 0; c < TILE; c += 16) {
+          uint32_t s[16], there = 0;
+          tmem_ld_32x16(s_addr + c, s);
+          tmem_ld_wait();
+#pragma unroll 1
+          for (int i = 0; i < 16; ++i) there |= (uint32_t)(key0 + c + i < end && !(holes && p.row_of(key0 + c + i, gr.slot) < 0)) << i;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(there >> i & 1)) s[c + i] = -INFINITY;
+          for (int i = 0; i < 16; ++i)
+            if (!(there >> i & 1)) s[i] = 0xff800000u;
+          tmem_st_32x16(s_addr + c, s);
         }
+        tmem_st_wait();
       }
-      float mx[4] = {s[0], s[1], s[2], s[3]};
+      // Two passes over the scores, 64 and 32 at a time: all 128 in registers made a loop of 40 KB, and the warps waited for instructions
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 4; i < TILE; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+      for (int c = 0; c < TILE; c += 64) {
+        float s[64];
+        tmem_ld_32x32(s_addr + c, s);
+        tmem_ld_32x32(s_addr + c + 32, s + 32);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+      }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
       const bool moved = top > m_ref + 8.f;      // also for the first key (m_ref = -inf)
       if (__any_sync(0xffffffffu, moved)) {
@@ -176,7 +183,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
         l *= corr;
         if (moved) m_ref = top;
         if (j > 0) {                             // the product before has ended: these scores follow it in the pipe
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < HD; c += 16) {
             uint32_t v[16];
             tmem_ld_32x16(o_addr + c, v);
@@ -189,18 +196,26 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
       }
       const float from = m_ref == -INFINITY ? 0.f : m_ref;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      // 32 scores become 16 words of first terms and 16 of second terms, in their own place
+#pragma unroll 1
+      for (int c = 0; c < TILE; c += 64) {
+        float s[64];
+        tmem_ld_32x32(s_addr + c, s);
+        tmem_ld_32x32(s_addr + c + 32, s + 32);
+        tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < TILE; c += 32) {
-        uint32_t hi[16], lo[16];
+        for (int half = 0; half < 64; half += 32) {
+          uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float a = prefix_weight(fmaf(s[c + 2 * i], p.scale_log2, -from)), b = prefix_weight(fmaf(s[c + 2 * i + 1], p.scale_log2, -from));
-          sum[(2 * i) & 3] += a;
-          sum[(2 * i + 1) & 3] += b;
-          two_terms(a, b, &hi[i], &lo[i]);
+          for (int i = 0; i < 16; ++i) {
+            const float a = prefix_weight(fmaf(s[half + 2 * i], p.scale_log2, -from)), b = prefix_weight(fmaf(s[half + 2 * i + 1], p.scale_log2, -from));
+            sum[(2 * i) & 3] += a;
+            sum[(2 * i + 1) & 3] += b;
+            two_terms(a, b, &hi[i], &lo[i]);
+          }
+          tmem_st_32x16(s_addr + c + half, hi);
+          tmem_st_32x16(s_addr + c + half + 16, lo);
         }
-        tmem_st_32x16(s_addr + c / 2, hi);
-        tmem_st_32x16(s_addr + 64 + c / 2, lo);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
@@ -231,7 +246,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
       if (two) p.sums[at + 1] = make_float2(-INFINITY, 0.f);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8 && lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc_bf16(TILE, TILE), idesc_o = umma_idesc_bf16(TILE, HD) | 1u << 16;      // V's columns run along the rows
       auto scores = [&](int u) {
@@ -260,7 +275,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
         for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int k = 0; k < TILE / 16; ++k)
-            umma_ta(tmem + 256 + X * 128, tmem + X * 128 + term * 64 + k * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, j > 0 || term > 0 || k > 0);
+            umma_ta(tmem + 256 + X * 128, tmem + X * 128 + (k >> 1) * 32 + term * 16 + (k & 1) * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, j > 0 || term > 0 || k > 0);
         if (!two || X == 1) umma_commit(&B->v_empty[s]);
         if (u + 2 >= units) umma_commit(&B->o_full[X]);
         if (u + 2 < units) ok = scores(u + 2);
@@ -270,53 +285,49 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(PrefixParams p) {
         umma_commit(&B->drained);
         mbar_wait(&B->drained, 0, SPIN_LIMIT);
       }
-    } else if (warp >= 12) {
-      // groups of copies: keys, then values, tile by tile. A group that has landed is told to the tensor cores' thread, by a warp for its share
-      const int pw = warp - 12;
-      constexpr int CH = HD / 8, PENDING = 3;
-      int issued = 0, told = 0;
-      auto tell = [&](int until) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        for (; told < until; ++told)
-          if (lane == 0) mbar_arrive(told & 1 ? &B->v_full[(told >> 1) % ST] : &B->k_full[(told >> 1) % ST]);
-      };
-      auto row_at = [&](int kt) {
-        const int pos = begin + kt * TILE + pw * 32 + lane;
-        if (kt >= nt || pos >= end) return -1;
-        const int row = p.row_of(pos, gr.slot);
-        if (row < 0 && p.status) atomicOr(p.status, IFAB_STATUS_BAD_INDEX);
-        return row;
+    } else if (warp == 12 || warp == 13) {
+      // a warp for keys, one for values; a lane a box (rows of one page, 64 columns). A page that is not there is asked for behind the caches' end: zeros
+      const bool values = warp == 13;
+      const CUtensorMap* map = values ? &map_v : &map_k;
+      uint64_t *full = values ? B->v_full : B->k_full, *empty = values ? B->v_empty : B->k_empty;
+      unsigned char* ring = smem + (values ? L::V : L::K);
+      const int b = lane / L::PANELS, panel = lane % L::PANELS;
+      const bool mine = b < TILE / box;
+      static_assert(TILE / 8 * L::PANELS <= 32, "a lane a box");
+      auto row_at = [&](int kt) {                // of this lane's box; the caches' end: there is none
+        const int key = begin + kt * TILE + b * box, row = mine && kt < nt && key < end ? p.row_of(key, gr.slot) : -2;
+        return row >= 0 ? row : p.num_pages * p.page_tokens - 1 - row;
       };
       bool ok = true;
-      int next = row_at(0);
-      for (int kt = 0; kt < nt && ok; ++kt) {
-        const int row = next, s = kt % ST;
+      int next = row_at(0), issued = 0;
+      for (int kt = 0; kt < nt; ++kt) {
+        const int s = kt % ST, row = next;
+        if (kt >= ST && !__all_sync(0xffffffffu, mbar_wait(&empty[s], (kt / ST - 1) & 1, SPIN_LIMIT) && !*abort_flag)) { ok = false; break; }
+        const bool cut = values && kt == nt - 1 && (end - begin) % TILE;       // rows behind the stretch: whatever they hold, it must not count
+        uint64_t* bar = cut ? &B->cut : &full[s];
+        if (lane == 0) mbar_expect_tx(bar, L::BYTES);
+        __syncwarp();
+        if (mine) tma_load_2d(ring + s * L::BYTES + panel * L::PANEL + b * box * 128, map, bar, kvh * HD + panel * 64, row);
+        issued = kt + 1;
+        if (row == p.num_pages * p.page_tokens && p.status) atomicOr(p.status, IFAB_STATUS_BAD_INDEX);
         next = row_at(kt + 1);
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          uint64_t* empty = part ? &B->v_empty[s] : &B->k_empty[s];
-          if (kt >= ST && !__all_sync(0xffffffffu, mbar_try_wait(empty, (kt / ST - 1) & 1))) {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            tell(issued);
-            if (!__all_sync(0xffffffffu, mbar_wait(empty, (kt / ST - 1) & 1, SPIN_LIMIT) && !*abort_flag)) { ok = false; break; }
+        if (cut) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&B->cut, 0, SPIN_LIMIT))) { ok = false; break; }
+          const int live = end - begin - kt * TILE;
+          for (int i = lane; i < (TILE - live) * L::PANELS * 8; i += 32) {
+            const int key = live + i / (L::PANELS * 8), c = i % (L::PANELS * 8);
+            *reinterpret_cast<uint4*>(ring + s * L::BYTES + (c >> 3) * L::PANEL + key * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
-          const bf16* cache = (part ? p.v_cache : p.k_cache) + (long)kvh * HD;
-          const uint32_t to = smem_u32(smem + (part ? L::V : L::K) + s * L::BYTES);
-#pragma unroll
-          for (int i = 0; i < CH; ++i) {
-            const int k = i * (32 / CH) + lane / CH, c = lane % CH, at = __shfl_sync(0xffffffffu, row, k), key = pw * 32 + k;
-            copy16_zero(to + (c >> 3) * L::PANEL + (key >> 3) * 1024 + (key & 7) * 128 + (((c & 7) ^ (key & 7)) << 4), cache + (at < 0 ? 0 : at * kv_elems + c * 8), at >= 0);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          ++issued;
-          asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
-          if (issued - PENDING > told) tell(issued - PENDING);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
         }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      if (ok) tell(issued);
-      else if (lane == 0) fail();
+      if (!ok) {                                 // what was requested lands before the CTA ends
+        if (lane == 0) fail();
+        for (int j = max(0, issued - ST); j < issued; ++j)
+          if (!(values && j == nt - 1 && (end - begin) % TILE)) mbar_wait(&full[j % ST], (j / ST) & 1, SPIN_LIMIT);
+      }
     }
   }
   tc_fence_before();
@@ -331,11 +342,20 @@ template <int HD>
 int launch(const PrefixParams& p, long items, cudaStream_t s) {
   auto k = prefix_tiles_kernel<HD>;
   if (int rc = opt_in_smem(k, Layout<HD>::SMEM)) return rc;
-  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)Layout<HD>::SMEM, s, p);
+  int box = TILE;                                // rows of a box: they never pass a page's end
+  while (p.page_tokens % box) box /= 2;
+  const uint64_t rows = (uint64_t)p.num_pages * p.page_tokens, cols = (uint64_t)p.Hkv * HD;
+  CUtensorMap map_k, map_v;
+  if (int rc = make_tmap_bf16_2d(&map_k, p.k_cache, rows, cols, cols, (uint32_t)box)) return rc;
+  if (int rc = make_tmap_bf16_2d(&map_v, p.v_cache, rows, cols, cols, (uint32_t)box)) return rc;
+  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)Layout<HD>::SMEM, s, map_k, map_v, p, box);
 }
 
 }  // namespace
 
 namespace ifab {
-int launch_prefix_tiles(const PrefixParams& p, int head_dim, long items, cudaStream_t s) { return head_dim == 64 ? launch<64>(p, items, s) : launch<128>(p, items, s); }
+int launch_prefix_tiles(const PrefixParams& p, int head_dim, long items, cudaStream_t s) {
+  if (p.page_tokens % 8) return -1;
+  return head_dim == 64 ? launch<64>(p, items, s) : launch<128>(p, items, s);
+}
 }  // namespace ifab
