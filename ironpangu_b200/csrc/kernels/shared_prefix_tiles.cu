@@ -37,13 +37,31 @@ struct Bars {
   int abort, holes;
 };
 
-// D[tmem] (+)= A[tmem] * B[smem]; issued by one thread
-__device__ __forceinline__ void umma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+// D[tmem] (+)= A B with A in shared or in tensor memory, and a commit, by the one lane that is elected. The whole warp comes by: operands that are the same in all lanes lie in uniform registers
+// then, where a lane's own would have to be brought there for every product (94 cycles a product, 64 of them its own, while the other warps compute)
+__device__ __forceinline__ void umma_elected(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ta_elected(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
       "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 // MN-major with 128-byte swizzle: rows of 64 columns; eight rows further 1024 bytes, 64 columns further a panel
@@ -65,6 +83,30 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
+// pairs of floats
+__device__ __forceinline__ uint64_t both(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float a) { return both(a, a); }
+__device__ __forceinline__ void halves(uint64_t v, float* a, float* b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float power_of_2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PrefixParams p, int box) {
   using L = Layout<HD>;
@@ -195,7 +237,8 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
         }
       }
       const float from = m_ref == -INFINITY ? 0.f : m_ref;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = twice(p.scale_log2), from2 = twice(-from), above2 = twice(1.f + 0x1p-20f);
+      uint64_t sum[2] = {0, 0};
       // 32 scores become 16 words of first terms and 16 of second terms, in their own place
 #pragma unroll 1
       for (int c = 0; c < TILE; c += 64) {
@@ -208,16 +251,25 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float a = prefix_weight(fmaf(s[half + 2 * i], p.scale_log2, -from)), b = prefix_weight(fmaf(s[half + 2 * i + 1], p.scale_log2, -from));
-            sum[(2 * i) & 3] += a;
-            sum[(2 * i + 1) & 3] += b;
-            two_terms(a, b, &hi[i], &lo[i]);
+            // two weights at a time: the first term is cut off, the second one is what that leaves and 2^-20 of the weight, so that no weight has one of 0
+            float a, b;
+            halves(fma2(both(s[half + 2 * i], s[half + 2 * i + 1]), scale2, from2), &a, &b);
+            a = power_of_2(a);
+            b = power_of_2(b);
+            const uint64_t ab = both(a, b);
+            sum[i & 1] = add2(sum[i & 1], ab);
+            float ra, rb;
+            halves(fma2(ab, above2, both(-__uint_as_float(__float_as_uint(a) & 0xffff0000u), -__uint_as_float(__float_as_uint(b) & 0xffff0000u))), &ra, &rb);
+            hi[i] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+            lo[i] = __byte_perm(__float_as_uint(ra), __float_as_uint(rb), 0x7632);
           }
           tmem_st_32x16(s_addr + c + half, hi);
           tmem_st_32x16(s_addr + c + half + 16, lo);
         }
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float even, odd;
+      halves(add2(sum[0], sum[1]), &even, &odd);
+      l += even + odd;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -247,42 +299,48 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 8 && lane == 0) {
+    if (warp == 8) {
       constexpr uint32_t idesc_s = umma_idesc_bf16(TILE, TILE), idesc_o = umma_idesc_bf16(TILE, HD) | 1u << 16;      // V's columns run along the rows
-      auto scores = [&](int u) {
-        const int kt = two ? u >> 1 : u, X = u & 1, s = kt % ST;
-        if (!mbar_wait(&B->k_full[s], (kt / ST) & 1, SPIN_LIMIT) || *abort_flag) return false;
-        tc_fence_after();
-        const uint32_t qa = smem_u32(smem + L::Q + (two ? X : 0) * L::BYTES), ka = smem_u32(smem + L::K + s * L::BYTES);
+      const auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+      const uint32_t base = uniform(smem_u32(smem)), tm = uniform(tmem), all = uniform((uint32_t)units);
+      const bool pair = uniform(two);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, SPIN_LIMIT)); };
+      auto keys = [&](uint32_t u) {
+        const uint32_t kt = pair ? u >> 1 : u;
+        return wait(&B->k_full[kt % ST], (kt / ST) & 1);
+      };
+      auto scores = [&](uint32_t u) {
+        const uint32_t kt = pair ? u >> 1 : u, X = u & 1, s = kt % ST;
+        const uint64_t da = umma_desc_sw128(base + L::Q + (pair ? X : 0) * L::BYTES), db = umma_desc_sw128(base + L::K + s * L::BYTES);
 #pragma unroll
-        for (int pp = 0; pp < L::PANELS; ++pp) {
-          const uint64_t da = umma_desc_sw128(qa + pp * L::PANEL), db = umma_desc_sw128(ka + pp * L::PANEL);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem + X * 128, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc_s, pp > 0 || k > 0);
-        }
-        umma_commit(&B->s_full[X]);
-        if (!two || X == 1) umma_commit(&B->k_empty[s]);
-        return true;
+        for (int k = 0; k < HD / 16; ++k) umma_elected(tm + X * 128, da + (uint64_t)((k >> 2) * (L::PANEL >> 4) + (k & 3) * 2), db + (uint64_t)((k >> 2) * (L::PANEL >> 4) + (k & 3) * 2), idesc_s, k > 0);
+        commit_elected(&B->s_full[X]);
+        if (!pair || X == 1) commit_elected(&B->k_empty[s]);
       };
       bool ok = true;
-      for (int u = 0; u < min(2, units) && ok; ++u) ok = scores(u);
-      for (int u = 0; u < units && ok; ++u) {
-        const int kt = two ? u >> 1 : u, X = u & 1, s = kt % ST, j = u >> 1;
-        if (!mbar_wait(&B->p_ready[X], j & 1, SPIN_LIMIT) || !mbar_wait(&B->v_full[s], (kt / ST) & 1, SPIN_LIMIT) || *abort_flag) { ok = false; break; }
+      for (uint32_t u = 0; u < min(2u, all) && ok; ++u) {
+        ok = keys(u);
         tc_fence_after();
-        const uint64_t dv = desc_rows(smem_u32(smem + L::V + s * L::BYTES), L::PANEL);
+        if (ok) scores(u);
+      }
+      for (uint32_t u = 0; u < all && ok; ++u) {
+        const uint32_t kt = pair ? u >> 1 : u, X = u & 1, s = kt % ST, j = u >> 1;
+        // the weights come last: what else is waited for costs the pipe nothing then
+        if (!wait(&B->v_full[s], (kt / ST) & 1) || (u + 2 < all && !keys(u + 2)) || *abort_flag || !wait(&B->p_ready[X], j & 1)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t dv = desc_rows(base + L::V + s * L::BYTES, L::PANEL);
 #pragma unroll
         for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int k = 0; k < TILE / 16; ++k)
-            umma_ta(tmem + 256 + X * 128, tmem + X * 128 + (k >> 1) * 32 + term * 16 + (k & 1) * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, j > 0 || term > 0 || k > 0);
-        if (!two || X == 1) umma_commit(&B->v_empty[s]);
-        if (u + 2 >= units) umma_commit(&B->o_full[X]);
-        if (u + 2 < units) ok = scores(u + 2);
+            umma_ta_elected(tm + 256 + X * 128, tm + X * 128 + (k >> 1) * 32 + term * 16 + (k & 1) * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, j > 0 || term > 0 || k > 0);
+        if (!pair || X == 1) commit_elected(&B->v_empty[s]);
+        if (u + 2 >= all) commit_elected(&B->o_full[X]);
+        if (u + 2 < all) scores(u + 2);
       }
       if (!ok) {
-        fail();
-        umma_commit(&B->drained);
+        if (lane == 0) fail();
+        commit_elected(&B->drained);
         mbar_wait(&B->drained, 0, SPIN_LIMIT);
       }
     } else if (warp == 12 || warp == 13) {
