@@ -128,6 +128,18 @@ inline int opt_in_smem(KernelT kernel, size_t smem) {
   return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
 }
 
+// The same once for a device and a kernel: half a microsecond of a call's host time
+template <auto Kernel>
+inline int opt_in_smem_once(size_t smem) {
+  static uint64_t done = 0;             // a bit a device; two threads that come at once do it twice
+  int dev;
+  if (int rc = (int)cudaGetDevice(&dev)) return rc;
+  if (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev & 1)) return 0;
+  if (int rc = opt_in_smem(Kernel, smem)) return rc;
+  if (dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
+  return 0;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Cross-GPU flag protocol. Flags are 64-bit epochs in memory that every rank maps. A writer
 // publishes its data with plain stores, then one thread issues a system-scope release store of

@@ -476,7 +476,7 @@ template <typename In>
 int launch(const DrawParams& p, int ranks, cudaStream_t s) {
   const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)p.slice * sizeof(float);
   auto k = draw_kernel<In>;
-  if (int rc = opt_in_smem(k, smem)) return rc;
+  if (int rc = opt_in_smem_once<draw_kernel<In>>((sizeof(Shared) + 15) / 16 * 16 + MAX_SLICE * sizeof(float))) return rc;
   return launch_chain_cluster(k, dim3((unsigned)(p.T * ranks)), dim3(NT), (unsigned)ranks, smem, s, p);
 }
 

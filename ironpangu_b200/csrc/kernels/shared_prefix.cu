@@ -3,13 +3,17 @@
 //   out[t, h] = sum_j softmax_j(scale q[t, h] . k[j, h / G]) v[j, h / G],  j = 0 .. pos_t
 //   positions j < n of a group's rows lie in the pages of the group's slot, j >= n in those of the row's own slot
 //
-// A softmax over two parts is put together from their maxima, sums and sums of values, so the parts are worked on by CTAs of their own, as are stretches of a long part:
+// A softmax over two parts is put together from their maxima, sums and sums of values, so the parts are worked on by CTAs of their own, as are stretches of a long part; each leaves m, l and O of
+// its rows and heads in the scratch.
 //
-//   parts kernel   one CTA per (tile of 16 WM rows x heads of a group, kv head, stretch of the prefix) and per (row, kv head, stretch of its own keys): m, l and O of each row and head into
-//                  the scratch. Products on the tensor cores as m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
-//   merge kernel   one warp per (row, head): the stretches' parts, weighted by e^(m - largest m), over the sum
-//
-// With few rows this is bound by the bytes of the prefix; a tile of 64 rows and heads is where m16n8k16 keeps up with them.
+//   up to 32 rows and heads in a group
+//     parts kernel   one CTA per (tile of 16 WM pairs of a group's rows and heads, kv head, stretch of the prefix) and per (row, kv head, stretch of its own keys): products on the tensor cores as
+//                    m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
+//     merge kernel   four warps per (row, head): the parts, weighted by e^(m - largest m), over the sum
+//   more
+//     tiles kernel   the prefix on tcgen05 (shared_prefix_tiles.cu)
+//     own kernel     one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result. With too few rows to fill the chip: the parts kernel without a
+//                    prefix and the merge kernel
 #include <algorithm>
 
 #include "mma16816.cuh"
@@ -19,66 +23,79 @@ using namespace ifab;
 
 namespace {
 
-constexpr int KEYS = 64, STAGES = 3, WARPS = 4, NT = 32 * WARPS;
+constexpr int NT = 128, OWN_STAGES = 2, OWN_CTAS = 3;
 
-template <int HD>
-struct Ring {
-  static constexpr int ROW = HD * 2, CH = HD / 8, STAGE = 2 * KEYS * ROW, BYTES = STAGES * STAGE;
-  static constexpr int SMEM = BYTES + WARPS * 16 * 8;          // behind the ring: maxima and sums of the warps
-  static_assert(WARPS * 16 * HD * 4 <= BYTES, "the warps' results take the ring's place");
+// What a unit of W warps (a CTA of four, or a warp by itself) has in shared memory: its ring of tiles of 16 W keys, where they lie, and where its pairs' queries and results lie (-1: nobody's)
+template <int HD, int W, int PAIRS, int STAGES_>
+struct alignas(128) Unit {
+  static constexpr int STAGES = STAGES_, KEYS = 16 * W, ROW = HD * 2, CH = HD / 8, STAGE = 2 * KEYS * ROW, RING = STAGES * STAGE;
+  unsigned char ring[RING];
+  int rows[STAGES + 1][KEYS];
+  int whole[STAGES + 1][2];
+  float2 ml[W * 16];
+  long query[PAIRS], part[PAIRS];
+  static_assert(W * 16 * HD * 4 <= RING, "the warps' results take the ring's place");
 };
 
-// One stretch of keys [begin, end) of the pages of `slot` against 16 WM (row, head) pairs. WM warps side by side have 16 pairs each, the others of a group of them other keys of a tile.
-// `pair(i, &t, &h)`: pair i's row and head; false: nobody's
-template <int HD, int WM, typename Pair>
-__device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* smem, int begin, int end, int slot, int kvh, int part, Pair pair) {
-  using R = Ring<HD>;
-  constexpr int WK = WARPS / WM, KW = KEYS / WK;                // warps of other keys, keys of a warp
-  __shared__ int rows[STAGES + 1][KEYS];
-  __shared__ int whole[STAGES + 1][2];
-  __shared__ long pair_q[16 * WM], pair_part[16 * WM];          // where a pair's query and result lie, -1: nobody's
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
+// One stretch of keys [begin, end) of the pages of `slot` against 16 WM pairs. WM warps side by side have 16 pairs each, the others other keys of a tile.
+// `pair(i, &t, &h)`: pair i's row and head; false: nobody's. `finish(i, M, L, v)`, by a warp: maxima, sums and sums of values of the pairs from i on, AT_ONCE of them, HD / 32 columns a lane
+template <int HD, int W, int WM, int STAGES, int AT_ONCE, typename Pair, typename Finish>
+__device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * WM, STAGES>& u, int begin, int end, int slot, int kvh, int part, Pair pair, Finish finish) {
+  using U = Unit<HD, W, 16 * WM, STAGES>;
+  constexpr int WK = W / WM, KEYS = U::KEYS, KW = KEYS / WK, N = 32 * W, E = HD / 32;      // warps of other keys, keys of a warp, threads of the unit
+  const int tid = threadIdx.x % N, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c2 = (lane & 3) * 2;
   const int wm = warp % WM, wk = warp / WM;
-  const uint32_t ring = smem_addr(smem);
+  const uint32_t ring = smem_addr(u.ring);
   const long kv_elems = (long)p.Hkv * HD;
   const int tiles = (end - begin + KEYS - 1) / KEYS;
-  // where the keys of tile i lie (two warps), -1: nowhere
-  auto locate = [&](int i) {
-    if (warp < 2 && i < tiles) {
-      const int key = begin + i * KEYS + threadIdx.x;
-      const int r = key < end ? p.row_of(key, slot) : -1;
-      rows[i % (STAGES + 1)][threadIdx.x] = r;
-      if (key < end && r < 0 && p.status) atomicOr(p.status, IFAB_STATUS_BAD_INDEX);
-      const bool all = __all_sync(0xffffffffu, r >= 0);
-      if (lane == 0) whole[i % (STAGES + 1)][warp] = all;
+  auto sync = [] {
+    if (W == 1) __syncwarp();
+    else __syncthreads();
+  };
+  // Where the keys of tile i lie, a thread a key; -1: nowhere. Asked for at a tile's start and noted at its end: the page table's answer takes as long as the tile
+  auto ask = [&](int i) {
+    const int key = begin + i * KEYS + tid;
+    return tid < KEYS && i < tiles && key < end ? p.row_of(key, slot) : -1;
+  };
+  auto note = [&](int i, int r) {
+    if (warp < (KEYS + 31) / 32 && i < tiles) {
+      if (tid < KEYS) u.rows[i % (STAGES + 1)][tid] = r;
+      if (tid < KEYS && begin + i * KEYS + tid < end && r < 0 && p.status) atomicOr(p.status, IFAB_STATUS_BAD_INDEX);
+      const bool all = __all_sync(0xffffffffu, r >= 0 || tid >= KEYS);
+      if (lane == 0) u.whole[i % (STAGES + 1)][warp] = all;
     }
   };
   auto load = [&](int i) {
     if (i < tiles) {
-      const uint32_t dst0 = ring + (i % STAGES) * R::STAGE;
-      const int ch = threadIdx.x % R::CH;
+      const uint32_t dst0 = ring + (i % STAGES) * U::STAGE;
+      const int ch = tid % U::CH;
 #pragma unroll
-      for (int j = 0; j < KEYS * R::CH / NT; ++j) {
-        const int key = threadIdx.x / R::CH + j * (NT / R::CH);
-        const int r = rows[i % (STAGES + 1)][key];
+      for (int j = 0; j < KEYS * U::CH / N; ++j) {
+        const int key = tid / U::CH + j * (N / U::CH);
+        const int r = u.rows[i % (STAGES + 1)][key];
         const long at = r < 0 ? 0 : r * kv_elems + (long)kvh * HD + ch * 8;
-        const uint32_t dst = dst0 + key * R::ROW + ((ch ^ (key & 7)) << 4);
+        const uint32_t dst = dst0 + key * U::ROW + ((ch ^ (key & 7)) << 4);
         copy16(dst, p.k_cache + at, r >= 0);
-        copy16(dst + KEYS * R::ROW, p.v_cache + at, r >= 0);
+        copy16(dst + KEYS * U::ROW, p.v_cache + at, r >= 0);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  {
+    int r[STAGES];
 #pragma unroll
-  for (int i = 0; i < STAGES; ++i) locate(i);
-  if (threadIdx.x >= NT - 16 * WM) {
-    const int i = threadIdx.x - (NT - 16 * WM);
+    for (int i = 0; i < STAGES; ++i) r[i] = ask(i);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) note(i, r[i]);
+  }
+  if (tid >= N - 16 * WM) {
+    const int i = tid - (N - 16 * WM);
     int t, h;
     const bool live = pair(i, &t, &h);
-    pair_q[i] = live ? (long)t * p.ldq + (long)h * HD : -1;
-    pair_part[i] = live ? p.part_of(t, h, part) : -1;
+    u.query[i] = live ? (long)t * p.ldq + (long)h * HD : -1;
+    u.part[i] = live ? p.part_of(t, h, part) : -1;
   }
-  __syncthreads();
+  sync();
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) load(i);
 
@@ -87,7 +104,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
     const bf16* src[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const long at = pair_q[wm * 16 + g + 8 * e];
+      const long at = u.query[wm * 16 + g + 8 * e];
       src[e] = at >= 0 ? p.q + at + c2 : nullptr;
     }
 #pragma unroll
@@ -103,9 +120,10 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
 
   for (int i = 0; i < tiles; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-    __syncthreads();                             // tile i has landed for all threads, tile i - 1 is read
+    sync();                                      // tile i has landed for all threads, tile i - 1 is read
+    const int ahead = ask(i + STAGES);
     load(i + STAGES - 1);
-    const uint32_t kb = ring + (i % STAGES) * R::STAGE + wk * KW * R::ROW, vb = kb + KEYS * R::ROW;
+    const uint32_t kb = ring + (i % STAGES) * U::STAGE + wk * KW * U::ROW, vb = kb + KEYS * U::ROW;
     float s[KW / 8][4];
 #pragma unroll
     for (int n = 0; n < KW / 8; ++n)
@@ -117,18 +135,18 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
       for (int n = 0; n < KW / 16; ++n) {
         uint32_t b[4];
         const int key = n * 16 + (lane >> 4) * 8 + (lane & 7), ch = 2 * kk + ((lane >> 3) & 1);
-        ldsm4(kb + key * R::ROW + ((ch ^ (key & 7)) << 4), b);
+        ldsm4(kb + key * U::ROW + ((ch ^ (key & 7)) << 4), b);
         mma16816(s[2 * n], q[kk][0], q[kk][1], q[kk][2], q[kk][3], b[0], b[1]);
         mma16816(s[2 * n + 1], q[kk][0], q[kk][1], q[kk][2], q[kk][3], b[2], b[3]);
       }
-    const bool all = whole[i % (STAGES + 1)][0] && whole[i % (STAGES + 1)][1];
+    const bool all = u.whole[i % (STAGES + 1)][0] && (KEYS <= 32 || u.whole[i % (STAGES + 1)][1]);
     float mn[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[n][e] *= p.scale_log2;
-        if (!all && rows[i % (STAGES + 1)][wk * KW + 8 * n + c2 + (e & 1)] < 0) s[n][e] = -INFINITY;
+        if (!all && u.rows[i % (STAGES + 1)][wk * KW + 8 * n + c2 + (e & 1)] < 0) s[n][e] = -INFINITY;
         mn[e >> 1] = fmaxf(mn[e >> 1], s[n][e]);
       }
 #pragma unroll
@@ -165,7 +183,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
       for (int j = 0; j < HD / 16; ++j) {
         uint32_t b[4];
         const int key = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * j + (lane >> 4);
-        ldsm4t(vb + key * R::ROW + ((ch ^ (key & 7)) << 4), b);
+        ldsm4t(vb + key * U::ROW + ((ch ^ (key & 7)) << 4), b);
         mma16816(acc[2 * j], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
         mma16816(acc[2 * j + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
         mma16816(acc[2 * j], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
@@ -173,68 +191,121 @@ __device__ __forceinline__ void attend(const PrefixParams& p, unsigned char* sme
       }
     }
     __syncwarp();
-    if (i + STAGES < tiles) locate(i + STAGES);
+    note(i + STAGES, ahead);
   }
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
   }
-  if constexpr (WK > 1) {                        // warps of the same pairs and other keys: the first one adds up, over the ring
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
-    float* sm_acc = reinterpret_cast<float*>(smem) + warp * 16 * HD;
-    float2* sm_ml = reinterpret_cast<float2*>(smem + R::BYTES);
-    if ((lane & 3) == 0) {
-      sm_ml[warp * 16 + g] = prefix_sums(m[0], l[0]);
-      sm_ml[warp * 16 + g + 8] = prefix_sums(m[1], l[1]);
-    }
+  // by pairs, over the ring: warps of the same pairs and other keys are added up
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  sync();
+  float* all_acc = reinterpret_cast<float*>(u.ring);
+  float* my_acc = all_acc + warp * 16 * HD;
+  if ((lane & 3) == 0) {
+    u.ml[warp * 16 + g] = prefix_sums(m[0], l[0]);
+    u.ml[warp * 16 + g + 8] = prefix_sums(m[1], l[1]);
+  }
 #pragma unroll
-    for (int j = 0; j < HD / 8; ++j) {
-      *reinterpret_cast<float2*>(sm_acc + g * HD + 8 * j + c2) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2*>(sm_acc + (g + 8) * HD + 8 * j + c2) = make_float2(acc[j][2], acc[j][3]);
-    }
-    __syncthreads();
-    for (int i = warp; i < 16 * WM; i += WARPS) {
-      const long at = pair_part[i];
-      if (at < 0) continue;
-      float w[WK], M = -INFINITY, L = 0.f;
+  for (int j = 0; j < HD / 8; ++j) {
+    *reinterpret_cast<float2*>(my_acc + g * HD + 8 * j + c2) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(my_acc + (g + 8) * HD + 8 * j + c2) = make_float2(acc[j][2], acc[j][3]);
+  }
+  sync();
+  for (int i0 = warp * AT_ONCE; i0 < 16 * WM; i0 += W * AT_ONCE) {
+    if (AT_ONCE == 1 ? u.part[i0] < 0 : i0 >= p.G) continue;             // (several at once: pairs of one row, all that there are come first)
+    float M[AT_ONCE], L[AT_ONCE], v[AT_ONCE][E];
 #pragma unroll
-      for (int k = 0; k < WK; ++k) M = fmaxf(M, w[k] = sm_ml[(k * WM + i / 16) * 16 + i % 16].x);
+    for (int n = 0; n < AT_ONCE; ++n) {
+      const int i = i0 + n;
+      float w[WK];
+      M[n] = -INFINITY;
+      L[n] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[n][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < WK; ++k) M[n] = fmaxf(M[n], w[k] = u.ml[(k * WM + i / 16) * 16 + i % 16].x);
 #pragma unroll
       for (int k = 0; k < WK; ++k) {
-        w[k] = w[k] == -INFINITY ? 0.f : exp2f(w[k] - M);
-        L += w[k] * sm_ml[(k * WM + i / 16) * 16 + i % 16].y;
+        const int at = (k * WM + i / 16) * 16 + i % 16;
+        w[k] = w[k] == -INFINITY ? 0.f : exp2f(w[k] - M[n]);
+        if (w[k] == 0.f) continue;               // nothing, or an infinite value that weighs nothing
+        L[n] += w[k] * u.ml[at].y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[n][e] += w[k] * all_acc[at * HD + lane * E + e];
       }
-      for (int c = lane * 2; c < HD; c += 64) {
-        float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < WK; ++k) {
-          const float2 a = *reinterpret_cast<const float2*>(reinterpret_cast<float*>(smem) + ((k * WM + i / 16) * 16 + i % 16) * HD + c);
-          v.x += w[k] * a.x;
-          v.y += w[k] * a.y;
-        }
-        *reinterpret_cast<float2*>(p.parts + at * HD + c) = v;
-      }
-      if (lane == 0) p.sums[at] = make_float2(M, L);
     }
-  } else {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const long at = pair_part[wm * 16 + g + 8 * e];
-      if (at < 0) continue;
-#pragma unroll
-      for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<float2*>(p.parts + at * HD + 8 * j + c2) = make_float2(acc[j][2 * e], acc[j][2 * e + 1]);
-      if ((lane & 3) == 0) p.sums[at] = prefix_sums(m[e], l[e]);
-    }
+    finish(i0, M, L, v);
   }
 }
 
-// grid: prefix items (stretch fastest, then kv head, then tile), then own items (stretch, kv head, row)
+template <int E>
+__device__ __forceinline__ void store_part(const PrefixParams& p, long at, float M, float L, const float (&v)[E], int lane) {
+  if (E == 4) *reinterpret_cast<float4*>(p.parts + at * (32 * E) + lane * E) = make_float4(v[0], v[1], v[E - 2], v[E - 1]);
+  else *reinterpret_cast<float2*>(p.parts + at * (32 * E) + lane * E) = make_float2(v[0], v[1]);
+  if (lane == 0) p.sums[at] = make_float2(M, L);
+}
+__device__ __forceinline__ float largest(const PrefixParams& p, long base, int n, int lane) {
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, p.sums[base + i].x);
+  return warp_max(M);
+}
+// Adds parts [first, last) of P pairs, `base` + k `apart`, to the L and v of a warp, relative to M, which is not below their maxima: S parts of each pair are requested together. Parts that weigh
+// nothing count as nothing, whatever they hold
+template <int E, int P, int S>
+__device__ __forceinline__ void add_parts(const PrefixParams& p, long base, long apart, int pairs, int first, int last, const float (&M)[P], float (&L)[P], float (&v)[P][E], int lane) {
+  for (int i0 = first; i0 < last; i0 += 32) {
+    float w[P];
+    uint32_t left = 0;
+#pragma unroll
+    for (int n = 0; n < P; ++n) {
+      const float2 ml = n < pairs && i0 + lane < last ? p.sums[base + n * apart + i0 + lane] : make_float2(-INFINITY, 0.f);
+      w[n] = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M[n]);
+      const float l = w[n] != 0.f ? w[n] * ml.y : 0.f;
+      L[n] += warp_sum(l);
+      left |= __ballot_sync(0xffffffffu, w[n] != 0.f);
+    }
+    const int some = left ? __ffs(left) - 1 : 0;         // what a place without a part reads, to no effect: loads that depend on nothing stay together
+    while (left) {
+      float a[P][S][E], by[P][S];
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        const int j = left ? __ffs(left) - 1 : some;
+#pragma unroll
+        for (int n = 0; n < P; ++n) {
+          by[n][k] = __shfl_sync(0xffffffffu, w[n], j);
+          if (!left) by[n][k] = 0.f;
+          const float* src = p.parts + (base + (n < pairs ? n : 0) * apart + i0 + j) * (32 * E) + lane * E;
+          if (E == 4) *reinterpret_cast<float4*>(a[n][k]) = *reinterpret_cast<const float4*>(src);
+          else *reinterpret_cast<float2*>(a[n][k]) = *reinterpret_cast<const float2*>(src);
+        }
+        left &= left - 1;
+      }
+#pragma unroll
+      for (int n = 0; n < P; ++n)
+#pragma unroll
+        for (int k = 0; k < S; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[n][e] = by[n][k] != 0.f ? fmaf(by[n][k], a[n][k][e], v[n][e]) : v[n][e];
+    }
+  }
+}
+template <int E>
+__device__ __forceinline__ void store_result(bf16* dst, float L, const float (&v)[E], int lane) {
+  const float inv = L != 0.f ? 1.f / L : 0.f;      // (a NaN among the scores stays one)
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(dst + lane * E + e) = __floats2bfloat162_rn(v[e] * inv, v[e + 1] * inv);
+}
+
+// Grid: prefix items (stretch fastest, then kv head, then tile), then own items (stretch, kv head, row). Every part of a row that is somebody's gets its sums, if only to say that it is nothing,
+// so that the merge need not know about groups
 template <int HD, int WM>
 __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int prefix_items) {
   extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const float2 nothing = make_float2(-INFINITY, 0.f);
   grid_dep_launch();
   grid_dep_wait();
   int item = blockIdx.x;
@@ -249,130 +320,166 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
       if (tile < tiles) break;
       tile -= tiles;
     }
-    const int per = p.per_split(gr.shared, p.prefix_splits), begin = split * per;
+    const int per = p.per_split(gr.shared, p.prefix_splits), begin = split * per, x0 = tile * 16 * WM;
+    for (int x = x0 + threadIdx.x; x < min(x0 + 16 * WM, gr.rows * p.G); x += NT) {
+      const int t = gr.first + x / p.G;
+      if (begin >= gr.shared || !p.sees(gr, t)) p.sums[p.part_of(t, kvh * p.G + x % p.G, split)] = nothing;
+    }
     if (begin >= gr.shared) return;
-    attend<HD, WM>(p, smem, begin, min(begin + per, gr.shared), gr.slot, kvh, split, [&](int i, int* t, int* h) {
-      const int x = tile * 16 * WM + i;
-      if (x >= gr.rows * p.G) return false;
-      *t = gr.first + x / p.G;
-      *h = kvh * p.G + x % p.G;
-      return p.sees(gr, *t);
-    });
+    auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, 3>*>(smem);
+    attend<HD, 4, WM, 3, 1>(
+        p, u, begin, min(begin + per, gr.shared), gr.slot, kvh, split,
+        [&](int i, int* t, int* h) {
+          const int x = x0 + i;
+          if (x >= gr.rows * p.G) return false;
+          *t = gr.first + x / p.G;
+          *h = kvh * p.G + x % p.G;
+          return p.sees(gr, *t);
+        },
+        [&](int i, const float (&M)[1], const float (&L)[1], const float (&v)[1][E]) { store_part<E>(p, u.part[i], M[0], L[0], v[0], lane); });
   } else {
     item -= prefix_items;
-    const int split = item % p.own_splits, kvh = item / p.own_splits % p.Hkv, t0 = item / p.own_splits / p.Hkv;
-    const PrefixOwn own = p.own(t0, p.naming(t0));
+    const int split = item % p.own_splits, kvh = item / p.own_splits % p.Hkv, t0 = item / p.own_splits / p.Hkv, prefix_parts = p.streams * p.prefix_splits;
+    const PrefixGroup gr = p.naming(t0);
+    const PrefixOwn own = p.own(t0, gr);
     const int per = p.per_split(own.end - own.begin, p.own_splits), begin = own.begin + split * per;
-    if (begin >= own.end) return;
-    attend<HD, 1>(p, smem, begin, min(begin + per, own.end), own.slot, kvh, p.streams * p.prefix_splits + split, [&](int i, int* t, int* h) {
-      *t = t0;
-      *h = kvh * p.G + i;
-      return i < p.G;
-    });
+    if (p.positions[t0] < 0) return;
+    if (!gr.rows && split == 0)
+      for (int i = threadIdx.x; i < p.G * prefix_parts; i += NT) p.sums[p.part_of(t0, kvh * p.G + i / prefix_parts, i % prefix_parts)] = nothing;
+    if (begin >= own.end) {
+      for (int i = threadIdx.x; i < p.G; i += NT) p.sums[p.part_of(t0, kvh * p.G + i, prefix_parts + split)] = nothing;
+      return;
+    }
+    auto& u = *reinterpret_cast<Unit<HD, 4, 16, 3>*>(smem);
+    attend<HD, 4, 1, 3, 1>(
+        p, u, begin, min(begin + per, own.end), own.slot, kvh, prefix_parts + split,
+        [&](int i, int* t, int* h) {
+          *t = t0;
+          *h = kvh * p.G + i;
+          return i < p.G;
+        },
+        [&](int i, const float (&M)[1], const float (&L)[1], const float (&v)[1][E]) { store_part<E>(p, u.part[i], M[0], L[0], v[0], lane); });
   }
 }
 
-// W warps per (row, head), each every W-th part, several parts' loads in flight
-template <int HD, int W>
-__global__ void __launch_bounds__(128) prefix_merge_kernel(PrefixParams p, bf16* out, long ldo) {
-  constexpr int E = HD / 32, AT_ONCE = 4;
-  __shared__ float sm[W > 1 ? W : 1][W > 1 ? HD + 1 : 1];
+// four warps per (row, head), a stretch of its parts each
+template <int HD>
+__global__ void __launch_bounds__(NT) prefix_merge_kernel(PrefixParams p, bf16* out, long ldo) {
+  constexpr int E = HD / 32, W = NT / 32;
+  __shared__ float sm[W][HD], sm_l[W];
   grid_dep_launch();
   grid_dep_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w0 = warp % W;
-  const long pair = (long)blockIdx.x * (4 / W) + warp / W;
-  const int t = (int)(pair / p.Hq), h = (int)(pair % p.Hq);
-  if (t >= p.T || p.positions[t] < 0) return;    // (with W = 4 a whole CTA)
-  const PrefixGroup gr = p.naming(t);
-  const PrefixOwn own = p.own(t, gr);
-  const int n = p.sees(gr, t) ? gr.shared : 0, own_n = own.end - own.begin;
-  const int per = p.per_split(n, max(1, p.prefix_splits)), own_per = p.per_split(own_n, p.own_splits);
-  const int ns = n > 0 ? (n + per - 1) / per * p.streams : 0, no = own_n > 0 ? (own_n + own_per - 1) / own_per : 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   const long base = p.part_of(t, h, 0);
-  auto slot_of = [&](int i) { return base + (i < ns ? i : p.streams * p.prefix_splits + i - ns); };
-  float M = -INFINITY;
-  for (int i = lane; i < ns + no; i += 32) M = fmaxf(M, p.sums[slot_of(i)].x);
-  M = warp_max(M);
-  float v[E] = {}, L = 0.f;
-  for (int i0 = w0; i0 < ns + no; i0 += AT_ONCE * W) {
-    float2 ml[AT_ONCE], a[AT_ONCE][E / 2];
+  const int n = p.streams * p.prefix_splits + p.own_splits, each = (n + W - 1) / W;
+  const float M[1] = {largest(p, base, n, lane)};
+  if (p.positions[t] < 0) return;
+  float part[1][E] = {}, sum[1] = {0.f};
+  add_parts<E, 1, 8>(p, base, 0, 1, min(n, warp * each), min(n, (warp + 1) * each), M, sum, part, lane);
+  float L = sum[0];
+  float(&v)[E] = part[0];
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const int i = i0 + k * W;
-      ml[k] = make_float2(-INFINITY, 0.f);
-      if (i >= ns + no) continue;
-      const long s = slot_of(i);
-      ml[k] = p.sums[s];
+  for (int e = 0; e < E; ++e) sm[warp][lane * E + e] = v[e];
+  if (lane == 0) sm_l[warp] = L;
+  __syncthreads();
+  if (warp) return;
 #pragma unroll
-      for (int e = 0; e < E / 2; ++e) a[k][e] = *reinterpret_cast<const float2*>(p.parts + s * HD + lane * E + 2 * e);
-    }
+  for (int k = 1; k < W; ++k) {
+    L += sm_l[k];
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const float w = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - M);
-      if (w == 0.f) continue;                    // nothing, or an infinite value that weighs nothing
-      L += w * ml[k].y;
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        v[2 * e] += w * a[k][e].x;
-        v[2 * e + 1] += w * a[k][e].y;
-      }
-    }
+    for (int e = 0; e < E; ++e) v[e] += sm[k][lane * E + e];
   }
-  if constexpr (W > 1) {
+  store_result<E>(out + (long)t * ldo + (long)h * HD, L, v, lane);
+}
+
+// W warps per (row, kv head): the row's own keys, what the prefix's kernel left, the result
+template <int HD, int W>
+__global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p, bf16* out, long ldo) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int E = HD / 32, UNITS = NT / 32 / W, P = W == 1 ? 4 : 1, S = W == 1 ? 2 : 8;
+  grid_dep_launch();
+  grid_dep_wait();
+  const int lane = threadIdx.x & 31, unit = threadIdx.x / (32 * W);
+  const long item = (long)blockIdx.x * UNITS + unit;
+  const int kvh = (int)(item % p.Hkv);
+  const long t0 = item / p.Hkv;
+  if (t0 >= p.T || p.positions[t0] < 0) return;
+  const PrefixGroup gr = p.naming((int)t0);
+  const PrefixOwn own = p.own((int)t0, gr);
+  const int per = p.per_split(gr.shared, max(1, p.prefix_splits)), parts = p.sees(gr, (int)t0) ? (gr.shared + per - 1) / per * p.streams : 0;
+  auto& u = reinterpret_cast<Unit<HD, W, 16, OWN_STAGES>*>(smem)[unit];
+  attend<HD, W, 1, OWN_STAGES, P>(
+      p, u, own.begin, own.end, own.slot, kvh, 0,
+      [&](int i, int* t, int* h) {
+        *t = (int)t0;
+        *h = kvh * p.G + i;
+        return i < p.G;
+      },
+      [&](int i, const float (&M)[P], const float (&L)[P], const float (&mine)[P][E]) {
+        const int h = kvh * p.G + i, pairs = min(P, p.G - i);
+        const long base = p.part_of((int)t0, h, 0), apart = p.part_of(0, 1, 0);
+        float top[P], sum[P], v[P][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) sm[w0][lane * E + e] = v[e];
-    if (lane == 0) sm[w0][HD] = L;
-    __syncthreads();
-    if (w0) return;
+        for (int n = 0; n < P; ++n) top[n] = n < pairs ? fmaxf(M[n], largest(p, base + n * apart, parts, lane)) : 0.f;
 #pragma unroll
-    for (int k = 1; k < W; ++k) {
-      L += sm[k][HD];
+        for (int n = 0; n < P; ++n) {
+          const float w = M[n] == -INFINITY ? 0.f : exp2f(M[n] - top[n]);
+          sum[n] = w != 0.f ? w * L[n] : 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] += sm[k][lane * E + e];
-    }
-  }
-  const float inv = L != 0.f ? 1.f / L : 0.f;      // (a NaN among the scores stays one)
-  bf16* dst = out + (long)t * ldo + (long)h * HD + lane * E;
+          for (int e = 0; e < E; ++e) v[n][e] = w != 0.f ? w * mine[n][e] : 0.f;
+        }
+        add_parts<E, P, S>(p, base, apart, pairs, 0, parts, top, sum, v, lane);
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(v[e] * inv, v[e + 1] * inv);
+        for (int n = 0; n < P; ++n)
+          if (n < pairs) store_result<E>(out + t0 * ldo + (long)(h + n) * HD, sum[n], v[n], lane);
+      });
 }
 
 // how a call is shared out
 struct Plan {
-  int wm, tiles, prefix_splits, own_splits, streams, least;     // wm 0: the prefix on tcgen05
+  int wm, tiles, prefix_splits, own_splits, streams, own_warps;     // wm 0: the prefix on tcgen05; own_warps 0: own parts and a merge, else the own kernel
 };
-Plan plan_of(int T, int Hkv, int G, int groups, bool tiles) {          // tiles: pages that tcgen05's form takes
+Plan plan_of(int T, int Hkv, int G, int groups, bool tcgen05) {
   Plan a{};
-  auto splits = [](long items, long ctas, int most) { return (int)std::max(1l, std::min((long)most, (ctas + items - 1) / std::max(1l, items))); };
+  auto splits = [](long items, long ctas, int most) { return (int)std::max(1l, std::min((long)most, ctas / std::max(1l, items))); };
   const int rows = groups ? (T + groups - 1) / groups * G : 1;
-  a.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : tiles ? 0 : 4;
+  const long items = (long)T * Hkv;
+  a.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : tcgen05 ? 0 : 4;
   a.streams = a.wm ? 1 : 2;
   const int tile = a.wm ? 16 * a.wm : 256;
   a.tiles = groups ? (int)std::max((long)groups, ((long)T * G - groups) / tile + groups) : 0;        // at most, however the rows are shared out
-  a.prefix_splits = groups ? a.wm ? splits((long)a.tiles * Hkv, 296, 64) : std::max(1, std::min(148, (int)(148 / std::max(1l, (long)a.tiles * Hkv)))) : 0;
-  a.own_splits = splits((long)T * Hkv, 296, 16);
-  a.least = 128;
+  // One wave: 148 CTAs of either kind side by side, two an SM; tcgen05's have an SM each
+  a.prefix_splits = groups ? splits((long)a.tiles * Hkv, 148, 148) : 0;
+  a.own_splits = splits(items, 148, 16);
+  a.own_warps = a.wm || items < 148 ? 0 : items < 1184 ? 4 : 1;
   return a;
 }
 
 template <int HD, int WM>
 int launch_parts(const PrefixParams& p, long prefix_items, cudaStream_t s) {
   auto k = prefix_parts_kernel<HD, WM>;
-  if (int rc = opt_in_smem(k, Ring<HD>::SMEM)) return rc;
+  constexpr int smem = std::max(sizeof(Unit<HD, 4, 16 * WM, 3>), sizeof(Unit<HD, 4, 16, 3>));
+  if (int rc = opt_in_smem_once<prefix_parts_kernel<HD, WM>>(smem)) return rc;
   const long items = prefix_items + (long)p.T * p.Hkv * p.own_splits;
   if (items > 0x7fffffff) return -1;
-  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)Ring<HD>::SMEM, s, p, (int)prefix_items);
+  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)smem, s, p, (int)prefix_items);
+}
+template <int HD, int W>
+int launch_own(const PrefixParams& p, bf16* out, long ldo, cudaStream_t s) {
+  auto k = prefix_own_kernel<HD, W>;
+  constexpr int units = NT / 32 / W, smem = units * sizeof(Unit<HD, W, 16, OWN_STAGES>);
+  if (int rc = opt_in_smem_once<prefix_own_kernel<HD, W>>(smem)) return rc;
+  return launch_chain(k, dim3((unsigned)(((long)p.T * p.Hkv + units - 1) / units)), dim3(NT), (size_t)smem, s, p, out, ldo);
 }
 template <int HD>
 int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream_t s) {
   const long items = (long)a.tiles * p.Hkv * a.prefix_splits;
-  if (items > 0x7fffffff) return -1;
+  if (items > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
   if (!a.wm)
     if (int rc = launch_prefix_tiles(p, HD, items, s)) return rc;
+  if (a.own_warps) return a.own_warps == 4 ? launch_own<HD, 4>(p, out, ldo, s) : launch_own<HD, 1>(p, out, ldo, s);
   if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, items, s) : a.wm == 2 ? launch_parts<HD, 2>(p, items, s) : launch_parts<HD, 1>(p, a.wm ? items : 0, s)) return rc;
-  const long pairs = (long)p.T * p.Hq;
-  if (a.streams * a.prefix_splits + a.own_splits > 4 && pairs <= 0x7fffffff) return launch_chain(prefix_merge_kernel<HD, 4>, dim3((unsigned)pairs), dim3(128), 0, s, p, out, ldo);
-  return launch_chain(prefix_merge_kernel<HD, 1>, dim3((unsigned)((pairs + 3) / 4)), dim3(128), 0, s, p, out, ldo);
+  return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)((long)p.T * p.Hq)), dim3(NT), 0, s, p, out, ldo);
 }
 
 }  // namespace
@@ -386,8 +493,9 @@ extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_
 extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
                                             int num_slots, int max_pages, int page_tokens, int num_pages, const int32_t* groups, int num_groups, float scale, int T, int Hq, int Hkv,
                                             int head_dim, void* scratch, uint64_t scratch_bytes, void* out, long ldo, uint32_t* status, void* stream) {
+  if (!(scale > 0.f) || scale > 3.4e38f) return -1;
   if (T < 1 || T > 1 << 20 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || (head_dim != 64 && head_dim != 128) || num_groups < 0 || num_groups > 64 || (num_groups && !groups)) return -1;
-  if (num_slots < 1 || max_pages < 1 || page_tokens < 1 || num_pages < 1 || (long)num_pages * page_tokens > 0x7fffffff || (long)max_pages * page_tokens > 0x7fffffff - 2 * KEYS) return -1;
+  if (num_slots < 1 || max_pages < 1 || page_tokens < 1 || num_pages < 1 || (long)num_pages * page_tokens > 0x7fffffff || (long)max_pages * page_tokens > 0x7fffffff - 256) return -1;
   if (ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)scratch | (uintptr_t)groups) % 16) return -1;
   const Plan a = plan_of(T, Hkv, Hq / Hkv, num_groups, page_tokens % 8 == 0);
   if (ifab_shared_prefix_scratch(T, Hq, Hkv, head_dim, num_groups) > scratch_bytes) return -5;
@@ -397,7 +505,7 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   p.num_slots = num_slots; p.max_pages = max_pages; p.page_tokens = page_tokens; p.num_pages = num_pages; p.groups = num_groups;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
-  p.prefix_splits = a.prefix_splits; p.own_splits = a.own_splits; p.streams = a.streams; p.least = a.least;
+  p.prefix_splits = a.prefix_splits; p.own_splits = a.own_splits; p.streams = a.streams;
   p.parts = (float*)scratch;
   p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.streams * a.prefix_splits + a.own_splits) * head_dim);
   p.status = status;

@@ -23,7 +23,7 @@ struct PrefixParams {
   float scale_log2;                              // of a score in powers of two
   int T, Hq, Hkv, G;
   int prefix_splits, own_splits;                 // stretches that a group's prefix, a row's own positions are shared out to at most
-  int streams, least;                            // parts of a stretch of the prefix; fewest keys of one
+  int streams;                                   // parts of a stretch of the prefix
   float* parts;                                  // [T, Hq, streams prefix_splits + own_splits, head_dim]: sums of values
   float2* sums;                                  // [T, Hq, streams prefix_splits + own_splits]: maximum (in powers of two), sum of weights
   uint32_t* status;
@@ -64,7 +64,7 @@ struct PrefixParams {
     return end >= g.shared ? PrefixOwn{g.shared, end, slots[t]} : PrefixOwn{0, end, g.slot};       // a position within the prefix
   }
   // keys of a stretch: whole tiles of the kernels'
-  __device__ __forceinline__ int per_split(int n, int splits) const { return max(least, ((n + splits - 1) / splits + 127) / 128 * 128); }
+  __device__ __forceinline__ int per_split(int n, int splits) const { return max(128, ((n + splits - 1) / splits + 127) / 128 * 128); }
   __device__ __forceinline__ long part_of(int t, int h, int i) const { return ((long)t * Hq + h) * (streams * prefix_splits + own_splits) + i; }
 };
 

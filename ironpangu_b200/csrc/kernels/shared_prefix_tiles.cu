@@ -152,9 +152,15 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     const int tiles = (gr.rows * p.G + 2 * TILE - 1) / (2 * TILE);
     if (tile < tiles) break;
     tile -= tiles;
-    gr.shared = 0;
+    gr = PrefixGroup{0, 0, 0, 0};
   }
   const int per = p.per_split(gr.shared, p.prefix_splits), begin = split * per, end = min(begin + per, gr.shared);
+  // parts of rows that do not see the prefix, or that the stretches leave over, are nothing: the merge kernel goes by their sums alone
+  for (int x = tile * 2 * TILE + tid; x < min((tile + 1) * 2 * TILE, gr.rows * p.G); x += NT) {
+    const int t = gr.first + x / p.G;
+    const long at = p.part_of(t, kvh * p.G + x % p.G, 2 * split);
+    if (begin >= end || !p.sees(gr, t)) p.sums[at] = p.sums[at + 1] = make_float2(-INFINITY, 0.f);
+  }
   if (begin >= end) {
     if (warp == 8) tmem_dealloc(tmem, 512);
     return;
@@ -181,7 +187,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
   };
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int X = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16, s_addr = tmem + lane_addr + X * 128, o_addr = tmem + lane_addr + 256 + X * 128;
     const int steps = two ? nt : (nt - X + 1) / 2;
@@ -298,7 +304,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
       if (two) p.sums[at + 1] = make_float2(-INFINITY, 0.f);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 8) {
       constexpr uint32_t idesc_s = umma_idesc_bf16(TILE, TILE), idesc_o = umma_idesc_bf16(TILE, HD) | 1u << 16;      // V's columns run along the rows
       const auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
@@ -399,7 +405,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
 template <int HD>
 int launch(const PrefixParams& p, long items, cudaStream_t s) {
   auto k = prefix_tiles_kernel<HD>;
-  if (int rc = opt_in_smem(k, Layout<HD>::SMEM)) return rc;
+  if (int rc = opt_in_smem_once<prefix_tiles_kernel<HD>>(Layout<HD>::SMEM)) return rc;
   int box = TILE;                                // rows of a box: they never pass a page's end
   while (p.page_tokens % box) box /= 2;
   const uint64_t rows = (uint64_t)p.num_pages * p.page_tokens, cols = (uint64_t)p.Hkv * HD;

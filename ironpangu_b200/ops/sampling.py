@@ -20,14 +20,6 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(f"sampling: {what}")
 
 
-def _row(t: Optional[torch.Tensor], dtype: torch.dtype, T: int, dev: int, what: str) -> Optional[int]:
-    if t is None:
-        return None
-    if not (t.dtype is dtype and t.shape == (T,) and t.get_device() == dev and (T < 2 or t.stride(0) == 1)):
-        _need(False, f"{what} must be contiguous {str(dtype)[6:]} [{T}] beside the logits")
-    return t.data_ptr()
-
-
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, inv_temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
            top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None, probs: bool = False, out_ids: Optional[torch.Tensor] = None,
            out_probs: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
@@ -41,27 +33,57 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, inv_temperature: Opt
     Per-row values, contiguous ``[T]``, none: no such cut. ``uniforms`` f32 within [0, 1); from 1 on the last kept token is drawn, below 0 the first. ``inv_temperature`` f32: 0 and less, infinity and NaN take the first token
     (probability 1). ``top_k`` int32: below 1, or V and more, keeps all. ``top_p`` f32: 1 and more, or NaN, keeps all. ``min_p`` f32: 0 and less, or NaN, keeps all. Logits of -inf and NaN are never drawn;
     a row of nothing else gets id -1 and probability 0. Beside a logit of +inf only such logits are drawn."""
-    shape, dev = logits.shape, logits.get_device()
-    f32 = logits.dtype is F32
-    if not (len(shape) == 2 and (f32 or logits.dtype is BF16) and 1 <= shape[1] <= MAX_VOCAB and shape[0] <= MAX_ROWS and dev >= 0 and (logits.stride(1) == 1 or shape[1] == 1)):
-        _need(len(shape) == 2 and logits.dtype in (F32, BF16) and shape[1] >= 1, "logits must be f32 or bf16 [T, V]")
-        _need(dev >= 0, "the logits are on the host")
-        _need(shape[1] <= MAX_VOCAB and shape[0] <= MAX_ROWS, f"{shape[0]} rows of {shape[1]} logits are not supported")
-        _need(False, "a row's logits must lie one behind the other")
+    # what is wrong with a call is said in _refuse: messages that are made for every call cost as much as its launch
+    shape, dev, dt = logits.shape, logits.get_device(), logits.dtype
+    f32 = dt is F32
+    if not (len(shape) == 2 and (f32 or dt is BF16) and dev >= 0 and (logits.stride(1) == 1 or shape[1] == 1)):
+        _refuse(logits, uniforms, inv_temperature, top_k, top_p, min_p, out_ids, out_probs)
     T, V = shape
-    ld = logits.stride(0) if T > 1 else V
-    _need(ld >= V, "rows of logits must lie apart")
-    up = _row(uniforms, F32, T, dev, "uniforms")
-    _need(up is not None, "uniforms are missing")
-    args = (_row(inv_temperature, F32, T, dev, "inv_temperature"), _row(top_k, I32, T, dev, "top_k"), _row(top_p, F32, T, dev, "top_p"), _row(min_p, F32, T, dev, "min_p"), up)
+    given = [uniforms.data_ptr()] if _is_row(uniforms, F32, T, dev) else _refuse(logits, uniforms, inv_temperature, top_k, top_p, min_p, out_ids, out_probs)
+    for t, want in ((inv_temperature, F32), (top_k, I32), (top_p, F32), (min_p, F32)):
+        if t is None:
+            given.append(None)
+        elif t.dtype is want and t.shape == (T,) and t.get_device() == dev and t.is_contiguous():
+            given.append(t.data_ptr())
+        else:
+            _refuse(logits, uniforms, inv_temperature, top_k, top_p, min_p, out_ids, out_probs)
     if out_ids is None:
         out_ids = torch.empty(T, dtype=I32, device=logits.device)
-    if out_probs is None and probs:
-        out_probs = torch.empty(T, dtype=F32, device=logits.device)
-    outs = _row(out_ids, I32, T, dev, "out_ids"), _row(out_probs, F32, T, dev, "out_probs")
+    elif not _is_row(out_ids, I32, T, dev):
+        _refuse(logits, uniforms, inv_temperature, top_k, top_p, min_p, out_ids, out_probs)
+    if out_probs is None:
+        if probs:
+            out_probs = torch.empty(T, dtype=F32, device=logits.device)
+    elif not _is_row(out_probs, F32, T, dev):
+        _refuse(logits, uniforms, inv_temperature, top_k, top_p, min_p, out_ids, out_probs)
     if T:
+        u, it, k, p, m = given
+        args = (logits.data_ptr(), logits.stride(0) if T > 1 else V, f32, T, V, it, k, p, m, u, out_ids.data_ptr(), None if out_probs is None else out_probs.data_ptr())
         if dev == torch.cuda.current_device():
-            check(_lib.load().ifab_draw(logits.data_ptr(), ld, f32, T, V, *args, *outs, _lib.current_stream(dev)), "sampling.sample")
+            rc = _lib.load().ifab_draw(*args, _lib.current_stream(dev))
         else:
-            _lib.call_on(dev, "ifab_draw", logits.data_ptr(), ld, f32, T, V, *args, *outs)
+            with torch.cuda.device(dev):
+                rc = _lib.load().ifab_draw(*args, _lib.current_stream(dev))
+        if rc == -1:
+            _refuse(logits, uniforms, inv_temperature, top_k, top_p, min_p, out_ids, out_probs)
+        check(rc, "sampling.sample")
     return out_ids if out_probs is None else (out_ids, out_probs)
+
+
+def _is_row(t: Optional[torch.Tensor], dtype: torch.dtype, T: int, dev: int) -> bool:
+    return t is not None and t.dtype is dtype and t.shape == (T,) and t.get_device() == dev and t.is_contiguous()
+
+
+def _refuse(logits, uniforms, inv_temperature, top_k, top_p, min_p, out_ids, out_probs) -> None:
+    shape, dev = logits.shape, logits.get_device()
+    _need(len(shape) == 2 and logits.dtype in (F32, BF16), "logits must be f32 or bf16 [T, V]")
+    _need(dev >= 0, "the logits are on the host")
+    T, V = shape
+    _need(1 <= V <= MAX_VOCAB and T <= MAX_ROWS, f"{T} rows of {V} logits are not supported")
+    _need(logits.stride(1) == 1 or V == 1, "a row's logits must lie one behind the other")
+    _need(T < 2 or logits.stride(0) >= V, "rows of logits must lie apart")
+    _need(uniforms is not None, "uniforms are missing")
+    for t, dtype, what in ((uniforms, F32, "uniforms"), (inv_temperature, F32, "inv_temperature"), (top_k, I32, "top_k"), (top_p, F32, "top_p"), (min_p, F32, "min_p"), (out_ids, I32, "out_ids"),
+                           (out_probs, F32, "out_probs")):
+        _need(t is None or _is_row(t, dtype, T, dev), f"{what} must be contiguous {str(dtype)[6:]} [{T}] beside the logits")
+    raise AssertionError("sampling.sample: a call was refused without a reason")

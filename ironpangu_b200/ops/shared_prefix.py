@@ -2,6 +2,7 @@
 one prompt, or questions behind one document. ``ops.decode.gqa_decode_attention`` reads them once for every row."""
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -21,7 +22,7 @@ def _need(ok: bool, what: str) -> None:
 def scratch_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, groups: int = 1) -> int:
     """Bytes that :func:`attention` takes as ``scratch`` for a call of so many rows (and for any of fewer in as many groups, the most of all of them)."""
     _need(rows >= 0 and groups >= 0 and kv_heads >= 1 and heads % kv_heads == 0, f"{rows} rows of {heads} heads over {kv_heads} in {groups} groups")
-    return max((_lib.load().ifab_shared_prefix_scratch(t, heads, kv_heads, head_dim, groups) for t in range(1, rows + 1)), default=0)
+    return max((_scratch.__wrapped__(t, heads, kv_heads, head_dim, groups) for t in range(1, rows + 1)), default=0)
 
 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor, groups: torch.Tensor, *, heads: int,
@@ -36,50 +37,71 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos
     Heads of 64 or 128 columns, up to 16 of them over a key head. Scores, maxima, sums and sums of values are f32, weights enter their products with 15 bits, the result is rounded once. Pages that
     are not there, slots, positions and groups out of range are skipped and set ``IFAB_STATUS_BAD_INDEX`` in the status word; a row that sees nothing gets zeros. ``scratch``: uint8 on 16 bytes,
     :func:`scratch_bytes`; calls that may run at the same time need one each."""
-    dev, T = q.get_device(), q.shape[0]
-    if not (q.dim() == 2 and q.dtype is BF16 and dev >= 0 and q.stride(1) == 1 and kv_heads >= 1 and heads % kv_heads == 0 and heads // kv_heads <= 16 and head_dim in (64, 128)
-            and q.shape[1] >= heads * head_dim and T <= MAX_ROWS):
-        _need(q.dim() == 2 and q.dtype == BF16 and (q.stride(1) == 1), "queries must be bf16 [T, heads * head_dim], columns contiguous")
-        _need(dev >= 0, "the queries are on the host")
-        _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0 and heads // kv_heads <= 16 and head_dim in (64, 128), f"{heads} heads over {kv_heads} of {head_dim} columns are not supported")
-        _need(T <= MAX_ROWS, f"{T} rows are not supported")
-        _need(False, f"queries of {q.shape[1]} columns for {heads} heads of {head_dim}")
-    pages, pt = k_cache.shape[:2] if k_cache.dim() == 4 else (0, 0)
-    for t, what in ((k_cache, "keys"), (v_cache, "values")):
-        if not (t.dtype is BF16 and t.get_device() == dev and t.shape == (pages, pt, kv_heads, head_dim) and t.is_contiguous() and pages > 0 and pt > 0):
-            _need(False, f"{what} must be contiguous bf16 [pages, page_tokens, {kv_heads}, {head_dim}] beside the queries")
-    for t, what in ((positions, "positions"), (slots, "slots")):
-        if not (t.dtype is I32 and t.shape == (T,) and t.get_device() == dev and (T < 2 or t.stride(0) == 1)):
-            _need(False, f"{what} must be contiguous int32 [{T}] beside the queries")
-    for t, what in ((page_table, "page_table"), (groups, "groups")):
-        if not (t.dim() == 2 and t.dtype is I32 and t.get_device() == dev and t.is_contiguous()):
-            _need(False, f"{what} must be contiguous int32 beside the queries")
-    n = groups.shape[0]
-    if not (n <= MAX_GROUPS and groups.shape[1] == 4):
-        _need(False, f"groups must be [up to {MAX_GROUPS}, 4]")
-    num_slots, max_pages = page_table.shape
-    if not (num_slots >= 1 and max_pages >= 1 and pages * pt < 1 << 31 and max_pages * pt < (1 << 31) - 128):
-        _need(False, f"{pages} pages of {pt} positions, {max_pages} of {num_slots} slots are not supported")
+    # what is wrong with a call is said in _refuse: messages that are made for every call cost as much as its launches. Numbers are left to the library's own checks
+    qs, ks, ps, gs, dev = q.shape, k_cache.shape, page_table.shape, groups.shape, q.get_device()
+    if not (len(qs) == 2 and len(ks) == 4 and len(ps) == 2 and len(gs) == 2 and dev >= 0 and q.dtype is BF16 and k_cache.dtype is BF16 and v_cache.dtype is BF16 and positions.dtype is I32
+            and slots.dtype is I32 and page_table.dtype is I32 and groups.dtype is I32 and ks[2] == kv_heads and ks[3] == head_dim and v_cache.shape == ks and qs[1] >= heads * head_dim
+            and positions.shape == qs[:1] and slots.shape == qs[:1] and gs[1] == 4 and q.stride(1) == 1 and k_cache.is_contiguous() and v_cache.is_contiguous() and page_table.is_contiguous()
+            and groups.is_contiguous() and positions.is_contiguous() and slots.is_contiguous() and k_cache.get_device() == dev and v_cache.get_device() == dev and positions.get_device() == dev
+            and slots.get_device() == dev and page_table.get_device() == dev and groups.get_device() == dev):
+        _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out)
+    T, n, cols = qs[0], gs[0], heads * head_dim
     if out is None:
-        out = torch.empty(T, heads * head_dim, dtype=BF16, device=q.device)
-    elif not (out.dtype is BF16 and out.shape == (T, heads * head_dim) and out.get_device() == dev and out.stride(1) == 1 and (T < 2 or out.stride(0) >= heads * head_dim)):
-        _need(False, f"the output must be bf16 [{T}, {heads * head_dim}] beside the queries, its rows apart")
+        out = torch.empty((T, cols), dtype=BF16, device=q.device)
+        ldo = cols
+    else:
+        ldo = out.stride(0) if T > 1 else cols
+        if not (out.dtype is BF16 and out.shape == (T, cols) and out.get_device() == dev and out.stride(1) == 1 and ldo >= cols):
+            _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out)
     if T == 0:
         return out
-    lib = _lib.load()
-    need = lib.ifab_shared_prefix_scratch(T, heads, kv_heads, head_dim, n)
+    need = _scratch(T, heads, kv_heads, head_dim, n)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
     elif not (scratch.dtype is torch.uint8 and scratch.get_device() == dev and scratch.is_contiguous() and scratch.numel() >= need):
-        _need(False, f"scratch must be {need} bytes (uint8) beside the queries")
-    ldq, ldo = (q.stride(0), out.stride(0)) if T > 1 else (heads * head_dim, heads * head_dim)
-    qp, kp, vp, op, sp, gp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), scratch.data_ptr(), groups.data_ptr()
-    if (qp | kp | vp | op | sp | gp) % 16 or ldq % 8 or ldo % 8:
-        _need(False, "rows, caches, groups and scratch must lie on 16 bytes")
-    args = (qp, ldq, kp, vp, positions.data_ptr(), slots.data_ptr(), page_table.data_ptr(), num_slots, max_pages, pt, pages, gp, n, scale, T, heads, kv_heads, head_dim, sp, scratch.numel(), op, ldo,
-            status_ptr)
+        _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out)
+    args = (q.data_ptr(), q.stride(0) if T > 1 else cols, k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), page_table.data_ptr(), ps[0], ps[1], ks[1], ks[0],
+            groups.data_ptr(), n, scale, T, heads, kv_heads, head_dim, scratch.data_ptr(), need, out.data_ptr(), ldo, status_ptr)
     if dev == torch.cuda.current_device():
-        _lib.check(lib.ifab_shared_prefix_attention(*args, _lib.current_stream(dev)), "shared_prefix.attention")
+        rc = _lib.load().ifab_shared_prefix_attention(*args, _lib.current_stream(dev))
     else:
-        _lib.call_on(dev, "ifab_shared_prefix_attention", *args)
+        with torch.cuda.device(dev):
+            rc = _lib.load().ifab_shared_prefix_attention(*args, _lib.current_stream(dev))
+    if rc == -1:
+        _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out)
+    _lib.check(rc, "shared_prefix.attention")
     return out
+
+
+@lru_cache(maxsize=256)
+def _scratch(rows: int, heads: int, kv_heads: int, head_dim: int, groups: int) -> int:
+    return _lib.load().ifab_shared_prefix_scratch(rows, heads, kv_heads, head_dim, groups) if rows >= 1 and kv_heads >= 1 and heads >= 1 and groups >= 0 else 0
+
+
+def _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out) -> None:
+    dev, T = q.get_device(), q.shape[0] if q.dim() else 0
+    _need(q.dim() == 2 and q.dtype == BF16 and q.stride(1) == 1, "queries must be bf16 [T, heads * head_dim], columns contiguous")
+    _need(dev >= 0, "the queries are on the host")
+    _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0 and heads // kv_heads <= 16 and head_dim in (64, 128), f"{heads} heads over {kv_heads} of {head_dim} columns are not supported")
+    _need(T <= MAX_ROWS, f"{T} rows are not supported")
+    _need(q.shape[1] >= heads * head_dim, f"queries of {q.shape[1]} columns for {heads} heads of {head_dim}")
+    pages, pt = k_cache.shape[:2] if k_cache.dim() == 4 else (0, 0)
+    for t, what in ((k_cache, "keys"), (v_cache, "values")):
+        _need(t.dtype == BF16 and t.get_device() == dev and t.shape == (pages, pt, kv_heads, head_dim) and t.is_contiguous() and pages > 0 and pt > 0,
+              f"{what} must be contiguous bf16 [pages, page_tokens, {kv_heads}, {head_dim}] beside the queries")
+    for t, what in ((positions, "positions"), (slots, "slots")):
+        _need(t.dtype == I32 and t.shape == (T,) and t.get_device() == dev and t.is_contiguous(), f"{what} must be contiguous int32 [{T}] beside the queries")
+    for t, what in ((page_table, "page_table"), (groups, "groups")):
+        _need(t.dim() == 2 and t.dtype == I32 and t.get_device() == dev and t.is_contiguous(), f"{what} must be contiguous int32 beside the queries")
+    _need(groups.shape[0] <= MAX_GROUPS and groups.shape[1] == 4, f"groups must be [up to {MAX_GROUPS}, 4]")
+    num_slots, max_pages = page_table.shape
+    _need(num_slots >= 1 and max_pages >= 1 and pages * pt < 1 << 31 and max_pages * pt < (1 << 31) - 256, f"{pages} pages of {pt} positions, {max_pages} of {num_slots} slots are not supported")
+    _need(0 < scale < float("inf"), f"a scale of {scale}")
+    _need(out is None or (out.dtype == BF16 and out.shape == (T, heads * head_dim) and out.get_device() == dev and out.stride(1) == 1 and (T < 2 or out.stride(0) >= heads * head_dim)),
+          f"the output must be bf16 [{T}, {heads * head_dim}] beside the queries, its rows apart")
+    need = _scratch(T, heads, kv_heads, head_dim, groups.shape[0])
+    _need(scratch is None or (scratch.dtype == torch.uint8 and scratch.get_device() == dev and scratch.is_contiguous() and scratch.numel() >= need),
+          f"scratch must be {need} bytes (uint8) beside the queries")
+    near = all(t is None or t.data_ptr() % 16 == 0 for t in (q, k_cache, v_cache, groups, scratch, out)) and all(t is None or T < 2 or t.stride(0) % 8 == 0 for t in (q, out))
+    _need(near, "rows, caches, groups and scratch must lie on 16 bytes")
+    raise RuntimeError(f"shared_prefix.attention: {T} rows of {heads} heads are too many for one call")
