@@ -7,7 +7,7 @@ down GEMV fused with all-reduce + residual. 6 launches per layer, no stand-alone
 rank 5, as the qkv launch rotates and appends, and the linears are streams through rings in shared memory.
 Query rows of different sequences (continuous batching) share every launch: each row carries its
 own position and sequence slot. Sampling is greedy (fused with the lm_head) or top-k / top-p on the
-device. :func:`quantise_weights` puts the linears' weights into 4 bits (one rank). With ``page_pool`` the pages come from a pool on the device
+device. :meth:`DenseDecoder.share_prefix` has rows whose sequences share a prompt read its keys and values once for all of them. :func:`quantise_weights` puts the linears' weights into 4 bits (one rank). With ``page_pool`` the pages come from a pool on the device
 (``ops/pages.py``), so that sequences can be forked inside a step. The reference's dense family runs per-layer composites of vendor ops with an all-gather
 after every sharded projection (native/src/inferfabric_acl.cpp:688-755, 1236-1433).
 """
@@ -20,7 +20,7 @@ from typing import Dict, Optional
 import torch
 
 from ..ops import decode as K
-from ..ops import int4
+from ..ops import int4, shared_prefix
 from ..ops.pages import PagePool
 from ..parallel.fabric import Fabric
 
@@ -198,6 +198,18 @@ class DenseDecoder:
         self.logits = e(T, self.vl, dt=torch.float32) if keep_logits else None
         self.launches_per_forward = 1 + (T + 7) // 8 + ((6 if T <= 8 else 8 if T <= int4.STREAM_ROWS else 12) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
         self._graph = None
+        self.prefix_groups, self._prefix_scratch = None, []
+
+    def share_prefix(self, groups: Optional[torch.Tensor]) -> None:
+        """From the next :meth:`forward` on - captured ones keep what they were captured with - the rows' attention goes by ``groups`` (``ops.shared_prefix.attention``: int32 ``[n, 4]`` on the device,
+        read at every step; heads of 64 or 128 columns). None: every row reads all of its own sequence again."""
+        if groups is not None:
+            if self.cfg.head_dim not in (64, 128) or self.hq > 16 * self.hk:
+                raise ValueError(f"rows of {self.hq} heads over {self.hk} of {self.cfg.head_dim} columns share no prefix")
+            need = shared_prefix.scratch_bytes(self.T, self.hq, self.hk, self.cfg.head_dim, groups.shape[0])
+            if not self._prefix_scratch or self._prefix_scratch[-1].numel() < need:
+                self._prefix_scratch.append(torch.empty(need, dtype=torch.uint8, device=groups.device))      # (captured steps go on using the one before)
+        self.prefix_groups = groups
 
     def _row_parallel(self, a: torch.Tensor, w: torch.Tensor, x: torch.Tensor) -> None:
         """``x += a @ w.T`` summed over the ranks (one rank: the same bits without the call counter)."""
@@ -236,10 +248,14 @@ class DenseDecoder:
                 K.gemv(x, w[p + "qkv"], norm_w=w[p + "attn_norm"], eps=c.eps, out=qkv, rings=fab.world == 1)
                 K.gqa_rope_kv_write(qkv, pos, slot, self.page_table, self.k_cache[l], self.v_cache[l], heads=self.hq,
                                     kv_heads=self.hk, head_dim=c.head_dim, theta=c.theta, status_ptr=st)
-            K.gqa_decode_attention(qkv, self.k_cache[l], self.v_cache[l], pos, slot, self.page_table, heads=self.hq,
-                                   kv_heads=self.hk, head_dim=c.head_dim, scale=1.0 / math.sqrt(c.head_dim),
-                                   keys_per_split=self.kps, max_splits=self.max_splits, scratch=self.scratch,
-                                   out=self.attn[:T], status_ptr=st)
+            if self.prefix_groups is not None:
+                shared_prefix.attention(qkv, self.k_cache[l], self.v_cache[l], pos, slot, self.page_table, self.prefix_groups, heads=self.hq, kv_heads=self.hk, head_dim=c.head_dim,
+                                        scale=1.0 / math.sqrt(c.head_dim), scratch=self._prefix_scratch[-1], out=self.attn[:T], status_ptr=st)
+            else:
+                K.gqa_decode_attention(qkv, self.k_cache[l], self.v_cache[l], pos, slot, self.page_table, heads=self.hq,
+                                       kv_heads=self.hk, head_dim=c.head_dim, scale=1.0 / math.sqrt(c.head_dim),
+                                       keys_per_split=self.kps, max_splits=self.max_splits, scratch=self.scratch,
+                                       out=self.attn[:T], status_ptr=st)
             self._row_parallel(self.attn[:T], w[p + "o_proj"], x)
             if self.int4:
                 self.normed_linear(x, w[p + "gate_up"], w[p + "ffn_norm"], self.act[:T])

@@ -2,6 +2,9 @@
 of all of them - pages taken, layers, sampling, the sampled tokens fed back - is one CUDA graph without the host. Continuations can be drawn again with repeats
 (:meth:`Continuations.resample`: those that were not drawn end, those drawn twice go on separately, as particles and beams do), set aside in a second pool and packed.
 
+With ``shared_prefix`` a step's attention reads the prompt's keys and values once for all continuations (``ops/shared_prefix.py``). Tokens are drawn among the best 64 at most
+(``ops.decode.sample_topk``), or from the whole vocabulary (``ops/sampling.py``) with random numbers of a table that a start fills.
+
 The decoder is a ``models.dense_gqa.DenseDecoder`` with ``page_pool`` and ``keep_logits``, bf16 or 4-bit weights; slot 0 holds the prompt and slot 1 + i continuation i."""
 from __future__ import annotations
 
@@ -11,13 +14,14 @@ import torch
 
 from ..ops import decode as K
 from ..ops import pages as P
+from ..ops import sampling
 
 I32 = torch.int32
 
 
 class Continuations:
-    def __init__(self, decoder, *, prefill=None, store_pages: int = 0):
-        """``prefill``: a ``models.dense_prefill.DensePrefill`` of the decoder; without one the prompt goes through the decode kernels. ``store_pages``: pages of the second
+    def __init__(self, decoder, *, prefill=None, store_pages: int = 0, shared_prefix: bool = False):
+        """``shared_prefix``: heads of 64 or 128 columns; the results differ in their rounding from those without. ``prefill``: a ``models.dense_prefill.DensePrefill`` of the decoder; without one the prompt goes through the decode kernels. ``store_pages``: pages of the second
         pool that :meth:`set_aside` copies to."""
         if decoder.pool is None or decoder.logits is None:
             raise ValueError("continuations need a decoder with page_pool and keep_logits")
@@ -31,6 +35,12 @@ class Continuations:
         self.inv_temp, self.top_p = torch.ones(self.width, device=dev), torch.ones(self.width, device=dev)
         self.ids = torch.zeros(self.width, dtype=I32, device=dev)
         self._scratch = torch.empty(self.width * ((decoder.logits.shape[1] + 4095) // 4096) * 128, dtype=torch.float32, device=dev)
+        self._group = torch.zeros(1, 4, dtype=I32, device=dev) if shared_prefix else None          # rows, prompt's positions and slot
+        if shared_prefix:
+            decoder.share_prefix(self._group)     # (raises where the decoder's heads cannot)
+            decoder.share_prefix(None)
+        self.whole = False                    # drawn from the whole vocabulary
+        self._table = None                    # random numbers, a row a step
         self._graphs = {}
         self.n = self.length = 0              # continuations, positions of each
         self.store = [torch.empty(store_pages, *c.shape[1:], dtype=c.dtype, device=dev) for c in decoder.k_cache + decoder.v_cache] if store_pages else []
@@ -40,16 +50,22 @@ class Continuations:
         self._ran = self._broken = False      # there was a run, whose reports may still lie in the status words; the continuations are not what their tokens say
 
     # -- prompt --------------------------------------------------------------------------------------------------------------
-    def start(self, prompt: Sequence[int], n: int, *, temperature: float = 1.0, top_k: int = 50, top_p: float = 1.0, seed: int = 0) -> torch.Tensor:
-        """Runs the prompt, forks it ``n`` times and samples the first token of each continuation (device tensor ``[n]``). ``temperature`` 0: greedy. Continuations that were
+    def start(self, prompt: Sequence[int], n: int, *, temperature: float = 1.0, top_k: int = 50, top_p: float = 1.0, min_p: float = 0.0, seed: int = 0) -> torch.Tensor:
+        """Runs the prompt, forks it ``n`` times and samples the first token of each continuation (device tensor ``[n]``). ``temperature`` 0: greedy. ``top_k`` 0 (all tokens) or above 64, or a
+        ``min_p``, draws from the whole vocabulary: one rank, up to 2^18 tokens, other random numbers than those of a ``top_k`` up to 64. Continuations that were
         there are ended first, and nothing that :meth:`check` would have said about them is said any more. Where this raises there are none."""
         d = self.dec
         if not 1 <= n <= self.width:
             raise ValueError(f"{n} continuations: this decoder takes 1 to {self.width}")
         if not 1 <= len(prompt) <= d.max_context:
             raise ValueError(f"a prompt of {len(prompt)} tokens in a context of {d.max_context}")
-        if not 1 <= top_k <= 64:
-            raise ValueError(f"top_k of {top_k}: 1 to 64")
+        if not 0 <= top_k < 1 << 31:
+            raise ValueError(f"top_k of {top_k}: 0 (all) or more")
+        if not 0.0 <= min_p <= 1.0:
+            raise ValueError(f"min_p of {min_p}: 0 to 1")
+        whole = temperature > 0 and (not 1 <= top_k <= 64 or min_p > 0)
+        if whole and (d.fabric.world > 1 or d.logits.shape[1] > sampling.MAX_VOCAB):
+            raise ValueError(f"top_k of {top_k}: 1 to 64, and no min_p, on several ranks and from more than {sampling.MAX_VOCAB} tokens")
         self.end()
         if self._ran:
             self.pool.status.zero_()
@@ -57,6 +73,9 @@ class Continuations:
                 d.fabric.clear_status()
         self._ran = True
         try:
+            self.whole = whole
+            if whole:
+                self._draw_numbers(len(prompt), n, top_k, min_p, seed)
             self._begin(prompt, n, temperature, top_k, top_p, seed)
             self.check()
         except BaseException:
@@ -65,8 +84,22 @@ class Continuations:
         self.n, self.length = n, len(prompt)
         return self.ids[:n]
 
+    def _draw_numbers(self, length: int, n: int, top_k: int, min_p: float, seed: int) -> None:
+        """Random numbers of all steps that the context leaves, for graphs that take a row of them a step."""
+        dev, rows = self._tokens.device, self.dec.max_context - length + 1
+        if self._table is None:
+            self._table = torch.zeros(self.dec.max_context + 1, self.width, device=dev)
+            self._at, self._numbers = torch.zeros(1, dtype=torch.int64, device=dev), torch.zeros(1, self.width, device=dev)
+            self._top_k, self._min_p = torch.zeros(self.width, dtype=I32, device=dev), torch.zeros(self.width, device=dev)
+        self._table[:rows, :n].copy_(torch.rand(rows, n, generator=torch.Generator(device=dev).manual_seed(seed % (1 << 63)), device=dev))
+        self._at.zero_()
+        self._top_k.fill_(top_k)
+        self._min_p.fill_(min_p)
+
     def _begin(self, prompt: Sequence[int], n: int, temperature: float, top_k: int, top_p: float, seed: int) -> None:
         d = self.dec
+        if self._group is not None:
+            d.share_prefix(None)              # the prompt's own rows stand alone
         self.top_k = 1 if temperature <= 0 else top_k
         self.inv_temp[:n].fill_(1e4 if temperature <= 0 else 1.0 / temperature)
         self.top_p[:n].fill_(1.0 if temperature <= 0 else top_p)
@@ -96,11 +129,20 @@ class Continuations:
         if n > 1:
             d.logits[1:n].copy_(d.logits[:1].expand(n - 1, -1))
         self._sample(n)
+        if self._group is not None:
+            self._group.copy_(torch.tensor([[0, n, len(prompt), 0]], dtype=I32))
+            d.share_prefix(self._group)
         d.positions[:n].fill_(len(prompt))
         d.slots[:n].copy_(self._children[:n])
 
     def _sample(self, n: int) -> None:
         d = self.dec
+        if self.whole:
+            torch.index_select(self._table, 0, self._at, out=self._numbers)
+            self._at.add_(1)
+            sampling.sample(d.logits[:n], self._numbers[0, :n], inv_temperature=self.inv_temp[:n], top_k=self._top_k[:n], top_p=self.top_p[:n], min_p=self._min_p[:n], out_ids=self.ids[:n])
+            d.tokens[:n].copy_(self.ids[:n])
+            return
         for t in range(0, n, 64):             # the sampling kernel takes 64 rows
             e = min(n, t + 64)
             K.sample_topk(d.logits[t:e], d.fabric, top_k=self.top_k, inv_temperature=self.inv_temp[t:e], top_p=self.top_p[t:e], seeds=self.seeds[t:e],
@@ -123,7 +165,7 @@ class Continuations:
         if self.length >= self.dec.max_context:
             raise OverflowError("the continuations run past the context")
         self.length += 1
-        key = (self.n, self.top_k)
+        key = (self.n, 0 if self.whole else self.top_k)
         g = self._graphs.get(key)
         if g is not None:
             g.replay()
@@ -178,6 +220,8 @@ class Continuations:
             self._release()
 
     def _release(self) -> None:
+        if self._group is not None:
+            self.dec.share_prefix(None)
         self.pool.free(self._children)
         self.pool.free(self._first)
         for ids in self._aside.values():
