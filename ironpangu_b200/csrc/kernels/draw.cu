@@ -4,11 +4,11 @@
 //   kept: the first top_k; of them those with exp(z_i - z_max) >= min_p; of them the shortest run whose mass reaches top_p of theirs; at least one
 //   drawn: the first kept id, ids rising, at which the sum of exp(z - z_max) exceeds u times that of all kept
 //
-// A row is a cluster of CTAs that keep the row's logits in shared memory: they are read from memory once. What the cuts ask for is a place in the order (the k-th token, the token at
+// A row is a cluster of CTAs that keep the row's logits in shared memory where they fit: they are read from memory once. What the cuts ask for is a place in the order (the k-th token, the token at
 // which the mass passes a share), which is found without a sort: a histogram over the row, equal stretches of the values, says in which of 1024 bins the place lies; the bin's tokens - a
 // few - are gathered and put in order by counting. A bin with more tokens than the list takes (ties, values far apart) is split again by the bits of (value, id), 10 at a time.
 //
-// Weights are e^(z - z_max) in double, summed as integers of 2^-44: the sums decide between tokens, so they must not depend on an order of additions, and a weight below 2^-45 of the
+// Weights are summed as integers of 2^-44: the sums decide between tokens, so they must not depend on an order of additions, and a weight below 2^-45 of the
 // largest is nothing. 2^18 weights of at most 1 stay below 2^62.
 #include <climits>
 #include <utility>
@@ -23,8 +23,8 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int NT = 512, WARPS = NT / 32, BINS = 1024, LIST = 1024, MAX_CLUSTER = 8, ID_BITS = 20, PARTS = 32;
-constexpr int MAX_VOCAB = 1 << 18, MAX_SLICE = MAX_VOCAB / MAX_CLUSTER;
+constexpr int NT = 512, WARPS = NT / 32, BINS = 1024, LIST = 1024, MAX_CLUSTER = 8, ID_BITS = 20, PARTS = 128;
+constexpr int MAX_VOCAB = 1 << 18, PART_EIGHTS = 1 << 12;
 typedef unsigned long long u64;
 
 struct DrawParams {
@@ -49,22 +49,24 @@ struct __align__(16) Entry {
   u64 place, mass;
 };
 struct Shared {
-  uint32_t part[3][BINS];                      // this CTA's tokens by bin: their number, or their mass in three words (which its tokens cannot overflow: 17 bits of each, 2^15 tokens)
-  Entry list[LIST];
-  u64 total[BINS];                             // the row's
-  double parts[PARTS];                         // 2^(i / 32)
+  union {
+    uint32_t part[3][BINS];                    // tokens by bin: their number, or their mass in three words, 17 bits of a token in each, which 2^15 tokens cannot overflow
+    Entry list[LIST];                          // (when the bins have been added up)
+  };
+  u64 mine[BINS], total[BINS];                 // this CTA's, the row's
+  u64 parts[PARTS];                            // 2^(62 - i / 128) + 2^31
   uint32_t listed[2];                          // by turns
   u64 from[MAX_CLUSTER];                       // a value of each CTA
-  float most[MAX_CLUSTER], least[MAX_CLUSTER];
+  float most[MAX_CLUSTER];
   int best[MAX_CLUSTER];
   u64 warp_sum[WARPS];
-  float warp_a[WARPS], warp_b[WARPS];
+  float warp_a[WARPS];
   int warp_i[WARPS];
   int bin;
   u64 above;
   Cut cut;
 };
-static_assert(MAX_SLICE <= 1 << 15, "17 bits of each token's mass in 32");
+static_assert(8 * PART_EIGHTS <= 1 << 15, "17 bits of each token's mass in 32");
 
 // of values that are no NaN: unsigned integers in their order
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -75,27 +77,67 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k
 // (value, id) in the order of the tokens
 __device__ __forceinline__ u64 place_of(float v, int id) { return (u64)key_of(v) << ID_BITS | (u64)((1 << ID_BITS) - 1 - id); }
 
+// Weights e^((v - most) it) in units of 2^-44, rounded. With c = it log2 e as two floats,
+//   v c = n / 128 + r: n / 128 by an addition of 1.5 2^16, whose floats lie 1 / 128 apart, and r (at most 1 / 256) by a product that is rounded only then, so both without loss
+//   weight = 2^-((n_most - n) / 128) (1 + q), q = 2^(r - r_most) - 1 by Taylor's series: of at most 0.0055, it is off by 2^-31 as a float
+// The first factor is a table's (62 bits) and a shift, so weights are off by 2^-31 of themselves, unsystematically, and the largest value's is 1 exactly. What a row costs is instructions, and that is
+// half of them in 64-bit arithmetic. Factors that floats hold badly, and values whose v c the addition does not take, go the 64-bit way.
 struct Weights {
   float most, floor;           // below `floor` a weight is less than 2^-45
   double it, z_most;
-  const double* parts;
-  __device__ __forceinline__ Weights(float most, float it_, const double* parts) : most(most), it((double)it_), z_most((double)most * (double)it_), parts(parts) {
-    const double lowest = (z_most - 32.0) / it;          // e^-32 < 2^-46
+  const u64* parts;            // 2^(62 - i / 128) + 2^31: the upper word is rounded
+  float ch, cl, r_most;
+  int n_most;
+  bool fast;
+  static constexpr float MAGIC = 98304.f, C1 = 0.69314718f * 0x1p38f, C2 = 0.24022651f * 0x1p38f, C3 = 0.055504109f * 0x1p38f;
+  __device__ __forceinline__ Weights(float most, float it_, const u64* parts) : most(most), it((double)it_), z_most((double)most * (double)it_), parts(parts) {
+    const double lowest = (z_most - 32.0) / it, c = it * 1.4426950408889634;          // e^-32 < 2^-46
     floor = most == INFINITY ? INFINITY : lowest > -3.4e38 ? __double2float_rd(lowest) : -3.4028234664e38f;
+    fast = c < 0x1p90 && c > 0x1p-90 && fabs(most * c) < 8192.0;
+    ch = (float)c;
+    cl = (float)(c - (double)ch);
+    const float y = __fmaf_rn(most, ch, MAGIC);
+    n_most = __float_as_int(y);
+    r_most = __fmaf_rn(most, cl, __fmaf_rn(most, ch, MAGIC - y));
   }
   // of `most` itself 1, an infinite one among them; a product of two floats is exact
   __device__ __forceinline__ double real(float v) const { return v == most ? 1.0 : exp((double)v * it - z_most); }
-  // In units of 2^-44, rounded. e^d = 2^(n / 32) e^r, r = d - n ln 2 / 32 of at most 0.011 by Taylor's series up to r^5 / 120 (what it leaves is below 2^-48), without a branch, so that
-  // several tokens' chains run side by side: exp() took 25 cycles a token of each lane with 16 warps.
+  __device__ __forceinline__ u64 slow(float v) const {
+    const u64 m = (u64)__double_as_longlong(real(v) + 256.0) & ((1ull << 52) - 1);       // 256 + w has its last bit at 2^-44
+    return v == most ? 1ull << 44 : v >= floor ? m : 0;
+  }
+  // The weights of v (a NaN's is 0): those up to 2^-15 by `small(i, 32 bits)`, which the others get as 0, the others by `large(i, 64 bits)` beside that
+  template <int N, typename Small, typename Large>
+  __device__ __forceinline__ void of(const float (&v)[N], Small small, Large large) const {
+    if (!fast) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        small(i, 0u);
+        large(i, slow(v[i]));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = __fmaf_rn(v[i], ch, MAGIC), r = __fmaf_rn(v[i], cl, __fmaf_rn(v[i], ch, MAGIC - y)) - r_most;
+      const float q = __fmaf_rn(__fmaf_rn(r, C3, C2), r, C1) * r;
+      const int n = n_most - __float_as_int(y), by = (n >> 7) - 15;              // 0 or more; what the upper word is shifted by before its last bit is rounded away
+      const u64 t = parts[n & 127];
+      u64 part;
+      asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(part) : "r"((int)(t >> 38)), "r"(__float2int_rn(q)), "l"(t));
+      const uint32_t top = (uint32_t)(part >> 32);                               // 30 bits of it
+      uint32_t m;
+      asm("shr.u32 %0, %1, %2;" : "=r"(m) : "r"(top), "r"(by));                  // (32 and more, and less than 0, leave 0)
+      const bool there = v[i] >= floor;                                          // what lies below, or is none, has been anything
+      small(i, there ? (m + 1) >> 1 : 0u);
+      if (there & (by < 0)) large(i, (u64)top << (-1 - by));
+    }
+  }
   __device__ __forceinline__ u64 fixed(float v) const {
-    const double d = (double)fmaxf(v, floor) * it - z_most;
-    const double turn = fma(d, 32 * 1.4426950408889634, 6755399441055744.0);          // 1.5 2^52: the last bits are n
-    const int n = (int)__double_as_longlong(turn);
-    const double r = fma(turn - 6755399441055744.0, -0.6931471805599453 / 32, d);
-    const double e = fma(fma(fma(fma(fma(r, 1.0 / 120, 1.0 / 24), r, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0) * parts[n & (PARTS - 1)];
-    const double scaled = __longlong_as_double(__double_as_longlong(e) + ((u64)(long long)(n >> 5) << 52));
-    const u64 m = (u64)__double_as_longlong(scaled + 256.0) & ((1ull << 52) - 1);       // 256 + w has its last bit at 2^-44
-    return v == most ? 1ull << 44 : v < floor ? 0 : m;
+    const float a[1] = {v};
+    u64 w = 0;
+    of(a, [&](int, uint32_t m) { w = m; }, [&](int, u64 m) { w = m; });
+    return w;
   }
 };
 
@@ -106,60 +148,154 @@ __device__ __forceinline__ u64 warp_total(u64 v) {
   return v;
 }
 
-__device__ __forceinline__ float clean(float v) { return v != v ? -INFINITY : v + 0.f; }      // a NaN is never drawn; -0 is 0
+// The lowest value of those up to `most` for which `enough`, which is so for no value and all above it, holds, by a warp: near `guess`, or 32 places at a time, 32 times finer every round
+template <typename F>
+__device__ float lowest(F enough, float guess, float most, int lane) {
+  const uint32_t end = key_of(most), least = key_of(-INFINITY);
+  const uint32_t near = key_of(guess) > least + 16 ? key_of(guess) - 16 : least;
+  uint32_t vote = __ballot_sync(0xffffffffu, near + lane < end && enough(value_of(near + lane)));
+  if (vote && !(vote & 1) && near + 31 < end) return value_of(near + __ffs(vote) - 1);
+  uint32_t at = least, step = 1u << 27;          // it lies in (at, at + 32 steps], or is `most` itself
+  for (int round = 0; round < 7; ++round) {
+    const u64 mine = (u64)at + (u64)(lane + 1) * step;
+    vote = __ballot_sync(0xffffffffu, mine >= end || enough(value_of((uint32_t)mine)));
+    at += (uint32_t)(vote ? __ffs(vote) - 1 : 32) * step;
+    step = step >= 32 ? step / 32 : 1;
+  }
+  const u64 key = (u64)at + 1;
+  return key >= end ? most : value_of((uint32_t)key);
+}
 
-// The place in the order at which what lies ahead reaches a number of tokens, or a share of their mass
-template <bool MASS>
+__device__ __forceinline__ float clean(float v) { return v + 0.f; }      // -0 is 0; a NaN is above nothing, so it is nowhere
+
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ float load_one(const bf16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float4 load_four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load_four(const bf16* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+}
+
+// A CTA's tokens by eights, in shared memory (HELD) or where they come from; those behind the last one are -inf, with ids that no place reaches
+template <typename In, bool HELD>
+struct Row {
+  float4* own;                 // HELD: the tokens. Otherwise a ring of each thread, through which what it reads comes AHEAD eights ahead of its use (one ahead in registers: 1260 cycles a four)
+  const In* src;
+  int n, full;                 // tokens; eights that can be read as such
+  static constexpr int AHEAD = 4, SLOT = 8 * sizeof(In);
+  __device__ __forceinline__ float at(int i) const { return HELD ? reinterpret_cast<const float*>(own)[i] : load_one(src + i); }
+  __device__ __forceinline__ float4 slow(int i) const { return make_float4(i < n ? at(i) : -INFINITY, i + 1 < n ? at(i + 1) : -INFINITY, i + 2 < n ? at(i + 2) : -INFINITY, i + 3 < n ? at(i + 3) : -INFINITY); }
+  __device__ __forceinline__ static void eight(const In* p, float4& a, float4& b) {
+    a = load_four(p);
+    b = load_four(p + 4);
+  }
+  __device__ __forceinline__ static void request(uint32_t to, const In* from) {
+#pragma unroll
+    for (int i = 0; i < SLOT; i += 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i), "l"((const char*)from + i) : "memory");
+  }
+  // f(first token, four of them) for the eights first, first + step, ... below last
+  template <typename F>
+  __device__ __forceinline__ void each(int first, int last, int step, F f) const {
+    if constexpr (HELD) {
+      for (int o = first; o < last; o += step) {
+        const float4 a = own[2 * o], b = own[2 * o + 1];
+        f(8 * o, a);
+        f(8 * o + 4, b);
+      }
+    } else {
+      const int whole = min(last, full);
+      const In* next = src + 8 * first;
+      const uint32_t ring = (uint32_t)__cvta_generic_to_shared(own) + threadIdx.x * SLOT;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (first + k * step < whole) request(ring + k * NT * SLOT, next);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next += 8 * step;
+      }
+      uint32_t slot = 0;
+      int o = first;
+      for (; o < whole; o += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        float4 a, b;
+        eight(reinterpret_cast<const In*>(reinterpret_cast<const char*>(own) + threadIdx.x * SLOT + slot), a, b);
+        f(8 * o, a);
+        f(8 * o + 4, b);
+        if (o + AHEAD * step < whole) request(ring + slot, next);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next += 8 * step;
+        slot = slot == (AHEAD - 1) * NT * SLOT ? 0 : slot + NT * SLOT;
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      for (; o < last; o += step) {
+        f(8 * o, slow(8 * o));
+        f(8 * o + 4, slow(8 * o + 4));
+      }
+    }
+  }
+};
+
+// The place in the order at which what lies ahead reaches a number of tokens, or a share of their mass. Tokens of -inf and NaN are not among them
+template <bool MASS, typename R>
 struct Search {
   Shared* s;
-  const float4* vals;
-  int quads, base, tid, rank, ranks;           // quads: fours of tokens in this CTA; those behind the last one are -inf, with ids that no place reaches
+  R row;
+  int eights, base, tid, rank, ranks;          // eights: of tokens in this CTA
   uint32_t* turn;
   Cut cut;
   Weights w;
-  float top, scale;            // bins of equal stretches below `top`
-  float first_bin;
-  u64 lo, hi;                  // places within first_bin, once it is split
+  float top, scale;            // bins of equal stretches below `top`; scale 0: one for all
+  float from, below;           // values of the bin that was found: from <= v, not below <= v
+  u64 lo, hi;                  // places within it, once it is split
   bool split;
+  static constexpr float MAGIC = 12582912.f;
 
-  __device__ __forceinline__ float stretch(float v) const { return scale > 0.f ? fminf((top - v) * scale, (float)(BINS - 1)) : 0.f; }
+  // 1.5 2^23 + bin: whole numbers are what floats hold there. The bin rises as v falls
+  __device__ __forceinline__ float stretch(float v) const { return fminf(__fmaf_rn(top - v, scale, MAGIC), scale > 0.f ? MAGIC + (BINS - 1) : MAGIC); }
+  __device__ __forceinline__ bool near(float v) const { return (v >= from) & !(v >= below); }
   __device__ __forceinline__ bool member(float v, int id) const {
-    const float at = stretch(v);
-    bool in = (at >= first_bin) & (at < first_bin + 1.f) & cut.has(v, id);
-    if (split) in = in & (place_of(v, id) >= lo) & (place_of(v, id) <= hi);
-    return in;
+    const u64 at = place_of(clean(v), id);
+    return near(v) && cut.has(v, id) && (!split || (at >= lo && at <= hi));
   }
 
   template <typename Bin>
   __device__ void count(Bin bin) {
-    for (int b = tid; b < BINS * (MASS ? 3 : 1); b += NT) s->part[0][b] = 0;
-    __syncthreads();
-    for (int c = tid; c < quads; c += NT) {
-      const float4 q = vals[c];
-      const float v[4] = {q.x, q.y, q.z, q.w};
-      u64 m[4];
+    const bool whole = cut.x == -INFINITY;
+    for (int b = tid; b < BINS; b += NT) s->mine[b] = 0;
+    for (int first = 0; first < eights || first == 0; first += PART_EIGHTS) {
+      for (int b = tid; b < BINS * (MASS ? 3 : 1); b += NT) s->part[0][b] = 0;
+      __syncthreads();
+      row.each(first + tid, min(eights, first + PART_EIGHTS), NT, [&](int i, const float4& q) {
+        const float v[4] = {q.x, q.y, q.z, q.w};
+        int b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m[j] = MASS ? w.fixed(v[j]) : 1;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int id = base + 4 * c + j;
-        if (!cut.has(v[j], id)) continue;
-        const int b = bin(v[j], id);
-        if (b < 0) continue;
-        if (!MASS) {
-          atomicAdd(&s->part[0][b], 1u);
-          continue;
+        for (int j = 0; j < 4; ++j) {
+          const int id = base + i + j;
+          b[j] = whole || cut.has(v[j], id) ? bin(v[j], id) : -1;
+          if (!MASS && b[j] >= 0 && v[j] > -INFINITY) atomicAdd(&s->part[0][b[j]], 1u);
         }
         constexpr uint32_t low = (1u << 17) - 1;
-        const uint32_t a0 = (uint32_t)m[j] & low, a1 = (uint32_t)(m[j] >> 17) & low, a2 = (uint32_t)(m[j] >> 34);
-        if (a0) atomicAdd(&s->part[0][b], a0);
-        if (a1) atomicAdd(&s->part[1][b], a1);
-        if (a2) atomicAdd(&s->part[2][b], a2);
-      }
+        if (MASS)
+          w.of(
+              v,
+              [&](int j, uint32_t m) {
+                if (b[j] < 0) return;
+                atomicAdd(&s->part[0][b[j]], m & low);               // (additions of 0 cost less than branches)
+                atomicAdd(&s->part[1][b[j]], m >> 17);
+              },
+              [&](int j, u64 m) {
+                if (b[j] < 0) return;
+                atomicAdd(&s->part[0][b[j]], (uint32_t)m & low);
+                atomicAdd(&s->part[1][b[j]], (uint32_t)(m >> 17) & low);
+                atomicAdd(&s->part[2][b[j]], (uint32_t)(m >> 34));
+              });
+      });
+      __syncthreads();
+      for (int b = tid; b < BINS; b += NT) s->mine[b] += MASS ? s->part[0][b] + ((u64)s->part[1][b] << 17) + ((u64)s->part[2][b] << 34) : s->part[0][b];
+      __syncthreads();
     }
   }
-  // Sums over the cluster, then the bin at which the order passes the place `want`; `above` counts on from `from`. fresh: `want` follows from `share` and the total
-  __device__ void find(cg::cluster_group& cluster, u64 from, bool fresh, u64* want, float share) {
+  // Sums over the cluster, then the bin at which the order passes the place `want`; `above` counts on from `ahead`. Returns all that there is. fresh: `want` follows from `share` and the total
+  __device__ u64 find(cg::cluster_group& cluster, u64 ahead, bool fresh, u64* want, float share) {
     cluster.sync();
     // each CTA adds up its share of the bins, four threads a bin
     const int lane = tid & 31, warp = tid >> 5, four = tid & 3;
@@ -168,11 +304,7 @@ struct Search {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = four + 4 * h;
-        if (r < ranks) {
-          const Shared* o = cluster.map_shared_rank(s, r);
-          m += o->part[0][b];
-          if (MASS) m += ((u64)o->part[1][b] << 17) + ((u64)o->part[2][b] << 34);
-        }
+        if (r < ranks) m += cluster.map_shared_rank(s, r)->mine[b];
       }
       m += __shfl_xor_sync(0xffffffffu, m, 1);
       m += __shfl_xor_sync(0xffffffffu, m, 2);
@@ -192,7 +324,7 @@ struct Search {
     }
     if (lane == 31) s->warp_sum[warp] = sum;
     __syncthreads();
-    u64 before = from, all = from;
+    u64 before = ahead, all = ahead;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
       const u64 x = s->warp_sum[i];
@@ -210,42 +342,45 @@ struct Search {
       s->above = second ? mid : excl;
     }
     __syncthreads();
+    return all;
   }
   // the members into every CTA's list; their number (of which the list holds LIST at most)
   __device__ uint32_t gather(cg::cluster_group& cluster) {
     uint32_t* counter = &cluster.map_shared_rank(s, 0)->listed[*turn & 1];
     if (rank == 0 && tid == 0) s->listed[(*turn + 1) & 1] = 0;        // the next turn's; the turn before has been read ahead of a barrier of the cluster
     *turn += 1;
-    for (int c = tid; c < quads; c += NT) {
-      const float4 q = vals[c];
+    row.each(tid, eights, NT, [&](int i, const float4& q) {
       const float v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int id = base + 4 * c + j;
-        if (!member(v[j], id)) continue;
+        const int id = base + i + j;
+        if (!near(v[j]) || !member(v[j], id)) continue;
         const uint32_t at = atomicAdd(counter, 1u);
         if (at < LIST) {
-          const Entry e{place_of(v[j], id), MASS ? w.fixed(v[j]) : 1};
+          const Entry e{place_of(clean(v[j]), id), MASS ? w.fixed(v[j]) : 1};
           for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(s, r)->list[at] = e;
         }
       }
-    }
+    });
     cluster.sync();
     return *counter;
   }
 
   __device__ Cut run(cg::cluster_group& cluster, u64 want, float share) {
-    count([&](float v, int) { return (int)stretch(v); });
-    find(cluster, 0, true, &want, share);
-    first_bin = (float)s->bin;
+    count([&](float v, int) { return __float_as_int(stretch(v)) & (BINS - 1); });
+    if (find(cluster, 0, true, &want, share) < want) return Cut{-INFINITY, INT_MAX};          // fewer tokens than that
     u64 above = s->above;
+    const float bin = MAGIC + s->bin;
+    const int lane = tid & 31;
+    from = fmaxf(lowest([&](float v) { return stretch(v) <= bin; }, scale > 0.f ? top - (s->bin + 0.5f) / scale : 0.f, top, lane), -3.4028234664e38f);
+    below = s->bin ? lowest([&](float v) { return stretch(v) < bin; }, top - (s->bin - 0.5f) / scale, top, lane) : NAN;
     split = false;
     lo = 0;
     hi = (1ull << (32 + ID_BITS)) - 1;
     uint32_t m = gather(cluster);
     for (int shift = 32 + ID_BITS - 10; m > LIST; shift = max(0, shift - 10)) {
       split = true;
-      count([&](float v, int id) { return member(v, id) ? (int)((hi - place_of(v, id)) >> shift) : -1; });
+      count([&](float v, int id) { return near(v) && member(v, id) ? (int)((hi - place_of(clean(v), id)) >> shift) : -1; });
       find(cluster, above, false, &want, share);
       above = s->above;
       hi -= (u64)s->bin << shift;
@@ -267,87 +402,66 @@ struct Search {
   }
 };
 
-__device__ __forceinline__ float load_one(const float* p) { return __ldcs(p); }
-__device__ __forceinline__ float load_one(const bf16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void load_eight(const float* p, float (&f)[8]) {
-  const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-__device__ __forceinline__ void load_eight(const bf16* p, float (&f)[8]) { unpack8(__ldcs(reinterpret_cast<const uint4*>(p)), f); }
-
-template <typename In>
+template <typename In, bool HELD>
 __global__ void __launch_bounds__(NT, 2) draw_kernel(DrawParams p) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared* s = reinterpret_cast<Shared*>(raw);
-  float* vals = reinterpret_cast<float*>(raw + (sizeof(Shared) + 15) / 16 * 16);
-  float4* quad = reinterpret_cast<float4*>(vals);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / ranks;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int base = rank * p.slice, n = max(0, min(p.slice, p.V - base)), quads = (n + 3) / 4;
+  const int base = rank * p.slice, n = max(0, min(p.slice, p.V - base)), eights = (n + 7) / 8;
+  using R = Row<In, HELD>;
+  const R tokens{reinterpret_cast<float4*>(raw + (sizeof(Shared) + 15) / 16 * 16), reinterpret_cast<const In*>(p.logits) + (long)row * p.ld + base, n, p.wide ? n / 8 : 0};
   grid_dep_launch();
   if (tid < 2) s->listed[tid] = 0;
-  if (tid < PARTS) s->parts[tid] = exp2((double)tid / PARTS);
+  if (tid < PARTS) s->parts[tid] = (u64)(exp2(-(double)tid / PARTS) * 0x1p62) + (1ull << 31);
   auto here = cluster.barrier_arrive();          // the others' memory is written to once they run
   grid_dep_wait();
-  const In* src = reinterpret_cast<const In*>(p.logits) + (long)row * p.ld + base;
-  float most = -INFINITY, least = INFINITY;
-  const int whole = p.wide ? n / 8 : 0;
-  constexpr int AT_ONCE = 4;
-  for (int c0 = tid; c0 < whole; c0 += AT_ONCE * NT) {
-    float f[AT_ONCE][8];
+  float most = -INFINITY;
+  auto take = [&](int i, const float4& q) {
+    most = fmaxf(fmaxf(most, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));         // (passes over NaN)
+    if (HELD) tokens.own[i / 4] = q;
+  };
+  if constexpr (HELD) {
+    constexpr int AT_ONCE = 5;                   // (a row of 160000 over eight CTAs at one go)
+    for (int o0 = tid; o0 < tokens.full; o0 += AT_ONCE * NT) {
+      float4 a[AT_ONCE], b[AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k)
-      if (c0 + k * NT < whole) load_eight(src + 8 * (c0 + k * NT), f[k]);
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (o0 + k * NT < tokens.full) R::eight(tokens.src + 8 * (o0 + k * NT), a[k], b[k]);
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const int c = c0 + k * NT;
-      if (c >= whole) break;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        f[k][j] = clean(f[k][j]);
-        most = fmaxf(most, f[k][j]);
-        if (f[k][j] != -INFINITY) least = fminf(least, f[k][j]);
-      }
-      quad[2 * c] = make_float4(f[k][0], f[k][1], f[k][2], f[k][3]);
-      quad[2 * c + 1] = make_float4(f[k][4], f[k][5], f[k][6], f[k][7]);
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (o0 + k * NT < tokens.full) {
+          take(8 * (o0 + k * NT), a[k]);
+          take(8 * (o0 + k * NT) + 4, b[k]);
+        }
     }
-  }
-  for (int i = 8 * whole + tid; i < 4 * quads; i += NT) {
-    const float v = i < n ? clean(load_one(src + i)) : -INFINITY;
-    vals[i] = v;
-    most = fmaxf(most, v);
-    if (v != -INFINITY) least = fminf(least, v);
+    for (int i = 8 * tokens.full + tid; i < 8 * eights; i += NT) {
+      const float v = i < n ? load_one(tokens.src + i) : -INFINITY;
+      reinterpret_cast<float*>(tokens.own)[i] = v;
+      most = fmaxf(most, v);
+    }
+  } else {
+    tokens.each(tid, eights, NT, take);
   }
   most = warp_max(most);
-  least = -warp_max(-least);
-  if (lane == 0) {
-    s->warp_a[warp] = most;
-    s->warp_b[warp] = least;
-  }
+  if (lane == 0) s->warp_a[warp] = most;
   __syncthreads();
-  for (int i = 0; i < WARPS; ++i) {
-    most = fmaxf(most, s->warp_a[i]);
-    least = fminf(least, s->warp_b[i]);
-  }
+  most = warp_max(s->warp_a[lane % WARPS]);
   cluster.barrier_wait(std::move(here));
-  if (tid < ranks) {
-    Shared* o = cluster.map_shared_rank(s, tid);
-    o->most[rank] = most;
-    o->least[rank] = least;
-  }
+  if (tid < ranks) cluster.map_shared_rank(s, tid)->most[rank] = most;
   cluster.sync();
-  for (int r = 0; r < ranks; ++r) {
-    most = fmaxf(most, s->most[r]);
-    least = fminf(least, s->least[r]);
-  }
+  for (int r = 0; r < ranks; ++r) most = fmaxf(most, s->most[r]);
   const float it = p.inv_temperature ? p.inv_temperature[row] : 1.f;
   const bool greedy = !(it > 0.f) || it == INFINITY;
   if (greedy || most == -INFINITY) {              // the first of the largest; nothing where everything is masked
     int id = INT_MAX;
-    for (int i = tid; i < n; i += NT)
-      if (vals[i] == most) { id = base + i; break; }
+    tokens.each(tid, eights, NT, [&](int i, const float4& q) {
+      const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v[j] == most && id == INT_MAX) id = base + i + j;
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) id = min(id, __shfl_xor_sync(0xffffffffu, id, o));
     if (lane == 0) s->warp_i[warp] = id;
@@ -369,62 +483,39 @@ __global__ void __launch_bounds__(NT, 2) draw_kernel(DrawParams p) {
   const Cut all{-INFINITY, INT_MAX};
   Cut cut = all;
   const Weights w(most, it, s->parts);
-  const float span = fminf(most, 3.0e38f) - least;
-  const float scale = span > 0.f && span < 3.0e38f && most < INFINITY ? (float)(BINS - 1) / span : 0.f;
+  const float scale = most < INFINITY ? fminf(it * ((BINS - 1) / 24.f), 1e30f) : 0.f;         // the bins reach down to weights of e^-24; what lies below is in the last one
   uint32_t turn = 0;
   const int k = p.top_k ? p.top_k[row] : 0;
   const float least_share = p.min_p ? p.min_p[row] : 0.f, share = p.top_p ? p.top_p[row] : 1.f;
   // of a weight limit above 1 the first token is left
   const int count = least_share > 1.f ? 1 : k;
   if (count >= 1 && count < p.V) {
-    Search<false> f{s, quad, quads, base, tid, rank, ranks, &turn, all, w, most, scale};
+    Search<false, R> f{s, tokens, eights, base, tid, rank, ranks, &turn, all, w, most, scale};
     cut = f.run(cluster, count, 0.f);
   }
   if (least_share > 0.f && least_share <= 1.f) {
-    // the lowest value whose weight is enough: the predicate is monotone in the value's key, so each lane tries one of 32 places, 32 times finer every round
-    uint32_t at = key_of(-INFINITY), step = 1u << 27;         // the value lies in (at, at + 32 steps], or is the largest itself
-    const uint32_t end = key_of(most);
-    for (int round = 0; round < 7; ++round) {
-      const u64 mine = (u64)at + (u64)(lane + 1) * step;
-      const bool enough = mine >= end || w.real(value_of((uint32_t)mine)) >= (double)least_share;
-      const uint32_t vote = __ballot_sync(0xffffffffu, enough);
-      const int first = vote ? __ffs(vote) - 1 : 32;
-      at += (uint32_t)first * step;
-      step = step >= 32 ? step / 32 : 1;
-    }
-    const u64 key = (u64)at + 1;
-    const float v = key >= end ? most : value_of((uint32_t)key);
+    const float v = lowest([&](float x) { return w.real(x) >= (double)least_share; }, (float)((w.z_most + log((double)least_share)) / w.it), most, lane);
     if (v > cut.x) cut = Cut{v, INT_MAX};
   }
   if (share < 1.f) {
-    Search<true> f{s, quad, quads, base, tid, rank, ranks, &turn, cut, w, most, scale};
+    Search<true, R> f{s, tokens, eights, base, tid, rank, ranks, &turn, cut, w, most, scale};
     cut = f.run(cluster, 0, share);
   }
 
   // the kept tokens' masses: a warp's stretch of ids each, so that sums by rising ids need no more than the stretches' sums
-  const int each = (quads + WARPS - 1) / WARPS, first = min(quads, warp * each), last = min(quads, first + each);
-  auto kept = [&](int c, u64 (&m)[4]) {
-    const float4 q = quad[c];
+  const int each = (eights + WARPS - 1) / WARPS, first = min(eights, warp * each), last = min(eights, first + each);
+  const bool everyone = cut.x == -INFINITY;
+  // m(j, weight) for the kept ones of a four, maybe in two calls
+  auto kept = [&](int i, const float4& q, auto m) {
     const float v[4] = {q.x, q.y, q.z, q.w};
+    if (!everyone && !__any_sync(__activemask(), (v[0] >= cut.x) | (v[1] >= cut.x) | (v[2] >= cut.x) | (v[3] >= cut.x))) return;
     bool has[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) has[j] = cut.has(v[j], base + 4 * c + j);
-    if (__any_sync(__activemask(), has[0] || has[1] || has[2] || has[3])) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = w.fixed(v[j]);
-        if (!has[j]) m[j] = 0;
-      }
-    } else {
-      m[0] = m[1] = m[2] = m[3] = 0;
-    }
+    for (int j = 0; j < 4; ++j) has[j] = everyone || cut.has(v[j], base + i + j);
+    w.of(v, [&](int j, uint32_t x) { m(j, (u64)(has[j] ? x : 0u)); }, [&](int j, u64 x) { if (has[j]) m(j, x); });
   };
   u64 sum = 0;
-  for (int c = first + lane; c < last; c += 32) {
-    u64 m[4];
-    kept(c, m);
-    sum += (m[0] + m[1]) + (m[2] + m[3]);
-  }
+  tokens.each(first + lane, last, 32, [&](int i, const float4& q) { kept(i, q, [&](int, u64 x) { sum += x; }); });
   sum = warp_total(sum);
   if (lane == 0) s->warp_sum[warp] = sum;
   __syncthreads();
@@ -445,10 +536,10 @@ __global__ void __launch_bounds__(NT, 2) draw_kernel(DrawParams p) {
   if (target < before || target >= before + s->from[rank]) return;
   for (int i = 0; i < warp; ++i) before += s->warp_sum[i];
   if (target < before || target >= before + s->warp_sum[warp]) return;
-  for (int c0 = first; c0 < last && target >= before; c0 += 32) {
-    const int c = c0 + lane;
+  for (int i0 = 8 * first; i0 < 8 * last && target >= before; i0 += 128) {
+    const int i = i0 + 4 * lane;
     u64 m[4] = {0, 0, 0, 0};
-    if (c < last) kept(c, m);
+    if (i < 8 * last) kept(i, tokens.slow(i), [&](int j, u64 x) { m[j] += x; });
     const u64 mine = (m[0] + m[1]) + (m[2] + m[3]);
     u64 incl = mine;
 #pragma unroll
@@ -462,8 +553,8 @@ __global__ void __launch_bounds__(NT, 2) draw_kernel(DrawParams p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (target >= run && target < run + m[j]) {
-          p.out_ids[row] = base + 4 * c + j;
-          if (p.out_probs) p.out_probs[row] = (float)(w.real(vals[4 * c + j]) / ((double)total * 0x1p-44));
+          p.out_ids[row] = base + i + j;
+          if (p.out_probs) p.out_probs[row] = (float)(w.real(tokens.at(i + j)) / ((double)total * 0x1p-44));
         }
         run += m[j];
       }
@@ -472,12 +563,10 @@ __global__ void __launch_bounds__(NT, 2) draw_kernel(DrawParams p) {
   }
 }
 
-template <typename In>
-int launch(const DrawParams& p, int ranks, cudaStream_t s) {
-  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)p.slice * sizeof(float);
-  auto k = draw_kernel<In>;
-  if (int rc = opt_in_smem_once<draw_kernel<In>>((sizeof(Shared) + 15) / 16 * 16 + MAX_SLICE * sizeof(float))) return rc;
-  return launch_chain_cluster(k, dim3((unsigned)(p.T * ranks)), dim3(NT), (unsigned)ranks, smem, s, p);
+template <typename In, bool HELD>
+int launch(const DrawParams& p, int ranks, size_t smem, cudaStream_t s) {
+  if (int rc = opt_in_smem_once<draw_kernel<In, HELD>>(200 * 1024)) return rc;
+  return launch_clusters(true, draw_kernel<In, HELD>, dim3((unsigned)(p.T * ranks)), dim3(NT), (unsigned)ranks, smem, s, p);
 }
 
 }  // namespace
@@ -485,11 +574,15 @@ int launch(const DrawParams& p, int ranks, cudaStream_t s) {
 extern "C" int ifab_draw(const void* logits, long ld, int f32, int T, int V, const float* inv_temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                          const float* uniforms, int32_t* out_ids, float* out_probs, void* stream) {
   if (!logits || !uniforms || !out_ids || T < 1 || T > 1 << 20 || V < 1 || V > MAX_VOCAB || (T > 1 && ld < V)) return -1;
+  // As many CTAs a row as run at once, two an SM. Few rows are held in shared memory; of many, a CTA's share does not fit, and is read again from the L2 cache by each pass
   int ranks = MAX_CLUSTER;
-  while (ranks > 1 && V < 1024 * ranks) ranks /= 2;
-  const int slice = ((V + ranks - 1) / ranks + 7) / 8 * 8;
-  const int size = f32 ? 4 : 2;
+  while (ranks > 1 && (V < 1024 * ranks || (long)T * ranks > 296)) ranks /= 2;
+  const int slice = ((V + ranks - 1) / ranks + 7) / 8 * 8, size = f32 ? 4 : 2;
+  const size_t fixed = (sizeof(Shared) + 15) / 16 * 16, held = fixed + (size_t)slice * sizeof(float), rings = fixed + (size_t)Row<float, false>::AHEAD * NT * 8 * size;
+  const bool holds = held <= ((long)T * ranks <= 148 ? 200 : 112) * 1024;
   const bool wide = (uintptr_t)logits % 16 == 0 && (T == 1 || ld * size % 16 == 0);
   const DrawParams p{logits, ld, T, V, slice, wide, inv_temperature, top_p, min_p, uniforms, top_k, out_ids, out_probs};
-  return f32 ? launch<float>(p, ranks, (cudaStream_t)stream) : launch<bf16>(p, ranks, (cudaStream_t)stream);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (holds) return f32 ? launch<float, true>(p, ranks, held, s) : launch<bf16, true>(p, ranks, held, s);
+  return f32 ? launch<float, false>(p, ranks, rings, s) : launch<bf16, false>(p, ranks, rings, s);
 }
