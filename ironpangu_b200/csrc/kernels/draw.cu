@@ -77,6 +77,9 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k
 // (value, id) in the order of the tokens
 __device__ __forceinline__ u64 place_of(float v, int id) { return (u64)key_of(v) << ID_BITS | (u64)((1 << ID_BITS) - 1 - id); }
 
+// the cut whose last token lies there
+__device__ __forceinline__ Cut cut_at(u64 place) { return {value_of((uint32_t)(place >> ID_BITS)), (1 << ID_BITS) - 1 - (int)(place & ((1 << ID_BITS) - 1))}; }
+
 // Weights e^((v - most) it) in units of 2^-44, rounded. With c = it log2 e as two floats,
 //   v c = n / 128 + r: n / 128 by an addition of 1.5 2^16, whose floats lie 1 / 128 apart, and r (at most 1 / 256) by a product that is rounded only then, so both without loss
 //   weight = 2^-((n_most - n) / 128) (1 + q), q = 2^(r - r_most) - 1 by Taylor's series: of at most 0.0055, it is off by 2^-31 as a float
@@ -117,21 +120,31 @@ struct Weights {
       }
       return;
     }
+    uint32_t top[N];                                       // 30 bits of a weight
+    int by[N];                                             // 0 or more: what they are shifted by before their last bit is rounded away
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < N; ++i) {                          // (all of them ahead of what is done with them: chains that run side by side)
       const float y = __fmaf_rn(v[i], ch, MAGIC), r = __fmaf_rn(v[i], cl, __fmaf_rn(v[i], ch, MAGIC - y)) - r_most;
       const float q = __fmaf_rn(__fmaf_rn(r, C3, C2), r, C1) * r;
-      const int n = n_most - __float_as_int(y), by = (n >> 7) - 15;              // 0 or more; what the upper word is shifted by before its last bit is rounded away
+      const int n = n_most - __float_as_int(y);
       const u64 t = parts[n & 127];
       u64 part;
       asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(part) : "r"((int)(t >> 38)), "r"(__float2int_rn(q)), "l"(t));
-      const uint32_t top = (uint32_t)(part >> 32);                               // 30 bits of it
-      uint32_t m;
-      asm("shr.u32 %0, %1, %2;" : "=r"(m) : "r"(top), "r"(by));                  // (32 and more, and less than 0, leave 0)
-      const bool there = v[i] >= floor;                                          // what lies below, or is none, has been anything
-      small(i, there ? (m + 1) >> 1 : 0u);
-      if (there & (by < 0)) large(i, (u64)top << (-1 - by));
+      top[i] = v[i] >= floor ? (uint32_t)(part >> 32) : 0u;                      // what lies below, or is none, has been anything
+      by[i] = (n >> 7) - 15;
     }
+    int least = by[0];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t m;
+      asm("shr.u32 %0, %1, %2;" : "=r"(m) : "r"(top[i]), "r"(by[i]));            // (32 and more, and less than 0, leave 0)
+      small(i, (m + 1) >> 1);
+      least = min(least, by[i]);
+    }
+    if (least < 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (by[i] < 0 && top[i]) large(i, (u64)top[i] << (-1 - by[i]));
   }
   __device__ __forceinline__ u64 fixed(float v) const {
     const float a[1] = {v};
@@ -266,6 +279,7 @@ struct Search {
       __syncthreads();
       row.each(first + tid, min(eights, first + PART_EIGHTS), NT, [&](int i, const float4& q) {
         const float v[4] = {q.x, q.y, q.z, q.w};
+        if (!whole && !__any_sync(__activemask(), (v[0] >= cut.x) | (v[1] >= cut.x) | (v[2] >= cut.x) | (v[3] >= cut.x))) return;
         int b[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -387,15 +401,51 @@ struct Search {
       lo = hi - ((1ull << shift) - 1);
       m = gather(cluster);
     }
-    for (uint32_t i = tid; i < m; i += NT) {
-      const Entry mine = s->list[i];
-      u64 ahead = above;
+    if (m <= 128) {                              // in order by counting: a pair of them costs 7 instructions
+      if (tid < m) {
+        const Entry mine = s->list[tid];
+        u64 ahead = above;
 #pragma unroll 8
-      for (uint32_t j = 0; j < m; ++j) {
-        const Entry e = s->list[j];
-        ahead += e.place > mine.place ? e.mass : 0;
+        for (uint32_t j = 0; j < m; ++j) {
+          const Entry e = s->list[j];
+          ahead += e.place > mine.place ? e.mass : 0;
+        }
+        if (ahead < want && want <= ahead + mine.mass) s->cut = cut_at(mine.place);
       }
-      if (ahead < want && want <= ahead + mine.mass) s->cut = Cut{value_of((uint32_t)(mine.place >> ID_BITS)), (1 << ID_BITS) - 1 - (int)(mine.place & ((1 << ID_BITS) - 1))};
+    } else {                                     // a bitonic sort, then their sums: 1000 tokens by counting took as long as a pass over the row
+      uint32_t size = 256;
+      while (size < m) size *= 2;
+      for (uint32_t i = m + tid; i < size; i += NT) s->list[i] = Entry{0, 0};
+      static_assert(LIST <= 2 * NT, "a pair a thread");
+      for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+          __syncthreads();
+          if (tid < size / 2) {
+            const uint32_t at = 2 * tid - (tid & (j - 1));
+            const Entry x = s->list[at], y = s->list[at + j];
+            if ((x.place < y.place) == ((at & k) == 0)) {
+              s->list[at] = y;
+              s->list[at + j] = x;
+            }
+          }
+        }
+      __syncthreads();
+      const bool mine = 2 * tid < size;
+      const Entry x = mine ? s->list[2 * tid] : Entry{0, 0}, y = mine ? s->list[2 * tid + 1] : Entry{0, 0};
+      u64 sum = x.mass + y.mass;
+      const int warp = tid >> 5;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 z = shfl_up64(sum, o);
+        if (lane >= o) sum += z;
+      }
+      if (lane == 31) s->warp_sum[warp] = sum;
+      __syncthreads();
+      u64 ahead = above + sum - x.mass - y.mass;
+      for (int i = 0; i < warp; ++i) ahead += s->warp_sum[i];
+      if (ahead < want && want <= ahead + x.mass) s->cut = cut_at(x.place);
+      ahead += x.mass;
+      if (ahead < want && want <= ahead + y.mass) s->cut = cut_at(y.place);
     }
     __syncthreads();
     return s->cut;
