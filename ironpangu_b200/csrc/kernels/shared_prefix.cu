@@ -6,14 +6,15 @@
 // A softmax over two parts is put together from their maxima, sums and sums of values, so the parts are worked on by CTAs of their own, as are stretches of a long part; each leaves m, l and O of
 // its rows and heads in the scratch.
 //
-//   up to 32 rows and heads in a group
-//     parts kernel   one CTA per (tile of 16 WM pairs of a group's rows and heads, kv head, stretch of the prefix) and per (row, kv head, stretch of its own keys): products on the tensor cores as
+//   tiles kernel     the prefix of a group with much work, on tcgen05 (shared_prefix_tiles.cu)
+//   parts kernel     the prefix of the others and the rows' own positions: one CTA per (tile of 16 WM pairs of a group's rows and heads, kv head, stretch of the prefix) and per (row, kv head, stretch of its own keys): products on the tensor cores as
 //                    m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
-//     merge kernel   four warps per (row, head): the parts, weighted by e^(m - largest m), over the sum
-//   more
-//     tiles kernel   the prefix on tcgen05 (shared_prefix_tiles.cu)
-//     own kernel     one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result. With too few rows to fill the chip: the parts kernel without a
-//                    prefix and the merge kernel
+//   merge kernel     four warps per (row, head): the parts, weighted by e^(m - largest m), over the sum
+//   own kernel       where rows fill the chip, in place of the two before it: one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result
+//
+// How long a prefix is is known on the device only, so both of the first two kernels start where a group might be either's, and one of them has nothing to do. us with the parts kernel and with the tiles
+// kernel, rows of 4 heads over each of 8 kv heads, behind 500 / 4000 / 30000 positions: 8 rows 11.7 / 16.3 / 60.8 and 23.5 / 29 / 50, 16 rows 15.6 / 23.1 / 90.5 and 25.0 / 33.2 / 56.4; over 4 kv heads
+// 16 rows 15.5 / 18.7 / 51.6 and 24.9 / 29.3 / 37.9.
 #include <algorithm>
 
 #include "mma16816.cuh"
@@ -310,8 +311,8 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
   grid_dep_wait();
   int item = blockIdx.x;
   if (item < prefix_items) {
-    const int split = item % p.prefix_splits, kvh = item / p.prefix_splits % p.Hkv;
-    int tile = item / p.prefix_splits / p.Hkv, end = 0;
+    const int split = item % p.part_splits, kvh = item / p.part_splits % p.Hkv;
+    int tile = item / p.part_splits / p.Hkv, end = 0;
     PrefixGroup gr;
     for (int i = 0;; ++i) {
       if (i == p.groups) return;
@@ -320,10 +321,14 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
       if (tile < tiles) break;
       tile -= tiles;
     }
-    const int per = p.per_split(gr.shared, p.prefix_splits), begin = split * per, x0 = tile * 16 * WM;
+    if (p.by_tiles()) return;
+    const int per = p.per_split(gr.shared, p.part_splits), begin = split * per, x0 = tile * 16 * WM;
     for (int x = x0 + threadIdx.x; x < min(x0 + 16 * WM, gr.rows * p.G); x += NT) {
       const int t = gr.first + x / p.G;
-      if (begin >= gr.shared || !p.sees(gr, t)) p.sums[p.part_of(t, kvh * p.G + x % p.G, split)] = nothing;
+      const long at = p.part_of(t, kvh * p.G + x % p.G, split);
+      if (begin >= gr.shared || !p.sees(gr, t)) p.sums[at] = nothing;
+      if (split == 0)
+        for (int i = p.part_splits; i < p.prefix_parts; ++i) p.sums[at + i] = nothing;
     }
     if (begin >= gr.shared) return;
     auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, 3>*>(smem);
@@ -339,20 +344,20 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
         [&](int i, const float (&M)[1], const float (&L)[1], const float (&v)[1][E]) { store_part<E>(p, u.part[i], M[0], L[0], v[0], lane); });
   } else {
     item -= prefix_items;
-    const int split = item % p.own_splits, kvh = item / p.own_splits % p.Hkv, t0 = item / p.own_splits / p.Hkv, prefix_parts = p.streams * p.prefix_splits;
+    const int split = item % p.own_splits, kvh = item / p.own_splits % p.Hkv, t0 = item / p.own_splits / p.Hkv;
     const PrefixGroup gr = p.naming(t0);
     const PrefixOwn own = p.own(t0, gr);
     const int per = p.per_split(own.end - own.begin, p.own_splits), begin = own.begin + split * per;
     if (p.positions[t0] < 0) return;
     if (!gr.rows && split == 0)
-      for (int i = threadIdx.x; i < p.G * prefix_parts; i += NT) p.sums[p.part_of(t0, kvh * p.G + i / prefix_parts, i % prefix_parts)] = nothing;
+      for (int i = threadIdx.x; i < p.G * p.prefix_parts; i += NT) p.sums[p.part_of(t0, kvh * p.G + i / p.prefix_parts, i % p.prefix_parts)] = nothing;
     if (begin >= own.end) {
-      for (int i = threadIdx.x; i < p.G; i += NT) p.sums[p.part_of(t0, kvh * p.G + i, prefix_parts + split)] = nothing;
+      for (int i = threadIdx.x; i < p.G; i += NT) p.sums[p.part_of(t0, kvh * p.G + i, p.prefix_parts + split)] = nothing;
       return;
     }
     auto& u = *reinterpret_cast<Unit<HD, 4, 16, 3>*>(smem);
     attend<HD, 4, 1, 3, 1>(
-        p, u, begin, min(begin + per, own.end), own.slot, kvh, prefix_parts + split,
+        p, u, begin, min(begin + per, own.end), own.slot, kvh, p.prefix_parts + split,
         [&](int i, int* t, int* h) {
           *t = t0;
           *h = kvh * p.G + i;
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(NT) prefix_merge_kernel(PrefixParams p, bf16* 
   grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   const long base = p.part_of(t, h, 0);
-  const int n = p.streams * p.prefix_splits + p.own_splits, each = (n + W - 1) / W;
+  const int n = p.prefix_parts + p.own_splits, each = (n + W - 1) / W;
   const float M[1] = {largest(p, base, n, lane)};
   if (p.positions[t] < 0) return;
   float part[1][E] = {}, sum[1] = {0.f};
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p
   if (t0 >= p.T || p.positions[t0] < 0) return;
   const PrefixGroup gr = p.naming((int)t0);
   const PrefixOwn own = p.own((int)t0, gr);
-  const int per = p.per_split(gr.shared, max(1, p.prefix_splits)), parts = p.sees(gr, (int)t0) ? (gr.shared + per - 1) / per * p.streams : 0;
+  const int per = p.per_split(gr.shared, max(1, p.tile_splits)), parts = p.sees(gr, (int)t0) ? (gr.shared + per - 1) / per * 2 : 0;
   auto& u = reinterpret_cast<Unit<HD, W, 16, OWN_STAGES>*>(smem)[unit];
   attend<HD, W, 1, OWN_STAGES, P>(
       p, u, own.begin, own.end, own.slot, kvh, 0,
@@ -437,21 +442,35 @@ __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p
 
 // how a call is shared out
 struct Plan {
-  int wm, tiles, prefix_splits, own_splits, streams, own_warps;     // wm 0: the prefix on tcgen05; own_warps 0: own parts and a merge, else the own kernel
+  int wm;                                // tiles of 16 wm pairs by the parts kernel; 0: none of a prefix
+  bool tiles;                            // by the tiles kernel
+  int own_warps;                         // of the own kernel's units; 0: own parts by the parts kernel, and a merge
+  int part_tiles, part_splits, tile_tiles, tile_splits, own_splits;
+  long tiles_from;
+  int prefix_parts() const { return std::max(part_splits, 2 * tile_splits); }
 };
-Plan plan_of(int T, int Hkv, int G, int groups, bool tcgen05) {
+// `most`: positions that a slot has room for
+Plan plan_of(int T, int Hkv, int G, int groups, bool tcgen05, long most) {
   Plan a{};
   auto splits = [](long items, long ctas, int most) { return (int)std::max(1l, std::min((long)most, ctas / std::max(1l, items))); };
-  const int rows = groups ? (T + groups - 1) / groups * G : 1;
+  auto tiles = [&](int pairs) { return groups ? (int)std::max((long)groups, ((long)T * G - groups) / pairs + groups) : 0; };          // at most, however the rows are shared out
   const long items = (long)T * Hkv;
-  a.wm = rows <= 16 ? 1 : rows <= 32 ? 2 : tcgen05 ? 0 : 4;
-  a.streams = a.wm ? 1 : 2;
-  const int tile = a.wm ? 16 * a.wm : 256;
-  a.tiles = groups ? (int)std::max((long)groups, ((long)T * G - groups) / tile + groups) : 0;        // at most, however the rows are shared out
-  // One wave: 148 CTAs of either kind side by side, two an SM; tcgen05's have an SM each
-  a.prefix_splits = groups ? splits((long)a.tiles * Hkv, 148, 148) : 0;
-  a.own_splits = splits(items, 148, 16);
-  a.own_warps = a.wm || items < 148 ? 0 : items < 1184 ? 4 : 1;
+  const int rows = groups ? (T + groups - 1) / groups * G : 1;
+  const bool full = items >= 400;
+  a.tiles_from = !tcgen05 ? 1l << 62 : full ? 0 : 3500000 / Hkv;        // by the figures above
+  a.tiles = groups && ((long)T * G + 16 * groups) * most >= a.tiles_from;
+  a.wm = !groups || (a.tiles && full) ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  // One wave: 148 CTAs of the prefix and as many of the rows' own positions side by side, two an SM; the tiles kernel's have an SM each
+  if (a.wm) {
+    a.part_tiles = tiles(16 * a.wm);
+    a.part_splits = splits((long)a.part_tiles * Hkv, 148, 148);
+  }
+  if (a.tiles) {
+    a.tile_tiles = tiles(256);
+    a.tile_splits = splits((long)a.tile_tiles * Hkv, 148, 148);
+  }
+  a.own_splits = splits(items, a.tiles ? 296 : 148, 16);
+  a.own_warps = !a.tiles || !full ? 0 : items < 1184 ? 4 : 1;
   return a;
 }
 
@@ -473,12 +492,12 @@ int launch_own(const PrefixParams& p, bf16* out, long ldo, cudaStream_t s) {
 }
 template <int HD>
 int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream_t s) {
-  const long items = (long)a.tiles * p.Hkv * a.prefix_splits;
-  if (items > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
-  if (!a.wm)
-    if (int rc = launch_prefix_tiles(p, HD, items, s)) return rc;
+  const long parts = (long)a.part_tiles * p.Hkv * a.part_splits, tiles = (long)a.tile_tiles * p.Hkv * a.tile_splits;
+  if (parts > 0x7fffffff || tiles > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
+  if (a.tiles)
+    if (int rc = launch_prefix_tiles(p, HD, tiles, s)) return rc;
   if (a.own_warps) return a.own_warps == 4 ? launch_own<HD, 4>(p, out, ldo, s) : launch_own<HD, 1>(p, out, ldo, s);
-  if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, items, s) : a.wm == 2 ? launch_parts<HD, 2>(p, items, s) : launch_parts<HD, 1>(p, a.wm ? items : 0, s)) return rc;
+  if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, parts, s) : a.wm == 2 ? launch_parts<HD, 2>(p, parts, s) : launch_parts<HD, 1>(p, parts, s)) return rc;
   return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)((long)p.T * p.Hq)), dim3(NT), 0, s, p, out, ldo);
 }
 
@@ -486,8 +505,12 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
 
 extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_dim, int groups) {
   if (T < 1 || Hkv < 1 || Hq % Hkv || groups < 0) return 0;
-  const Plan a = plan_of(T, Hkv, Hq / Hkv, groups, true), b = plan_of(T, Hkv, Hq / Hkv, groups, false);
-  return (uint64_t)T * Hq * (std::max(a.streams * a.prefix_splits, b.streams * b.prefix_splits) + a.own_splits) * (head_dim + 2) * sizeof(float);
+  int most = 0;
+  for (int with = 0; with < 2; ++with) {         // whatever the pages
+    const Plan a = plan_of(T, Hkv, Hq / Hkv, groups, with, 0x7fffffff);
+    most = std::max(most, a.prefix_parts() + a.own_splits);
+  }
+  return (uint64_t)T * Hq * most * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
@@ -497,7 +520,7 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   if (T < 1 || T > 1 << 20 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || (head_dim != 64 && head_dim != 128) || num_groups < 0 || num_groups > 64 || (num_groups && !groups)) return -1;
   if (num_slots < 1 || max_pages < 1 || page_tokens < 1 || num_pages < 1 || (long)num_pages * page_tokens > 0x7fffffff || (long)max_pages * page_tokens > 0x7fffffff - 256) return -1;
   if (ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)scratch | (uintptr_t)groups) % 16) return -1;
-  const Plan a = plan_of(T, Hkv, Hq / Hkv, num_groups, page_tokens % 8 == 0);
+  const Plan a = plan_of(T, Hkv, Hq / Hkv, num_groups, page_tokens % 8 == 0, (long)max_pages * page_tokens);
   if (ifab_shared_prefix_scratch(T, Hq, Hkv, head_dim, num_groups) > scratch_bytes) return -5;
   PrefixParams p;
   p.q = (const bf16*)q; p.ldq = ldq; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache;
@@ -505,9 +528,9 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   p.num_slots = num_slots; p.max_pages = max_pages; p.page_tokens = page_tokens; p.num_pages = num_pages; p.groups = num_groups;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
-  p.prefix_splits = a.prefix_splits; p.own_splits = a.own_splits; p.streams = a.streams;
+  p.part_splits = a.part_splits; p.tile_splits = a.tile_splits; p.own_splits = a.own_splits; p.prefix_parts = a.prefix_parts(); p.tiles_from = a.tiles_from;
   p.parts = (float*)scratch;
-  p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.streams * a.prefix_splits + a.own_splits) * head_dim);
+  p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.prefix_parts() + a.own_splits) * head_dim);
   p.status = status;
   return head_dim == 64 ? launch<64>(p, a, (bf16*)out, ldo, (cudaStream_t)stream) : launch<128>(p, a, (bf16*)out, ldo, (cudaStream_t)stream);
 }

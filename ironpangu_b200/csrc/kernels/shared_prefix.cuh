@@ -22,10 +22,12 @@ struct PrefixParams {
   int num_slots, max_pages, page_tokens, num_pages, groups;
   float scale_log2;                              // of a score in powers of two
   int T, Hq, Hkv, G;
-  int prefix_splits, own_splits;                 // stretches that a group's prefix, a row's own positions are shared out to at most
-  int streams;                                   // parts of a stretch of the prefix
-  float* parts;                                  // [T, Hq, streams prefix_splits + own_splits, head_dim]: sums of values
-  float2* sums;                                  // [T, Hq, streams prefix_splits + own_splits]: maximum (in powers of two), sum of weights
+  // stretches that a group's prefix (by the parts kernel; by the tiles kernel, which leaves two parts of each) and a row's own positions are shared out to at most
+  int part_splits, tile_splits, own_splits;
+  int prefix_parts;                              // parts that a row and head has room for ahead of those of its own positions
+  long tiles_from;                               // pairs by positions of all prefixes from which on the tiles kernel has them
+  float* parts;                                  // [T, Hq, prefix_parts + own_splits, head_dim]: sums of values
+  float2* sums;                                  // [T, Hq, prefix_parts + own_splits]: maximum (in powers of two), sum of weights
   uint32_t* status;
 
   // row of the caches; -1: there is none
@@ -53,6 +55,15 @@ struct PrefixParams {
     }
     return {0, 0, 0, 0};
   }
+  __device__ __forceinline__ bool by_tiles() const {
+    long work = 0;
+    int end = 0;
+    for (int i = 0; i < groups; ++i) {
+      const PrefixGroup g = group(i, &end);
+      work += (long)((g.rows * G + 15) / 16 * 16) * g.shared;
+    }
+    return work >= tiles_from;
+  }
   // whether a row of a group sees its prefix as a whole
   __device__ __forceinline__ bool sees(const PrefixGroup& g, int t) const { return g.rows && positions[t] >= 0 && positions[t] + 1 >= g.shared; }
   __device__ __forceinline__ PrefixOwn own(int t, const PrefixGroup& g) const {
@@ -65,7 +76,7 @@ struct PrefixParams {
   }
   // keys of a stretch: whole tiles of the kernels'
   __device__ __forceinline__ int per_split(int n, int splits) const { return max(128, ((n + splits - 1) / splits + 127) / 128 * 128); }
-  __device__ __forceinline__ long part_of(int t, int h, int i) const { return ((long)t * Hq + h) * (streams * prefix_splits + own_splits) + i; }
+  __device__ __forceinline__ long part_of(int t, int h, int i) const { return ((long)t * Hq + h) * (prefix_parts + own_splits) + i; }
 };
 
 // Weights of a softmax, powers of two, as two bf16 terms: both are cut off below the value, so that none is 0 or negative and an infinite value of a key stays infinite (as in

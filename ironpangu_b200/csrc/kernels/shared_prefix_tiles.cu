@@ -135,17 +135,11 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
-  if (warp == 8) tmem_alloc(&B->tmem, 512);      // S of the streams at 0 and 128, O at 256 and 384. Ahead of the launch of dependents, which might hold some and wait for this kernel
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = B->tmem;
-  grid_dep_launch();
   grid_dep_wait();
 
   // this CTA's work
-  const int split = blockIdx.x % p.prefix_splits, kvh = blockIdx.x / p.prefix_splits % p.Hkv;
-  int tile = blockIdx.x / p.prefix_splits / p.Hkv, end_rows = 0;
+  const int split = blockIdx.x % p.tile_splits, kvh = blockIdx.x / p.tile_splits % p.Hkv;
+  int tile = blockIdx.x / p.tile_splits / p.Hkv, end_rows = 0;
   PrefixGroup gr{0, 0, 0, 0};
   for (int i = 0; i < p.groups; ++i) {
     gr = p.group(i, &end_rows);
@@ -154,17 +148,23 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     tile -= tiles;
     gr = PrefixGroup{0, 0, 0, 0};
   }
-  const int per = p.per_split(gr.shared, p.prefix_splits), begin = split * per, end = min(begin + per, gr.shared);
+  if (p.tiles_from && !p.by_tiles()) gr = PrefixGroup{0, 0, 0, 0};         // they are the parts kernel's
+  const int per = p.per_split(gr.shared, p.tile_splits), begin = split * per, end = min(begin + per, gr.shared);
   // parts of rows that do not see the prefix, or that the stretches leave over, are nothing: the merge kernel goes by their sums alone
   for (int x = tile * 2 * TILE + tid; x < min((tile + 1) * 2 * TILE, gr.rows * p.G); x += NT) {
     const int t = gr.first + x / p.G;
     const long at = p.part_of(t, kvh * p.G + x % p.G, 2 * split);
     if (begin >= end || !p.sees(gr, t)) p.sums[at] = p.sums[at + 1] = make_float2(-INFINITY, 0.f);
+    if (split == 0)
+      for (int i = 2 * p.tile_splits; i < p.prefix_parts; ++i) p.sums[at + i] = make_float2(-INFINITY, 0.f);
   }
-  if (begin >= end) {
-    if (warp == 8) tmem_dealloc(tmem, 512);
-    return;
-  }
+  if (begin >= end) return;                      // (dependents may start then, as below)
+  if (warp == 8) tmem_alloc(&B->tmem, 512);      // S of the streams at 0 and 128, O at 256 and 384. Ahead of the launch of dependents, which might hold some and wait for this kernel
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = B->tmem;
+  grid_dep_launch();
   const int x0 = tile * 2 * TILE, pairs = gr.rows * p.G, nt = (end - begin + TILE - 1) / TILE;
   const bool two = pairs - x0 > TILE;            // two halves of pairs, or two streams of keys
   const int units = two ? 2 * nt : nt;           // products of scores: unit u is stream u & 1
