@@ -7,14 +7,14 @@
 // its rows and heads in the scratch.
 //
 //   tiles kernel     the prefix of a group with much work, on tcgen05 (shared_prefix_tiles.cu)
-//   parts kernel     the prefix of the others and the rows' own positions: one CTA per (tile of 16 WM pairs of a group's rows and heads, kv head, stretch of the prefix) and per (row, kv head, stretch of its own keys): products on the tensor cores as
-//                    m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
+//   parts kernel     the prefix of the others and the rows' own positions: one CTA per (tile of 16 WM pairs of a group's rows and heads, kv head, stretch of the prefix) and per (row, kv head, stretch
+//                    of its own keys): products on the tensor cores as m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
 //   merge kernel     four warps per (row, head): the parts, weighted by e^(m - largest m), over the sum
 //   own kernel       where rows fill the chip, in place of the two before it: one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result
 //
-// How long a prefix is is known on the device only, so both of the first two kernels start where a group might be either's, and one of them has nothing to do. us with the parts kernel and with the tiles
-// kernel, rows of 4 heads over each of 8 kv heads, behind 500 / 4000 / 30000 positions: 8 rows 11.7 / 16.3 / 60.8 and 23.5 / 29 / 50, 16 rows 15.6 / 23.1 / 90.5 and 25.0 / 33.2 / 56.4; over 4 kv heads
-// 16 rows 15.5 / 18.7 / 51.6 and 24.9 / 29.3 / 37.9.
+// How long a prefix is is known on the device only, so both of the first two kernels start where a group might be either's, and one of them has nothing to do. us with the parts kernel and with the
+// tiles kernel, rows of 4 heads over each of 8 kv heads, behind 500 / 4000 / 30000 positions: 8 rows 11.7 / 16.3 / 60.8 and 23.5 / 29 / 50, 16 rows 15.6 / 23.1 / 90.5 and 25.0 / 33.2 / 56.4; over 4 kv
+// heads 16 rows 15.5 / 18.7 / 51.6 and 24.9 / 29.3 / 37.9.
 #include <algorithm>
 
 #include "mma16816.cuh"

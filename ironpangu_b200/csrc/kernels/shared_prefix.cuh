@@ -65,7 +65,7 @@ struct PrefixParams {
     return work >= tiles_from;
   }
   // whether a row of a group sees its prefix as a whole
-  __device__ __forceinline__ bool sees(const PrefixGroup& g, int t) const { return g.rows && positions[t] >= 0 && positions[t] + 1 >= g.shared; }
+  __device__ __forceinline__ bool sees(const PrefixGroup& g, int t) const { return g.rows && positions[t] >= 0 && positions[t] >= g.shared - 1; }
   __device__ __forceinline__ PrefixOwn own(int t, const PrefixGroup& g) const {
     const int pos = positions[t], most = max_pages * page_tokens;
     if (pos < 0) return {0, 0, 0};

@@ -319,6 +319,150 @@ def test_beside_the_kernel_that_reads_the_prefix_for_every_row():
     assert float((other.float() - got.float()).abs().max()) <= 2 ** -7 * float(got.float().abs().max())
 
 
+def stale(b):
+    """A scratch that a call has to fill by itself: NaN wherever it reads what it did not write."""
+    return torch.full((S.scratch_bytes(b.q.shape[0], b.heads, b.kv, b.dim, b.groups.shape[0]),), 255, dtype=torch.uint8, device="cuda")
+
+
+# From 400 rows by kv heads on, prefixes are read by tiles of 256 pairs on tcgen05 and own positions by four warps each, from 1184 on by one warp; groups of 128 pairs at most have streams of keys
+@gpu
+@pytest.mark.parametrize("rows,heads,kv,dim,page", [(200, 8, 2, 128, 16), (201, 8, 2, 64, 8), (100, 4, 4, 64, 64), (407, 7, 1, 128, 128), (601, 8, 2, 128, 16), (1200, 16, 1, 64, 24), (301, 12, 4, 128, 256)])
+def test_many_rows(rows, heads, kv, dim, page):
+    for shared, own in ((1, 1), (0, 3), (127, 0), (128, 1), (129, 2), (500, 130), (1300, 17)):
+        b = Batch([(rows, shared, own)], heads=heads, kv=kv, dim=dim, page=page, seed=rows + shared)
+        b.check(rows=[0, 1, 31, 32, 64, rows // 2, rows - 1], scratch=stale(b))
+
+
+@gpu
+@pytest.mark.parametrize("kv,dim", [(2, 128), (8, 64)])
+def test_many_rows_in_groups(kv, dim):
+    rng = random.Random(kv)
+    own = lambda: rng.randint(1, 60)
+    b = Batch([(3, None, 77), (15, 300, own), (1, 2000, 5), (32, 129, own), (2, None, own), (33, 1030, own), (64, 700, own), (65, 128, own), (4, 0, own), (1, 16, 16)], heads=4 * kv, kv=kv, dim=dim, seed=5)
+    b.check(rows=[0, 2, 3, 10, 17, 18, 19, 50, 51, 52, 53, 85, 86, 100, 149, 150, 214, 215, 218, 219], scratch=stale(b))
+
+
+@gpu
+def test_many_rows_within_the_prefix_and_nobodys():
+    b = Batch([(220, 700, lambda: 5)], heads=8, kv=2, dim=128, seed=20)
+    b.positions[:7] = torch.tensor([0, 1, 127, 128, 698, 699, 700], dtype=I32)
+    b.positions[100:110] = -1
+    b.slots[105] = 1 << 30
+    b.k[b.table[0, 699 // 16].long(), 699 % 16] = float("nan")       # the prefix's last position
+    out = torch.full((220, 8 * 128), 7.0, dtype=BF16, device="cuda")
+    got = b.run(out=out, scratch=stale(b))
+    assert bool((got[100:110] == 7).all())
+    seen = b.positions >= 699
+    assert bool(got[seen].isnan().all()) and not bool(got[~seen].isnan().any())
+    b.check(rows=[0, 1, 2, 3, 4], got=got)
+
+
+@gpu
+@pytest.mark.parametrize("rows,page", [(220, 16), (25, 8)])
+def test_many_rows_and_pages_that_are_not_there(rows, page):
+    b = Batch([(rows, 900, lambda: 40), (220, 400, lambda: 3)], heads=8, kv=2, dim=128, page=page, seed=21)
+    at = 1 + rows
+    b.table[0, 2], b.table[0, 899 // page], b.table[1, 920 // page], b.table[at, :] = -1, 1 << 29, -7, -1
+    b.check(rows=[0, 1, 17, rows - 1, rows, rows + 219], status=BAD_INDEX, scratch=stale(b))
+
+
+@gpu
+@pytest.mark.parametrize("shared", [300, 400])
+def test_many_rows_and_what_none_sees(shared):
+    b = Batch([(30, shared, lambda: 9), (190, shared, lambda: 9), (2, None, 50)], heads=8, kv=2, dim=128, seed=22)
+    plain = b.run(scratch=stale(b))
+    b.table_list = b.table.tolist()
+    keep = torch.zeros(b.k.shape[:2], dtype=torch.bool, device="cuda")
+    for t in range(222):
+        pages, inside = (torch.tensor(x, device="cuda") for x in zip(*b.rows_of(t)))
+        keep[pages, inside] = True
+    for value in (float("nan"), float("inf"), -float("inf"), torch.finfo(BF16).min):
+        k, v = b.k.clone(), b.v.clone()
+        b.k[~keep], b.v[~keep] = value, value
+        assert torch.equal(b.run(), plain)
+        b.k, b.v = k, v
+    page = b.table[0, 2].long()                    # of the first group's prefix
+    b.v[page, 3, 0, 5], b.v[page, 4, 1, 6] = float("inf"), -float("inf")
+    got = b.run().view(222, 8, 128)
+    assert bool((got[:30, :4, 5] == float("inf")).all()) and bool((got[:30, 4:, 6] == -float("inf")).all()) and torch.equal(got[30:].reshape(192, -1), plain[30:])
+    assert not bool(got.isnan().any()) and int(b.status) == 0
+
+
+@gpu
+def test_many_rows_and_large_scores():
+    b = Batch([(210, 600, lambda: 40)], heads=8, kv=2, dim=128, seed=23)
+    b.q *= 30
+    b.scale = 1.0
+    got = b.run()
+    out, _ = b.want(rows=[0, 100, 209])
+    for t in out:                                  # as for few rows
+        assert float((got[t].to(F64) - out[t]).abs().max()) <= 2 ** -8 * 5 + float(out[t].abs().max()) * 2 ** -8
+    assert bool(got.isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (64, 8, 64)])
+def test_the_work_of_a_prefix_decides(heads, kv, dim):
+    """16 rows over a few thousand positions: below and from 3.5 million pairs by positions over the kv heads on, replayed from one graph."""
+    b = Batch([(16, 7168, lambda: 33)], heads=heads, kv=kv, dim=dim, page=64, seed=24)
+    edge = 3500000 // kv // (16 * heads // kv)
+    scratch = stale(b)
+    out = torch.empty_like(b.q)
+    b.run(out=out, scratch=scratch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.run(out=out, scratch=scratch)
+    for shared in (7168, 1, edge // 64 * 64, (edge // 64 + 1) * 64, 0, 6000, 7168):
+        b.groups[0, 2] = shared
+        b.positions.fill_(shared + 20)
+        out.fill_(9.0)
+        graph.replay()
+        b.check(rows=[0, 15], got=out)
+
+
+@gpu
+def test_a_long_prefix_of_two_groups_and_rows_within_it():
+    b = Batch([(18, 9001, lambda: 30), (3, 100, lambda: 10), (30, 5000, lambda: 300)], heads=32, kv=8, dim=128, page=16, seed=25)
+    b.positions[3:6] = torch.tensor([0, 5000, 8999], dtype=I32)
+    b.positions[19] = -1
+    b.check(rows=[0, 3, 4, 5, 17, 18, 20, 21, 50], scratch=stale(b))
+
+
+@gpu
+def test_many_rows_over_caches_beyond_32_bits():
+    pages, pt, kv, dim = (1 << 31) // (16 * 8 * 128) + 40, 16, 8, 128       # more than 2^31 elements
+    b = Batch([(60, 200, lambda: 4)], heads=16, kv=kv, dim=dim, seed=26)
+    small, n = (b.k, b.v), b.k.shape[0]
+    b.k, b.v = (torch.empty(pages, pt, kv, dim, dtype=BF16, device="cuda") for _ in range(2))
+    for big, s in zip((b.k, b.v), small):
+        big[pages - n:] = s
+    b.table = torch.where(b.table >= 0, b.table + (pages - n), b.table)
+    b.check(rows=[0, 30, 59], scratch=stale(b))
+
+
+@gpu
+def test_many_rows_captured_and_on_two_streams():
+    b, c = (Batch([(205, 600, lambda: 30)], heads=8, kv=2, dim=128, seed=s) for s in (27, 28))
+    want_b, want_c = b.run(), c.run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got_b = b.run()
+    with torch.cuda.stream(side):
+        got_c = c.run()
+    torch.cuda.synchronize()
+    assert torch.equal(got_b, want_b) and torch.equal(got_c, want_c)
+    out = torch.empty_like(want_b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.run(out=out)
+    graph.replay()
+    assert torch.equal(out, want_b)
+    b.groups[0, 2] = 112
+    b.positions -= 400
+    graph.replay()
+    b.check(rows=[0, 100, 204], got=out)
+
+
 def test_refused_on_the_host():
     q, c, i = torch.zeros(2, 512, dtype=BF16), torch.zeros(4, 16, 2, 64, dtype=BF16), torch.zeros(2, dtype=I32)
     with pytest.raises(ValueError, match="on the host"):
