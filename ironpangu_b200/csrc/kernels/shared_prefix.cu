@@ -10,7 +10,8 @@
 //   parts kernel     the prefix of the others and the rows' own positions: one CTA per (tile of 16 WM pairs of a group's rows and heads, kv head, stretch of the prefix) and per (row, kv head, stretch
 //                    of its own keys): products on the tensor cores as m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
 //   merge kernel     four warps per (row, head): the parts, weighted by e^(m - largest m), over the sum
-//   own kernel       where rows fill the chip, in place of the two before it: one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result
+//   own kernel       where rows fill the chip, in place of the two before it: one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result.
+//                    Four rows of a question read their keys together: eight questions of 128 rows behind 16384 positions 412 us instead of 432
 //
 // How long a prefix is is known on the device only, so both of the first two kernels start where a group might be either's, and one of them has nothing to do. us with the parts kernel and with the
 // tiles kernel, rows of 4 heads over each of 8 kv heads, behind 500 / 4000 / 30000 positions: 8 rows 11.7 / 16.3 / 60.8 and 23.5 / 29 / 50, 16 rows 15.6 / 23.1 / 90.5 and 25.0 / 33.2 / 56.4; over 4 kv
@@ -39,9 +40,10 @@ struct alignas(128) Unit {
 };
 
 // One stretch of keys [begin, end) of the pages of `slot` against 16 WM pairs. WM warps side by side have 16 pairs each, the others other keys of a tile.
-// `pair(i, &t, &h)`: pair i's row and head; false: nobody's. `finish(i, M, L, v)`, by a warp: maxima, sums and sums of values of the pairs from i on, AT_ONCE of them, HD / 32 columns a lane
-template <int HD, int W, int WM, int STAGES, int AT_ONCE, typename Pair, typename Finish>
-__device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * WM, STAGES>& u, int begin, int end, int slot, int kvh, int part, Pair pair, Finish finish) {
+// `pair(i, &t, &h)`: pair i's row and head; false: nobody's. `finish(i, M, L, v)`, by a warp: maxima, sums and sums of values of the pairs from i on, AT_ONCE of them, HD / 32 columns a lane.
+// `last(i)`, with EACH: where the keys of pair i end, `least` the first of these ends; keys behind it weigh nothing then. False: so that a value that is not finite must not count, nothing was finished
+template <int HD, int W, int WM, int STAGES, int AT_ONCE, bool EACH, typename Pair, typename Last, typename Finish>
+__device__ __forceinline__ bool attend(const PrefixParams& p, Unit<HD, W, 16 * WM, STAGES>& u, int begin, int end, int slot, int kvh, int part, int least, Pair pair, Last last, Finish finish) {
   using U = Unit<HD, W, 16 * WM, STAGES>;
   constexpr int WK = W / WM, KEYS = U::KEYS, KW = KEYS / WK, N = 32 * W, E = HD / 32;      // warps of other keys, keys of a warp, threads of the unit
   const int tid = threadIdx.x % N, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c2 = (lane & 3) * 2;
@@ -119,6 +121,10 @@ __device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * W
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
 
+  int ends[2];                                   // of pairs g and g + 8, from this thread's first key on
+#pragma unroll
+  for (int e = 0; e < 2; ++e) ends[e] = EACH ? last(wm * 16 + g + 8 * e) - begin - wk * KW - c2 : 0;
+
   for (int i = 0; i < tiles; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     sync();                                      // tile i has landed for all threads, tile i - 1 is read
@@ -140,14 +146,14 @@ __device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * W
         mma16816(s[2 * n], q[kk][0], q[kk][1], q[kk][2], q[kk][3], b[0], b[1]);
         mma16816(s[2 * n + 1], q[kk][0], q[kk][1], q[kk][2], q[kk][3], b[2], b[3]);
       }
-    const bool all = u.whole[i % (STAGES + 1)][0] && (KEYS <= 32 || u.whole[i % (STAGES + 1)][1]);
+    const bool all = u.whole[i % (STAGES + 1)][0] && (KEYS <= 32 || u.whole[i % (STAGES + 1)][1]) && (!EACH || begin + (i + 1) * KEYS <= least);
     float mn[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[n][e] *= p.scale_log2;
-        if (!all && u.rows[i % (STAGES + 1)][wk * KW + 8 * n + c2 + (e & 1)] < 0) s[n][e] = -INFINITY;
+        if (!all && (u.rows[i % (STAGES + 1)][wk * KW + 8 * n + c2 + (e & 1)] < 0 || (EACH && i * KEYS + 8 * n + (e & 1) >= ends[e >> 1]))) s[n][e] = -INFINITY;
         mn[e >> 1] = fmaxf(mn[e >> 1], s[n][e]);
       }
 #pragma unroll
@@ -172,14 +178,14 @@ __device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * W
     for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] = s[n][e] == -INFINITY ? PREFIX_LEAST_WEIGHT : prefix_weight(s[n][e] - m[e >> 1]);
+        s[n][e] = s[n][e] == -INFINITY ? (EACH ? 0.f : PREFIX_LEAST_WEIGHT) : prefix_weight(s[n][e] - m[e >> 1]);
         l[e >> 1] += s[n][e];
       }
 #pragma unroll
     for (int kk = 0; kk < KW / 16; ++kk) {
       uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) two_terms(s[2 * kk + (j >> 1)][2 * (j & 1)], s[2 * kk + (j >> 1)][2 * (j & 1) + 1], &hi[j], &lo[j]);
+      for (int j = 0; j < 4; ++j) two_terms<EACH>(s[2 * kk + (j >> 1)][2 * (j & 1)], s[2 * kk + (j >> 1)][2 * (j & 1) + 1], &hi[j], &lo[j]);
 #pragma unroll
       for (int j = 0; j < HD / 16; ++j) {
         uint32_t b[4];
@@ -201,7 +207,16 @@ __device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * W
   }
   // by pairs, over the ring: warps of the same pairs and other keys are added up
   asm volatile("cp.async.wait_group 0;" ::: "memory");
-  sync();
+  if (EACH) {
+    float finite = 0.f;
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) finite = fmaf(acc[j][e], 0.f, finite);
+    if (__syncthreads_or(finite != 0.f)) return false;
+  } else {
+    sync();
+  }
   float* all_acc = reinterpret_cast<float*>(u.ring);
   float* my_acc = all_acc + warp * 16 * HD;
   if ((lane & 3) == 0) {
@@ -215,7 +230,10 @@ __device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * W
   }
   sync();
   for (int i0 = warp * AT_ONCE; i0 < 16 * WM; i0 += W * AT_ONCE) {
-    if (AT_ONCE == 1 ? u.part[i0] < 0 : i0 >= p.G) continue;             // (several at once: pairs of one row, all that there are come first)
+    bool any = false;
+#pragma unroll
+    for (int n = 0; n < AT_ONCE; ++n) any = any || u.part[i0 + n] >= 0;
+    if (!any) continue;
     float M[AT_ONCE], L[AT_ONCE], v[AT_ONCE][E];
 #pragma unroll
     for (int n = 0; n < AT_ONCE; ++n) {
@@ -239,7 +257,11 @@ __device__ __forceinline__ void attend(const PrefixParams& p, Unit<HD, W, 16 * W
     }
     finish(i0, M, L, v);
   }
+  return true;
 }
+struct NoLast {
+  __device__ int operator()(int) const { return 0; }
+};
 
 template <int E>
 __device__ __forceinline__ void store_part(const PrefixParams& p, long at, float M, float L, const float (&v)[E], int lane) {
@@ -252,16 +274,16 @@ __device__ __forceinline__ float largest(const PrefixParams& p, long base, int n
   for (int i = lane; i < n; i += 32) M = fmaxf(M, p.sums[base + i].x);
   return warp_max(M);
 }
-// Adds parts [first, last) of P pairs, `base` + k `apart`, to the L and v of a warp, relative to M, which is not below their maxima: S parts of each pair are requested together. Parts that weigh
-// nothing count as nothing, whatever they hold
+// Adds parts [first, last) of P pairs, each of them from `base` on (negative: nobody's), to the L and v of a warp, relative to M, which is not below their maxima: S parts of each pair are requested
+// together. Parts that weigh nothing count as nothing, whatever they hold
 template <int E, int P, int S>
-__device__ __forceinline__ void add_parts(const PrefixParams& p, long base, long apart, int pairs, int first, int last, const float (&M)[P], float (&L)[P], float (&v)[P][E], int lane) {
+__device__ __forceinline__ void add_parts(const PrefixParams& p, const long (&base)[P], int first, int last, const float (&M)[P], float (&L)[P], float (&v)[P][E], int lane) {
   for (int i0 = first; i0 < last; i0 += 32) {
     float w[P];
     uint32_t left = 0;
 #pragma unroll
     for (int n = 0; n < P; ++n) {
-      const float2 ml = n < pairs && i0 + lane < last ? p.sums[base + n * apart + i0 + lane] : make_float2(-INFINITY, 0.f);
+      const float2 ml = base[n] >= 0 && i0 + lane < last ? p.sums[base[n] + i0 + lane] : make_float2(-INFINITY, 0.f);
       w[n] = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M[n]);
       const float l = w[n] != 0.f ? w[n] * ml.y : 0.f;
       L[n] += warp_sum(l);
@@ -277,7 +299,7 @@ __device__ __forceinline__ void add_parts(const PrefixParams& p, long base, long
         for (int n = 0; n < P; ++n) {
           by[n][k] = __shfl_sync(0xffffffffu, w[n], j);
           if (!left) by[n][k] = 0.f;
-          const float* src = p.parts + (base + (n < pairs ? n : 0) * apart + i0 + j) * (32 * E) + lane * E;
+          const float* src = p.parts + (max(base[n], 0l) + i0 + j) * (32 * E) + lane * E;
           if (E == 4) *reinterpret_cast<float4*>(a[n][k]) = *reinterpret_cast<const float4*>(src);
           else *reinterpret_cast<float2*>(a[n][k]) = *reinterpret_cast<const float2*>(src);
         }
@@ -332,8 +354,8 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
     }
     if (begin >= gr.shared) return;
     auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, 3>*>(smem);
-    attend<HD, 4, WM, 3, 1>(
-        p, u, begin, min(begin + per, gr.shared), gr.slot, kvh, split,
+    attend<HD, 4, WM, 3, 1, false>(
+        p, u, begin, min(begin + per, gr.shared), gr.slot, kvh, split, 0,
         [&](int i, int* t, int* h) {
           const int x = x0 + i;
           if (x >= gr.rows * p.G) return false;
@@ -341,6 +363,7 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
           *h = kvh * p.G + x % p.G;
           return p.sees(gr, *t);
         },
+        NoLast{},
         [&](int i, const float (&M)[1], const float (&L)[1], const float (&v)[1][E]) { store_part<E>(p, u.part[i], M[0], L[0], v[0], lane); });
   } else {
     item -= prefix_items;
@@ -356,13 +379,14 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
       return;
     }
     auto& u = *reinterpret_cast<Unit<HD, 4, 16, 3>*>(smem);
-    attend<HD, 4, 1, 3, 1>(
-        p, u, begin, min(begin + per, own.end), own.slot, kvh, p.prefix_parts + split,
+    attend<HD, 4, 1, 3, 1, false>(
+        p, u, begin, min(begin + per, own.end), own.slot, kvh, p.prefix_parts + split, 0,
         [&](int i, int* t, int* h) {
           *t = t0;
           *h = kvh * p.G + i;
           return i < p.G;
         },
+        NoLast{},
         [&](int i, const float (&M)[1], const float (&L)[1], const float (&v)[1][E]) { store_part<E>(p, u.part[i], M[0], L[0], v[0], lane); });
   }
 }
@@ -378,9 +402,10 @@ __global__ void __launch_bounds__(NT) prefix_merge_kernel(PrefixParams p, bf16* 
   const long base = p.part_of(t, h, 0);
   const int n = p.prefix_parts + p.own_splits, each = (n + W - 1) / W;
   const float M[1] = {largest(p, base, n, lane)};
+  const long bases[1] = {base};
   if (p.positions[t] < 0) return;
   float part[1][E] = {}, sum[1] = {0.f};
-  add_parts<E, 1, 8>(p, base, 0, 1, min(n, warp * each), min(n, (warp + 1) * each), M, sum, part, lane);
+  add_parts<E, 1, 8>(p, bases, min(n, warp * each), min(n, (warp + 1) * each), M, sum, part, lane);
   float L = sum[0];
   float(&v)[E] = part[0];
 #pragma unroll
@@ -397,46 +422,86 @@ __global__ void __launch_bounds__(NT) prefix_merge_kernel(PrefixParams p, bf16* 
   store_result<E>(out + (long)t * ldo + (long)h * HD, L, v, lane);
 }
 
-// W warps per (row, kv head): the row's own keys, what the prefix's kernel left, the result
-template <int HD, int W>
+// Results of P pairs over kv head `kvh` from pair j of the rows from t0 on: their own sums M, L and `mine`, and `parts` that the prefix's kernel left of each from bases[n] on (negative: nobody's)
+template <int E, int P, int S>
+__device__ __forceinline__ void finish_pairs(const PrefixParams& p, bf16* out, long ldo, long t0, int kvh, int j, const long* bases, int parts, const float (&M)[P], const float (&L)[P],
+                                             const float (&mine)[P][E], int lane) {
+  long base[P];
+  float top[P], sum[P], v[P][E];
+#pragma unroll
+  for (int n = 0; n < P; ++n) base[n] = bases[n];
+#pragma unroll
+  for (int n = 0; n < P; ++n) top[n] = base[n] >= 0 ? fmaxf(M[n], largest(p, base[n], parts, lane)) : 0.f;
+#pragma unroll
+  for (int n = 0; n < P; ++n) {
+    const float w = M[n] == -INFINITY ? 0.f : exp2f(M[n] - top[n]);
+    sum[n] = w != 0.f ? w * L[n] : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[n][e] = w != 0.f ? w * mine[n][e] : 0.f;
+  }
+  add_parts<E, P, S>(p, base, 0, parts, top, sum, v, lane);
+#pragma unroll
+  for (int n = 0; n < P; ++n)
+    if (base[n] >= 0) store_result<E>(out + (t0 + (j + n) / p.G) * ldo + (long)(kvh * p.G + (j + n) % p.G) * (32 * E), sum[n], v[n], lane);
+}
+
+// The row's own keys, what the prefix's kernel left, the result: four warps per (row, kv head), or (W = 1) a warp. With W = 1 a CTA has a kv head of four rows where these are of one sequence, as a
+// question's are: they read its keys together, as 16 WM pairs that each see their own positions. Else it has four kv heads of one row, or as near to that as their number allows: warps of one length
+template <int HD, int W, int WM>
 __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p, bf16* out, long ldo) {
   extern __shared__ __align__(16) unsigned char smem[];
-  constexpr int E = HD / 32, UNITS = NT / 32 / W, P = W == 1 ? 4 : 1, S = W == 1 ? 2 : 8;
+  constexpr int E = HD / 32, ROWS = 4 / W, P = W == 1 ? 4 : 1, S = W == 1 ? 2 : 8;
   grid_dep_launch();
   grid_dep_wait();
-  const int lane = threadIdx.x & 31, unit = threadIdx.x / (32 * W);
-  const long item = (long)blockIdx.x * UNITS + unit;
-  const int kvh = (int)(item % p.Hkv);
-  const long t0 = item / p.Hkv;
-  if (t0 >= p.T || p.positions[t0] < 0) return;
-  const PrefixGroup gr = p.naming((int)t0);
-  const PrefixOwn own = p.own((int)t0, gr);
-  const int per = p.per_split(gr.shared, max(1, p.tile_splits)), parts = p.sees(gr, (int)t0) ? (gr.shared + per - 1) / per * 2 : 0;
+  const int lane = threadIdx.x & 31, unit = threadIdx.x / (32 * W), c = blockIdx.x % p.Hkv;
+  const long t0 = (long)(blockIdx.x / p.Hkv) * ROWS;
+  int r = (c * ROWS + unit) / p.Hkv, kvh = (c * ROWS + unit) % p.Hkv;
+  PrefixOwn own{0, 0, -1};                       // of row r, with W = 1 of row lane % 4 to begin with
+  int parts = -1;                                // that the prefix's kernel left of it; -1: nobody's row
+  const long t = t0 + (W == 1 ? lane % ROWS : 0);
+  if (t < p.T && p.positions[t] >= 0) {
+    const PrefixGroup gr = p.naming((int)t);
+    const int per = p.per_split(gr.shared, p.tile_splits);
+    own = p.own((int)t, gr);
+    parts = p.sees(gr, (int)t) ? (gr.shared + per - 1) / per * 2 : 0;
+  }
+  if constexpr (W == 1) {
+    constexpr uint32_t ALL = 0xffffffffu;
+    const uint32_t live = __ballot_sync(ALL, parts >= 0);
+    if (!live) return;
+    const int leader = __ffs(live) - 1, begin = __shfl_sync(ALL, own.begin, leader), slot = __shfl_sync(ALL, own.slot, leader), left = __shfl_sync(ALL, parts, leader);
+    if (__all_sync(ALL, parts < 0 || (own.begin == begin && own.slot == slot && parts == left)) && (live & 15) > (live & -live)) {
+      auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, OWN_STAGES>*>(smem);
+      if (attend<HD, 4, WM, OWN_STAGES, P, true>(
+              p, u, begin, __reduce_max_sync(ALL, own.end), slot, c, 0, __reduce_min_sync(ALL, parts >= 0 ? own.end : 0x7fffffff),
+              [&](int i, int* t, int* h) {
+                *t = (int)t0 + i / p.G;
+                *h = c * p.G + i % p.G;
+                return i < ROWS * p.G && (live >> i / p.G & 1);
+              },
+              [&](int i) { return __shfl_sync(ALL, own.end, i / p.G % ROWS); },          // (of nobody's pairs: anything)
+              [&](int i, const float (&M)[P], const float (&L)[P], const float (&v)[P][E]) {
+                finish_pairs<E, P, S>(p, out, ldo, t0, c, i, u.part + i, left, M, L, v, lane);
+              }))
+        return;
+      r = unit;
+      kvh = c;
+    }
+    own = PrefixOwn{__shfl_sync(ALL, own.begin, r), __shfl_sync(ALL, own.end, r), __shfl_sync(ALL, own.slot, r)};
+    parts = __shfl_sync(ALL, parts, r);
+  }
+  if (parts < 0) return;
   auto& u = reinterpret_cast<Unit<HD, W, 16, OWN_STAGES>*>(smem)[unit];
-  attend<HD, W, 1, OWN_STAGES, P>(
-      p, u, own.begin, own.end, own.slot, kvh, 0,
+  attend<HD, W, 1, OWN_STAGES, P, false>(
+      p, u, own.begin, own.end, own.slot, kvh, 0, 0,
       [&](int i, int* t, int* h) {
-        *t = (int)t0;
+        *t = (int)t0 + r;
         *h = kvh * p.G + i;
         return i < p.G;
       },
+      NoLast{},
       [&](int i, const float (&M)[P], const float (&L)[P], const float (&mine)[P][E]) {
-        const int h = kvh * p.G + i, pairs = min(P, p.G - i);
-        const long base = p.part_of((int)t0, h, 0), apart = p.part_of(0, 1, 0);
-        float top[P], sum[P], v[P][E];
-#pragma unroll
-        for (int n = 0; n < P; ++n) top[n] = n < pairs ? fmaxf(M[n], largest(p, base + n * apart, parts, lane)) : 0.f;
-#pragma unroll
-        for (int n = 0; n < P; ++n) {
-          const float w = M[n] == -INFINITY ? 0.f : exp2f(M[n] - top[n]);
-          sum[n] = w != 0.f ? w * L[n] : 0.f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) v[n][e] = w != 0.f ? w * mine[n][e] : 0.f;
-        }
-        add_parts<E, P, S>(p, base, apart, pairs, 0, parts, top, sum, v, lane);
-#pragma unroll
-        for (int n = 0; n < P; ++n)
-          if (n < pairs) store_result<E>(out + t0 * ldo + (long)(h + n) * HD, sum[n], v[n], lane);
+        finish_pairs<E, P, S>(p, out, ldo, t0, kvh, r * p.G + i, u.part + i, parts, M, L, mine, lane);
       });
 }
 
@@ -470,6 +535,8 @@ Plan plan_of(int T, int Hkv, int G, int groups, bool tcgen05, long most) {
     a.tile_splits = splits((long)a.tile_tiles * Hkv, 148, 148);
   }
   a.own_splits = splits(items, a.tiles ? 296 : 148, 16);
+  // us of a call with four warps and with one, 32 heads over 8, behind 2000 positions: rows with up to 100 own ones, 160 of them 52.9 and 48.7, 256 of them 77.5 and 68.8; with up to 800, 99 and 130,
+  // 138 and 156; questions of 32 rows, five, 52.5 and 43.2, of 128 rows, two with up to 700, 116 and 77 (without blocks 108)
   a.own_warps = !a.tiles || !full ? 0 : items < 1184 ? 4 : 1;
   return a;
 }
@@ -483,12 +550,12 @@ int launch_parts(const PrefixParams& p, long prefix_items, cudaStream_t s) {
   if (items > 0x7fffffff) return -1;
   return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)smem, s, p, (int)prefix_items);
 }
-template <int HD, int W>
+template <int HD, int W, int WM>
 int launch_own(const PrefixParams& p, bf16* out, long ldo, cudaStream_t s) {
-  auto k = prefix_own_kernel<HD, W>;
-  constexpr int units = NT / 32 / W, smem = units * sizeof(Unit<HD, W, 16, OWN_STAGES>);
-  if (int rc = opt_in_smem_once<prefix_own_kernel<HD, W>>(smem)) return rc;
-  return launch_chain(k, dim3((unsigned)(((long)p.T * p.Hkv + units - 1) / units)), dim3(NT), (size_t)smem, s, p, out, ldo);
+  auto k = prefix_own_kernel<HD, W, WM>;
+  constexpr int rows = 4 / W, smem = std::max(rows * sizeof(Unit<HD, W, 16, OWN_STAGES>), sizeof(Unit<HD, 4, 16 * WM, OWN_STAGES>));
+  if (int rc = opt_in_smem_once<prefix_own_kernel<HD, W, WM>>(smem)) return rc;
+  return launch_chain(k, dim3((unsigned)((long)(p.T + rows - 1) / rows * p.Hkv)), dim3(NT), (size_t)smem, s, p, out, ldo);
 }
 template <int HD>
 int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream_t s) {
@@ -496,7 +563,8 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
   if (parts > 0x7fffffff || tiles > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
   if (a.tiles)
     if (int rc = launch_prefix_tiles(p, HD, tiles, s)) return rc;
-  if (a.own_warps) return a.own_warps == 4 ? launch_own<HD, 4>(p, out, ldo, s) : launch_own<HD, 1>(p, out, ldo, s);
+  if (a.own_warps == 4) return launch_own<HD, 4, 1>(p, out, ldo, s);
+  if (a.own_warps == 1) return p.G <= 4 ? launch_own<HD, 1, 1>(p, out, ldo, s) : p.G <= 8 ? launch_own<HD, 1, 2>(p, out, ldo, s) : launch_own<HD, 1, 4>(p, out, ldo, s);
   if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, parts, s) : a.wm == 2 ? launch_parts<HD, 2>(p, parts, s) : launch_parts<HD, 1>(p, parts, s)) return rc;
   return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)((long)p.T * p.Hq)), dim3(NT), 0, s, p, out, ldo);
 }

@@ -90,8 +90,10 @@ __device__ __forceinline__ float prefix_weight(float x) {       // 2^x; NaN stay
 }
 // what a part leaves beside its sums of values: a NaN counts wherever its maximum lies
 __device__ __forceinline__ float2 prefix_sums(float m, float l) { return make_float2(l != l ? INFINITY : m, l); }
+template <bool NONE>                             // whether there are weights of 0: both their terms are 0
 __device__ __forceinline__ void two_terms(float a, float b, uint32_t* hi, uint32_t* lo) {
-  const float a0 = __uint_as_float((__float_as_uint(a) - 1u) & 0xffff0000u), b0 = __uint_as_float((__float_as_uint(b) - 1u) & 0xffff0000u);
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  const float a0 = __uint_as_float((x - (NONE ? min(x, 1u) : 1u)) & 0xffff0000u), b0 = __uint_as_float((y - (NONE ? min(y, 1u) : 1u)) & 0xffff0000u);
   *hi = __byte_perm(__float_as_uint(a0), __float_as_uint(b0), 0x7632);
   *lo = __byte_perm(__float_as_uint(a - a0), __float_as_uint(b - b0), 0x7632);
 }

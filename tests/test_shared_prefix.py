@@ -463,6 +463,57 @@ def test_many_rows_captured_and_on_two_streams():
     b.check(rows=[0, 100, 204], got=out)
 
 
+@gpu
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 128), (16, 8, 64), (24, 8, 128), (32, 8, 128), (40, 8, 128), (64, 8, 64), (112, 8, 128), (128, 8, 128), (16, 4, 128), (21, 3, 64), (16, 1, 128)])
+def test_questions_of_many_rows(heads, kv, dim):
+    """Rows of one sequence that read their own keys together, four by four, wherever their question begins and ends."""
+    for each, count in ((4, -(-1184 // kv) // 4), (37, 1 + 1184 // kv // 37), (130, 1 + 1184 // kv // 130)):
+        b = Batch([(count, 70, each + 60), (2, None, each)], heads=heads, kv=kv, dim=dim, each=each, seed=each)
+        b.positions[1], b.positions[each + 2] = -1, -1
+        out = torch.full_like(b.q, 7.0)
+        got = b.run(out=out, scratch=stale(b))
+        assert bool((got[[1, each + 2]] == 7).all())
+        b.check(rows=[0, 2, 3, each - 1, each, each + 1, count * each // 2, count * each - 1, count * each, (count + 2) * each - 1], got=got)
+
+
+@gpu
+def test_questions_whose_later_rows_see_what_is_not_finite():
+    b = Batch([(10, 70, 40)], heads=32, kv=8, dim=128, each=16, seed=31)
+    plain = b.run()
+    lowest = torch.finfo(BF16).min
+    def cell(t, back):                             # where row t's key `back` positions before its own lies
+        pos = int(b.positions[t]) - back
+        return b.table[int(b.slots[t]), pos // 16].long(), pos % 16
+    for row, change in ((5, float("nan")), (22, float("inf")), (39, lowest), (54, -float("inf"))):
+        page, at = cell(row, 0)
+        b.v[page, at] = change
+    page, at = cell(70, 0)
+    b.k[page, at] = float("nan")
+    page, at = cell(86, 0)
+    b.k[page, at, 3] = lowest                      # scores of 1e38 times a sum of either sign
+    inplace = b.q.clone()
+    got = b.run(out=inplace, q=inplace)
+    assert torch.equal(got.view(torch.int16), b.run().view(torch.int16))
+    for t in range(160):
+        first = {0: 5, 1: 22, 2: 39, 3: 54, 4: 70, 5: 86}.get(t // 16, 1 << 30)
+        if t < first:
+            assert torch.equal(got[t], plain[t]) or bool(((got[t].to(F64) - plain[t].to(F64)).abs() <= 2 ** -7 * plain[t].to(F64).abs() + 2 ** -13 * 8).all())
+    b.check(rows=[0, 4, 16, 21, 32, 38, 48, 53, 64, 69, 80, 85, 100, 159], got=got)
+    assert bool(got[5:16].isnan().all()) and bool((got[22:32] == float("inf")).all()) and bool((got[54:64] == -float("inf")).all()) and bool(got[70:80].isnan().all())
+    assert bool(got[39:48].isfinite().all())
+
+
+@gpu
+def test_the_same_row_many_times():
+    b = Batch([(3, 100, 40), (1, None, 33)], heads=32, kv=8, dim=128, seed=32)
+    again = torch.arange(4, device="cuda").repeat_interleave(50)
+    b.q, b.positions, b.slots = b.q[again].contiguous(), b.positions[again].contiguous(), b.slots[again].contiguous()
+    b.groups[0, 1] = 150
+    got = b.check(rows=[0, 49, 50, 149, 150, 199])
+    for first in range(0, 200, 50):
+        assert float((got[first:first + 50].float() - got[first].float()).abs().max()) <= 2 ** -7 * float(got[first].float().abs().max())
+
+
 def test_refused_on_the_host():
     q, c, i = torch.zeros(2, 512, dtype=BF16), torch.zeros(4, 16, 2, 64, dtype=BF16), torch.zeros(2, dtype=I32)
     with pytest.raises(ValueError, match="on the host"):
