@@ -124,6 +124,34 @@ def test_masked_and_infinite_logits():
     check(with_low[:6], u[:6], top_p=[0.9] * 6)
 
 
+SHARES = [0.05, 0.3, 0.5, 0.8, 0.9, 0.99, 0.9999, 0.99999]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,spread,it", [(1 << 18, 0.5, 1.0), (1 << 18, 2.0, 0.05), (151936, 0.1, 1.0), (32000, 3.0, 0.01), (5000, 0.02, 1.0), (1 << 18, 2.0, 8.0), (40000, 1e-6, 1.0), (40000, 1e4, 1.0)])
+def test_shares_that_end_among_many_tokens(V, spread, it, dtype):
+    """Where the mass reaches the share, thousands of tokens lie close: more than one list takes, in f32 with values of their own."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = (torch.randn(8, V, generator=g, device="cuda") * spread).to(dtype)
+    u = torch.rand(8, generator=g, device="cuda").tolist()
+    check(x, u, it=[it] * 8, top_p=SHARES)
+    check(x, u, it=[it] * 8, top_p=SHARES[::-1], top_k=[V // 2, V // 3, 2000, 1500, 0, V - 1, V, 3])
+    check(x, u, it=[it] * 8, top_p=SHARES, min_p=[0.9, 0.5, 0.1, 0.01, 1e-4, 0.99, 0.2, 0.0])
+
+
+@gpu
+def test_shares_of_values_that_are_nearly_equal():
+    g = torch.Generator(device="cuda").manual_seed(9)
+    steps = torch.randint(0, 40, (8, 60000), generator=g, device="cuda").float()
+    x = 1 + steps * 2 ** -23                       # forty values side by side, 1500 tokens each
+    check(x, [0.1, 0.2, 0.3, 0.4, 0.5, 0.6, 0.7, 0.999], top_p=SHARES)
+    x[:, ::2] -= 30                                # half of them weigh nothing
+    check(x, [0.1, 0.2, 0.3, 0.4, 0.5, 0.6, 0.7, 0.999], top_p=SHARES)
+    x[:, 5] = 4.0
+    check(x, [0.1, 0.2, 0.3, 0.4, 0.5, 0.6, 0.7, 0.999], top_p=SHARES, top_k=[20000] * 8)
+
+
 @gpu
 def test_random_numbers_at_and_beyond_their_ends():
     x, _ = some(6, 5000, 11)
