@@ -15,7 +15,7 @@
 //
 // How long a prefix is is known on the device only, so both of the first two kernels start where a group might be either's, and one of them has nothing to do. us with the parts kernel and with the
 // tiles kernel, rows of 4 heads over each of 8 kv heads, behind 500 / 4000 / 30000 positions: 8 rows 11.7 / 16.3 / 60.8 and 23.5 / 29 / 50, 16 rows 15.6 / 23.1 / 90.5 and 25.0 / 33.2 / 56.4; over 4 kv
-// heads 16 rows 15.5 / 18.7 / 51.6 and 24.9 / 29.3 / 37.9.
+// heads 16 rows 15.5 / 18.7 / 51.6 and 24.9 / 29.3 / 37.9. Three groups of 27 rows behind up to 5000 / 9000 / 15000 positions 36 / 51 / 80 and 39 / 41 / 47.
 #include <algorithm>
 
 #include "mma16816.cuh"
@@ -515,21 +515,23 @@ struct Plan {
   int prefix_parts() const { return std::max(part_splits, 2 * tile_splits); }
 };
 // `most`: positions that a slot has room for
-Plan plan_of(int T, int Hkv, int G, int groups, bool tcgen05, long most) {
+Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long most) {
   Plan a{};
   auto splits = [](long items, long ctas, int most) { return (int)std::max(1l, std::min((long)most, ctas / std::max(1l, items))); };
   auto tiles = [&](int pairs) { return groups ? (int)std::max((long)groups, ((long)T * G - groups) / pairs + groups) : 0; };          // at most, however the rows are shared out
   const long items = (long)T * Hkv;
   const int rows = groups ? (T + groups - 1) / groups * G : 1;
   const bool full = items >= 400;
-  a.tiles_from = !tcgen05 ? 1l << 62 : full ? 0 : 3500000 / Hkv;        // by the figures above
-  a.tiles = groups && ((long)T * G + 16 * groups) * most >= a.tiles_from;
-  a.wm = !groups || (a.tiles && full) ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  a.wm = !groups || (tcgen05 && full) ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   // One wave: 148 CTAs of the prefix and as many of the rows' own positions side by side, two an SM; the tiles kernel's have an SM each
   if (a.wm) {
     a.part_tiles = tiles(16 * a.wm);
     a.part_splits = splits((long)a.part_tiles * Hkv, 148, 148);
   }
+  // The parts kernel takes as long as the longest prefix is, times the tiles that there may be, and is as fast as the tiles kernel at 3.1 to 5.5 million pairs by positions of 128 columns
+  const long pairs = 16l * a.wm * a.part_tiles * Hkv;
+  a.tiles_from = !tcgen05 ? 1l << 62 : full ? 0 : 3500000l * 128 / head_dim / std::max(1l, pairs);
+  a.tiles = groups && most >= a.tiles_from;
   if (a.tiles) {
     a.tile_tiles = tiles(256);
     a.tile_splits = splits((long)a.tile_tiles * Hkv, 148, 148);
@@ -575,7 +577,7 @@ extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_
   if (T < 1 || Hkv < 1 || Hq % Hkv || groups < 0) return 0;
   int most = 0;
   for (int with = 0; with < 2; ++with) {         // whatever the pages
-    const Plan a = plan_of(T, Hkv, Hq / Hkv, groups, with, 0x7fffffff);
+    const Plan a = plan_of(T, Hkv, Hq / Hkv, head_dim, groups, with, 0x7fffffff);
     most = std::max(most, a.prefix_parts() + a.own_splits);
   }
   return (uint64_t)T * Hq * most * (head_dim + 2) * sizeof(float);
@@ -588,7 +590,7 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   if (T < 1 || T > 1 << 20 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || (head_dim != 64 && head_dim != 128) || num_groups < 0 || num_groups > 64 || (num_groups && !groups)) return -1;
   if (num_slots < 1 || max_pages < 1 || page_tokens < 1 || num_pages < 1 || (long)num_pages * page_tokens > 0x7fffffff || (long)max_pages * page_tokens > 0x7fffffff - 256) return -1;
   if (ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)scratch | (uintptr_t)groups) % 16) return -1;
-  const Plan a = plan_of(T, Hkv, Hq / Hkv, num_groups, page_tokens % 8 == 0, (long)max_pages * page_tokens);
+  const Plan a = plan_of(T, Hkv, Hq / Hkv, head_dim, num_groups, page_tokens % 8 == 0, (long)max_pages * page_tokens);
   if (ifab_shared_prefix_scratch(T, Hq, Hkv, head_dim, num_groups) > scratch_bytes) return -5;
   PrefixParams p;
   p.q = (const bf16*)q; p.ldq = ldq; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache;

@@ -25,7 +25,7 @@ struct PrefixParams {
   // stretches that a group's prefix (by the parts kernel; by the tiles kernel, which leaves two parts of each) and a row's own positions are shared out to at most
   int part_splits, tile_splits, own_splits;
   int prefix_parts;                              // parts that a row and head has room for ahead of those of its own positions
-  long tiles_from;                               // pairs by positions of all prefixes from which on the tiles kernel has them
+  long tiles_from;                               // length of the longest prefix from which on the tiles kernel has all of them
   float* parts;                                  // [T, Hq, prefix_parts + own_splits, head_dim]: sums of values
   float2* sums;                                  // [T, Hq, prefix_parts + own_splits]: maximum (in powers of two), sum of weights
   uint32_t* status;
@@ -56,13 +56,9 @@ struct PrefixParams {
     return {0, 0, 0, 0};
   }
   __device__ __forceinline__ bool by_tiles() const {
-    long work = 0;
-    int end = 0;
-    for (int i = 0; i < groups; ++i) {
-      const PrefixGroup g = group(i, &end);
-      work += (long)((g.rows * G + 15) / 16 * 16) * g.shared;
-    }
-    return work >= tiles_from;
+    int longest = 0, end = 0;
+    for (int i = 0; i < groups; ++i) longest = max(longest, group(i, &end).shared);
+    return longest >= tiles_from;
   }
   // whether a row of a group sees its prefix as a whole
   __device__ __forceinline__ bool sees(const PrefixGroup& g, int t) const { return g.rows && positions[t] >= 0 && positions[t] >= g.shared - 1; }

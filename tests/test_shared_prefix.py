@@ -403,9 +403,9 @@ def test_many_rows_and_large_scores():
 @gpu
 @pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (64, 8, 64)])
 def test_the_work_of_a_prefix_decides(heads, kv, dim):
-    """16 rows over a few thousand positions: below and from 3.5 million pairs by positions over the kv heads on, replayed from one graph."""
+    """16 rows over a few thousand positions: below and from 3.5 million pairs by positions on (7 million of 64 columns), replayed from one graph."""
     b = Batch([(16, 7168, lambda: 33)], heads=heads, kv=kv, dim=dim, page=64, seed=24)
-    edge = 3500000 // kv // (16 * heads // kv)
+    edge = 3500000 * 128 // dim // kv // (16 * heads // kv)
     scratch = stale(b)
     out = torch.empty_like(b.q)
     b.run(out=out, scratch=scratch)
