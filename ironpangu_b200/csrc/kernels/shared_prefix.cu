@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p
   const long t = t0 + (W == 1 ? lane % ROWS : 0);
   if (t < p.T && p.positions[t] >= 0) {
     const PrefixGroup gr = p.naming((int)t);
-    const int per = p.per_split(gr.shared, p.tile_splits);
+    const int per = p.per_tile_split(gr.shared);
     own = p.own((int)t, gr);
     parts = p.sees(gr, (int)t) ? (gr.shared + per - 1) / per * 2 : 0;
   }
@@ -510,7 +510,7 @@ struct Plan {
   int wm;                                // tiles of 16 wm pairs by the parts kernel; 0: none of a prefix
   bool tiles;                            // by the tiles kernel
   int own_warps;                         // of the own kernel's units; 0: own parts by the parts kernel, and a merge
-  int part_tiles, part_splits, tile_tiles, tile_splits, own_splits;
+  int part_tiles, part_splits, tile_tiles, tile_splits, tile_share, tile_shares, own_splits;
   long tiles_from;
   int prefix_parts() const { return std::max(part_splits, 2 * tile_splits); }
 };
@@ -534,7 +534,26 @@ Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long
   a.tiles = groups && most >= a.tiles_from;
   if (a.tiles) {
     a.tile_tiles = tiles(256);
-    a.tile_splits = splits((long)a.tile_tiles * Hkv, 148, 148);
+    // Stretches for whole waves of 148 CTAs. SMs that a wave leaves over have short stretches, by up to four turns: 960 rows of 14 heads over 2 behind 16384 positions (56 items) 157 us, without 180; 1024
+    // of 16 over 16 (64 items, four turns) 229, without 241; by seven (128 items) 370 and 397, but also 428 and 412. 400 rows of 128 heads over 8 (200 items) in two stretches 396, in one 465. Groups have half a tile less than they may have each, on the average
+    const long items = (long)a.tile_tiles * Hkv, likely = std::max(1l, (long)(a.tile_tiles - groups / 2) * Hkv);
+    a.tile_share = a.tile_shares = a.tile_splits = 1;
+    if (items <= 148) {
+      const int n = (int)(148 / items), left = (int)(148 - n * items), turns = left ? (int)((items + left - 1) / left) : 0;
+      const bool more = turns && turns <= 4 && n * turns < 12;
+      a.tile_splits = n + more;
+      a.tile_share = more ? turns : 1;
+      a.tile_shares = more ? n * turns + 1 : n;
+    } else {
+      float best = 1e30f;
+      for (int n = 1; n <= 3; ++n) {
+        const float time = (float)((likely * n + 147) / 148) / n + 0.05f * n;
+        if (time < best) {
+          best = time;
+          a.tile_splits = a.tile_shares = n;
+        }
+      }
+    }
   }
   a.own_splits = splits(items, a.tiles ? 296 : 148, 16);
   // us of a call with four warps and with one, 32 heads over 8, behind 2000 positions: rows with up to 100 own ones, 160 of them 52.9 and 48.7, 256 of them 77.5 and 68.8; with up to 800, 99 and 130,
@@ -561,8 +580,8 @@ int launch_own(const PrefixParams& p, bf16* out, long ldo, cudaStream_t s) {
 }
 template <int HD>
 int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream_t s) {
-  const long parts = (long)a.part_tiles * p.Hkv * a.part_splits, tiles = (long)a.tile_tiles * p.Hkv * a.tile_splits;
-  if (parts > 0x7fffffff || tiles > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
+  const long parts = (long)a.part_tiles * p.Hkv * a.part_splits, tiles = (long)a.tile_tiles * p.Hkv;
+  if (parts > 0x7fffffff || tiles * a.tile_splits > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
   if (a.tiles)
     if (int rc = launch_prefix_tiles(p, HD, tiles, s)) return rc;
   if (a.own_warps == 4) return launch_own<HD, 4, 1>(p, out, ldo, s);
@@ -598,7 +617,7 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   p.num_slots = num_slots; p.max_pages = max_pages; p.page_tokens = page_tokens; p.num_pages = num_pages; p.groups = num_groups;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
-  p.part_splits = a.part_splits; p.tile_splits = a.tile_splits; p.own_splits = a.own_splits; p.prefix_parts = a.prefix_parts(); p.tiles_from = a.tiles_from;
+  p.part_splits = a.part_splits; p.tile_splits = a.tile_splits; p.tile_share = a.tile_share; p.tile_shares = std::max(1, a.tile_shares); p.own_splits = a.own_splits; p.prefix_parts = a.prefix_parts(); p.tiles_from = a.tiles_from;
   p.parts = (float*)scratch;
   p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.prefix_parts() + a.own_splits) * head_dim);
   p.status = status;

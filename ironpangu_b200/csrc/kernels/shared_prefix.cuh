@@ -24,6 +24,7 @@ struct PrefixParams {
   int T, Hq, Hkv, G;
   // stretches that a group's prefix (by the parts kernel; by the tiles kernel, which leaves two parts of each) and a row's own positions are shared out to at most
   int part_splits, tile_splits, own_splits;
+  int tile_share, tile_shares;                   // a stretch of the tiles kernel's but the last one is so large a share of the prefix, where last ones come by `tile_share` turns
   int prefix_parts;                              // parts that a row and head has room for ahead of those of its own positions
   long tiles_from;                               // length of the longest prefix from which on the tiles kernel has all of them
   float* parts;                                  // [T, Hq, prefix_parts + own_splits, head_dim]: sums of values
@@ -72,6 +73,8 @@ struct PrefixParams {
   }
   // keys of a stretch: whole tiles of the kernels'
   __device__ __forceinline__ int per_split(int n, int splits) const { return max(128, ((n + splits - 1) / splits + 127) / 128 * 128); }
+  // (a stretch's start and end take as long as 256 keys)
+  __device__ __forceinline__ int per_tile_split(int n) const { return max(128, (int)(((long)n * tile_share + (tile_share - 1) * 256 + tile_shares - 1) / tile_shares + 127) / 128 * 128); }
   __device__ __forceinline__ long part_of(int t, int h, int i) const { return ((long)t * Hq + h) * (prefix_parts + own_splits) + i; }
 };
 
@@ -94,7 +97,7 @@ __device__ __forceinline__ void two_terms(float a, float b, uint32_t* hi, uint32
   *lo = __byte_perm(__float_as_uint(a - a0), __float_as_uint(b - b0), 0x7632);
 }
 
-// shared_prefix_tiles.cu: `items` = tiles of 256 pairs, however the rows are shared out, by kv heads by stretches
+// shared_prefix_tiles.cu: `items` = tiles of 256 pairs, however the rows are shared out, by kv heads
 int launch_prefix_tiles(const PrefixParams& p, int head_dim, long items, cudaStream_t s);
 
 }  // namespace ifab

@@ -108,7 +108,7 @@ __device__ __forceinline__ float power_of_2(float x) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PrefixParams p, int box) {
+__global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PrefixParams p, int items, int box) {
   using L = Layout<HD>;
   constexpr int ST = L::STAGES;
   extern __shared__ unsigned char smem_raw[];
@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
   grid_dep_wait();
 
   // this CTA's work
-  const int split = blockIdx.x % p.tile_splits, kvh = blockIdx.x / p.tile_splits % p.Hkv;
-  int tile = blockIdx.x / p.tile_splits / p.Hkv, end_rows = 0;
+  const int item = blockIdx.x % items, split = blockIdx.x / items, kvh = item % p.Hkv;          // (the last stretch, which may be shorter, last)
+  int tile = item / p.Hkv, end_rows = 0;
   PrefixGroup gr{0, 0, 0, 0};
   for (int i = 0; i < p.groups; ++i) {
     gr = p.group(i, &end_rows);
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     gr = PrefixGroup{0, 0, 0, 0};
   }
   if (p.tiles_from && !p.by_tiles()) gr = PrefixGroup{0, 0, 0, 0};         // they are the parts kernel's
-  const int per = p.per_split(gr.shared, p.tile_splits), begin = split * per, end = min(begin + per, gr.shared);
+  const int per = p.per_tile_split(gr.shared), begin = split * per, end = min(begin + per, gr.shared);
   // parts of rows that do not see the prefix, or that the stretches leave over, are nothing: the merge kernel goes by their sums alone
   for (int x = tile * 2 * TILE + tid; x < min((tile + 1) * 2 * TILE, gr.rows * p.G); x += NT) {
     const int t = gr.first + x / p.G;
@@ -412,7 +412,7 @@ int launch(const PrefixParams& p, long items, cudaStream_t s) {
   CUtensorMap map_k, map_v;
   if (int rc = make_tmap_bf16_2d(&map_k, p.k_cache, rows, cols, cols, (uint32_t)box)) return rc;
   if (int rc = make_tmap_bf16_2d(&map_v, p.v_cache, rows, cols, cols, (uint32_t)box)) return rc;
-  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)Layout<HD>::SMEM, s, map_k, map_v, p, box);
+  return launch_chain(k, dim3((unsigned)(items * p.tile_splits)), dim3(NT), (size_t)Layout<HD>::SMEM, s, map_k, map_v, p, (int)items, box);
 }
 
 }  // namespace

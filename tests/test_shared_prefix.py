@@ -334,6 +334,16 @@ def test_many_rows(rows, heads, kv, dim, page):
 
 
 @gpu
+@pytest.mark.parametrize("rows,heads,kv,dim", [(208, 128, 8, 128), (400, 128, 8, 64), (1024, 8, 4, 64), (900, 14, 2, 128), (640, 64, 16, 64), (1030, 16, 16, 64), (2500, 32, 8, 64)])
+def test_stretches_that_fill_the_chip(rows, heads, kv, dim):
+    for groups in (1, 3):
+        each = rows // groups
+        for shared in (130, 1300, 6500):
+            b = Batch([(each, shared - 16 * i, 3) for i in range(groups)], heads=heads, kv=kv, dim=dim, page=16, seed=rows)
+            b.check(rows=[0, each // 2, each - 1, each * groups - 1], scratch=stale(b))
+
+
+@gpu
 @pytest.mark.parametrize("kv,dim", [(2, 128), (8, 64)])
 def test_many_rows_in_groups(kv, dim):
     rng = random.Random(kv)
