@@ -564,8 +564,10 @@ int ifab_draw(const void* logits, long ld, int f32, int T, int V, const float* i
 /* ---- attention of rows that share a prefix (shared_prefix.cu) ------------------------------------
  * q [T, >= Hq * head_dim], caches [num_pages, page_tokens, Hkv, head_dim] bf16, head_dim 64 or 128, Hq / Hkv up to 16; page_table [num_slots, max_pages]. groups [num_groups][4] (up to 64): first row,
  * rows, shared positions, slot through whose pages these rows see the positions below that; a row sees the others up to its own through slots[t]. Rows of negative positions are left as they are.
- * Everything on 16 bytes, ldq and ldo multiples of 8. Bytes of scratch: ifab_shared_prefix_scratch. */
+ * Everything on 16 bytes, ldq and ldo multiples of 8. Bytes of scratch: ifab_shared_prefix_scratch; the most that calls
+ * of up to T rows take: ifab_shared_prefix_scratch_up_to. */
 uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_dim, int groups);
+uint64_t ifab_shared_prefix_scratch_up_to(int T, int Hq, int Hkv, int head_dim, int groups);
 int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
                                  int num_slots, int max_pages, int page_tokens, int num_pages, const int32_t* groups, int num_groups, float scale, int T, int Hq, int Hkv,
                                  int head_dim, void* scratch, uint64_t scratch_bytes, void* out, long ldo, uint32_t* status, void* stream);

@@ -593,7 +593,7 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
 }  // namespace
 
 extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_dim, int groups) {
-  if (T < 1 || Hkv < 1 || Hq % Hkv || groups < 0) return 0;
+  if (T < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || groups < 0 || (head_dim != 64 && head_dim != 128)) return 0;
   int most = 0;
   for (int with = 0; with < 2; ++with) {         // whatever the pages
     const Plan a = plan_of(T, Hkv, Hq / Hkv, head_dim, groups, with, 0x7fffffff);
@@ -602,10 +602,16 @@ extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_
   return (uint64_t)T * Hq * most * (head_dim + 2) * sizeof(float);
 }
 
+extern "C" uint64_t ifab_shared_prefix_scratch_up_to(int T, int Hq, int Hkv, int head_dim, int groups) {
+  uint64_t most = 0;
+  for (int t = 1; t <= T; ++t) most = std::max(most, ifab_shared_prefix_scratch(t, Hq, Hkv, head_dim, groups));
+  return most;
+}
+
 extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
                                             int num_slots, int max_pages, int page_tokens, int num_pages, const int32_t* groups, int num_groups, float scale, int T, int Hq, int Hkv,
                                             int head_dim, void* scratch, uint64_t scratch_bytes, void* out, long ldo, uint32_t* status, void* stream) {
-  if (!(scale > 0.f) || scale > 3.4e38f) return -1;
+  if (!(scale > 0.f) || scale > 3.4e38f || !q || !k_cache || !v_cache || !positions || !slots || !page_table || !scratch || !out) return -1;
   if (T < 1 || T > 1 << 20 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || (head_dim != 64 && head_dim != 128) || num_groups < 0 || num_groups > 64 || (num_groups && !groups)) return -1;
   if (num_slots < 1 || max_pages < 1 || page_tokens < 1 || num_pages < 1 || (long)num_pages * page_tokens > 0x7fffffff || (long)max_pages * page_tokens > 0x7fffffff - 256) return -1;
   if (ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)scratch | (uintptr_t)groups) % 16) return -1;

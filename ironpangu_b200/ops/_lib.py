@@ -257,7 +257,7 @@ def load(build: bool = True, units=None):
                 continue
             fn.argtypes = sig
             fn.restype = c_int
-        for name, n in (("ifab_int4_bytes", 5), ("ifab_int4_gemm_scratch", 2), ("ifab_pages_work_words", 3), ("ifab_shared_prefix_scratch", 5)):
+        for name, n in (("ifab_int4_bytes", 5), ("ifab_int4_gemm_scratch", 2), ("ifab_pages_work_words", 3), ("ifab_shared_prefix_scratch", 5), ("ifab_shared_prefix_scratch_up_to", 5)):
             fn = getattr(lib, name, None)
             if fn is not None:
                 fn.argtypes, fn.restype = [c_int] * n, c_u64

@@ -21,8 +21,9 @@ def _need(ok: bool, what: str) -> None:
 
 def scratch_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, groups: int = 1) -> int:
     """Bytes that :func:`attention` takes as ``scratch`` for a call of so many rows (and for any of fewer in as many groups, the most of all of them)."""
-    _need(rows >= 0 and groups >= 0 and kv_heads >= 1 and heads % kv_heads == 0, f"{rows} rows of {heads} heads over {kv_heads} in {groups} groups")
-    return max((_scratch.__wrapped__(t, heads, kv_heads, head_dim, groups) for t in range(1, rows + 1)), default=0)
+    _need(0 <= rows <= MAX_ROWS and 0 <= groups <= MAX_GROUPS and kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0 and heads // kv_heads <= 16 and head_dim in (64, 128),
+          f"{rows} rows of {heads} heads over {kv_heads} of {head_dim} columns in {groups} groups are not supported")
+    return _lib.load().ifab_shared_prefix_scratch_up_to(rows, heads, kv_heads, head_dim, groups)
 
 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor, groups: torch.Tensor, *, heads: int,

@@ -532,6 +532,27 @@ def test_refused_on_the_host():
         S.attention(q.float(), c, c, i, i, i.view(1, 2), torch.zeros(1, 4, dtype=I32), heads=8, kv_heads=2, head_dim=64, scale=1.0)
 
 
+def test_scratch_refused_and_enough():
+    for bad in ((-1, 8, 2, 64), (1 << 21, 8, 2, 64), (4, 7, 2, 64), (4, 8, 0, 64), (4, 34, 2, 64), (4, 8, 2, 0), (4, 8, 2, 32), (4, 8, 2, 64, 65), (4, 8, 2, 64, -1), (4, 0, 2, 64)):
+        with pytest.raises(ValueError, match="not supported"):
+            S.scratch_bytes(*bad)
+    for heads, kv, dim, groups in ((8, 2, 128, 1), (16, 1, 64, 3), (32, 8, 64, 64), (128, 8, 128, 0)):
+        most = 0
+        for rows in range(1, 700):
+            most = max(most, S._scratch(rows, heads, kv, dim, groups))
+            if rows % 97 == 0:
+                assert S.scratch_bytes(rows, heads, kv, dim, groups) == most
+    assert S.scratch_bytes(0, 8, 2, 64) == 0 and S.scratch_bytes(1 << 20, 8, 2, 64) > 1 << 32
+
+
+@gpu
+def test_heads_of_no_columns_are_refused():
+    z = lambda *s: torch.zeros(s, dtype=BF16, device="cuda")
+    i = torch.zeros(2, dtype=I32, device="cuda")
+    with pytest.raises(ValueError, match="columns"):
+        S.attention(z(2, 8), z(4, 16, 2, 0), z(4, 16, 2, 0), i, i, i.view(1, 2), i[:0].view(0, 4), heads=8, kv_heads=2, head_dim=0, scale=1.0)
+
+
 @gpu
 def test_refused():
     b = Batch([(4, 20, 3)], heads=8, kv=2, dim=64, seed=1)
