@@ -8,6 +8,9 @@
 // which the mass passes a share), which is found without a sort: a histogram over the row, equal stretches of the values, says in which of 1024 bins the place lies; the bin's tokens - a
 // few - are gathered and put in order by counting. A bin with more tokens than the list takes (ties, values far apart) is split again by the bits of (value, id), 10 at a time.
 //
+// What bounds it: for one row dependent steps - loads, a handful of barriers of the cluster, searches by a warp - of 11 to 17 us; for many, instructions (64 rows of 151936 f32 without a cut 44 us, 256
+// rows of 128000 bf16 with a share of the mass 203 us, 57 % of the issue slots, 0.9 and 0.3 TB/s): 40 a token for a weight that is summed without an error, 12 for one that only says where to look.
+//
 // Weights are summed as integers of 2^-44: the sums decide between tokens, so they must not depend on an order of additions, and a weight below 2^-45 of the
 // largest is nothing. 2^18 weights of at most 1 stay below 2^62.
 #include <climits>
@@ -85,7 +88,7 @@ __device__ __forceinline__ Cut cut_at(u64 place) { return {value_of((uint32_t)(p
 // Weights e^((v - most) it) in units of 2^-44, rounded. With c = it log2 e as two floats,
 //   v c = n / 128 + r: n / 128 by an addition of 1.5 2^16, whose floats lie 1 / 128 apart, and r (at most 1 / 256) by a product that is rounded only then, so both without loss
 //   weight = 2^-((n_most - n) / 128) (1 + q), q = 2^(r - r_most) - 1 by Taylor's series: of at most 0.0055, it is off by 2^-31 as a float
-// The first factor is a table's (62 bits) and a shift, so weights are off by 2^-31 of themselves, unsystematically, and the largest value's is 1 exactly. What a row costs is instructions, and that is
+// The first factor is a table's (62 bits) and a shift, so weights are off by 2^-31 of themselves and a little, 2^-30 at most, unsystematically, and the largest value's is 1 exactly. What a row costs is instructions, and that is
 // half of them in 64-bit arithmetic. Factors that floats hold badly, and values whose v c the addition does not take, go the 64-bit way.
 struct Weights {
   float most, floor;           // below `floor` a weight is less than 2^-45
@@ -500,7 +503,7 @@ struct Search {
   // The mass' share in two passes, where the bins' masses, to 2^-15 of all, say well enough between which tokens the place lies; leaves the kept masses of the warps' stretches. In a bin, a weight is
   // that of the bin's middle times 1 - x + x^2 / 2, which is summed in 17 bits and off by x^3 / 6 < 2^-21: 12 instructions and one addition in shared memory a token, where weights of 2^-44 take 40 and
   // two. The last pass takes those, of all tokens, and has the list. (What is less than e^-24 counts as that in the last bin: 2^-16 of the largest weight, if all tokens lie there.) Where the bin has
-  // more tokens than the list takes, one more pass, which counts only, has it in 1024 stretches. 256 rows of 128000 bf16 291 to 225 us, 27 of 151936 with cuts of their own 49 to 39 us.
+  // more tokens than the list takes, one more pass, which counts only, has it in 1024 stretches. 256 rows of 128000 bf16 291 to 212 us, 27 of 151936 with cuts of their own 49 to 40 us.
   // False: the place is among the smallest weights, or too many tokens are nearly equal
   __device__ bool quick(cg::cluster_group& cluster, float share, int first, int last, int each) {
     constexpr float WIDTH = 24.f / (BINS - 1);
@@ -527,7 +530,9 @@ struct Search {
     split = false;
     u64 members = 0;
     for (int b = b0; b <= b1; ++b) members += s->total[b] >> 16;
-    if (members > LIST * 15 / 16) {
+    // A pass more or a longer list, which every CTA of a cluster writes to every other's: 27 rows of 151936 over eight CTAs each 51.9 us with lists of up to 960, 42.5 of 384, 41.0 of 128; 256 rows of
+    // 128000, a CTA each, 210, 214 and 220
+    if (members > (ranks > 1 ? 256 : LIST * 15 / 16)) {
       const float finer = (float)BINS / (b1 - b0 + 1), start = -(b0 - 0.5f) * finer - 0.5f, scale2 = scale * finer, width = WIDTH / finer;
       const u64 ahead = s->above;
       auto place = [&](float v) { return fminf(fmaxf(__fmaf_rn(top - v, scale2, start), 0.f), BINS - 1) + MAGIC; };

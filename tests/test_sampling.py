@@ -39,7 +39,7 @@ def plain(logits, u, it=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
 def check(logits, u, it=None, top_k=None, top_p=None, min_p=None):
     """`logits` on the device; the others lists or None. Probabilities: rounded once to f32 (2^-24 relative), of sums that are off by 2^-45 a token (V 2^-45 of at least 1)
-    and 2^-31 of each weight, so of themselves."""
+    and 2^-30 of each weight, so of themselves."""
     T, V = logits.shape
     dev = lambda v, dt: None if v is None else torch.tensor(v, dtype=dt, device="cuda")
     args = dict(inv_temperature=dev(it, F32), top_k=dev(top_k, I32), top_p=dev(top_p, F32), min_p=dev(min_p, F32))
@@ -49,7 +49,7 @@ def check(logits, u, it=None, top_k=None, top_p=None, min_p=None):
     for t in range(T):
         want, p = plain(x[t], f(u, t, 0), f(it, t, 1.0), 0 if top_k is None else top_k[t], f(top_p, t, 1.0), f(min_p, t, 0.0))
         assert ids[t] == want, f"row {t}: {ids[t]}, {want} wanted"
-        assert abs(probs[t] - p) <= p * (2 ** -24 + V * 2 ** -45 + 2 ** -31), f"row {t}: probability {probs[t]}, {p} wanted"
+        assert abs(probs[t] - p) <= p * (2 ** -24 + V * 2 ** -45 + 2 ** -30), f"row {t}: probability {probs[t]}, {p} wanted"
     return ids
 
 
