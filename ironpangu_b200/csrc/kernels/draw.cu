@@ -88,8 +88,8 @@ __device__ __forceinline__ Cut cut_at(u64 place) { return {value_of((uint32_t)(p
 // Weights e^((v - most) it) in units of 2^-44, rounded. With c = it log2 e as two floats,
 //   v c = n / 128 + r: n / 128 by an addition of 1.5 2^16, whose floats lie 1 / 128 apart, and r (at most 1 / 256) by a product that is rounded only then, so both without loss
 //   weight = 2^-((n_most - n) / 128) (1 + q), q = 2^(r - r_most) - 1 by Taylor's series: of at most 0.0055, it is off by 2^-31 as a float
-// The first factor is a table's (62 bits) and a shift, so weights are off by 2^-31 of themselves and a little, 2^-30 at most, unsystematically, and the largest value's is 1 exactly. What a row costs is instructions, and that is
-// half of them in 64-bit arithmetic. Factors that floats hold badly, and values whose v c the addition does not take, go the 64-bit way.
+// The first factor is a table's (62 bits) and a shift, so weights are off by 2^-31 of themselves and a little, 2^-30 at most, unsystematically, and the largest value's is 1 exactly. What a row costs is
+// instructions, and that is half of them in 64-bit arithmetic. Factors that floats hold badly, and values whose v c the addition does not take, go the 64-bit way.
 struct Weights {
   float most, floor;           // below `floor` a weight is less than 2^-45
   double it, z_most;

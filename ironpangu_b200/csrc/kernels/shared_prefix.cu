@@ -534,8 +534,9 @@ Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long
   a.tiles = groups && most >= a.tiles_from;
   if (a.tiles) {
     a.tile_tiles = tiles(256);
-    // Stretches for whole waves of 148 CTAs. SMs that a wave leaves over have short stretches, by up to four turns: 960 rows of 14 heads over 2 behind 16384 positions (56 items) 157 us, without 180; 1024
-    // of 16 over 16 (64 items, four turns) 229, without 241; by seven (128 items) 370 and 397, but also 428 and 412. 400 rows of 128 heads over 8 (200 items) in two stretches 396, in one 465. Groups have half a tile less than they may have each, on the average
+    // Stretches for whole waves of 148 CTAs. SMs that a wave leaves over have short stretches, by up to four turns: 960 rows of 14 heads over 2 behind 16384 positions (56 items) 157 us, without 180;
+    // 1024 rows of 16 over 16 (64 items, four turns) 229, without 241; by seven turns (128 items) 370 and 397, but also 428 and 412. 400 rows of 128 heads over 8 (200 items) in two stretches 396, in
+    // one 465. Groups have half a tile less than they may have each, on the average
     const long items = (long)a.tile_tiles * Hkv, likely = std::max(1l, (long)(a.tile_tiles - groups / 2) * Hkv);
     a.tile_share = a.tile_shares = a.tile_splits = 1;
     if (items <= 148) {
@@ -623,7 +624,8 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   p.num_slots = num_slots; p.max_pages = max_pages; p.page_tokens = page_tokens; p.num_pages = num_pages; p.groups = num_groups;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
-  p.part_splits = a.part_splits; p.tile_splits = a.tile_splits; p.tile_share = a.tile_share; p.tile_shares = std::max(1, a.tile_shares); p.own_splits = a.own_splits; p.prefix_parts = a.prefix_parts(); p.tiles_from = a.tiles_from;
+  p.part_splits = a.part_splits; p.tile_splits = a.tile_splits; p.own_splits = a.own_splits; p.prefix_parts = a.prefix_parts(); p.tiles_from = a.tiles_from;
+  p.tile_share = a.tile_share; p.tile_shares = std::max(1, a.tile_shares);
   p.parts = (float*)scratch;
   p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.prefix_parts() + a.own_splits) * head_dim);
   p.status = status;

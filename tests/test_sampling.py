@@ -125,6 +125,13 @@ def test_masked_and_infinite_logits():
     check(with_low[:6], u[:6], top_p=[0.9] * 6)
 
 
+@gpu
+@pytest.mark.parametrize("T,V", [(3000, 61), (700, 1500), (297, 4096)])
+def test_a_great_many_rows(T, V):
+    x, u = some(T, V, T)
+    check(x, u, it=[0.4 + 0.2 * (t % 7) for t in range(T)], top_k=[t % 50 for t in range(T)], top_p=[0.3 + 0.1 * (t % 9) for t in range(T)], min_p=[0.02 * (t % 3) for t in range(T)])
+
+
 SHARES = [0.05, 0.3, 0.5, 0.8, 0.9, 0.99, 0.9999, 0.99999]
 
 

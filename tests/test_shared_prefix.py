@@ -524,6 +524,41 @@ def test_the_same_row_many_times():
         assert float((got[first:first + 50].float() - got[first].float()).abs().max()) <= 2 ** -7 * float(got[first].float().abs().max())
 
 
+@gpu
+def test_a_great_many_rows():
+    b = Batch([(500, 300, 75), (500, 333, 71)], heads=4, kv=1, dim=64, each=70, seed=41)
+    b.check(rows=[0, 69, 70, 34999, 35000, 35001, 50000, 69999], scratch=stale(b))
+
+
+@gpu
+@pytest.mark.parametrize("page", [1, 5, 12, 1000])
+def test_many_rows_over_pages_of_any_size(page):
+    rng = random.Random(page)
+    b = Batch([(3, None, 40), (200, 450, lambda: rng.randint(1, 80)), (20, 131, 5)], heads=8, kv=2, dim=128, page=page, seed=42)
+    b.check(rows=[0, 2, 3, 100, 202, 203, 222], scratch=stale(b))
+
+
+@gpu
+@pytest.mark.parametrize("most", [7, 40])
+def test_as_many_groups_as_there_may_be(most):
+    rng = random.Random(most)
+    own = lambda: rng.randint(1, 30)
+    b = Batch([(1 + i % most, 17 * i, own) for i in range(64)], heads=8, kv=2, dim=64, seed=43)
+    T = b.q.shape[0]
+    b.check(rows=[0, 1, 2, T // 3, T // 2, T - 2, T - 1], scratch=stale(b))
+
+
+@gpu
+def test_many_rows_in_the_queries_place():
+    b = Batch([(220, 300, lambda: 11)], heads=8, kv=2, dim=64, seed=44)
+    plain = b.run()
+    wide = torch.full((220, 1000), 9.0, dtype=BF16, device="cuda")
+    wide[:, 8:520] = b.q
+    b.run(q=wide[:, 8:], out=wide[:, 8:520])
+    assert torch.equal(wide[:, 8:520], plain) and bool((wide[:, :8] == 9).all()) and bool((wide[:, 520:] == 9).all())
+    b.check(rows=[0, 219], got=plain)
+
+
 def test_refused_on_the_host():
     q, c, i = torch.zeros(2, 512, dtype=BF16), torch.zeros(4, 16, 2, 64, dtype=BF16), torch.zeros(2, dtype=I32)
     with pytest.raises(ValueError, match="on the host"):
