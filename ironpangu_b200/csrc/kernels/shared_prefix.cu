@@ -11,7 +11,9 @@
 //                    of its own keys): products on the tensor cores as m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
 //   merge kernel     four warps per (row, head): the parts, weighted by e^(m - largest m), over the sum
 //   own kernel       where rows fill the chip, in place of the two before it: one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result.
-//                    Four rows of a question read their keys together: eight questions of 128 rows behind 16384 positions 412 us instead of 432
+//                    Four rows of a question read their keys together: eight questions of 128 rows behind 16384 positions 412 us, without that 432
+//
+// Behind the tiles kernel the two others start where an SM is free, ahead of its end: 64 rows behind 30011 positions 92.5 to 87.2 us, 27 in three groups 41.2 to 38.9, the 1024 412 to 408.
 //
 // How long a prefix is is known on the device only, so both of the first two kernels start where a group might be either's, and one of them has nothing to do. us with the parts kernel and with the
 // tiles kernel, rows of 4 heads over each of 8 kv heads, behind 500 / 4000 / 30000 positions: 8 rows 11.7 / 16.3 / 60.8 and 23.5 / 29 / 50, 16 rows 15.6 / 23.1 / 90.5 and 25.0 / 33.2 / 56.4; over 4 kv
@@ -321,17 +323,13 @@ __device__ __forceinline__ void store_result(bf16* dst, float L, const float (&v
   for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(dst + lane * E + e) = __floats2bfloat162_rn(v[e] * inv, v[e + 1] * inv);
 }
 
-// Grid: prefix items (stretch fastest, then kv head, then tile), then own items (stretch, kv head, row). Every part of a row that is somebody's gets its sums, if only to say that it is nothing,
+// Items: those of prefixes (stretch fastest, then kv head, then tile), then own ones (stretch, kv head, row). Every part of a row that is somebody's gets its sums, if only to say that it is nothing,
 // so that the merge need not know about groups
 template <int HD, int WM>
-__global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int prefix_items) {
-  extern __shared__ __align__(16) unsigned char smem[];
+__device__ __forceinline__ void part_item(const PrefixParams& p, int item, int prefix_items, unsigned char* smem) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31;
   const float2 nothing = make_float2(-INFINITY, 0.f);
-  grid_dep_launch();
-  grid_dep_wait();
-  int item = blockIdx.x;
   if (item < prefix_items) {
     const int split = item % p.part_splits, kvh = item / p.part_splits % p.Hkv;
     int tile = item / p.part_splits / p.Hkv, end = 0;
@@ -391,6 +389,17 @@ __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int
   }
 }
 
+template <int HD, int WM>
+__global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int prefix_items, bool behind_tiles) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  grid_dep_launch();
+  // The tiles kernel lets this one start when all its CTAs are past their own wait, so what kernels before it wrote is there, and their parts are of other places; the wait comes last then, so that
+  // the end of this kernel says that the other one has ended
+  if (!behind_tiles) grid_dep_wait();
+  part_item<HD, WM>(p, blockIdx.x, prefix_items, smem);
+  if (behind_tiles) grid_dep_wait();
+}
+
 // four warps per (row, head), a stretch of its parts each
 template <int HD>
 __global__ void __launch_bounds__(NT) prefix_merge_kernel(PrefixParams p, bf16* out, long ldo) {
@@ -428,6 +437,7 @@ __device__ __forceinline__ void finish_pairs(const PrefixParams& p, bf16* out, l
                                              const float (&mine)[P][E], int lane) {
   long base[P];
   float top[P], sum[P], v[P][E];
+  grid_dep_wait();
 #pragma unroll
   for (int n = 0; n < P; ++n) base[n] = bases[n];
 #pragma unroll
@@ -451,8 +461,8 @@ template <int HD, int W, int WM>
 __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p, bf16* out, long ldo) {
   extern __shared__ __align__(16) unsigned char smem[];
   constexpr int E = HD / 32, ROWS = 4 / W, P = W == 1 ? 4 : 1, S = W == 1 ? 2 : 8;
+  // The tiles kernel, which is ahead, lets this one start when all its CTAs are past their own wait, so what kernels before it wrote is there; its parts are read, and results written, behind the wait
   grid_dep_launch();
-  grid_dep_wait();
   const int lane = threadIdx.x & 31, unit = threadIdx.x / (32 * W), c = blockIdx.x % p.Hkv;
   const long t0 = (long)(blockIdx.x / p.Hkv) * ROWS;
   int r = (c * ROWS + unit) / p.Hkv, kvh = (c * ROWS + unit) % p.Hkv;
@@ -468,7 +478,10 @@ __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p
   if constexpr (W == 1) {
     constexpr uint32_t ALL = 0xffffffffu;
     const uint32_t live = __ballot_sync(ALL, parts >= 0);
-    if (!live) return;
+    if (!live) {
+      grid_dep_wait();                           // (as every path does: that this kernel has ended says that the one ahead has)
+      return;
+    }
     const int leader = __ffs(live) - 1, begin = __shfl_sync(ALL, own.begin, leader), slot = __shfl_sync(ALL, own.slot, leader), left = __shfl_sync(ALL, parts, leader);
     if (__all_sync(ALL, parts < 0 || (own.begin == begin && own.slot == slot && parts == left)) && (live & 15) > (live & -live)) {
       auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, OWN_STAGES>*>(smem);
@@ -490,7 +503,10 @@ __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p
     own = PrefixOwn{__shfl_sync(ALL, own.begin, r), __shfl_sync(ALL, own.end, r), __shfl_sync(ALL, own.slot, r)};
     parts = __shfl_sync(ALL, parts, r);
   }
-  if (parts < 0) return;
+  if (parts < 0) {
+    grid_dep_wait();
+    return;
+  }
   auto& u = reinterpret_cast<Unit<HD, W, 16, OWN_STAGES>*>(smem)[unit];
   attend<HD, W, 1, OWN_STAGES, P, false>(
       p, u, own.begin, own.end, own.slot, kvh, 0, 0,
@@ -564,13 +580,13 @@ Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long
 }
 
 template <int HD, int WM>
-int launch_parts(const PrefixParams& p, long prefix_items, cudaStream_t s) {
+int launch_parts(const PrefixParams& p, long prefix_items, bool behind_tiles, cudaStream_t s) {
   auto k = prefix_parts_kernel<HD, WM>;
   constexpr int smem = std::max(sizeof(Unit<HD, 4, 16 * WM, 3>), sizeof(Unit<HD, 4, 16, 3>));
   if (int rc = opt_in_smem_once<prefix_parts_kernel<HD, WM>>(smem)) return rc;
   const long items = prefix_items + (long)p.T * p.Hkv * p.own_splits;
   if (items > 0x7fffffff) return -1;
-  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)smem, s, p, (int)prefix_items);
+  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)smem, s, p, (int)prefix_items, behind_tiles);
 }
 template <int HD, int W, int WM>
 int launch_own(const PrefixParams& p, bf16* out, long ldo, cudaStream_t s) {
@@ -587,7 +603,7 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
     if (int rc = launch_prefix_tiles(p, HD, tiles, s)) return rc;
   if (a.own_warps == 4) return launch_own<HD, 4, 1>(p, out, ldo, s);
   if (a.own_warps == 1) return p.G <= 4 ? launch_own<HD, 1, 1>(p, out, ldo, s) : p.G <= 8 ? launch_own<HD, 1, 2>(p, out, ldo, s) : launch_own<HD, 1, 4>(p, out, ldo, s);
-  if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, parts, s) : a.wm == 2 ? launch_parts<HD, 2>(p, parts, s) : launch_parts<HD, 1>(p, parts, s)) return rc;
+  if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, parts, a.tiles, s) : a.wm == 2 ? launch_parts<HD, 2>(p, parts, a.tiles, s) : launch_parts<HD, 1>(p, parts, a.tiles, s)) return rc;
   return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)((long)p.T * p.Hq)), dim3(NT), 0, s, p, out, ldo);
 }
 
