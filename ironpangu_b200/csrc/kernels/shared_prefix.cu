@@ -44,7 +44,9 @@ struct alignas(128) Unit {
 // One stretch of keys [begin, end) of the pages of `slot` against 16 WM pairs. WM warps side by side have 16 pairs each, the others other keys of a tile.
 // `pair(i, &t, &h)`: pair i's row and head; false: nobody's. `finish(i, M, L, v)`, by a warp: maxima, sums and sums of values of the pairs from i on, AT_ONCE of them, HD / 32 columns a lane.
 // `last(i)`, with EACH: where the keys of pair i end, `least` the first of these ends; keys behind it weigh nothing then. False: so that a value that is not finite must not count, nothing was finished
-template <int HD, int W, int WM, int STAGES, int AT_ONCE, bool EACH, typename Pair, typename Last, typename Finish>
+// The tensor core cuts off what does not fit a sum, 1.1e-8 of it a key (shared_prefix_tiles.cu). FAR: so a tile's sums of values start from 0 and are then added, rounded to nearest, to those of the tiles
+// before
+template <int HD, int W, int WM, int STAGES, int AT_ONCE, bool EACH, bool FAR, typename Pair, typename Last, typename Finish>
 __device__ __forceinline__ bool attend(const PrefixParams& p, Unit<HD, W, 16 * WM, STAGES>& u, int begin, int end, int slot, int kvh, int part, int least, Pair pair, Last last, Finish finish) {
   using U = Unit<HD, W, 16 * WM, STAGES>;
   constexpr int WK = W / WM, KEYS = U::KEYS, KW = KEYS / WK, N = 32 * W, E = HD / 32;      // warps of other keys, keys of a warp, threads of the unit
@@ -183,20 +185,41 @@ __device__ __forceinline__ bool attend(const PrefixParams& p, Unit<HD, W, 16 * W
         s[n][e] = s[n][e] == -INFINITY ? (EACH ? 0.f : PREFIX_LEAST_WEIGHT) : prefix_weight(s[n][e] - m[e >> 1]);
         l[e >> 1] += s[n][e];
       }
-#pragma unroll
-    for (int kk = 0; kk < KW / 16; ++kk) {
-      uint32_t hi[4], lo[4];
+    auto terms = [&](int kk, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) two_terms<EACH>(s[2 * kk + (j >> 1)][2 * (j & 1)], s[2 * kk + (j >> 1)][2 * (j & 1) + 1], &hi[j], &lo[j]);
+    };
+    auto products = [&](int kk, int j, const uint32_t (&hi)[4], const uint32_t (&lo)[4], float (&even)[4], float (&odd)[4]) {
+      uint32_t b[4];
+      const int key = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * j + (lane >> 4);
+      ldsm4t(vb + key * U::ROW + ((ch ^ (key & 7)) << 4), b);
+      mma16816(even, hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
+      mma16816(odd, hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
+      mma16816(even, lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
+      mma16816(odd, lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
+    };
+    if constexpr (!FAR) {
+#pragma unroll
+      for (int kk = 0; kk < KW / 16; ++kk) {
+        uint32_t hi[4], lo[4];
+        terms(kk, hi, lo);
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) products(kk, j, hi, lo, acc[2 * j], acc[2 * j + 1]);
+      }
+    } else {
+      uint32_t hi[KW / 16][4], lo[KW / 16][4];
+#pragma unroll
+      for (int kk = 0; kk < KW / 16; ++kk) terms(kk, hi[kk], lo[kk]);
 #pragma unroll
       for (int j = 0; j < HD / 16; ++j) {
-        uint32_t b[4];
-        const int key = kk * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * j + (lane >> 4);
-        ldsm4t(vb + key * U::ROW + ((ch ^ (key & 7)) << 4), b);
-        mma16816(acc[2 * j], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
-        mma16816(acc[2 * j + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
-        mma16816(acc[2 * j], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
-        mma16816(acc[2 * j + 1], lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
+        float even[4] = {}, odd[4] = {};
+#pragma unroll
+        for (int kk = 0; kk < KW / 16; ++kk) products(kk, j, hi[kk], lo[kk], even, odd);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[2 * j][e] += even[e];
+          acc[2 * j + 1][e] += odd[e];
+        }
       }
     }
     __syncwarp();
@@ -325,7 +348,7 @@ __device__ __forceinline__ void store_result(bf16* dst, float L, const float (&v
 
 // Items: those of prefixes (stretch fastest, then kv head, then tile), then own ones (stretch, kv head, row). Every part of a row that is somebody's gets its sums, if only to say that it is nothing,
 // so that the merge need not know about groups
-template <int HD, int WM>
+template <int HD, int WM, bool FAR>
 __device__ __forceinline__ void part_item(const PrefixParams& p, int item, int prefix_items, unsigned char* smem) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31;
@@ -352,7 +375,7 @@ __device__ __forceinline__ void part_item(const PrefixParams& p, int item, int p
     }
     if (begin >= gr.shared) return;
     auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, 3>*>(smem);
-    attend<HD, 4, WM, 3, 1, false>(
+    attend<HD, 4, WM, 3, 1, false, FAR>(
         p, u, begin, min(begin + per, gr.shared), gr.slot, kvh, split, 0,
         [&](int i, int* t, int* h) {
           const int x = x0 + i;
@@ -377,7 +400,7 @@ __device__ __forceinline__ void part_item(const PrefixParams& p, int item, int p
       return;
     }
     auto& u = *reinterpret_cast<Unit<HD, 4, 16, 3>*>(smem);
-    attend<HD, 4, 1, 3, 1, false>(
+    attend<HD, 4, 1, 3, 1, false, FAR>(
         p, u, begin, min(begin + per, own.end), own.slot, kvh, p.prefix_parts + split, 0,
         [&](int i, int* t, int* h) {
           *t = t0;
@@ -389,14 +412,14 @@ __device__ __forceinline__ void part_item(const PrefixParams& p, int item, int p
   }
 }
 
-template <int HD, int WM>
+template <int HD, int WM, bool FAR>
 __global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int prefix_items, bool behind_tiles) {
   extern __shared__ __align__(16) unsigned char smem[];
   grid_dep_launch();
   // The tiles kernel lets this one start when all its CTAs are past their own wait, so what kernels before it wrote is there, and their parts are of other places; the wait comes last then, so that
   // the end of this kernel says that the other one has ended
   if (!behind_tiles) grid_dep_wait();
-  part_item<HD, WM>(p, blockIdx.x, prefix_items, smem);
+  part_item<HD, WM, FAR>(p, blockIdx.x, prefix_items, smem);
   if (behind_tiles) grid_dep_wait();
 }
 
@@ -457,7 +480,7 @@ __device__ __forceinline__ void finish_pairs(const PrefixParams& p, bf16* out, l
 
 // The row's own keys, what the prefix's kernel left, the result: four warps per (row, kv head), or (W = 1) a warp. With W = 1 a CTA has a kv head of four rows where these are of one sequence, as a
 // question's are: they read its keys together, as 16 WM pairs that each see their own positions. Else it has four kv heads of one row, or as near to that as their number allows: warps of one length
-template <int HD, int W, int WM>
+template <int HD, int W, int WM, bool FAR>
 __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p, bf16* out, long ldo) {
   extern __shared__ __align__(16) unsigned char smem[];
   constexpr int E = HD / 32, ROWS = 4 / W, P = W == 1 ? 4 : 1, S = W == 1 ? 2 : 8;
@@ -485,7 +508,7 @@ __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p
     const int leader = __ffs(live) - 1, begin = __shfl_sync(ALL, own.begin, leader), slot = __shfl_sync(ALL, own.slot, leader), left = __shfl_sync(ALL, parts, leader);
     if (__all_sync(ALL, parts < 0 || (own.begin == begin && own.slot == slot && parts == left)) && (live & 15) > (live & -live)) {
       auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, OWN_STAGES>*>(smem);
-      if (attend<HD, 4, WM, OWN_STAGES, P, true>(
+      if (attend<HD, 4, WM, OWN_STAGES, P, true, FAR>(
               p, u, begin, __reduce_max_sync(ALL, own.end), slot, c, 0, __reduce_min_sync(ALL, parts >= 0 ? own.end : 0x7fffffff),
               [&](int i, int* t, int* h) {
                 *t = (int)t0 + i / p.G;
@@ -508,7 +531,7 @@ __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p
     return;
   }
   auto& u = reinterpret_cast<Unit<HD, W, 16, OWN_STAGES>*>(smem)[unit];
-  attend<HD, W, 1, OWN_STAGES, P, false>(
+  attend<HD, W, 1, OWN_STAGES, P, false, FAR>(
       p, u, own.begin, own.end, own.slot, kvh, 0, 0,
       [&](int i, int* t, int* h) {
         *t = (int)t0 + r;
@@ -528,6 +551,7 @@ struct Plan {
   int own_warps;                         // of the own kernel's units; 0: own parts by the parts kernel, and a merge
   int part_tiles, part_splits, tile_tiles, tile_splits, tile_share, tile_shares, own_splits;
   long tiles_from;
+  bool far;                              // a warp may have more keys than it adds up in one sum
   int prefix_parts() const { return std::max(part_splits, 2 * tile_splits); }
 };
 // `most`: positions that a slot has room for
@@ -576,35 +600,43 @@ Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long
   // us of a call with four warps and with one, 32 heads over 8, behind 2000 positions: rows with up to 100 own ones, 160 of them 52.9 and 48.7, 256 of them 77.5 and 68.8; with up to 800, 99 and 130,
   // 138 and 156; questions of 32 rows, five, 52.5 and 43.2, of 128 rows, two with up to 700, 116 and 77 (without blocks 108)
   a.own_warps = !a.tiles || !full ? 0 : items < 1184 ? 4 : 1;
+  // Keys of a warp of the parts and the own kernels at most, by the room that slots have. With sums of a tile each 8 rows behind 4000 positions take 15.6 us, without 14.5
+  const long prefix = a.wm ? std::min(most, a.tiles_from) / a.part_splits * a.wm / 4 : 0, own = most / a.own_splits / (a.own_warps == 1 ? 1 : 4);
+  a.far = std::max(prefix, own) > 2048;
   return a;
 }
 
-template <int HD, int WM>
+template <int HD, int WM, bool FAR>
 int launch_parts(const PrefixParams& p, long prefix_items, bool behind_tiles, cudaStream_t s) {
-  auto k = prefix_parts_kernel<HD, WM>;
+  auto k = prefix_parts_kernel<HD, WM, FAR>;
   constexpr int smem = std::max(sizeof(Unit<HD, 4, 16 * WM, 3>), sizeof(Unit<HD, 4, 16, 3>));
-  if (int rc = opt_in_smem_once<prefix_parts_kernel<HD, WM>>(smem)) return rc;
+  if (int rc = opt_in_smem_once<prefix_parts_kernel<HD, WM, FAR>>(smem)) return rc;
   const long items = prefix_items + (long)p.T * p.Hkv * p.own_splits;
   if (items > 0x7fffffff) return -1;
   return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)smem, s, p, (int)prefix_items, behind_tiles);
 }
-template <int HD, int W, int WM>
+template <int HD, int W, int WM, bool FAR>
 int launch_own(const PrefixParams& p, bf16* out, long ldo, cudaStream_t s) {
-  auto k = prefix_own_kernel<HD, W, WM>;
+  auto k = prefix_own_kernel<HD, W, WM, FAR>;
   constexpr int rows = 4 / W, smem = std::max(rows * sizeof(Unit<HD, W, 16, OWN_STAGES>), sizeof(Unit<HD, 4, 16 * WM, OWN_STAGES>));
-  if (int rc = opt_in_smem_once<prefix_own_kernel<HD, W, WM>>(smem)) return rc;
+  if (int rc = opt_in_smem_once<prefix_own_kernel<HD, W, WM, FAR>>(smem)) return rc;
   return launch_chain(k, dim3((unsigned)((long)(p.T + rows - 1) / rows * p.Hkv)), dim3(NT), (size_t)smem, s, p, out, ldo);
+}
+template <int HD, bool FAR>
+int launch_rest(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream_t s) {
+  if (a.own_warps == 4) return launch_own<HD, 4, 1, FAR>(p, out, ldo, s);
+  if (a.own_warps == 1) return p.G <= 4 ? launch_own<HD, 1, 1, FAR>(p, out, ldo, s) : p.G <= 8 ? launch_own<HD, 1, 2, FAR>(p, out, ldo, s) : launch_own<HD, 1, 4, FAR>(p, out, ldo, s);
+  const long parts = (long)a.part_tiles * p.Hkv * a.part_splits;
+  if (int rc = a.wm == 4 ? launch_parts<HD, 4, FAR>(p, parts, a.tiles, s) : a.wm == 2 ? launch_parts<HD, 2, FAR>(p, parts, a.tiles, s) : launch_parts<HD, 1, FAR>(p, parts, a.tiles, s)) return rc;
+  return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)((long)p.T * p.Hq)), dim3(NT), 0, s, p, out, ldo);
 }
 template <int HD>
 int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream_t s) {
-  const long parts = (long)a.part_tiles * p.Hkv * a.part_splits, tiles = (long)a.tile_tiles * p.Hkv;
-  if (parts > 0x7fffffff || tiles * a.tile_splits > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
+  const long tiles = (long)a.tile_tiles * p.Hkv;
+  if ((long)a.part_tiles * p.Hkv * a.part_splits > 0x7fffffff || tiles * a.tile_splits > 0x7fffffff || (long)p.T * p.Hq > 0x7fffffff) return -1;
   if (a.tiles)
     if (int rc = launch_prefix_tiles(p, HD, tiles, s)) return rc;
-  if (a.own_warps == 4) return launch_own<HD, 4, 1>(p, out, ldo, s);
-  if (a.own_warps == 1) return p.G <= 4 ? launch_own<HD, 1, 1>(p, out, ldo, s) : p.G <= 8 ? launch_own<HD, 1, 2>(p, out, ldo, s) : launch_own<HD, 1, 4>(p, out, ldo, s);
-  if (int rc = a.wm == 4 ? launch_parts<HD, 4>(p, parts, a.tiles, s) : a.wm == 2 ? launch_parts<HD, 2>(p, parts, a.tiles, s) : launch_parts<HD, 1>(p, parts, a.tiles, s)) return rc;
-  return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)((long)p.T * p.Hq)), dim3(NT), 0, s, p, out, ldo);
+  return a.far ? launch_rest<HD, true>(p, a, out, ldo, s) : launch_rest<HD, false>(p, a, out, ldo, s);
 }
 
 }  // namespace

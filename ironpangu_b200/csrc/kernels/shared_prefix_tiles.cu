@@ -22,13 +22,16 @@ using namespace ifab::tc;
 namespace {
 
 constexpr int TILE = 128, NT = 512;
+// The tensor core cuts off what does not fit a sum: values of one sign lose 1.1e-8 of their sum a key (measured: 16384 keys 1.8e-4, 262144 3.1e-3). So a sum goes on for FOLD tiles (4096 keys: 2^-14.4)
+// and is then added, rounded to nearest, to what the part in the scratch has. 1024 rows behind 16384 positions 436 us, with 8192 keys 424, with 2048 451, in one sum 420
+constexpr int FOLD = 32;
 constexpr uint32_t SPIN_LIMIT = 4000000u;
 
 template <int HD>
 struct Layout {
   static constexpr int PANELS = HD / 64, PANEL = TILE * 128, BYTES = PANELS * PANEL;        // 64 columns of 128 rows; a tile of queries, keys or values
   static constexpr int STAGES = HD == 128 ? 2 : 4;
-  static constexpr int Q = 0, K = Q + 2 * BYTES, V = K + STAGES * BYTES, BARS = V + STAGES * BYTES, SMEM = BARS + 512 + 1024;
+  static constexpr int Q = 0, K = Q + 2 * BYTES, V = K + STAGES * BYTES, BARS = V + STAGES * BYTES, FOLD_BUF = BARS + 512, SMEM = FOLD_BUF + 8 * 4096 + 1024;
 };
 template <int STAGES>
 struct Bars {
@@ -105,6 +108,42 @@ __device__ __forceinline__ float power_of_2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// A warp's parts: what they have times `carry` (first: they have nothing), and the sums of values in tensor memory, a pair a lane; `to`: where the pair's part lies, negative: nobody's. 32 columns at a
+// time by way of `buf`, so that eight lanes write a pair's 128 bytes, and without a look at what is there where that stays as it is: 1024 rows behind 16384 positions, a sum of 2048 keys, 522 us with a
+// pair a lane, 490 with loads, 451. A call of its own, so that the loop around it has its registers to itself
+template <int HD>
+__device__ __noinline__ void fold(uint32_t o_addr, unsigned char* buf, float* parts, long to, bool first, float carry) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int c = 0; c < HD; c += 32) {
+    float v[32];
+    tmem_ld_32x32(o_addr + c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(buf + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 4 * i + (lane >> 3);
+      const long dst = __shfl_sync(0xffffffffu, to, row);
+      const float by = __shfl_sync(0xffffffffu, carry, row);
+      float4 sum = *reinterpret_cast<const float4*>(buf + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+      float4* part = reinterpret_cast<float4*>(parts + max(dst, 0l) + c + (lane & 7) * 4);
+      if (dst < 0) continue;
+      if (first) {
+        *part = sum;
+      } else if (by == 1.f) {                    // without waiting for what is there
+        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(part), "f"(sum.x), "f"(sum.y), "f"(sum.z), "f"(sum.w) : "memory");
+      } else {
+        float4 had;
+        asm volatile("ld.relaxed.gpu.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(had.x), "=f"(had.y), "=f"(had.z), "=f"(had.w) : "l"(part) : "memory");
+        *part = make_float4(fmaf(had.x, by, sum.x), fmaf(had.y, by, sum.y), fmaf(had.z, by, sum.z), fmaf(had.w, by, sum.w));
+      }
+    }
+    __syncwarp();
+  }
 }
 
 template <int HD>
@@ -192,7 +231,15 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16, s_addr = tmem + lane_addr + X * 128, o_addr = tmem + lane_addr + 256 + X * 128;
     const int steps = two ? nt : (nt - X + 1) / 2;
     const bool holes = B->holes;
-    float m_ref = -INFINITY, l = 0.f;
+    auto part_at = [&]() {                       // of this thread's pair; -1: nobody's
+      const int x = x0 + (two ? X * TILE : 0) + r;
+      return x < pairs && p.sees(gr, gr.first + x / p.G) ? p.part_of(gr.first + x / p.G, kvh * p.G + x % p.G, 2 * split) : -1l;
+    };
+    auto add_up = [&](bool first, float carry) {
+      const long at = part_at();
+      fold<HD>(o_addr, smem + L::FOLD_BUF + warp * 4096, p.parts, at < 0 ? -1 : (at + (two ? 0 : X)) * HD, first, carry);
+    };
+    float m_ref = -INFINITY, l = 0.f, carry = 1.f;
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
       if (!__all_sync(0xffffffffu, mbar_wait(&B->s_full[X], j & 1, SPIN_LIMIT) && !*abort_flag)) { ok = false; break; }
@@ -225,12 +272,17 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
         for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-      const bool moved = top > m_ref + 8.f;      // also for the first key (m_ref = -inf)
+      const bool moved = top > m_ref + 8.f, fresh = j % FOLD == 0;       // also for the first key (m_ref = -inf)
+      if (fresh && j > 0) {                      // the product before has ended: these scores follow it in the pipe
+        add_up(j == FOLD, carry);
+        carry = 1.f;
+      }
       if (__any_sync(0xffffffffu, moved)) {
         const float corr = moved ? exp2f(m_ref - top) : 1.f;
         l *= corr;
+        carry *= corr;
         if (moved) m_ref = top;
-        if (j > 0) {                             // the product before has ended: these scores follow it in the pipe
+        if (!fresh) {
 #pragma unroll 1
           for (int c = 0; c < HD; c += 16) {
             uint32_t v[16];
@@ -284,22 +336,22 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&B->o_full[X], 0, SPIN_LIMIT) && !*abort_flag);
     tc_fence_after();
     if (!ok && lane == 0) fail();
-    const int x = x0 + (two ? X * TILE : 0) + r;
-    const bool mine = x < pairs && p.sees(gr, gr.first + x / p.G);
-    const long at = mine ? p.part_of(gr.first + x / p.G, kvh * p.G + x % p.G, 2 * split) : 0;
-    if (ok && steps > 0) {
+    const long at = part_at();
+    if (ok && steps > FOLD) {
+      add_up(false, carry);
+    } else if (ok && steps > 0) {              // (a pair a lane: by way of shared memory 27 rows in three groups take 41 us, so 39.5)
       float* to = p.parts + (at + (two ? 0 : X)) * HD;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
         float v[32];
         tmem_ld_32x32(o_addr + c, v);
         tmem_ld_wait();
-        if (mine)
+        if (at >= 0)
 #pragma unroll
           for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
       }
     }
-    if (mine) {
+    if (at >= 0) {
       p.sums[at + (two ? 0 : X)] = !ok ? make_float2(INFINITY, NAN) : steps > 0 ? prefix_sums(m_ref, l) : make_float2(-INFINITY, 0.f);
       if (two) p.sums[at + 1] = make_float2(-INFINITY, 0.f);
     }
@@ -339,7 +391,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
         for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int k = 0; k < TILE / 16; ++k)
-            umma_ta_elected(tm + 256 + X * 128, tm + X * 128 + (k >> 1) * 32 + term * 16 + (k & 1) * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, j > 0 || term > 0 || k > 0);
+            umma_ta_elected(tm + 256 + X * 128, tm + X * 128 + (k >> 1) * 32 + term * 16 + (k & 1) * 8, dv + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, j % FOLD > 0 || term > 0 || k > 0);
         if (!pair || X == 1) commit_elected(&B->v_empty[s]);
         if (u + 2 >= all) commit_elected(&B->o_full[X]);
         if (u + 2 < all) scores(u + 2);

@@ -35,7 +35,8 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos
     positions, slot. The rows of a group see the positions below the shared ones through that slot's pages, which are read once for all, and the others through their own; a row whose own position
     lies within the prefix sees the prefix up to it. Groups come in the order of their rows; rows that none names see everything through their own slot; a group of no rows counts as none.
 
-    Heads of 64 or 128 columns, up to 16 of them over a key head. Scores, maxima, sums and sums of values are f32, weights enter their products with 15 bits, the result is rounded once. Pages that
+    Heads of 64 or 128 columns, up to 16 of them over a key head. Scores, maxima, sums and sums of values are f32, of which the tensor cores add up 4096 keys at a time (and cut off
+    2^-14.4 at most); weights enter their products with 15 bits, the result is rounded once. Pages that
     are not there, slots, positions and groups out of range are skipped and set ``IFAB_STATUS_BAD_INDEX`` in the status word; a row that sees nothing gets zeros. ``scratch``: uint8 on 16 bytes,
     :func:`scratch_bytes`; calls that may run at the same time need one each."""
     # what is wrong with a call is said in _refuse: messages that are made for every call cost as much as its launches. Numbers are left to the library's own checks
