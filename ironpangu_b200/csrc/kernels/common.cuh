@@ -62,8 +62,9 @@ __device__ __forceinline__ uint4 ld_stream16(const void* p) {
 // programmatic-stream-serialization attribute: it may start while its predecessor is still
 // running. `grid_dep_launch` lets the successor start; `grid_dep_wait` blocks until the predecessor
 // grid has completed and its writes are visible. Before the wait a kernel may only read data that
-// no kernel writes (weights) and must not write global memory; every kernel of the chain executes
-// the wait, so completion order stays transitive.
+// no kernel writes (weights) and must not write global memory, but for what it has acquired from a
+// kernel that released it behind its own wait (`PrefixParams::take_over` in shared_prefix.cuh); every
+// kernel of the chain executes the wait, so completion order stays transitive.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -13,12 +13,14 @@
 //   own kernel       where rows fill the chip, in place of the two before it: one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result.
 //                    Four rows of a question read their keys together: eight questions of 128 rows behind 16384 positions 412 us, without that 432
 //
-// Behind the tiles kernel the two others start where an SM is free, ahead of its end: 64 rows behind 30011 positions 92.5 to 87.2 us, 27 in three groups 41.2 to 38.9, the 1024 412 to 408.
+// Behind the tiles kernel the two others start where an SM is free, ahead of its end (PrefixParams::take_over).
 //
 // How long a prefix is is known on the device only, so both of the first two kernels start where a group might be either's, and one of them has nothing to do. us with the parts kernel and with the
 // tiles kernel, rows of 4 heads over each of 8 kv heads, behind 500 / 4000 / 30000 positions: 8 rows 11.7 / 16.3 / 60.8 and 23.5 / 29 / 50, 16 rows 15.6 / 23.1 / 90.5 and 25.0 / 33.2 / 56.4; over 4 kv
 // heads 16 rows 15.5 / 18.7 / 51.6 and 24.9 / 29.3 / 37.9. Three groups of 27 rows behind up to 5000 / 9000 / 15000 positions 36 / 51 / 80 and 39 / 41 / 47.
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 
 #include "mma16816.cuh"
 #include "shared_prefix.cuh"
@@ -413,14 +415,12 @@ __device__ __forceinline__ void part_item(const PrefixParams& p, int item, int p
 }
 
 template <int HD, int WM, bool FAR>
-__global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int prefix_items, bool behind_tiles) {
+__global__ void __launch_bounds__(NT, 2) prefix_parts_kernel(PrefixParams p, int prefix_items) {
   extern __shared__ __align__(16) unsigned char smem[];
   grid_dep_launch();
-  // The tiles kernel lets this one start when all its CTAs are past their own wait, so what kernels before it wrote is there, and their parts are of other places; the wait comes last then, so that
-  // the end of this kernel says that the other one has ended
-  if (!behind_tiles) grid_dep_wait();
+  p.take_over();                                   // (the parts of the tiles kernel are of other places)
   part_item<HD, WM, FAR>(p, blockIdx.x, prefix_items, smem);
-  if (behind_tiles) grid_dep_wait();
+  grid_dep_wait();                               // that this kernel has ended says that the one ahead has
 }
 
 // four warps per (row, head), a stretch of its parts each
@@ -484,8 +484,9 @@ template <int HD, int W, int WM, bool FAR>
 __global__ void __launch_bounds__(NT, OWN_CTAS) prefix_own_kernel(PrefixParams p, bf16* out, long ldo) {
   extern __shared__ __align__(16) unsigned char smem[];
   constexpr int E = HD / 32, ROWS = 4 / W, P = W == 1 ? 4 : 1, S = W == 1 ? 2 : 8;
-  // The tiles kernel, which is ahead, lets this one start when all its CTAs are past their own wait, so what kernels before it wrote is there; its parts are read, and results written, behind the wait
+  // The tiles kernel's parts are read, and results written, behind the wait
   grid_dep_launch();
+  p.take_over();
   const int lane = threadIdx.x & 31, unit = threadIdx.x / (32 * W), c = blockIdx.x % p.Hkv;
   const long t0 = (long)(blockIdx.x / p.Hkv) * ROWS;
   int r = (c * ROWS + unit) / p.Hkv, kvh = (c * ROWS + unit) % p.Hkv;
@@ -607,13 +608,13 @@ Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long
 }
 
 template <int HD, int WM, bool FAR>
-int launch_parts(const PrefixParams& p, long prefix_items, bool behind_tiles, cudaStream_t s) {
+int launch_parts(const PrefixParams& p, long prefix_items, cudaStream_t s) {
   auto k = prefix_parts_kernel<HD, WM, FAR>;
   constexpr int smem = std::max(sizeof(Unit<HD, 4, 16 * WM, 3>), sizeof(Unit<HD, 4, 16, 3>));
   if (int rc = opt_in_smem_once<prefix_parts_kernel<HD, WM, FAR>>(smem)) return rc;
   const long items = prefix_items + (long)p.T * p.Hkv * p.own_splits;
   if (items > 0x7fffffff) return -1;
-  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)smem, s, p, (int)prefix_items, behind_tiles);
+  return launch_chain(k, dim3((unsigned)items), dim3(NT), (size_t)smem, s, p, (int)prefix_items);
 }
 template <int HD, int W, int WM, bool FAR>
 int launch_own(const PrefixParams& p, bf16* out, long ldo, cudaStream_t s) {
@@ -627,7 +628,7 @@ int launch_rest(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaS
   if (a.own_warps == 4) return launch_own<HD, 4, 1, FAR>(p, out, ldo, s);
   if (a.own_warps == 1) return p.G <= 4 ? launch_own<HD, 1, 1, FAR>(p, out, ldo, s) : p.G <= 8 ? launch_own<HD, 1, 2, FAR>(p, out, ldo, s) : launch_own<HD, 1, 4, FAR>(p, out, ldo, s);
   const long parts = (long)a.part_tiles * p.Hkv * a.part_splits;
-  if (int rc = a.wm == 4 ? launch_parts<HD, 4, FAR>(p, parts, a.tiles, s) : a.wm == 2 ? launch_parts<HD, 2, FAR>(p, parts, a.tiles, s) : launch_parts<HD, 1, FAR>(p, parts, a.tiles, s)) return rc;
+  if (int rc = a.wm == 4 ? launch_parts<HD, 4, FAR>(p, parts, s) : a.wm == 2 ? launch_parts<HD, 2, FAR>(p, parts, s) : launch_parts<HD, 1, FAR>(p, parts, s)) return rc;
   return launch_chain(prefix_merge_kernel<HD>, dim3((unsigned)((long)p.T * p.Hq)), dim3(NT), 0, s, p, out, ldo);
 }
 template <int HD>
@@ -639,6 +640,14 @@ int launch(const PrefixParams& p, const Plan& a, bf16* out, long ldo, cudaStream
   return a.far ? launch_rest<HD, true>(p, a, out, ldo, s) : launch_rest<HD, false>(p, a, out, ldo, s);
 }
 
+// Not 0, another one each time, and nothing that a scratch holds by chance: a count from the clock on, its bits mixed
+unsigned long long next_number() {
+  static std::atomic<uint64_t> calls{(uint64_t)std::chrono::system_clock::now().time_since_epoch().count()};
+  uint64_t x = calls.fetch_add(1, std::memory_order_relaxed) * 0x9e3779b97f4a7c15ull;
+  x = (x ^ (x >> 32)) * 0xd6e8feb86659fd93ull;
+  return (x ^ (x >> 32)) | 1;
+}
+
 }  // namespace
 
 extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_dim, int groups) {
@@ -648,7 +657,7 @@ extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_
     const Plan a = plan_of(T, Hkv, Hq / Hkv, head_dim, groups, with, 0x7fffffff);
     most = std::max(most, a.prefix_parts() + a.own_splits);
   }
-  return (uint64_t)T * Hq * most * (head_dim + 2) * sizeof(float);
+  return (uint64_t)T * Hq * most * (head_dim + 2) * sizeof(float) + sizeof(uint64_t);
 }
 
 extern "C" uint64_t ifab_shared_prefix_scratch_up_to(int T, int Hq, int Hkv, int head_dim, int groups) {
@@ -677,5 +686,7 @@ extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void*
   p.parts = (float*)scratch;
   p.sums = (float2*)((float*)scratch + (uint64_t)T * Hq * (a.prefix_parts() + a.own_splits) * head_dim);
   p.status = status;
+  p.word = (unsigned long long*)(p.sums + (uint64_t)T * Hq * (a.prefix_parts() + a.own_splits));
+  p.number = a.tiles ? next_number() : 0;
   return head_dim == 64 ? launch<64>(p, a, (bf16*)out, ldo, (cudaStream_t)stream) : launch<128>(p, a, (bf16*)out, ldo, (cudaStream_t)stream);
 }

@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     tma_prefetch_desc(&map_v);
   }
   grid_dep_wait();
+  if (blockIdx.x == 0 && tid == 0) p.hand_on();
 
   // this CTA's work
   const int item = blockIdx.x % items, split = blockIdx.x / items, kvh = item % p.Hkv;          // (the last stretch, which may be shorter, last)
