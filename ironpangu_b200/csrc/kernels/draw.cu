@@ -761,13 +761,13 @@ __global__ void __launch_bounds__(NT, 2) draw_kernel(DrawParams p) {
     for (int i = 0; i < WARPS; ++i) mine += s->warp_sum[i];
     cluster.map_shared_rank(s, tid)->from[rank] = mine;
   }
+  const float u = p.uniforms[row];               // ahead of the barrier, as all that is read of the row's: results may lie in its place
   cluster.sync();
   u64 before = 0, total = 0;
   for (int r = 0; r < ranks; ++r) {
     if (r < rank) before += s->from[r];
     total += s->from[r];
   }
-  const float u = p.uniforms[row];
   const double t = (double)u * (double)total;
   const u64 target = t > 0.0 ? (t < (double)(total - 1) ? (u64)t : total - 1) : 0;      // drawn is the first sum above it
   if (target < before || target >= before + s->from[rank]) return;
