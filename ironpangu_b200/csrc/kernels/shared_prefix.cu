@@ -657,7 +657,7 @@ extern "C" uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_
     const Plan a = plan_of(T, Hkv, Hq / Hkv, head_dim, groups, with, 0x7fffffff);
     most = std::max(most, a.prefix_parts() + a.own_splits);
   }
-  return (uint64_t)T * Hq * most * (head_dim + 2) * sizeof(float) + sizeof(uint64_t);
+  return ((uint64_t)T * Hq * most * (head_dim + 2) * sizeof(float) + sizeof(uint64_t) + 15) / 16 * 16;
 }
 
 extern "C" uint64_t ifab_shared_prefix_scratch_up_to(int T, int Hq, int Hkv, int head_dim, int groups) {
