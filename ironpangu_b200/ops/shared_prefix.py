@@ -38,7 +38,7 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos
     Heads of 64 or 128 columns, up to 16 of them over a key head. Scores, maxima, sums and sums of values are f32, of which the tensor cores add up 4096 keys at a time (and cut off
     2^-14.4 at most); weights enter their products with 15 bits, the result is rounded once. Pages that
     are not there, slots, positions and groups out of range are skipped and set ``IFAB_STATUS_BAD_INDEX`` in the status word; a row that sees nothing gets zeros. ``scratch``: uint8 on 16 bytes,
-    :func:`scratch_bytes`; calls that may run at the same time need one each."""
+    :func:`scratch_bytes`; calls that may run at the same time need one each. ``out`` may lie in the queries' place, row over row, and overlaps nothing else that the call reads."""
     # what is wrong with a call is said in _refuse: messages that are made for every call cost as much as its launches. Numbers are left to the library's own checks
     qs, ks, ps, gs, dev = q.shape, k_cache.shape, page_table.shape, groups.shape, q.get_device()
     if not (len(qs) == 2 and len(ks) == 4 and len(ps) == 2 and len(gs) == 2 and dev >= 0 and q.dtype is BF16 and k_cache.dtype is BF16 and v_cache.dtype is BF16 and positions.dtype is I32
@@ -52,15 +52,15 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos
         out = torch.empty((T, cols), dtype=BF16, device=q.device)
         ldo = cols
     else:
-        ldo = out.stride(0) if T > 1 else cols
-        if not (out.dtype is BF16 and out.shape == (T, cols) and out.get_device() == dev and out.stride(1) == 1 and ldo >= cols):
+        ldo = out.stride(0) if T > 1 and len(out.shape) == 2 else cols
+        if not (out.dtype is BF16 and out.shape == (T, cols) and out.get_device() == dev and out.stride(1) == 1 and ldo >= cols and _apart(out, q, cols, (k_cache, v_cache, positions, slots, page_table, groups))):
             _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out)
     if T == 0:
         return out
     need = _scratch(T, heads, kv_heads, head_dim, n)
     if scratch is None:
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif not (scratch.dtype is torch.uint8 and scratch.get_device() == dev and scratch.is_contiguous() and scratch.numel() >= need):
+    elif not (scratch.dtype is torch.uint8 and scratch.get_device() == dev and scratch.is_contiguous() and scratch.numel() >= need and _apart(out, q, cols, (scratch,))):
         _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out)
     args = (q.data_ptr(), q.stride(0) if T > 1 else cols, k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), page_table.data_ptr(), ps[0], ps[1], ks[1], ks[0],
             groups.data_ptr(), n, scale, T, heads, kv_heads, head_dim, scratch.data_ptr(), need, out.data_ptr(), ldo, status_ptr)
@@ -73,6 +73,23 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos
         _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv_heads, head_dim, scale, scratch, out)
     _lib.check(rc, "shared_prefix.attention")
     return out
+
+
+def _apart(out: torch.Tensor, q: torch.Tensor, cols: int, others) -> bool:
+    """Whether no row of the output lies over queries, but in the place of its own, and none between the ends of the others."""
+    T, o, p = out.shape[0], out.data_ptr(), q.data_ptr()
+    if T == 0:
+        return True
+    ldo, ldq = (t.stride(0) if T > 1 else cols for t in (out, q))
+    end = o + 2 * ((T - 1) * ldo + cols)
+    for t in others:
+        at = t.data_ptr()
+        if at < end and o < at + t.numel() * t.element_size():
+            return False
+    if (o == p and ldo == ldq) or o >= p + 2 * ((T - 1) * ldq + cols) or p >= end:
+        return True
+    ahead = (p - o) // 2 % ldo           # columns side by side, in rows of one pitch
+    return ldo == ldq and ahead >= cols and ahead + cols <= ldo
 
 
 @lru_cache(maxsize=256)
@@ -101,9 +118,12 @@ def _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv
     _need(0 < scale < float("inf"), f"a scale of {scale}")
     _need(out is None or (out.dtype == BF16 and out.shape == (T, heads * head_dim) and out.get_device() == dev and out.stride(1) == 1 and (T < 2 or out.stride(0) >= heads * head_dim)),
           f"the output must be bf16 [{T}, {heads * head_dim}] beside the queries, its rows apart")
+    _need(out is None or _apart(out, q, heads * head_dim, (k_cache, v_cache, positions, slots, page_table, groups)),
+          "the output must overlap nothing that is read, but for the queries row over row")
     need = _scratch(T, heads, kv_heads, head_dim, groups.shape[0])
     _need(scratch is None or (scratch.dtype == torch.uint8 and scratch.get_device() == dev and scratch.is_contiguous() and scratch.numel() >= need),
           f"scratch must be {need} bytes (uint8) beside the queries")
+    _need(scratch is None or out is None or _apart(out, q, heads * head_dim, (scratch,)), "the output must not overlap the scratch")
     near = all(t is None or t.data_ptr() % 16 == 0 for t in (q, k_cache, v_cache, groups, scratch, out)) and all(t is None or T < 2 or t.stride(0) % 8 == 0 for t in (q, out))
     _need(near, "rows, caches, groups and scratch must lie on 16 bytes")
     raise RuntimeError(f"shared_prefix.attention: {T} rows of {heads} heads are too many for one call")
