@@ -204,12 +204,16 @@ class DenseDecoder:
         """From the next :meth:`forward` on - captured ones keep what they were captured with - the rows' attention goes by ``groups`` (``ops.shared_prefix.attention``: int32 ``[n, 4]`` on the device,
         read at every step; heads of 64 or 128 columns). None: every row reads all of its own sequence again."""
         if groups is not None:
-            if self.cfg.head_dim not in (64, 128) or self.hq > 16 * self.hk:
-                raise ValueError(f"rows of {self.hq} heads over {self.hk} of {self.cfg.head_dim} columns share no prefix")
-            need = shared_prefix.scratch_bytes(self.T, self.hq, self.hk, self.cfg.head_dim, groups.shape[0])
-            if not self._prefix_scratch or self._prefix_scratch[-1].numel() < need:
-                self._prefix_scratch.append(torch.empty(need, dtype=torch.uint8, device=groups.device))      # (captured steps go on using the one before)
+            self.prefix_room(groups)
         self.prefix_groups = groups
+
+    def prefix_room(self, groups: torch.Tensor) -> None:
+        """Scratch for steps by ``groups``; ValueError where the heads share no prefix."""
+        if self.cfg.head_dim not in (64, 128) or self.hq > 16 * self.hk:
+            raise ValueError(f"rows of {self.hq} heads over {self.hk} of {self.cfg.head_dim} columns share no prefix")
+        need = shared_prefix.scratch_bytes(self.T, self.hq, self.hk, self.cfg.head_dim, groups.shape[0])
+        if not self._prefix_scratch or self._prefix_scratch[-1].numel() < need:
+            self._prefix_scratch.append(torch.empty(need, dtype=torch.uint8, device=groups.device))      # (captured steps go on using the one before)
 
     def _row_parallel(self, a: torch.Tensor, w: torch.Tensor, x: torch.Tensor) -> None:
         """``x += a @ w.T`` summed over the ranks (one rank: the same bits without the call counter)."""

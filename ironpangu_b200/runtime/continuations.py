@@ -21,7 +21,7 @@ I32 = torch.int32
 
 class Continuations:
     def __init__(self, decoder, *, prefill=None, store_pages: int = 0, shared_prefix: bool = False):
-        """``shared_prefix``: heads of 64 or 128 columns; the results differ in their rounding from those without. ``prefill``: a ``models.dense_prefill.DensePrefill`` of the decoder; without one the prompt goes through the decode kernels. ``store_pages``: pages of the second
+        """``shared_prefix``: heads of 64 or 128 columns; the results differ in their rounding from those without. Groups that ``decoder.share_prefix`` was given are for other rows and do not count here. ``prefill``: a ``models.dense_prefill.DensePrefill`` of the decoder; without one the prompt goes through the decode kernels. ``store_pages``: pages of the second
         pool that :meth:`set_aside` copies to."""
         if decoder.pool is None or decoder.logits is None:
             raise ValueError("continuations need a decoder with page_pool and keep_logits")
@@ -37,8 +37,7 @@ class Continuations:
         self._scratch = torch.empty(self.width * ((decoder.logits.shape[1] + 4095) // 4096) * 128, dtype=torch.float32, device=dev)
         self._group = torch.zeros(1, 4, dtype=I32, device=dev) if shared_prefix else None          # rows, prompt's positions and slot
         if shared_prefix:
-            decoder.share_prefix(self._group)     # (raises where the decoder's heads cannot)
-            decoder.share_prefix(None)
+            decoder.prefix_room(self._group)
         self.whole = False                    # drawn from the whole vocabulary
         self._table = None                    # random numbers, a row a step
         self._graphs = {}
@@ -98,8 +97,6 @@ class Continuations:
 
     def _begin(self, prompt: Sequence[int], n: int, temperature: float, top_k: int, top_p: float, seed: int) -> None:
         d = self.dec
-        if self._group is not None:
-            d.share_prefix(None)              # the prompt's own rows stand alone
         self.top_k = 1 if temperature <= 0 else top_k
         self.inv_temp[:n].fill_(1e4 if temperature <= 0 else 1.0 / temperature)
         self.top_p[:n].fill_(1.0 if temperature <= 0 else top_p)
@@ -121,7 +118,7 @@ class Continuations:
                 d.tokens[:m].copy_(part)
                 d.positions[:m].copy_(torch.arange(p, p + m, dtype=I32))
                 d.slots[:m].zero_()
-                d.forward(m)
+                self._forward(m, None)        # the prompt's own rows stand alone
                 last = m - 1
         self.pool.fork(self._first.expand(n).contiguous(), self._children[:n])
         if last:
@@ -131,7 +128,6 @@ class Continuations:
         self._sample(n)
         if self._group is not None:
             self._group.copy_(torch.tensor([[0, n, len(prompt), 0]], dtype=I32))
-            d.share_prefix(self._group)
         d.positions[:n].fill_(len(prompt))
         d.slots[:n].copy_(self._children[:n])
 
@@ -149,12 +145,21 @@ class Continuations:
                           counters=self.counters[t:e], scratch=self._scratch, out_ids=self.ids[t:e])
         d.tokens[:n].copy_(self.ids[:n])
 
+    def _forward(self, n: int, groups: Optional[torch.Tensor]) -> None:
+        """The decoder's groups are set for these rows alone: others, and other objects, may use it in between."""
+        d = self.dec
+        before, d.prefix_groups = d.prefix_groups, groups
+        try:
+            d.forward(n)
+        finally:
+            d.prefix_groups = before
+
     # -- steps ---------------------------------------------------------------------------------------------------------------
     def _step(self, n: int) -> None:
         d = self.dec
         torch.add(d.positions[:n], 1, out=self._lengths[:n])
         self.pool.extend(self._children[:n], self._lengths[:n])
-        d.forward(n)
+        self._forward(n, self._group)
         self._sample(n)
         d.positions[:n].add_(1)
 
@@ -220,8 +225,6 @@ class Continuations:
             self._release()
 
     def _release(self) -> None:
-        if self._group is not None:
-            self.dec.share_prefix(None)
         self.pool.free(self._children)
         self.pool.free(self._first)
         for ids in self._aside.values():
