@@ -62,7 +62,9 @@ class Continuations:
             raise ValueError(f"top_k of {top_k}: 0 (all) or more")
         if not 0.0 <= min_p <= 1.0:
             raise ValueError(f"min_p of {min_p}: 0 to 1")
-        whole = temperature > 0 and (not 1 <= top_k <= 64 or min_p > 0)
+        whole = not temperature <= 0 and (not 1 <= top_k <= 64 or min_p > 0)
+        if whole and temperature != temperature:
+            raise ValueError("a temperature that is no number")
         if whole and (d.fabric.world > 1 or d.logits.shape[1] > sampling.MAX_VOCAB):
             raise ValueError(f"top_k of {top_k}: 1 to 64, and no min_p, on several ranks and from more than {sampling.MAX_VOCAB} tokens")
         self.end()
@@ -98,7 +100,8 @@ class Continuations:
     def _begin(self, prompt: Sequence[int], n: int, temperature: float, top_k: int, top_p: float, seed: int) -> None:
         d = self.dec
         self.top_k = 1 if temperature <= 0 else top_k
-        self.inv_temp[:n].fill_(1e4 if temperature <= 0 else 1.0 / temperature)
+        # of the whole vocabulary, 0 would take the first token where an endless temperature makes all kept ones alike
+        self.inv_temp[:n].fill_(1e4 if temperature <= 0 else max(1.0 / temperature, 2.0 ** -126) if self.whole else 1.0 / temperature)
         self.top_p[:n].fill_(1.0 if temperature <= 0 else top_p)
         first = (seed * 0x9E3779B1 + (1 << 63)) % (1 << 64) - (1 << 63)      # of 64 bits, as any seed is
         self.seeds[:n].copy_(torch.arange(n, dtype=torch.int64) + first)
