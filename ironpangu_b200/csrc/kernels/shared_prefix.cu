@@ -669,7 +669,8 @@ extern "C" uint64_t ifab_shared_prefix_scratch_up_to(int T, int Hq, int Hkv, int
 extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
                                             int num_slots, int max_pages, int page_tokens, int num_pages, const int32_t* groups, int num_groups, float scale, int T, int Hq, int Hkv,
                                             int head_dim, void* scratch, uint64_t scratch_bytes, void* out, long ldo, uint32_t* status, void* stream) {
-  if (!(scale > 0.f) || scale > 3.4e38f || !q || !k_cache || !v_cache || !positions || !slots || !page_table || !scratch || !out) return -1;
+  if (!(scale > 0.f) || scale > 2.35e38f) return -1;           // as a factor of powers of two it is finite
+  if (!q || !k_cache || !v_cache || !positions || !slots || !page_table || !scratch || !out) return -1;
   if (T < 1 || T > 1 << 20 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || (head_dim != 64 && head_dim != 128) || num_groups < 0 || num_groups > 64 || (num_groups && !groups)) return -1;
   if (num_slots < 1 || max_pages < 1 || page_tokens < 1 || num_pages < 1 || (long)num_pages * page_tokens > 0x7fffffff || (long)max_pages * page_tokens > 0x7fffffff - 256) return -1;
   if (ldq % 8 || ldo % 8 || ((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)scratch | (uintptr_t)groups) % 16) return -1;

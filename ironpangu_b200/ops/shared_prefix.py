@@ -2,6 +2,7 @@
 one prompt, or questions behind one document. ``ops.decode.gqa_decode_attention`` reads them once for every row."""
 from __future__ import annotations
 
+from ctypes import c_float
 from functools import lru_cache
 from typing import Optional
 
@@ -115,7 +116,7 @@ def _refuse(q, k_cache, v_cache, positions, slots, page_table, groups, heads, kv
     _need(groups.shape[0] <= MAX_GROUPS and groups.shape[1] == 4, f"groups must be [up to {MAX_GROUPS}, 4]")
     num_slots, max_pages = page_table.shape
     _need(num_slots >= 1 and max_pages >= 1 and pages * pt < 1 << 31 and max_pages * pt < (1 << 31) - 256, f"{pages} pages of {pt} positions, {max_pages} of {num_slots} slots are not supported")
-    _need(0 < scale < float("inf"), f"a scale of {scale}")
+    _need(0 < c_float(scale).value <= 2.35e38, f"a scale of {scale}: above 0, to 2.35e38, as f32")
     _need(out is None or (out.dtype == BF16 and out.shape == (T, heads * head_dim) and out.get_device() == dev and out.stride(1) == 1 and (T < 2 or out.stride(0) >= heads * head_dim)),
           f"the output must be bf16 [{T}, {heads * head_dim}] beside the queries, its rows apart")
     _need(out is None or _apart(out, q, heads * head_dim, (k_cache, v_cache, positions, slots, page_table, groups)),
