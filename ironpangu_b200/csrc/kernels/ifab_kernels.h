@@ -568,6 +568,7 @@ int ifab_draw(const void* logits, long ld, int f32, int T, int V, const float* i
  * of up to T rows take: ifab_shared_prefix_scratch_up_to. */
 uint64_t ifab_shared_prefix_scratch(int T, int Hq, int Hkv, int head_dim, int groups);
 uint64_t ifab_shared_prefix_scratch_up_to(int T, int Hq, int Hkv, int head_dim, int groups);
+int ifab_shared_prefix_launches(int T, int Hq, int Hkv, int head_dim, int groups, int page_tokens, int max_pages);      /* kernels that a call launches; -1: there is no such call */
 int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
                                  int num_slots, int max_pages, int page_tokens, int num_pages, const int32_t* groups, int num_groups, float scale, int T, int Hq, int Hkv,
                                  int head_dim, void* scratch, uint64_t scratch_bytes, void* out, long ldo, uint32_t* status, void* stream);

@@ -666,6 +666,12 @@ extern "C" uint64_t ifab_shared_prefix_scratch_up_to(int T, int Hq, int Hkv, int
   return most;
 }
 
+extern "C" int ifab_shared_prefix_launches(int T, int Hq, int Hkv, int head_dim, int groups, int page_tokens, int max_pages) {
+  if (T < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || groups < 0 || (head_dim != 64 && head_dim != 128) || page_tokens < 1 || max_pages < 1) return -1;
+  const Plan a = plan_of(T, Hkv, Hq / Hkv, head_dim, groups, page_tokens % 8 == 0, (long)max_pages * page_tokens);
+  return a.tiles + (a.own_warps ? 1 : 2);
+}
+
 extern "C" int ifab_shared_prefix_attention(const void* q, long ldq, const void* k_cache, const void* v_cache, const int32_t* positions, const int32_t* slots, const int32_t* page_table,
                                             int num_slots, int max_pages, int page_tokens, int num_pages, const int32_t* groups, int num_groups, float scale, int T, int Hq, int Hkv,
                                             int head_dim, void* scratch, uint64_t scratch_bytes, void* out, long ldo, uint32_t* status, void* stream) {

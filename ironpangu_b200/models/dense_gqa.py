@@ -196,9 +196,17 @@ class DenseDecoder:
         self.next_ids = torch.zeros(T, dtype=torch.int32, device=dev)
         self.next_vals = torch.zeros(T, dtype=torch.float32, device=dev)
         self.logits = e(T, self.vl, dt=torch.float32) if keep_logits else None
-        self.launches_per_forward = 1 + (T + 7) // 8 + ((6 if T <= 8 else 8 if T <= int4.STREAM_ROWS else 12) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
+        self._launches = 1 + (T + 7) // 8 + ((6 if T <= 8 else 8 if T <= int4.STREAM_ROWS else 12) if self.int4 else 5 if self.world == 1 and T <= 8 else 6) * c.layers      # one more a layer where few rows of long contexts merge their splits in a launch of their own
         self._graph = None
         self.prefix_groups, self._prefix_scratch = None, []
+
+    @property
+    def launches_per_forward(self) -> int:
+        """Of ``max_tokens`` rows."""
+        if self.prefix_groups is None:
+            return self._launches
+        c = self.cfg
+        return self._launches + c.layers * (shared_prefix.launches(self.T, self.hq, self.hk, c.head_dim, self.prefix_groups.shape[0], c.page_tokens, self.max_pages) - 1)
 
     def share_prefix(self, groups: Optional[torch.Tensor]) -> None:
         """From the next :meth:`forward` on - captured ones keep what they were captured with - the rows' attention goes by ``groups`` (``ops.shared_prefix.attention``: int32 ``[n, 4]`` on the device,

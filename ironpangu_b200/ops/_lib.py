@@ -64,6 +64,7 @@ _SIGS = {
     "ifab_pages_free": [_P, _P, _P, c_int, _P],
     "ifab_pages_compact": [_P, _P, _P],
     "ifab_shared_prefix_attention": [_P, c_long, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, c_int, c_float, c_int, c_int, c_int, c_int, _P, c_u64, _P, c_long, _P, _P],
+    "ifab_shared_prefix_launches": [c_int] * 7,
     "ifab_draw": [_P, c_long, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P],
     "ifab_gemv_bf16": [_P, c_long, _P, _P, c_float, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],
     "ifab_gemv_rows_bf16": [_P, c_long, _P, _P, c_float, c_int, _P, c_long, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],

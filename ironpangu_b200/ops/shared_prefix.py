@@ -27,6 +27,13 @@ def scratch_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, groups: i
     return _lib.load().ifab_shared_prefix_scratch_up_to(rows, heads, kv_heads, head_dim, groups)
 
 
+def launches(rows: int, heads: int, kv_heads: int, head_dim: int, groups: int, page_tokens: int, max_pages: int) -> int:
+    """Kernels that :func:`attention` launches for so many rows, where a slot has room for ``max_pages`` pages."""
+    n = _lib.load().ifab_shared_prefix_launches(rows, heads, kv_heads, head_dim, groups, page_tokens, max_pages)
+    _need(n > 0, f"{rows} rows of {heads} heads over {kv_heads} of {head_dim} columns in {groups} groups are not supported")
+    return n
+
+
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor, groups: torch.Tensor, *, heads: int,
               kv_heads: int, head_dim: int, scale: float, scratch: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, status_ptr: Optional[int] = None) -> torch.Tensor:
     """Softmax attention of bf16 rows ``q`` ``[T, >= heads * head_dim]`` (the q columns of a packed projection's rows) over the positions up to their own. ``out`` ``[T, heads * head_dim]`` bf16.
