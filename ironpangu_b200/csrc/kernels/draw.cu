@@ -12,7 +12,7 @@
 // rows of 128000 bf16 with a share of the mass 203 us, 57 % of the issue slots, 0.9 and 0.3 TB/s): 40 a token for a weight that is summed without an error, 12 for one that only says where to look.
 //
 // Weights are summed as integers of 2^-44: the sums decide between tokens, so they must not depend on an order of additions, and a weight below 2^-45 of the
-// largest is nothing. 2^18 weights of at most 1 stay below 2^62.
+// largest is nothing. 2^18 weights of at most 1 are 2^62 at most.
 #include <climits>
 #include <utility>
 
@@ -88,8 +88,10 @@ __device__ __forceinline__ Cut cut_at(u64 place) { return {value_of((uint32_t)(p
 // Weights e^((v - most) it) in units of 2^-44, rounded. With c = it log2 e as two floats,
 //   v c = n / 128 + r: n / 128 by an addition of 1.5 2^16, whose floats lie 1 / 128 apart, and r (at most 1 / 256) by a product that is rounded only then, so both without loss
 //   weight = 2^-((n_most - n) / 128) (1 + q), q = 2^(r - r_most) - 1 by Taylor's series: of at most 0.0055, it is off by 2^-31 as a float
-// The first factor is a table's (62 bits) and a shift, so weights are off by 2^-31 of themselves and a little, 2^-30 at most, unsystematically, and the largest value's is 1 exactly. What a row costs is
-// instructions, and that is half of them in 64-bit arithmetic. Factors that floats hold badly, and values whose v c the addition does not take, go the 64-bit way.
+// The first factor is a table's (62 bits) and a shift, the product's upper word is taken: the largest value's weight is 1 exactly, another one's is off by 2^-28 of itself and 2^-45 at most. In units of
+// 2^-30 of a weight: r less r_most, sums below 2^-6.8 in floats, 0.9; the cubic's coefficients and roundings 0.8, what it leaves out 0.1; 24 bits of the table under q 0.8; the product's last bit 1.0; where
+// the weight lies below 2^-15, its rounding to units of 2^-44 beside. What a row costs is instructions, and that is half of them in 64-bit arithmetic. Factors that floats hold badly, and values whose v c
+// the addition does not take, go the 64-bit way.
 struct Weights {
   float most, floor;           // below `floor` a weight is less than 2^-45
   double it, z_most;

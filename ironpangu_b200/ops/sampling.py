@@ -28,7 +28,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, inv_temperature: Opt
 
     A token weighs ``w = exp((logit - largest logit) * inv_temperature)``; tokens are ordered by falling logits, equal ones by rising ids. Kept are the first ``top_k``; of them those with
     ``w >= min_p``; of them those ahead of which less than ``top_p`` of their mass lies; always the first one. Drawn is the first kept token, by rising ids, at which the sum of the kept weights exceeds
-    ``uniforms`` times that of all. The sums are integers of 2^-44: no order of additions changes a result, and weights below 2^-45 count as 0. A weight is off by 2^-30 of itself at most.
+    ``uniforms`` times that of all. The sums are integers of 2^-44: no order of additions changes a result, and weights below 2^-45 count as 0. A weight is off by 2^-28 of
+    itself and 2^-45 at most.
 
     Per-row values, contiguous ``[T]``, none: no such cut. ``uniforms`` f32 within [0, 1); from 1 on the last kept token is drawn, below 0 the first. ``inv_temperature`` f32: 0 and less, infinity and NaN take the first token
     (probability 1). ``top_k`` int32: below 1, or V and more, keeps all. ``top_p`` f32: 1 and more, or NaN, keeps all. ``min_p`` f32: 0 and less, or NaN, keeps all. Logits of -inf and NaN are never drawn;
