@@ -151,7 +151,11 @@ class Continuations:
     def _forward(self, n: int, groups: Optional[torch.Tensor]) -> None:
         """The decoder's groups are set for these rows alone: others, and other objects, may use it in between."""
         d = self.dec
-        before, d.prefix_groups = d.prefix_groups, groups
+        before = getattr(d, "prefix_groups", None)
+        if before is groups:
+            d.forward(n)
+            return
+        d.prefix_groups = groups
         try:
             d.forward(n)
         finally:
