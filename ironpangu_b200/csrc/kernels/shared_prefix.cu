@@ -378,7 +378,7 @@ __device__ __forceinline__ void part_item(const PrefixParams& p, int item, int p
     if (begin >= gr.shared) return;
     auto& u = *reinterpret_cast<Unit<HD, 4, 16 * WM, 3>*>(smem);
     attend<HD, 4, WM, 3, 1, false, FAR>(
-        p, u, begin, min(begin + per, gr.shared), gr.slot, kvh, split, 0,
+        p, u, begin, begin + min(per, gr.shared - begin), gr.slot, kvh, split, 0,
         [&](int i, int* t, int* h) {
           const int x = x0 + i;
           if (x >= gr.rows * p.G) return false;
@@ -403,7 +403,7 @@ __device__ __forceinline__ void part_item(const PrefixParams& p, int item, int p
     }
     auto& u = *reinterpret_cast<Unit<HD, 4, 16, 3>*>(smem);
     attend<HD, 4, 1, 3, 1, false, FAR>(
-        p, u, begin, min(begin + per, own.end), own.slot, kvh, p.prefix_parts + split, 0,
+        p, u, begin, begin + min(per, own.end - begin), own.slot, kvh, p.prefix_parts + split, 0,
         [&](int i, int* t, int* h) {
           *t = t0;
           *h = kvh * p.G + i;

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(NT, 1) prefix_tiles_kernel(const __grid_consta
     gr = PrefixGroup{0, 0, 0, 0};
   }
   if (p.tiles_from && !p.by_tiles()) gr = PrefixGroup{0, 0, 0, 0};         // they are the parts kernel's
-  const int per = p.per_tile_split(gr.shared), begin = split * per, end = min(begin + per, gr.shared);
+  const int per = p.per_tile_split(gr.shared), begin = split * per, end = begin + min(per, gr.shared - begin);       // (whole stretches may pass 32 bits)
   // parts of rows that do not see the prefix, or that the stretches leave over, are nothing: the merge kernel goes by their sums alone
   for (int x = tile * 2 * TILE + tid; x < min((tile + 1) * 2 * TILE, gr.rows * p.G); x += NT) {
     const int t = gr.first + x / p.G;

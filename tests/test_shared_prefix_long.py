@@ -83,3 +83,20 @@ def test_long_own_positions(rows, heads, kv, shared, own, slots):
     """A warp a row; four rows of a sequence together; the same of more heads; four warps a row; rows that no group names."""
     _check(_error(rows, heads, kv, 128, 16, shared, own, [0, rows // 2, rows - 1], slots=slots))
     _check(_error(rows, heads, kv, 128, 16, shared, 20000, [0, rows // 2, rows - 1], slots=slots, rising=25.0))
+
+
+@gpu
+@pytest.mark.parametrize("page,most", [(1, (1 << 31) - 257), (8, ((1 << 31) - 257) // 8)])
+def test_prefixes_to_the_end_of_32_bits(page, most):
+    """The last positions that there may be, of pages that are all the same but for the last: all weight lies there. Stretches of whole tiles would end behind 2^31."""
+    g = torch.Generator(device="cuda").manual_seed(page)
+    k, v = torch.zeros(2, page, 1, 64, dtype=BF16, device="cuda"), torch.randn(2, page, 1, 64, generator=g, device="cuda").to(BF16)
+    k[1] = 5.0
+    table = torch.zeros(1, most, dtype=I32, device="cuda")
+    table[0, -1] = 1
+    n = most * page
+    i32 = lambda x: torch.tensor(x, dtype=I32, device="cuda")
+    status = torch.zeros(1, dtype=I32, device="cuda")
+    out = S.attention(torch.full((1, 64), 5.0, dtype=BF16, device="cuda"), k, v, i32([n - 1]), i32([0]), table, i32([[0, 1, n, 0]]), heads=1, kv_heads=1, head_dim=64, scale=0.125, status_ptr=status.data_ptr())
+    want = v[1, :, 0].double().mean(0)             # the other 2^31 keys weigh e^-200 each
+    assert bool(((out[0].double() - want).abs() <= want.abs() * 2 ** -8 + v[1, :, 0].double().abs().mean(0) * 2 ** -13.5).all()) and int(status) == 0
