@@ -8,8 +8,10 @@
 // which the mass passes a share), which is found without a sort: a histogram over the row, equal stretches of the values, says in which of 1024 bins the place lies; the bin's tokens - a
 // few - are gathered and put in order by counting. A bin with more tokens than the list takes (ties, values far apart) is split again by the bits of (value, id), 10 at a time.
 //
-// What bounds it: for one row dependent steps - loads, a handful of barriers of the cluster, searches by a warp - of 11 to 17 us; for many, instructions (64 rows of 151936 f32 without a cut 44 us, 256
-// rows of 128000 bf16 with a share of the mass 203 us, 57 % of the issue slots, 0.9 and 0.3 TB/s): 40 a token for a weight that is summed without an error, 12 for one that only says where to look.
+// What bounds it: for one row dependent steps - loads, a handful of barriers of the cluster, searches by a warp - of 11 to 18 us; for many, instructions, of which a token takes 6 to 7 for
+// the largest value, 47 for a weight that is summed without an error, 41 to 52 more where a share of the mass is looked for (counted: 54 and 60 without a cut, 94 and 112 with a share, bf16 and f32).
+// 64 rows of 151936 f32 without a cut 44 us, 256 rows of 128000 bf16 with a share 214 us (0.9 and 0.3 TB/s): instructions in 52 and 64 % of the issue slots of SMs that are at work, and SMs are that two
+// thirds of the time, as 256 CTAs lie two on 108 of them and one on 40.
 //
 // Weights are summed as integers of 2^-44: the sums decide between tokens, so they must not depend on an order of additions, and a weight below 2^-45 of the
 // largest is nothing. 2^18 weights of at most 1 are 2^62 at most.
@@ -503,8 +505,8 @@ struct Search {
     __syncthreads();
   }
   // The mass' share in two passes, where the bins' masses, to 2^-15 of all, say well enough between which tokens the place lies; leaves the kept masses of the warps' stretches. In a bin, a weight is
-  // that of the bin's middle times 1 - x + x^2 / 2, which is summed in 17 bits and off by x^3 / 6 < 2^-21: 12 instructions and one addition in shared memory a token, where weights of 2^-44 take 40 and
-  // two. The last pass takes those, of all tokens, and has the list. (What is less than e^-24 counts as that in the last bin: 2^-16 of the largest weight, if all tokens lie there.) Where the bin has
+  // that of the bin's middle times 1 - x + x^2 / 2, which is summed in 17 bits and off by x^3 / 6 < 2^-21: one addition in shared memory a token, and a part of the instructions, where weights of 2^-44
+  // take two. The last pass takes those, of all tokens, and has the list. (What is less than e^-24 counts as that in the last bin: 2^-16 of the largest weight, if all tokens lie there.) Where the bin has
   // more tokens than the list takes, one more pass, which counts only, has it in 1024 stretches. 256 rows of 128000 bf16 291 to 212 us, 27 of 151936 with cuts of their own 49 to 40 us.
   // False: the place is among the smallest weights, or too many tokens are nearly equal
   __device__ bool quick(cg::cluster_group& cluster, float share, int first, int last, int each) {

@@ -11,7 +11,7 @@
 //                    of its own keys): products on the tensor cores as m16n8k16, running maximum and sum in 32 bits, tiles of 64 keys through a ring in shared memory
 //   merge kernel     four warps per (row, head): the parts, weighted by e^(m - largest m), over the sum
 //   own kernel       where rows fill the chip, in place of the two before it: one CTA, with very many rows one warp, per (row, kv head): its own keys, then the prefix's parts and the result.
-//                    Four rows of a question read their keys together: eight questions of 128 rows behind 16384 positions 412 us, without that 432
+//                    Four rows of a question read their keys together: eight questions of 128 rows behind 16384 positions 426 us, without that 450
 //
 // Behind the tiles kernel the two others start where an SM is free, ahead of its end (PrefixParams::take_over).
 //
@@ -575,9 +575,10 @@ Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long
   a.tiles = groups && most >= a.tiles_from;
   if (a.tiles) {
     a.tile_tiles = tiles(256);
-    // Stretches for whole waves of 148 CTAs. SMs that a wave leaves over have short stretches, by up to four turns: 960 rows of 14 heads over 2 behind 16384 positions (56 items) 157 us, without 180;
-    // 1024 rows of 16 over 16 (64 items, four turns) 229, without 241; by seven turns (128 items) 370 and 397, but also 428 and 412. 400 rows of 128 heads over 8 (200 items) in two stretches 396, in
-    // one 465. Groups have half a tile less than they may have each, on the average
+    // Stretches for whole waves of 148 CTAs. SMs that a wave leaves over have short stretches, by up to four turns: us behind 16384 positions with and without them, rows of
+    // 16 heads over 4, two turns (56 items) 190 and 216, three (100) 335 and 404, four (116) 371 and 413, (64) 222 and 220; of 32 over 8 by seven turns (128) 442 and 426. Behind 5000 positions 104 and 103,
+    // 180 and 173, 200 and 182, 123 and 107: how long a prefix is is known on the device only, and here it is taken for long. 400 rows of 128 heads over 8 (200 items) in two stretches 623, in one 770.
+    // Groups have half a tile less than they may have each, on the average
     const long items = (long)a.tile_tiles * Hkv, likely = std::max(1l, (long)(a.tile_tiles - groups / 2) * Hkv);
     a.tile_share = a.tile_shares = a.tile_splits = 1;
     if (items <= 148) {
@@ -599,7 +600,8 @@ Plan plan_of(int T, int Hkv, int G, int head_dim, int groups, bool tcgen05, long
   }
   a.own_splits = splits(items, a.tiles ? 296 : 148, 16);
   // us of a call with four warps and with one, 32 heads over 8, behind 2000 positions: rows with up to 100 own ones, 160 of them 52.9 and 48.7, 256 of them 77.5 and 68.8; with up to 800, 99 and 130,
-  // 138 and 156; questions of 32 rows, five, 52.5 and 43.2, of 128 rows, two with up to 700, 116 and 77 (without blocks 108)
+  // 138 and 156; questions of 32 rows, five, 52.5 and 43.2, of 128 rows, two with up to 700, 116 and 68 (without blocks 118). Own positions are taken for few here: how many they are is known on
+  // the device only, and rows of the many have one unit all the same (256 rows with 4000 own ones each 1010 us, 150 rows of which one is in no group and at position 30000 2455)
   a.own_warps = !a.tiles || !full ? 0 : items < 1184 ? 4 : 1;
   // Keys of a warp of the parts and the own kernels at most, by the room that slots have. With sums of a tile each 8 rows behind 4000 positions take 15.6 us, without 14.5
   const long prefix = a.wm ? std::min(most, a.tiles_from) / a.part_splits * a.wm / 4 : 0, own = most / a.own_splits / (a.own_warps == 1 ? 1 : 4);

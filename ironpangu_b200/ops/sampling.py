@@ -89,8 +89,8 @@ def _apart(logits: torch.Tensor, given, out_ids: torch.Tensor, out_probs: Option
         if any(p is not None and p != o and o < p + n and p < o + n for p in given):
             return False
         if o < first + (T - 1) * pitch + V * size and first < o + n:
-            ahead = (o - first) % pitch              # it may lie between two rows
-            if o < first or ahead < V * size or ahead + n > pitch:
+            ahead = (o - first) % max(pitch, 1)      # it may lie between two rows
+            if pitch < V * size or o < first or ahead < V * size or ahead + n > pitch:
                 return False
     return len(outs) < 2 or abs(outs[0] - outs[1]) >= n
 

@@ -1,5 +1,9 @@
 """Attention of query rows that share a long prefix, whose keys and values are read once for all of them (``csrc/kernels/shared_prefix.cu``): decode steps of several continuations of
-one prompt, or questions behind one document. ``ops.decode.gqa_decode_attention`` reads them once for every row."""
+one prompt, or questions behind one document. ``ops.decode.gqa_decode_attention`` reads them once for every row, and is as fast up to some 16000 shared positions of 2 rows, 2500 of 8,
+700 of 32, 250 of 64 and of 200 (16 heads over 4 of 128 columns, 40 own positions; 32 over 8: 2500, 1000, 200, 500 and none).
+
+Rows' own positions are taken for few: from 400 rows by key heads on a row's go to one CTA, from 1184 on to one warp. A row of tens of thousands of own positions - one that no group names, or that lies far
+within its group's prefix - is better off in a call of the other kernel: beside 150 rows of 8 key heads it takes 2.5 ms here, the whole call 0.8 ms there."""
 from __future__ import annotations
 
 from ctypes import c_float
@@ -92,7 +96,7 @@ def _apart(out: torch.Tensor, q: torch.Tensor, cols: int, others) -> bool:
     end = o + 2 * ((T - 1) * ldo + cols)
     for t in others:
         at = t.data_ptr()
-        if at < end and o < at + t.numel() * t.element_size():
+        if at < end and o < at + t.nbytes:
             return False
     if (o == p and ldo == ldq) or o >= p + 2 * ((T - 1) * ldq + cols) or p >= end:
         return True

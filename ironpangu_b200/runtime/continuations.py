@@ -21,7 +21,8 @@ I32 = torch.int32
 
 class Continuations:
     def __init__(self, decoder, *, prefill=None, store_pages: int = 0, shared_prefix: bool = False):
-        """``shared_prefix``: heads of 64 or 128 columns; the results differ in their rounding from those without. Groups that ``decoder.share_prefix`` was given are for other rows and do not count here. ``prefill``: a ``models.dense_prefill.DensePrefill`` of the decoder; without one the prompt goes through the decode kernels. ``store_pages``: pages of the second
+        """``shared_prefix``: heads of 64 or 128 columns; the results differ in their rounding from those without. A step of the 2B model, bf16, takes 1 to 4 % longer behind 200 tokens of prompt and 10 to
+        16 % less behind 12000 (4, 8 and 32 continuations); it is the same behind 2400, 3800 and 950. Groups that ``decoder.share_prefix`` was given are for other rows and do not count here. ``prefill``: a ``models.dense_prefill.DensePrefill`` of the decoder; without one the prompt goes through the decode kernels. ``store_pages``: pages of the second
         pool that :meth:`set_aside` copies to."""
         if decoder.pool is None or decoder.logits is None:
             raise ValueError("continuations need a decoder with page_pool and keep_logits")

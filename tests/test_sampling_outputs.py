@@ -54,3 +54,11 @@ def test_refused_over_what_is_read_or_written():
         got = sampling.sample(wide[:, :V], u, out_ids=out_ids, out_probs=out_probs, probs=True)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.equal(wide[:, :V], x)
+
+
+@gpu
+def test_refused_over_rows_that_are_one():
+    x, u, _, _ = _case(1, 64, 2)
+    one = x.expand(3, 64)
+    with pytest.raises(ValueError, match="lie apart"):
+        sampling.sample(one, u.expand(3).contiguous(), out_probs=x[0, :3])
