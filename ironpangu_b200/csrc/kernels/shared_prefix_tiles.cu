@@ -134,7 +134,7 @@ __device__ __noinline__ void fold(uint32_t o_addr, unsigned char* buf, float* pa
       if (dst < 0) continue;
       if (first) {
         *part = sum;
-      } else if (by == 1.f) {                    // without waiting for what is there
+      } else if (by == 1.f) {                    // without waiting for what is there (a place is one thread's, whose additions follow one another)
         asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(part), "f"(sum.x), "f"(sum.y), "f"(sum.z), "f"(sum.w) : "memory");
       } else {
         float4 had;
